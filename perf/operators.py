@@ -7,11 +7,13 @@ dict with a ``kind`` and its sizes:
   read, along its columns (what a training step keeps of it), or (``weight``) an FP32 master
   weight in blocks of 128 x 128 with its transpose.
 * ``mm``: the product of two e4m3 matrices with a scale per block of 128, from operands that
-  are there already: BF16 (a projection or its input gradient) or FP32 (a weight gradient).
+  are there already: the second in blocks of 128 x 128 (a projection or its input gradient)
+  or, with ``by_rows``, of 1 x 128 as the first (a weight gradient).
 * ``linear``: a projection as inference runs it: BF16 rows quantized, then the product with
   the weight that was quantized when the model was loaded.
-* ``train``: a projection's training step from the FP32 master weight: both operands and the
-  gradient quantized, Y, dX and the FP32 dW.
+* ``train``: a projection's training step, its operands and the gradient quantized in it: Y
+  and dX in 8 bits, and dW: of a BF16 weight in 8 bits too, of an FP32 master (``master``) as
+  the FP32 sums of the BF16 operands' products.
 * ``logits``: log probability of a given token, entropy and the ``top_k`` likeliest tokens of
   each row of logits; with ``grad`` also the gradient of the logits.
 * ``head``: log probability and entropy from the hidden state and the head weight; with
@@ -53,11 +55,11 @@ def listed():
          "weight": True, "scales": "float32"},
         # The reference's measured input projection on 8-bit operands.
         {"name": "mm_8192x10240x2048", "kind": "mm", "rows": 8192, "n": 10240, "k": 2048,
-         "scales": "e8m0", "out": "bf16"},
+         "scales": "e8m0", "by_rows": False},
         # The same kind of product under FP32 scales, as published 8-bit checkpoints hold
         # them, on a ragged last batch at the default width.
         {"name": "mm_f32_scales_1999x8960x1280", "kind": "mm", "rows": 1999, "n": 8960,
-         "k": 1280, "scales": "float32", "out": "bf16"},
+         "k": 1280, "scales": "float32", "by_rows": False},
         # One token through the down projection of the benchmarked layer: a decoding step.
         {"name": "linear_1x2048x5632", "kind": "linear", "rows": 1, "n": 2048, "k": 5632,
          "scales": "e8m0"},
@@ -66,7 +68,7 @@ def listed():
          "scales": "e8m0"},
         # The benchmarked layer's up/gate projection, forward and backward.
         {"name": "train_16384x11264x2048", "kind": "train", "rows": 16384, "n": 11264,
-         "k": 2048, "scales": "e8m0"},
+         "k": 2048, "scales": "e8m0", "master": False},
         # One decoding step's logits with the likeliest eight tokens: the smallest call.
         {"name": "logits_1x32768_top8", "kind": "logits", "rows": 1, "vocab": 32768,
          "dtype": "bf16", "top_k": 8, "temperature": 1.0, "masked": False, "grad": False},
@@ -121,9 +123,11 @@ def draw(rng):
     case["n"] = _width(rng, 512, 11264)
     case["rows"] = _log(rng, 1, 128) if kind == "linear" else _log(rng, 128, 16384)
     if kind == "mm":
-        case["out"] = rng.choice(["bf16", "bf16", "float32"])
+        case["by_rows"] = rng.random() < 0.33
         if rng.random() < 0.4:
             case["rows"] = _log(rng, 1, 128)
+    elif kind == "train":
+        case["master"] = rng.random() < 0.4
     return case
 
 
@@ -174,12 +178,10 @@ def _inputs(case, seed):
     x = draws(rows, k, dtype=F32).mul_(torch.where(loud, 10.0, 1.0)).to(BF16)
     if kind == "quantize":
         return {"x": x}
-    t = {"x": x, "weight": draws(case["n"], k, std=0.02, dtype=F32)}
+    bf16 = kind == "train" and not case["master"] or kind == "mm" and case["by_rows"]
+    t = {"x": x, "weight": draws(case["n"], k, std=0.02, dtype=BF16 if bf16 else F32)}
     if kind == "train":
         t["grad"] = draws(rows, case["n"], std=1e-2)
-    elif kind == "mm" and case["out"] == "float32":
-        # A weight gradient's operands: both sides have a scale per row and block.
-        t["weight"] = draws(case["n"], k, std=1e-2)
     return t
 
 
@@ -188,10 +190,9 @@ def prepare(case, seed):
     state["case"] = case
     kind = case["kind"]
     if kind == "mm":
-        per_row = case["out"] == "float32"
         state["a"], state["a_scale"] = _quantize(state.pop("x"), case["scales"], 1)
         state["b"], state["b_scale"] = _quantize(state.pop("weight"), case["scales"],
-                                                 1 if per_row else BLOCK)
+                                                 1 if case["by_rows"] else BLOCK)
     elif kind == "linear":
         state["b"], state["b_scale"] = _quantize(state.pop("weight"), case["scales"], BLOCK)
     elif kind == "train":
@@ -282,8 +283,7 @@ def _plain(state):
         return {"q": q, "scale": scale, "qt": qt, "scale_t": scale_t}
     if kind == "mm":
         a, b = _dequantize(state["a"], state["a_scale"]), _dequantize(state["b"], state["b_scale"])
-        out = a @ b.T
-        return {"out": out if case["out"] == "float32" else out.to(BF16)}
+        return {"out": (a @ b.T).to(BF16)}
     if kind == "linear":
         a = _dequantize(*_quantize(state["x"], case["scales"], 1))
         return {"y": (a @ _dequantize(state["b"], state["b_scale"]).T).to(BF16)}
@@ -293,8 +293,11 @@ def _plain(state):
         w = _dequantize(*_quantize(weight, scales, BLOCK))
         y = (_dequantize(*_quantize(x, scales, 1)) @ w.T).to(BF16)
         dx = (_dequantize(*_quantize(grad, scales, 1)) @ w).to(BF16)
-        dweight = (_dequantize(*_quantize(grad.T, scales, 1))
-                   @ _dequantize(*_quantize(x.T, scales, 1)).T)
+        if case["master"]:
+            dweight = grad.float().T @ x.float()
+        else:
+            dweight = (_dequantize(*_quantize(grad.T, scales, 1))
+                       @ _dequantize(*_quantize(x.T, scales, 1)).T).to(BF16)
         return {"y": y, "dx": dx, "dweight": dweight}
     tokens, temperature = state["tokens"], case["temperature"]
     if kind == "logits":
@@ -336,9 +339,7 @@ def _own(state):
                 q, scale, qt, scale_t = fp8.quantize_rows_and_columns(state["x"], scale_dtype)
             return {"q": q, "scale": scale, "qt": qt, "scale_t": scale_t}
         if kind == "mm":
-            out_dtype = F32 if case["out"] == "float32" else BF16
-            return {"out": fp8.fp8_mm(state["a"], state["a_scale"], state["b"], state["b_scale"],
-                                      out_dtype)}
+            return {"out": fp8.fp8_mm(state["a"], state["a_scale"], state["b"], state["b_scale"])}
         if kind == "linear":
             q, scale = fp8.quantize_rows(state["x"], scale_dtype)
             return {"y": fp8.fp8_mm(q, scale, state["b"], state["b_scale"])}
@@ -393,12 +394,11 @@ def work(case):
         return {"bytes": rows * k * ((4 if case["weight"] else 2) + 2) + 2 * scale * blocks,
                 "flops": 0}
     n = case["n"]
-    out = 4 if case.get("out") == "float32" else 2
     if kind == "train":
-        return {"bytes": 2 * (2 * rows * k + 2 * rows * n) + 4 * 2 * n * k,
+        return {"bytes": 2 * (2 * rows * k + 2 * rows * n) + (8 if case["master"] else 4) * n * k,
                 "flops": 6 * rows * n * k}
     a = 2 if kind == "linear" else 1
-    return {"bytes": rows * k * a + n * k + out * rows * n, "flops": 2 * rows * n * k}
+    return {"bytes": rows * k * a + n * k + 2 * rows * n, "flops": 2 * rows * n * k}
 
 
 # --- the same values in 64 bits -------------------------------------------------------------
@@ -474,7 +474,7 @@ def exact(case, seed):
         qt, scale_t, _value = _exact_quantized(x.T, scales, 1)
         return {"q": q, "scale": scale, "qt": qt, "scale_t": scale_t}
     if kind == "mm":
-        rows_of_b = 1 if case["out"] == "float32" else BLOCK
+        rows_of_b = 1 if case["by_rows"] else BLOCK
         return {"out": _exact_quantized(x, scales, 1)[2]
                 @ _exact_quantized(t["weight"], scales, rows_of_b)[2].T}
     w = _exact_quantized(t["weight"], scales, BLOCK)[2]
@@ -482,6 +482,8 @@ def exact(case, seed):
     if kind == "linear":
         return {"y": y}
     grad = t["grad"]
-    return {"y": y, "dx": _exact_quantized(grad, scales, 1)[2] @ w,
-            "dweight": _exact_quantized(grad.T, scales, 1)[2]
+    dx = _exact_quantized(grad, scales, 1)[2] @ w
+    if case["master"]:
+        return {"y": y, "dx": dx, "dweight": grad.to(F64).T @ x.to(F64)}
+    return {"y": y, "dx": dx, "dweight": _exact_quantized(grad.T, scales, 1)[2]
             @ _exact_quantized(x.T, scales, 1)[2].T}
