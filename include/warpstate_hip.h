@@ -373,6 +373,48 @@ int ws_backward_layout(const void* q_memory, const void* q_local, const float* s
                        float scale, int algorithm, void* scratch_q, void* scratch_k,
                        void* stream);
 
+/* --- 8-bit products -------------------------------------------------------------------
+ *
+ * e4m3 (OCP, largest finite value 448) matrices with one scale per block of 128: 1 x 128
+ * along the reduction, or 128 x 128. Scale types: WS_SCALE_E8M0, a byte e + 127 for 2^e (255:
+ * NaN), scale (r, b) at r * ld + b; WS_SCALE_F32, a float, scale (r, b) at b * ld + r, where r
+ * counts rows, or groups of 128 rows, and b the blocks along the reduction.
+ */
+enum WsScaleType { WS_SCALE_E8M0 = 0, WS_SCALE_F32 = 1 };
+enum WsQuantForm { WS_QUANT_ROWS = 1, WS_QUANT_COLUMNS = 2, WS_QUANT_BLOCKS = 4 };
+
+/* x [rows, cols] (row stride ldx, BF16 or, with x_f32, FP32) to e4m3. `form`:
+ *   WS_QUANT_ROWS     q [rows, cols], scale [rows, ceil(cols / 128)];
+ *   WS_QUANT_COLUMNS  qt [cols, rows] (transposed), scale_t [cols, ceil(rows / 128)];
+ *   both of them      from one read of x;
+ *   WS_QUANT_BLOCKS   q [rows, cols], scale [ceil(rows / 128), ceil(cols / 128)], and, with qt,
+ *                     the same values transposed: qt [cols, rows], scale_t the transpose of scale.
+ * Scales: e8m0, the least power of two (at least 2^-126) under which the block's magnitudes
+ * are at most 448; FP32, max(amax, 2^-100) / 448. q = rne(x / scale) (FP32 scales: x times
+ * 448 / max(amax, 2^-100)). A block with an infinity or a NaN gets the scale NaN (e8m0) or
+ * its amax / 448 (FP32). ldq and ldqt are multiples of 16 and their buffers 16-byte aligned;
+ * bytes past cols (rows of x for qt) up to the next multiple of 16 are written as zeros. */
+int ws_fp8_quantize(const void* x, int64_t ldx, int x_f32, int64_t rows, int64_t cols, int form,
+                    int scale_type, void* q, int64_t ldq, void* scale, int64_t ld_scale, void* qt,
+                    int64_t ldqt, void* scale_t, int64_t ld_scale_t, void* stream);
+
+/* Byte matrix src (r, c) at r * s_row + c * s_col into dst rows of ldd bytes (a multiple of 16,
+ * 16-byte aligned), zeros past cols: an operand of ws_fp8_mm from any layout. */
+int ws_fp8_pack(const void* src, int64_t s_row, int64_t s_col, void* dst, int64_t ldd, int64_t rows,
+                int64_t cols, void* stream);
+
+/* BF16 C [m, n] (row stride ldc) = sum over blocks b of scale_a scale_b (A_b B_b^T) with e4m3 A
+ * [m, k] (row stride lda) and B [n, k] (nn.Linear layout, row stride ldb), FP32 accumulation (of
+ * groups of eight products whose terms the instruction cuts at 13 bits below the largest). k, lda and ldb are
+ * multiples of 16 and the operands 16-byte aligned (bytes past a matrix's own reduction have
+ * to be zero: ws_fp8_pack). *_block_rows is 1 (a scale per row and block) or 128 (per 128 rows
+ * and block). e8m0 scales: 4-byte aligned, ld a multiple of 4, rows readable to the next
+ * multiple of 4 bytes. FP32 scales of B with b_block_rows 1: 16-byte aligned, ld a multiple of
+ * 4. */
+int ws_fp8_mm(const void* a, int64_t lda, const void* scale_a, int64_t ld_scale_a, int a_block_rows,
+              const void* b, int64_t ldb, const void* scale_b, int64_t ld_scale_b, int b_block_rows,
+              int scale_type, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,168 @@
+// C ABI: quantization to e4m3 in blocks of 128 and the block-scaled 8-bit product.
+#include "../../include/warpstate_hip.h"
+#include "gemm_fp8.h"
+#include "launch.h"
+
+using namespace ws;
+
+namespace {
+
+template <bool F32, int SCALE, int FORM>
+int run_quantize(const QuantParams& p, bool vec, hipStream_t s) {
+  const long tiles = (long)cdiv(p.rows, kQBlock) * p.col_tiles;
+  if (!fits_i32(tiles)) return set_error(kInvalid, "too many 128 x 128 tiles");
+  if (vec)
+    hipLaunchKernelGGL((quantize_kernel<F32, SCALE, FORM, true>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((quantize_kernel<F32, SCALE, FORM, false>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+  return hip_check(hipGetLastError(), "quantize launch");
+}
+template <bool F32, int SCALE>
+int dispatch_quantize(const QuantParams& p, int form, bool vec, hipStream_t s) {
+  switch (form) {
+    case kQuantRows: return run_quantize<F32, SCALE, kQuantRows>(p, vec, s);
+    case kQuantCols: return run_quantize<F32, SCALE, kQuantCols>(p, vec, s);
+    case kQuantRows | kQuantCols: return run_quantize<F32, SCALE, kQuantRows | kQuantCols>(p, vec, s);
+    case kQuantBlocks: return run_quantize<F32, SCALE, kQuantBlocks>(p, vec, s);
+  }
+  return set_error(kInvalid, "unknown quantization form %d", form);
+}
+
+template <class Cfg, int SCALE, bool BROW>
+int run_fp8_ring(GemmParams p, const Fp8Params& sp, hipStream_t s) {
+  const void* kern = reinterpret_cast<const void*>(&gemm_fp8_ring_kernel<Cfg, SCALE, BROW>);
+  if (int rc = ensure_lds(kern, Cfg::kLds)) return rc;
+  p.tiles_m = cdiv(p.M, Cfg::BM);
+  p.tiles_n = cdiv(p.N, Cfg::BN);
+  p.total_tiles = p.tiles_m * p.tiles_n;
+  hipLaunchKernelGGL((gemm_fp8_ring_kernel<Cfg, SCALE, BROW>), dim3(p.total_tiles), dim3(Cfg::NT),
+                     Cfg::kLds, s, p, sp);
+  return hip_check(hipGetLastError(), "8-bit product launch");
+}
+template <int SCALE, bool BROW>
+int run_fp8(const GemmParams& p, const Fp8Params& sp, hipStream_t s) {
+  return run_fp8_ring<Ring128x2, SCALE, BROW>(p, sp, s);
+}
+
+int check_scale(const Fp8Scale& s, long rows, long k_blocks, int type, bool vec4, const char* which) {
+  if (!s.ptr) return set_error(kInvalid, "null scale pointer (%s)", which);
+  const long scale_rows = (rows + (1L << s.shift) - 1) >> s.shift;
+  if (type == kScaleE8M0) {
+    if (s.ld < k_blocks || s.ld % 4 || !al(s.ptr, 4))
+      return set_error(kInvalid, "e8m0 scales of %s need 4-byte aligned rows that hold every block", which);
+    if (256 * s.ld + 4 >= 0x7fffffffL) return set_error(kInvalid, "scale rows of %s are too long", which);
+  } else if (s.ld < scale_rows || !al(s.ptr, vec4 ? 16 : 4) || (vec4 && s.ld % 4)) {
+    return set_error(kInvalid, "FP32 scales of %s need a column of every row's scales per block%s", which,
+                     vec4 ? ", in aligned groups of four" : "");
+  }
+  return kOk;
+}
+
+}  // namespace
+
+extern "C" int ws_fp8_quantize(const void* x, int64_t ldx, int x_f32, int64_t rows, int64_t cols,
+                               int form, int scale_type, void* q, int64_t ldq, void* scale,
+                               int64_t ld_scale, void* qt, int64_t ldqt, void* scale_t,
+                               int64_t ld_scale_t, void* stream) {
+  if (!x) return set_error(kInvalid, "null operand pointer");
+  if (rows < 1 || cols < 1 || !fits_i32(rows) || !fits_i32(cols) || rows > 0x7fffff00L || cols > 0x7fffff00L)
+    return set_error(kInvalid, "invalid quantization sizes rows=%ld cols=%ld", (long)rows, (long)cols);
+  if (ldx < cols) return set_error(kInvalid, "leading dimension < cols");
+  if (x_f32 != 0 && x_f32 != 1) return set_error(kInvalid, "unknown input type %d", x_f32);
+  if (scale_type != kScaleE8M0 && scale_type != kScaleF32)
+    return set_error(kInvalid, "unknown scale type %d", scale_type);
+  if (form != kQuantRows && form != kQuantCols && form != (kQuantRows | kQuantCols) && form != kQuantBlocks)
+    return set_error(kInvalid, "unknown quantization form %d", form);
+  const bool e8 = scale_type == kScaleE8M0;
+  const long row_blocks = cdiv(rows, kQBlock), col_blocks = cdiv(cols, kQBlock);
+  const long scale_rows = form == kQuantBlocks ? row_blocks : rows;
+  const long scale_rows_t = form == kQuantBlocks ? col_blocks : cols;
+  if (form != kQuantCols) {
+    if (!q || !scale) return set_error(kInvalid, "null output pointer");
+    if (ldq < cols || ldq % 16 || !al(q, 16))
+      return set_error(kInvalid, "quantized rows need 16-byte aligned storage of a multiple of 16 bytes");
+    if (ld_scale < (e8 ? col_blocks : scale_rows) || (!e8 && !al(scale, 4)))
+      return set_error(kInvalid, "scale leading dimension too small");
+  }
+  if ((form & kQuantCols) || qt) {
+    if (!qt || !scale_t) return set_error(kInvalid, "null output pointer");
+    if (ldqt < rows || ldqt % 16 || !al(qt, 16))
+      return set_error(kInvalid, "quantized columns need 16-byte aligned storage of a multiple of 16 bytes");
+    if (ld_scale_t < (e8 ? row_blocks : scale_rows_t) || (!e8 && !al(scale_t, 4)))
+      return set_error(kInvalid, "transposed scale leading dimension too small");
+  }
+  QuantParams p{};
+  p.x = x;
+  p.ldx = ldx;
+  p.rows = (int)rows; p.cols = (int)cols; p.col_tiles = (int)col_blocks;
+  p.q_cols = (int)((cols + 15) / 16 * 16);
+  p.qt_cols = (int)((rows + 15) / 16 * 16);
+  p.q = static_cast<unsigned char*>(q);
+  p.ldq = ldq;
+  p.qt = static_cast<unsigned char*>(qt);
+  p.ldqt = ldqt;
+  p.scale = scale;
+  p.ld_scale = ld_scale;
+  p.scale_t = scale_t;
+  p.ld_scale_t = ld_scale_t;
+  const bool vec = al(x, 16) && ldx % (x_f32 ? 4 : 8) == 0;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (x_f32)
+    return e8 ? dispatch_quantize<true, kScaleE8M0>(p, form, vec, s)
+              : dispatch_quantize<true, kScaleF32>(p, form, vec, s);
+  return e8 ? dispatch_quantize<false, kScaleE8M0>(p, form, vec, s)
+            : dispatch_quantize<false, kScaleF32>(p, form, vec, s);
+}
+
+extern "C" int ws_fp8_pack(const void* src, int64_t s_row, int64_t s_col, void* dst, int64_t ldd,
+                           int64_t rows, int64_t cols, void* stream) {
+  if (!src || !dst) return set_error(kInvalid, "null operand pointer");
+  if (rows < 1 || cols < 1 || !fits_i32(rows) || !fits_i32(cols) || s_row < 1 || s_col < 1)
+    return set_error(kInvalid, "invalid matrix to pack");
+  if (ldd < cols || ldd % 16 || !al(dst, 16))
+    return set_error(kInvalid, "packed rows need 16-byte aligned storage of a multiple of 16 bytes");
+  const long blocks = (rows * (ldd / 16) + 255) / 256;
+  if (!fits_i32(blocks)) return set_error(kInvalid, "matrix to pack is too large");
+  hipLaunchKernelGGL(pack_bytes_kernel, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const unsigned char*>(src), (long)s_row, (long)s_col,
+                     static_cast<unsigned char*>(dst), (long)ldd, (long)rows, (long)cols);
+  return hip_check(hipGetLastError(), "pack launch");
+}
+
+extern "C" int ws_fp8_mm(const void* a, int64_t lda, const void* scale_a, int64_t ld_scale_a,
+                         int a_block_rows, const void* b, int64_t ldb, const void* scale_b,
+                         int64_t ld_scale_b, int b_block_rows, int scale_type, void* c, int64_t ldc,
+                         int64_t m, int64_t n, int64_t k, void* stream) {
+  if (!a || !b || !c) return set_error(kInvalid, "null operand pointer");
+  if (m < 1 || n < 1 || k < 1 || !fits_i32(m) || !fits_i32(n) || !fits_i32(k))
+    return set_error(kInvalid, "matrix sizes must be positive 32-bit integers (m=%ld n=%ld k=%ld)",
+                     (long)m, (long)n, (long)k);
+  if (k % 16 || lda % 16 || ldb % 16 || lda < k || ldb < k || !al(a, 16) || !al(b, 16))
+    return set_error(kInvalid, "8-bit operands need rows of whole 16-byte pieces (ws_fp8_pack)");
+  if (257 * lda >= 0x7fffffffL || 257 * ldb >= 0x7fffffffL)
+    return set_error(kInvalid, "operand rows are too long: 257 rows span 2 GiB or more");
+  if (scale_type != kScaleE8M0 && scale_type != kScaleF32)
+    return set_error(kInvalid, "unknown scale type %d", scale_type);
+  if ((a_block_rows != 1 && a_block_rows != kQBlock) || (b_block_rows != 1 && b_block_rows != kQBlock))
+    return set_error(kInvalid, "a scale covers 1 or 128 rows");
+  if (ldc < n) return set_error(kInvalid, "output leading dimension < n");
+  if (!al(c, 2)) return set_error(kInvalid, "misaligned output");
+  if (int rc = check_out_stride(ldc, 2, "output")) return rc;
+  Fp8Params sp{{scale_a, ld_scale_a, a_block_rows == 1 ? 0 : 7}, {scale_b, ld_scale_b, b_block_rows == 1 ? 0 : 7}};
+  const long k_blocks = cdiv(k, kQBlock);
+  if (int rc = check_scale(sp.a, m, k_blocks, scale_type, false, "A")) return rc;
+  if (int rc = check_scale(sp.b, n, k_blocks, scale_type, b_block_rows == 1, "B")) return rc;
+  GemmParams p{};
+  // The loaders count K in pairs of bytes.
+  p.a = OperandDesc{static_cast<const unsigned short*>(a), lda / 2, 1};
+  p.b = OperandDesc{static_cast<const unsigned short*>(b), ldb / 2, 1};
+  p.M = (int)m; p.N = (int)n; p.K = (int)(k / 2);
+  p.c = static_cast<unsigned short*>(c);
+  p.ldc = ldc;
+  p.vec_out = n % 4 == 0 && ldc % 4 == 0 && al(c, 8);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool brow = b_block_rows == 1;
+  if (scale_type == kScaleE8M0)
+    return brow ? run_fp8<kScaleE8M0, true>(p, sp, s) : run_fp8<kScaleE8M0, false>(p, sp, s);
+  return brow ? run_fp8<kScaleF32, true>(p, sp, s) : run_fp8<kScaleF32, false>(p, sp, s);
+}

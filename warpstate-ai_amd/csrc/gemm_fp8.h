@@ -1,0 +1,257 @@
+// Product of two e4m3 matrices with a scale per block of 128 along the reduction:
+//   C[m, n] = sum_b sA[m, b] sB[n, b] sum_{k in block b} A[m, k] B[n, k],
+// A [M, K] and B [N, K] (nn.Linear layout) with contiguous rows, C in BF16. Sums are FP32
+// between the instruction's groups of eight products; within a group each product is cut at
+// 2^-13 of the largest one's power of two (measured: beside a product of 1, one of 2^-13 is
+// kept and one of 2^-14 lost; between groups, 2^-23 is kept). That costs about 1e-4 of a
+// result's size, against 2e-3 of its BF16 rounding, and is why FP32 results are not offered:
+// products of BF16 operands, with twice the matrix-pipe time, give those.
+//
+// A 128-byte row piece of e4m3 is one scale block and also exactly what 64 BF16 values take,
+// so a k-tile is one block and the operand tiles, their direct-to-LDS loads, their swizzle
+// and the accumulator layout are those of the BF16 kernels (gemm_fast.h, gemm_ring.h), with
+// K counted in pairs of bytes by the loaders. Where those run two v_mfma_f32_16x16x32_bf16
+// on a pair of 16-byte chunks, one v_mfma_f32_16x16x128_f8f6f4 takes both chunks: the same
+// matrix-pipe time per k-tile for twice the products. The chunks (l >> 4) and 4 + (l >> 4) of
+// a row go to lane l: the k order is another than the instruction's own, but the same for
+// both operands, and a block has one scale.
+//
+// Scales. e8m0: the instruction's own block scales (v_mfma_scale), no arithmetic beside it. A
+// lane gives the scale byte of its operand row; a dword holds the four bytes of four k-tiles, and is
+// shifted by one byte per k-tile. FP32: the block's product starts from zero, and
+// acc = fma(product, sA * sB, acc), four FP32 operations per MFMA beside it.
+#pragma once
+
+#include "gemm_ring.h"
+#include "quant.h"
+
+namespace ws {
+
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+
+// Scales of an operand: (r, b) as an e8m0 byte at r * ld + b (ld a multiple of 4, base 4-byte
+// aligned, rows readable to the next multiple of 4) or as FP32 at b * ld + r (for B with a
+// scale per row, base 16-byte aligned and ld a multiple of 4); one row of scales per
+// 2^shift operand rows.
+struct Fp8Scale {
+  const void* ptr;
+  long ld;
+  int shift;
+};
+struct Fp8Params {
+  Fp8Scale a, b;
+};
+
+__device__ __forceinline__ i32x8_t join_frag(bf16x8_t lo, bf16x8_t hi) {
+  const u32x4_t a = __builtin_bit_cast(u32x4_t, lo), b = __builtin_bit_cast(u32x4_t, hi);
+  return i32x8_t{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+}
+
+// (Functions of their own: with template-dependent arguments the builtin's target check fails
+// on the compiler's host pass.)
+__device__ __forceinline__ f32x4_v mfma_e4m3_scaled(i32x8_t b, i32x8_t a, f32x4_v c, unsigned sb,
+                                                    unsigned sa) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, (int)sb, 0, (int)sa);
+}
+__device__ __forceinline__ f32x4_v mfma_e4m3(i32x8_t b, i32x8_t a, f32x4_v c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, 0, 0, 0);
+}
+
+__device__ __forceinline__ unsigned load_u32(__amdgpu_buffer_rsrc_t rs, unsigned off, unsigned soff) {
+  return __builtin_amdgcn_raw_buffer_load_b32(rs, off, soff, 0);
+}
+
+// The scales of one wave's FA x FB blocks for one k-tile at a time. BROW: B has a scale per
+// row; otherwise the wave's columns lie in one block of 128.
+template <int SCALE, bool BROW, int FA, int FB>
+struct WaveScales {
+  static constexpr bool kE8 = SCALE == kScaleE8M0;
+  static constexpr int NB = BROW ? FB : 1;
+  static constexpr int kWords = kE8 || !BROW ? 1 : 4;  // per B block: a lane's four columns under FP32
+  const char *base_a, *base_b;
+  long step_a, step_b;  // bytes per k-tile (FP32)
+  unsigned off_a[FA], off_b[NB];
+  unsigned a[FA], b[NB][kWords];
+
+  // m_base, n_base: first row and column of the wave's tile.
+  __device__ __forceinline__ void init(const Fp8Params& p, int m_base, int n_base, int M, int N,
+                                       int lane) {
+    // A wave past the last row or column reads the last one's scales (four columns' at a time
+    // for a scale per row under FP32); nothing of it is stored.
+    const long ra = min(m_base, M - 1) >> p.a.shift;
+    const long rb = min(n_base, kWords == 4 ? (N - 1) & ~3 : N - 1) >> p.b.shift;
+    const int unit = kE8 ? 1 : 4;
+    base_a = static_cast<const char*>(p.a.ptr) + ra * (kE8 ? p.a.ld : 4);
+    base_b = static_cast<const char*>(p.b.ptr) + rb * (kE8 ? p.b.ld : 4);
+    step_a = p.a.ld * unit;
+    step_b = p.b.ld * unit;
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+      const long r = (min(m_base + 16 * i + (lane & 15), M - 1) >> p.a.shift) - ra;
+      off_a[i] = (unsigned)(r * (kE8 ? p.a.ld : 4));
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      if constexpr (!BROW) off_b[j] = 0;
+      else if constexpr (kE8) off_b[j] = (unsigned)((min(n_base + 16 * j + (lane & 15), N - 1) - rb) * p.b.ld);
+      else off_b[j] = (unsigned)(4 * (min(n_base + 16 * j + 4 * (lane >> 4), (N - 1) & ~3) - rb));
+    }
+  }
+  // Issues the loads of k-tile kt (e8m0: of kt .. kt + 3, kt a multiple of 4).
+  __device__ __forceinline__ void load(int kt) {
+    __amdgpu_buffer_rsrc_t ra = make_rsrc(base_a + (kE8 ? (long)kt : kt * step_a), 0x7fffffff);
+    __amdgpu_buffer_rsrc_t rb = make_rsrc(base_b + (kE8 ? (long)kt : kt * step_b), 0x7fffffff);
+#pragma unroll
+    for (int i = 0; i < FA; ++i) a[i] = load_u32(ra, off_a[i], 0);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      if constexpr (kWords == 1) {
+        b[j][0] = load_u32(rb, off_b[j], 0);
+      } else {
+        const u32x4_t v = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rb, off_b[j], 0, 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[j][e] = v[e];
+      }
+    }
+  }
+  // e8m0: on to the next k-tile's byte.
+  __device__ __forceinline__ void shift() {
+#pragma unroll
+    for (int i = 0; i < FA; ++i) a[i] >>= 8;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) b[j][0] >>= 8;
+  }
+  // acc += scaled product of A block i and B block j.
+  __device__ __forceinline__ void mac(f32x4_v& acc, i32x8_t fb, i32x8_t fa, int i, int j) const {
+    if constexpr (kE8) {
+      acc = mfma_e4m3_scaled(fb, fa, acc, b[BROW ? j : 0][0], a[i]);
+    } else {
+      const f32x4_v p = mfma_e4m3(fb, fa, f32x4_v{0.f, 0.f, 0.f, 0.f});
+      const float sa = __uint_as_float(a[i]);
+      if constexpr (BROW) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[e] = __builtin_fmaf(p[e], sa * __uint_as_float(b[j][e < kWords ? e : 0]), acc[e]);
+      } else {
+        const float s = sa * __uint_as_float(b[0][0]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(p[e], s, acc[e]);
+      }
+    }
+  }
+};
+
+// BF16 output. Outputs that are no whole aligned vectors (GemmParams::vec_out 0) go out
+// element by element.
+struct Fp8Epi {
+  template <int FA, int FB>
+  __device__ __forceinline__ static void run(const GemmParams& p, Acc16<FA, FB>& acc, int m_base,
+                                             int n_base, int lane, int tm, int tn, int wn,
+                                             unsigned char* stage) {
+    if (p.vec_out) {
+      FEpiStore<false, false>::run(p, acc, m_base, n_base, lane, tm, tn, wn, stage);
+      return;
+    }
+    opaque_lane(lane);
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+      const int m = m_base + 16 * i + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = n_base + 16 * j + 4 * (lane >> 4) + e;
+          if (m < p.M && n < p.N) p.c[(long)m * p.ldc + n] = to_bf16_bits(acc.v[i][j][e]);
+        }
+    }
+  }
+};
+
+// Macro-tiles up to 128 x 128 (RingCfg): S LDS stages, one workgroup per tile. The scales of a
+// k-tile are requested before the operand loads of the same turn, so the waits that count
+// operand loads only wait for more than they need.
+template <class Cfg, int SCALE, bool BROW>
+__global__ void __launch_bounds__(Cfg::NT) gemm_fp8_ring_kernel(const GemmParams p, const Fp8Params sp) {
+  constexpr int FA = Cfg::FA, FB = Cfg::FB, S = Cfg::S;
+  constexpr int TM = Cfg::TM, TN = Cfg::TN;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char rsmem[];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+  const int ke = cdiv(p.K, kFBK);
+
+  int tm, tn;
+  tile_position(xcd_remap(blockIdx.x, p.total_tiles, kRingWindow), p.tiles_m, p.tiles_n, tm, tn);
+  const int row0_a = tm * Cfg::BM, row0_b = tn * Cfg::BN;
+
+  RingTile<Cfg::BM, Cfg::NT, kKContig, false> la;
+  RingTile<Cfg::BN, Cfg::NT, kKContig, false> lb;
+  la.init(p.a, row0_a, p.M, 0, wave, lane);
+  lb.init(p.b, row0_b, p.N, 0, wave, lane);
+  constexpr int kWaitLoads = (RingTile<Cfg::BM, Cfg::NT, kKContig, false>::kIns +
+                              RingTile<Cfg::BN, Cfg::NT, kKContig, false>::kIns) * (S - 2);
+
+  Acc16<FA, FB> acc;
+#pragma unroll
+  for (int i = 0; i < FA; ++i)
+#pragma unroll
+    for (int j = 0; j < FB; ++j) acc.v[i][j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+
+  auto issue = [&](int kt, int stage) {
+    unsigned char* st = rsmem + stage * Cfg::kStage;
+    la.issue(p.a, row0_a, kt * kFBK, p.K, st, wave, lane);
+    lb.issue(p.b, row0_b, kt * kFBK, p.K, st + Cfg::kTileA, wave, lane);
+  };
+  typedef WaveScales<SCALE, BROW, FA, FB> Scales;
+  Scales cur, nxt;
+  nxt.init(sp, row0_a + wm * TM, row0_b + wn * TN, p.M, p.N, lane);
+  nxt.load(0);
+#pragma unroll
+  for (int s = 0; s + 1 < S; ++s) issue(s, s);
+  int rd = 0, wr = S - 1;
+  for (int kt = 0; kt < ke; ++kt) {
+    __builtin_amdgcn_s_waitcnt(wait_vmcnt(kWaitLoads));
+    __builtin_amdgcn_s_barrier();
+    if constexpr (Scales::kE8) {
+      if ((kt & 3) == 0) {
+        cur = nxt;
+        if (kt + 4 < ke) nxt.load(kt + 4);
+      } else {
+        cur.shift();
+      }
+    } else {
+      cur = nxt;
+      if (kt + 1 < ke) nxt.load(kt + 1);
+    }
+    // Stage wr was read in the previous k-tile, which every wave has left (barrier).
+    issue(kt + S - 1, wr);
+    wr = wr + 1 == S ? 0 : wr + 1;
+    __builtin_amdgcn_sched_barrier(0);
+    const unsigned char* sa = rsmem + rd * Cfg::kStage;
+    const unsigned char* sb = sa + Cfg::kTileA;
+    i32x8_t af[FA], bf[FB];
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+      af[i] = join_frag(read_frag(sa, wm * TM + 16 * i, 0, lane), read_frag(sa, wm * TM + 16 * i, 1, lane));
+#pragma unroll
+    for (int j = 0; j < FB; ++j)
+      bf[j] = join_frag(read_frag(sb, wn * TN + 16 * j, 0, lane), read_frag(sb, wn * TN + 16 * j, 1, lane));
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+      for (int j = 0; j < FB; ++j) cur.mac(acc.v[i][j], bf[j], af[i], i, j);
+    rd = rd + 1 == S ? 0 : rd + 1;
+    // This wave's fragment reads are complete (its MFMAs have issued) before the barrier
+    // that lets other waves' loads overwrite the stage.
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // The loads past the last k-tile land, and every wave is done reading, before the
+  // epilogue's staging writes.
+  __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
+  __builtin_amdgcn_s_barrier();
+  Fp8Epi::run(p, acc, row0_a + wm * TM, row0_b + wn * TN, lane, tm, tn, wn,
+           rsmem + wave * epi_wave<FA, FB>());
+}
+
+}  // namespace ws

@@ -84,6 +84,11 @@ SIGNATURES = {
                                        _c_void_p, _i64, _i64, _i64, _c_void_p]),
     "ws_backward_layout": (_i32, [_c_void_p] * 15 + [_i64] * 5 + [_f32, _i32, _c_void_p,
                                                                    _c_void_p, _c_void_p]),
+    "ws_fp8_quantize": (_i32, [_c_void_p, _i64, _i32, _i64, _i64, _i32, _i32, _c_void_p, _i64,
+                               _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p]),
+    "ws_fp8_pack": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p]),
+    "ws_fp8_mm": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _i32, _c_void_p, _i64, _c_void_p, _i64,
+                         _i32, _i32, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p]),
 }
 
 
@@ -156,6 +161,17 @@ def call(name: str, *args) -> None:
     if status != 0:
         message = lib.ws_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed (status {status}): {message}")
+
+
+def call_on(tensor: torch.Tensor, name: str, *args) -> None:
+    """``call`` with the tensor's device current (launch limits and compute units are looked up
+    for the current device) and the calling thread's stream of that device as last argument."""
+    index = tensor.get_device()
+    if index == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        return
+    with torch.cuda.device(index):
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def query(name: str, *args) -> int:
