@@ -415,6 +415,52 @@ int ws_fp8_mm(const void* a, int64_t lda, const void* scale_a, int64_t ld_scale_
               const void* b, int64_t ldb, const void* scale_b, int64_t ld_scale_b, int b_block_rows,
               int scale_type, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, void* stream);
 
+/* --- token scores ---------------------------------------------------------------------
+ *
+ * For each row of logits l (times inv_temperature > 0): logprob = l[token] - lse, entropy =
+ * lse - sum p l, lse = log sum e^l, FP32. A token of -100 has logprob 0 and takes no gradient;
+ * any other token outside [0, vocab) gets NaN. Logits of -inf have probability 0; a row of
+ * nothing else gets NaN.
+ */
+
+/* From logits [rows, vocab] (row stride ld, BF16 or, with f32, FP32; any alignment of their
+ * type; vocab at most 524288). top_k (0 to min(64, vocab)): top_ids and top_logprobs [rows,
+ * top_k] receive the largest logits' ids and log probabilities, largest first, equal logits by
+ * their lowest id. `workspace`: 16-byte aligned, ws_token_scores_workspace_bytes (null if that is 0). */
+int64_t ws_token_scores_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k);
+int ws_token_scores(const void* logits, int64_t ld, int f32, const int64_t* tokens, int64_t rows,
+                    int64_t vocab, float inv_temperature, int64_t top_k, void* workspace, float* lse,
+                    float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids,
+                    void* stream);
+/* dlogits [rows, vocab] (row stride ld_out, the logits' type; may be the logits) of
+ * sum(dlogprob logprob + dentropy entropy); either of the two may be null (zero). lse and
+ * entropy are the forward's. A row whose two upstream gradients are zero gets zeros. */
+int ws_token_scores_backward(const void* logits, int64_t ld, int f32, const int64_t* tokens,
+                             int64_t rows, int64_t vocab, float inv_temperature, const float* lse,
+                             const float* entropy, const float* dlogprob, const float* dentropy,
+                             void* dlogits, int64_t ld_out, void* stream);
+
+/* From hidden [rows, d] and the head weight [vocab, d] (BF16, 16-byte aligned rows, d a
+ * multiple of 8): the logits are the FP32 products, and exist in registers only. */
+int64_t ws_linear_token_scores_workspace_floats(int64_t rows, int64_t vocab);
+int ws_linear_token_scores(const void* hidden, int64_t ld_hidden, const void* weight,
+                           int64_t ld_weight, const int64_t* tokens, int64_t rows, int64_t vocab,
+                           int64_t d, float inv_temperature, float* workspace, float* lse,
+                           float* logprob, float* entropy, void* stream);
+/* Gradients of sum(dlogprob logprob + dentropy entropy): dhidden [rows, d] BF16 and dweight
+ * [vocab, d] FP32 (written), each nullable. The logits are recomputed chunk_rows rows at a
+ * time, and their gradient, rounded to BF16, feeds the two products. weight_t: null, or the
+ * weight transposed ([d, vocab], vocab a multiple of 8). `workspace`: 256-byte aligned. */
+int64_t ws_linear_token_scores_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d,
+                                                        int64_t chunk_rows);
+int ws_linear_token_scores_backward(const void* hidden, int64_t ld_hidden, const void* weight,
+                                    int64_t ld_weight, const void* weight_t, const int64_t* tokens,
+                                    const float* lse, const float* entropy, const float* dlogprob,
+                                    const float* dentropy, int64_t rows, int64_t vocab, int64_t d,
+                                    float inv_temperature, void* workspace, int64_t chunk_rows,
+                                    void* dhidden, int64_t ld_dhidden, float* dweight,
+                                    int64_t ld_dweight, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,11 +1,8 @@
 // C ABI: LM-head GEMM with fused cross-entropy (forward statistics and dHidden).
 #include "../../include/warpstate_hip.h"
 #include "launch.h"
+#include "lm_head.h"
 #include "rowops.h"
-
-namespace ws {
-int operand_mode(const OperandDesc& d, long rows, long k, int tile_rows);
-}
 
 using namespace ws;
 
@@ -85,11 +82,10 @@ extern "C" int ws_linear_ce_forward(const void* hidden, int64_t ld_hidden, const
 
 // Workspace of the backward: [scale, 256 B][chunk x vocab BF16 logit gradients]
 // [splits x chunk x d FP32 dHidden partials], each part 256-byte aligned.
-static inline long round256(long b) { return (b + 255) / 256 * 256; }
 
 // Split-K factor of a chunk's dHidden GEMM: as many slices as fit one round of workgroups,
 // at most 16 (1000 x 1280 over a 32768 vocabulary, 20 tiles: 12 slices 86 us, 8 slices 132).
-static inline int ce_dh_splits(long chunk, long d, long vocab) {
+int ws::ce_dh_splits(long chunk, long d, long vocab) {
   const long tiles = (long)cdiv(chunk, 256) * cdiv(d, 256);
   long splits = 256 / tiles;
   const long k_tiles = cdiv(vocab, 64);
@@ -97,13 +93,6 @@ static inline int ce_dh_splits(long chunk, long d, long vocab) {
   if (splits > k_tiles / 4) splits = k_tiles / 4;
   return splits < 1 ? 1 : (int)splits;
 }
-
-// Row length of a chunk's logits and logit gradients: the vocabulary, or, when it is no
-// multiple of 8, the next multiple of 64, so that the chunk's GEMMs keep 16-byte rows and the
-// vector loaders (loss and gradients of 4352 x 1280 over 10883: 2265 us on the generic kernels,
-// 456 padded). The padding holds zero gradients; the products read no weight row and write no
-// gradient row past the vocabulary.
-static inline long ce_row(long vocab) { return vocab % 8 ? (vocab + 63) / 64 * 64 : vocab; }
 
 extern "C" int64_t ws_linear_ce_workspace_bytes(int64_t rows, int64_t vocab, int64_t d,
                                                 int64_t chunk_rows) {
@@ -113,14 +102,6 @@ extern "C" int64_t ws_linear_ce_workspace_bytes(int64_t rows, int64_t vocab, int
 }
 
 // --- per-chunk pieces shared by the backward and the fused pass -------------------------
-
-// Operand descriptors of one row chunk [start, start + r) of the LM head.
-struct CeChunk {
-  const unsigned short* hidden;  // first row of the chunk
-  long ld_hidden;
-  long start, r;
-  long ldg;  // row length of its logits / logit gradients (ce_row, or the vocabulary)
-};
 
 // The chunk row length a call uses: padded only where the logits GEMM takes the fast path,
 // whose epilogues write the padding.
@@ -173,19 +154,19 @@ static int ce_chunk_gradients(const CeChunk& c, const void* weight, long ld_weig
                                                                           LaunchCfg{0, 1}, s);
 }
 
-// Head weight gradient of the chunk: dW [vocab, d] += f32(r(G^T @ hidden_chunk)), or = when
-// `write` (the first chunk of a gradient that starts from nothing: no cleared buffer and no
+// Head weight gradient of the chunk: dW [vocab, d] += f32(r(G^T @ hidden_chunk)) (without
+// `round` the FP32 product as it is), or = when `write` (the first chunk of a gradient that starts from nothing: no cleared buffer and no
 // read of it; 32768 x 1280 over 1000 rows 174 -> 118 us).
-static int ce_chunk_weight_grad(const CeChunk& c, const unsigned short* gl, long vocab, long d,
-                                float* dweight, long ld_dweight, bool write, const int* skip,
-                                hipStream_t s) {
+int ws::ce_chunk_weight_grad(const CeChunk& c, const unsigned short* gl, long vocab, long d,
+                             float* dweight, long ld_dweight, bool write, const int* skip,
+                             hipStream_t s, bool round) {
   GemmParams w{};
   w.a = OperandDesc{gl, 1, c.ldg};  // G^T [vocab, r]: vocab contiguous
   w.b = OperandDesc{c.hidden, 1, c.ld_hidden};
   w.M = (int)vocab; w.N = (int)d; w.K = (int)c.r;
   w.g = dweight;
   w.ldg = ld_dweight;
-  w.round_acc = kAccRound | (write ? kAccStore : 0);
+  w.round_acc = (round ? kAccRound : 0) | (write ? kAccStore : 0);
   w.skip_if = skip;
   w.vec_out = (d % 4 == 0) && (ld_dweight % 4 == 0) && (reinterpret_cast<unsigned long>(dweight) % 16 == 0);
   const int wa = ce_grad_mode(w.a, c, vocab, vocab, c.r, kMNContig);
@@ -198,10 +179,10 @@ static int ce_chunk_weight_grad(const CeChunk& c, const unsigned short* gl, long
 
 // dHidden of the chunk: r(G [r, vocab] @ W [vocab, d]) into out (row stride ld_out), split
 // over the vocabulary through FP32 partials when one chunk alone would not fill the GPU.
-static int ce_chunk_dhidden(const CeChunk& c, const unsigned short* gl, const void* weight,
-                            long ld_weight, const void* weight_t, long vocab, long d,
-                            int splits, long chunk, float* partials, unsigned short* out,
-                            long ld_out, const int* skip, hipStream_t s) {
+int ws::ce_chunk_dhidden(const CeChunk& c, const unsigned short* gl, const void* weight,
+                         long ld_weight, const void* weight_t, long vocab, long d, int splits,
+                         long chunk, float* partials, unsigned short* out, long ld_out,
+                         const int* skip, hipStream_t s) {
   GemmParams q{};
   q.a = OperandDesc{gl, c.ldg, 1};
   // B [vocab, d]: the head weight (d contiguous) or its transpose (vocab contiguous), which has

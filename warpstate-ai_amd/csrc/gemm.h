@@ -95,6 +95,11 @@ struct GemmParams {
   // tile counts above are then unused).
   int group_count;
   GemmMember grp[kMaxGroup];
+  // Token scores: logits are the products times logit_scale (1 / temperature); a third
+  // statistic per part, and four coefficients per row of the logits' gradient.
+  float logit_scale;
+  float* part_wsum;
+  const float* row_coef;
 };
 
 // --------------------------------------------------------------------------------------

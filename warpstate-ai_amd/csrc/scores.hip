@@ -1,0 +1,239 @@
+// C ABI: token scores (log probability, entropy, likeliest tokens) and their gradients, from
+// logits and from the LM head's operands.
+#include "../../include/warpstate_hip.h"
+#include "lm_head.h"
+#include "score_epilogue.h"
+#include "scores.h"
+
+using namespace ws;
+
+namespace {
+
+constexpr int kLargeEpt = 32, kSmallEpt = 8;
+
+// Logits per thread: 8 (parts of 2048) while 32 would leave most compute units without a
+// workgroup, as long as 64 parts cover the row.
+int score_ept(long rows, long vocab) {
+  const long parts = cdiv(vocab, 256 * kLargeEpt);
+  return rows * parts < 2 * device_cus() && cdiv(vocab, 256 * kSmallEpt) <= kMaxScoreParts ? kSmallEpt
+                                                                                           : kLargeEpt;
+}
+int score_parts(long rows, long vocab) { return cdiv(vocab, 256 * score_ept(rows, vocab)); }
+
+template <bool F32, int EPT>
+void launch_rows(const ScoreParams& p, hipStream_t s) {
+  const dim3 grid((unsigned)((long)p.rows * p.parts));
+  if (p.top_k > 0) hipLaunchKernelGGL((score_rows_kernel<F32, EPT, true>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((score_rows_kernel<F32, EPT, false>), grid, dim3(256), 0, s, p);
+}
+template <bool F32>
+int run_scores(const ScoreParams& p, int ept, hipStream_t s) {
+  if (ept == kSmallEpt) launch_rows<F32, kSmallEpt>(p, s);
+  else launch_rows<F32, kLargeEpt>(p, s);
+  if (int rc = hip_check(hipGetLastError(), "token score launch")) return rc;
+  if (p.parts == 1) return kOk;
+  hipLaunchKernelGGL((score_join_kernel<F32>), dim3(cdiv(p.rows, 4)), dim3(256), 0, s, p);
+  return hip_check(hipGetLastError(), "token score join launch");
+}
+
+int check_logits(const void* logits, long ld, int f32, long rows, long vocab, const void* tokens, float inv_t) {
+  if (!logits || !tokens) return set_error(kInvalid, "null operand pointer");
+  if (rows < 1 || vocab < 1 || !fits_i32(rows) || vocab > (long)kMaxScoreParts * 256 * kLargeEpt)
+    return set_error(kInvalid, "token scores take at least one row and 1 to %ld logits a row",
+                     (long)kMaxScoreParts * 256 * kLargeEpt);
+  if (ld < vocab) return set_error(kInvalid, "leading dimension < vocab");
+  if (f32 != 0 && f32 != 1) return set_error(kInvalid, "unknown logit type %d", f32);
+  if (!(inv_t > 0.0f) || inv_t > 3.4e38f) return set_error(kInvalid, "the temperature must be positive and finite");
+  if (!fits_i32(rows * cdiv(vocab, 2048))) return set_error(kInvalid, "too many logits for one launch");
+  return kOk;
+}
+
+}  // namespace
+
+extern "C" int64_t ws_token_scores_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k) {
+  if (rows < 1 || vocab < 1 || top_k < 0) return 0;
+  const long parts = score_parts(rows, vocab);
+  return parts == 1 ? 0 : rows * parts * (16 + 8 * top_k);
+}
+
+extern "C" int ws_token_scores(const void* logits, int64_t ld, int f32, const int64_t* tokens,
+                               int64_t rows, int64_t vocab, float inv_temperature, int64_t top_k,
+                               void* workspace, float* lse, float* logprob, float* entropy,
+                               float* top_logprobs, int64_t* top_ids, void* stream) {
+  if (int rc = check_logits(logits, ld, f32, rows, vocab, tokens, inv_temperature)) return rc;
+  if (!lse || !logprob || !entropy) return set_error(kInvalid, "null output pointer");
+  if (top_k < 0 || top_k > kMaxTopK || top_k > vocab)
+    return set_error(kInvalid, "top_k must lie in [0, min(%d, vocab)]", kMaxTopK);
+  if (top_k && (!top_logprobs || !top_ids)) return set_error(kInvalid, "null output pointer");
+  const int ept = score_ept(rows, vocab);
+  ScoreParams p{};
+  p.logits = logits;
+  p.ld = ld;
+  p.rows = (int)rows; p.vocab = (int)vocab; p.top_k = (int)top_k;
+  p.parts = score_parts(rows, vocab);
+  p.inv_t = inv_temperature;
+  p.tokens = reinterpret_cast<const long*>(tokens);
+  p.out = ScoreOut{lse, logprob, entropy};
+  p.top_logprobs = top_logprobs;
+  p.top_ids = reinterpret_cast<long*>(top_ids);
+  if (p.parts > 1) {
+    if (!workspace || !al(workspace, 16)) return set_error(kInvalid, "the workspace must be 16-byte aligned");
+    p.stats = static_cast<f32x4_t*>(workspace);
+    p.keys = reinterpret_cast<unsigned long*>(p.stats + rows * p.parts);
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return f32 ? run_scores<true>(p, ept, s) : run_scores<false>(p, ept, s);
+}
+
+extern "C" int ws_token_scores_backward(const void* logits, int64_t ld, int f32, const int64_t* tokens,
+                                        int64_t rows, int64_t vocab, float inv_temperature,
+                                        const float* lse, const float* entropy, const float* dlogprob,
+                                        const float* dentropy, void* dlogits, int64_t ld_out, void* stream) {
+  if (int rc = check_logits(logits, ld, f32, rows, vocab, tokens, inv_temperature)) return rc;
+  if (!lse || !entropy || !dlogits) return set_error(kInvalid, "null pointer");
+  if (ld_out < vocab) return set_error(kInvalid, "output leading dimension < vocab");
+  ScoreParams p{};
+  p.logits = logits;
+  p.ld = ld;
+  p.rows = (int)rows; p.vocab = (int)vocab;
+  p.inv_t = inv_temperature;
+  p.tokens = reinterpret_cast<const long*>(tokens);
+  p.out = ScoreOut{const_cast<float*>(lse), nullptr, const_cast<float*>(entropy)};
+  const int segments = cdiv(vocab, 2048);
+  const dim3 grid((unsigned)(rows * segments));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (f32)
+    hipLaunchKernelGGL((score_grad_kernel<true>), grid, dim3(256), 0, s, p, dlogprob, dentropy, dlogits,
+                       (long)ld_out, segments);
+  else
+    hipLaunchKernelGGL((score_grad_kernel<false>), grid, dim3(256), 0, s, p, dlogprob, dentropy, dlogits,
+                       (long)ld_out, segments);
+  return hip_check(hipGetLastError(), "token score gradient launch");
+}
+
+// --- from the LM head's operands ------------------------------------------------------------
+
+namespace {
+
+int check_head(const void* hidden, long ld_hidden, const void* weight, long ld_weight, const void* tokens,
+               long rows, long vocab, long d, float inv_t, GemmParams& p) {
+  if (!hidden || !weight || !tokens) return set_error(kInvalid, "null operand pointer");
+  if (rows < 1 || vocab < 1 || d < 1 || !fits_i32(rows) || !fits_i32(vocab) || !fits_i32(d))
+    return set_error(kInvalid, "invalid LM-head sizes rows=%ld vocab=%ld d=%ld", rows, vocab, d);
+  if (ld_hidden < d || ld_weight < d) return set_error(kInvalid, "leading dimension < d");
+  if (!(inv_t > 0.0f) || inv_t > 3.4e38f) return set_error(kInvalid, "the temperature must be positive and finite");
+  p = GemmParams{};
+  p.a = OperandDesc{static_cast<const unsigned short*>(hidden), ld_hidden, 1};
+  p.b = OperandDesc{static_cast<const unsigned short*>(weight), ld_weight, 1};  // B = W^T
+  p.M = (int)rows; p.N = (int)vocab; p.K = (int)d;
+  p.vec_out = 1;
+  p.logit_scale = inv_t;
+  if (operand_mode(p.a, rows, d, 256) != kKContig || operand_mode(p.b, vocab, d, 256) != kKContig ||
+      !fast_ok(p, kKContig, kKContig, false))
+    return set_error(kInvalid, "hidden and weight need 16-byte aligned rows of a multiple of 8 elements");
+  return kOk;
+}
+// One partial per 128 columns.
+long head_parts(long vocab) { return (long)cdiv(vocab, 256) * 2; }
+
+}  // namespace
+
+extern "C" int64_t ws_linear_token_scores_workspace_floats(int64_t rows, int64_t vocab) {
+  if (rows < 1 || vocab < 1) return 0;
+  return rows * (3 * head_parts(vocab) + 1);
+}
+
+extern "C" int ws_linear_token_scores(const void* hidden, int64_t ld_hidden, const void* weight,
+                                      int64_t ld_weight, const int64_t* tokens, int64_t rows,
+                                      int64_t vocab, int64_t d, float inv_temperature, float* workspace,
+                                      float* lse, float* logprob, float* entropy, void* stream) {
+  GemmParams p;
+  if (int rc = check_head(hidden, ld_hidden, weight, ld_weight, tokens, rows, vocab, d, inv_temperature, p))
+    return rc;
+  if (!workspace || !lse || !logprob || !entropy) return set_error(kInvalid, "null output pointer");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const long parts = head_parts(vocab);
+  p.targets = reinterpret_cast<const long*>(tokens);
+  p.part_max = workspace;
+  p.part_sum = p.part_max + rows * parts;
+  p.part_wsum = p.part_sum + rows * parts;
+  p.tgt_logit = p.part_wsum + rows * parts;
+  p.parts_per_row = (int)parts;
+  if (int rc = run_fast<kKContig, kKContig, false, FEpiScoreStats>(p, kFusedCfg, s)) return rc;
+  hipLaunchKernelGGL(score_combine_kernel, dim3(cdiv(rows, 4)), dim3(256), 0, s, p.part_max, p.part_sum,
+                     p.part_wsum, p.parts_per_row, p.tgt_logit, p.targets, ScoreOut{lse, logprob, entropy},
+                     (int)rows, (int)vocab);
+  return hip_check(hipGetLastError(), "token score combine launch");
+}
+
+// Workspace of the backward: [rows x 4 FP32 coefficients][chunk x row BF16 logit gradients]
+// [splits x chunk x d FP32 dHidden partials], each part 256-byte aligned.
+extern "C" int64_t ws_linear_token_scores_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d,
+                                                                   int64_t chunk_rows) {
+  if (rows < 1 || vocab < 1 || d < 1 || chunk_rows < 1) return 0;
+  const long chunk = chunk_rows < rows ? chunk_rows : rows;
+  const int splits = ce_dh_splits(chunk, d, vocab);
+  return round256(rows * 16) + round256(chunk * ce_row(vocab) * 2) +
+         (splits > 1 ? round256((long)splits * chunk * d * 4) : 0);
+}
+
+extern "C" int ws_linear_token_scores_backward(const void* hidden, int64_t ld_hidden, const void* weight,
+                                               int64_t ld_weight, const void* weight_t,
+                                               const int64_t* tokens, const float* lse,
+                                               const float* entropy, const float* dlogprob,
+                                               const float* dentropy, int64_t rows, int64_t vocab, int64_t d,
+                                               float inv_temperature, void* workspace, int64_t chunk_rows,
+                                               void* dhidden, int64_t ld_dhidden, float* dweight,
+                                               int64_t ld_dweight, void* stream) {
+  GemmParams p;
+  if (int rc = check_head(hidden, ld_hidden, weight, ld_weight, tokens, rows, vocab, d, inv_temperature, p))
+    return rc;
+  if (!lse || !entropy || !workspace || (!dhidden && !dweight)) return set_error(kInvalid, "null pointer");
+  if (!al(workspace, 256)) return set_error(kInvalid, "workspace must be 256-byte aligned");
+  const long chunk = chunk_rows < rows ? chunk_rows : rows;
+  const long ldg = ce_row(vocab);
+  if (chunk_rows < 1 || !fits_i32(chunk * ldg)) return set_error(kInvalid, "bad chunk_rows");
+  if (int rc = check_out_stride(ldg, 2, "logit-gradient chunk")) return rc;
+  if (dhidden) {
+    if (ld_dhidden < d) return set_error(kInvalid, "dhidden leading dimension < d");
+    if (int rc = check_out_stride(ld_dhidden, 2, "dhidden")) return rc;
+    if (int rc = check_out_stride(d, 4, "dhidden partial")) return rc;
+  }
+  if (dweight) {
+    if (ld_dweight < d) return set_error(kInvalid, "dweight leading dimension < d");
+    if (int rc = check_out_stride(ld_dweight, 4, "dweight")) return rc;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  auto* base = static_cast<unsigned char*>(workspace);
+  auto* coef = reinterpret_cast<f32x4_t*>(base);
+  auto* gl = reinterpret_cast<unsigned short*>(base + round256(rows * 16));
+  auto* partials = reinterpret_cast<float*>(base + round256(rows * 16) + round256(chunk * ldg * 2));
+  const int splits = ce_dh_splits(chunk, d, vocab);
+  hipLaunchKernelGGL(score_coef_kernel, dim3(cdiv(rows, 256)), dim3(256), 0, s,
+                     reinterpret_cast<const long*>(tokens), lse, entropy, dlogprob, dentropy, inv_temperature,
+                     (int)rows, (int)vocab, coef);
+  if (int rc = hip_check(hipGetLastError(), "token score coefficient launch")) return rc;
+  for (long start = 0; start < rows; start += chunk) {
+    const CeChunk c{static_cast<const unsigned short*>(hidden) + start * ld_hidden, ld_hidden, start,
+                    rows - start < chunk ? rows - start : chunk, ldg};
+    GemmParams g = p;
+    g.a.ptr = c.hidden;
+    g.M = (int)c.r;
+    g.c = gl;
+    g.ldc = ldg;
+    g.targets = reinterpret_cast<const long*>(tokens) + start;
+    g.row_coef = reinterpret_cast<const float*>(coef + start);
+    if (int rc = run_fast<kKContig, kKContig, false, FEpiScoreGrad>(g, kFusedCfg, s)) return rc;
+    if (dweight) {
+      if (int rc = ce_chunk_weight_grad(c, gl, vocab, d, dweight, ld_dweight, start == 0, nullptr, s, false))
+        return rc;
+    }
+    if (dhidden) {
+      if (int rc = ce_chunk_dhidden(c, gl, weight, ld_weight, weight_t, vocab, d, splits, chunk, partials,
+                                    static_cast<unsigned short*>(dhidden) + start * ld_dhidden, ld_dhidden,
+                                    nullptr, s))
+        return rc;
+    }
+  }
+  return kOk;
+}

@@ -89,6 +89,18 @@ SIGNATURES = {
     "ws_fp8_pack": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p]),
     "ws_fp8_mm": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _i32, _c_void_p, _i64, _c_void_p, _i64,
                          _i32, _i32, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p]),
+    "ws_token_scores_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "ws_token_scores": (_i32, [_c_void_p, _i64, _i32, _c_void_p, _i64, _i64, _f32, _i64]
+                        + [_c_void_p] * 7),
+    "ws_token_scores_backward": (_i32, [_c_void_p, _i64, _i32, _c_void_p, _i64, _i64, _f32]
+                                 + [_c_void_p] * 5 + [_i64, _c_void_p]),
+    "ws_linear_token_scores_workspace_floats": (_i64, [_i64, _i64]),
+    "ws_linear_token_scores": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64,
+                                      _f32] + [_c_void_p] * 5),
+    "ws_linear_token_scores_backward_workspace_bytes": (_i64, [_i64] * 4),
+    "ws_linear_token_scores_backward": (_i32, [_c_void_p, _i64, _c_void_p, _i64] + [_c_void_p] * 6
+                                        + [_i64, _i64, _i64, _f32, _c_void_p, _i64, _c_void_p, _i64,
+                                           _c_void_p, _i64, _c_void_p]),
 }
 
 
@@ -176,6 +188,15 @@ def call_on(tensor: torch.Tensor, name: str, *args) -> None:
 
 def query(name: str, *args) -> int:
     return int(getattr(library(), name)(*args))
+
+
+def query_on(tensor: torch.Tensor, name: str, *args) -> int:
+    """``query`` with the tensor's device current (sizes that follow its compute units)."""
+    index = tensor.get_device()
+    if index == torch._C._cuda_getDevice():
+        return query(name, *args)
+    with torch.cuda.device(index):
+        return query(name, *args)
 
 
 def stream(tensor: torch.Tensor) -> int:
