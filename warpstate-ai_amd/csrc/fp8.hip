@@ -40,8 +40,30 @@ int run_fp8_ring(GemmParams p, const Fp8Params& sp, hipStream_t s) {
   return hip_check(hipGetLastError(), "8-bit product launch");
 }
 template <int SCALE, bool BROW>
+int run_fp8_256(GemmParams p, const Fp8Params& sp, hipStream_t s) {
+  const void* kern = reinterpret_cast<const void*>(&gemm_fp8_kernel<SCALE, BROW>);
+  if (int rc = ensure_lds(kern, kFLdsBytes)) return rc;
+  p.tiles_m = cdiv(p.M, kFBM);
+  p.tiles_n = cdiv(p.N, kFBN);
+  p.total_tiles = p.tiles_m * p.tiles_n;
+  const int cus = device_cus();
+  hipLaunchKernelGGL((gemm_fp8_kernel<SCALE, BROW>), dim3(p.total_tiles < cus ? p.total_tiles : cus),
+                     dim3(kFNT), kFLdsBytes, s, p, sp);
+  return hip_check(hipGetLastError(), "8-bit product launch");
+}
+template <int SCALE, bool BROW>
 int run_fp8(const GemmParams& p, const Fp8Params& sp, hipStream_t s) {
-  return run_fp8_ring<Ring128x2, SCALE, BROW>(p, sp, s);
+  const int tile = pick_tile(p.M, p.N, p.K, kKContig, kKContig, false, kEpiStore);
+  switch (tile) {
+    case kTile256:
+      // (FP32 scales of B per row would not fit the registers.)
+      if constexpr (SCALE == kScaleE8M0 || !BROW) return run_fp8_256<SCALE, BROW>(p, sp, s);
+      [[fallthrough]];
+    case kTile128x2: return run_fp8_ring<Ring128x2, SCALE, BROW>(p, sp, s);
+    case kTile128x1: return run_fp8_ring<Ring128x1, SCALE, BROW>(p, sp, s);
+    case kTile64x128: return run_fp8_ring<Ring64x128, SCALE, BROW>(p, sp, s);
+    default: return run_fp8_ring<Ring64, SCALE, BROW>(p, sp, s);
+  }
 }
 
 int check_scale(const Fp8Scale& s, long rows, long k_blocks, int type, bool vec4, const char* which) {

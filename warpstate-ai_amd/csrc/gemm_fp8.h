@@ -141,8 +141,8 @@ struct WaveScales {
   }
 };
 
-// BF16 output. Outputs that are no whole aligned vectors (GemmParams::vec_out 0) go out
-// element by element.
+// BF16 output through the wave's LDS staging rows, as 16-byte row pieces. Outputs that are no
+// whole aligned vectors (GemmParams::vec_out 0) leave the staging rows element by element.
 struct Fp8Epi {
   template <int FA, int FB>
   __device__ __forceinline__ static void run(const GemmParams& p, Acc16<FA, FB>& acc, int m_base,
@@ -152,17 +152,25 @@ struct Fp8Epi {
       FEpiStore<false, false>::run(p, acc, m_base, n_base, lane, tm, tn, wn, stage);
       return;
     }
+    constexpr int kRow = epi_row<FB>(), LPR = FB * 2, RPI = 64 / LPR;
     opaque_lane(lane);
 #pragma unroll
-    for (int i = 0; i < FA; ++i) {
-      const int m = m_base + 16 * i + (lane & 15);
+    for (int i = 0; i < FA; ++i)
 #pragma unroll
-      for (int j = 0; j < FB; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = n_base + 16 * j + 4 * (lane >> 4) + e;
-          if (m < p.M && n < p.N) p.c[(long)m * p.ldc + n] = to_bf16_bits(acc.v[i][j][e]);
-        }
+      for (int j = 0; j < FB; ++j) {
+        const u32x2_t w = {pack_bf16x2(acc.v[i][j][0], acc.v[i][j][1]), pack_bf16x2(acc.v[i][j][2], acc.v[i][j][3])};
+        *reinterpret_cast<u32x2_t*>(stage + (16 * i + (lane & 15)) * kRow + (16 * j + 4 * (lane >> 4)) * 2) = w;
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's staging writes landed
+    const int c8 = 8 * (lane % LPR);
+#pragma unroll 1
+    for (int r = lane / LPR; r < FA * 16; r += RPI) {
+      if (m_base + r >= p.M) break;
+      const auto* src = reinterpret_cast<const unsigned short*>(stage + r * kRow + c8 * 2);
+      unsigned short* out = p.c + (long)(m_base + r) * p.ldc + n_base + c8;
+#pragma unroll 1
+      for (int e = 0; e < 8 && n_base + c8 + e < p.N; ++e) out[e] = src[e];
     }
   }
 };
@@ -252,6 +260,138 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_fp8_ring_kernel(const GemmParams
   __builtin_amdgcn_s_barrier();
   Fp8Epi::run(p, acc, row0_a + wm * TM, row0_b + wn * TN, lane, tm, tn, wn,
            rsmem + wave * epi_wave<FA, FB>());
+}
+
+// 256 x 256 tiles: the two-group pipeline of gemm_fast.h (its comment has the schedule), A in
+// two LDS stages and B in three. A k-tile is 24 fragment reads and 32 MFMAs, as many LDS bytes
+// and as much matrix-pipe time as there. The scales are requested at the head of a read phase,
+// ahead of its operand loads (a wait that leaves those in flight has then seen the scales), and
+// used in the MFMA phase after it.
+// Fragment of the 16-row block at `at` (its lane's first chunk): the chunks c and c ^ 4.
+__device__ __forceinline__ i32x8_t fp8_frag(const unsigned char* tile, unsigned at) {
+  return join_frag(*reinterpret_cast<const bf16x8_t*>(tile + at), *reinterpret_cast<const bf16x8_t*>(tile + (at ^ 64)));
+}
+
+template <int SCALE, bool BROW>
+__global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, const Fp8Params sp) {
+  constexpr int TM = kFBM / kFWM, TN = kFBN / kFWN;  // 64 x 128
+  constexpr int FA = TM / 16, FB = TN / 16;          // 4 x 8
+  extern __shared__ __attribute__((aligned(1024))) unsigned char fsmem[];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / kFWN, wn = wave % kFWN;
+  const bool first = wave < 4;  // the group that runs a phase ahead and loads A
+  const int ke = cdiv(p.K, kFBK);
+
+  unsigned char* const sA = fsmem;
+  unsigned char* const sB = fsmem + 2 * kFTileBytes;
+  const unsigned aoff = frag_base<kKContig>(wm * TM, lane), boff = frag_base<kKContig>(wn * TN, lane);
+
+  for (int w = blockIdx.x; w < p.total_tiles; w += gridDim.x) {
+    int tm, tn;
+    tile_position(xcd_remap(w, p.total_tiles, gridDim.x), p.tiles_m, p.tiles_n, tm, tn);
+    const int row0_a = tm * kFBM, row0_b = tn * kFBN;
+    Acc16<FA, FB> acc;
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+      for (int j = 0; j < FB; ++j) acc.v[i][j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+    WaveScales<SCALE, BROW, FA, FB> sc;
+    sc.init(sp, row0_a + wm * TM, row0_b + wn * TN, p.M, p.N, lane);
+
+    typedef RingTile<256, 256, kKContig, false> Tile;
+    const int gw = wave & 3;
+    Tile l;
+    if (first) l.init(p.a, row0_a, p.M, 0, gw, lane);
+    else l.init(p.b, row0_b, p.N, 0, gw, lane);
+    const unsigned short* base = first ? p.a.ptr + (long)row0_a * p.a.s_row : p.b.ptr + (long)row0_b * p.b.s_row;
+    auto load = [&](int kt, unsigned char* stage, auto whole) {
+      __amdgpu_buffer_rsrc_t rs = make_rsrc(base + (long)kt * kFBK, 0x7fffffff);
+      unsigned char* dst = stage + gw * 1024;
+      if (decltype(whole)::value || (kt + 1) * kFBK <= p.K) {
+#pragma unroll
+        for (int i = 0; i < kFIns; ++i) dma16(rs, dst + i * 4096, l.off[i]);
+      } else {
+        // Ragged: chunks at k >= K land as zeros. The lane index goes through an empty asm so
+        // that the k offsets are not kept live across the loop.
+        int q = lane;
+        asm volatile("" : "+v"(q));
+#pragma unroll
+        for (int i = 0; i < kFIns; ++i)
+          dma16(rs, dst + i * 4096, kt * kFBK + Tile::k_of(i, gw, q) >= p.K ? kOOB : l.off[i]);
+      }
+    };
+    if (first) {
+      load(0, sA, std::false_type{});
+      __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
+    } else {
+      load(0, sB, std::false_type{});
+      if (1 < ke) {
+        load(1, sB + kFTileBytes, std::false_type{});
+        __builtin_amdgcn_s_waitcnt(wait_vmcnt(kFIns));  // B(0)
+      } else {
+        __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
+      }
+    }
+    __builtin_amdgcn_s_barrier();
+    if (!first) __builtin_amdgcn_s_barrier();  // one phase behind from here on
+    unsigned ast = 0, bst = 0;  // byte offsets of the k-tile's stages
+    // k-tile kt; the last two (TAIL) load nothing past the end, and the one before them may
+    // load a ragged one. (With the ragged case in the loop, as a branch, the compiler loses
+    // count of the loads that follow the scales' and waits for those of the k-tile ahead.)
+    auto k_tile = [&](int kt, auto tail, auto whole) {
+      constexpr bool TAIL = decltype(tail)::value;
+      // Read phase. A(kt + 1) goes to the stage A(kt - 1) used and B(kt + 2) to the one
+      // B(kt - 1) used: both groups have read those.
+      if (SCALE == kScaleF32 || (kt & 3) == 0) sc.load(kt);
+      else sc.shift();
+      __builtin_amdgcn_sched_barrier(0);
+      if (!TAIL)
+        load(first ? kt + 1 : kt + 2,
+             first ? sA + (ast ^ kFTileBytes) : sB + (bst == 0 ? 2 * kFTileBytes : bst - kFTileBytes), whole);
+      else if (first && kt + 1 < ke)
+        load(kt + 1, sA + (ast ^ kFTileBytes), whole);
+      __builtin_amdgcn_sched_barrier(0);
+      i32x8_t fa[FA], fb[FB / 2];
+#pragma unroll
+      for (int i = 0; i < FA; ++i) fa[i] = fp8_frag(sA + ast, aoff + 2048 * i);
+#pragma unroll
+      for (int j = 0; j < FB / 2; ++j) fb[j] = fp8_frag(sB + bst, boff + 2048 * j);
+      __builtin_amdgcn_sched_barrier(0);
+      // B(kt + 1) has landed (only the second group has older operand loads in flight here), and
+      // this wave's reads are done. In the last k-tile neither group has a load in flight from
+      // here on, so that the first group's epilogue may stage through LDS.
+      if (!TAIL) __builtin_amdgcn_s_waitcnt(wait_vmcnt(kFIns));
+      if (TAIL && !first) __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      // MFMA phase. The second half of B's blocks is read into the first half's registers as
+      // those are used up; B(kt)'s stage is not refilled before the next phase but one.
+#pragma unroll
+      for (int j = 0; j < FB; ++j) {
+#pragma unroll
+        for (int i = 0; i < FA; ++i) sc.mac(acc.v[i][j], fb[j % (FB / 2)], fa[i], i, j);
+        // Keeps these MFMAs before the read below and the barrier.
+        asm volatile("" : "+v"(acc.v[0][j]), "+v"(acc.v[1][j]), "+v"(acc.v[2][j]), "+v"(acc.v[3][j])::"memory");
+        if (j < FB / 2) fb[j] = fp8_frag(sB + bst, boff + 2048 * (j + FB / 2));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (first) __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));  // A(kt + 1) has landed
+      // The second group's last MFMA phase ends the loop: the first group is past it.
+      if (!TAIL || first || kt + 1 < ke) __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      ast ^= kFTileBytes;
+      bst = bst == 2 * kFTileBytes ? 0 : bst + kFTileBytes;
+    };
+    int kt = 0;
+    for (; kt + 3 < ke; ++kt) k_tile(kt, std::false_type{}, std::true_type{});
+    if (kt + 2 < ke) k_tile(kt++, std::false_type{}, std::false_type{});
+    for (; kt < ke; ++kt) k_tile(kt, std::true_type{}, std::false_type{});
+    Fp8Epi::run(p, acc, row0_a + wm * TM, row0_b + wn * TN, lane, tm, tn, wn, fsmem + wave * kFStageWave);
+    __builtin_amdgcn_s_barrier();
+  }
 }
 
 }  // namespace ws
