@@ -61,17 +61,26 @@ __device__ __forceinline__ unsigned load_u32(__amdgpu_buffer_rsrc_t rs, unsigned
   return __builtin_amdgcn_raw_buffer_load_b32(rs, off, soff, 0);
 }
 
-// The scales of one wave's FA x FB blocks for one k-tile at a time. BROW: B has a scale per
-// row; otherwise the wave's columns lie in one block of 128.
+// The scales of one wave's FA x FB blocks for one k-tile at a time: load() requests them,
+// ready() makes them usable once they are there. BROW: B has a scale per row; otherwise the
+// wave's columns lie in one block of 128.
+//
+// e8m0: a lane requests the dword of one row, so that one load covers 64 rows, and ready()
+// hands lane l the words of rows 16 i + (l & 15) through the LDS crossbar. (With a load per
+// block, 4 lanes asking for each of its 16 rows, the 12 loads every four k-tiles cost a
+// 11264 x 2048 x 16384 product a fifth of its time: 411 us against 324 with B in blocks.)
 template <int SCALE, bool BROW, int FA, int FB>
 struct WaveScales {
   static constexpr bool kE8 = SCALE == kScaleE8M0;
   static constexpr int NB = BROW ? FB : 1;
   static constexpr int kWords = kE8 || !BROW ? 1 : 4;  // per B block: a lane's four columns under FP32
+  static constexpr int LA = kE8 ? (16 * FA + 63) / 64 : FA;
+  static constexpr int LB = kE8 && BROW ? (16 * FB + 63) / 64 : NB;
   const char *base_a, *base_b;
   long step_a, step_b;  // bytes per k-tile (FP32)
-  unsigned off_a[FA], off_b[NB];
+  unsigned off_a[LA], off_b[LB];
   unsigned a[FA], b[NB][kWords];
+  unsigned raw_a[kE8 ? LA : 1], raw_b[kE8 ? LB : 1];
 
   // m_base, n_base: first row and column of the wave's tile.
   __device__ __forceinline__ void init(const Fp8Params& p, int m_base, int n_base, int M, int N,
@@ -86,21 +95,28 @@ struct WaveScales {
     step_a = p.a.ld * unit;
     step_b = p.b.ld * unit;
 #pragma unroll
-    for (int i = 0; i < FA; ++i) {
-      const long r = (min(m_base + 16 * i + (lane & 15), M - 1) >> p.a.shift) - ra;
-      off_a[i] = (unsigned)(r * (kE8 ? p.a.ld : 4));
+    for (int i = 0; i < LA; ++i) {
+      const int row = m_base + (kE8 ? 64 * i + lane % (FA < 4 ? 16 * FA : 64) : 16 * i + (lane & 15));
+      off_a[i] = (unsigned)(((min(row, M - 1) >> p.a.shift) - ra) * (kE8 ? p.a.ld : 4));
     }
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
+    for (int j = 0; j < LB; ++j) {
       if constexpr (!BROW) off_b[j] = 0;
-      else if constexpr (kE8) off_b[j] = (unsigned)((min(n_base + 16 * j + (lane & 15), N - 1) - rb) * p.b.ld);
+      else if constexpr (kE8) off_b[j] = (unsigned)((min(n_base + 64 * j + lane % (FB < 4 ? 16 * FB : 64), N - 1) - rb) * p.b.ld);
       else off_b[j] = (unsigned)(4 * (min(n_base + 16 * j + 4 * (lane >> 4), (N - 1) & ~3) - rb));
     }
   }
-  // Issues the loads of k-tile kt (e8m0: of kt .. kt + 3, kt a multiple of 4).
+  // Requests the scales of k-tile kt (e8m0: of kt .. kt + 3, kt a multiple of 4).
   __device__ __forceinline__ void load(int kt) {
     __amdgpu_buffer_rsrc_t ra = make_rsrc(base_a + (kE8 ? (long)kt : kt * step_a), 0x7fffffff);
     __amdgpu_buffer_rsrc_t rb = make_rsrc(base_b + (kE8 ? (long)kt : kt * step_b), 0x7fffffff);
+    if constexpr (kE8) {
+#pragma unroll
+      for (int i = 0; i < LA; ++i) raw_a[i] = load_u32(ra, off_a[i], 0);
+#pragma unroll
+      for (int j = 0; j < LB; ++j) raw_b[j] = load_u32(rb, off_b[j], 0);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < FA; ++i) a[i] = load_u32(ra, off_a[i], 0);
 #pragma unroll
@@ -114,6 +130,18 @@ struct WaveScales {
       }
     }
   }
+  // e8m0, after a load(): the words to the lanes that use them.
+  __device__ __forceinline__ void ready(int lane) {
+    if constexpr (kE8) {
+#pragma unroll
+      for (int i = 0; i < FA; ++i)
+        a[i] = (unsigned)__builtin_amdgcn_ds_bpermute(4 * (16 * (i % 4) + (lane & 15)), (int)raw_a[i / 4]);
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        b[j][0] = BROW ? (unsigned)__builtin_amdgcn_ds_bpermute(4 * (16 * (j % 4) + (lane & 15)), (int)raw_b[BROW ? j / 4 : 0])
+                       : raw_b[0];
+    }
+  }
   // e8m0: on to the next k-tile's byte.
   __device__ __forceinline__ void shift() {
 #pragma unroll
@@ -121,22 +149,22 @@ struct WaveScales {
 #pragma unroll
     for (int j = 0; j < NB; ++j) b[j][0] >>= 8;
   }
-  // acc += scaled product of A block i and B block j.
+  // Scaled product of A block i and B block j, added to acc (e8m0).
   __device__ __forceinline__ void mac(f32x4_v& acc, i32x8_t fb, i32x8_t fa, int i, int j) const {
-    if constexpr (kE8) {
-      acc = mfma_e4m3_scaled(fb, fa, acc, b[BROW ? j : 0][0], a[i]);
+    if constexpr (kE8) acc = mfma_e4m3_scaled(fb, fa, acc, b[BROW ? j : 0][0], a[i]);
+    else add(acc, mfma_e4m3(fb, fa, f32x4_v{0.f, 0.f, 0.f, 0.f}), i, j);
+  }
+  // FP32: acc += p times the blocks' scales.
+  __device__ __forceinline__ void add(f32x4_v& acc, f32x4_v p, int i, int j) const {
+    const float sa = __uint_as_float(a[i]);
+    if constexpr (BROW) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        acc[e] = __builtin_fmaf(p[e], sa * __uint_as_float(b[j][e < kWords ? e : 0]), acc[e]);
     } else {
-      const f32x4_v p = mfma_e4m3(fb, fa, f32x4_v{0.f, 0.f, 0.f, 0.f});
-      const float sa = __uint_as_float(a[i]);
-      if constexpr (BROW) {
+      const float s = sa * __uint_as_float(b[0][0]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          acc[e] = __builtin_fmaf(p[e], sa * __uint_as_float(b[j][e < kWords ? e : 0]), acc[e]);
-      } else {
-        const float s = sa * __uint_as_float(b[0][0]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(p[e], s, acc[e]);
-      }
+      for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(p[e], s, acc[e]);
     }
   }
 };
@@ -223,6 +251,7 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_fp8_ring_kernel(const GemmParams
     __builtin_amdgcn_s_barrier();
     if constexpr (Scales::kE8) {
       if ((kt & 3) == 0) {
+        nxt.ready(lane);
         cur = nxt;
         if (kt + 4 < ke) nxt.load(kt + 4);
       } else {
@@ -272,6 +301,11 @@ __device__ __forceinline__ i32x8_t fp8_frag(const unsigned char* tile, unsigned 
   return join_frag(*reinterpret_cast<const bf16x8_t*>(tile + at), *reinterpret_cast<const bf16x8_t*>(tile + (at ^ 64)));
 }
 
+// Keeps what made these values before the LDS reads and barriers that follow.
+__device__ __forceinline__ void pin(f32x4_v& a, f32x4_v& b) {
+  asm volatile("" : "+v"(a), "+v"(b)::"memory");
+}
+
 template <int SCALE, bool BROW>
 __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, const Fp8Params sp) {
   constexpr int TM = kFBM / kFWM, TN = kFBN / kFWN;  // 64 x 128
@@ -300,26 +334,25 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
     WaveScales<SCALE, BROW, FA, FB> sc;
     sc.init(sp, row0_a + wm * TM, row0_b + wn * TN, p.M, p.N, lane);
 
-    typedef RingTile<256, 256, kKContig, false> Tile;
-    const int gw = wave & 3;
-    Tile l;
-    if (first) l.init(p.a, row0_a, p.M, 0, gw, lane);
-    else l.init(p.b, row0_b, p.N, 0, gw, lane);
+    // This wave's share of its group's operand tile: one quarter, eight loads of 8 rows each,
+    // 32 rows apart. Rows past the matrix take the last one's bytes (their results are not
+    // stored), so the offsets need no registers of their own: three instructions per load,
+    // against eight registers, which the FP32 scales' partial products need.
+    const int gw = wave & 3, r0 = gw * 8 + (lane >> 3), c16 = 16 * ((lane & 7) ^ swz(r0));
+    const int r_last = (first ? p.M - row0_a : p.N - row0_b) - 1;
+    const unsigned ld = (unsigned)(2 * (first ? p.a.s_row : p.b.s_row));
     const unsigned short* base = first ? p.a.ptr + (long)row0_a * p.a.s_row : p.b.ptr + (long)row0_b * p.b.s_row;
     auto load = [&](int kt, unsigned char* stage, auto whole) {
       __amdgpu_buffer_rsrc_t rs = make_rsrc(base + (long)kt * kFBK, 0x7fffffff);
       unsigned char* dst = stage + gw * 1024;
-      if (decltype(whole)::value || (kt + 1) * kFBK <= p.K) {
+      int r = r0;
+      asm volatile("" : "+v"(r));  // not hoisted out of the loop
+      // Chunks at k >= K land as zeros.
+      const bool ok = decltype(whole)::value || kt * kFBK + (c16 >> 1) < p.K;
 #pragma unroll
-        for (int i = 0; i < kFIns; ++i) dma16(rs, dst + i * 4096, l.off[i]);
-      } else {
-        // Ragged: chunks at k >= K land as zeros. The lane index goes through an empty asm so
-        // that the k offsets are not kept live across the loop.
-        int q = lane;
-        asm volatile("" : "+v"(q));
-#pragma unroll
-        for (int i = 0; i < kFIns; ++i)
-          dma16(rs, dst + i * 4096, kt * kFBK + Tile::k_of(i, gw, q) >= p.K ? kOOB : l.off[i]);
+      for (int i = 0; i < kFIns; ++i) {
+        const unsigned off = __umul24((unsigned)min(r + 32 * i, r_last), ld) + (unsigned)c16;
+        dma16(rs, dst + i * 4096, ok ? off : kOOB);
       }
     };
     if (first) {
@@ -364,18 +397,44 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
       // here on, so that the first group's epilogue may stage through LDS.
       if (!TAIL) __builtin_amdgcn_s_waitcnt(wait_vmcnt(kFIns));
       if (TAIL && !first) __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
+      if (SCALE == kScaleE8M0 && (kt & 3) == 0) sc.ready(lane);
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
       // MFMA phase. The second half of B's blocks is read into the first half's registers as
       // those are used up; B(kt)'s stage is not refilled before the next phase but one.
+      if constexpr (SCALE == kScaleE8M0) {
 #pragma unroll
-      for (int j = 0; j < FB; ++j) {
+        for (int j = 0; j < FB; ++j) {
 #pragma unroll
-        for (int i = 0; i < FA; ++i) sc.mac(acc.v[i][j], fb[j % (FB / 2)], fa[i], i, j);
-        // Keeps these MFMAs before the read below and the barrier.
-        asm volatile("" : "+v"(acc.v[0][j]), "+v"(acc.v[1][j]), "+v"(acc.v[2][j]), "+v"(acc.v[3][j])::"memory");
-        if (j < FB / 2) fb[j] = fp8_frag(sB + bst, boff + 2048 * (j + FB / 2));
+          for (int i = 0; i < FA; ++i) sc.mac(acc.v[i][j], fb[j % (FB / 2)], fa[i], i, j);
+          pin(acc.v[0][j], acc.v[1][j]);
+          pin(acc.v[2][j], acc.v[3][j]);
+          if (j < FB / 2) fb[j] = fp8_frag(sB + bst, boff + 2048 * (j + FB / 2));
+          // (Left to the scheduler, all four reads go through one block's registers, each
+          // waited for at once.)
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        // The additions of two blocks run behind the next two blocks' MFMAs.
+        f32x4_v prod[2][2];
+#pragma unroll
+        for (int q = 0; q <= 2 * FB; ++q) {
+          const int j = q / 2, i = 2 * (q % 2);
+          if (q < 2 * FB) {
+            prod[q & 1][0] = mfma_e4m3(fb[j % (FB / 2)], fa[i], f32x4_v{0.f, 0.f, 0.f, 0.f});
+            prod[q & 1][1] = mfma_e4m3(fb[j % (FB / 2)], fa[i + 1], f32x4_v{0.f, 0.f, 0.f, 0.f});
+            pin(prod[q & 1][0], prod[q & 1][1]);
+            if (i == 2 && j < FB / 2) fb[j] = fp8_frag(sB + bst, boff + 2048 * (j + FB / 2));
+          }
+          if (q > 0) {
+            const int jp = (q - 1) / 2, ip = 2 * ((q - 1) % 2);
+            sc.add(acc.v[ip][jp], prod[(q - 1) & 1][0], ip, jp);
+            sc.add(acc.v[ip + 1][jp], prod[(q - 1) & 1][1], ip + 1, jp);
+            pin(acc.v[ip][jp], acc.v[ip + 1][jp]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
       if (first) __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));  // A(kt + 1) has landed
