@@ -410,10 +410,18 @@ int ws_fp8_pack(const void* src, int64_t s_row, int64_t s_col, void* dst, int64_
  * to be zero: ws_fp8_pack). *_block_rows is 1 (a scale per row and block) or 128 (per 128 rows
  * and block). e8m0 scales: 4-byte aligned, ld a multiple of 4, rows readable to the next
  * multiple of 4 bytes. FP32 scales of B with b_block_rows 1: 16-byte aligned, ld a multiple of
- * 4. */
+ * 4. `workspace`: 16-byte aligned, ws_fp8_mm_workspace_bytes (null if that is 0): slices of the
+ * reduction where the tiles alone would leave compute units idle. */
+int64_t ws_fp8_mm_workspace_bytes(int64_t m, int64_t n, int64_t k, int b_block_rows, int scale_type);
+/* What ws_fp8_mm runs these sizes on, without a launch: 0 256 x 256, 1 and 2 128 x 128 (two or
+ * one workgroup on a compute unit), 3 64 x 128, 4 64 x 64, 5 the kernel for few rows; -1 for
+ * invalid sizes. workspace_bytes and splits (slices of the reduction) are nullable. */
+int ws_fp8_mm_plan(int64_t m, int64_t n, int64_t k, int b_block_rows, int scale_type,
+                   int64_t* workspace_bytes, int* splits);
 int ws_fp8_mm(const void* a, int64_t lda, const void* scale_a, int64_t ld_scale_a, int a_block_rows,
               const void* b, int64_t ldb, const void* scale_b, int64_t ld_scale_b, int b_block_rows,
-              int scale_type, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k, void* stream);
+              int scale_type, void* c, int64_t ldc, int64_t m, int64_t n, int64_t k,
+              void* workspace, void* stream);
 
 /* --- token scores ---------------------------------------------------------------------
  *

@@ -49,7 +49,7 @@ def test_quantization_arguments(over, match):
 
 def _mm(**over):
     a = dict(a=P, lda=256, sa=P, ld_sa=4, ra=1, b=P, ldb=256, sb=P, ld_sb=4, rb=128, scale=0, c=P,
-             ldc=8, m=8, n=8, k=256)
+             ldc=8, m=8, n=8, k=256, ws=None)
     a.update(over)
     _hip.call("ws_fp8_mm", *a.values(), None)
 
@@ -62,7 +62,8 @@ def _mm(**over):
     (dict(ldc=4_200_000), "row stride"), (dict(sa=None), "null scale"), (dict(ld_sa=3), "e8m0"),
     (dict(ld_sb=0), "e8m0"), (dict(scale=1, ld_sa=7), "FP32 scales of A"),
     (dict(scale=1, ld_sa=8, rb=1, ld_sb=10), "FP32 scales of B"),
-    (dict(scale=1, ld_sa=8, rb=1, ld_sb=8, sb=P + 4), "FP32 scales of B")])
+    (dict(scale=1, ld_sa=8, rb=1, ld_sb=8, sb=P + 4), "FP32 scales of B"),
+    (dict(m=64, k=8192, lda=8192, ldb=8192, ld_sa=64, ld_sb=64), "workspace")])
 def test_product_arguments(over, match):
     with pytest.raises(RuntimeError, match=match):
         _mm(**over)
@@ -90,3 +91,25 @@ def test_reference_rounding_is_e4m3():
     x = np.concatenate([x, -x]).astype(np.float32)
     want = torch.from_numpy(x).to(E4M3).double().numpy()
     np.testing.assert_array_equal(e4m3_round(x.astype(np.float64)), want)
+
+
+def _plan(m, n, k, rows=128, scale=0):
+    import ctypes
+
+    need, splits = ctypes.c_int64(), ctypes.c_int()
+    tile = _hip.library().ws_fp8_mm_plan(m, n, k, rows, scale, ctypes.byref(need), ctypes.byref(splits))
+    return tile, need.value, splits.value
+
+
+def test_plans():
+    """Few rows take their own kernel, full rounds of 256 x 256 tiles run whole, and tiles that
+    would leave compute units idle are split along the reduction, with room for every slice."""
+    assert _plan(1, 2048, 5632)[0] == 5 and _plan(32, 2048, 5632)[0] == 5
+    assert _plan(8192, 8192, 8192) == (0, 0, 1)
+    assert _plan(0, 8, 16)[0] == -1
+    for shape in ((64, 2048, 5632), (128, 1280, 4480), (11264, 2048, 16384), (1280, 1280, 16384)):
+        tile, need, splits = _plan(*shape)
+        assert splits > 1 and need % (4 * splits) == 0 and need > 0, shape
+        assert _hip.query("ws_fp8_mm_workspace_bytes", *shape, 128, 0) == need
+    # FP32 scales by rows never take the 256 x 256 tile.
+    assert all(_plan(m, 8192, 4096, 1, 1)[0] != 0 for m in (512, 4096, 16384))

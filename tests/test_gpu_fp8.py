@@ -150,6 +150,51 @@ def test_exact_product(m, n, k, a_blocks, b_blocks, scale_dtype):
     assert torch.equal(got.cpu(), want)
 
 
+# (m, n, k, tile of ws_fp8_mm_plan, split): every macro-tile, whole and in slices of the
+# reduction, ragged in every dimension.
+PLANNED = [(2937, 3001, 128, 0, False), (3300, 2700, 1000, 0, False), (3717, 4947, 688, 0, True),
+           (1380, 3173, 128, 1, False), (198, 5393, 9232, 1, True), (1020, 3933, 2864, 2, False),
+           (73, 5450, 9472, 2, True), (286, 6767, 128, 3, False), (285, 3444, 4368, 3, True),
+           (34, 33, 160, 4, False), (37, 39, 1168, 4, True), (64, 2048, 5632, 4, True),
+           (32, 37, 176, 5, False), (17, 2000, 2064, 5, False)]
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+@pytest.mark.parametrize("a_blocks,b_blocks", KINDS)
+@pytest.mark.parametrize("m,n,k,tile,split", PLANNED)
+def test_exact_product_on_every_tile(m, n, k, tile, split, a_blocks, b_blocks, scale_dtype):
+    """As test_exact_product, the reference an FP32 product on the GPU: sums of at most 9472
+    products of at most 16 in units of 1/4 need 21 bits, so FP32 holds them exactly."""
+    import ctypes
+
+    from ops import _hip
+
+    splits = ctypes.c_int()
+    plan = _hip.library().ws_fp8_mm_plan(m, n, -(-k // 16) * 16, BLOCK if b_blocks else 1,
+                                         int(scale_dtype == F32), None, ctypes.byref(splits))
+    if scale_dtype == F32 and not b_blocks and tile == 0:
+        assert plan != 0  # no such kernel: the product runs on smaller tiles
+    else:
+        assert (plan, splits.value > 1) == (tile, split)
+    g = torch.Generator("cuda").manual_seed(m + n + k)
+    kb = -(-k // BLOCK)
+
+    def operand(rows, blocks):
+        q = torch.randint(-2, 3, (rows, k), generator=g, device="cuda").float()
+        r = -(-rows // BLOCK) if blocks else rows
+        scale = torch.randint(-1, 2, (r, kb), generator=g, device="cuda").float().exp2()
+        wide = scale.repeat_interleave(BLOCK if blocks else 1, 0)[:rows]
+        return q.to(E4M3), scale, q * wide.repeat_interleave(BLOCK, 1)[:, :k]
+
+    a, sa, fa = operand(m, a_blocks)
+    b, sb, fb = operand(n, b_blocks)
+    cast = (lambda s: (s.log2() + 127).to(torch.uint8).view(E8M0)) if scale_dtype == E8M0 else (lambda s: s)
+    guard = torch.full((m + 2, n), 3.0, dtype=BF16, device="cuda")
+    got = _fp8().fp8_mm(a, cast(sa), b, cast(sb), out=guard[1:-1])
+    assert torch.equal(got, (fa @ fb.T).to(BF16))
+    assert bool((guard[0] == 3.0).all()) and bool((guard[-1] == 3.0).all())
+
+
 @pytest.mark.parametrize("scale_dtype", SCALES)
 def test_product_of_other_layouts(scale_dtype):
     """Operands by columns, odd strides and unaligned starts, scales in the other order, and an

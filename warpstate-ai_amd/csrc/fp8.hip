@@ -28,6 +28,60 @@ int dispatch_quantize(const QuantParams& p, int form, bool vec, hipStream_t s) {
   return set_error(kInvalid, "unknown quantization form %d", form);
 }
 
+// How a product runs: a macro-tile (FastTile), or kTileFew, and the slices along K of the
+// tiles from `whole` on.
+constexpr int kTileFew = kFastTiles;
+struct Fp8Plan {
+  int tile, whole, splits, slice_kt;
+  long partials;  // floats
+};
+
+// us of adding `splits` slices of `tiles` tiles (written and read once, mostly in cache).
+inline float join_time(long tiles, int bm, int bn, int splits) {
+  return 3.0f + (float)tiles * (float)(bm * bn) * 8.0f * (float)splits / 6e6f;
+}
+
+// The macro-tile by the BF16 kernels' cost table: a k-tile of 128 bytes a row takes as many LDS
+// bytes and as much matrix-pipe time in either type.
+Fp8Plan fp8_plan(long m, long n, long k, bool brow, int scale_type) {
+  const long pairs = k / 2;  // the loaders' count
+  const int kt = cdiv(pairs, kFBK), cus = device_cus();
+  Fp8Plan best{kTileFew, 0, 1, kt, 0};
+  if (m <= 32) return best;
+  float t = 1e30f;
+  for (int tile = 0; tile < kFastTiles; ++tile) {
+    if (tile == kTile256 && scale_type == kScaleF32 && brow) continue;  // (would not fit the registers)
+    const TileCost& c = tile_cost(tile, kKContig, kKContig);
+    const long tiles = (long)cdiv(m, c.bm) * cdiv(n, c.bn);
+    const int whole = tile == kTile256 ? (int)(tiles / cus * cus) : 0;
+    const long rest = tiles - whole;
+    float plain = tile_time(tile, m, n, pairs, kKContig, kKContig, cus, false, kEpiStore);
+    if (plain < t) {
+      t = plain;
+      best = Fp8Plan{tile, (int)tiles, 1, kt, 0};
+    }
+    const int room = cus * (c.pair > 0.0f ? 2 : 1);  // workgroups at once
+    for (int want = 2; rest > 0 && want <= 16 && rest * want <= room; ++want) {
+      const int slice = cdiv(cdiv(kt, want), 4) * 4, splits = cdiv(kt, slice);
+      if (splits < 2 || rest * splits > room) continue;
+      const bool paired = rest * splits > cus;
+      float time = (float)(whole / cus) * (c.alone * (float)kt + c.fixed) +
+                   (paired ? c.pair : c.alone) * (float)slice + c.fixed + join_time(rest, c.bm, c.bn, splits);
+      if (time < t) {
+        t = time;
+        best = Fp8Plan{tile, whole, splits, slice, rest * splits * c.bm * c.bn};
+      }
+    }
+  }
+  return best;
+}
+
+template <int BM, int BN>
+int run_join(const GemmParams& p, const Fp8Params& sp, int window, hipStream_t s) {
+  hipLaunchKernelGGL((fp8_join_kernel<BM, BN>), dim3(BM * BN / 1024, p.total_tiles - sp.whole), dim3(256), 0, s, p,
+                     sp, window);
+  return hip_check(hipGetLastError(), "8-bit product join launch");
+}
 template <class Cfg, int SCALE, bool BROW>
 int run_fp8_ring(GemmParams p, const Fp8Params& sp, hipStream_t s) {
   const void* kern = reinterpret_cast<const void*>(&gemm_fp8_ring_kernel<Cfg, SCALE, BROW>);
@@ -35,9 +89,10 @@ int run_fp8_ring(GemmParams p, const Fp8Params& sp, hipStream_t s) {
   p.tiles_m = cdiv(p.M, Cfg::BM);
   p.tiles_n = cdiv(p.N, Cfg::BN);
   p.total_tiles = p.tiles_m * p.tiles_n;
-  hipLaunchKernelGGL((gemm_fp8_ring_kernel<Cfg, SCALE, BROW>), dim3(p.total_tiles), dim3(Cfg::NT),
+  hipLaunchKernelGGL((gemm_fp8_ring_kernel<Cfg, SCALE, BROW>), dim3(p.total_tiles, sp.splits), dim3(Cfg::NT),
                      Cfg::kLds, s, p, sp);
-  return hip_check(hipGetLastError(), "8-bit product launch");
+  if (int rc = hip_check(hipGetLastError(), "8-bit product launch")) return rc;
+  return sp.splits > 1 ? run_join<Cfg::BM, Cfg::BN>(p, sp, kRingWindow, s) : kOk;
 }
 template <int SCALE, bool BROW>
 int run_fp8_256(GemmParams p, const Fp8Params& sp, hipStream_t s) {
@@ -46,24 +101,34 @@ int run_fp8_256(GemmParams p, const Fp8Params& sp, hipStream_t s) {
   p.tiles_m = cdiv(p.M, kFBM);
   p.tiles_n = cdiv(p.N, kFBN);
   p.total_tiles = p.tiles_m * p.tiles_n;
-  const int cus = device_cus();
-  hipLaunchKernelGGL((gemm_fp8_kernel<SCALE, BROW>), dim3(p.total_tiles < cus ? p.total_tiles : cus),
-                     dim3(kFNT), kFLdsBytes, s, p, sp);
+  const int cus = device_cus(), items = sp.whole + (p.total_tiles - sp.whole) * sp.splits;
+  const int grid = items < cus ? items : cus;
+  hipLaunchKernelGGL((gemm_fp8_kernel<SCALE, BROW>), dim3(grid), dim3(kFNT), kFLdsBytes, s, p, sp);
+  if (int rc = hip_check(hipGetLastError(), "8-bit product launch")) return rc;
+  return sp.splits > 1 ? run_join<kFBM, kFBN>(p, sp, grid, s) : kOk;
+}
+template <int FA, int FB, int SCALE, bool BROW>
+int run_fp8_skinny(const GemmParams& p, const Fp8Params& sp, hipStream_t s) {
+  hipLaunchKernelGGL((gemm_fp8_skinny_kernel<FA, FB, SCALE, BROW>), dim3(cdiv(p.N, 16 * FB)), dim3(512), 0, s, p, sp);
   return hip_check(hipGetLastError(), "8-bit product launch");
 }
+template <int FB, int SCALE, bool BROW>
+int run_fp8_few(const GemmParams& p, const Fp8Params& sp, hipStream_t s) {
+  return p.M <= 16 ? run_fp8_skinny<1, FB, SCALE, BROW>(p, sp, s) : run_fp8_skinny<2, FB, SCALE, BROW>(p, sp, s);
+}
 template <int SCALE, bool BROW>
-int run_fp8(const GemmParams& p, const Fp8Params& sp, hipStream_t s) {
-  const int tile = pick_tile(p.M, p.N, p.K, kKContig, kKContig, false, kEpiStore);
+int run_fp8(const GemmParams& p, const Fp8Params& sp, int tile, hipStream_t s) {
   switch (tile) {
+    case kTileFew: return run_fp8_few<1, SCALE, BROW>(p, sp, s);
     case kTile256:
-      // (FP32 scales of B per row would not fit the registers.)
       if constexpr (SCALE == kScaleE8M0 || !BROW) return run_fp8_256<SCALE, BROW>(p, sp, s);
-      [[fallthrough]];
+      break;
     case kTile128x2: return run_fp8_ring<Ring128x2, SCALE, BROW>(p, sp, s);
     case kTile128x1: return run_fp8_ring<Ring128x1, SCALE, BROW>(p, sp, s);
     case kTile64x128: return run_fp8_ring<Ring64x128, SCALE, BROW>(p, sp, s);
-    default: return run_fp8_ring<Ring64, SCALE, BROW>(p, sp, s);
+    case kTile64: return run_fp8_ring<Ring64, SCALE, BROW>(p, sp, s);
   }
+  return set_error(kInvalid, "no 8-bit macro-tile %d", tile);
 }
 
 int check_scale(const Fp8Scale& s, long rows, long k_blocks, int type, bool vec4, const char* which) {
@@ -151,10 +216,29 @@ extern "C" int ws_fp8_pack(const void* src, int64_t s_row, int64_t s_col, void* 
   return hip_check(hipGetLastError(), "pack launch");
 }
 
+extern "C" int ws_fp8_mm_plan(int64_t m, int64_t n, int64_t k, int b_block_rows, int scale_type,
+                              int64_t* workspace_bytes, int* splits) {
+  if (m < 1 || n < 1 || k < 1 || !fits_i32(m) || !fits_i32(n) || !fits_i32(k)) {
+    set_error(kInvalid, "matrix sizes must be positive 32-bit integers");
+    return -1;
+  }
+  const Fp8Plan plan = fp8_plan(m, n, k, b_block_rows == 1, scale_type);
+  if (workspace_bytes) *workspace_bytes = plan.partials * 4;
+  if (splits) *splits = plan.splits;
+  return plan.tile;
+}
+
+extern "C" int64_t ws_fp8_mm_workspace_bytes(int64_t m, int64_t n, int64_t k, int b_block_rows,
+                                             int scale_type) {
+  int64_t bytes = 0;
+  ws_fp8_mm_plan(m, n, k, b_block_rows, scale_type, &bytes, nullptr);
+  return bytes;
+}
+
 extern "C" int ws_fp8_mm(const void* a, int64_t lda, const void* scale_a, int64_t ld_scale_a,
                          int a_block_rows, const void* b, int64_t ldb, const void* scale_b,
                          int64_t ld_scale_b, int b_block_rows, int scale_type, void* c, int64_t ldc,
-                         int64_t m, int64_t n, int64_t k, void* stream) {
+                         int64_t m, int64_t n, int64_t k, void* workspace, void* stream) {
   if (!a || !b || !c) return set_error(kInvalid, "null operand pointer");
   if (m < 1 || n < 1 || k < 1 || !fits_i32(m) || !fits_i32(n) || !fits_i32(k))
     return set_error(kInvalid, "matrix sizes must be positive 32-bit integers (m=%ld n=%ld k=%ld)",
@@ -170,7 +254,11 @@ extern "C" int ws_fp8_mm(const void* a, int64_t lda, const void* scale_a, int64_
   if (ldc < n) return set_error(kInvalid, "output leading dimension < n");
   if (!al(c, 2)) return set_error(kInvalid, "misaligned output");
   if (int rc = check_out_stride(ldc, 2, "output")) return rc;
-  Fp8Params sp{{scale_a, ld_scale_a, a_block_rows == 1 ? 0 : 7}, {scale_b, ld_scale_b, b_block_rows == 1 ? 0 : 7}};
+  const Fp8Plan plan = fp8_plan(m, n, k, b_block_rows == 1, scale_type);
+  if (plan.partials && (!workspace || !al(workspace, 16)))
+    return set_error(kInvalid, "this product needs a 16-byte aligned workspace");
+  const Fp8Params sp{{scale_a, ld_scale_a, a_block_rows == 1 ? 0 : 7}, {scale_b, ld_scale_b, b_block_rows == 1 ? 0 : 7},
+                     plan.whole, plan.splits, plan.slice_kt, static_cast<float*>(workspace)};
   const long k_blocks = cdiv(k, kQBlock);
   if (int rc = check_scale(sp.a, m, k_blocks, scale_type, false, "A")) return rc;
   if (int rc = check_scale(sp.b, n, k_blocks, scale_type, b_block_rows == 1, "B")) return rc;
@@ -185,6 +273,6 @@ extern "C" int ws_fp8_mm(const void* a, int64_t lda, const void* scale_a, int64_
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool brow = b_block_rows == 1;
   if (scale_type == kScaleE8M0)
-    return brow ? run_fp8<kScaleE8M0, true>(p, sp, s) : run_fp8<kScaleE8M0, false>(p, sp, s);
-  return brow ? run_fp8<kScaleF32, true>(p, sp, s) : run_fp8<kScaleF32, false>(p, sp, s);
+    return brow ? run_fp8<kScaleE8M0, true>(p, sp, plan.tile, s) : run_fp8<kScaleE8M0, false>(p, sp, plan.tile, s);
+  return brow ? run_fp8<kScaleF32, true>(p, sp, plan.tile, s) : run_fp8<kScaleF32, false>(p, sp, plan.tile, s);
 }

@@ -38,8 +38,13 @@ struct Fp8Scale {
   long ld;
   int shift;
 };
+// Tiles of the raster from `whole` on are split along K into `splits` slices of slice_kt
+// k-tiles (a multiple of 4: a dword of e8m0 scales), whose FP32 sums go to blocks of
+// BM x BN floats (tile, slice) of `partials`; fp8_join_kernel adds them.
 struct Fp8Params {
   Fp8Scale a, b;
+  int whole, splits, slice_kt;
+  float* partials;
 };
 
 __device__ __forceinline__ i32x8_t join_frag(bf16x8_t lo, bf16x8_t hi) {
@@ -203,7 +208,41 @@ struct Fp8Epi {
   }
 };
 
-// Macro-tiles up to 128 x 128 (RingCfg): S LDS stages, one workgroup per tile. The scales of a
+// A tile's sums as FP32, rows of `width` floats; `block` is this wave's first element.
+template <int FA, int FB>
+__device__ __forceinline__ void fp8_partial(Acc16<FA, FB>& acc, float* block, int width, int lane) {
+  opaque_lane(lane);
+#pragma unroll
+  for (int i = 0; i < FA; ++i)
+#pragma unroll
+    for (int j = 0; j < FB; ++j)
+      *reinterpret_cast<f32x4_v*>(block + (16 * i + (lane & 15)) * width + 16 * j + 4 * (lane >> 4)) = acc.v[i][j];
+}
+
+// Adds the slices of split tiles in order and rounds once. blockIdx.y is the tile after
+// `whole`; a block of 256 threads takes 1024 elements.
+template <int BM, int BN>
+static __global__ void __launch_bounds__(256) fp8_join_kernel(const GemmParams p, const Fp8Params sp, int window) {
+  int tm, tn;
+  tile_position(xcd_remap(sp.whole + blockIdx.y, p.total_tiles, window), p.tiles_m, p.tiles_n, tm, tn);
+  const int e = (blockIdx.x * 256 + threadIdx.x) * 4;
+  const int m = tm * BM + e / BN, n = tn * BN + e % BN;
+  if (m >= p.M || n >= p.N) return;
+  const float* src = sp.partials + (long)blockIdx.y * sp.splits * (BM * BN) + e;
+  f32x4_v v = *reinterpret_cast<const f32x4_v*>(src);
+  for (int s = 1; s < sp.splits; ++s) v += *reinterpret_cast<const f32x4_v*>(src + (long)s * (BM * BN));
+  unsigned short* out = p.c + (long)m * p.ldc + n;
+  if (p.vec_out) {
+    *reinterpret_cast<u32x2_t*>(out) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < p.N) out[i] = to_bf16_bits(v[i]);
+  }
+}
+
+// Macro-tiles up to 128 x 128 (RingCfg): S LDS stages, one workgroup per tile, or per
+// slice of a tile's k-tiles. The scales of a
 // k-tile are requested before the operand loads of the same turn, so the waits that count
 // operand loads only wait for more than they need.
 template <class Cfg, int SCALE, bool BROW>
@@ -215,7 +254,7 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_fp8_ring_kernel(const GemmParams
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
-  const int ke = cdiv(p.K, kFBK);
+  const int kb = blockIdx.y * sp.slice_kt, ke = min(cdiv(p.K, kFBK), kb + sp.slice_kt);
 
   int tm, tn;
   tile_position(xcd_remap(blockIdx.x, p.total_tiles, kRingWindow), p.tiles_m, p.tiles_n, tm, tn);
@@ -242,11 +281,11 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_fp8_ring_kernel(const GemmParams
   typedef WaveScales<SCALE, BROW, FA, FB> Scales;
   Scales cur, nxt;
   nxt.init(sp, row0_a + wm * TM, row0_b + wn * TN, p.M, p.N, lane);
-  nxt.load(0);
+  nxt.load(kb);
 #pragma unroll
-  for (int s = 0; s + 1 < S; ++s) issue(s, s);
+  for (int s = 0; s + 1 < S; ++s) issue(kb + s, s);
   int rd = 0, wr = S - 1;
-  for (int kt = 0; kt < ke; ++kt) {
+  for (int kt = kb; kt < ke; ++kt) {
     __builtin_amdgcn_s_waitcnt(wait_vmcnt(kWaitLoads));
     __builtin_amdgcn_s_barrier();
     if constexpr (Scales::kE8) {
@@ -287,6 +326,11 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_fp8_ring_kernel(const GemmParams
   // epilogue's staging writes.
   __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
   __builtin_amdgcn_s_barrier();
+  if (sp.splits > 1) {
+    fp8_partial(acc, sp.partials + ((long)blockIdx.x * sp.splits + blockIdx.y) * (Cfg::BM * Cfg::BN) +
+                         wm * TM * Cfg::BN + wn * TN, Cfg::BN, lane);
+    return;
+  }
   Fp8Epi::run(p, acc, row0_a + wm * TM, row0_b + wn * TN, lane, tm, tn, wn,
            rsmem + wave * epi_wave<FA, FB>());
 }
@@ -316,15 +360,19 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / kFWN, wn = wave % kFWN;
   const bool first = wave < 4;  // the group that runs a phase ahead and loads A
-  const int ke = cdiv(p.K, kFBK);
+  const int items = sp.whole + (p.total_tiles - sp.whole) * sp.splits;
 
   unsigned char* const sA = fsmem;
   unsigned char* const sB = fsmem + 2 * kFTileBytes;
   const unsigned aoff = frag_base<kKContig>(wm * TM, lane), boff = frag_base<kKContig>(wn * TN, lane);
 
-  for (int w = blockIdx.x; w < p.total_tiles; w += gridDim.x) {
+  for (int w = blockIdx.x; w < items; w += gridDim.x) {
+    const bool slice = w >= sp.whole;
+    const int piece = w - sp.whole, tile = slice ? sp.whole + piece / sp.splits : w;
+    const int kb = slice ? piece % sp.splits * sp.slice_kt : 0;
+    const int ke = slice ? min(cdiv(p.K, kFBK), kb + sp.slice_kt) : cdiv(p.K, kFBK);
     int tm, tn;
-    tile_position(xcd_remap(w, p.total_tiles, gridDim.x), p.tiles_m, p.tiles_n, tm, tn);
+    tile_position(xcd_remap(tile, p.total_tiles, gridDim.x), p.tiles_m, p.tiles_n, tm, tn);
     const int row0_a = tm * kFBM, row0_b = tn * kFBN;
     Acc16<FA, FB> acc;
 #pragma unroll
@@ -356,13 +404,13 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
       }
     };
     if (first) {
-      load(0, sA, std::false_type{});
+      load(kb, sA, std::false_type{});
       __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
     } else {
-      load(0, sB, std::false_type{});
-      if (1 < ke) {
-        load(1, sB + kFTileBytes, std::false_type{});
-        __builtin_amdgcn_s_waitcnt(wait_vmcnt(kFIns));  // B(0)
+      load(kb, sB, std::false_type{});
+      if (kb + 1 < ke) {
+        load(kb + 1, sB + kFTileBytes, std::false_type{});
+        __builtin_amdgcn_s_waitcnt(wait_vmcnt(kFIns));  // B(kb)
       } else {
         __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
       }
@@ -444,12 +492,139 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
       ast ^= kFTileBytes;
       bst = bst == 2 * kFTileBytes ? 0 : bst + kFTileBytes;
     };
-    int kt = 0;
+    int kt = kb;
     for (; kt + 3 < ke; ++kt) k_tile(kt, std::false_type{}, std::true_type{});
     if (kt + 2 < ke) k_tile(kt++, std::false_type{}, std::false_type{});
     for (; kt < ke; ++kt) k_tile(kt, std::true_type{}, std::false_type{});
-    Fp8Epi::run(p, acc, row0_a + wm * TM, row0_b + wn * TN, lane, tm, tn, wn, fsmem + wave * kFStageWave);
+    if (slice)
+      fp8_partial(acc, sp.partials + (long)piece * (kFBM * kFBN) + wm * TM * kFBN + wn * TN, kFBN, lane);
+    else
+      Fp8Epi::run(p, acc, row0_a + wm * TM, row0_b + wn * TN, lane, tm, tn, wn, fsmem + wave * kFStageWave);
     __builtin_amdgcn_s_barrier();
+  }
+}
+
+// Few rows of A (at most 64: decoding, a short prompt): bound by reading B once. A workgroup of
+// eight waves takes all rows and 16 FB columns; the waves share the k-tiles in turn and read their
+// fragments straight from memory (B's rows as whole 128-byte lines, A's from L2), the next
+// kAhead k-tiles requested before the current ones are used, and their partial products are
+// added in LDS in wave order.
+template <int FA, int FB, int SCALE, bool BROW>
+__global__ void __launch_bounds__(512) gemm_fp8_skinny_kernel(const GemmParams p, const Fp8Params sp) {
+  constexpr int kWaves = 8, kAhead = FA + FB <= 3 ? 4 : 2;
+  constexpr bool kE8 = SCALE == kScaleE8M0;
+  constexpr int kSB = kE8 || !BROW ? 1 : 4;
+  __shared__ f32x4_v red[kWaves][FA * FB][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16 * FB;
+  const int ke = cdiv(p.K, kFBK);
+  const long lda = 2 * p.a.s_row, ldb = 2 * p.b.s_row;
+  const int kb = 2 * p.K;  // bytes of a row
+  const unsigned char *pa[FA], *pb[FB];
+  const char *psa[FA], *psb[FB];
+  const int chunk = 16 * (lane >> 4);
+#pragma unroll
+  for (int i = 0; i < FA; ++i) {
+    const int r = min(16 * i + (lane & 15), p.M - 1);
+    pa[i] = reinterpret_cast<const unsigned char*>(p.a.ptr) + r * lda + chunk;
+    const long q = r >> sp.a.shift;
+    psa[i] = static_cast<const char*>(sp.a.ptr) + (kE8 ? q * sp.a.ld : 4 * q);
+  }
+#pragma unroll
+  for (int j = 0; j < FB; ++j) {
+    const int r = min(n0 + 16 * j + (lane & 15), p.N - 1);
+    pb[j] = reinterpret_cast<const unsigned char*>(p.b.ptr) + r * ldb + chunk;
+    // FP32 by rows: a lane's four columns at once (past the end the last whole four).
+    const long q = kSB == 4 ? min(n0 + 16 * j + 4 * (lane >> 4), (p.N - 1) & ~3) : r >> sp.b.shift;
+    psb[j] = static_cast<const char*>(sp.b.ptr) + (kE8 ? q * sp.b.ld : 4 * q);
+  }
+  const long step_a = kE8 ? 1 : 4 * sp.a.ld, step_b = kE8 ? 1 : 4 * sp.b.ld;
+  struct Piece {
+    i32x8_t a[FA], b[FB];
+    unsigned sa[FA], sb[FB][kSB];
+  };
+  auto load8 = [&](const unsigned char* row, int kt) {
+    const u32x4_t zero = {0, 0, 0, 0};
+    const int at = kt * 128;
+    const u32x4_t lo = at + chunk < kb ? *reinterpret_cast<const u32x4_t*>(row + at) : zero;
+    const u32x4_t hi = at + 64 + chunk < kb ? *reinterpret_cast<const u32x4_t*>(row + at + 64) : zero;
+    return join_frag(__builtin_bit_cast(bf16x8_t, lo), __builtin_bit_cast(bf16x8_t, hi));
+  };
+  auto fetch = [&](Piece& x, int kt) {
+    if (kt >= ke) return;  // uniform
+#pragma unroll
+    for (int j = 0; j < FB; ++j) x.b[j] = load8(pb[j], kt);
+#pragma unroll
+    for (int i = 0; i < FA; ++i) x.a[i] = load8(pa[i], kt);
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+      const char* q = psa[i] + kt * step_a;
+      x.sa[i] = kE8 ? (unsigned)*reinterpret_cast<const unsigned char*>(q) : *reinterpret_cast<const unsigned*>(q);
+    }
+#pragma unroll
+    for (int j = 0; j < FB; ++j) {
+      const char* q = psb[j] + kt * step_b;
+      if constexpr (kSB == 4) {
+        const u32x4_t v = *reinterpret_cast<const u32x4_t*>(q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.sb[j][e] = v[e];
+      } else {
+        x.sb[j][0] = kE8 ? (unsigned)*reinterpret_cast<const unsigned char*>(q) : *reinterpret_cast<const unsigned*>(q);
+      }
+    }
+  };
+  f32x4_v acc[FA][FB];
+#pragma unroll
+  for (int i = 0; i < FA; ++i)
+#pragma unroll
+    for (int j = 0; j < FB; ++j) acc[i][j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+  auto use = [&](const Piece& x, int kt) {
+    if (kt >= ke) return;  // uniform
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+      for (int j = 0; j < FB; ++j) {
+        if constexpr (kE8) {
+          acc[i][j] = mfma_e4m3_scaled(x.b[j], x.a[i], acc[i][j], x.sb[j][0], x.sa[i]);
+        } else {
+          const f32x4_v v = mfma_e4m3(x.b[j], x.a[i], f32x4_v{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[i][j][e] = __builtin_fmaf(v[e], __uint_as_float(x.sa[i]) * __uint_as_float(x.sb[j][kSB == 4 ? e : 0]),
+                                          acc[i][j][e]);
+        }
+      }
+  };
+  Piece piece[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) fetch(piece[u], wave + u * kWaves);
+  for (int kt = wave; kt < ke; kt += kAhead * kWaves) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      use(piece[u], kt + u * kWaves);
+      fetch(piece[u], kt + (u + kAhead) * kWaves);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FA; ++i)
+#pragma unroll
+    for (int j = 0; j < FB; ++j) red[wave][i * FB + j][lane] = acc[i][j];
+  __syncthreads();
+  for (int q = threadIdx.x; q < FA * FB * 64; q += 512) {
+    const int blk = q >> 6, l = q & 63;
+    f32x4_v v = red[0][blk][l];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v += red[w][blk][l];
+    const int m = 16 * (blk / FB) + (l & 15), n = n0 + 16 * (blk % FB) + 4 * (l >> 4);
+    if (m >= p.M) continue;
+    unsigned short* out = p.c + (long)m * p.ldc + n;
+    if (p.vec_out) {
+      if (n + 3 < p.N) *reinterpret_cast<u32x2_t*>(out) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < p.N) out[e] = to_bf16_bits(v[e]);
+    }
   }
 }
 

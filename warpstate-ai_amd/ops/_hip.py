@@ -88,7 +88,10 @@ SIGNATURES = {
                                _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p]),
     "ws_fp8_pack": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p]),
     "ws_fp8_mm": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _i32, _c_void_p, _i64, _c_void_p, _i64,
-                         _i32, _i32, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p]),
+                         _i32, _i32, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _c_void_p]),
+    "ws_fp8_mm_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32]),
+    "ws_fp8_mm_plan": (_i32, [_i64, _i64, _i64, _i32, _i32, ctypes.POINTER(_i64),
+                              ctypes.POINTER(_i32)]),
     "ws_token_scores_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "ws_token_scores": (_i32, [_c_void_p, _i64, _i32, _c_void_p, _i64, _i64, _f32, _i64]
                         + [_c_void_p] * 7),

@@ -211,10 +211,12 @@ def _check_operand(q: Tensor, name: str) -> None:
 
 def _launch(a: Tensor, lda: int, sa: Tensor, ld_sa: int, rows_a: int, b: Tensor, ldb: int,
             sb: Tensor, ld_sb: int, rows_b: int, e8m0: bool, out: Tensor, k: int) -> None:
-    m, n = out.shape
+    (m, n), k16 = out.shape, _ceil(k, 16)
+    need = _hip.query_on(a, "ws_fp8_mm_workspace_bytes", m, n, k16, rows_b, int(not e8m0))
+    work = torch.empty((need,), dtype=torch.uint8, device=a.device) if need else None
     _hip.call_on(a, "ws_fp8_mm", a.data_ptr(), lda, sa.data_ptr(), ld_sa, rows_a, b.data_ptr(), ldb,
                  sb.data_ptr(), ld_sb, rows_b, int(not e8m0), out.data_ptr(),
-                 out.stride(0) if m > 1 else n, m, n, _ceil(k, 16))
+                 out.stride(0) if m > 1 else n, m, n, k16, _hip.ptr(work))
 
 
 def fp8_mm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor,
