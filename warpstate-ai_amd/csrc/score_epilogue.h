@@ -7,8 +7,8 @@
 
 namespace ws {
 
-// Per row, over this wave's FB * 16 columns: the maximum m of the scaled logits, S = sum
-// e^(l - m) and W = sum e^(l - m) (l - m), one partial per (row, wave column block), and the
+// Per row, over this wave's FB * 16 columns: the maximum m of the scaled logits (in units of log
+// 2), S and W (scores.h), one partial per (row, wave column block), and the
 // token's logit. The four lanes l, l^16, l^32, l^48 share a row.
 struct FEpiScoreStats {
   template <int FA, int FB>
@@ -19,7 +19,7 @@ struct FEpiScoreStats {
     const int part = n_base / (FB * 16);
     const int c0 = 4 * (lane >> 4);  // this lane's first column of each 16-column block
     const int ncols = p.N - n_base;  // columns of this wave inside the vocabulary
-    const float scale = p.logit_scale;
+    const float scale = p.logit_scale * kLog2e;
 #pragma unroll
     for (int i = 0; i < FA; ++i) {
       const int m = m_base + 16 * i + (lane & 15);
@@ -54,7 +54,7 @@ struct FEpiScoreStats {
 #pragma unroll
       for (int j = 0; j < FB; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) score_add(st, acc.v[i][j][e], ref);
+        for (int e = 0; e < 4; ++e) score_add(st, acc.v[i][j][e] - ref);
       st.s += __shfl_xor(st.s, 16, kWave);
       st.s += __shfl_xor(st.s, 32, kWave);
       st.w += __shfl_xor(st.w, 16, kWave);

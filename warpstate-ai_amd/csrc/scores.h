@@ -1,7 +1,7 @@
 // Token scores: of each row of logits l (scaled by 1 / temperature), the log probability of a
 // given token, the entropy, and the k likeliest tokens,
 //   lse = m + log S,  S = sum e^(l - m),  W = sum e^(l - m) (l - m),  m = max l,
-//   logprob = l_t - lse,  entropy = log S - W / S,
+//   logprob = (l_t - m) - log S,  entropy = log S - W / S,
 // and their gradient, with g and h the upstream gradients of logprob and entropy:
 //   dl_j = g [j = t] - p_j (g + h (log p_j + entropy)),  p_j = e^(l_j - lse).
 // A part of a row is summed up as (m, S, W); parts join by rescaling to the larger maximum m':
@@ -11,53 +11,64 @@
 // vocabulary gets NaN. All sums are FP32.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace ws {
 
 constexpr long kIgnored = -100;
 
+// Logits, maxima and W are held in units of log 2 (l log2 e), so that e^l is the hardware's
+// base-2 exponential without a multiplication.
 struct ScoreStats {
   float m, s, w;
 };
-// l - m where l may be -inf: 0 then, for products with a zero weight.
-__device__ __forceinline__ float score_shift(float l, float m) { return l == -INFINITY ? 0.0f : l - m; }
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 // The finite reference point for a maximum that may be -inf (nothing seen yet).
 __device__ __forceinline__ float score_ref(float m) { return m == -INFINITY ? 0.0f : m; }
-__device__ __forceinline__ void score_add(ScoreStats& a, float l, float ref) {
-  const float e = exp_e(l - ref);
+// Adds a logit y above the reference point. y = -inf adds nothing: the bound keeps 0 y from
+// being a NaN.
+__device__ __forceinline__ void score_add(ScoreStats& a, float y) {
+  const float e = exp2_hw(y);
   a.s += e;
-  a.w += e * score_shift(l, ref);
+  a.w = __builtin_fmaf(e, fmaxf(y, -1e30f), a.w);
 }
 __device__ __forceinline__ ScoreStats score_join(const ScoreStats& a, const ScoreStats& b) {
   ScoreStats r;
   r.m = fmaxf(a.m, b.m);
   const float ref = score_ref(r.m);
-  const float ea = exp_e(a.m - ref), eb = exp_e(b.m - ref);
-  r.s = ea * a.s + eb * b.s;
-  r.w = ea * (a.w + score_shift(a.m, ref) * a.s) + eb * (b.w + score_shift(b.m, ref) * b.s);
+  const float ya = a.m - ref, yb = b.m - ref;
+  const float ea = exp2_hw(ya), eb = exp2_hw(yb);
+  r.s = __builtin_fmaf(ea, a.s, eb * b.s);
+  // (An empty part has m = -inf, s = w = 0.)
+  r.w = ea * __builtin_fmaf(fmaxf(ya, -1e30f), a.s, a.w) + eb * __builtin_fmaf(fmaxf(yb, -1e30f), b.s, b.w);
   return r;
 }
-__device__ __forceinline__ ScoreStats score_join_wave(ScoreStats v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
+// Joins the values of `lanes` (a power of two) neighbouring lanes.
+__device__ __forceinline__ ScoreStats score_join_lanes(ScoreStats v, int lanes) {
+  for (int off = lanes / 2; off >= 1; off >>= 1) {
     const ScoreStats o = {__shfl_xor(v.m, off, kWave), __shfl_xor(v.s, off, kWave), __shfl_xor(v.w, off, kWave)};
     v = score_join(v, o);
   }
   return v;
 }
 
-// Outputs of a row. `target` is the scaled logit of its token (read only where that is valid).
+// Outputs of a row, in natural units. `target` is its token's logit in units of log 2 (read
+// only where the token is valid).
 struct ScoreOut {
   float *lse, *logprob, *entropy;
 };
-__device__ __forceinline__ float score_finish(const ScoreOut& o, long row, const ScoreStats& st, long token,
-                                              long vocab, float target) {
-  const float log_s = log_e(st.s), lse = st.m + log_s;
-  o.lse[row] = lse;
-  o.entropy[row] = log_s - st.w / st.s;
-  o.logprob[row] = token == kIgnored ? 0.0f : token >= 0 && token < vocab ? target - lse : NAN;
-  return lse;
+// log2 S of finished sums: a logit y has log2 p = (y - m) - log2 S.
+__device__ __forceinline__ float score_log(const ScoreStats& st) { return __builtin_amdgcn_logf(st.s); }
+__device__ __forceinline__ void score_finish(const ScoreOut& o, long row, const ScoreStats& st, long token,
+                                             long vocab, float target) {
+  const float log_s = score_log(st);
+  o.lse[row] = (st.m + log_s) * kLn2;
+  o.entropy[row] = (log_s - st.w / st.s) * kLn2;
+  o.logprob[row] = token == kIgnored               ? 0.0f
+                   : token >= 0 && token < vocab ? ((target - st.m) - log_s) * kLn2
+                                                   : NAN;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -66,14 +77,25 @@ __device__ __forceinline__ float score_finish(const ScoreOut& o, long row, const
 // it, and the part's k likeliest tokens. Rows longer than that are split over workgroups and
 // joined by score_join_kernel.
 //
-// The k largest of a part, by (logit, lowest id first): an order-preserving integer of the logit with the
-// complemented id below it makes every key different. The part's 64 groups of four threads
-// give their largest keys; the k-th largest of those, T, is at most the part's k-th largest key,
-// so every key >= T is a candidate, and in ordinary data few others are. They are collected in
-// LDS (in any order) and each is placed by the number of larger ones.
+// The k largest of a part, by (logit, lowest id first). The part's groups (the threads, or for
+// k up to 16 the 64 groups of four threads) give their largest logits; a T that at least k of
+// those reach is at most the part's k-th largest logit, so every logit >= T is a candidate, and
+// in ordinary data few others are. T is the k-th largest group cut to 16 bits of its key (an
+// order-preserving integer of the logit), found bit by bit with ballots over the groups, in
+// every wave alike. Each wave collects its candidates in LDS as keys above the complemented
+// id, so that all are different, and each is placed by the number of larger ones. Rows with
+// many logits equal to T (a mask that leaves fewer than k, say) go another way
+// (score_top_slow): the threshold there is the k-th largest of the groups' largest keys, which
+// tells equal logits apart by their ids, and if the largest logits crowd into few threads, so
+// that even that leaves too many, the keys are taken one maximum at a time.
+//
+// Few registers (eight workgroups on a compute unit), no scratch and few barriers are what it is
+// built for: 4096 x 32768 with the top 20 took 128 us while every logit's 64-bit key was formed
+// and compared in 121 registers, 125 with 112 bytes of scratch for a call, 82 inlined.
 constexpr int kScoreGroups = 64;
 constexpr int kMaxTopK = kScoreGroups;
-constexpr int kScoreCandidates = 2048;
+constexpr int kScoreCandidates = 2048, kScoreWaveCandidates = kScoreCandidates / 4;
+constexpr int kScoreFewK = 16;
 constexpr int kMaxScoreParts = 64;
 
 // Ascending in the logit's order; -0 as 0. The lowest key, 0, is no logit's (-inf has
@@ -130,7 +152,7 @@ struct ScoreParams {
   const void* logits;
   long ld;
   int rows, vocab, parts, top_k;
-  float inv_t;
+  float inv_t, scale;  // 1 / temperature, and that times log2 e
   const long* tokens;
   ScoreOut out;
   float* top_logprobs;
@@ -140,175 +162,267 @@ struct ScoreParams {
   unsigned long* keys;
 };
 
-__device__ __forceinline__ void score_top(const ScoreParams& p, long row, int i, unsigned long key, float lse) {
-  p.top_logprobs[row * p.top_k + i] = score_unkey((unsigned)(key >> 32)) * p.inv_t - lse;
+__device__ __forceinline__ void score_top(const ScoreParams& p, long row, int i, unsigned long key,
+                                          const ScoreStats& st, float log_s) {
+  const float y = score_unkey((unsigned)(key >> 32)) * p.scale;
+  p.top_logprobs[row * p.top_k + i] = ((y - st.m) - log_s) * kLn2;
   p.top_ids[row * p.top_k + i] = (long)(unsigned)~(unsigned)key;
+}
+
+__device__ __forceinline__ unsigned long max_u64(unsigned long a, unsigned long b) { return a > b ? a : b; }
+
+constexpr int kScoreWaves = 4;
+struct ScoreShared {
+  unsigned long group_keys[kScoreGroups], cand[kScoreCandidates], best[kMaxTopK], reduce[kScoreWaves], threshold;
+  int count, wave_count[kScoreWaves];
+};
+
+// A part's logits read again, eight at a time: f(key) of each inside the row.
+template <bool F32, int EPT, class F>
+__device__ __forceinline__ void score_each_key(const ScoreParams& p, long row, int first, F&& f) {
+#pragma unroll 1
+  for (int i = 0; i < EPT / 8; ++i) {
+    const int id = first + 2048 * i;
+    const long left = (long)p.vocab - id;
+    float v[8];
+    load_logits8<F32>(p.logits, row * p.ld + id, left, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) f(score_pack(score_key(v[e]), (unsigned)(id + e)));
+  }
+}
+
+// The part's k largest keys into sh.best where the list of candidates overflowed.
+template <bool F32, int EPT>
+__device__ __forceinline__ void score_top_slow(const ScoreParams& p, long row, int first, ScoreShared& sh) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, k = p.top_k;
+  if (t == 0) sh.count = 0;
+  unsigned long mine = 0;
+  score_each_key<F32, EPT>(p, row, first, [&](unsigned long key) { mine = max_u64(mine, key); });
+  unsigned long g = max_u64(mine, shfl_xor_u64(mine, 1));
+  g = max_u64(g, shfl_xor_u64(g, 2));
+  if ((t & 3) == 0) sh.group_keys[t >> 2] = g;
+  if (t == 0) sh.threshold = 0;
+  __syncthreads();
+  if (wave == 0) {
+    const unsigned long my = sh.group_keys[lane];
+    int larger = 0;
+    for (int o = 0; o < kScoreGroups; ++o) larger += sh.group_keys[o] > my;
+    if (larger == k - 1 && my != 0) sh.threshold = my;
+  }
+  __syncthreads();
+  const unsigned long T = sh.threshold;
+  if (mine >= T) {
+    score_each_key<F32, EPT>(p, row, first, [&](unsigned long key) {
+      if (key < T) return;
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kScoreCandidates) sh.cand[at] = key;
+    });
+  }
+  __syncthreads();
+  const int n = sh.count;
+  if (n <= kScoreCandidates) {
+    for (int c = t; c < n; c += 256) {
+      const unsigned long my = sh.cand[c];
+      int larger = 0;
+      for (int o = 0; o < n; ++o) larger += sh.cand[o] > my;
+      if (larger < k) sh.best[larger] = my;
+    }
+    // A part with fewer logits than k: the lowest key, which no logit has, for the others.
+    for (int c = n + t; c < k; c += 256) sh.best[c] = 0;
+    __syncthreads();
+    return;
+  }
+  unsigned long last = ~0ul;
+  for (int q = 0; q < k; ++q) {
+    unsigned long m = 0;
+    score_each_key<F32, EPT>(p, row, first, [&](unsigned long key) { m = key < last && key > m ? key : m; });
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) m = max_u64(m, shfl_xor_u64(m, off));
+    if (lane == 0) sh.reduce[wave] = m;
+    __syncthreads();
+    last = max_u64(max_u64(sh.reduce[0], sh.reduce[1]), max_u64(sh.reduce[2], sh.reduce[3]));
+    if (t == 0) sh.best[q] = last;
+    __syncthreads();
+  }
 }
 
 template <bool F32, int EPT, bool TOPK>
 static __global__ void __launch_bounds__(256) score_rows_kernel(const ScoreParams p) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const long row = blockIdx.x / p.parts;
-  const int part = blockIdx.x % p.parts;
-  const int first = part * 256 * EPT + 8 * t;  // element e of piece i: id first + 2048 i + e
+  // Element e of piece i: id first + 2048 i + e.
+  const int first = (int)(blockIdx.x % p.parts) * 256 * EPT + 8 * t;
   float x[EPT];
 #pragma unroll
   for (int i = 0; i < EPT / 8; ++i) {
     float v[8];
-    load_logits8<F32>(p.logits, row * p.ld + first + 2048 * i, (long)p.vocab - (first + 2048 * i), v);
+    const int id = first + 2048 * i;
+    load_logits8<F32>(p.logits, row * p.ld + id, (long)p.vocab - id, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[8 * i + e] = v[e];
   }
-
-  __shared__ float red[3][4];
-  __shared__ unsigned long groups[TOPK ? kScoreGroups : 1], cand[TOPK ? kScoreCandidates : 1], best[TOPK ? kMaxTopK : 1];
-  __shared__ unsigned long threshold, reduce4[4];
-  __shared__ int count;
-
+  __shared__ __attribute__((aligned(16))) float groups[256];
+  __shared__ float red[2][kScoreWaves];
+  __shared__ std::conditional_t<TOPK, ScoreShared, int> sh;
   float mx = x[0];
 #pragma unroll
   for (int i = 1; i < EPT; ++i) mx = fmaxf(mx, x[i]);
-  mx = wave_max(mx);
-  if (lane == 0) red[0][wave] = mx;
-  unsigned long mine = 0;
-  if constexpr (TOPK) {
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const int id = first + 2048 * (i / 8) + i % 8;
-      const unsigned long key = score_pack(id < p.vocab ? score_key(x[i]) : 0u, (unsigned)id);
-      mine = key > mine ? key : mine;
-    }
-    unsigned long group = mine;
-#pragma unroll
-    for (int off = 1; off <= 2; off <<= 1) {
-      const unsigned long o = shfl_xor_u64(group, off);
-      group = o > group ? o : group;
-    }
-    if ((t & 3) == 0) groups[t >> 2] = group;
-    if (t == 0) count = 0;
-  }
+  groups[t] = mx;
   __syncthreads();
+  const f32x4_t group = *reinterpret_cast<const f32x4_t*>(&groups[4 * lane]);
+  const float four = fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3]));
   ScoreStats st;
-  st.m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])) * p.inv_t;
+  st.m = wave_max(four) * p.scale;
   st.s = st.w = 0.0f;
+  if constexpr (TOPK) {
+    unsigned T = 0;
+    if (p.top_k <= kScoreFewK) {
+      const unsigned key = score_key(four);
+#pragma unroll
+      for (int b = 31; b >= 16; --b) {
+        const unsigned with = T | 1u << b;
+        if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= with)) >= p.top_k) T = with;
+      }
+    } else {
+      const unsigned key[4] = {score_key(group[0]), score_key(group[1]), score_key(group[2]), score_key(group[3])};
+#pragma unroll
+      for (int b = 31; b >= 16; --b) {
+        const unsigned with = T | 1u << b;
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[e] >= with));
+        if (n >= p.top_k) T = with;
+      }
+    }
+    // Keys up to -inf's leave too many: the other way.
+    int found = kScoreWaveCandidates + 1;
+    if (T > 0x007fffffu) {
+      const float cut = score_unkey(T);
+      found = 0;
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) {
+        const bool hit = x[i] >= cut;
+        const unsigned long hits = __builtin_amdgcn_ballot_w64(hit);
+        if (hits != 0) {
+          const int at = found + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(hits >> 32),
+                                                                 __builtin_amdgcn_mbcnt_lo((unsigned)hits, 0));
+          if (hit && at < kScoreWaveCandidates)
+            sh.cand[wave * kScoreWaveCandidates + at] =
+                score_pack(score_key(x[i]), (unsigned)(first + 2048 * (i / 8) + i % 8));
+          found += __builtin_popcountll(hits);
+        }
+      }
+    }
+    if (lane == 0) sh.wave_count[wave] = found;
+  }
   const float ref = score_ref(st.m);
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) score_add(st, x[i] * p.inv_t, ref);
+  for (int i = 0; i < EPT; ++i) score_add(st, __builtin_fmaf(x[i], p.scale, -ref));
   st.s = wave_sum(st.s);
   st.w = wave_sum(st.w);
   if (lane == 0) {
-    red[1][wave] = st.s;
-    red[2][wave] = st.w;
-  }
-  if constexpr (TOPK) {
-    if (wave == 0) {
-      const unsigned long my = groups[lane];
-      int larger = 0;
-      for (int g = 0; g < kScoreGroups; ++g) larger += groups[g] > my;
-      if (larger == p.top_k - 1) threshold = my;
-    }
+    red[0][wave] = st.s;
+    red[1][wave] = st.w;
   }
   __syncthreads();
-  st.s = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-  st.w = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+  st.s = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
+  st.w = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
   if constexpr (TOPK) {
-    const unsigned long T = threshold;
-    if (mine >= T) {
+    int n[kScoreWaves], most = 0, all = 0;
 #pragma unroll
-      for (int i = 0; i < EPT; ++i) {
-        const int id = first + 2048 * (i / 8) + i % 8;
-        const unsigned long key = score_pack(id < p.vocab ? score_key(x[i]) : 0u, (unsigned)id);
-        if (key >= T) {
-          const int at = atomicAdd(&count, 1);
-          if (at < kScoreCandidates) cand[at] = key;
-        }
-      }
+    for (int w = 0; w < kScoreWaves; ++w) {
+      n[w] = __builtin_amdgcn_readfirstlane(sh.wave_count[w]);
+      most = max(most, n[w]);
+      all += n[w];
     }
-    __syncthreads();
-    const int n = count;
-    if (n <= kScoreCandidates) {
-      for (int c = t; c < n; c += 256) {
-        const unsigned long my = cand[c];
+    // (A NaN compares false: a row of them can leave fewer than k.)
+    if (most > kScoreWaveCandidates || all < p.top_k) {
+      __syncthreads();  // every thread has read the counts
+      score_top_slow<F32, EPT>(p, row, first, sh);
+    } else {
+      for (int c = lane; c < n[wave]; c += 64) {
+        const unsigned long my = sh.cand[wave * kScoreWaveCandidates + c];
         int larger = 0;
-        for (int o = 0; o < n; ++o) larger += cand[o] > my;
-        if (larger < p.top_k) best[larger] = my;
+#pragma unroll
+        for (int w = 0; w < kScoreWaves; ++w)
+#pragma unroll 4
+          for (int o = 0; o < n[w]; ++o) larger += sh.cand[w * kScoreWaveCandidates + o] > my;
+        if (larger < p.top_k) sh.best[larger] = my;
       }
       __syncthreads();
-    } else {
-      // More candidates than LDS holds (the largest logits crowded into few threads): one
-      // maximum at a time.
-      unsigned long last = ~0ul;
-      for (int k = 0; k < p.top_k; ++k) {
-        unsigned long m = 0;
-#pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-          const int id = first + 2048 * (i / 8) + i % 8;
-          const unsigned long key = score_pack(id < p.vocab ? score_key(x[i]) : 0u, (unsigned)id);
-          m = key < last && key > m ? key : m;
-        }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) {
-          const unsigned long o = shfl_xor_u64(m, off);
-          m = o > m ? o : m;
-        }
-        if (lane == 0) reduce4[wave] = m;
-        __syncthreads();
-        const unsigned long a = reduce4[0] > reduce4[1] ? reduce4[0] : reduce4[1];
-        const unsigned long b = reduce4[2] > reduce4[3] ? reduce4[2] : reduce4[3];
-        last = a > b ? a : b;
-        if (t == 0) best[k] = last;
-        __syncthreads();
-      }
     }
   }
   if (p.parts > 1) {
     if (t == 0) p.stats[blockIdx.x] = f32x4_t{st.m, st.s, st.w, 0.0f};
-    if (TOPK && t < p.top_k) p.keys[(long)blockIdx.x * p.top_k + t] = best[t];
+    if constexpr (TOPK) {
+      if (t < p.top_k) p.keys[(long)blockIdx.x * p.top_k + t] = sh.best[t];
+    }
     return;
   }
-  const long token = p.tokens[row];
-  const float lse = st.m + log_e(st.s);
   if (t == 0) {
-    const bool valid = token >= 0 && token < p.vocab;
-    score_finish(p.out, row, st, token, p.vocab,
-                 valid ? load_logit<F32>(p.logits, row * p.ld + token) * p.inv_t : 0.0f);
-  }
-  if (TOPK && t < p.top_k) score_top(p, row, t, best[t], lse);
-}
-
-// Joins the parts of split rows, one wave per row: lane i holds part i (at most 64), its sums
-// and the head of its sorted keys; each of the k steps takes the largest head.
-template <bool F32>
-static __global__ void __launch_bounds__(256) score_join_kernel(const ScoreParams p) {
-  const int lane = threadIdx.x & 63;
-  const long row = blockIdx.x * 4L + (threadIdx.x >> 6);
-  if (row >= p.rows) return;
-  ScoreStats st = {-INFINITY, 0.0f, 0.0f};
-  const long part = row * p.parts + lane;
-  if (lane < p.parts) {
-    const f32x4_t v = p.stats[part];
-    st = ScoreStats{v[0], v[1], v[2]};
-  }
-  st = score_join_wave(st);
-  const float lse = st.m + log_e(st.s);
-  if (lane == 0) {
     const long token = p.tokens[row];
     const bool valid = token >= 0 && token < p.vocab;
     score_finish(p.out, row, st, token, p.vocab,
-                 valid ? load_logit<F32>(p.logits, row * p.ld + token) * p.inv_t : 0.0f);
+                 valid ? load_logit<F32>(p.logits, row * p.ld + token) * p.scale : 0.0f);
   }
-  const unsigned long* keys = p.keys + part * p.top_k;
-  int at = 0;
-  unsigned long head = p.top_k > 0 && lane < p.parts ? keys[0] : 0ul;
-  for (int k = 0; k < p.top_k; ++k) {
-    unsigned long m = head;
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-      const unsigned long o = shfl_xor_u64(m, off);
-      m = o > m ? o : m;
+  if constexpr (TOPK) {
+    if (t < p.top_k) score_top(p, row, t, sh.best[t], st, score_log(st));
+  }
+}
+
+// Joins the parts of split rows, 256 / threads rows per workgroup. The first `lanes` lanes of a row's
+// threads (a power of two, at least the parts) join its sums. A key's place among the row's is
+// its place in its own part's sorted list and the number of larger keys in every other's, found
+// by bisection in LDS, all keys at once (taking the largest head k times over cost 12 us for 4096
+// rows and the top 20).
+template <bool F32>
+static __global__ void __launch_bounds__(256) score_join_kernel(const ScoreParams p, int threads, int lanes) {
+  extern __shared__ unsigned long join_keys[];
+  __shared__ float joined[4][2];
+  const int t = threadIdx.x % threads, slot = threadIdx.x / threads;
+  const long row = (long)blockIdx.x * (256 / threads) + slot;
+  const int k = p.top_k, total = p.parts * k;
+  const bool ok = row < p.rows;
+  unsigned long* keys = join_keys + slot * total;
+  if (ok)
+    for (int i = t; i < total; i += threads) keys[i] = p.keys[row * total + i];
+  ScoreStats st = {-INFINITY, 0.0f, 0.0f};
+  if (ok && t < p.parts) {
+    const f32x4_t v = p.stats[row * p.parts + t];
+    st = ScoreStats{v[0], v[1], v[2]};
+  }
+  st = score_join_lanes(st, lanes);
+  if (ok && t == 0) {
+    const long token = p.tokens[row];
+    const bool valid = token >= 0 && token < p.vocab;
+    score_finish(p.out, row, st, token, p.vocab,
+                 valid ? load_logit<F32>(p.logits, row * p.ld + token) * p.scale : 0.0f);
+    joined[slot][0] = st.m;
+    joined[slot][1] = score_log(st);
+  }
+  if (k == 0) return;  // uniform
+  __syncthreads();
+  if (!ok) return;
+  st.m = joined[slot][0];
+  const float log_s = joined[slot][1];
+  for (int i = t; i < total; i += threads) {
+    const unsigned long my = keys[i];
+    const int part = i / k;
+    int larger = i - part * k;
+    for (int q = 0; q < p.parts && larger < k; ++q) {
+      if (q == part) continue;
+      // The first place in part q's descending list whose key is not larger.
+      int lo = 0, hi = k;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (keys[q * k + mid] > my) lo = mid + 1;
+        else hi = mid;
+      }
+      larger += lo;
     }
-    if (lane == 0) score_top(p, row, k, m, lse);
-    if (head == m && lane < p.parts) head = ++at < p.top_k ? keys[at] : 0ul;
+    // (The key 0 of a part with fewer logits than k is never among the row's k largest.)
+    if (larger < k && my != 0) score_top(p, row, larger, my, st, log_s);
   }
 }
 
@@ -401,7 +515,7 @@ static __global__ void __launch_bounds__(256) score_combine_kernel(const float* 
     const long i = row * parts + q;
     st = score_join(st, ScoreStats{pm[i], ps[i], pw[i]});
   }
-  st = score_join_wave(st);
+  st = score_join_lanes(st, kWave);
   if (lane == 0) {
     const long token = tokens[row];
     score_finish(out, row, st, token, vocab, token >= 0 && token < vocab ? target[row] : 0.0f);

@@ -32,7 +32,11 @@ int run_scores(const ScoreParams& p, int ept, hipStream_t s) {
   else launch_rows<F32, kLargeEpt>(p, s);
   if (int rc = hip_check(hipGetLastError(), "token score launch")) return rc;
   if (p.parts == 1) return kOk;
-  hipLaunchKernelGGL((score_join_kernel<F32>), dim3(cdiv(p.rows, 4)), dim3(256), 0, s, p);
+  int lanes = 2, threads = 64;
+  while (lanes < p.parts) lanes *= 2;
+  while (threads < p.parts * p.top_k && threads < 256) threads *= 2;
+  const int rows = 256 / threads, lds = rows * p.parts * p.top_k * 8;
+  hipLaunchKernelGGL((score_join_kernel<F32>), dim3(cdiv(p.rows, rows)), dim3(256), lds, s, p, threads, lanes);
   return hip_check(hipGetLastError(), "token score join launch");
 }
 
@@ -72,6 +76,7 @@ extern "C" int ws_token_scores(const void* logits, int64_t ld, int f32, const in
   p.rows = (int)rows; p.vocab = (int)vocab; p.top_k = (int)top_k;
   p.parts = score_parts(rows, vocab);
   p.inv_t = inv_temperature;
+  p.scale = inv_temperature * kLog2e;
   p.tokens = reinterpret_cast<const long*>(tokens);
   p.out = ScoreOut{lse, logprob, entropy};
   p.top_logprobs = top_logprobs;
