@@ -285,3 +285,51 @@ def test_products_in_a_captured_graph():
         torch.cuda.synchronize()
         got = out.clone()
         assert torch.equal(got, step())
+
+
+def test_python_launches_agree_with_the_native_ones(monkeypatch):
+    from ops import _hip
+
+    fp8 = _fp8()
+    assert _hip.host_ops() is not None
+    x, w = _matrix(130, 272, BF16, 3).clamp(-9, 9), _matrix(96, 272, F32, 4).clamp(-9, 9)
+
+    def run():
+        out = []
+        for scale_dtype in SCALES:
+            q = fp8.quantize_rows_and_columns(x, scale_dtype)
+            b = fp8.quantize_weight(w, scale_dtype)
+            out += [*q, *b, *fp8.quantize_columns(x, scale_dtype), fp8.fp8_mm(*q[:2], *b[:2])]
+        return out
+
+    native = run()
+    monkeypatch.setattr(_hip, "host_ops", lambda: None)
+    for a, b in zip(native, run()):
+        assert a.dtype == b.dtype and a.shape == b.shape and np.array_equal(values(a), values(b))
+
+
+def test_linear_saves_no_more_than_it_reads():
+    """A BF16 weight's step keeps 8-bit copies only; a call without gradients keeps nothing;
+    compiled calls give the eager values."""
+    fp8 = _fp8()
+    x, w = _matrix(64, 256, BF16, 1).clamp(-9, 9), torch.randn((128, 256), device="cuda").to(BF16)
+    plain = fp8.fp8_linear(x, w)
+    assert not plain.requires_grad
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    kept = []
+
+    def pack(t):
+        kept.append(t)
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        y = fp8.fp8_linear(x, w)
+    assert torch.equal(y, plain) and all(t.dtype == torch.uint8 for t in kept)
+    dy = torch.randn_like(y)
+    want = torch.autograd.grad(y, [x, w], dy)
+    compiled = torch.compile(fp8.fp8_linear, fullgraph=True)
+    out = compiled(x, w)
+    assert torch.equal(out, plain)
+    for a, b in zip(torch.autograd.grad(out, [x, w], dy), want):
+        assert torch.equal(a, b)

@@ -346,3 +346,53 @@ def test_scores_in_a_captured_graph():
         kept = [t.clone() for t in out]
         for a, b in zip(kept, step()):
             assert torch.equal(a, b)
+
+
+def test_python_launches_agree_with_the_native_ones(monkeypatch):
+    from ops import _hip
+
+    ts = _scores()
+    assert _hip.host_ops() is not None
+    logits, tokens = _logits(37, 9001, BF16, 3).cuda(), _tokens(37, 9001, 3).cuda()
+    hidden = torch.randn((37, 60), generator=torch.Generator().manual_seed(1)).cuda()
+    weight = torch.randn((9001, 60), generator=torch.Generator().manual_seed(2)).cuda()
+    g, h = torch.randn(37, device="cuda"), torch.randn(37, device="cuda")
+
+    def run():
+        x = logits.clone().requires_grad_(True)
+        got = ts.token_scores(x, tokens, 9, 0.9)
+        grads = torch.autograd.grad([got.logprob, got.entropy], [x], [g, h])
+        leaves = [hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)]
+        scores = ts.linear_token_scores(*leaves, tokens, 0.9, 20)
+        return (*got, *grads, *scores, *torch.autograd.grad(scores, leaves, [g, h]))
+
+    native = run()
+    monkeypatch.setattr(_hip, "host_ops", lambda: None)
+    for a, b in zip(native, run()):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_second_derivatives_are_refused():
+    ts = _scores()
+    x = _logits(3, 50, F32, 3).cuda().requires_grad_(True)
+    out = ts.token_scores(x, _tokens(3, 50, 3).cuda()).logprob.sum()
+    with pytest.raises(RuntimeError, match="differentiate"):
+        dx, = torch.autograd.grad(out, [x], create_graph=True)
+        torch.autograd.grad(dx.sum(), [x])
+    hidden = torch.randn((3, 16), device="cuda", requires_grad=True)
+    weight = torch.randn((50, 16), device="cuda", requires_grad=True)
+    out = ts.linear_token_scores(hidden, weight, _tokens(3, 50, 3).cuda())[0].sum()
+    with pytest.raises(RuntimeError, match="differentiate"):
+        dh, = torch.autograd.grad(out, [hidden], create_graph=True)
+        torch.autograd.grad(dh.sum(), [hidden])
+
+
+def test_a_changed_operand_is_noticed():
+    ts = _scores()
+    hidden = torch.randn((3, 16), device="cuda").to(BF16).requires_grad_(True)
+    weight = torch.randn((50, 16), device="cuda").to(BF16).requires_grad_(True)
+    out = ts.linear_token_scores(hidden, weight, torch.arange(3, device="cuda"))[0].sum()
+    with torch.no_grad():
+        weight.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, [hidden])

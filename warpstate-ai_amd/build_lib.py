@@ -1,5 +1,7 @@
-"""Compile ``csrc/*.hip`` for gfx950 into ``lib/libwarpstate_hip.so``, and the operators'
-host-side autograd kernels (``csrc/autograd.cpp``) into ``lib/libwarpstate_autograd.so``.
+"""Compile ``csrc/*.hip`` for gfx950 into ``lib/libwarpstate_hip.so``, the operators' host-side
+autograd kernels (``csrc/autograd.cpp``) into ``lib/libwarpstate_autograd.so`` and the host side
+of the 8-bit projections and token scores (``csrc/host_ops.cpp``) into
+``lib/libwarpstate_host.so``.
 
 Every translation unit is compiled on each call (in parallel), then linked into a fresh
 library that atomically replaces the old one. Objects go to ``_build/``.
@@ -19,6 +21,8 @@ CSRC = PACKAGE / "csrc"
 BUILD = PACKAGE / "_build"
 LIBRARY = PACKAGE / "lib" / "libwarpstate_hip.so"
 AUTOGRAD = PACKAGE / "lib" / "libwarpstate_autograd.so"
+HOST = PACKAGE / "lib" / "libwarpstate_host.so"
+ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")
 ARCH = "gfx950"
@@ -63,6 +67,24 @@ def _build_autograd() -> Path:
     return AUTOGRAD
 
 
+def host_command(source: Path, target: Path) -> list[str]:
+    """The host compiler's command for the C++ operators: PyTorch's and HIP's headers, linked
+    to the kernels' library beside it."""
+    return [*autograd_command(source, target), "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+            f"-I{ROCM}/include", "-lc10_hip", f"-L{LIBRARY.parent}", f"-l:{LIBRARY.name}",
+            "-Wl,-rpath,$ORIGIN"]
+
+
+def _build_host() -> Path:
+    staging = HOST.with_name(HOST.name + ".tmp")
+    cmd = host_command(CSRC / "host_ops.cpp", staging)
+    result = subprocess.run(cmd, capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError(f"{CXX} failed for host_ops.cpp:\n{result.stderr}")
+    os.replace(staging, HOST)
+    return HOST
+
+
 def build(jobs: int | None = None) -> Path:
     sources = sorted(CSRC.glob("*.hip"))
     if not sources:
@@ -81,6 +103,7 @@ def build(jobs: int | None = None) -> Path:
     os.replace(staging, LIBRARY)
     # Last, so that a host without PyTorch's headers is left with the kernels.
     autograd.result()
+    _build_host()
     return LIBRARY
 
 

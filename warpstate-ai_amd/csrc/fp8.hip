@@ -7,14 +7,18 @@ using namespace ws;
 
 namespace {
 
-template <bool F32, int SCALE, int FORM>
+template <bool F32, int SCALE, int FORM, int R = 8>
 int run_quantize(const QuantParams& p, bool vec, hipStream_t s) {
-  const long tiles = (long)cdiv(p.rows, kQBlock) * p.col_tiles;
+  const long tiles = (long)cdiv(p.rows, 16 * R) * p.col_tiles;
   if (!fits_i32(tiles)) return set_error(kInvalid, "too many 128 x 128 tiles");
+  if constexpr (FORM == kQuantRows && R == 8) {
+    // Few tiles: a row per thread (1 x 5632: 5.9 -> QROWS1 us).
+    if (tiles < device_cus()) return run_quantize<F32, SCALE, FORM, 1>(p, vec, s);
+  }
   if (vec)
-    hipLaunchKernelGGL((quantize_kernel<F32, SCALE, FORM, true>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((quantize_kernel<F32, SCALE, FORM, true, R>), dim3((unsigned)tiles), dim3(256), 0, s, p);
   else
-    hipLaunchKernelGGL((quantize_kernel<F32, SCALE, FORM, false>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((quantize_kernel<F32, SCALE, FORM, false, R>), dim3((unsigned)tiles), dim3(256), 0, s, p);
   return hip_check(hipGetLastError(), "quantize launch");
 }
 template <bool F32, int SCALE>

@@ -1,0 +1,379 @@
+// Host side of the 8-bit projections and the token scores as PyTorch operators in C++.
+//
+// ops/fp8_execution.py and ops/token_scores.py check their arguments in Python and launch
+// through ctypes; allocating the outputs, the calls and above all the autograd nodes then take
+// longer than the kernels at small sizes (one 32768-token row: 23 us of host time for 11 us of
+// kernels; scores and gradient of 1000 x 10883 logits: 109 us for 35). These do the same allocations
+// and make the same C calls without Python. Their arguments are the checked ones.
+//
+// Operators named native_* exist only with this library; warpstate::fp8_linear is defined in
+// Python, with a Python kernel and autograd formula that these replace on CUDA.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <limits>
+
+#include "../../include/warpstate_hip.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+typedef std::tuple<Tensor, Tensor, Tensor, Tensor> FourTensors;
+typedef std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> FiveTensors;
+
+constexpr int64_t kBlock = 128;
+constexpr int64_t kTransposeMinRows = 1024;  // fused_execution.TRANSPOSE_MIN_ROWS
+
+void check(int status, const char* name) {
+  TORCH_CHECK(status == 0, name, " failed (status ", status, "): ", ws_last_error());
+}
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
+int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+void* ptr(const Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
+Tensor bytes(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options().dtype(at::kByte)); }
+Tensor floats(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options().dtype(at::kFloat)); }
+
+// --- 8-bit operands -------------------------------------------------------------------------
+
+Tensor scales(const Tensor& like, int64_t rows, int64_t n, bool e8m0) {
+  return e8m0 ? bytes(like, {rows, up(n, 4)}) : floats(like, {n, up(rows, 4)});
+}
+
+FourTensors quantize(const Tensor& x, bool e8m0, int64_t form, bool transposed) {
+  c10::DeviceGuard guard(x.device());
+  const int64_t rows = x.size(0), cols = x.size(1);
+  const bool block = form == WS_QUANT_BLOCKS;
+  Tensor q, scale, qt, scale_t;
+  if (form != WS_QUANT_COLUMNS) {
+    q = bytes(x, {rows, up(cols, 16)});
+    scale = scales(x, block ? blocks(rows) : rows, blocks(cols), e8m0);
+  }
+  if ((form & WS_QUANT_COLUMNS) || transposed) {
+    qt = bytes(x, {cols, up(rows, 16)});
+    scale_t = scales(x, block ? blocks(cols) : cols, blocks(rows), e8m0);
+  }
+  auto ld = [](const Tensor& t) { return t.defined() ? t.size(1) : 0; };
+  check(ws_fp8_quantize(x.const_data_ptr(), row_stride(x), x.scalar_type() == at::kFloat, rows, cols, (int)form,
+                        e8m0 ? WS_SCALE_E8M0 : WS_SCALE_F32, ptr(q), ld(q), ptr(scale), ld(scale), ptr(qt), ld(qt),
+                        ptr(scale_t), ld(scale_t), stream_of(x)),
+        "ws_fp8_quantize");
+  return {q, scale, qt, scale_t};
+}
+
+void product(const Tensor& a, int64_t lda, const Tensor& sa, int64_t ld_sa, int64_t rows_a, const Tensor& b,
+             int64_t ldb, const Tensor& sb, int64_t ld_sb, int64_t rows_b, bool e8m0, const Tensor& out, int64_t k) {
+  c10::DeviceGuard guard(a.device());
+  const int64_t m = out.size(0), n = out.size(1), wide = up(k, 16);
+  const int type = e8m0 ? WS_SCALE_E8M0 : WS_SCALE_F32;
+  const int64_t need = ws_fp8_mm_workspace_bytes(m, n, wide, (int)rows_b, type);
+  Tensor work = need ? bytes(a, {need}) : Tensor();
+  check(ws_fp8_mm(a.const_data_ptr(), lda, sa.const_data_ptr(), ld_sa, (int)rows_a, b.const_data_ptr(), ldb,
+                  sb.const_data_ptr(), ld_sb, (int)rows_b, type, out.data_ptr(), row_stride(out), m, n, wide,
+                  ptr(work), stream_of(a)),
+        "ws_fp8_mm");
+}
+Tensor native_product(const Tensor& a, int64_t lda, const Tensor& sa, int64_t ld_sa, int64_t rows_a,
+                      const Tensor& b, int64_t ldb, const Tensor& sb, int64_t ld_sb, int64_t rows_b, bool e8m0) {
+  Tensor out = at::empty({a.size(0), b.size(0)}, a.options().dtype(at::kBFloat16));
+  product(a, lda, sa, ld_sa, rows_a, b, ldb, sb, ld_sb, rows_b, e8m0, out, a.size(1));
+  return out;
+}
+// On whole buffers of quantize().
+void product_of(const Tensor& a, const Tensor& sa, int64_t rows_a, const Tensor& b, const Tensor& sb,
+                int64_t rows_b, bool e8m0, const Tensor& out, int64_t k) {
+  product(a, a.size(1), sa, sa.size(1), rows_a, b, b.size(1), sb, sb.size(1), rows_b, e8m0, out, k);
+}
+
+FiveTensors linear_forward(const Tensor& x, const Tensor& weight, bool e8m0, bool keep_x, bool keep_w) {
+  auto [w, w_scale, wt, wt_scale] = quantize(weight, e8m0, WS_QUANT_BLOCKS, keep_w);
+  auto [q, scale, qt, qt_scale] = quantize(x, e8m0, keep_x ? WS_QUANT_ROWS | WS_QUANT_COLUMNS : WS_QUANT_ROWS, false);
+  Tensor y = at::empty({x.size(0), weight.size(0)}, x.options());
+  product_of(q, scale, 1, w, w_scale, kBlock, e8m0, y, x.size(1));
+  auto kept = [&](Tensor& t) { return t.defined() ? t : bytes(x, {0, 0}); };
+  return {y, kept(qt), kept(qt_scale), kept(wt), kept(wt_scale)};
+}
+
+std::tuple<Tensor, Tensor> linear_backward(const Tensor& grad_in, const Tensor& x, const Tensor& qt,
+                                           const Tensor& qt_scale, const Tensor& wt, const Tensor& wt_scale,
+                                           int64_t k, bool e8m0, bool want_x, bool want_w, bool master) {
+  const Tensor grad = grad_in.contiguous();
+  const int64_t m = grad.size(0), n = grad.size(1);
+  const int64_t form = (want_x ? WS_QUANT_ROWS : 0) | (want_w && !master ? WS_QUANT_COLUMNS : 0);
+  Tensor g, g_scale, gt, gt_scale;
+  if (form) std::tie(g, g_scale, gt, gt_scale) = quantize(grad, e8m0, form, false);
+  Tensor dx = want_x ? at::empty({m, k}, grad.options()) : at::empty({0}, grad.options());
+  if (want_x) product_of(g, g_scale, 1, wt, wt_scale, kBlock, e8m0, dx, n);
+  const auto dw_options = grad.options().dtype(master ? at::kFloat : at::kBFloat16);
+  if (!want_w) return {dx, at::empty({0}, dw_options)};
+  Tensor dw = at::empty({n, k}, dw_options);
+  if (master) {
+    // fused_execution.mm_f32 of grad^T and x, FP32 sums unrounded.
+    c10::DeviceGuard guard(grad.device());
+    const ws_accumulate_problem item{grad.const_data_ptr(), 1, n, x.const_data_ptr(), x.stride(0), x.stride(1),
+                                     dw.data_ptr<float>(), k, n, k};
+    const int64_t need = ws_mm_accumulate_group_workspace_floats(&item, 1, m);
+    Tensor work = need ? floats(grad, {need}) : Tensor();
+    check(ws_mm_store_f32_group(&item, 1, m, 0, need ? work.data_ptr<float>() : nullptr, stream_of(grad)),
+          "ws_mm_store_f32_group");
+  } else {
+    product_of(gt, gt_scale, 1, qt, qt_scale, 1, e8m0, dw, m);
+  }
+  return {dx, dw};
+}
+
+struct Fp8LinearFn : Function<Fp8LinearFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, bool e8m0, bool keep_x,
+                               bool keep_w) {
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("warpstate::fp8_linear", "")
+                               .typed<FiveTensors(const Tensor&, const Tensor&, bool, bool, bool)>();
+    ctx->set_materialize_grads(false);
+    at::AutoDispatchBelowAutograd guard;
+    auto [y, qt, qt_scale, wt, wt_scale] = op.call(x, weight, e8m0, keep_x, keep_w);
+    const bool master = weight.scalar_type() == at::kFloat;
+    // x itself only where its weight gradient reads it.
+    ctx->save_for_backward({master && weight.requires_grad() ? x : qt, qt, qt_scale, wt, wt_scale});
+    ctx->saved_data["k"] = x.sym_size(1);
+    ctx->saved_data["e8m0"] = e8m0;
+    ctx->saved_data["want_x"] = x.requires_grad();
+    ctx->saved_data["want_w"] = weight.requires_grad();
+    ctx->saved_data["master"] = master;
+    return {y, qt, qt_scale, wt, wt_scale};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    typedef const Tensor& T;
+    static const auto op =
+        c10::Dispatcher::singleton()
+            .findSchemaOrThrow("warpstate::fp8_linear_backward", "")
+            .typed<std::tuple<Tensor, Tensor>(T, T, T, T, T, T, c10::SymInt, bool, bool, bool, bool)>();
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto s = ctx->get_saved_variables();
+    const bool want_x = ctx->saved_data["want_x"].toBool(), want_w = ctx->saved_data["want_w"].toBool();
+    auto call = [&] {
+      return op.call(grads[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["k"].toSymInt(),
+                     ctx->saved_data["e8m0"].toBool(), want_x, want_w, ctx->saved_data["master"].toBool());
+    };
+    std::tuple<Tensor, Tensor> d;
+    if (at::GradMode::is_enabled()) {  // the operator's own autograd kernel refuses a second derivative
+      d = call();
+    } else {
+      at::AutoDispatchBelowAutograd guard;
+      d = call();
+    }
+    return {want_x ? std::get<0>(d) : Tensor(), want_w ? std::get<1>(d) : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+FiveTensors linear(const Tensor& x, const Tensor& weight, bool e8m0, bool keep_x, bool keep_w) {
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad())) {
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("warpstate::fp8_linear", "")
+                               .typed<FiveTensors(const Tensor&, const Tensor&, bool, bool, bool)>();
+    at::AutoDispatchBelowAutograd guard;
+    return op.call(x, weight, e8m0, keep_x, keep_w);
+  }
+  variable_list v = Fp8LinearFn::apply(x, weight, e8m0, keep_x, keep_w);
+  return {v[0], v[1], v[2], v[3], v[4]};
+}
+
+// --- token scores ---------------------------------------------------------------------------
+
+// (logprob, entropy, top logprobs, top ids, lse).
+FiveTensors scores_forward(const Tensor& logits, const Tensor& tokens, int64_t top_k, double inv_t) {
+  c10::DeviceGuard guard(logits.device());
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  Tensor logprob = floats(logits, {rows}), entropy = floats(logits, {rows}), lse = floats(logits, {rows});
+  Tensor top = floats(logits, {rows, top_k});
+  Tensor ids = at::empty({rows, top_k}, logits.options().dtype(at::kLong));
+  if (rows) {
+    const int64_t need = ws_token_scores_workspace_bytes(rows, vocab, top_k);
+    Tensor work = need ? bytes(logits, {need}) : Tensor();
+    check(ws_token_scores(logits.const_data_ptr(), row_stride(logits), logits.scalar_type() == at::kFloat,
+                          tokens.const_data_ptr<int64_t>(), rows, vocab, (float)inv_t, top_k, ptr(work),
+                          lse.data_ptr<float>(), logprob.data_ptr<float>(), entropy.data_ptr<float>(),
+                          top.data_ptr<float>(), ids.data_ptr<int64_t>(), stream_of(logits)),
+          "ws_token_scores");
+  }
+  return {logprob, entropy, top, ids, lse};
+}
+
+// An upstream gradient as the kernels read it.
+Tensor upstream(const Tensor& g) { return g.defined() ? g.to(at::kFloat).contiguous() : g; }
+const float* float_ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
+
+// First derivatives only: a backward that is itself recorded would lose the second.
+void refuse_second() {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "token scores cannot be differentiated twice");
+}
+
+struct TokenScoresFn : Function<TokenScoresFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, int64_t top_k,
+                               double inv_t) {
+    auto [logprob, entropy, top, ids, lse] = [&] {
+      at::AutoDispatchBelowAutograd guard;
+      return scores_forward(logits, tokens, top_k, inv_t);
+    }();
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, tokens, lse, entropy});
+    ctx->saved_data["inv_t"] = inv_t;
+    ctx->mark_non_differentiable({top, ids});
+    return {logprob, entropy, top, ids};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list none(4);
+    if (!grads[0].defined() && !grads[1].defined()) return none;
+    refuse_second();
+    const auto s = ctx->get_saved_variables();
+    const Tensor &logits = s[0], &tokens = s[1];
+    c10::DeviceGuard guard(logits.device());
+    const int64_t rows = logits.size(0), vocab = logits.size(1);
+    Tensor out = at::empty({rows, vocab}, logits.options());
+    if (rows) {
+      const Tensor g = upstream(grads[0]), h = upstream(grads[1]);
+      check(ws_token_scores_backward(logits.const_data_ptr(), row_stride(logits),
+                                     logits.scalar_type() == at::kFloat, tokens.const_data_ptr<int64_t>(), rows,
+                                     vocab, (float)ctx->saved_data["inv_t"].toDouble(), float_ptr(s[2]),
+                                     float_ptr(s[3]), float_ptr(g), float_ptr(h), out.data_ptr(), vocab,
+                                     stream_of(logits)),
+            "ws_token_scores_backward");
+    }
+    none[0] = out;
+    return none;
+  }
+};
+FourTensors native_token_scores(const Tensor& logits, const Tensor& tokens, int64_t top_k, double inv_t) {
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    variable_list v = TokenScoresFn::apply(logits, tokens, top_k, inv_t);
+    return {v[0], v[1], v[2], v[3]};
+  }
+  at::AutoDispatchBelowAutograd guard;
+  auto [logprob, entropy, top, ids, lse] = scores_forward(logits, tokens, top_k, inv_t);
+  return {logprob, entropy, top, ids};
+}
+
+// hidden and weight as the kernels read them (BF16, 16-byte rows, equal padded widths).
+std::tuple<Tensor, Tensor, Tensor> head_forward(const Tensor& h, const Tensor& w, const Tensor& tokens, double inv_t) {
+  c10::DeviceGuard guard(h.device());
+  const int64_t rows = h.size(0), d = h.size(1), vocab = w.size(0);
+  Tensor logprob = floats(h, {rows}), entropy = floats(h, {rows}), lse = floats(h, {rows});
+  if (rows) {
+    Tensor work = floats(h, {ws_linear_token_scores_workspace_floats(rows, vocab)});
+    check(ws_linear_token_scores(h.const_data_ptr(), row_stride(h), w.const_data_ptr(), row_stride(w),
+                                 tokens.const_data_ptr<int64_t>(), rows, vocab, d, (float)inv_t,
+                                 work.data_ptr<float>(), lse.data_ptr<float>(), logprob.data_ptr<float>(),
+                                 entropy.data_ptr<float>(), stream_of(h)),
+          "ws_linear_token_scores");
+  }
+  return {logprob, entropy, lse};
+}
+
+struct HeadScoresFn : Function<HeadScoresFn> {
+  // Gradients go to the tensors that h and w were made from.
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& h,
+                               const Tensor& w, const Tensor& tokens, double inv_t, int64_t chunk_rows) {
+    auto [logprob, entropy, lse] = [&] {
+      at::AutoDispatchBelowAutograd guard;
+      return head_forward(h, w, tokens, inv_t);
+    }();
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({h, w, tokens, lse, entropy});
+    ctx->saved_data["inv_t"] = inv_t;
+    ctx->saved_data["chunk_rows"] = chunk_rows;
+    ctx->saved_data["want_h"] = hidden.requires_grad();
+    ctx->saved_data["want_w"] = weight.requires_grad();
+    ctx->saved_data["width"] = hidden.size(1);
+    ctx->saved_data["hidden_type"] = hidden.scalar_type();
+    ctx->saved_data["weight_type"] = weight.scalar_type();
+    return {logprob, entropy};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list d(7);
+    if (!grads[0].defined() && !grads[1].defined()) return d;
+    refuse_second();
+    const auto s = ctx->get_saved_variables();
+    const Tensor &h = s[0], &w = s[1];
+    const bool want_h = ctx->saved_data["want_h"].toBool(), want_w = ctx->saved_data["want_w"].toBool();
+    c10::DeviceGuard guard(h.device());
+    const int64_t rows = h.size(0), width = h.size(1), vocab = w.size(0);
+    const int64_t chunk = ctx->saved_data["chunk_rows"].toInt();
+    if (want_h) d[0] = at::empty({rows, width}, h.options());
+    Tensor dw = want_w ? floats(h, {vocab, width}) : Tensor();
+    if (rows) {
+      const Tensor g = upstream(grads[0]), e = upstream(grads[1]);
+      Tensor work = bytes(h, {ws_linear_token_scores_backward_workspace_bytes(rows, vocab, width, chunk)});
+      // The dHidden product reads the head weight along the vocabulary.
+      Tensor wt;
+      if (want_h && rows >= kTransposeMinRows && vocab % 8 == 0) {
+        wt = at::empty({width, vocab}, w.options());
+        check(ws_transpose_bf16(w.const_data_ptr(), row_stride(w), wt.data_ptr(), vocab, width, stream_of(w)),
+              "ws_transpose_bf16");
+      }
+      check(ws_linear_token_scores_backward(h.const_data_ptr(), row_stride(h), w.const_data_ptr(), row_stride(w),
+                                            ptr(wt), s[2].const_data_ptr<int64_t>(), float_ptr(s[3]),
+                                            float_ptr(s[4]), float_ptr(g), float_ptr(e), rows, vocab, width,
+                                            (float)ctx->saved_data["inv_t"].toDouble(), work.data_ptr(), chunk,
+                                            want_h ? d[0].data_ptr() : nullptr, width,
+                                            want_w ? dw.data_ptr<float>() : nullptr, width, stream_of(h)),
+            "ws_linear_token_scores_backward");
+    } else if (want_w) {
+      dw.zero_();
+    }
+    const int64_t cols = ctx->saved_data["width"].toInt();
+    if (want_h) d[0] = d[0].narrow(1, 0, cols).to(ctx->saved_data["hidden_type"].toScalarType());
+    if (want_w) d[1] = dw.narrow(1, 0, cols).to(ctx->saved_data["weight_type"].toScalarType());
+    return d;
+  }
+};
+std::tuple<Tensor, Tensor> native_head_scores(const Tensor& hidden, const Tensor& weight, const Tensor& h,
+                                              const Tensor& w, const Tensor& tokens, double inv_t,
+                                              int64_t chunk_rows) {
+  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
+    variable_list v = HeadScoresFn::apply(hidden, weight, h, w, tokens, inv_t, chunk_rows);
+    return {v[0], v[1]};
+  }
+  at::AutoDispatchBelowAutograd guard;
+  auto [logprob, entropy, lse] = head_forward(h, w, tokens, inv_t);
+  return {logprob, entropy};
+}
+
+// Undefined tensors cannot leave an operator: empty ones in the place of forms not wanted.
+FourTensors native_quantize(const Tensor& x, bool e8m0, int64_t form, bool transposed) {
+  auto [q, scale, qt, scale_t] = quantize(x, e8m0, form, transposed);
+  auto known = [&](Tensor& t) { return t.defined() ? t : bytes(x, {0, 0}); };
+  return {known(q), known(scale), known(qt), known(scale_t)};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(warpstate, m) {
+  m.def("native_quantize(Tensor x, bool e8m0, int form, bool transposed) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "native_product(Tensor a, int lda, Tensor sa, int ld_sa, int rows_a, Tensor b, int ldb, Tensor sb, "
+      "int ld_sb, int rows_b, bool e8m0) -> Tensor");
+  m.def(
+      "native_token_scores(Tensor logits, Tensor tokens, int top_k, float inv_t) -> (Tensor, Tensor, Tensor, "
+      "Tensor)");
+  m.def(
+      "native_head_scores(Tensor hidden, Tensor weight, Tensor h, Tensor w, Tensor tokens, float inv_t, "
+      "int chunk_rows) -> (Tensor, Tensor)");
+}
+TORCH_LIBRARY_IMPL(warpstate, CUDA, m) {
+  m.impl("native_quantize", &native_quantize);
+  m.impl("native_product", &native_product);
+  m.impl("native_token_scores", &native_token_scores);
+  m.impl("native_head_scores", &native_head_scores);
+  m.impl("fp8_linear", &linear_forward);
+  m.impl("fp8_linear_backward", &linear_backward);
+}
+TORCH_LIBRARY_IMPL(warpstate, AutogradCUDA, m) {
+  m.impl("native_token_scores", &native_token_scores);
+  m.impl("native_head_scores", &native_head_scores);
+  m.impl("fp8_linear", &linear);
+}

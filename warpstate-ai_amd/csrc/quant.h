@@ -86,18 +86,20 @@ struct QuantRow {
 
 // VEC: rows start on 16-byte boundaries (and their strides keep them there), so that whole
 // pieces of eight elements are loaded as vectors; others are loaded one element at a time.
-template <bool F32, int SCALE, int FORM, bool VEC>
+// R: rows per thread, 8, or 1 for few rows quantized by rows (tiles of 16 x 128).
+template <bool F32, int SCALE, int FORM, bool VEC, int R>
 static __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
   constexpr bool kRows = FORM & kQuantRows, kCols = FORM & kQuantCols, kBlocks = FORM & kQuantBlocks;
   static_assert(!kBlocks || !kRows, "a tile has row scales or one block scale");
+  static_assert(R == 8 || FORM == kQuantRows, "whole blocks of 128 rows");
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int tr = blockIdx.x / p.col_tiles, tc = blockIdx.x % p.col_tiles;
-  const int r0 = tr * kQBlock + 8 * (t >> 4), c0 = tc * kQBlock + 8 * (t & 15);
+  const int r0 = tr * 16 * R + R * (t >> 4), c0 = tc * kQBlock + 8 * (t & 15);
   const int left = p.cols - c0;  // columns of this thread's pieces inside the matrix
 
-  QuantRow<F32> x[8];
+  QuantRow<F32> x[R];
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
+  for (int r = 0; r < R; ++r) {
     const bool ok = r0 + r < p.rows;
     if (VEC && ok && left >= 8) {
       if constexpr (F32) {
@@ -150,7 +152,7 @@ static __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams 
   }
   if constexpr (kRows || kBlocks) {
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int r = 0; r < R; ++r) {
       float inv = inv_block;
       if constexpr (kRows) {
         unsigned m = 0;
@@ -172,45 +174,47 @@ static __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams 
       }
     }
   }
-  if (!kCols && !(kBlocks && p.qt)) return;  // uniform
-  // Transposed: this thread's eight columns, eight row bytes each, into LDS rows of the
-  // transposed tile, then whole rows out.
-  if constexpr (kCols) {
+  if constexpr (kCols || kBlocks) {
+    if (!kCols && !p.qt) return;  // uniform
+    // Transposed: this thread's eight columns, eight row bytes each, into LDS rows of the
+    // transposed tile, then whole rows out.
+    if constexpr (kCols) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        unsigned m = 0;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) m = max(m, x[r].magnitude(e));
+        m = max(m, (unsigned)__shfl_xor((int)m, 16, kWave));
+        m = max(m, (unsigned)__shfl_xor((int)m, 32, kWave));
+        if (lane < 16) amax[wave][8 * lane + e] = m;
+      }
+      __syncthreads();
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      unsigned m = 0;
+      const int c = 8 * (t & 15) + e;
+      float inv = inv_block;
+      if constexpr (kCols) {
+        unsigned scale;
+        inv = block_inverse<SCALE>(max(max(amax[0][c], amax[1][c]), max(amax[2][c], amax[3][c])), scale);
+        if (t < 16 && tc * kQBlock + c < p.cols)
+          store_scale<SCALE>(p.scale_t, p.ld_scale_t, tc * kQBlock + c, tr, scale);
+      }
+      u32x2_t o;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) m = max(m, x[r].magnitude(e));
-      m = max(m, (unsigned)__shfl_xor((int)m, 16, kWave));
-      m = max(m, (unsigned)__shfl_xor((int)m, 32, kWave));
-      if (lane < 16) amax[wave][8 * lane + e] = m;
+      for (int d = 0; d < 2; ++d)
+        o[d] = pack_e4m3(x[4 * d].at(e) * inv, x[4 * d + 1].at(e) * inv, x[4 * d + 2].at(e) * inv,
+                         x[4 * d + 3].at(e) * inv);
+      *reinterpret_cast<u32x2_t*>(&tile[c][8 * (t >> 4)]) = o;
     }
     __syncthreads();
-  }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int c = 8 * (t & 15) + e;
-    float inv = inv_block;
-    if constexpr (kCols) {
-      unsigned scale;
-      inv = block_inverse<SCALE>(max(max(amax[0][c], amax[1][c]), max(amax[2][c], amax[3][c])), scale);
-      if (t < 16 && tc * kQBlock + c < p.cols)
-        store_scale<SCALE>(p.scale_t, p.ld_scale_t, tc * kQBlock + c, tr, scale);
+    for (int i = 0; i < 4; ++i) {
+      const int c = 32 * i + (t >> 3), byte = 16 * (t & 7);
+      if (tc * kQBlock + c < p.cols && tr * kQBlock + byte < p.qt_cols)
+        *reinterpret_cast<u32x4_t*>(p.qt + (long)(tc * kQBlock + c) * p.ldqt + tr * kQBlock + byte) =
+            *reinterpret_cast<const u32x4_t*>(&tile[c][byte]);
     }
-    u32x2_t o;
-#pragma unroll
-    for (int d = 0; d < 2; ++d)
-      o[d] = pack_e4m3(x[4 * d].at(e) * inv, x[4 * d + 1].at(e) * inv, x[4 * d + 2].at(e) * inv,
-                       x[4 * d + 3].at(e) * inv);
-    *reinterpret_cast<u32x2_t*>(&tile[c][8 * (t >> 4)]) = o;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = 32 * i + (t >> 3), byte = 16 * (t & 7);
-    if (tc * kQBlock + c < p.cols && tr * kQBlock + byte < p.qt_cols)
-      *reinterpret_cast<u32x4_t*>(p.qt + (long)(tc * kQBlock + c) * p.ldqt + tr * kQBlock + byte) =
-          *reinterpret_cast<const u32x4_t*>(&tile[c][byte]);
   }
 }
 

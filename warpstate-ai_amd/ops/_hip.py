@@ -18,6 +18,7 @@ import torch
 
 LIBRARY_PATH = Path(__file__).resolve().parents[1] / "lib" / "libwarpstate_hip.so"
 AUTOGRAD_PATH = LIBRARY_PATH.with_name("libwarpstate_autograd.so")
+HOST_PATH = LIBRARY_PATH.with_name("libwarpstate_host.so")
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -167,6 +168,29 @@ def load_autograd() -> None:
                           RuntimeWarning, stacklevel=2)
             return
         _autograd_loaded = True
+
+
+_host_ops = None
+_host_tried = False
+
+
+def host_ops():
+    """The operators of ``csrc/host_ops.cpp`` (``torch.ops.warpstate``), loaded once, or None
+    where they are not built or belong to another PyTorch: their callers then allocate and
+    launch from Python, with the same results for more host time. Where the kernels are built,
+    that is warned about."""
+    global _host_ops, _host_tried
+    if not _host_tried:
+        with _lock:
+            if not _host_tried and LIBRARY_PATH.exists():
+                try:
+                    torch.ops.load_library(str(HOST_PATH))
+                    _host_ops = torch.ops.warpstate
+                except OSError as error:
+                    warnings.warn(f"native operators not loaded ({error}); launching from Python "
+                                  "(run __graft_entry__.build())", RuntimeWarning, stacklevel=3)
+                _host_tried = True
+    return _host_ops
 
 
 def call(name: str, *args) -> None:

@@ -78,6 +78,11 @@ def _scales(rows: int, blocks: int, e8m0: bool, device) -> Tensor:
 def _quantize(x: Tensor, e8m0: bool, form: int, transposed: bool = False):
     """(q, scale, qt, scale_t) as the kernel's whole buffers (``_data``, ``_scales``), None for
     the forms that are not wanted."""
+    native = _hip.host_ops()
+    if native is not None:
+        q, scale, qt, scale_t = native.native_quantize(x, e8m0, form, transposed)
+        return (*((q, scale) if form != _COLUMNS else (None, None)),
+                *((qt, scale_t) if form & _COLUMNS or transposed else (None, None)))
     rows, cols = x.shape
     row_blocks, col_blocks = _blocks(rows), _blocks(cols)
     q = scale = qt = scale_t = None
@@ -241,7 +246,7 @@ def fp8_mm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor,
     if a_scale.dtype not in _SCALE_TYPES:
         raise ValueError("Scales are torch.float8_e8m0fnu or torch.float32")
     if out is None:
-        out = torch.empty((m, n), dtype=BF16, device=a.device)
+        pass
     elif out.shape != (m, n) or out.device != a.device or out.dtype != BF16:
         raise ValueError(f"out must be a BF16 tensor of shape {[m, n]} on {a.device}")
     elif (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
@@ -251,6 +256,13 @@ def fp8_mm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor,
     sb, ld_sb, rows_b = _scale(b_scale, b, dtype, b_scale.shape[0] == n, "b_scale")
     a, b = _operand(a), _operand(b)
     wide = _ceil(k, 16)
+    native = _hip.host_ops() if out is None else None
+    if native is not None:
+        return native.native_product(a, a.stride(0) if m > 1 else wide, sa, ld_sa, rows_a, b,
+                                     b.stride(0) if n > 1 else wide, sb, ld_sb, rows_b,
+                                     dtype == E8M0)
+    if out is None:
+        out = torch.empty((m, n), dtype=BF16, device=a.device)
     _launch(a, a.stride(0) if m > 1 else wide, sa, ld_sa, rows_a, b, b.stride(0) if n > 1 else wide,
             sb, ld_sb, rows_b, dtype == E8M0, out, k)
     return out
@@ -346,6 +358,8 @@ def _linear_autograd(ctx, grad, *_buffers):
 
 
 _fp8_linear.register_autograd(_linear_autograd, setup_context=_linear_setup)
+
+_hip.host_ops()
 
 
 def fp8_linear(x: Tensor, weight: Tensor, scale_dtype: torch.dtype = E8M0) -> Tensor:

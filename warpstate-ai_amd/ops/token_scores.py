@@ -133,8 +133,9 @@ def token_scores(logits: Tensor, tokens: Tensor, top_k: int = 0,
     if not 0 <= top_k <= min(MAX_TOP_K, vocab):
         raise ValueError(f"top_k must lie in [0, {min(MAX_TOP_K, vocab)}], not {top_k}")
     tokens = _check_tokens(tokens, rows, logits.device)
-    return TokenScores(*_TokenScores.apply(_unit_rows(logits), tokens, int(top_k),
-                                           _inverse(temperature)))
+    native = _hip.host_ops()
+    scores = _TokenScores.apply if native is None else native.native_token_scores
+    return TokenScores(*scores(_unit_rows(logits), tokens, int(top_k), _inverse(temperature)))
 
 
 def _head_operand(t: Tensor) -> Tensor:
@@ -151,9 +152,10 @@ def _head_operand(t: Tensor) -> Tensor:
 
 
 class _LinearTokenScores(torch.autograd.Function):
+    """Scores from ``_head_operand``'s h and w, with gradients to the tensors they came from."""
+
     @staticmethod
-    def forward(ctx, hidden, weight, tokens, inv_t, chunk_rows):
-        h, w = _head_operand(hidden), _head_operand(weight)
+    def forward(ctx, hidden, weight, h, w, tokens, inv_t, chunk_rows):
         rows, d = h.shape
         vocab = w.shape[0]
         logprob, entropy, lse = torch.empty((3, rows), dtype=F32, device=h.device).unbind()
@@ -171,7 +173,7 @@ class _LinearTokenScores(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dlogprob, dentropy):
-        none = (None,) * 5
+        none = (None,) * 7
         want_h, want_w = ctx.needs_input_grad[:2]
         if (dlogprob is None and dentropy is None) or not (want_h or want_w):
             return none
@@ -196,7 +198,7 @@ class _LinearTokenScores(torch.autograd.Function):
         elif want_w:
             dw.zero_()
         return (None if dh is None else dh[:, :width].to(hidden_dtype),
-                None if dw is None else dw[:, :width].to(weight_dtype), None, None, None)
+                None if dw is None else dw[:, :width].to(weight_dtype), *none[2:])
 
 
 @torch.compiler.disable
@@ -220,4 +222,7 @@ def linear_token_scores(hidden: Tensor, weight: Tensor, tokens: Tensor, temperat
     if chunk_rows < 1:
         raise ValueError("chunk_rows must be positive")
     tokens = _check_tokens(tokens, hidden.shape[0], hidden.device)
-    return _LinearTokenScores.apply(hidden, weight, tokens, _inverse(temperature), int(chunk_rows))
+    native = _hip.host_ops()
+    scores = _LinearTokenScores.apply if native is None else native.native_head_scores
+    return scores(hidden, weight, _head_operand(hidden.detach()), _head_operand(weight.detach()),
+                  tokens, _inverse(temperature), int(chunk_rows))
