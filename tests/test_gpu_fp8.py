@@ -333,3 +333,37 @@ def test_linear_saves_no_more_than_it_reads():
     assert torch.equal(out, plain)
     for a, b in zip(torch.autograd.grad(out, [x, w], dy), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_refusals_on_the_gpu(native, monkeypatch):
+    """The same errors from either host path, before any launch."""
+    from ops import _hip
+
+    fp8 = _fp8()
+    if not native:
+        monkeypatch.setattr(_hip, "host_ops", lambda: None)
+    a, sa, b, sb = _operands(20, 40, 256, E8M0, False, True, 2)
+    cases = [((a.view(torch.uint8), sa, b, sb), "float8_e4m3fn"), ((a, sa, b[:, :128], sb), "Expected a"),
+             ((a, sa.view(torch.uint8), b, sb), "Scales are"), ((a, sa, b, values_f32(sb)), "float8_e8m0fnu"),
+             ((a, sa[:, :1], b, sb), "one scale per row"), ((a, sa, b, sa), "one scale per row"),
+             ((a, sa[:7], b, sb), "one scale per row"), ((a[:0], sa, b, sb), "non-empty"),
+             ((a, sa.cpu(), b, sb), "scales on")]
+    for args, match in cases:
+        with pytest.raises(ValueError, match=match):
+            fp8.fp8_mm(*args)
+    for out in (torch.empty((20, 40), device="cuda"), torch.empty((20, 41), device="cuda", dtype=BF16),
+                torch.empty((40, 20), device="cuda", dtype=BF16).T):
+        with pytest.raises(ValueError, match="out must"):
+            fp8.fp8_mm(a, sa, b, sb, out=out)
+    for x, match in ((torch.zeros(4, 4, device="cuda", dtype=torch.float16), "BF16 or FP32"),
+                     (torch.zeros(4, device="cuda"), "non-empty matrix"),
+                     (torch.zeros((0, 4), device="cuda"), "non-empty matrix")):
+        with pytest.raises(ValueError, match=match):
+            fp8.quantize_rows(x)
+    with pytest.raises(ValueError, match="Scales are"):
+        fp8.quantize_rows(torch.zeros(4, 4, device="cuda"), torch.float16)
+
+
+def values_f32(scale):
+    return torch.from_numpy(values(scale)).float().cuda()

@@ -14,7 +14,7 @@ def test_library_loads():
 
     native = _hip.host_ops()
     assert native is torch.ops.warpstate
-    for name in ("native_quantize", "native_product", "native_token_scores", "native_head_scores"):
+    for name in ("native_quantize", "native_quantize_rows", "native_fp8_mm", "native_token_scores", "native_head_scores"):
         assert hasattr(native, name)
 
 

@@ -14,7 +14,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
-#include <limits>
+#include <algorithm>
 
 #include "../../include/warpstate_hip.h"
 
@@ -80,12 +80,109 @@ void product(const Tensor& a, int64_t lda, const Tensor& sa, int64_t ld_sa, int6
                   ptr(work), stream_of(a)),
         "ws_fp8_mm");
 }
-Tensor native_product(const Tensor& a, int64_t lda, const Tensor& sa, int64_t ld_sa, int64_t rows_a,
-                      const Tensor& b, int64_t ldb, const Tensor& sb, int64_t ld_sb, int64_t rows_b, bool e8m0) {
-  Tensor out = at::empty({a.size(0), b.size(0)}, a.options().dtype(at::kBFloat16));
-  product(a, lda, sa, ld_sa, rows_a, b, ldb, sb, ld_sb, rows_b, e8m0, out, a.size(1));
+
+// --- quantize_rows and fp8_mm of ops/fp8_execution.py, with their checks -----------------------
+
+std::tuple<Tensor, Tensor> native_quantize_rows(const Tensor& x_in, bool e8m0) {
+  TORCH_CHECK_VALUE(x_in.scalar_type() == at::kBFloat16 || x_in.scalar_type() == at::kFloat,
+                    "Quantization takes BF16 or FP32 matrices");
+  TORCH_CHECK_VALUE(x_in.dim() == 2 && x_in.numel() > 0, "Quantization takes a non-empty matrix");
+  const int64_t rows = x_in.size(0), cols = x_in.size(1);
+  const bool unit = (x_in.stride(1) == 1 || cols == 1) && (rows == 1 || x_in.stride(0) >= cols);
+  const Tensor x = unit ? x_in : x_in.contiguous();
+  c10::DeviceGuard guard(x.device());
+  Tensor q = at::empty({rows, up(cols, 16)}, x.options().dtype(at::kFloat8_e4m3fn));
+  const int64_t n = blocks(cols);
+  Tensor scale = e8m0 ? at::empty({rows, up(n, 4)}, x.options().dtype(at::kFloat8_e8m0fnu)) : floats(x, {n, up(rows, 4)});
+  check(ws_fp8_quantize(x.const_data_ptr(), row_stride(x), x.scalar_type() == at::kFloat, rows, cols, WS_QUANT_ROWS,
+                        e8m0 ? WS_SCALE_E8M0 : WS_SCALE_F32, q.data_ptr(), q.size(1), scale.data_ptr(),
+                        scale.size(1), nullptr, 0, nullptr, 0, stream_of(x)),
+        "ws_fp8_quantize");
+  if (q.size(1) != cols) q = q.narrow(1, 0, cols);
+  if (!e8m0) return {q, scale.narrow(1, 0, rows).t()};
+  return {q, scale.size(1) == n ? scale : scale.narrow(1, 0, n)};
+}
+
+void check_operand(const Tensor& q, const char* name) {
+  TORCH_CHECK_VALUE(q.is_cuda(), "8-bit kernels require CUDA tensors");
+  TORCH_CHECK_VALUE(q.scalar_type() == at::kFloat8_e4m3fn && q.dim() == 2 && q.numel() > 0, name,
+                    " must be a non-empty float8_e4m3fn matrix");
+}
+
+// An operand with rows of whole 16-byte pieces: itself, or a zero-padded copy.
+Tensor packed(const Tensor& q_in) {
+  const int64_t rows = q_in.size(0), k = q_in.size(1);
+  if (q_in.stride(1) == 1 && k % 16 == 0 && reinterpret_cast<uintptr_t>(q_in.const_data_ptr()) % 16 == 0 &&
+      (rows == 1 || (q_in.stride(0) % 16 == 0 && q_in.stride(0) >= k)))
+    return q_in;
+  Tensor q = q_in.view(at::kByte);
+  if (std::min(q.stride(0), q.stride(1)) < 1) q = q.contiguous();  // an expanded matrix
+  Tensor out = bytes(q, {rows, up(k, 16)});
+  check(ws_fp8_pack(q.const_data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.size(1), rows, k, stream_of(q)),
+        "ws_fp8_pack");
   return out;
 }
+
+struct ScaleOperand {
+  Tensor t;
+  int64_t ld, rows;  // operand rows per scale row
+};
+// Scales in the layout the product reads: themselves, or a copy. `vector`: four rows' FP32
+// scales are read at a time.
+ScaleOperand scale_operand(const Tensor& scale, const Tensor& q, at::ScalarType type, bool vector, const char* name) {
+  const int64_t rows = q.size(0), nb = blocks(q.size(1));
+  TORCH_CHECK_VALUE(scale.scalar_type() == type && scale.device() == q.device() && scale.dim() == 2, name,
+                    " must be a matrix of ", type == at::kFloat ? "float32" : "float8_e8m0fnu", " scales on ",
+                    q.device());
+  const int64_t n = scale.size(0);
+  int64_t block_rows = 1;
+  if (n != rows || scale.size(1) != nb) {
+    block_rows = kBlock;
+    TORCH_CHECK_VALUE(n == blocks(rows) && scale.size(1) == nb, name,
+                      " must have one scale per row or per 128 rows and one per 128 columns, [", rows, ", ", nb,
+                      "] or [", blocks(rows), ", ", nb, "], not ", scale.sizes());
+  }
+  const int64_t s0 = scale.stride(0), s1 = scale.stride(1);
+  const int64_t size = (int64_t)scale.storage().nbytes(), first = scale.storage_offset();
+  const uintptr_t at = reinterpret_cast<uintptr_t>(scale.const_data_ptr());
+  if (type != at::kFloat) {
+    // The kernel reads whole dwords of a row.
+    const int64_t ld = n > 1 ? s0 : up(nb, 4);
+    if ((s1 == 1 || nb == 1) && ld % 4 == 0 && ld >= nb && at % 4 == 0 && first + (n - 1) * ld + up(nb, 4) <= size)
+      return {scale, ld, block_rows};
+    Tensor copy = bytes(scale, {n, up(nb, 4)});
+    copy.narrow(1, 0, nb).copy_(scale.view(at::kByte));
+    return {copy, copy.size(1), block_rows};
+  }
+  const int64_t ld = nb > 1 ? s1 : up(n, 4);
+  if ((s0 == 1 || n == 1) && ld >= n &&
+      (!vector || (ld % 4 == 0 && at % 16 == 0 && 4 * (first + (nb - 1) * ld + up(n, 4)) <= size)))
+    return {scale, ld, block_rows};
+  Tensor copy = floats(scale, {nb, up(n, 4)});
+  copy.narrow(1, 0, n).copy_(scale.t());
+  return {copy, copy.size(1), block_rows};
+}
+
+Tensor native_fp8_mm(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale) {
+  check_operand(a, "a");
+  check_operand(b, "b");
+  const int64_t m = a.size(0), k = a.size(1), n = b.size(0);
+  TORCH_CHECK_VALUE(b.size(1) == k && a.device() == b.device(), "Expected a [M, K] and b [N, K] on one device, got ",
+                    a.sizes(), " and ", b.sizes());
+  const at::ScalarType type = a_scale.scalar_type();
+  TORCH_CHECK_VALUE(type == at::kFloat || type == at::kFloat8_e8m0fnu,
+                    "Scales are torch.float8_e8m0fnu or torch.float32");
+  c10::DeviceGuard guard(a.device());
+  const ScaleOperand sa = scale_operand(a_scale, a, type, false, "a_scale");
+  const ScaleOperand sb = scale_operand(b_scale, b, type, b_scale.dim() == 2 && b_scale.size(0) == n, "b_scale");
+  const Tensor pa = packed(a), pb = packed(b);
+  const int64_t wide = up(k, 16);
+  Tensor out = at::empty({m, n}, a.options().dtype(at::kBFloat16));
+  product(pa, m > 1 ? pa.stride(0) : wide, sa.t, sa.ld, sa.rows, pb, n > 1 ? pb.stride(0) : wide, sb.t, sb.ld,
+          sb.rows, type != at::kFloat, out, k);
+  return out;
+}
+
 // On whole buffers of quantize().
 void product_of(const Tensor& a, const Tensor& sa, int64_t rows_a, const Tensor& b, const Tensor& sb,
                 int64_t rows_b, bool e8m0, const Tensor& out, int64_t k) {
@@ -354,9 +451,8 @@ FourTensors native_quantize(const Tensor& x, bool e8m0, int64_t form, bool trans
 
 TORCH_LIBRARY_FRAGMENT(warpstate, m) {
   m.def("native_quantize(Tensor x, bool e8m0, int form, bool transposed) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.def(
-      "native_product(Tensor a, int lda, Tensor sa, int ld_sa, int rows_a, Tensor b, int ldb, Tensor sb, "
-      "int ld_sb, int rows_b, bool e8m0) -> Tensor");
+  m.def("native_quantize_rows(Tensor x, bool e8m0) -> (Tensor, Tensor)");
+  m.def("native_fp8_mm(Tensor a, Tensor a_scale, Tensor b, Tensor b_scale) -> Tensor");
   m.def(
       "native_token_scores(Tensor logits, Tensor tokens, int top_k, float inv_t) -> (Tensor, Tensor, Tensor, "
       "Tensor)");
@@ -366,7 +462,8 @@ TORCH_LIBRARY_FRAGMENT(warpstate, m) {
 }
 TORCH_LIBRARY_IMPL(warpstate, CUDA, m) {
   m.impl("native_quantize", &native_quantize);
-  m.impl("native_product", &native_product);
+  m.impl("native_quantize_rows", &native_quantize_rows);
+  m.impl("native_fp8_mm", &native_fp8_mm);
   m.impl("native_token_scores", &native_token_scores);
   m.impl("native_head_scores", &native_head_scores);
   m.impl("fp8_linear", &linear_forward);

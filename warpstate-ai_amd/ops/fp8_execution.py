@@ -120,6 +120,10 @@ def quantize_rows(x: Tensor, scale_dtype: torch.dtype = E8M0) -> tuple[Tensor, T
     magnitude amax is the least power of two 2^e >= amax / 448 (e >= -126), or
     max(amax, 2^-100) / 448 in FP32. A block that holds an infinity or a NaN dequantizes to
     NaN there (everywhere under e8m0). The block's zeros stay zeros."""
+    native = _hip.host_ops()
+    if native is not None and x.is_cuda and scale_dtype in _SCALE_TYPES:
+        return native.native_quantize_rows(x.detach() if x.requires_grad else x,
+                                           scale_dtype == E8M0)
     x, e8m0 = _check_input(x, scale_dtype)
     q, scale = _quantize(x, e8m0, _ROWS)[:2]
     return _views(q, scale, x.shape[1], e8m0, x.shape[0])
@@ -237,8 +241,11 @@ def fp8_mm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor,
     there is no FP32 result. ``out`` (BF16, unit column stride) receives the result instead of
     a new tensor. Operands in other layouts than rows of whole 16-byte pieces, and scales in
     other layouts than ``quantize_rows`` gives, are copied first. No gradient is recorded."""
-    _check_operand(a, "a")
-    _check_operand(b, "b")
+    native = _hip.host_ops()
+    if native is not None and out is None and a.is_cuda:
+        return native.native_fp8_mm(a, a_scale, b, b_scale)
+    for q, name in ((a, "a"), (b, "b")):
+        _check_operand(q, name)
     (m, k), n = a.shape, b.shape[0]
     if b.shape[1] != k or a.device != b.device:
         raise ValueError(f"Expected a [M, K] and b [N, K] on one device, got {list(a.shape)} and "
@@ -246,7 +253,7 @@ def fp8_mm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor,
     if a_scale.dtype not in _SCALE_TYPES:
         raise ValueError("Scales are torch.float8_e8m0fnu or torch.float32")
     if out is None:
-        pass
+        out = torch.empty((m, n), dtype=BF16, device=a.device)
     elif out.shape != (m, n) or out.device != a.device or out.dtype != BF16:
         raise ValueError(f"out must be a BF16 tensor of shape {[m, n]} on {a.device}")
     elif (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
@@ -256,13 +263,6 @@ def fp8_mm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor,
     sb, ld_sb, rows_b = _scale(b_scale, b, dtype, b_scale.shape[0] == n, "b_scale")
     a, b = _operand(a), _operand(b)
     wide = _ceil(k, 16)
-    native = _hip.host_ops() if out is None else None
-    if native is not None:
-        return native.native_product(a, a.stride(0) if m > 1 else wide, sa, ld_sa, rows_a, b,
-                                     b.stride(0) if n > 1 else wide, sb, ld_sb, rows_b,
-                                     dtype == E8M0)
-    if out is None:
-        out = torch.empty((m, n), dtype=BF16, device=a.device)
     _launch(a, a.stride(0) if m > 1 else wide, sa, ld_sa, rows_a, b, b.stride(0) if n > 1 else wide,
             sb, ld_sb, rows_b, dtype == E8M0, out, k)
     return out
