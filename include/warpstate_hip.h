@@ -450,13 +450,13 @@ int ws_token_scores_backward(const void* logits, int64_t ld, int f32, const int6
 
 /* From hidden [rows, d] and the head weight [vocab, d] (BF16, 16-byte aligned rows, d a
  * multiple of 8): the logits are the FP32 products, and exist in registers only. */
-int64_t ws_linear_token_scores_workspace_floats(int64_t rows, int64_t vocab);
+int64_t ws_linear_token_scores_workspace_floats(int64_t rows, int64_t vocab, int64_t d);
 int ws_linear_token_scores(const void* hidden, int64_t ld_hidden, const void* weight,
                            int64_t ld_weight, const int64_t* tokens, int64_t rows, int64_t vocab,
                            int64_t d, float inv_temperature, float* workspace, float* lse,
                            float* logprob, float* entropy, void* stream);
 /* Gradients of sum(dlogprob logprob + dentropy entropy): dhidden [rows, d] BF16 and dweight
- * [vocab, d] FP32 (written), each nullable. The logits are recomputed chunk_rows rows at a
+ * [vocab, d] FP32 or, with dweight_bf16 (one chunk, ld_dweight = d), BF16 (written), each nullable. The logits are recomputed chunk_rows rows at a
  * time, and their gradient, rounded to BF16, feeds the two products. weight_t: null, or the
  * weight transposed ([d, vocab], vocab a multiple of 8). `workspace`: 256-byte aligned. */
 int64_t ws_linear_token_scores_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d,
@@ -466,8 +466,8 @@ int ws_linear_token_scores_backward(const void* hidden, int64_t ld_hidden, const
                                     const float* lse, const float* entropy, const float* dlogprob,
                                     const float* dentropy, int64_t rows, int64_t vocab, int64_t d,
                                     float inv_temperature, void* workspace, int64_t chunk_rows,
-                                    void* dhidden, int64_t ld_dhidden, float* dweight,
-                                    int64_t ld_dweight, void* stream);
+                                    void* dhidden, int64_t ld_dhidden, void* dweight,
+                                    int64_t ld_dweight, int dweight_bf16, void* stream);
 
 #ifdef __cplusplus
 }

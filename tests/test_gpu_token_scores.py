@@ -257,7 +257,7 @@ def test_empty_batch():
     assert dh.shape == (0, 16) and not bool(dw.any())
 
 
-HEADS = [(1, 8, 5), (3, 64, 130), (130, 40, 517), (257, 136, 1000), (300, 100, 264), (70, 256, 2304)]
+HEADS = [(1, 8, 5), (3, 64, 130), (2100, 64, 2056), (700, 72, 1501), (130, 40, 517), (257, 136, 1000), (300, 100, 264), (70, 256, 2304)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])

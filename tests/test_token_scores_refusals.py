@@ -73,7 +73,7 @@ def test_head_arguments(over, match):
 
 def _head_backward(**over):
     a = dict(h=P, ldh=64, w=P, ldw=64, wt=None, t=P, lse=P, en=P, g=P, e=P, rows=4, vocab=50, d=64, inv=1.0,
-             ws=P, chunk=4, dh=P, ldd=64, dw=P, lddw=64)
+             ws=P, chunk=4, dh=P, ldd=64, dw=P, lddw=64, bf=0)
     a.update(over)
     _hip.call("ws_linear_token_scores_backward", *a.values(), None)
 
@@ -81,7 +81,7 @@ def _head_backward(**over):
 @pytest.mark.parametrize("over,match", [
     (dict(ws=P + 16), "256-byte"), (dict(chunk=0), "chunk_rows"), (dict(dh=None, dw=None), "null"),
     (dict(ldd=63), "dhidden leading"), (dict(lddw=63), "dweight leading"), (dict(lse=None), "null"),
-    (dict(ldd=4_200_000), "row stride"),
+    (dict(ldd=4_200_000), "row stride"), (dict(bf=1, chunk=3), "one chunk"), (dict(bf=1, lddw=72), "one chunk"),
     (dict(rows=1 << 20, chunk=1 << 20, vocab=32768), "chunk_rows")])
 def test_head_backward_arguments(over, match):
     with pytest.raises(RuntimeError, match=match):
@@ -93,7 +93,8 @@ def test_workspace_queries():
     assert q("ws_token_scores_workspace_bytes", 1000, 8192, 5) == 0  # a part per row
     assert q("ws_token_scores_workspace_bytes", 1000, 8193, 5) == 1000 * 2 * (16 + 40)
     assert q("ws_token_scores_workspace_bytes", 1, 32768, 8) == 16 * (16 + 64)  # parts of 2048
-    assert q("ws_linear_token_scores_workspace_floats", 10, 1000) == 10 * (3 * 8 + 1)
+    assert q("ws_linear_token_scores_workspace_floats", 16384, 1000, 512) == 16384 * (3 * 8 + 1)  # parts of 128
+    assert q("ws_linear_token_scores_workspace_floats", 10, 1000, 512) == 10 * (3 * 16 + 1)  # parts of 64
     # Coefficients, one chunk of logit gradients padded to whole 64-column pieces.
     assert q("ws_linear_token_scores_backward_workspace_bytes", 4096, 10883, 2048, 4096) >= \
         4096 * 16 + 4096 * 10944 * 2

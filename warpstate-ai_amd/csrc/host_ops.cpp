@@ -361,7 +361,7 @@ std::tuple<Tensor, Tensor, Tensor> head_forward(const Tensor& h, const Tensor& w
   const int64_t rows = h.size(0), d = h.size(1), vocab = w.size(0);
   Tensor logprob = floats(h, {rows}), entropy = floats(h, {rows}), lse = floats(h, {rows});
   if (rows) {
-    Tensor work = floats(h, {ws_linear_token_scores_workspace_floats(rows, vocab)});
+    Tensor work = floats(h, {ws_linear_token_scores_workspace_floats(rows, vocab, d)});
     check(ws_linear_token_scores(h.const_data_ptr(), row_stride(h), w.const_data_ptr(), row_stride(w),
                                  tokens.const_data_ptr<int64_t>(), rows, vocab, d, (float)inv_t,
                                  work.data_ptr<float>(), lse.data_ptr<float>(), logprob.data_ptr<float>(),
@@ -401,7 +401,10 @@ struct HeadScoresFn : Function<HeadScoresFn> {
     const int64_t rows = h.size(0), width = h.size(1), vocab = w.size(0);
     const int64_t chunk = ctx->saved_data["chunk_rows"].toInt();
     if (want_h) d[0] = at::empty({rows, width}, h.options());
-    Tensor dw = want_w ? floats(h, {vocab, width}) : Tensor();
+    // A BF16 weight's gradient is rounded as it is written where one chunk makes all of it.
+    const bool bf16 = ctx->saved_data["weight_type"].toScalarType() == at::kBFloat16 && rows <= chunk && vocab % 8 == 0;
+    Tensor dw;
+    if (want_w) dw = at::empty({vocab, width}, h.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
     if (rows) {
       const Tensor g = upstream(grads[0]), e = upstream(grads[1]);
       Tensor work = bytes(h, {ws_linear_token_scores_backward_workspace_bytes(rows, vocab, width, chunk)});
@@ -417,7 +420,7 @@ struct HeadScoresFn : Function<HeadScoresFn> {
                                             float_ptr(s[4]), float_ptr(g), float_ptr(e), rows, vocab, width,
                                             (float)ctx->saved_data["inv_t"].toDouble(), work.data_ptr(), chunk,
                                             want_h ? d[0].data_ptr() : nullptr, width,
-                                            want_w ? dw.data_ptr<float>() : nullptr, width, stream_of(h)),
+                                            want_w ? dw.data_ptr() : nullptr, width, bf16, stream_of(h)),
             "ws_linear_token_scores_backward");
     } else if (want_w) {
       dw.zero_();

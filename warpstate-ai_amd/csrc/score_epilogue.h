@@ -77,7 +77,9 @@ struct FEpiScoreGrad {
   __device__ __forceinline__ static void run(const GemmParams& p, Acc16<FA, FB>& acc, int m_base,
                                              int n_base, int lane, int tm, int tn, int wn,
                                              unsigned char* stage) {
-    static_assert(FA * 16 == 64 && FB * 16 == 128, "staging holds a 64 x 128 wave tile");
+    // LPR lanes cover a row of the wave tile (8 columns each), RPI rows per instruction.
+    constexpr int LPR = FB * 2, RPI = 64 / LPR, NQ = FA * 16 / RPI;
+    static_assert(64 % LPR == 0 && NQ >= 1, "whole rows per instruction");
     opaque_lane(lane);
     const int c0 = 4 * (lane >> 4), ncols = p.N - n_base;
     const float scale = p.logit_scale;
@@ -106,12 +108,12 @@ struct FEpiScoreGrad {
     }
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's staging writes landed
-    const int c8 = 8 * (lane & 15);
+    const int c8 = 8 * (lane % LPR);
     const bool full = n_base + c8 + 7 < (int)p.ldc;
     __amdgpu_buffer_rsrc_t rc = make_rsrc(p.c + (long)m_base * p.ldc + n_base, 0x7fffffff);
 #pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      const int r = 4 * q + (lane >> 4);
+    for (int q = 0; q < NQ; ++q) {
+      const int r = RPI * q + lane / LPR;
       const bool ok = m_base + r < p.M && full;
       const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + r * epi_row<FB>() + c8 * 2);
       __builtin_amdgcn_raw_buffer_store_b128(v, rc, store_off(ok, (long)r * p.ldc + c8, 2), 0, kEpiNT);

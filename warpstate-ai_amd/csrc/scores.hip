@@ -138,14 +138,29 @@ int check_head(const void* hidden, long ld_hidden, const void* weight, long ld_w
     return set_error(kInvalid, "hidden and weight need 16-byte aligned rows of a multiple of 8 elements");
   return kOk;
 }
-// One partial per 128 columns.
-long head_parts(long vocab) { return (long)cdiv(vocab, 256) * 2; }
+// The logits product's macro-tile: with few rows most compute units would idle on 256 x 256, and
+// reading the head weight is what bounds it (HEADTILE).
+int head_tile(long rows, long vocab, long d) {
+  const int tile = pick_tile(rows, vocab, d, kKContig, kKContig, false, kEpiStore);
+  return tile == kTile256 || tile == kTile128x2 ? tile : kTile64x128;
+}
+// One partial per column block of a wave: 128 columns, or 64 of the smaller tiles.
+long head_parts(int tile, long vocab) { return (long)cdiv(vocab, tile == kTile256 ? 256 : 128) * 2; }
+
+template <class Epi>
+int run_head(const GemmParams& p, int tile, hipStream_t s) {
+  switch (tile) {
+    case kTile256: return run_fast<kKContig, kKContig, false, Epi>(p, kFusedCfg, s);
+    case kTile128x2: return run_ring<Ring128x2, kKContig, kKContig, false, Epi>(p, 1, s);
+    default: return run_ring<Ring64x128, kKContig, kKContig, false, Epi>(p, 1, s);
+  }
+}
 
 }  // namespace
 
-extern "C" int64_t ws_linear_token_scores_workspace_floats(int64_t rows, int64_t vocab) {
-  if (rows < 1 || vocab < 1) return 0;
-  return rows * (3 * head_parts(vocab) + 1);
+extern "C" int64_t ws_linear_token_scores_workspace_floats(int64_t rows, int64_t vocab, int64_t d) {
+  if (rows < 1 || vocab < 1 || d < 1) return 0;
+  return rows * (3 * head_parts(head_tile(rows, vocab, d), vocab) + 1);
 }
 
 extern "C" int ws_linear_token_scores(const void* hidden, int64_t ld_hidden, const void* weight,
@@ -157,14 +172,15 @@ extern "C" int ws_linear_token_scores(const void* hidden, int64_t ld_hidden, con
     return rc;
   if (!workspace || !lse || !logprob || !entropy) return set_error(kInvalid, "null output pointer");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const long parts = head_parts(vocab);
+  const int tile = head_tile(rows, vocab, d);
+  const long parts = head_parts(tile, vocab);
   p.targets = reinterpret_cast<const long*>(tokens);
   p.part_max = workspace;
   p.part_sum = p.part_max + rows * parts;
   p.part_wsum = p.part_sum + rows * parts;
   p.tgt_logit = p.part_wsum + rows * parts;
   p.parts_per_row = (int)parts;
-  if (int rc = run_fast<kKContig, kKContig, false, FEpiScoreStats>(p, kFusedCfg, s)) return rc;
+  if (int rc = run_head<FEpiScoreStats>(p, tile, s)) return rc;
   hipLaunchKernelGGL(score_combine_kernel, dim3(cdiv(rows, 4)), dim3(256), 0, s, p.part_max, p.part_sum,
                      p.part_wsum, p.parts_per_row, p.tgt_logit, p.targets, ScoreOut{lse, logprob, entropy},
                      (int)rows, (int)vocab);
@@ -188,8 +204,8 @@ extern "C" int ws_linear_token_scores_backward(const void* hidden, int64_t ld_hi
                                                const float* entropy, const float* dlogprob,
                                                const float* dentropy, int64_t rows, int64_t vocab, int64_t d,
                                                float inv_temperature, void* workspace, int64_t chunk_rows,
-                                               void* dhidden, int64_t ld_dhidden, float* dweight,
-                                               int64_t ld_dweight, void* stream) {
+                                               void* dhidden, int64_t ld_dhidden, void* dweight,
+                                               int64_t ld_dweight, int dweight_bf16, void* stream) {
   GemmParams p;
   if (int rc = check_head(hidden, ld_hidden, weight, ld_weight, tokens, rows, vocab, d, inv_temperature, p))
     return rc;
@@ -207,6 +223,8 @@ extern "C" int ws_linear_token_scores_backward(const void* hidden, int64_t ld_hi
   if (dweight) {
     if (ld_dweight < d) return set_error(kInvalid, "dweight leading dimension < d");
     if (int rc = check_out_stride(ld_dweight, 4, "dweight")) return rc;
+    if (dweight_bf16 && (ld_dweight != d || chunk < rows))
+      return set_error(kInvalid, "a BF16 weight gradient is contiguous and of one chunk");
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto* base = static_cast<unsigned char*>(workspace);
@@ -228,9 +246,12 @@ extern "C" int ws_linear_token_scores_backward(const void* hidden, int64_t ld_hi
     g.ldc = ldg;
     g.targets = reinterpret_cast<const long*>(tokens) + start;
     g.row_coef = reinterpret_cast<const float*>(coef + start);
-    if (int rc = run_fast<kKContig, kKContig, false, FEpiScoreGrad>(g, kFusedCfg, s)) return rc;
-    if (dweight) {
-      if (int rc = ce_chunk_weight_grad(c, gl, vocab, d, dweight, ld_dweight, start == 0, nullptr, s, false))
+    if (int rc = run_head<FEpiScoreGrad>(g, head_tile(c.r, vocab, d), s)) return rc;
+    if (dweight && dweight_bf16) {
+      if (int rc = ws_mm(gl, 1, ldg, c.hidden, ld_hidden, 1, dweight, vocab, d, c.r, 1, 0, stream)) return rc;
+    } else if (dweight) {
+      if (int rc = ce_chunk_weight_grad(c, gl, vocab, d, static_cast<float*>(dweight), ld_dweight, start == 0,
+                                        nullptr, s, false))
         return rc;
     }
     if (dhidden) {

@@ -98,13 +98,13 @@ SIGNATURES = {
                         + [_c_void_p] * 7),
     "ws_token_scores_backward": (_i32, [_c_void_p, _i64, _i32, _c_void_p, _i64, _i64, _f32]
                                  + [_c_void_p] * 5 + [_i64, _c_void_p]),
-    "ws_linear_token_scores_workspace_floats": (_i64, [_i64, _i64]),
+    "ws_linear_token_scores_workspace_floats": (_i64, [_i64, _i64, _i64]),
     "ws_linear_token_scores": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64,
                                       _f32] + [_c_void_p] * 5),
     "ws_linear_token_scores_backward_workspace_bytes": (_i64, [_i64] * 4),
     "ws_linear_token_scores_backward": (_i32, [_c_void_p, _i64, _c_void_p, _i64] + [_c_void_p] * 6
                                         + [_i64, _i64, _i64, _f32, _c_void_p, _i64, _c_void_p, _i64,
-                                           _c_void_p, _i64, _c_void_p]),
+                                           _c_void_p, _i64, _i32, _c_void_p]),
 }
 
 

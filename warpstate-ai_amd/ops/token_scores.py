@@ -27,10 +27,14 @@ from typing import NamedTuple
 import torch
 
 from ops import _hip
-from ops.fused_execution import DEFAULT_CE_CHUNK_ROWS, TRANSPOSE_MIN_ROWS, transpose
+from ops.fused_execution import TRANSPOSE_MIN_ROWS, transpose
 
 BF16, F32 = torch.bfloat16, torch.float32
 Tensor = torch.Tensor
+# Rows of the backward's chunks: their BF16 logit gradients take 1 GiB at a vocabulary of 32768. A
+# batch of one chunk writes a BF16 weight's gradient at once, without an FP32 sum beside it
+# (CHUNKNOTE).
+DEFAULT_CHUNK_ROWS = 16384
 MAX_TOP_K = 64
 MAX_VOCAB = 524288
 
@@ -160,7 +164,7 @@ class _LinearTokenScores(torch.autograd.Function):
         vocab = w.shape[0]
         logprob, entropy, lse = torch.empty((3, rows), dtype=F32, device=h.device).unbind()
         if rows:
-            need = _hip.query("ws_linear_token_scores_workspace_floats", rows, vocab)
+            need = _hip.query_on(h, "ws_linear_token_scores_workspace_floats", rows, vocab, d)
             work = torch.empty((need,), dtype=F32, device=h.device)
             _hip.call_on(h, "ws_linear_token_scores", h.data_ptr(), _row_stride(h), w.data_ptr(),
                          _row_stride(w), tokens.data_ptr(), rows, vocab, d, inv_t, work.data_ptr(),
@@ -182,7 +186,10 @@ class _LinearTokenScores(torch.autograd.Function):
         rows, d = h.shape
         vocab = w.shape[0]
         dh = torch.empty((rows, d), dtype=BF16, device=h.device) if want_h else None
-        dw = torch.empty((vocab, d), dtype=F32, device=h.device) if want_w else None
+        # A BF16 weight's gradient is rounded as it is written where one chunk makes all of it.
+        bf16 = weight_dtype == BF16 and rows <= chunk_rows and vocab % 8 == 0
+        dw = (torch.empty((vocab, d), dtype=BF16 if bf16 else F32, device=h.device) if want_w
+              else None)
         if rows:
             g, e = _grads(dlogprob, dentropy)
             need = _hip.query("ws_linear_token_scores_backward_workspace_bytes", rows, vocab, d,
@@ -194,7 +201,8 @@ class _LinearTokenScores(torch.autograd.Function):
             _hip.call_on(h, "ws_linear_token_scores_backward", h.data_ptr(), _row_stride(h),
                          w.data_ptr(), _row_stride(w), _hip.ptr(wt), tokens.data_ptr(),
                          lse.data_ptr(), entropy.data_ptr(), _hip.ptr(g), _hip.ptr(e), rows, vocab,
-                         d, inv_t, work.data_ptr(), chunk_rows, _hip.ptr(dh), d, _hip.ptr(dw), d)
+                         d, inv_t, work.data_ptr(), chunk_rows, _hip.ptr(dh), d, _hip.ptr(dw), d,
+                         int(bf16))
         elif want_w:
             dw.zero_()
         return (None if dh is None else dh[:, :width].to(hidden_dtype),
@@ -203,7 +211,7 @@ class _LinearTokenScores(torch.autograd.Function):
 
 @torch.compiler.disable
 def linear_token_scores(hidden: Tensor, weight: Tensor, tokens: Tensor, temperature: float = 1.0,
-                        chunk_rows: int = DEFAULT_CE_CHUNK_ROWS) -> tuple[Tensor, Tensor]:
+                        chunk_rows: int = DEFAULT_CHUNK_ROWS) -> tuple[Tensor, Tensor]:
     """(logprob, entropy) [rows] FP32 of ``tokens`` under the logits hidden @ weight.T, for hidden
     [rows, d] and the head weight [vocab, d], BF16 or FP32 (rounded to BF16 first, as F.linear
     under BF16 autocast does), with autograd to both.
