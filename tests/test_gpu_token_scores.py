@@ -396,3 +396,30 @@ def test_a_changed_operand_is_noticed():
         weight.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(out, [hidden])
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_refusals_on_the_gpu(native, monkeypatch):
+    """The same errors from either host path, before any launch."""
+    from ops import _hip
+
+    ts = _scores()
+    if not native:
+        monkeypatch.setattr(_hip, "host_ops", lambda: None)
+    x, tokens = _logits(4, 30, F32, 1).cuda(), _tokens(4, 30, 1).cuda()
+    cases = [((x.half(), tokens), "BF16 or FP32 logits"), ((x[0], tokens), "BF16 or FP32 logits"),
+             ((x[:, :0], tokens), "1 to 524288"), ((x, tokens[:3]), "int64 vector"),
+             ((x, tokens.int()), "int64 vector"), ((x, tokens.cpu()), "int64 vector"),
+             ((x, tokens, 31), "top_k must lie"), ((x, tokens, -1), "top_k must lie"),
+             ((torch.zeros((1, 524289), device="cuda"), tokens[:1]), "1 to 524288"),
+             ((x, tokens, 1, 0.0), "temperature"), ((x, tokens, 1, float("nan")), "temperature")]
+    for args, match in cases:
+        with pytest.raises(ValueError, match=match):
+            ts.token_scores(*args)
+    h, w = torch.zeros((4, 16), device="cuda"), torch.zeros((30, 16), device="cuda")
+    cases = [((h.half(), w, tokens), "BF16 or FP32"), ((h, w[:, :8], tokens), "Expected hidden"),
+             ((h, w[:0], tokens), "Expected hidden"), ((h, w, tokens[:2]), "int64 vector"),
+             ((h, w, tokens, -1.0), "temperature"), ((h, w, tokens, 1.0, 0), "chunk_rows")]
+    for args, match in cases:
+        with pytest.raises(ValueError, match=match):
+            ts.linear_token_scores(*args)

@@ -12,7 +12,7 @@ int run_quantize(const QuantParams& p, bool vec, hipStream_t s) {
   const long tiles = (long)cdiv(p.rows, 16 * R) * p.col_tiles;
   if (!fits_i32(tiles)) return set_error(kInvalid, "too many 128 x 128 tiles");
   if constexpr (FORM == kQuantRows && R == 8) {
-    // Few tiles: a row per thread (1 x 5632: 5.9 -> QROWS1 us).
+    // Few tiles: a row per thread (1 x 5632: 5.9 -> 2.9 us).
     if (tiles < device_cus()) return run_quantize<F32, SCALE, FORM, 1>(p, vec, s);
   }
   if (vec)

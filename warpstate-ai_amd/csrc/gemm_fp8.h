@@ -16,6 +16,12 @@
 // a row go to lane l: the k order is another than the instruction's own, but the same for
 // both operands, and a block has one scale.
 //
+// Rates (the 256 x 256 tile, e8m0 / FP32 scales, B in blocks): 8192 x 10240 x 2048 139 / 165 us
+// (2.5 / 2.1 PFLOP/s), 16384 x 2048 x 11264 254 / 318 us (3.0 / 2.4), where BF16 products reach
+// 1.4 to 1.5 and the instruction alone, in a loop on registers, 4.6. Between the two stand the
+// chain of a k-tile (fragment reads behind a barrier, then the MFMAs), the epilogue (about 4 us
+// a tile, a fifth of one with 16 k-tiles) and the clock under load.
+//
 // Scales. e8m0: the instruction's own block scales (v_mfma_scale), no arithmetic beside it. A
 // lane gives the scale byte of its operand row; a dword holds the four bytes of four k-tiles, and is
 // shifted by one byte per k-tile. FP32: the block's product starts from zero, and

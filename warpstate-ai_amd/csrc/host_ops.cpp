@@ -15,6 +15,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/warpstate_hip.h"
 
@@ -29,6 +30,7 @@ typedef std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> FiveTensors;
 
 constexpr int64_t kBlock = 128;
 constexpr int64_t kTransposeMinRows = 1024;  // fused_execution.TRANSPOSE_MIN_ROWS
+constexpr int64_t kMaxTopK = 64, kMaxVocab = 524288;
 
 void check(int status, const char* name) {
   TORCH_CHECK(status == 0, name, " failed (status ", status, "): ", ws_last_error());
@@ -345,7 +347,32 @@ struct TokenScoresFn : Function<TokenScoresFn> {
     return none;
   }
 };
-FourTensors native_token_scores(const Tensor& logits, const Tensor& tokens, int64_t top_k, double inv_t) {
+
+double inverse(double temperature) {
+  TORCH_CHECK_VALUE(temperature > 0.0 && std::isfinite(temperature) && 1.0 / temperature < 3.4e38,
+                    "The temperature must be positive and finite, not ", temperature);
+  return 1.0 / temperature;
+}
+Tensor checked_tokens(const Tensor& tokens, const Tensor& like) {
+  TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong && tokens.dim() == 1 && tokens.size(0) == like.size(0) &&
+                        tokens.device() == like.device(),
+                    "Tokens must be an int64 vector, one per row, on the operands' device");
+  return tokens.contiguous();
+}
+
+// token_scores of ops/token_scores.py, with its checks.
+FourTensors native_token_scores(const Tensor& logits_in, const Tensor& tokens_in, int64_t top_k, double temperature) {
+  TORCH_CHECK_VALUE((logits_in.scalar_type() == at::kBFloat16 || logits_in.scalar_type() == at::kFloat) &&
+                        logits_in.dim() == 2,
+                    "Expected BF16 or FP32 logits [rows, vocab]");
+  const int64_t rows = logits_in.size(0), vocab = logits_in.size(1);
+  TORCH_CHECK_VALUE(vocab >= 1 && vocab <= kMaxVocab, "Token scores take 1 to ", kMaxVocab, " logits a row, not ", vocab);
+  const int64_t most = std::min(kMaxTopK, vocab);
+  TORCH_CHECK_VALUE(top_k >= 0 && top_k <= most, "top_k must lie in [0, ", most, "], not ", top_k);
+  const Tensor tokens = checked_tokens(tokens_in, logits_in);
+  const double inv_t = inverse(temperature);
+  const bool unit = (logits_in.stride(1) == 1 || vocab == 1) && (rows <= 1 || logits_in.stride(0) >= vocab);
+  const Tensor logits = unit ? logits_in : logits_in.contiguous();
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     variable_list v = TokenScoresFn::apply(logits, tokens, top_k, inv_t);
     return {v[0], v[1], v[2], v[3]};
@@ -457,8 +484,8 @@ TORCH_LIBRARY_FRAGMENT(warpstate, m) {
   m.def("native_quantize_rows(Tensor x, bool e8m0) -> (Tensor, Tensor)");
   m.def("native_fp8_mm(Tensor a, Tensor a_scale, Tensor b, Tensor b_scale) -> Tensor");
   m.def(
-      "native_token_scores(Tensor logits, Tensor tokens, int top_k, float inv_t) -> (Tensor, Tensor, Tensor, "
-      "Tensor)");
+      "native_token_scores(Tensor logits, Tensor tokens, int top_k, float temperature) -> (Tensor, Tensor, "
+      "Tensor, Tensor)");
   m.def(
       "native_head_scores(Tensor hidden, Tensor weight, Tensor h, Tensor w, Tensor tokens, float inv_t, "
       "int chunk_rows) -> (Tensor, Tensor)");

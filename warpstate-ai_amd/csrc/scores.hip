@@ -138,8 +138,10 @@ int check_head(const void* hidden, long ld_hidden, const void* weight, long ld_w
     return set_error(kInvalid, "hidden and weight need 16-byte aligned rows of a multiple of 8 elements");
   return kOk;
 }
-// The logits product's macro-tile: with few rows most compute units would idle on 256 x 256, and
-// reading the head weight is what bounds it (HEADTILE).
+// The logits product's macro-tile: with few rows most compute units would idle on 256 x 256,
+// where reading the head weight is what bounds it (us, 256 x 256 / the choice: 64 x 2048 over
+// 32768 46 / 30, of which the weight takes 28 at the card's copy rate; 512 x 1280 over 10883
+// 36 / 27; 1000 rows over 32768 108 / 107).
 int head_tile(long rows, long vocab, long d) {
   const int tile = pick_tile(rows, vocab, d, kKContig, kKContig, false, kEpiStore);
   return tile == kTile256 || tile == kTile128x2 ? tile : kTile64x128;

@@ -31,9 +31,10 @@ from ops.fused_execution import TRANSPOSE_MIN_ROWS, transpose
 
 BF16, F32 = torch.bfloat16, torch.float32
 Tensor = torch.Tensor
-# Rows of the backward's chunks: their BF16 logit gradients take 1 GiB at a vocabulary of 32768. A
-# batch of one chunk writes a BF16 weight's gradient at once, without an FP32 sum beside it
-# (CHUNKNOTE).
+# Rows of the backward's chunks: their BF16 logit gradients take 1 GiB at a vocabulary of
+# 32768. A batch of one chunk writes a BF16 weight's gradient at once, without an FP32 sum beside
+# it (scores and gradients of 16384 rows, us, chunks of 8192 / 16384: 2048 over 32768 6426 /
+# 6240, 512 over 4096 610 / 399).
 DEFAULT_CHUNK_ROWS = 16384
 MAX_TOP_K = 64
 MAX_VOCAB = 524288
@@ -129,6 +130,9 @@ def token_scores(logits: Tensor, tokens: Tensor, top_k: int = 0,
     its likeliest tokens unspecified. Vocabularies up to 524288."""
     if not logits.is_cuda:
         raise ValueError("Token scores require CUDA tensors")
+    native = _hip.host_ops()
+    if native is not None:
+        return TokenScores(*native.native_token_scores(logits, tokens, top_k, temperature))
     if logits.dtype not in (BF16, F32) or logits.ndim != 2:
         raise ValueError("Expected BF16 or FP32 logits [rows, vocab]")
     rows, vocab = logits.shape
@@ -137,9 +141,8 @@ def token_scores(logits: Tensor, tokens: Tensor, top_k: int = 0,
     if not 0 <= top_k <= min(MAX_TOP_K, vocab):
         raise ValueError(f"top_k must lie in [0, {min(MAX_TOP_K, vocab)}], not {top_k}")
     tokens = _check_tokens(tokens, rows, logits.device)
-    native = _hip.host_ops()
-    scores = _TokenScores.apply if native is None else native.native_token_scores
-    return TokenScores(*scores(_unit_rows(logits), tokens, int(top_k), _inverse(temperature)))
+    return TokenScores(*_TokenScores.apply(_unit_rows(logits), tokens, int(top_k),
+                                           _inverse(temperature)))
 
 
 def _head_operand(t: Tensor) -> Tensor:
