@@ -390,8 +390,8 @@ enum WsQuantForm { WS_QUANT_ROWS = 1, WS_QUANT_COLUMNS = 2, WS_QUANT_BLOCKS = 4 
  *   WS_QUANT_BLOCKS   q [rows, cols], scale [ceil(rows / 128), ceil(cols / 128)], and, with qt,
  *                     the same values transposed: qt [cols, rows], scale_t the transpose of scale.
  * Scales: e8m0, the least power of two (at least 2^-126) under which the block's magnitudes
- * are at most 448; FP32, max(amax, 2^-100) / 448. q = rne(x / scale) (FP32 scales: x times
- * 448 / max(amax, 2^-100)). A block with an infinity or a NaN gets the scale NaN (e8m0) or
+ * are at most 448; FP32, a (1 / 448) with a = max(amax, 2^-100). q = rne(x / scale) (FP32
+ * scales: x times 448 (1 / a); every operation rounded to FP32). A block with an infinity or a NaN gets the scale NaN (e8m0) or
  * its amax / 448 (FP32). ldq and ldqt are multiples of 16 and their buffers 16-byte aligned;
  * bytes past cols (rows of x for qt) up to the next multiple of 16 are written as zeros. */
 int ws_fp8_quantize(const void* x, int64_t ldx, int x_f32, int64_t rows, int64_t cols, int form,

@@ -24,7 +24,7 @@ def block_scale(amax: float, scale_dtype) -> float:
             return 2.0 ** -126
         m, e = math.frexp(amax / 448.0)
         return 2.0 ** max(-126, e - 1 if m == 0.5 else e)
-    return float(np.float32(np.float32(max(amax, 2.0 ** -100)) / np.float32(448.0)))
+    return float(np.float32(max(amax, 2.0 ** -100)) * (np.float32(1.0) / np.float32(448.0)))
 
 
 def quantize(x: np.ndarray, scale_dtype, rows_per_block: int = 1):
@@ -39,8 +39,8 @@ def quantize(x: np.ndarray, scale_dtype, rows_per_block: int = 1):
             scale[i, b] = block_scale(amax, scale_dtype)
             if scale_dtype == E8M0:
                 scaled = x[at] / scale[i, b]
-            else:  # the factor is rounded once, and so is the product
-                factor = np.float32(448.0) / np.float32(max(amax, 2.0 ** -100))
+            else:  # every operation rounded to FP32
+                factor = np.float32(1.0) / np.float32(max(amax, 2.0 ** -100)) * np.float32(448.0)
                 scaled = (x[at].astype(np.float32) * factor).astype(np.float64)
             q[at] = e4m3_round(scaled)
     return q, scale

@@ -187,11 +187,15 @@ struct Fp8Epi {
   __device__ __forceinline__ static void run(const GemmParams& p, Acc16<FA, FB>& acc, int m_base,
                                              int n_base, int lane, int tm, int tn, int wn,
                                              unsigned char* stage) {
-    if (p.vec_out) {
+    constexpr int kRow = epi_row<FB>(), LPR = FB * 2, RPI = 64 / LPR, NQ = FA * 16 / RPI;
+    // All of the wave's columns inside (uniform): every staged piece is requested before the
+    // first is stored (FEpiStore tests each piece and waits for it: 8192 x 10240 x 2048
+    // EPIFIG).
+    const bool whole = p.vec_out && n_base + FB * 16 <= p.N;
+    if (p.vec_out && !whole) {
       FEpiStore<false, false>::run(p, acc, m_base, n_base, lane, tm, tn, wn, stage);
       return;
     }
-    constexpr int kRow = epi_row<FB>(), LPR = FB * 2, RPI = 64 / LPR;
     opaque_lane(lane);
 #pragma unroll
     for (int i = 0; i < FA; ++i)
@@ -203,6 +207,19 @@ struct Fp8Epi {
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's staging writes landed
     const int c8 = 8 * (lane % LPR);
+    if (whole) {
+      __amdgpu_buffer_rsrc_t rc = make_rsrc(p.c + (long)m_base * p.ldc + n_base, 0x7fffffff);
+      u32x4_t v[NQ];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+        v[q] = *reinterpret_cast<const u32x4_t*>(stage + (RPI * q + lane / LPR) * kRow + c8 * 2);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const int r = RPI * q + lane / LPR;
+        __builtin_amdgcn_raw_buffer_store_b128(v[q], rc, store_off(m_base + r < p.M, (long)r * p.ldc + c8, 2), 0, kEpiNT);
+      }
+      return;
+    }
 #pragma unroll 1
     for (int r = lane / LPR; r < FA * 16; r += RPI) {
       if (m_base + r >= p.M) break;
@@ -456,7 +473,16 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
       // MFMA phase. The second half of B's blocks is read into the first half's registers as
-      // those are used up; B(kt)'s stage is not refilled before the next phase but one.
+      // those are used up; B(kt)'s stage is not refilled before the next phase but one. In the
+      // last k-tile a wave of the second group that is ahead would stage its output over
+      // blocks that another still reads: the group meets once its reads are done, at a barrier that the
+      // first group takes before its epilogue.
+      auto reads_done = [&] {
+        if (TAIL && !first && kt + 1 == ke) {
+          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+          __builtin_amdgcn_s_barrier();
+        }
+      };
       if constexpr (SCALE == kScaleE8M0) {
 #pragma unroll
         for (int j = 0; j < FB; ++j) {
@@ -465,6 +491,7 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
           pin(acc.v[0][j], acc.v[1][j]);
           pin(acc.v[2][j], acc.v[3][j]);
           if (j < FB / 2) fb[j] = fp8_frag(sB + bst, boff + 2048 * (j + FB / 2));
+          if (j == FB / 2 - 1) reads_done();
           // (Left to the scheduler, all four reads go through one block's registers, each
           // waited for at once.)
           __builtin_amdgcn_sched_barrier(0);
@@ -480,6 +507,7 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
             prod[q & 1][1] = mfma_e4m3(fb[j % (FB / 2)], fa[i + 1], f32x4_v{0.f, 0.f, 0.f, 0.f});
             pin(prod[q & 1][0], prod[q & 1][1]);
             if (i == 2 && j < FB / 2) fb[j] = fp8_frag(sB + bst, boff + 2048 * (j + FB / 2));
+            if (i == 2 && j == FB / 2 - 1) reads_done();
           }
           if (q > 0) {
             const int jp = (q - 1) / 2, ip = 2 * ((q - 1) % 2);
@@ -502,6 +530,7 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
     for (; kt + 3 < ke; ++kt) k_tile(kt, std::false_type{}, std::true_type{});
     if (kt + 2 < ke) k_tile(kt++, std::false_type{}, std::false_type{});
     for (; kt < ke; ++kt) k_tile(kt, std::true_type{}, std::false_type{});
+    if (first) __builtin_amdgcn_s_barrier();  // the second group's reads of the last k-tile
     if (slice)
       fp8_partial(acc, sp.partials + (long)piece * (kFBM * kFBN) + wm * TM * kFBN + wn * TN, kFBN, lane);
     else

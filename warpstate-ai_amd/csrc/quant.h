@@ -4,9 +4,9 @@
 // same tensors as operands of a weight gradient, which reduces over the rows), or 128 x 128
 // (a weight). With amax the block's largest magnitude, the scale is
 //   e8m0: 2^e, e the least with amax / 2^e <= 448, in [-126, 127] (a byte e + 127), or
-//   FP32: a / 448, a = max(amax, 2^-100),
-// and q = rne(x * 1 / scale): exact scaling under e8m0; under FP32 the factor is 448 / a
-// rounded once, so that x * factor is at most 448 (1 + 2^-23), which rounds to 448. A block
+//   FP32: r(a r(1 / 448)), a = max(amax, 2^-100),
+// and q = rne(x * factor): 1 / scale exactly under e8m0; under FP32 r(448 r(1 / a)), within
+// 2^-23 of 448 / a, so that x * factor is at most 448 (1 + 2^-22), which rounds to 448. A block
 // with an infinity or a NaN gets the e8m0 NaN (255) or the FP32 scale inf / NaN, and its
 // infinities and NaNs become NaN (all of the block under e8m0). Magnitudes are compared as
 // integers, which ranks NaN above infinity above every number, so none is lost in the max.
@@ -53,11 +53,11 @@ __device__ __forceinline__ float block_inverse(unsigned amax_bits, unsigned& sca
     scale = (unsigned)code;
     return __uint_as_float(code == 255 ? 0x7fc00000u : (unsigned)(254 - code) << 23);
   } else {
-    // 2^-100 keeps 448 / a finite; the bits of a NaN stay the larger ones.
+    // 2^-100 keeps the factor finite; the bits of a NaN stay the larger ones.
     const unsigned floor_bits = 27u << 23;
     const float a = __uint_as_float(amax_bits > floor_bits ? amax_bits : floor_bits);
-    scale = __float_as_uint(a / kE4M3Max);
-    return kE4M3Max / a;
+    scale = __float_as_uint(a * (1.0f / kE4M3Max));
+    return (1.0f / a) * kE4M3Max;
   }
 }
 template <int SCALE>

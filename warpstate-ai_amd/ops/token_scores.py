@@ -31,11 +31,11 @@ from ops.fused_execution import TRANSPOSE_MIN_ROWS, transpose
 
 BF16, F32 = torch.bfloat16, torch.float32
 Tensor = torch.Tensor
-# Rows of the backward's chunks: their BF16 logit gradients take 1 GiB at a vocabulary of
+# Logit gradients of one chunk of the backward, BF16: 1 GiB, 16384 rows at a vocabulary of
 # 32768. A batch of one chunk writes a BF16 weight's gradient at once, without an FP32 sum beside
 # it (scores and gradients of 16384 rows, us, chunks of 8192 / 16384: 2048 over 32768 6426 /
 # 6240, 512 over 4096 610 / 399).
-DEFAULT_CHUNK_ROWS = 16384
+CHUNK_LOGITS = 1 << 29
 MAX_TOP_K = 64
 MAX_VOCAB = 524288
 
@@ -214,15 +214,15 @@ class _LinearTokenScores(torch.autograd.Function):
 
 @torch.compiler.disable
 def linear_token_scores(hidden: Tensor, weight: Tensor, tokens: Tensor, temperature: float = 1.0,
-                        chunk_rows: int = DEFAULT_CHUNK_ROWS) -> tuple[Tensor, Tensor]:
+                        chunk_rows: int | None = None) -> tuple[Tensor, Tensor]:
     """(logprob, entropy) [rows] FP32 of ``tokens`` under the logits hidden @ weight.T, for hidden
     [rows, d] and the head weight [vocab, d], BF16 or FP32 (rounded to BF16 first, as F.linear
     under BF16 autocast does), with autograd to both.
 
     The logits are FP32 and never leave the registers. The backward recomputes them
-    ``chunk_rows`` rows at a time; their gradient is rounded to BF16 once for the two products,
-    whose sums are FP32, and so is the weight's gradient over all chunks; both gradients come in
-    their operand's type. Under torch.compile it runs eagerly (a graph break)."""
+    ``chunk_rows`` rows at a time (None: as many as 1 GiB of BF16 gradients holds); their
+    gradient is rounded to BF16 once for the two products, whose sums are FP32, and so is the
+    weight's gradient over all chunks; both gradients come in their operand's type. Under torch.compile it runs eagerly (a graph break)."""
     if not (hidden.is_cuda and weight.is_cuda):
         raise ValueError("Token scores require CUDA tensors")
     if (hidden.ndim != 2 or weight.ndim != 2 or hidden.shape[1] != weight.shape[1]
@@ -230,6 +230,8 @@ def linear_token_scores(hidden: Tensor, weight: Tensor, tokens: Tensor, temperat
         raise ValueError("Expected hidden [rows, d] and weight [vocab, d] on one device")
     if hidden.dtype not in (BF16, F32) or weight.dtype not in (BF16, F32):
         raise ValueError("Head operands are BF16 or FP32")
+    if chunk_rows is None:
+        chunk_rows = max(256, CHUNK_LOGITS // weight.shape[0] // 256 * 256)
     if chunk_rows < 1:
         raise ValueError("chunk_rows must be positive")
     tokens = _check_tokens(tokens, hidden.shape[0], hidden.device)
