@@ -187,15 +187,11 @@ struct Fp8Epi {
   __device__ __forceinline__ static void run(const GemmParams& p, Acc16<FA, FB>& acc, int m_base,
                                              int n_base, int lane, int tm, int tn, int wn,
                                              unsigned char* stage) {
-    constexpr int kRow = epi_row<FB>(), LPR = FB * 2, RPI = 64 / LPR, NQ = FA * 16 / RPI;
-    // All of the wave's columns inside (uniform): every staged piece is requested before the
-    // first is stored (FEpiStore tests each piece and waits for it: 8192 x 10240 x 2048
-    // EPIFIG).
-    const bool whole = p.vec_out && n_base + FB * 16 <= p.N;
-    if (p.vec_out && !whole) {
+    if (p.vec_out) {
       FEpiStore<false, false>::run(p, acc, m_base, n_base, lane, tm, tn, wn, stage);
       return;
     }
+    constexpr int kRow = epi_row<FB>(), LPR = FB * 2, RPI = 64 / LPR;
     opaque_lane(lane);
 #pragma unroll
     for (int i = 0; i < FA; ++i)
@@ -207,19 +203,6 @@ struct Fp8Epi {
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's staging writes landed
     const int c8 = 8 * (lane % LPR);
-    if (whole) {
-      __amdgpu_buffer_rsrc_t rc = make_rsrc(p.c + (long)m_base * p.ldc + n_base, 0x7fffffff);
-      u32x4_t v[NQ];
-#pragma unroll
-      for (int q = 0; q < NQ; ++q)
-        v[q] = *reinterpret_cast<const u32x4_t*>(stage + (RPI * q + lane / LPR) * kRow + c8 * 2);
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        const int r = RPI * q + lane / LPR;
-        __builtin_amdgcn_raw_buffer_store_b128(v[q], rc, store_off(m_base + r < p.M, (long)r * p.ldc + c8, 2), 0, kEpiNT);
-      }
-      return;
-    }
 #pragma unroll 1
     for (int r = lane / LPR; r < FA * 16; r += RPI) {
       if (m_base + r >= p.M) break;
@@ -474,9 +457,9 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
       __builtin_amdgcn_sched_barrier(0);
       // MFMA phase. The second half of B's blocks is read into the first half's registers as
       // those are used up; B(kt)'s stage is not refilled before the next phase but one. In the
-      // last k-tile a wave of the second group that is ahead would stage its output over
-      // blocks that another still reads: the group meets once its reads are done, at a barrier that the
-      // first group takes before its epilogue.
+      // last k-tile a wave of the second group that is ahead would stage its output over blocks
+      // that another still reads: the group meets once its reads are done, at a barrier that
+      // the first group takes before its epilogue.
       auto reads_done = [&] {
         if (TAIL && !first && kt + 1 == ke) {
           __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)

@@ -222,7 +222,8 @@ def linear_token_scores(hidden: Tensor, weight: Tensor, tokens: Tensor, temperat
     The logits are FP32 and never leave the registers. The backward recomputes them
     ``chunk_rows`` rows at a time (None: as many as 1 GiB of BF16 gradients holds); their
     gradient is rounded to BF16 once for the two products, whose sums are FP32, and so is the
-    weight's gradient over all chunks; both gradients come in their operand's type. Under torch.compile it runs eagerly (a graph break)."""
+    weight's gradient over all chunks; both gradients come in their operand's type. Under
+    torch.compile it runs eagerly (a graph break)."""
     if not (hidden.is_cuda and weight.is_cuda):
         raise ValueError("Token scores require CUDA tensors")
     if (hidden.ndim != 2 or weight.ndim != 2 or hidden.shape[1] != weight.shape[1]
