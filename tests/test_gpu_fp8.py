@@ -287,6 +287,17 @@ def test_products_in_a_captured_graph():
         assert torch.equal(got, step())
 
 
+def test_product_inside_a_compiled_function():
+    fp8 = _fp8()
+    x = _matrix(130, 384, BF16, 21).clamp(-9, 9)
+    b, sb = fp8.quantize_weight(torch.randn((200, 384), device="cuda"))[:2]
+
+    def step(x):
+        return fp8.fp8_mm(*fp8.quantize_rows(x * 2.0), b, sb) + 1.0
+
+    assert torch.equal(torch.compile(step, backend="aot_eager")(x), step(x))
+
+
 def test_python_launches_agree_with_the_native_ones(monkeypatch):
     from ops import _hip
 

@@ -51,7 +51,12 @@ Fp8Plan fp8_plan(long m, long n, long k, bool brow, int scale_type) {
   const long pairs = k / 2;  // the loaders' count
   const int kt = cdiv(pairs, kFBK), cus = device_cus();
   Fp8Plan best{kTileFew, 0, 1, kt, 0};
-  if (m <= 32) return best;
+  // Few rows: reading A's fragments once per 16 columns costs less than tiles' prologues until
+  // the columns fill the card with tiles (16 rows) or with workgroups of 16 columns (32 rows,
+  // a reduction that eight waves share in few steps). us of e8m0 products, few rows' kernel /
+  // the best tile: 16 x 8192 x 2048 7.5 / 9.6, 16 x 16384 x 2048 12.3 / 9.9, 32 x 4096 x 2048 6.1 /
+  // 8.5, 32 x 6144 x 2048 10.4 / 9.4, 32 x 2048 x 5632 11.7 / 13.0, 32 x 2048 x 11264 20.6 / 15.7.
+  if (m <= 16 ? cdiv(n, 64) < cus : m <= 32 && cdiv(n, 16) <= cus && k <= 8192) return best;
   float t = 1e30f;
   for (int tile = 0; tile < kFastTiles; ++tile) {
     if (tile == kTile256 && scale_type == kScaleF32 && brow) continue;  // (would not fit the registers)
@@ -111,19 +116,19 @@ int run_fp8_256(GemmParams p, const Fp8Params& sp, hipStream_t s) {
   if (int rc = hip_check(hipGetLastError(), "8-bit product launch")) return rc;
   return sp.splits > 1 ? run_join<kFBM, kFBN>(p, sp, grid, s) : kOk;
 }
-template <int FA, int FB, int SCALE, bool BROW>
+template <int FA, int SCALE, bool BROW>
 int run_fp8_skinny(const GemmParams& p, const Fp8Params& sp, hipStream_t s) {
-  hipLaunchKernelGGL((gemm_fp8_skinny_kernel<FA, FB, SCALE, BROW>), dim3(cdiv(p.N, 16 * FB)), dim3(512), 0, s, p, sp);
+  hipLaunchKernelGGL((gemm_fp8_skinny_kernel<FA, SCALE, BROW>), dim3(cdiv(p.N, 16)), dim3(512), 0, s, p, sp);
   return hip_check(hipGetLastError(), "8-bit product launch");
 }
-template <int FB, int SCALE, bool BROW>
+template <int SCALE, bool BROW>
 int run_fp8_few(const GemmParams& p, const Fp8Params& sp, hipStream_t s) {
-  return p.M <= 16 ? run_fp8_skinny<1, FB, SCALE, BROW>(p, sp, s) : run_fp8_skinny<2, FB, SCALE, BROW>(p, sp, s);
+  return p.M <= 16 ? run_fp8_skinny<1, SCALE, BROW>(p, sp, s) : run_fp8_skinny<2, SCALE, BROW>(p, sp, s);
 }
 template <int SCALE, bool BROW>
 int run_fp8(const GemmParams& p, const Fp8Params& sp, int tile, hipStream_t s) {
   switch (tile) {
-    case kTileFew: return run_fp8_few<1, SCALE, BROW>(p, sp, s);
+    case kTileFew: return run_fp8_few<SCALE, BROW>(p, sp, s);
     case kTile256:
       if constexpr (SCALE == kScaleE8M0 || !BROW) return run_fp8_256<SCALE, BROW>(p, sp, s);
       break;

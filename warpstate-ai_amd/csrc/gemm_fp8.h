@@ -153,6 +153,21 @@ struct WaveScales {
                        : raw_b[0];
     }
   }
+  // Registers of their own for a copy's words. Sharing the request's, the next request goes to
+  // others and is waited for and copied within the same k-tile, with the operand loads ahead of
+  // it (e8m0, B in blocks, 16 x 11264 x 2048: 64 x 128 tiles 16.1 -> 12.4 us, 64 x 64 10.8 -> 9.8).
+  __device__ __forceinline__ void keep() {
+    if constexpr (!kE8) {
+#pragma unroll
+      for (int i = 0; i < FA; ++i) asm volatile("" : "+v"(a[i]));
+    }
+    if constexpr (!kE8 || !BROW) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < kWords; ++e) asm volatile("" : "+v"(b[j][e]));
+    }
+  }
   // e8m0: on to the next k-tile's byte.
   __device__ __forceinline__ void shift() {
 #pragma unroll
@@ -298,12 +313,14 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_fp8_ring_kernel(const GemmParams
       if ((kt & 3) == 0) {
         nxt.ready(lane);
         cur = nxt;
+        cur.keep();
         if (kt + 4 < ke) nxt.load(kt + 4);
       } else {
         cur.shift();
       }
     } else {
       cur = nxt;
+      cur.keep();
       if (kt + 1 < ke) nxt.load(kt + 1);
     }
     // Stage wr was read in the previous k-tile, which every wave has left (barrier).
@@ -522,24 +539,25 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
   }
 }
 
-// Few rows of A (at most 64: decoding, a short prompt): bound by reading B once. A workgroup of
-// eight waves takes all rows and 16 FB columns; the waves share the k-tiles in turn and read their
+// Few rows of A (at most 32: decoding, a short prompt): bound by reading B once. A workgroup of
+// eight waves takes all rows and 16 columns (sixteen waves, with fewer k-tiles each, were slower
+// everywhere: 1 x 11264 x 2048 10.5 us against 8.2); the waves share the k-tiles in turn and read their
 // fragments straight from memory (B's rows as whole 128-byte lines, A's from L2), the next
 // kAhead k-tiles requested before the current ones are used, and their partial products are
 // added in LDS in wave order.
-template <int FA, int FB, int SCALE, bool BROW>
+template <int FA, int SCALE, bool BROW>
 __global__ void __launch_bounds__(512) gemm_fp8_skinny_kernel(const GemmParams p, const Fp8Params sp) {
-  constexpr int kWaves = 8, kAhead = FA + FB <= 3 ? 4 : 2;
+  constexpr int kWaves = 8, kAhead = 4;
   constexpr bool kE8 = SCALE == kScaleE8M0;
   constexpr int kSB = kE8 || !BROW ? 1 : 4;
-  __shared__ f32x4_v red[kWaves][FA * FB][64];
+  __shared__ f32x4_v red[kWaves][FA][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = blockIdx.x * 16 * FB;
+  const int n0 = blockIdx.x * 16;
   const int ke = cdiv(p.K, kFBK);
   const long lda = 2 * p.a.s_row, ldb = 2 * p.b.s_row;
   const int kb = 2 * p.K;  // bytes of a row
-  const unsigned char *pa[FA], *pb[FB];
-  const char *psa[FA], *psb[FB];
+  const unsigned char *pa[FA], *pb;
+  const char *psa[FA], *psb;
   const int chunk = 16 * (lane >> 4);
 #pragma unroll
   for (int i = 0; i < FA; ++i) {
@@ -548,18 +566,17 @@ __global__ void __launch_bounds__(512) gemm_fp8_skinny_kernel(const GemmParams p
     const long q = r >> sp.a.shift;
     psa[i] = static_cast<const char*>(sp.a.ptr) + (kE8 ? q * sp.a.ld : 4 * q);
   }
-#pragma unroll
-  for (int j = 0; j < FB; ++j) {
-    const int r = min(n0 + 16 * j + (lane & 15), p.N - 1);
-    pb[j] = reinterpret_cast<const unsigned char*>(p.b.ptr) + r * ldb + chunk;
+  {
+    const int r = min(n0 + (lane & 15), p.N - 1);
+    pb = reinterpret_cast<const unsigned char*>(p.b.ptr) + r * ldb + chunk;
     // FP32 by rows: a lane's four columns at once (past the end the last whole four).
-    const long q = kSB == 4 ? min(n0 + 16 * j + 4 * (lane >> 4), (p.N - 1) & ~3) : r >> sp.b.shift;
-    psb[j] = static_cast<const char*>(sp.b.ptr) + (kE8 ? q * sp.b.ld : 4 * q);
+    const long q = kSB == 4 ? min(n0 + 4 * (lane >> 4), (p.N - 1) & ~3) : r >> sp.b.shift;
+    psb = static_cast<const char*>(sp.b.ptr) + (kE8 ? q * sp.b.ld : 4 * q);
   }
   const long step_a = kE8 ? 1 : 4 * sp.a.ld, step_b = kE8 ? 1 : 4 * sp.b.ld;
   struct Piece {
-    i32x8_t a[FA], b[FB];
-    unsigned sa[FA], sb[FB][kSB];
+    i32x8_t a[FA], b;
+    unsigned sa[FA], sb[kSB];
   };
   auto load8 = [&](const unsigned char* row, int kt) {
     const u32x4_t zero = {0, 0, 0, 0};
@@ -570,8 +587,7 @@ __global__ void __launch_bounds__(512) gemm_fp8_skinny_kernel(const GemmParams p
   };
   auto fetch = [&](Piece& x, int kt) {
     if (kt >= ke) return;  // uniform
-#pragma unroll
-    for (int j = 0; j < FB; ++j) x.b[j] = load8(pb[j], kt);
+    x.b = load8(pb, kt);
 #pragma unroll
     for (int i = 0; i < FA; ++i) x.a[i] = load8(pa[i], kt);
 #pragma unroll
@@ -579,39 +595,31 @@ __global__ void __launch_bounds__(512) gemm_fp8_skinny_kernel(const GemmParams p
       const char* q = psa[i] + kt * step_a;
       x.sa[i] = kE8 ? (unsigned)*reinterpret_cast<const unsigned char*>(q) : *reinterpret_cast<const unsigned*>(q);
     }
+    const char* q = psb + kt * step_b;
+    if constexpr (kSB == 4) {
+      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(q);
 #pragma unroll
-    for (int j = 0; j < FB; ++j) {
-      const char* q = psb[j] + kt * step_b;
-      if constexpr (kSB == 4) {
-        const u32x4_t v = *reinterpret_cast<const u32x4_t*>(q);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x.sb[j][e] = v[e];
-      } else {
-        x.sb[j][0] = kE8 ? (unsigned)*reinterpret_cast<const unsigned char*>(q) : *reinterpret_cast<const unsigned*>(q);
-      }
+      for (int e = 0; e < 4; ++e) x.sb[e] = v[e];
+    } else {
+      x.sb[0] = kE8 ? (unsigned)*reinterpret_cast<const unsigned char*>(q) : *reinterpret_cast<const unsigned*>(q);
     }
   };
-  f32x4_v acc[FA][FB];
+  f32x4_v acc[FA];
 #pragma unroll
-  for (int i = 0; i < FA; ++i)
-#pragma unroll
-    for (int j = 0; j < FB; ++j) acc[i][j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < FA; ++i) acc[i] = f32x4_v{0.f, 0.f, 0.f, 0.f};
   auto use = [&](const Piece& x, int kt) {
     if (kt >= ke) return;  // uniform
 #pragma unroll
-    for (int i = 0; i < FA; ++i)
+    for (int i = 0; i < FA; ++i) {
+      if constexpr (kE8) {
+        acc[i] = mfma_e4m3_scaled(x.b, x.a[i], acc[i], x.sb[0], x.sa[i]);
+      } else {
+        const f32x4_v v = mfma_e4m3(x.b, x.a[i], f32x4_v{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-      for (int j = 0; j < FB; ++j) {
-        if constexpr (kE8) {
-          acc[i][j] = mfma_e4m3_scaled(x.b[j], x.a[i], acc[i][j], x.sb[j][0], x.sa[i]);
-        } else {
-          const f32x4_v v = mfma_e4m3(x.b[j], x.a[i], f32x4_v{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            acc[i][j][e] = __builtin_fmaf(v[e], __uint_as_float(x.sa[i]) * __uint_as_float(x.sb[j][kSB == 4 ? e : 0]),
-                                          acc[i][j][e]);
-        }
+        for (int e = 0; e < 4; ++e)
+          acc[i][e] = __builtin_fmaf(v[e], __uint_as_float(x.sa[i]) * __uint_as_float(x.sb[kSB == 4 ? e : 0]), acc[i][e]);
       }
+    }
   };
   Piece piece[kAhead];
 #pragma unroll
@@ -624,16 +632,14 @@ __global__ void __launch_bounds__(512) gemm_fp8_skinny_kernel(const GemmParams p
     }
   }
 #pragma unroll
-  for (int i = 0; i < FA; ++i)
-#pragma unroll
-    for (int j = 0; j < FB; ++j) red[wave][i * FB + j][lane] = acc[i][j];
+  for (int i = 0; i < FA; ++i) red[wave][i][lane] = acc[i];
   __syncthreads();
-  for (int q = threadIdx.x; q < FA * FB * 64; q += 512) {
+  for (int q = threadIdx.x; q < FA * 64; q += 512) {
     const int blk = q >> 6, l = q & 63;
     f32x4_v v = red[0][blk][l];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) v += red[w][blk][l];
-    const int m = 16 * (blk / FB) + (l & 15), n = n0 + 16 * (blk % FB) + 4 * (l >> 4);
+    const int m = 16 * blk + (l & 15), n = n0 + 4 * (l >> 4);
     if (m >= p.M) continue;
     unsigned short* out = p.c + (long)m * p.ldc + n;
     if (p.vec_out) {
