@@ -348,6 +348,47 @@ def test_scores_in_a_captured_graph():
             assert torch.equal(a, b)
 
 
+def test_scores_inside_a_compiled_function():
+    """The calls break the graph and give what they give eagerly, gradients too."""
+    ts = _scores()
+    tokens = _tokens(37, 9001, 3).cuda()
+    up = torch.randn(37, device="cuda")
+    weight = torch.randn((900, 64), device="cuda").to(BF16)
+
+    def step(x, hidden):
+        got = ts.token_scores(x * 0.5, tokens, 5)
+        head, entropy = ts.linear_token_scores(hidden + 1.0, weight, tokens % 900)
+        return got.logprob * up + got.entropy + head - entropy, got.top_ids
+
+    compiled = torch.compile(step, backend="aot_eager")
+    results = []
+    for run in (step, compiled):
+        x = _logits(37, 9001, BF16, 3).cuda().requires_grad_(True)
+        hidden = torch.ones((37, 64), device="cuda", dtype=BF16, requires_grad=True)
+        score, ids = run(x, hidden)
+        results.append([score, ids, *torch.autograd.grad(score.sum(), [x, hidden])])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 255, 256, 257])
+def test_parts_joined_by_several_lanes_and_by_one(rows):
+    """Fewer rows than compute units join with several lanes on a key; both ways at top_k of
+    powers of two and between."""
+    ts = _scores()
+    logits = (_logits(rows, 34000, F32, rows) * 4).round() / 4  # with ties
+    tokens = _tokens(rows, 34000, rows)
+    tokens[0] = 0
+    x, t = logits.cuda(), tokens.cuda()
+    ids = _top(logits, 64)
+    want = _reference(logits, tokens, 1.0)[0]
+    tol = _bounds(logits, 1.0)[0]
+    for k in (1, 2, 3, 7, 8, 9, 31, 33, 63, 64):
+        got = ts.token_scores(x, t, k)
+        np.testing.assert_array_equal(got.top_ids.cpu().numpy(), ids[:, :k])
+        _near(got.logprob, want, tol)
+
+
 def test_python_launches_agree_with_the_native_ones(monkeypatch):
     from ops import _hip
 

@@ -32,11 +32,16 @@ int run_scores(const ScoreParams& p, int ept, hipStream_t s) {
   else launch_rows<F32, kLargeEpt>(p, s);
   if (int rc = hip_check(hipGetLastError(), "token score launch")) return rc;
   if (p.parts == 1) return kOk;
-  int lanes = 2, threads = 64;
+  int lanes = 2, threads = 64, per_key = 1;
   while (lanes < p.parts) lanes *= 2;
-  while (threads < p.parts * p.top_k && threads < 256) threads *= 2;
-  const int rows = 256 / threads, lds = rows * p.parts * p.top_k * 8;
-  hipLaunchKernelGGL((score_join_kernel<F32>), dim3(cdiv(p.rows, rows)), dim3(256), lds, s, p, threads, lanes);
+  const int total = p.parts * p.top_k;
+  // Enough rows fill the card with a thread per key.
+  if (p.rows < device_cus())
+    while (per_key * kScoreJoinAt < p.parts && 2 * per_key * total <= kScoreJoinThreads) per_key *= 2;
+  while (threads < total * per_key && threads < (per_key > 1 ? kScoreJoinThreads : 256)) threads *= 2;
+  const int block = threads > 256 ? threads : 256, rows = block / threads;
+  hipLaunchKernelGGL((score_join_kernel<F32>), dim3(cdiv(p.rows, rows)), dim3(block), rows * total * 8, s, p, threads,
+                     lanes, per_key);
   return hip_check(hipGetLastError(), "token score join launch");
 }
 
