@@ -121,3 +121,64 @@ def test_quantized_reference_is_what_the_product_reads():
     want_q, want_scale = quantize(values(w), E8M0, BLOCK)
     assert np.array_equal(dequantize(values(q), values(scale)), dequantize(want_q, want_scale))
     assert np.array_equal(dequantize(values(qt), values(scale_t)).T, dequantize(want_q, want_scale))
+
+
+def _training_step(master, seed=5):
+    """(inputs, step): forward and every gradient of a projection and the head's scores, from
+    leaves made within the step."""
+    from ops import fp8_execution as fp8
+    from ops import token_scores as ts
+
+    rows, d, hidden, vocab = 300, 136, 264, 1037
+    g = torch.Generator().manual_seed(seed)
+    dtype = F32 if master else BF16
+    make = lambda t, *s: torch.randn(s, generator=g).to(t).cuda()
+    inputs = [make(BF16, rows, d), make(dtype, hidden, d), make(dtype, vocab, hidden),
+              torch.randint(0, vocab, (rows,), generator=g).cuda(), make(F32, rows)]
+
+    def step():
+        x, w, head = (t.detach().requires_grad_(True) for t in inputs[:3])
+        tokens, up = inputs[3:]
+        logprob, entropy = ts.linear_token_scores(fp8.fp8_linear(x, w), head, tokens, 0.8, 128)
+        return (logprob, entropy, *torch.autograd.grad([logprob, entropy], [x, w, head], [up, -up]))
+
+    return inputs, step
+
+
+@pytest.mark.parametrize("master", [True, False])
+def test_training_step_in_a_captured_graph(master):
+    """Three chunks of rows, both kinds of weight: each replay is the eager step on its inputs,
+    with eager work between the replays."""
+    inputs, step = _training_step(master)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(3):
+        g = torch.Generator().manual_seed(50 + seed)
+        inputs[0].copy_(torch.randn(inputs[0].shape, generator=g))
+        inputs[4].copy_(torch.randn(inputs[4].shape, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in out]
+        for a, b in zip(kept, step()):
+            assert torch.equal(a, b)
+
+
+def test_two_steps_on_two_streams():
+    """Steps that overlap share no workspace: each gives what it gives alone."""
+    steps = [_training_step(True, 5)[1], _training_step(False, 6)[1]]
+    want = [step() for step in steps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in steps]
+    got = [[], []]
+    for _ in range(5):
+        for i, (stream, step) in enumerate(zip(streams, steps)):
+            with torch.cuda.stream(stream):
+                got[i].append(step())
+    torch.cuda.synchronize()
+    for results, alone in zip(got, want):
+        for result in results:
+            for a, b in zip(result, alone):
+                assert torch.equal(a, b)
