@@ -391,9 +391,10 @@ enum WsQuantForm { WS_QUANT_ROWS = 1, WS_QUANT_COLUMNS = 2, WS_QUANT_BLOCKS = 4 
  *                     the same values transposed: qt [cols, rows], scale_t the transpose of scale.
  * Scales: e8m0, the least power of two (at least 2^-126) under which the block's magnitudes
  * are at most 448; FP32, a (1 / 448) with a = max(amax, 2^-100). q = rne(x / scale) (FP32
- * scales: x times 448 (1 / a); every operation rounded to FP32). A block with an infinity or a NaN gets the scale NaN (e8m0) or
- * its amax / 448 (FP32). ldq and ldqt are multiples of 16 and their buffers 16-byte aligned;
- * bytes past cols (rows of x for qt) up to the next multiple of 16 are written as zeros. */
+ * scales: x times 448 (1 / a); every operation rounded to FP32). A block with an infinity or a
+ * NaN gets the scale NaN (e8m0) or its amax / 448 (FP32). ldq and ldqt are multiples of 16 and
+ * their buffers 16-byte aligned; bytes past cols (rows of x for qt) up to the next multiple of
+ * 16 are written as zeros. */
 int ws_fp8_quantize(const void* x, int64_t ldx, int x_f32, int64_t rows, int64_t cols, int form,
                     int scale_type, void* q, int64_t ldq, void* scale, int64_t ld_scale, void* qt,
                     int64_t ldqt, void* scale_t, int64_t ld_scale_t, void* stream);
@@ -405,11 +406,11 @@ int ws_fp8_pack(const void* src, int64_t s_row, int64_t s_col, void* dst, int64_
 
 /* BF16 C [m, n] (row stride ldc) = sum over blocks b of scale_a scale_b (A_b B_b^T) with e4m3 A
  * [m, k] (row stride lda) and B [n, k] (nn.Linear layout, row stride ldb), FP32 accumulation (of
- * groups of eight products whose terms the instruction cuts at 13 bits below the largest). k, lda and ldb are
- * multiples of 16 and the operands 16-byte aligned (bytes past a matrix's own reduction have
- * to be zero: ws_fp8_pack). *_block_rows is 1 (a scale per row and block) or 128 (per 128 rows
- * and block). e8m0 scales: 4-byte aligned, ld a multiple of 4, rows readable to the next
- * multiple of 4 bytes. FP32 scales of B with b_block_rows 1: 16-byte aligned, ld a multiple of
+ * groups of eight products whose terms the instruction cuts at 13 bits below the largest). k,
+ * lda and ldb are multiples of 16 and the operands 16-byte aligned (bytes past a matrix's own
+ * reduction have to be zero: ws_fp8_pack). *_block_rows is 1 (a scale per row and block) or 128
+ * (per 128 rows and block). e8m0 scales: 4-byte aligned, ld a multiple of 4, rows readable to
+ * the next multiple of 4 bytes. FP32 scales of B with b_block_rows 1: 16-byte aligned, ld a multiple of
  * 4. `workspace`: 16-byte aligned, ws_fp8_mm_workspace_bytes (null if that is 0): slices of the
  * reduction where the tiles alone would leave compute units idle. */
 int64_t ws_fp8_mm_workspace_bytes(int64_t m, int64_t n, int64_t k, int b_block_rows, int scale_type);
@@ -434,7 +435,8 @@ int ws_fp8_mm(const void* a, int64_t lda, const void* scale_a, int64_t ld_scale_
 /* From logits [rows, vocab] (row stride ld, BF16 or, with f32, FP32; any alignment of their
  * type; vocab at most 524288). top_k (0 to min(64, vocab)): top_ids and top_logprobs [rows,
  * top_k] receive the largest logits' ids and log probabilities, largest first, equal logits by
- * their lowest id. `workspace`: 16-byte aligned, ws_token_scores_workspace_bytes (null if that is 0). */
+ * their lowest id. `workspace`: 16-byte aligned, ws_token_scores_workspace_bytes (null if that
+ * is 0). */
 int64_t ws_token_scores_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k);
 int ws_token_scores(const void* logits, int64_t ld, int f32, const int64_t* tokens, int64_t rows,
                     int64_t vocab, float inv_temperature, int64_t top_k, void* workspace, float* lse,
@@ -456,9 +458,10 @@ int ws_linear_token_scores(const void* hidden, int64_t ld_hidden, const void* we
                            int64_t d, float inv_temperature, float* workspace, float* lse,
                            float* logprob, float* entropy, void* stream);
 /* Gradients of sum(dlogprob logprob + dentropy entropy): dhidden [rows, d] BF16 and dweight
- * [vocab, d] FP32 or, with dweight_bf16 (one chunk, ld_dweight = d), BF16 (written), each nullable. The logits are recomputed chunk_rows rows at a
- * time, and their gradient, rounded to BF16, feeds the two products. weight_t: null, or the
- * weight transposed ([d, vocab], vocab a multiple of 8). `workspace`: 256-byte aligned. */
+ * [vocab, d] FP32 or, with dweight_bf16 (one chunk, ld_dweight = d), BF16 (written), each
+ * nullable. The logits are recomputed chunk_rows rows at a time, and their gradient, rounded to
+ * BF16, feeds the two products. weight_t: null, or the weight transposed ([d, vocab], vocab a
+ * multiple of 8). `workspace`: 256-byte aligned. */
 int64_t ws_linear_token_scores_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d,
                                                         int64_t chunk_rows);
 int ws_linear_token_scores_backward(const void* hidden, int64_t ld_hidden, const void* weight,

@@ -16,8 +16,8 @@
 // a row go to lane l: the k order is another than the instruction's own, but the same for
 // both operands, and a block has one scale.
 //
-// Rates (the 256 x 256 tile, e8m0 / FP32 scales, B in blocks): 8192 x 10240 x 2048 139 / 165 us
-// (2.5 / 2.1 PFLOP/s), 16384 x 2048 x 11264 254 / 318 us (3.0 / 2.4), where BF16 products reach
+// Rates (the 256 x 256 tile, e8m0 / FP32 scales, B in blocks): 8192 x 10240 x 2048 138 / 164 us
+// (2.5 / 2.1 PFLOP/s), 16384 x 2048 x 11264 246 / 310 us (3.1 / 2.4), where BF16 products reach
 // 1.4 to 1.5 and the instruction alone, in a loop on registers, 4.6. Between the two stand the
 // chain of a k-tile (fragment reads behind a barrier, then the MFMAs), the epilogue (about 4 us
 // a tile, a fifth of one with 16 k-tiles) and the clock under load.
@@ -541,10 +541,11 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
 
 // Few rows of A (at most 32: decoding, a short prompt): bound by reading B once. A workgroup of
 // eight waves takes all rows and 16 columns (sixteen waves, with fewer k-tiles each, were slower
-// everywhere: 1 x 11264 x 2048 10.5 us against 8.2); the waves share the k-tiles in turn and read their
-// fragments straight from memory (B's rows as whole 128-byte lines, A's from L2), the next
-// kAhead k-tiles requested before the current ones are used, and their partial products are
-// added in LDS in wave order.
+// everywhere: 1 x 11264 x 2048 10.5 us against 8.2); the waves share the k-tiles in turn and
+// read their fragments straight from memory (B's rows as whole 128-byte lines, A's from L2), the
+// next kAhead k-tiles requested before the current ones are used, and their partial products
+// are added in LDS in wave order. 1 x 2048 x 5632: 6.2 us, of which reading B at the card's copy rate
+// takes 2.4.
 template <int FA, int SCALE, bool BROW>
 __global__ void __launch_bounds__(512) gemm_fp8_skinny_kernel(const GemmParams p, const Fp8Params sp) {
   constexpr int kWaves = 8, kAhead = 4;

@@ -2,7 +2,7 @@
 //
 // ops/fp8_execution.py and ops/token_scores.py check their arguments in Python and launch
 // through ctypes; allocating the outputs, the calls and above all the autograd nodes then take
-// longer than the kernels at small sizes (one 32768-token row: 23 us of host time for 11 us of
+// longer than the kernels at small sizes (one 32768-token row: 23 us of host time for 9 us of
 // kernels; scores and gradient of 1000 x 10883 logits: 109 us for 35). These do the same allocations
 // and make the same C calls without Python. Their arguments are the checked ones.
 //
@@ -284,8 +284,8 @@ FiveTensors linear(const Tensor& x, const Tensor& weight, bool e8m0, bool keep_x
 
 // --- token scores ---------------------------------------------------------------------------
 
-// (logprob, entropy, top logprobs, top ids, lse). lse is undefined unless it is kept (each
-// allocation less is 0.7 us): it then lies ahead of the workspace.
+// (logprob, entropy, top logprobs, top ids, lse). lse is undefined unless it is kept: small calls
+// are bound by the host, so it shares the workspace's allocation instead.
 FiveTensors scores_forward(const Tensor& logits, const Tensor& tokens, int64_t top_k, double inv_t, bool keep_lse) {
   c10::DeviceGuard guard(logits.device());
   const int64_t rows = logits.size(0), vocab = logits.size(1);

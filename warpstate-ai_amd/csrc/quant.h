@@ -13,11 +13,12 @@
 //
 // HBM-bound: x is read once (2 or 4 bytes an element), every form wanted of it written once
 // (1 byte each). 16384 x 5632 BF16 by rows and columns takes 82 us, 4.5 TB/s (the card copies at
-// 4.8); an 8960 x 1280 FP32 weight in both forms 13.7 us, 5.0 TB/s. A workgroup of 256 threads takes a 128 x 128 tile, in which all three kinds of block
-// are whole, and holds it in registers as 8 x 8 elements per thread: thread t has rows
-// 8 (t >> 4) .., columns 8 (t & 15) ... A row's 16 threads are neighbouring lanes; a
-// column's 16 threads are four lanes in each of the four waves. The transposed form goes
-// through LDS so that its rows leave as whole 128-byte lines.
+// 4.8); an 8960 x 1280 FP32 weight in both forms 15.5 us, 4.4 TB/s. A workgroup of 256 threads
+// takes a 128 x 128 tile, in which all three kinds of block are whole, and holds it in
+// registers as 8 x 8 elements per thread: thread t has rows 8 (t >> 4) .., columns
+// 8 (t & 15) ... A row's 16 threads are neighbouring lanes; a column's 16 threads are four lanes
+// in each of the four waves. The transposed form goes through LDS so that its rows leave as
+// whole 128-byte lines.
 #pragma once
 
 #include "common.h"

@@ -128,7 +128,7 @@ def token_scores(logits: Tensor, tokens: Tensor, top_k: int = 0,
     zero, whose rows get zeros. NaN or +inf logits make their row's scores NaN and the order of
     its likeliest tokens unspecified. Vocabularies up to 524288. Under torch.compile it runs
     eagerly (a graph break)."""
-    # (As a decorator of this function, disable() takes 1 us of a call's 12.)
+    # (Not a decorator of this function, which would add its own calls to each eager one.)
     scores = _eager_token_scores if torch.compiler.is_compiling() else _scores
     return scores(logits, tokens, top_k, temperature)
 
