@@ -72,14 +72,20 @@ __device__ __forceinline__ unsigned load_u32(__amdgpu_buffer_rsrc_t rs, unsigned
   return __builtin_amdgcn_raw_buffer_load_b32(rs, off, soff, 0);
 }
 
-// The scales of one wave's FA x FB blocks for one k-tile at a time: load() requests them,
+// The scales of one wave's FA x FB blocks for one k-tile at a time: load() requests them and
 // ready() makes them usable once they are there. BROW: B has a scale per row; otherwise the
 // wave's columns lie in one block of 128.
 //
-// e8m0: a lane requests the dword of one row, so that one load covers 64 rows, and ready()
-// hands lane l the words of rows 16 i + (l & 15) through the LDS crossbar. (With a load per
-// block, 4 lanes asking for each of its 16 rows, the 12 loads every four k-tiles cost a
-// 11264 x 2048 x 16384 product a fifth of its time: 411 us against 324 with B in blocks.)
+// e8m0: a lane requests the dword of one row, so that one load covers 64 rows and four k-tiles,
+// and ready() hands lane l the words of rows 16 i + (l & 15) through the LDS crossbar. (With a load
+// per block, 4 lanes asking for each of its 16 rows, the 12 loads every four k-tiles cost a
+// 11264 x 2048 x 16384 product a fifth of its time: 411 us against 324 with B in blocks.) FP32: a
+// load per block, every k-tile; through the crossbar 512 x 4096 x 4096 took 20.0 us against 18.6.
+//
+// OWN (the next request follows at once): every word goes to a register of its own. Sharing the
+// request's, the next request would go to another, and be waited for and copied within the same
+// k-tile, with the operand loads ahead of it (e8m0, B in blocks, 16 x 11264 x 2048: 64 x 128 tiles
+// 16.1 -> 12.4 us, 64 x 64 10.8 -> 9.8).
 template <int SCALE, bool BROW, int FA, int FB>
 struct WaveScales {
   static constexpr bool kE8 = SCALE == kScaleE8M0;
@@ -88,10 +94,10 @@ struct WaveScales {
   static constexpr int LA = kE8 ? (16 * FA + 63) / 64 : FA;
   static constexpr int LB = kE8 && BROW ? (16 * FB + 63) / 64 : NB;
   const char *base_a, *base_b;
-  long step_a, step_b;  // bytes per k-tile (FP32)
+  long step_a, step_b;  // bytes per k-tile
   unsigned off_a[LA], off_b[LB];
   unsigned a[FA], b[NB][kWords];
-  unsigned raw_a[kE8 ? LA : 1], raw_b[kE8 ? LB : 1];
+  unsigned raw_a[LA], raw_b[LB][kWords];
 
   // m_base, n_base: first row and column of the wave's tile.
   __device__ __forceinline__ void init(const Fp8Params& p, int m_base, int n_base, int M, int N,
@@ -100,15 +106,15 @@ struct WaveScales {
     // for a scale per row under FP32); nothing of it is stored.
     const long ra = min(m_base, M - 1) >> p.a.shift;
     const long rb = min(n_base, kWords == 4 ? (N - 1) & ~3 : N - 1) >> p.b.shift;
-    const int unit = kE8 ? 1 : 4;
-    base_a = static_cast<const char*>(p.a.ptr) + ra * (kE8 ? p.a.ld : 4);
-    base_b = static_cast<const char*>(p.b.ptr) + rb * (kE8 ? p.b.ld : 4);
-    step_a = p.a.ld * unit;
-    step_b = p.b.ld * unit;
+    const long row_a = kE8 ? p.a.ld : 4, row_b = kE8 ? p.b.ld : 4;  // bytes per row
+    base_a = static_cast<const char*>(p.a.ptr) + ra * row_a;
+    base_b = static_cast<const char*>(p.b.ptr) + rb * row_b;
+    step_a = kE8 ? 1 : 4 * p.a.ld;
+    step_b = kE8 ? 1 : 4 * p.b.ld;
 #pragma unroll
     for (int i = 0; i < LA; ++i) {
       const int row = m_base + (kE8 ? 64 * i + lane % (FA < 4 ? 16 * FA : 64) : 16 * i + (lane & 15));
-      off_a[i] = (unsigned)(((min(row, M - 1) >> p.a.shift) - ra) * (kE8 ? p.a.ld : 4));
+      off_a[i] = (unsigned)(((min(row, M - 1) >> p.a.shift) - ra) * row_a);
     }
 #pragma unroll
     for (int j = 0; j < LB; ++j) {
@@ -119,53 +125,41 @@ struct WaveScales {
   }
   // Requests the scales of k-tile kt (e8m0: of kt .. kt + 3, kt a multiple of 4).
   __device__ __forceinline__ void load(int kt) {
-    __amdgpu_buffer_rsrc_t ra = make_rsrc(base_a + (kE8 ? (long)kt : kt * step_a), 0x7fffffff);
-    __amdgpu_buffer_rsrc_t rb = make_rsrc(base_b + (kE8 ? (long)kt : kt * step_b), 0x7fffffff);
-    if constexpr (kE8) {
+    __amdgpu_buffer_rsrc_t ra = make_rsrc(base_a + kt * step_a, 0x7fffffff);
+    __amdgpu_buffer_rsrc_t rb = make_rsrc(base_b + kt * step_b, 0x7fffffff);
 #pragma unroll
-      for (int i = 0; i < LA; ++i) raw_a[i] = load_u32(ra, off_a[i], 0);
+    for (int i = 0; i < LA; ++i) raw_a[i] = load_u32(ra, off_a[i], 0);
 #pragma unroll
-      for (int j = 0; j < LB; ++j) raw_b[j] = load_u32(rb, off_b[j], 0);
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < FA; ++i) a[i] = load_u32(ra, off_a[i], 0);
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
+    for (int j = 0; j < LB; ++j) {
       if constexpr (kWords == 1) {
-        b[j][0] = load_u32(rb, off_b[j], 0);
+        raw_b[j][0] = load_u32(rb, off_b[j], 0);
       } else {
         const u32x4_t v = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rb, off_b[j], 0, 0));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) b[j][e] = v[e];
+        for (int e = 0; e < 4; ++e) raw_b[j][e] = v[e];
       }
     }
   }
-  // e8m0, after a load(): the words to the lanes that use them.
+  // After a load(): the words to the lanes that use them.
+  template <bool OWN>
   __device__ __forceinline__ void ready(int lane) {
-    if constexpr (kE8) {
+    auto take = [](unsigned word) {
+      if (OWN) asm volatile("" : "+v"(word));
+      return word;
+    };
+    auto from = [&](unsigned word, int block) {
+      return (unsigned)__builtin_amdgcn_ds_bpermute(4 * (16 * (block % 4) + (lane & 15)), (int)word);
+    };
 #pragma unroll
-      for (int i = 0; i < FA; ++i)
-        a[i] = (unsigned)__builtin_amdgcn_ds_bpermute(4 * (16 * (i % 4) + (lane & 15)), (int)raw_a[i / 4]);
+    for (int i = 0; i < FA; ++i) a[i] = kE8 ? from(raw_a[i / (kE8 ? 4 : 1)], i) : take(raw_a[kE8 ? 0 : i]);
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
-        b[j][0] = BROW ? (unsigned)__builtin_amdgcn_ds_bpermute(4 * (16 * (j % 4) + (lane & 15)), (int)raw_b[BROW ? j / 4 : 0])
-                       : raw_b[0];
-    }
-  }
-  // Registers of their own for a copy's words. Sharing the request's, the next request goes to
-  // others and is waited for and copied within the same k-tile, with the operand loads ahead of
-  // it (e8m0, B in blocks, 16 x 11264 x 2048: 64 x 128 tiles 16.1 -> 12.4 us, 64 x 64 10.8 -> 9.8).
-  __device__ __forceinline__ void keep() {
-    if constexpr (!kE8) {
+    for (int j = 0; j < NB; ++j) {
+      if constexpr (kE8 && BROW) {
+        b[j][0] = from(raw_b[j / 4][0], j);
+      } else {
 #pragma unroll
-      for (int i = 0; i < FA; ++i) asm volatile("" : "+v"(a[i]));
-    }
-    if constexpr (!kE8 || !BROW) {
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int e = 0; e < kWords; ++e) asm volatile("" : "+v"(b[j][e]));
+        for (int e = 0; e < kWords; ++e) b[j][e] = take(raw_b[j][e]);
+      }
     }
   }
   // e8m0: on to the next k-tile's byte.
@@ -299,29 +293,21 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_fp8_ring_kernel(const GemmParams
     la.issue(p.a, row0_a, kt * kFBK, p.K, st, wave, lane);
     lb.issue(p.b, row0_b, kt * kFBK, p.K, st + Cfg::kTileA, wave, lane);
   };
-  typedef WaveScales<SCALE, BROW, FA, FB> Scales;
-  Scales cur, nxt;
-  nxt.init(sp, row0_a + wm * TM, row0_b + wn * TN, p.M, p.N, lane);
-  nxt.load(kb);
+  WaveScales<SCALE, BROW, FA, FB> sc;
+  sc.init(sp, row0_a + wm * TM, row0_b + wn * TN, p.M, p.N, lane);
+  sc.load(kb);
 #pragma unroll
   for (int s = 0; s + 1 < S; ++s) issue(kb + s, s);
   int rd = 0, wr = S - 1;
   for (int kt = kb; kt < ke; ++kt) {
     __builtin_amdgcn_s_waitcnt(wait_vmcnt(kWaitLoads));
     __builtin_amdgcn_s_barrier();
-    if constexpr (Scales::kE8) {
-      if ((kt & 3) == 0) {
-        nxt.ready(lane);
-        cur = nxt;
-        cur.keep();
-        if (kt + 4 < ke) nxt.load(kt + 4);
-      } else {
-        cur.shift();
-      }
+    constexpr int kStep = SCALE == kScaleE8M0 ? 4 : 1;  // k-tiles of one request
+    if (kt % kStep == 0) {
+      sc.template ready<true>(lane);
+      if (kt + kStep < ke) sc.load(kt + kStep);
     } else {
-      cur = nxt;
-      cur.keep();
-      if (kt + 1 < ke) nxt.load(kt + 1);
+      sc.shift();
     }
     // Stage wr was read in the previous k-tile, which every wave has left (barrier).
     issue(kt + S - 1, wr);
@@ -339,7 +325,7 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_fp8_ring_kernel(const GemmParams
 #pragma unroll
     for (int i = 0; i < FA; ++i)
 #pragma unroll
-      for (int j = 0; j < FB; ++j) cur.mac(acc.v[i][j], bf[j], af[i], i, j);
+      for (int j = 0; j < FB; ++j) sc.mac(acc.v[i][j], bf[j], af[i], i, j);
     rd = rd + 1 == S ? 0 : rd + 1;
     // This wave's fragment reads are complete (its MFMAs have issued) before the barrier
     // that lets other waves' loads overwrite the stage.
@@ -361,8 +347,7 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_fp8_ring_kernel(const GemmParams
 // 256 x 256 tiles: the two-group pipeline of gemm_fast.h (its comment has the schedule), A in
 // two LDS stages and B in three. A k-tile is 24 fragment reads and 32 MFMAs, as many LDS bytes
 // and as much matrix-pipe time as there. The scales are requested at the head of a read phase,
-// ahead of its operand loads (a wait that leaves those in flight has then seen the scales), and
-// used in the MFMA phase after it.
+// ahead of its operand loads: a wait that leaves those in flight has then seen the scales.
 // Fragment of the 16-row block at `at` (its lane's first chunk): the chunks c and c ^ 4.
 __device__ __forceinline__ i32x8_t fp8_frag(const unsigned char* tile, unsigned at) {
   return join_frag(*reinterpret_cast<const bf16x8_t*>(tile + at), *reinterpret_cast<const bf16x8_t*>(tile + (at ^ 64)));
@@ -404,6 +389,7 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
       for (int j = 0; j < FB; ++j) acc.v[i][j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
     WaveScales<SCALE, BROW, FA, FB> sc;
     sc.init(sp, row0_a + wm * TM, row0_b + wn * TN, p.M, p.N, lane);
+    if (SCALE == kScaleE8M0) sc.load(kb);
 
     // This wave's share of its group's operand tile: one quarter, eight loads of 8 rows each,
     // 32 rows apart. Rows past the matrix take the last one's bytes (their results are not
@@ -448,8 +434,18 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
       constexpr bool TAIL = decltype(tail)::value;
       // Read phase. A(kt + 1) goes to the stage A(kt - 1) used and B(kt + 2) to the one
       // B(kt - 1) used: both groups have read those.
-      if (SCALE == kScaleF32 || (kt & 3) == 0) sc.load(kt);
-      else sc.shift();
+      // e8m0 scales are requested four k-tiles ahead (the last request is repeated: with one left
+      // out, as a branch, the compiler loses count of the loads after it; requested where they are
+      // used, 8192 x 8192 x 8192 with B's scales by rows took 416 us against 404). FP32 scales, which
+      // would take more registers than there are, for this MFMA phase.
+      if constexpr (SCALE == kScaleF32) {
+        sc.load(kt);
+      } else if ((kt & 3) == 0) {
+        sc.template ready<true>(lane);
+        sc.load(min(kt + 4, (ke - 1) & ~3));
+      } else {
+        sc.shift();
+      }
       __builtin_amdgcn_sched_barrier(0);
       if (!TAIL)
         load(first ? kt + 1 : kt + 2,
@@ -463,12 +459,12 @@ __global__ void __launch_bounds__(kFNT) gemm_fp8_kernel(const GemmParams p, cons
 #pragma unroll
       for (int j = 0; j < FB / 2; ++j) fb[j] = fp8_frag(sB + bst, boff + 2048 * j);
       __builtin_amdgcn_sched_barrier(0);
-      // B(kt + 1) has landed (only the second group has older operand loads in flight here), and
-      // this wave's reads are done. In the last k-tile neither group has a load in flight from
+      // B(kt + 1) has landed (only the second group has older operand loads in flight here; the
+      // first would wait for the scales just requested), and this wave's reads are done. In the last k-tile neither group has a load in flight from
       // here on, so that the first group's epilogue may stage through LDS.
-      if (!TAIL) __builtin_amdgcn_s_waitcnt(wait_vmcnt(kFIns));
+      if (!TAIL && !first) __builtin_amdgcn_s_waitcnt(wait_vmcnt(kFIns));
       if (TAIL && !first) __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
-      if (SCALE == kScaleE8M0 && (kt & 3) == 0) sc.ready(lane);
+      if constexpr (SCALE == kScaleF32) sc.template ready<false>(lane);
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
