@@ -78,7 +78,7 @@ __device__ __forceinline__ void score_finish(const ScoreOut& o, long row, const 
 // joined by score_join_kernel.
 //
 // The k largest of a part, by (logit, lowest id first). The part's groups (the threads, or for
-// k up to 16 the 64 groups of four threads) give their largest logits; a T that at least k of
+// k up to 32 the 64 groups of four threads) give their largest logits; a T that at least k of
 // those reach is at most the part's k-th largest logit, so every logit >= T is a candidate, and
 // in ordinary data few others are. T is the k-th largest group cut to 16 bits of its key (an
 // order-preserving integer of the logit), found bit by bit with ballots over the groups, in
@@ -91,11 +91,13 @@ __device__ __forceinline__ void score_finish(const ScoreOut& o, long row, const 
 //
 // Few registers (eight workgroups on a compute unit), no scratch and few barriers are what it is
 // built for: 4096 x 32768 with the top 20 took 128 us while every logit's 64-bit key was formed
-// and compared in 121 registers, 125 with 112 bytes of scratch for a call, 82 inlined.
+// and compared in 121 registers, 125 with 112 bytes of scratch for a call, 83 inlined, 78 with the
+// 64 groups for k up to 32 (a quarter of the comparisons for a few more candidates: k = 32 90.6 ->
+// 87.7, k = 48 99.4 -> 104.4). Of that the sums take 67 (no top, 4.0 TB/s).
 constexpr int kScoreGroups = 64;
 constexpr int kMaxTopK = kScoreGroups;
 constexpr int kScoreCandidates = 2048, kScoreWaveCandidates = kScoreCandidates / 4;
-constexpr int kScoreFewK = 16;
+constexpr int kScoreFewK = 32;
 constexpr int kMaxScoreParts = 64;
 
 // Ascending in the logit's order; -0 as 0. The lowest key, 0, is no logit's (-inf has
