@@ -265,6 +265,24 @@ def test_linear_and_its_gradients(m, n, k, weight_dtype, scale_dtype):
     assert folded.shape == (1, m, n) and torch.equal(folded[0], y)
 
 
+@pytest.mark.parametrize("scale_dtype", SCALES)
+def test_operands_past_two_gib(scale_dtype):
+    """More than 2^31 elements: the last rows are quantized and multiplied as on their own."""
+    fp8 = _fp8()
+    rows, k = 2 ** 31 // 2048 + 5000, 2048
+    x = torch.empty((rows, k), dtype=BF16, device="cuda").normal_()
+    b, sb = fp8.quantize_weight(torch.randn((24, k), device="cuda"), scale_dtype)[:2]
+    q, scale = fp8.quantize_rows(x, scale_dtype)
+    tail = slice(rows - 5000, rows)
+    own_q, own_scale = fp8.quantize_rows(x[tail], scale_dtype)
+    assert torch.equal(q[tail].view(torch.uint8), own_q.view(torch.uint8))
+    assert np.array_equal(values(scale[tail]), values(own_scale))
+    got = fp8.fp8_mm(q, scale, b, sb)[tail]
+    _check(got[-300:], own_q[-300:], own_scale[-300:], b, sb)
+    qt, scale_t = fp8.quantize_columns(x.T, scale_dtype)  # rows of x.T: columns past 2^31
+    assert torch.equal(qt[tail].view(torch.uint8), own_q.view(torch.uint8))
+
+
 def test_products_in_a_captured_graph():
     """Quantization and both products replay with new inputs, and with eager work between."""
     fp8 = _fp8()

@@ -316,6 +316,69 @@ def test_head_operands_of_other_strides_and_bad_tokens():
     assert not bool(torch.isnan(got[1]).any())
 
 
+def test_head_of_a_large_vocabulary():
+    """More than 2^31 logits in five default chunks: scores and gradients of every row, against
+    64 bits 200 rows at a time. `extra`: the logits' own error, FP32 sums of d products, and 64
+    more additions per sum than _bounds counts. A gradient's FP32 sum of n terms is off by at
+    most n U of the terms' magnitudes."""
+    ts = _scores()
+    rows, d, vocab = 4100, 8, 524288
+    gen = torch.Generator().manual_seed(3)
+    hidden = torch.randn((rows, d), generator=gen).to(BF16).cuda().requires_grad_(True)
+    weight = torch.randn((vocab, d), generator=gen).to(BF16).cuda().requires_grad_(True)
+    tokens = torch.randint(0, vocab, (rows,), generator=gen).cuda()
+    tokens[5] = IGNORED
+    up_g, up_h = torch.randn(rows, generator=gen).cuda(), torch.randn(rows, generator=gen).cuda()
+    logprob, entropy = ts.linear_token_scores(hidden, weight, tokens)
+    dh, dw = torch.autograd.grad([logprob, entropy], [hidden, weight], [up_g, up_h])
+    logprob, entropy = logprob.detach(), entropy.detach()
+    wide, want_dw, dw_tol = weight.detach().double(), 0.0, 0.0
+    for a in range(0, rows, 200):
+        part = slice(a, a + 200)
+        x = hidden.detach()[part].double()
+        logits = x @ wide.T
+        extra = 2 * (d + 2) * U * float((x.abs() @ wide.abs().T).max()) + 64 * U
+        score_tol, entropy_tol, rel = _bounds(logits, 1.0, extra)
+        logp = torch.log_softmax(logits, -1)
+        p, valid, index = logp.exp(), tokens[part] != IGNORED, tokens[part].clamp_min(0)[:, None]
+        want_e = -(p * logp).sum(-1)
+        assert float((logprob[part] - logp.gather(1, index)[:, 0] * valid).abs().max()) <= score_tol
+        assert float((entropy[part] - want_e).abs().max()) <= entropy_tol
+        g, h = (up_g[part].double() * valid)[:, None], up_h[part].double()[:, None]
+        dl = -p * (g + h * (logp + want_e[:, None]))
+        dl.scatter_add_(1, index, g)
+        err = p * (g.abs() + h.abs() * (logp.abs() + want_e[:, None])) * (rel + score_tol + 16 * U)
+        err += p * h.abs() * (score_tol + entropy_tol)
+        err += (dl.abs() + err) * 2.0 ** -8
+        err.scatter_add_(1, index, g.abs() * (4 * U + 2.0 ** -8))
+        want = dl @ wide
+        tol = err @ wide.abs() + vocab * U * ((dl.abs() + err) @ wide.abs())
+        assert bool(((dh[part].double() - want).abs() <= tol + (want.abs() + tol) * 2.0 ** -8).all())
+        want_dw = want_dw + dl.T @ x
+        dw_tol = dw_tol + err.T @ x.abs() + rows * U * ((dl.abs() + err).T @ x.abs())
+    tol = dw_tol + (want_dw.abs() + dw_tol) * 2.0 ** -8 + 1e-30
+    assert bool(((dw.double() - want_dw).abs() <= tol).all())
+
+
+def test_logits_past_two_gib():
+    """More than 2^31 logits: the last rows are scored, and their gradient written, as on their
+    own."""
+    ts = _scores()
+    rows, vocab = 4100, 524288
+    x = torch.empty((rows, vocab), dtype=BF16, device="cuda").normal_().requires_grad_(True)
+    tokens = torch.arange(rows, device="cuda") * 127
+    g, h = torch.randn(rows, device="cuda"), torch.randn(rows, device="cuda")
+    got = ts.token_scores(x, tokens, 5)
+    dx, = torch.autograd.grad([got.logprob, got.entropy], [x], [g, h])
+    tail = slice(rows - 600, rows)  # as many rows as take the same parts
+    own = x.detach()[tail].clone().requires_grad_(True)
+    alone = ts.token_scores(own, tokens[tail], 5)
+    want, = torch.autograd.grad([alone.logprob, alone.entropy], [own], [g[tail], h[tail]])
+    for a, b in zip(got, alone):
+        assert torch.equal(a[tail], b)
+    assert torch.equal(dx[tail], want)
+
+
 def test_scores_in_a_captured_graph():
     """Forward and backward from logits, and the head's forward, replayed with new inputs and
     eager work between the replays."""
