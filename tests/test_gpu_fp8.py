@@ -223,6 +223,21 @@ def test_product_of_other_layouts(scale_dtype):
     assert bool((big == 7.0).all())
 
 
+@pytest.mark.parametrize("m,n,k", [(3300, 2700, 1000), (3717, 4948, 688), (1380, 3172, 128), (1020, 3932, 2864),
+                                   (286, 6764, 128), (285, 3444, 4368), (34, 36, 160), (17, 2004, 2064)])
+def test_output_inside_a_wider_buffer(m, n, k):
+    """Aligned columns of a larger matrix, half of a 16-byte piece at the end: every kernel leaves
+    the columns beside them and the rows behind them as they were."""
+    fp8 = _fp8()
+    a, sa, b, sb = _operands(m, n, k, E8M0, False, True, m + n)
+    want = fp8.fp8_mm(a, sa, b, sb)
+    big = torch.full((m + 9, n + 24), 7.0, dtype=BF16, device="cuda")
+    out = big[1:m + 1, 8:8 + n]
+    assert fp8.fp8_mm(a, sa, b, sb, out=out).data_ptr() == out.data_ptr() and torch.equal(out, want)
+    out.fill_(7.0)
+    assert bool((big == 7.0).all())
+
+
 def test_scaled_nan_reaches_its_row_only():
     fp8 = _fp8()
     x = _matrix(40, 256, BF16, 1, std=0.1)
