@@ -429,7 +429,8 @@ int ws_fp8_mm(const void* a, int64_t lda, const void* scale_a, int64_t ld_scale_
  * For each row of logits l (times inv_temperature > 0): logprob = l[token] - lse, entropy =
  * lse - sum p l, lse = log sum e^l, FP32. A token of -100 has logprob 0 and takes no gradient;
  * any other token outside [0, vocab) gets NaN. Logits of -inf have probability 0; a row of
- * nothing else gets NaN.
+ * nothing else gets NaN. Finite logits of any size have scores (a mask of the type's lowest value
+ * among them): only their distances to the row's largest are scaled.
  */
 
 /* From logits [rows, vocab] (row stride ld, BF16 or, with f32, FP32; any alignment of their
@@ -444,7 +445,8 @@ int ws_token_scores(const void* logits, int64_t ld, int f32, const int64_t* toke
                     void* stream);
 /* dlogits [rows, vocab] (row stride ld_out, the logits' type; may be the logits) of
  * sum(dlogprob logprob + dentropy entropy); either of the two may be null (zero). lse and
- * entropy are the forward's. A row whose two upstream gradients are zero gets zeros. */
+ * entropy are the forward's; a row with |lse| of 256 or more is summed again, in distances. A row
+ * whose two upstream gradients are zero gets zeros. */
 int ws_token_scores_backward(const void* logits, int64_t ld, int f32, const int64_t* tokens,
                              int64_t rows, int64_t vocab, float inv_temperature, const float* lse,
                              const float* entropy, const float* dlogprob, const float* dentropy,
@@ -461,7 +463,8 @@ int ws_linear_token_scores(const void* hidden, int64_t ld_hidden, const void* we
  * [vocab, d] FP32 or, with dweight_bf16 (one chunk, ld_dweight = d), BF16 (written), each
  * nullable. The logits are recomputed chunk_rows rows at a time, and their gradient, rounded to
  * BF16, feeds the two products. weight_t: null, or the weight transposed ([d, vocab], vocab a
- * multiple of 8). `workspace`: 256-byte aligned. */
+ * multiple of 8). Probabilities are e^(l - lse) with lse in FP32, off by up to 2^-24 |lse| as the
+ * FP32 logits themselves are. `workspace`: 256-byte aligned. */
 int64_t ws_linear_token_scores_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d,
                                                         int64_t chunk_rows);
 int ws_linear_token_scores_backward(const void* hidden, int64_t ld_hidden, const void* weight,

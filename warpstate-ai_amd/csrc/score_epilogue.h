@@ -7,9 +7,8 @@
 
 namespace ws {
 
-// Per row, over this wave's FB * 16 columns: the maximum m of the scaled logits (in units of log
-// 2), S and W (scores.h), one partial per (row, wave column block), and the
-// token's logit. The four lanes l, l^16, l^32, l^48 share a row.
+// Per row, over this wave's FB * 16 columns: the largest logit m, S and W (scores.h), one partial
+// per (row, wave column block), and the token's logit. The four lanes l, l^16, l^32, l^48 share a row.
 struct FEpiScoreStats {
   template <int FA, int FB>
   __device__ __forceinline__ static void run(const GemmParams& p, Acc16<FA, FB>& acc, int m_base,
@@ -27,17 +26,21 @@ struct FEpiScoreStats {
       // The row's token as a column of this wave's (-1 if outside).
       const long trel = (mok ? p.targets[m] : -1) - n_base;
       const int t = trel >= 0 && trel < FB * 16 && trel < ncols ? (int)trel : -1;
+      // Columns past the vocabulary add e^-inf = 0. (A branch of the whole wave: as selections,
+      // in every wave, they spilled registers and cost 8000 x 32768 x 1280 6 % of its time.)
+      if (ncols < FB * 16) {
+        asm volatile("");
+#pragma unroll
+        for (int j = 0; j < FB; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * j + c0 + e >= ncols) acc.v[i][j][e] = -INFINITY;
+      }
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < FB; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float l = acc.v[i][j][e] * scale;
-          // Columns past the vocabulary (a wave-uniform test first) add e^-inf = 0.
-          if (ncols < FB * 16 && 16 * j + c0 + e >= ncols) l = -INFINITY;
-          acc.v[i][j][e] = l;
-          mx = fmaxf(mx, l);
-        }
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, acc.v[i][j][e]);
       // The token's logit only in the waves where some row's token falls in these columns.
       if (__builtin_amdgcn_ballot_w64(t >= 0) != 0) {
         float tv = 0.0f;
@@ -54,7 +57,7 @@ struct FEpiScoreStats {
 #pragma unroll
       for (int j = 0; j < FB; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) score_add(st, acc.v[i][j][e] - ref);
+        for (int e = 0; e < 4; ++e) score_add(st, (acc.v[i][j][e] - ref) * scale);
       st.s += __shfl_xor(st.s, 16, kWave);
       st.s += __shfl_xor(st.s, 32, kWave);
       st.w += __shfl_xor(st.w, 16, kWave);
@@ -98,7 +101,7 @@ struct FEpiScoreGrad {
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[e] = score_grad(acc.v[i][j][e] * scale, c);
+          v[e] = score_grad(acc.v[i][j][e] * scale - c[0], c);
           if (some && 16 * j + c0 + e == t) v[e] += c[3];
           if (none || (ncols < FB * 16 && 16 * j + c0 + e >= ncols)) v[e] = 0.0f;
         }

@@ -19,8 +19,11 @@ namespace ws {
 
 constexpr long kIgnored = -100;
 
-// Logits, maxima and W are held in units of log 2 (l log2 e), so that e^l is the hardware's
-// base-2 exponential without a multiplication.
+// Logits and their maxima m are held as they are given: only a distance l - m, at most 0, is
+// scaled, by log2 e / temperature, so that e^(l - m) is the hardware's base-2 exponential and W is in
+// units of log 2. (Scaled first, finite logits above 2.36e38, such as a mask of the type's
+// lowest value, would overflow, and at 1e10 the scaled maximum's own rounding is hundreds.) A
+// distance beyond FP32's range is -inf, which adds nothing.
 struct ScoreStats {
   float m, s, w;
 };
@@ -34,11 +37,11 @@ __device__ __forceinline__ void score_add(ScoreStats& a, float y) {
   a.s += e;
   a.w = __builtin_fmaf(e, fmaxf(y, -1e30f), a.w);
 }
-__device__ __forceinline__ ScoreStats score_join(const ScoreStats& a, const ScoreStats& b) {
+__device__ __forceinline__ ScoreStats score_join(const ScoreStats& a, const ScoreStats& b, float scale) {
   ScoreStats r;
   r.m = fmaxf(a.m, b.m);
   const float ref = score_ref(r.m);
-  const float ya = a.m - ref, yb = b.m - ref;
+  const float ya = (a.m - ref) * scale, yb = (b.m - ref) * scale;
   const float ea = exp2_hw(ya), eb = exp2_hw(yb);
   r.s = __builtin_fmaf(ea, a.s, eb * b.s);
   // (An empty part has m = -inf, s = w = 0.)
@@ -46,28 +49,31 @@ __device__ __forceinline__ ScoreStats score_join(const ScoreStats& a, const Scor
   return r;
 }
 // Joins the values of `lanes` (a power of two) neighbouring lanes.
-__device__ __forceinline__ ScoreStats score_join_lanes(ScoreStats v, int lanes) {
+__device__ __forceinline__ ScoreStats score_join_lanes(ScoreStats v, int lanes, float scale) {
   for (int off = lanes / 2; off >= 1; off >>= 1) {
     const ScoreStats o = {__shfl_xor(v.m, off, kWave), __shfl_xor(v.s, off, kWave), __shfl_xor(v.w, off, kWave)};
-    v = score_join(v, o);
+    v = score_join(v, o, scale);
   }
   return v;
 }
 
-// Outputs of a row, in natural units. `target` is its token's logit in units of log 2 (read
-// only where the token is valid).
+// Outputs of a row. `target` is its token's logit (read only where the token is valid).
 struct ScoreOut {
   float *lse, *logprob, *entropy;
 };
-// log2 S of finished sums: a logit y has log2 p = (y - m) - log2 S.
+// log2 S of finished sums.
 __device__ __forceinline__ float score_log(const ScoreStats& st) { return __builtin_amdgcn_logf(st.s); }
+// A logit's log probability. The largest logit's own term makes S at least 1, so it is at most 0.
+__device__ __forceinline__ float score_logprob(float l, float m, float log_s, float inv_t) {
+  return (l - m) * inv_t - log_s * kLn2;
+}
 __device__ __forceinline__ void score_finish(const ScoreOut& o, long row, const ScoreStats& st, long token,
-                                             long vocab, float target) {
+                                             long vocab, float target, float inv_t) {
   const float log_s = score_log(st);
-  o.lse[row] = (st.m + log_s) * kLn2;
+  o.lse[row] = st.m * inv_t + log_s * kLn2;
   o.entropy[row] = (log_s - st.w / st.s) * kLn2;
   o.logprob[row] = token == kIgnored               ? 0.0f
-                   : token >= 0 && token < vocab ? ((target - st.m) - log_s) * kLn2
+                   : token >= 0 && token < vocab ? score_logprob(target, st.m, log_s, inv_t)
                                                    : NAN;
 }
 
@@ -93,7 +99,8 @@ __device__ __forceinline__ void score_finish(const ScoreOut& o, long row, const 
 // built for: 4096 x 32768 with the top 20 took 128 us while every logit's 64-bit key was formed
 // and compared in 121 registers, 125 with 112 bytes of scratch for a call, 83 inlined, 78 with the
 // 64 groups for k up to 32 (a quarter of the comparisons for a few more candidates: k = 32 90.6 ->
-// 87.7, k = 48 99.4 -> 104.4). Of that the sums take 67 (no top, 4.0 TB/s).
+// 87.7, k = 48 99.4 -> 104.4), 80 with distances taken before they are scaled. Of that the sums take
+// 67 (no top, 4.0 TB/s).
 constexpr int kScoreGroups = 64;
 constexpr int kMaxTopK = kScoreGroups;
 constexpr int kScoreCandidates = 2048, kScoreWaveCandidates = kScoreCandidates / 4;
@@ -166,8 +173,7 @@ struct ScoreParams {
 
 __device__ __forceinline__ void score_top(const ScoreParams& p, long row, int i, unsigned long key,
                                           const ScoreStats& st, float log_s) {
-  const float y = score_unkey((unsigned)(key >> 32)) * p.scale;
-  p.top_logprobs[row * p.top_k + i] = ((y - st.m) - log_s) * kLn2;
+  p.top_logprobs[row * p.top_k + i] = score_logprob(score_unkey((unsigned)(key >> 32)), st.m, log_s, p.inv_t);
   p.top_ids[row * p.top_k + i] = (long)(unsigned)~(unsigned)key;
 }
 
@@ -275,7 +281,7 @@ static __global__ void __launch_bounds__(256) score_rows_kernel(const ScoreParam
   const f32x4_t group = *reinterpret_cast<const f32x4_t*>(&groups[4 * lane]);
   const float four = fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3]));
   ScoreStats st;
-  st.m = wave_max(four) * p.scale;
+  st.m = wave_max(four);
   st.s = st.w = 0.0f;
   if constexpr (TOPK) {
     unsigned T = 0;
@@ -320,7 +326,7 @@ static __global__ void __launch_bounds__(256) score_rows_kernel(const ScoreParam
   }
   const float ref = score_ref(st.m);
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) score_add(st, __builtin_fmaf(x[i], p.scale, -ref));
+  for (int i = 0; i < EPT; ++i) score_add(st, (x[i] - ref) * p.scale);
   st.s = wave_sum(st.s);
   st.w = wave_sum(st.w);
   if (lane == 0) {
@@ -365,8 +371,8 @@ static __global__ void __launch_bounds__(256) score_rows_kernel(const ScoreParam
   if (t == 0) {
     const long token = p.tokens[row];
     const bool valid = token >= 0 && token < p.vocab;
-    score_finish(p.out, row, st, token, p.vocab,
-                 valid ? load_logit<F32>(p.logits, row * p.ld + token) * p.scale : 0.0f);
+    score_finish(p.out, row, st, token, p.vocab, valid ? load_logit<F32>(p.logits, row * p.ld + token) : 0.0f,
+                 p.inv_t);
   }
   if constexpr (TOPK) {
     if (t < p.top_k) score_top(p, row, t, sh.best[t], st, score_log(st));
@@ -399,15 +405,14 @@ static __global__ void __launch_bounds__(kScoreJoinThreads) score_join_kernel(co
   const long token = p.tokens[at];
   const f32x4_t part = p.stats[at * p.parts + min(t, p.parts - 1)];
   const unsigned long key = k ? p.keys[at * total + min(t, total - 1)] : 0;
-  const float target =
-      token >= 0 && token < p.vocab ? load_logit<F32>(p.logits, at * p.ld + token) * p.scale : 0.0f;
+  const float target = token >= 0 && token < p.vocab ? load_logit<F32>(p.logits, at * p.ld + token) : 0.0f;
   if (t < total) keys[t] = key;
   for (int i = t + threads; i < total; i += threads) keys[i] = p.keys[at * total + i];
   ScoreStats st = {-INFINITY, 0.0f, 0.0f};
   if (t < p.parts) st = ScoreStats{part[0], part[1], part[2]};
-  st = score_join_lanes(st, lanes);
+  st = score_join_lanes(st, lanes, p.scale);
   if (ok && t == 0) {
-    score_finish(p.out, row, st, token, p.vocab, target);
+    score_finish(p.out, row, st, token, p.vocab, target, p.inv_t);
     joined[slot][0] = st.m;
     joined[slot][1] = score_log(st);
   }
@@ -476,61 +481,107 @@ static __global__ void __launch_bounds__(256) score_coef_kernel(const long* toke
   coef[row] = f32x4_t{lse[row], h == 0.0f ? inv_t * g : inv_t * (g + h * entropy[row]), inv_t * h, inv_t * g};
 }
 
-// One gradient value from a scaled logit. p = 0 gives 0 (log p is -inf there).
-__device__ __forceinline__ float score_grad(float l, const f32x4_t& c) {
-  const float logp = l - c[0], pr = exp_e(logp);
+// One gradient value from a log probability. p = 0 gives 0 (log p may be -inf there).
+__device__ __forceinline__ float score_grad(float logp, const f32x4_t& c) {
+  const float pr = exp_e(logp);
   return pr == 0.0f ? 0.0f : -pr * (c[1] + c[2] * logp);
 }
 
+// A probability taken from an lse of up to this size is off by at most half a step of it, 2^-17.
+// Beyond, where the step comes to hide the sum of the row's distances (and with a mask of the
+// type's lowest value all of it), a row's gradient sums the row again (4096 x 32768 BF16 logits
+// 132 -> 596 us if every row is such, 1000 x 10883 38 -> 41).
+constexpr float kLseReach = 256.0f;
+
+// (m, S) of a whole row, by all of a workgroup's 256 threads (W is left out).
+template <bool F32>
+__device__ __forceinline__ ScoreStats score_row_sum(const ScoreParams& p, long row) {
+  const int t = threadIdx.x;
+  __shared__ float red[2][kScoreWaves];
+  ScoreStats st = {-INFINITY, 0.0f, 0.0f};
+#pragma unroll 1
+  for (int id = 8 * t; id < p.vocab; id += 2048) {
+    float x[8];
+    load_logits8<F32>(p.logits, row * p.ld + id, (long)p.vocab - id, x);
+    ScoreStats piece = {x[0], 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 1; e < 8; ++e) piece.m = fmaxf(piece.m, x[e]);
+    const float ref = score_ref(piece.m);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) piece.s += exp2_hw((x[e] - ref) * p.scale);
+    st = score_join(st, piece, p.scale);
+  }
+  st = score_join_lanes(st, kWave, p.scale);
+  if ((t & 63) == 0) {
+    red[0][t >> 6] = st.m;
+    red[1][t >> 6] = st.s;
+  }
+  __syncthreads();
+  st = ScoreStats{red[0][0], red[1][0], 0.0f};
+#pragma unroll
+  for (int w = 1; w < kScoreWaves; ++w) st = score_join(st, ScoreStats{red[0][w], red[1][w], 0.0f}, p.scale);
+  return st;
+}
+
+// A workgroup takes every `segments`-th piece of 2048 logits of a row: one piece, or, where the
+// gradient goes over the logits, all of them (no other workgroup may have written what it sums).
 template <bool F32>
 static __global__ void __launch_bounds__(256) score_grad_kernel(const ScoreParams p, const float* dlogprob,
                                                                 const float* dentropy, void* out, long ld_out,
                                                                 int segments) {
   const long row = blockIdx.x / segments;
-  const int id0 = (int)(blockIdx.x % segments) * 2048 + 8 * threadIdx.x;
-  if (id0 >= p.vocab) return;
   const long token = p.tokens[row];
   const bool valid = token >= 0 && token < p.vocab;
   const float g = dlogprob && token != kIgnored ? (valid ? dlogprob[row] : NAN) : 0.0f;
   const float h = dentropy ? dentropy[row] : 0.0f;
   // A row without upstream gradient has none, whatever its logits.
   const bool none = g == 0.0f && h == 0.0f;
-  const f32x4_t c = {p.out.lse[row], h == 0.0f ? p.inv_t * g : p.inv_t * (g + h * p.out.entropy[row]),
-                     p.inv_t * h, p.inv_t * g};
-  float x[8];
-  const long left = (long)p.vocab - id0;
-  if (none) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-  } else {
-    load_logits8<F32>(p.logits, row * p.ld + id0, left, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = score_grad(x[e] * p.inv_t, c);
-      if (id0 + e == token) x[e] += c[3];
-    }
+  // log p = (l - m) / temperature - log_s.
+  float m = 0.0f, log_s = p.out.lse[row];
+  if (!none && !(fabsf(log_s) < kLseReach)) {  // (the same for the whole workgroup)
+    const ScoreStats st = score_row_sum<F32>(p, row);
+    m = st.m;
+    log_s = score_log(st) * kLn2;
   }
-  const long at = row * ld_out + id0;
-  if constexpr (F32) {
-    float* o = static_cast<float*>(out) + at;
-    if (left >= 8) {
-      __builtin_memcpy(o, x, 32);
-    } else {
+  const f32x4_t c = {0.0f, h == 0.0f ? p.inv_t * g : p.inv_t * (g + h * p.out.entropy[row]), p.inv_t * h,
+                     p.inv_t * g};
+#pragma unroll 1
+  for (long id0 = blockIdx.x % segments * 2048L + 8 * threadIdx.x; id0 < p.vocab; id0 += segments * 2048L) {
+    float x[8];
+    const long left = p.vocab - id0;
+    if (none) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) o[e] = x[e];
+      for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+    } else {
+      load_logits8<F32>(p.logits, row * p.ld + id0, left, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = score_grad((x[e] - m) * p.inv_t - log_s, c);
+        if (id0 + e == token) x[e] += c[3];
+      }
     }
-  } else {
-    auto* o = static_cast<unsigned short*>(out) + at;
-    u32x4_t v;
+    const long at = row * ld_out + id0;
+    if constexpr (F32) {
+      float* o = static_cast<float*>(out) + at;
+      if (left >= 8) {
+        __builtin_memcpy(o, x, 32);
+      } else {
 #pragma unroll
-    for (int d = 0; d < 4; ++d) v[d] = pack_bf16x2(x[2 * d], x[2 * d + 1]);
-    if (left >= 8) {
-      __builtin_memcpy(o, &v, 16);
+        for (int e = 0; e < 8; ++e)
+          if (e < left) o[e] = x[e];
+      }
     } else {
+      auto* o = static_cast<unsigned short*>(out) + at;
+      u32x4_t v;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) o[e] = (unsigned short)(v[e >> 1] >> (16 * (e & 1)));
+      for (int d = 0; d < 4; ++d) v[d] = pack_bf16x2(x[2 * d], x[2 * d + 1]);
+      if (left >= 8) {
+        __builtin_memcpy(o, &v, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < left) o[e] = (unsigned short)(v[e >> 1] >> (16 * (e & 1)));
+      }
     }
   }
 }
@@ -540,19 +591,20 @@ static __global__ void __launch_bounds__(256) score_grad_kernel(const ScoreParam
 static __global__ void __launch_bounds__(256) score_combine_kernel(const float* pm, const float* ps,
                                                                    const float* pw, int parts,
                                                                    const float* target, const long* tokens,
-                                                                   ScoreOut out, int rows, int vocab) {
+                                                                   ScoreOut out, int rows, int vocab,
+                                                                   float inv_t) {
   const int lane = threadIdx.x & 63;
   const long row = blockIdx.x * 4L + (threadIdx.x >> 6);
   if (row >= rows) return;
   ScoreStats st = {-INFINITY, 0.0f, 0.0f};
   for (int q = lane; q < parts; q += 64) {
     const long i = row * parts + q;
-    st = score_join(st, ScoreStats{pm[i], ps[i], pw[i]});
+    st = score_join(st, ScoreStats{pm[i], ps[i], pw[i]}, inv_t * kLog2e);
   }
-  st = score_join_lanes(st, kWave);
+  st = score_join_lanes(st, kWave, inv_t * kLog2e);
   if (lane == 0) {
     const long token = tokens[row];
-    score_finish(out, row, st, token, vocab, token >= 0 && token < vocab ? target[row] : 0.0f);
+    score_finish(out, row, st, token, vocab, token >= 0 && token < vocab ? target[row] : 0.0f, inv_t);
   }
 }
 

@@ -107,9 +107,14 @@ extern "C" int ws_token_scores_backward(const void* logits, int64_t ld, int f32,
   p.ld = ld;
   p.rows = (int)rows; p.vocab = (int)vocab;
   p.inv_t = inv_temperature;
+  p.scale = inv_temperature * kLog2e;
   p.tokens = reinterpret_cast<const long*>(tokens);
   p.out = ScoreOut{const_cast<float*>(lse), nullptr, const_cast<float*>(entropy)};
-  const int segments = cdiv(vocab, 2048);
+  const auto* x = static_cast<const char*>(logits);
+  const auto* dx = static_cast<const char*>(dlogits);
+  const long size = f32 ? 4 : 2, span = ((rows - 1) * ld + vocab) * size, dspan = ((rows - 1) * ld_out + vocab) * size;
+  const bool in_place = x < dx + dspan && dx < x + span;
+  const int segments = in_place ? 1 : cdiv(vocab, 2048);
   const dim3 grid((unsigned)(rows * segments));
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (f32)
@@ -190,7 +195,7 @@ extern "C" int ws_linear_token_scores(const void* hidden, int64_t ld_hidden, con
   if (int rc = run_head<FEpiScoreStats>(p, tile, s)) return rc;
   hipLaunchKernelGGL(score_combine_kernel, dim3(cdiv(rows, 4)), dim3(256), 0, s, p.part_max, p.part_sum,
                      p.part_wsum, p.parts_per_row, p.tgt_logit, p.targets, ScoreOut{lse, logprob, entropy},
-                     (int)rows, (int)vocab);
+                     (int)rows, (int)vocab, inv_temperature);
   return hip_check(hipGetLastError(), "token score combine launch");
 }
 

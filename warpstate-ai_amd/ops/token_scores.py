@@ -126,7 +126,9 @@ def token_scores(logits: Tensor, tokens: Tensor, top_k: int = 0,
     One read of the logits forward, one read and one write backward. A row of -inf only has no
     distribution: its scores are NaN, and its gradient, unless both its upstream gradients are
     zero, whose rows get zeros. NaN or +inf logits make their row's scores NaN and the order of
-    its likeliest tokens unspecified. Vocabularies up to 524288. Under torch.compile it runs
+    its likeliest tokens unspecified. Finite logits have finite scores whatever their size, as
+    far as FP32 holds a distance over the temperature: a row masked with its type's lowest value
+    throughout is uniform. Vocabularies up to 524288. Under torch.compile it runs
     eagerly (a graph break)."""
     # (Not a decorator of this function, which would add its own calls to each eager one.)
     scores = _eager_token_scores if torch.compiler.is_compiling() else _scores
@@ -231,7 +233,8 @@ def linear_token_scores(hidden: Tensor, weight: Tensor, tokens: Tensor, temperat
     The logits are FP32 and never leave the registers. The backward recomputes them
     ``chunk_rows`` rows at a time (None: as many as 1 GiB of BF16 gradients holds); their
     gradient is rounded to BF16 once for the two products, whose sums are FP32, and so is the
-    weight's gradient over all chunks; both gradients come in their operand's type. Under
+    weight's gradient over all chunks; both gradients come in their operand's type. Its
+    probabilities are off by up to 2^-24 of the row's log-sum-exp, as the FP32 logits are. Under
     torch.compile it runs eagerly (a graph break)."""
     if not (hidden.is_cuda and weight.is_cuda):
         raise ValueError("Token scores require CUDA tensors")
