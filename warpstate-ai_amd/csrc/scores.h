@@ -466,8 +466,15 @@ static __global__ void __launch_bounds__(kScoreJoinThreads) score_join_kernel(co
 }
 
 // ---------------------------------------------------------------------------------------
+// A log probability's upstream gradient: none for an ignored token; of a token that has no score,
+// NaN unless it is zero (a row outside the loss).
+__device__ __forceinline__ float score_upstream(const float* dlogprob, long row, long token, bool valid) {
+  const float g = dlogprob && token != kIgnored ? dlogprob[row] : 0.0f;
+  return valid || g == 0.0f ? g : NAN;
+}
+
 // Coefficients of a row's gradient, dl_j / temperature = [j = t] c[3] - p_j (c[1] + c[2] log p_j)
-// with c[0] = lse. c[1] is NaN for a token that has no score.
+// with c[0] = lse. c[1] is NaN for a token that has no score but a gradient.
 static __global__ void __launch_bounds__(256) score_coef_kernel(const long* tokens, const float* lse,
                                                                 const float* entropy, const float* dlogprob,
                                                                 const float* dentropy, float inv_t, int rows,
@@ -476,7 +483,7 @@ static __global__ void __launch_bounds__(256) score_coef_kernel(const long* toke
   if (row >= rows) return;
   const long token = tokens[row];
   const bool valid = token >= 0 && token < vocab;
-  const float g = dlogprob && token != kIgnored ? (valid ? dlogprob[row] : NAN) : 0.0f;
+  const float g = score_upstream(dlogprob, row, token, valid);
   const float h = dentropy ? dentropy[row] : 0.0f;
   coef[row] = f32x4_t{lse[row], h == 0.0f ? inv_t * g : inv_t * (g + h * entropy[row]), inv_t * h, inv_t * g};
 }
@@ -532,7 +539,7 @@ static __global__ void __launch_bounds__(256) score_grad_kernel(const ScoreParam
   const long row = blockIdx.x / segments;
   const long token = p.tokens[row];
   const bool valid = token >= 0 && token < p.vocab;
-  const float g = dlogprob && token != kIgnored ? (valid ? dlogprob[row] : NAN) : 0.0f;
+  const float g = score_upstream(dlogprob, row, token, valid);
   const float h = dentropy ? dentropy[row] : 0.0f;
   // A row without upstream gradient has none, whatever its logits.
   const bool none = g == 0.0f && h == 0.0f;

@@ -15,8 +15,9 @@ logits over the temperature:
   training does), and no [rows, vocab] tensor is written but one chunk of BF16 logit gradients.
 
 A token of -100 is ignored: its log probability is 0 and passes no gradient. Its row still has
-an entropy, whose gradient it passes. Any other token outside the vocabulary gets NaN (a
-gradient of NaN if its log probability has one). Logits of -inf have probability 0.
+an entropy, whose gradient it passes. Any other token outside the vocabulary gets NaN (and a
+gradient of NaN, unless its log probability's upstream gradient is zero). Logits of -inf have
+probability 0.
 """
 
 from __future__ import annotations
