@@ -426,11 +426,11 @@ int ws_fp8_mm(const void* a, int64_t lda, const void* scale_a, int64_t ld_scale_
 
 /* --- token scores ---------------------------------------------------------------------
  *
- * For each row of logits l (times inv_temperature > 0): logprob = l[token] - lse, entropy =
- * lse - sum p l, lse = log sum e^l, FP32. A token of -100 has logprob 0 and takes no gradient;
- * any other token outside [0, vocab) gets NaN. Logits of -inf have probability 0; a row of
- * nothing else gets NaN. Finite logits of any size have scores (a mask of the type's lowest value
- * among them): only their distances to the row's largest are scaled.
+ * For each row of logits l (times inv_temperature, 2^-126 to 2.3e38): logprob = l[token] - lse,
+ * entropy = lse - sum p l, lse = log sum e^l, FP32. A token of -100 has logprob 0 and takes no
+ * gradient; any other token outside [0, vocab) gets NaN. Logits of -inf have probability 0; a row
+ * of nothing else gets NaN. Finite logits of any size have scores (a mask of the type's lowest
+ * value among them): only their distances to the row's largest are scaled.
  */
 
 /* From logits [rows, vocab] (row stride ld, BF16 or, with f32, FP32; any alignment of their

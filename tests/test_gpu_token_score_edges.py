@@ -1,5 +1,5 @@
 """Token scores at the edges of what their documentation allows: tokens without a score under
-masked losses, the smallest temperatures (GPU)."""
+masked losses, the smallest and largest temperatures (GPU)."""
 import pytest
 import torch
 
@@ -46,3 +46,40 @@ def test_rows_outside_the_loss_pass_no_gradient(rows, vocab):
     want = torch.autograd.grad(ts.linear_token_scores(hidden, weight, safe), [weight],
                                [up * (tokens == safe), eup])
     assert not bool(torch.isnan(got[0]).any()) and torch.equal(got[0], want[0])
+
+
+@pytest.mark.parametrize("temperature", [1e-38, 4.5e-39])
+def test_smallest_temperatures(temperature):
+    """All probability on the largest logits, in a row of equal ones on each alike."""
+    ts = _scores()
+    x = torch.tensor([[1.0, 2.0, 2.0, -1.0], [5.0, 5.0, 5.0, 5.0]]).cuda()
+    got = ts.token_scores(x, torch.tensor([1, 0]).cuda(), 2, temperature)
+    want = torch.tensor([2.0, 4.0]).log()
+    assert torch.allclose(got.logprob.cpu(), -want, rtol=2.0 ** -20) and torch.allclose(got.entropy.cpu(), want, rtol=2.0 ** -20)
+    assert got.top_ids.tolist() == [[1, 2], [0, 1]]
+
+
+def test_largest_temperature():
+    """Every finite logit counts alike."""
+    ts = _scores()
+    x = _logits(3, 300, F32, 1)
+    x[1, ::3] = -float("inf")
+    got = ts.token_scores(x.cuda(), torch.tensor([0, 1, 2]).cuda(), 2, 8.5e37)
+    want = torch.tensor([300.0, 200.0, 300.0]).log()
+    assert torch.allclose(got.logprob.cpu(), -want, rtol=2.0 ** -20) and torch.allclose(got.entropy.cpu(), want, rtol=2.0 ** -20)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("temperature", [4e-39, 3.0e-39, 8.6e37, 1e45, 1e300])
+def test_temperatures_beyond_fp32_are_refused(temperature, native, monkeypatch):
+    """log2 e over such a temperature overflows, or its inverse is no normal number."""
+    from ops import _hip
+
+    ts = _scores()
+    if not native:
+        monkeypatch.setattr(_hip, "host_ops", lambda: None)
+    x, tokens = torch.zeros((2, 16), device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="temperature"):
+        ts.token_scores(x, tokens, 0, temperature)
+    with pytest.raises(ValueError, match="temperature"):
+        ts.linear_token_scores(x, torch.zeros((4, 16), device="cuda"), tokens, temperature)

@@ -15,7 +15,6 @@
 #include <torch/library.h>
 
 #include <algorithm>
-#include <cmath>
 
 #include "../../include/warpstate_hip.h"
 
@@ -353,10 +352,12 @@ struct TokenScoresFn : Function<TokenScoresFn> {
   }
 };
 
+// A normal FP32 number, and finite times log2 e.
 double inverse(double temperature) {
-  TORCH_CHECK_VALUE(temperature > 0.0 && std::isfinite(temperature) && 1.0 / temperature < 3.4e38,
-                    "The temperature must be positive and finite, not ", temperature);
-  return 1.0 / temperature;
+  const double inv_t = 1.0 / temperature;
+  TORCH_CHECK_VALUE(inv_t >= 0x1p-126 && inv_t <= 2.3e38,
+                    "The temperature must lie between 4.4e-39 and 8.5e37, not ", temperature);
+  return inv_t;
 }
 Tensor checked_tokens(const Tensor& tokens, const Tensor& like) {
   TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong && tokens.dim() == 1 && tokens.size(0) == like.size(0) &&

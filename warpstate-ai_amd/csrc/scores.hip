@@ -10,6 +10,8 @@ using namespace ws;
 namespace {
 
 constexpr int kLargeEpt = 32, kSmallEpt = 8;
+// 1 / temperature: a normal FP32 number, and finite times log2 e.
+bool good_inv_t(float inv_t) { return inv_t >= 0x1p-126f && inv_t <= 2.3e38f; }
 
 // Logits per thread: 8 (parts of 2048) while 32 would leave most compute units without a
 // workgroup, as long as 64 parts cover the row.
@@ -52,7 +54,7 @@ int check_logits(const void* logits, long ld, int f32, long rows, long vocab, co
                      (long)kMaxScoreParts * 256 * kLargeEpt);
   if (ld < vocab) return set_error(kInvalid, "leading dimension < vocab");
   if (f32 != 0 && f32 != 1) return set_error(kInvalid, "unknown logit type %d", f32);
-  if (!(inv_t > 0.0f) || inv_t > 3.4e38f) return set_error(kInvalid, "the temperature must be positive and finite");
+  if (!good_inv_t(inv_t)) return set_error(kInvalid, "the temperature must lie between 4.4e-39 and 8.5e37");
   if (!fits_i32(rows * cdiv(vocab, 2048))) return set_error(kInvalid, "too many logits for one launch");
   return kOk;
 }
@@ -136,7 +138,7 @@ int check_head(const void* hidden, long ld_hidden, const void* weight, long ld_w
   if (rows < 1 || vocab < 1 || d < 1 || !fits_i32(rows) || !fits_i32(vocab) || !fits_i32(d))
     return set_error(kInvalid, "invalid LM-head sizes rows=%ld vocab=%ld d=%ld", rows, vocab, d);
   if (ld_hidden < d || ld_weight < d) return set_error(kInvalid, "leading dimension < d");
-  if (!(inv_t > 0.0f) || inv_t > 3.4e38f) return set_error(kInvalid, "the temperature must be positive and finite");
+  if (!good_inv_t(inv_t)) return set_error(kInvalid, "the temperature must lie between 4.4e-39 and 8.5e37");
   p = GemmParams{};
   p.a = OperandDesc{static_cast<const unsigned short*>(hidden), ld_hidden, 1};
   p.b = OperandDesc{static_cast<const unsigned short*>(weight), ld_weight, 1};  // B = W^T

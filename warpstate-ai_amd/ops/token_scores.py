@@ -39,6 +39,8 @@ Tensor = torch.Tensor
 CHUNK_LOGITS = 1 << 29
 MAX_TOP_K = 64
 MAX_VOCAB = 524288
+# 1 / temperature: a normal FP32 number, and finite times log2 e.
+INVERSE_RANGE = 2.0 ** -126, 2.3e38
 
 
 class TokenScores(NamedTuple):
@@ -57,9 +59,10 @@ def _check_tokens(tokens: Tensor, rows: int, device) -> Tensor:
 
 def _inverse(temperature: float) -> float:
     temperature = float(temperature)
-    if not (temperature > 0.0 and math.isfinite(temperature) and 1.0 / temperature < 3.4e38):
-        raise ValueError(f"The temperature must be positive and finite, not {temperature}")
-    return 1.0 / temperature
+    inverse = 1.0 / temperature if temperature else math.inf
+    if not INVERSE_RANGE[0] <= inverse <= INVERSE_RANGE[1]:
+        raise ValueError(f"The temperature must lie between 4.4e-39 and 8.5e37, not {temperature}")
+    return inverse
 
 
 def _grads(*grads: Tensor | None) -> list[Tensor | None]:
