@@ -7,7 +7,8 @@
 // and make the same C calls without Python. Their arguments are the checked ones.
 //
 // Operators named native_* exist only with this library; warpstate::fp8_linear is defined in
-// Python, with a Python kernel and autograd formula that these replace on CUDA.
+// Python, with a Python kernel and autograd formula that these replace on CUDA. None has a
+// forward-mode derivative; tensors that carry a tangent are refused.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -41,6 +42,12 @@ int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.siz
 void* ptr(const Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
 Tensor bytes(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options().dtype(at::kByte)); }
 Tensor floats(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options().dtype(at::kFloat)); }
+
+template <class... Inputs>
+void refuse_tangents(const char* name, const Inputs&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(inputs._fw_grad(/*level=*/0).defined() || ...), name,
+                              " has no forward-mode derivative");
+}
 
 // --- 8-bit operands -------------------------------------------------------------------------
 
@@ -270,6 +277,7 @@ struct Fp8LinearFn : Function<Fp8LinearFn> {
   }
 };
 FiveTensors linear(const Tensor& x, const Tensor& weight, bool e8m0, bool keep_x, bool keep_w) {
+  refuse_tangents("fp8_linear", x, weight);
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad())) {
     static const auto op = c10::Dispatcher::singleton()
                                .findSchemaOrThrow("warpstate::fp8_linear", "")
@@ -368,6 +376,7 @@ Tensor checked_tokens(const Tensor& tokens, const Tensor& like) {
 
 // token_scores of ops/token_scores.py, with its checks.
 FourTensors native_token_scores(const Tensor& logits_in, const Tensor& tokens_in, int64_t top_k, double temperature) {
+  refuse_tangents("token_scores", logits_in);
   TORCH_CHECK_VALUE((logits_in.scalar_type() == at::kBFloat16 || logits_in.scalar_type() == at::kFloat) &&
                         logits_in.dim() == 2,
                     "Expected BF16 or FP32 logits [rows, vocab]");
@@ -467,6 +476,7 @@ struct HeadScoresFn : Function<HeadScoresFn> {
 std::tuple<Tensor, Tensor> native_head_scores(const Tensor& hidden, const Tensor& weight, const Tensor& h,
                                               const Tensor& w, const Tensor& tokens, double inv_t,
                                               int64_t chunk_rows) {
+  refuse_tangents("linear_token_scores", hidden, weight);
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
     variable_list v = HeadScoresFn::apply(hidden, weight, h, w, tokens, inv_t, chunk_rows);
     return {v[0], v[1]};

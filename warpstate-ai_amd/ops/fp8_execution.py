@@ -24,6 +24,7 @@ binades goes unused.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ops import _hip
 from ops.fused_execution import mm_f32
@@ -362,6 +363,11 @@ _fp8_linear.register_autograd(_linear_autograd, setup_context=_linear_setup)
 _hip.host_ops()
 
 
+def _refuse_tangents(*tensors: Tensor) -> None:
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("fp8_linear has no forward-mode derivative")
+
+
 def fp8_linear(x: Tensor, weight: Tensor, scale_dtype: torch.dtype = E8M0) -> Tensor:
     """x @ weight.T of a bias-free projection in 8 bits, with autograd: x [..., K] BF16, weight
     [N, K] (nn.Linear layout), BF16 or an FP32 master.
@@ -371,7 +377,8 @@ def fp8_linear(x: Tensor, weight: Tensor, scale_dtype: torch.dtype = E8M0) -> Te
     r(q(dy)^T q(x)) with both operands quantized by columns; a step then keeps one byte per
     element of x and of W for the backward. An FP32 master's gradient is FP32, and the 8-bit
     matrix instruction's sums are not (``fp8_mm``): it is dy^T x of the BF16 tensors with FP32
-    sums (``mm_f32``), from x itself."""
+    sums (``mm_f32``), from x itself. First derivatives by
+    reverse mode only (forward-mode tensors and functorch's derivatives are refused)."""
     if x.dtype != BF16:
         raise ValueError("An 8-bit projection takes BF16 activations")
     if x.ndim < 1 or weight.ndim != 2 or x.shape[-1] != weight.shape[1]:
@@ -382,6 +389,8 @@ def fp8_linear(x: Tensor, weight: Tensor, scale_dtype: torch.dtype = E8M0) -> Te
     rows = x.reshape(-1, x.shape[-1])
     _check_input(rows, scale_dtype)
     _check_input(weight, scale_dtype)
+    if not torch.compiler.is_compiling() and _hip.host_ops() is None:
+        _refuse_tangents(x, weight)  # as the native autograd kernel does
     grad = torch.is_grad_enabled()
     y = _fp8_linear(rows.contiguous(), weight.contiguous(), scale_dtype == E8M0,
                     grad and weight.requires_grad and weight.dtype == BF16,

@@ -18,6 +18,9 @@ A token of -100 is ignored: its log probability is 0 and passes no gradient. Its
 an entropy, whose gradient it passes. Any other token outside the vocabulary gets NaN (and a
 gradient of NaN, unless its log probability's upstream gradient is zero). Logits of -inf have
 probability 0.
+
+First derivatives by reverse mode only: forward-mode tensors and functorch's derivatives are
+refused, and so is a second differentiation.
 """
 
 from __future__ import annotations
