@@ -1,5 +1,6 @@
 """The 8-bit projection and the token scores under PyTorch's other modes: forward-mode tensors and
-functorch's derivatives are refused (GPU)."""
+functorch's derivatives are refused, vmap and fake tensors reach the operators, a recorded backward
+gives the first derivative (GPU)."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -51,3 +52,46 @@ def test_functorch_derivatives_are_refused(name):
         torch.func.jvp(call, (x,), (torch.ones_like(x),))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda t: call(t).float().sum())(x)
+
+
+@pytest.mark.parametrize("name", ["scores", "projection"])
+def test_vmap(name):
+    call, x = _calls()[name]
+    many = torch.stack([x, x * 0.5, x + 1.0])
+    want = torch.stack([call(t) for t in many])
+    assert torch.equal(torch.func.vmap(call)(many), want)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_recorded_backward(name):
+    """create_graph gives the plain first derivative; the second is refused."""
+    call, x = _calls()[name]
+    leaf = x.clone().requires_grad_(True)
+    out = call(leaf).float()
+    up = torch.linspace(-1, 1, out.numel()).view(out.shape).cuda().requires_grad_(True)
+    want, = torch.autograd.grad((out * up.detach()).sum(), [leaf], retain_graph=True)
+    got, = torch.autograd.grad((out * up).sum(), [leaf], create_graph=True)
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(got.float().sum(), [leaf])
+    with pytest.raises(RuntimeError):
+        got, = torch.autograd.grad((call(leaf).float() * up).sum(), [leaf], create_graph=True)
+        torch.autograd.grad(got.float().sum(), [up])
+
+
+@pytest.mark.parametrize("requires", [False, True])
+def test_fake_logits(requires):
+    """Shapes and types of the scores and their gradient, without data."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from ops import token_scores as ts
+
+    with FakeTensorMode():
+        x = torch.empty((7, 300), dtype=BF16, device="cuda", requires_grad=requires)
+        got = ts.token_scores(x, torch.zeros(7, dtype=torch.int64, device="cuda"), 3)
+        assert [(tuple(t.shape), t.dtype) for t in got] == [((7,), F32), ((7,), F32), ((7, 3), F32),
+                                                             ((7, 3), torch.int64)]
+        assert got.logprob.requires_grad == requires
+        if requires:
+            dx, = torch.autograd.grad(got.logprob.sum() + got.entropy.sum(), [x])
+            assert dx.shape == x.shape and dx.dtype == BF16

@@ -7,8 +7,9 @@
 // and make the same C calls without Python. Their arguments are the checked ones.
 //
 // Operators named native_* exist only with this library; warpstate::fp8_linear is defined in
-// Python, with a Python kernel and autograd formula that these replace on CUDA. None has a
-// forward-mode derivative; tensors that carry a tangent are refused.
+// Python, with a Python kernel and autograd formula that these replace on CUDA. Autograd kernels read
+// no data: they call operators below autograd, so that wrapped and fake tensors reach kernels of
+// their own. None has a forward-mode derivative; tensors that carry a tangent are refused.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -43,6 +44,21 @@ void* ptr(const Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() 
 Tensor bytes(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options().dtype(at::kByte)); }
 Tensor floats(const Tensor& like, at::IntArrayRef sizes) { return at::empty(sizes, like.options().dtype(at::kFloat)); }
 
+template <class Signature>
+c10::TypedOperatorHandle<Signature> find(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
+}
+// The operator below autograd.
+template <class Op, class... Args>
+auto below(const Op& op, Args&&... args) {
+  at::AutoDispatchBelowAutograd guard;
+  return op.call(std::forward<Args>(args)...);
+}
+// Whether a call with these inputs records a node.
+template <class... Inputs>
+bool records(const Inputs&... inputs) {
+  return at::GradMode::is_enabled() && (inputs.requires_grad() || ...);
+}
 template <class... Inputs>
 void refuse_tangents(const char* name, const Inputs&... inputs) {
   TORCH_CHECK_NOT_IMPLEMENTED(!(inputs._fw_grad(/*level=*/0).defined() || ...), name,
@@ -237,12 +253,9 @@ std::tuple<Tensor, Tensor> linear_backward(const Tensor& grad_in, const Tensor& 
 struct Fp8LinearFn : Function<Fp8LinearFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, bool e8m0, bool keep_x,
                                bool keep_w) {
-    static const auto op = c10::Dispatcher::singleton()
-                               .findSchemaOrThrow("warpstate::fp8_linear", "")
-                               .typed<FiveTensors(const Tensor&, const Tensor&, bool, bool, bool)>();
+    static const auto op = find<FiveTensors(const Tensor&, const Tensor&, bool, bool, bool)>("warpstate::fp8_linear");
     ctx->set_materialize_grads(false);
-    at::AutoDispatchBelowAutograd guard;
-    auto [y, qt, qt_scale, wt, wt_scale] = op.call(x, weight, e8m0, keep_x, keep_w);
+    auto [y, qt, qt_scale, wt, wt_scale] = below(op, x, weight, e8m0, keep_x, keep_w);
     const bool master = weight.scalar_type() == at::kFloat;
     // x itself only where its weight gradient reads it.
     ctx->save_for_backward({master && weight.requires_grad() ? x : qt, qt, qt_scale, wt, wt_scale});
@@ -278,12 +291,9 @@ struct Fp8LinearFn : Function<Fp8LinearFn> {
 };
 FiveTensors linear(const Tensor& x, const Tensor& weight, bool e8m0, bool keep_x, bool keep_w) {
   refuse_tangents("fp8_linear", x, weight);
-  if (!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad())) {
-    static const auto op = c10::Dispatcher::singleton()
-                               .findSchemaOrThrow("warpstate::fp8_linear", "")
-                               .typed<FiveTensors(const Tensor&, const Tensor&, bool, bool, bool)>();
-    at::AutoDispatchBelowAutograd guard;
-    return op.call(x, weight, e8m0, keep_x, keep_w);
+  if (!records(x, weight)) {
+    static const auto op = find<FiveTensors(const Tensor&, const Tensor&, bool, bool, bool)>("warpstate::fp8_linear");
+    return below(op, x, weight, e8m0, keep_x, keep_w);
   }
   variable_list v = Fp8LinearFn::apply(x, weight, e8m0, keep_x, keep_w);
   return {v[0], v[1], v[2], v[3], v[4]};
@@ -316,21 +326,66 @@ FiveTensors scores_forward(const Tensor& logits, const Tensor& tokens, int64_t t
 }
 
 // An upstream gradient as the kernels read it.
-Tensor upstream(const Tensor& g) { return g.defined() ? g.to(at::kFloat).contiguous() : g; }
+Tensor upstream(const std::optional<Tensor>& g) {
+  return g.has_value() && g->defined() ? g->to(at::kFloat).contiguous() : Tensor();
+}
+std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 const float* float_ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
 
-// First derivatives only: a backward that is itself recorded would lose the second.
-void refuse_second() {
-  TORCH_CHECK(!at::GradMode::is_enabled(), "token scores cannot be differentiated twice");
+Tensor scores_backward(const Tensor& logits, const Tensor& tokens, const Tensor& lse, const Tensor& entropy,
+                       const std::optional<Tensor>& dlogprob, const std::optional<Tensor>& dentropy, double inv_t) {
+  c10::DeviceGuard guard(logits.device());
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  Tensor out = at::empty({rows, vocab}, logits.options());
+  if (rows) {
+    const Tensor g = upstream(dlogprob), h = upstream(dentropy);
+    check(ws_token_scores_backward(logits.const_data_ptr(), row_stride(logits), logits.scalar_type() == at::kFloat,
+                                   tokens.const_data_ptr<int64_t>(), rows, vocab, (float)inv_t, float_ptr(lse),
+                                   float_ptr(entropy), float_ptr(g), float_ptr(h), out.data_ptr(), vocab,
+                                   stream_of(logits)),
+          "ws_token_scores_backward");
+  }
+  return out;
+}
+
+// A backward operator: below autograd, unless its own gradient is being recorded (create_graph, a
+// functorch transform): then its autograd kernel records a node that refuses to be differentiated.
+template <class Op, class... Args>
+auto backward_op(const Op& op, Args&&... args) {
+  if (at::GradMode::is_enabled()) return op.call(std::forward<Args>(args)...);
+  return below(op, std::forward<Args>(args)...);
+}
+variable_list refuse_second() { TORCH_CHECK(false, "token scores cannot be differentiated twice"); }
+bool needs_grad(const std::optional<Tensor>& t) { return t.has_value() && t->defined() && t->requires_grad(); }
+
+typedef Tensor ScoresBackward(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&,
+                              const std::optional<Tensor>&, double);
+const auto& scores_backward_op() {
+  static const auto op = find<ScoresBackward>("warpstate::native_token_scores_backward");
+  return op;
+}
+struct ScoresBackwardFn : Function<ScoresBackwardFn> {
+  static Tensor forward(AutogradContext*, const Tensor& logits, const Tensor& tokens, const Tensor& lse,
+                        const Tensor& entropy, const std::optional<Tensor>& dlogprob,
+                        const std::optional<Tensor>& dentropy, double inv_t) {
+    return below(scores_backward_op(), logits, tokens, lse, entropy, dlogprob, dentropy, inv_t);
+  }
+  static variable_list backward(AutogradContext*, variable_list) { return refuse_second(); }
+};
+Tensor scores_backward_autograd(const Tensor& logits, const Tensor& tokens, const Tensor& lse, const Tensor& entropy,
+                                const std::optional<Tensor>& dlogprob, const std::optional<Tensor>& dentropy,
+                                double inv_t) {
+  if (records(logits, lse, entropy) || (at::GradMode::is_enabled() && (needs_grad(dlogprob) || needs_grad(dentropy))))
+    return ScoresBackwardFn::apply(logits, tokens, lse, entropy, dlogprob, dentropy, inv_t);
+  return below(scores_backward_op(), logits, tokens, lse, entropy, dlogprob, dentropy, inv_t);
 }
 
 struct TokenScoresFn : Function<TokenScoresFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, int64_t top_k,
                                double inv_t) {
-    auto [logprob, entropy, top, ids, lse] = [&] {
-      at::AutoDispatchBelowAutograd guard;
-      return scores_forward(logits, tokens, top_k, inv_t, true);
-    }();
+    static const auto op =
+        find<FiveTensors(const Tensor&, const Tensor&, int64_t, double)>("warpstate::native_token_scores_lse");
+    auto [logprob, entropy, top, ids, lse] = below(op, logits, tokens, top_k, inv_t);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({logits, tokens, lse, entropy});
     ctx->saved_data["inv_t"] = inv_t;
@@ -338,25 +393,12 @@ struct TokenScoresFn : Function<TokenScoresFn> {
     return {logprob, entropy, top, ids};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list none(4);
-    if (!grads[0].defined() && !grads[1].defined()) return none;
-    refuse_second();
+    variable_list d(4);
+    if (!grads[0].defined() && !grads[1].defined()) return d;
     const auto s = ctx->get_saved_variables();
-    const Tensor &logits = s[0], &tokens = s[1];
-    c10::DeviceGuard guard(logits.device());
-    const int64_t rows = logits.size(0), vocab = logits.size(1);
-    Tensor out = at::empty({rows, vocab}, logits.options());
-    if (rows) {
-      const Tensor g = upstream(grads[0]), h = upstream(grads[1]);
-      check(ws_token_scores_backward(logits.const_data_ptr(), row_stride(logits),
-                                     logits.scalar_type() == at::kFloat, tokens.const_data_ptr<int64_t>(), rows,
-                                     vocab, (float)ctx->saved_data["inv_t"].toDouble(), float_ptr(s[2]),
-                                     float_ptr(s[3]), float_ptr(g), float_ptr(h), out.data_ptr(), vocab,
-                                     stream_of(logits)),
-            "ws_token_scores_backward");
-    }
-    none[0] = out;
-    return none;
+    d[0] = backward_op(scores_backward_op(), s[0], s[1], s[2], s[3], maybe(grads[0]), maybe(grads[1]),
+                       ctx->saved_data["inv_t"].toDouble());
+    return d;
   }
 };
 
@@ -375,26 +417,39 @@ Tensor checked_tokens(const Tensor& tokens, const Tensor& like) {
 }
 
 // token_scores of ops/token_scores.py, with its checks.
-FourTensors native_token_scores(const Tensor& logits_in, const Tensor& tokens_in, int64_t top_k, double temperature) {
-  refuse_tangents("token_scores", logits_in);
-  TORCH_CHECK_VALUE((logits_in.scalar_type() == at::kBFloat16 || logits_in.scalar_type() == at::kFloat) &&
-                        logits_in.dim() == 2,
+struct CheckedScores {
+  Tensor logits, tokens;
+  double inv_t;
+};
+CheckedScores check_scores(const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature) {
+  TORCH_CHECK_VALUE((logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat) &&
+                        logits.dim() == 2,
                     "Expected BF16 or FP32 logits [rows, vocab]");
-  const int64_t rows = logits_in.size(0), vocab = logits_in.size(1);
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
   TORCH_CHECK_VALUE(vocab >= 1 && vocab <= kMaxVocab, "Token scores take 1 to ", kMaxVocab, " logits a row, not ", vocab);
   const int64_t most = std::min(kMaxTopK, vocab);
   TORCH_CHECK_VALUE(top_k >= 0 && top_k <= most, "top_k must lie in [0, ", most, "], not ", top_k);
-  const Tensor tokens = checked_tokens(tokens_in, logits_in);
-  const double inv_t = inverse(temperature);
-  const bool unit = (logits_in.stride(1) == 1 || vocab == 1) && (rows <= 1 || logits_in.stride(0) >= vocab);
-  const Tensor logits = unit ? logits_in : logits_in.contiguous();
-  if (at::GradMode::is_enabled() && logits.requires_grad()) {
-    variable_list v = TokenScoresFn::apply(logits, tokens, top_k, inv_t);
-    return {v[0], v[1], v[2], v[3]};
-  }
-  at::AutoDispatchBelowAutograd guard;
-  auto [logprob, entropy, top, ids, lse] = scores_forward(logits, tokens, top_k, inv_t, false);
+  const bool unit = (logits.stride(1) == 1 || vocab == 1) && (rows <= 1 || logits.stride(0) >= vocab);
+  return {unit ? logits : logits.contiguous(), checked_tokens(tokens, logits), inverse(temperature)};
+}
+FourTensors native_token_scores(const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature) {
+  const auto c = check_scores(logits, tokens, top_k, temperature);
+  auto [logprob, entropy, top, ids, lse] = scores_forward(c.logits, c.tokens, top_k, c.inv_t, false);
   return {logprob, entropy, top, ids};
+}
+FiveTensors scores_with_lse(const Tensor& logits, const Tensor& tokens, int64_t top_k, double inv_t) {
+  return scores_forward(logits, tokens, top_k, inv_t, true);
+}
+FourTensors token_scores_autograd(const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature) {
+  refuse_tangents("token_scores", logits);
+  if (!records(logits)) {
+    static const auto op =
+        find<FourTensors(const Tensor&, const Tensor&, int64_t, double)>("warpstate::native_token_scores");
+    return below(op, logits, tokens, top_k, temperature);
+  }
+  const auto c = check_scores(logits, tokens, top_k, temperature);
+  variable_list v = TokenScoresFn::apply(c.logits, c.tokens, top_k, c.inv_t);
+  return {v[0], v[1], v[2], v[3]};
 }
 
 // hidden and weight as the kernels read them (BF16, 16-byte rows, equal padded widths).
@@ -413,14 +468,78 @@ std::tuple<Tensor, Tensor, Tensor> head_forward(const Tensor& h, const Tensor& w
   return {logprob, entropy, lse};
 }
 
+// (dHidden, dWeight), each empty unless wanted, in the operands' padded width; dWeight in BF16 (of
+// one chunk) or FP32.
+std::tuple<Tensor, Tensor> head_backward(const Tensor& h, const Tensor& w, const Tensor& tokens, const Tensor& lse,
+                                         const Tensor& entropy, const std::optional<Tensor>& dlogprob,
+                                         const std::optional<Tensor>& dentropy, double inv_t, int64_t chunk_rows,
+                                         bool want_h, bool want_w, bool bf16) {
+  c10::DeviceGuard guard(h.device());
+  const int64_t rows = h.size(0), width = h.size(1), vocab = w.size(0);
+  Tensor dh = at::empty({want_h ? rows : 0, width}, h.options());
+  Tensor dw = at::empty({want_w ? vocab : 0, width}, h.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+  if (rows) {
+    const Tensor g = upstream(dlogprob), e = upstream(dentropy);
+    Tensor work = bytes(h, {ws_linear_token_scores_backward_workspace_bytes(rows, vocab, width, chunk_rows)});
+    // The dHidden product reads the head weight along the vocabulary.
+    Tensor wt;
+    if (want_h && rows >= kTransposeMinRows && vocab % 8 == 0) {
+      wt = at::empty({width, vocab}, w.options());
+      check(ws_transpose_bf16(w.const_data_ptr(), row_stride(w), wt.data_ptr(), vocab, width, stream_of(w)),
+            "ws_transpose_bf16");
+    }
+    check(ws_linear_token_scores_backward(h.const_data_ptr(), row_stride(h), w.const_data_ptr(), row_stride(w),
+                                          ptr(wt), tokens.const_data_ptr<int64_t>(), float_ptr(lse),
+                                          float_ptr(entropy), float_ptr(g), float_ptr(e), rows, vocab, width,
+                                          (float)inv_t, work.data_ptr(), chunk_rows, ptr(dh), width, ptr(dw), width,
+                                          bf16, stream_of(h)),
+          "ws_linear_token_scores_backward");
+  } else if (want_w) {
+    dw.zero_();
+  }
+  return {dh, dw};
+}
+
+typedef std::tuple<Tensor, Tensor> HeadBackward(const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                const Tensor&, const std::optional<Tensor>&,
+                                                const std::optional<Tensor>&, double, int64_t, bool, bool, bool);
+const auto& head_backward_op() {
+  static const auto op = find<HeadBackward>("warpstate::native_head_scores_backward");
+  return op;
+}
+struct HeadBackwardFn : Function<HeadBackwardFn> {
+  static variable_list forward(AutogradContext*, const Tensor& h, const Tensor& w, const Tensor& tokens,
+                               const Tensor& lse, const Tensor& entropy, const std::optional<Tensor>& dlogprob,
+                               const std::optional<Tensor>& dentropy, double inv_t, int64_t chunk_rows, bool want_h,
+                               bool want_w, bool bf16) {
+    auto [dh, dw] = below(head_backward_op(), h, w, tokens, lse, entropy, dlogprob, dentropy, inv_t, chunk_rows,
+                          want_h, want_w, bf16);
+    return {dh, dw};
+  }
+  static variable_list backward(AutogradContext*, variable_list) { return refuse_second(); }
+};
+std::tuple<Tensor, Tensor> head_backward_autograd(const Tensor& h, const Tensor& w, const Tensor& tokens,
+                                                  const Tensor& lse, const Tensor& entropy,
+                                                  const std::optional<Tensor>& dlogprob,
+                                                  const std::optional<Tensor>& dentropy, double inv_t,
+                                                  int64_t chunk_rows, bool want_h, bool want_w, bool bf16) {
+  if (records(h, w, lse, entropy) || (at::GradMode::is_enabled() && (needs_grad(dlogprob) || needs_grad(dentropy)))) {
+    variable_list v = HeadBackwardFn::apply(h, w, tokens, lse, entropy, dlogprob, dentropy, inv_t, chunk_rows, want_h,
+                                            want_w, bf16);
+    return {v[0], v[1]};
+  }
+  return below(head_backward_op(), h, w, tokens, lse, entropy, dlogprob, dentropy, inv_t, chunk_rows, want_h, want_w,
+               bf16);
+}
+
 struct HeadScoresFn : Function<HeadScoresFn> {
   // Gradients go to the tensors that h and w were made from.
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& h,
                                const Tensor& w, const Tensor& tokens, double inv_t, int64_t chunk_rows) {
-    auto [logprob, entropy, lse] = [&] {
-      at::AutoDispatchBelowAutograd guard;
-      return head_forward(h, w, tokens, inv_t);
-    }();
+    typedef const Tensor& T;
+    static const auto op =
+        find<std::tuple<Tensor, Tensor, Tensor>(T, T, T, double)>("warpstate::native_head_scores_lse");
+    auto [logprob, entropy, lse] = below(op, h, w, tokens, inv_t);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({h, w, tokens, lse, entropy});
     ctx->saved_data["inv_t"] = inv_t;
@@ -435,55 +554,55 @@ struct HeadScoresFn : Function<HeadScoresFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list d(7);
     if (!grads[0].defined() && !grads[1].defined()) return d;
-    refuse_second();
     const auto s = ctx->get_saved_variables();
-    const Tensor &h = s[0], &w = s[1];
     const bool want_h = ctx->saved_data["want_h"].toBool(), want_w = ctx->saved_data["want_w"].toBool();
-    c10::DeviceGuard guard(h.device());
-    const int64_t rows = h.size(0), width = h.size(1), vocab = w.size(0);
-    const int64_t chunk = ctx->saved_data["chunk_rows"].toInt();
-    if (want_h) d[0] = at::empty({rows, width}, h.options());
+    const int64_t rows = s[0].size(0), vocab = s[1].size(0), chunk = ctx->saved_data["chunk_rows"].toInt();
+    const auto weight_type = ctx->saved_data["weight_type"].toScalarType();
     // A BF16 weight's gradient is rounded as it is written where one chunk makes all of it.
-    const bool bf16 = ctx->saved_data["weight_type"].toScalarType() == at::kBFloat16 && rows <= chunk && vocab % 8 == 0;
-    Tensor dw;
-    if (want_w) dw = at::empty({vocab, width}, h.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
-    if (rows) {
-      const Tensor g = upstream(grads[0]), e = upstream(grads[1]);
-      Tensor work = bytes(h, {ws_linear_token_scores_backward_workspace_bytes(rows, vocab, width, chunk)});
-      // The dHidden product reads the head weight along the vocabulary.
-      Tensor wt;
-      if (want_h && rows >= kTransposeMinRows && vocab % 8 == 0) {
-        wt = at::empty({width, vocab}, w.options());
-        check(ws_transpose_bf16(w.const_data_ptr(), row_stride(w), wt.data_ptr(), vocab, width, stream_of(w)),
-              "ws_transpose_bf16");
-      }
-      check(ws_linear_token_scores_backward(h.const_data_ptr(), row_stride(h), w.const_data_ptr(), row_stride(w),
-                                            ptr(wt), s[2].const_data_ptr<int64_t>(), float_ptr(s[3]),
-                                            float_ptr(s[4]), float_ptr(g), float_ptr(e), rows, vocab, width,
-                                            (float)ctx->saved_data["inv_t"].toDouble(), work.data_ptr(), chunk,
-                                            want_h ? d[0].data_ptr() : nullptr, width,
-                                            want_w ? dw.data_ptr() : nullptr, width, bf16, stream_of(h)),
-            "ws_linear_token_scores_backward");
-    } else if (want_w) {
-      dw.zero_();
-    }
+    const bool bf16 = weight_type == at::kBFloat16 && rows <= chunk && vocab % 8 == 0;
+    auto [dh, dw] = backward_op(head_backward_op(), s[0], s[1], s[2], s[3], s[4], maybe(grads[0]), maybe(grads[1]),
+                                ctx->saved_data["inv_t"].toDouble(), chunk, want_h, want_w, bf16);
     const int64_t cols = ctx->saved_data["width"].toInt();
-    if (want_h) d[0] = d[0].narrow(1, 0, cols).to(ctx->saved_data["hidden_type"].toScalarType());
-    if (want_w) d[1] = dw.narrow(1, 0, cols).to(ctx->saved_data["weight_type"].toScalarType());
+    if (want_h) d[0] = dh.narrow(1, 0, cols).to(ctx->saved_data["hidden_type"].toScalarType());
+    if (want_w) d[1] = dw.narrow(1, 0, cols).to(weight_type);
     return d;
   }
 };
 std::tuple<Tensor, Tensor> native_head_scores(const Tensor& hidden, const Tensor& weight, const Tensor& h,
                                               const Tensor& w, const Tensor& tokens, double inv_t,
                                               int64_t chunk_rows) {
-  refuse_tangents("linear_token_scores", hidden, weight);
-  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())) {
-    variable_list v = HeadScoresFn::apply(hidden, weight, h, w, tokens, inv_t, chunk_rows);
-    return {v[0], v[1]};
-  }
-  at::AutoDispatchBelowAutograd guard;
   auto [logprob, entropy, lse] = head_forward(h, w, tokens, inv_t);
   return {logprob, entropy};
+}
+std::tuple<Tensor, Tensor> head_scores_autograd(const Tensor& hidden, const Tensor& weight, const Tensor& h,
+                                                const Tensor& w, const Tensor& tokens, double inv_t,
+                                                int64_t chunk_rows) {
+  refuse_tangents("linear_token_scores", hidden, weight);
+  if (!records(hidden, weight)) {
+    typedef const Tensor& T;
+    static const auto op =
+        find<std::tuple<Tensor, Tensor>(T, T, T, T, T, double, int64_t)>("warpstate::native_head_scores");
+    return below(op, hidden, weight, h, w, tokens, inv_t, chunk_rows);
+  }
+  variable_list v = HeadScoresFn::apply(hidden, weight, h, w, tokens, inv_t, chunk_rows);
+  return {v[0], v[1]};
+}
+
+// Shapes and types only: the logits' operators on fake tensors.
+FourTensors scores_meta(const Tensor& logits, const Tensor& tokens, int64_t top_k, double temperature) {
+  check_scores(logits, tokens, top_k, temperature);
+  const int64_t rows = logits.size(0);
+  return {floats(logits, {rows}), floats(logits, {rows}), floats(logits, {rows, top_k}),
+          at::empty({rows, top_k}, logits.options().dtype(at::kLong))};
+}
+FiveTensors scores_with_lse_meta(const Tensor& logits, const Tensor&, int64_t top_k, double) {
+  const int64_t rows = logits.size(0);
+  return {floats(logits, {rows}), floats(logits, {rows}), floats(logits, {rows, top_k}),
+          at::empty({rows, top_k}, logits.options().dtype(at::kLong)), floats(logits, {rows})};
+}
+Tensor scores_backward_meta(const Tensor& logits, const Tensor&, const Tensor&, const Tensor&,
+                            const std::optional<Tensor>&, const std::optional<Tensor>&, double) {
+  return at::empty({logits.size(0), logits.size(1)}, logits.options());
 }
 
 // Undefined tensors cannot leave an operator: empty ones in the place of forms not wanted.
@@ -503,6 +622,16 @@ TORCH_LIBRARY_FRAGMENT(warpstate, m) {
       "native_token_scores(Tensor logits, Tensor tokens, int top_k, float temperature) -> (Tensor, Tensor, "
       "Tensor, Tensor)");
   m.def(
+      "native_token_scores_lse(Tensor logits, Tensor tokens, int top_k, float inv_t) -> (Tensor, Tensor, Tensor, "
+      "Tensor, Tensor)");
+  m.def(
+      "native_token_scores_backward(Tensor logits, Tensor tokens, Tensor lse, Tensor entropy, Tensor? dlogprob, "
+      "Tensor? dentropy, float inv_t) -> Tensor");
+  m.def("native_head_scores_lse(Tensor h, Tensor w, Tensor tokens, float inv_t) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "native_head_scores_backward(Tensor h, Tensor w, Tensor tokens, Tensor lse, Tensor entropy, Tensor? dlogprob, "
+      "Tensor? dentropy, float inv_t, int chunk_rows, bool want_h, bool want_w, bool bf16) -> (Tensor, Tensor)");
+  m.def(
       "native_head_scores(Tensor hidden, Tensor weight, Tensor h, Tensor w, Tensor tokens, float inv_t, "
       "int chunk_rows) -> (Tensor, Tensor)");
 }
@@ -511,12 +640,23 @@ TORCH_LIBRARY_IMPL(warpstate, CUDA, m) {
   m.impl("native_quantize_rows", &native_quantize_rows);
   m.impl("native_fp8_mm", &native_fp8_mm);
   m.impl("native_token_scores", &native_token_scores);
+  m.impl("native_token_scores_lse", &scores_with_lse);
+  m.impl("native_token_scores_backward", &scores_backward);
   m.impl("native_head_scores", &native_head_scores);
+  m.impl("native_head_scores_lse", &head_forward);
+  m.impl("native_head_scores_backward", &head_backward);
   m.impl("fp8_linear", &linear_forward);
   m.impl("fp8_linear_backward", &linear_backward);
 }
 TORCH_LIBRARY_IMPL(warpstate, AutogradCUDA, m) {
-  m.impl("native_token_scores", &native_token_scores);
-  m.impl("native_head_scores", &native_head_scores);
+  m.impl("native_token_scores", &token_scores_autograd);
+  m.impl("native_token_scores_backward", &scores_backward_autograd);
+  m.impl("native_head_scores", &head_scores_autograd);
+  m.impl("native_head_scores_backward", &head_backward_autograd);
   m.impl("fp8_linear", &linear);
+}
+TORCH_LIBRARY_IMPL(warpstate, Meta, m) {
+  m.impl("native_token_scores", &scores_meta);
+  m.impl("native_token_scores_lse", &scores_with_lse_meta);
+  m.impl("native_token_scores_backward", &scores_backward_meta);
 }
