@@ -1,5 +1,5 @@
 """Token scores at the edges of what their documentation allows: tokens without a score under
-masked losses, the smallest and largest temperatures (GPU)."""
+masked losses, the smallest and largest temperatures, more rows than one launch takes (GPU)."""
 import pytest
 import torch
 
@@ -83,3 +83,23 @@ def test_temperatures_beyond_fp32_are_refused(temperature, native, monkeypatch):
         ts.token_scores(x, tokens, 0, temperature)
     with pytest.raises(ValueError, match="temperature"):
         ts.linear_token_scores(x, torch.zeros((4, 16), device="cuda"), tokens, temperature)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_more_rows_than_one_launch_takes(dtype):
+    """2^24 workgroups of 256 threads are 2^32 threads, which no launch has: the rows beyond are
+    scored, and their gradients written, as on their own."""
+    ts = _scores()
+    rows, vocab = 2 ** 24 + 3000, 3
+    x = torch.empty((rows, vocab), dtype=dtype, device="cuda").normal_().requires_grad_(True)
+    tokens = torch.arange(rows, device="cuda") % vocab
+    g, h = torch.randn(rows, device="cuda"), torch.randn(rows, device="cuda")
+    got = ts.token_scores(x, tokens, 2)
+    dx, = torch.autograd.grad([got.logprob, got.entropy], [x], [g, h])
+    for part in (slice(0, 5000), slice(2 ** 24 - 1500, 2 ** 24 + 1500), slice(rows - 2000, rows)):
+        own = x.detach()[part].clone().requires_grad_(True)
+        alone = ts.token_scores(own, tokens[part], 2)
+        want, = torch.autograd.grad([alone.logprob, alone.entropy], [own], [g[part], h[part]])
+        for a, b in zip(got, alone):
+            assert torch.equal(a[part], b)
+        assert torch.equal(dx[part], want) and bool(want.any())

@@ -7,10 +7,13 @@ using namespace ws;
 
 namespace {
 
+// Workgroups of 256 threads in one launch, which has fewer than 2^32 threads.
+bool fits_launch(long blocks) { return blocks < 1L << 24; }
+
 template <bool F32, int SCALE, int FORM, int R = 8>
 int run_quantize(const QuantParams& p, bool vec, hipStream_t s) {
   const long tiles = (long)cdiv(p.rows, 16 * R) * p.col_tiles;
-  if (!fits_i32(tiles)) return set_error(kInvalid, "too many 128 x 128 tiles");
+  if (!fits_launch(tiles)) return set_error(kInvalid, "too many 128 x 128 tiles");
   if constexpr (FORM == kQuantRows && R == 8) {
     // Few tiles: a row per thread (1 x 5632: 5.9 -> 2.9 us).
     if (tiles < device_cus()) return run_quantize<F32, SCALE, FORM, 1>(p, vec, s);
@@ -218,7 +221,7 @@ extern "C" int ws_fp8_pack(const void* src, int64_t s_row, int64_t s_col, void* 
   if (ldd < cols || ldd % 16 || !al(dst, 16))
     return set_error(kInvalid, "packed rows need 16-byte aligned storage of a multiple of 16 bytes");
   const long blocks = (rows * (ldd / 16) + 255) / 256;
-  if (!fits_i32(blocks)) return set_error(kInvalid, "matrix to pack is too large");
+  if (!fits_launch(blocks)) return set_error(kInvalid, "matrix to pack is too large");
   hipLaunchKernelGGL(pack_bytes_kernel, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream),
                      static_cast<const unsigned char*>(src), (long)s_row, (long)s_col,
                      static_cast<unsigned char*>(dst), (long)ldd, (long)rows, (long)cols);

@@ -28,8 +28,36 @@ void launch_rows(const ScoreParams& p, hipStream_t s) {
   if (p.top_k > 0) hipLaunchKernelGGL((score_rows_kernel<F32, EPT, true>), grid, dim3(256), 0, s, p);
   else hipLaunchKernelGGL((score_rows_kernel<F32, EPT, false>), grid, dim3(256), 0, s, p);
 }
+// A launch has fewer than 2^32 threads, so more workgroups of 256 go in several launches.
+constexpr long kMaxLaunchBlocks = (1L << 24) - 1;
+long launch_row_count(long blocks_per_row) { return kMaxLaunchBlocks / blocks_per_row; }
+
+// The rows from `first` on, at most `count` of them.
+ScoreParams some_rows(ScoreParams p, long first, long count, bool f32) {
+  p.rows = (int)(p.rows - first < count ? p.rows - first : count);
+  p.logits = static_cast<const char*>(p.logits) + first * p.ld * (f32 ? 4 : 2);
+  p.tokens += first;
+  p.out.lse += first;
+  p.out.entropy += first;
+  if (p.out.logprob) p.out.logprob += first;
+  if (p.top_k) {
+    p.top_logprobs += first * p.top_k;
+    p.top_ids += first * p.top_k;
+  }
+  if (p.stats) p.stats += first * p.parts;
+  if (p.keys) p.keys += first * p.parts * p.top_k;
+  return p;
+}
+
 template <bool F32>
-int run_scores(const ScoreParams& p, int ept, hipStream_t s) {
+int run_scores(const ScoreParams& all, int ept, hipStream_t s) {
+  const long count = launch_row_count(all.parts);
+  if (all.rows > count) {
+    for (long first = 0; first < all.rows; first += count)
+      if (int rc = run_scores<F32>(some_rows(all, first, count, F32), ept, s)) return rc;
+    return kOk;
+  }
+  const ScoreParams& p = all;
   if (ept == kSmallEpt) launch_rows<F32, kSmallEpt>(p, s);
   else launch_rows<F32, kLargeEpt>(p, s);
   if (int rc = hip_check(hipGetLastError(), "token score launch")) return rc;
@@ -117,14 +145,19 @@ extern "C" int ws_token_scores_backward(const void* logits, int64_t ld, int f32,
   const long size = f32 ? 4 : 2, span = ((rows - 1) * ld + vocab) * size, dspan = ((rows - 1) * ld_out + vocab) * size;
   const bool in_place = x < dx + dspan && dx < x + span;
   const int segments = in_place ? 1 : cdiv(vocab, 2048);
-  const dim3 grid((unsigned)(rows * segments));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (f32)
-    hipLaunchKernelGGL((score_grad_kernel<true>), grid, dim3(256), 0, s, p, dlogprob, dentropy, dlogits,
-                       (long)ld_out, segments);
-  else
-    hipLaunchKernelGGL((score_grad_kernel<false>), grid, dim3(256), 0, s, p, dlogprob, dentropy, dlogits,
-                       (long)ld_out, segments);
+  const long count = launch_row_count(segments);
+  for (long first = 0; first < rows; first += count) {
+    const ScoreParams q = some_rows(p, first, count, f32);
+    const float* g = dlogprob ? dlogprob + first : nullptr;
+    const float* h = dentropy ? dentropy + first : nullptr;
+    void* out = static_cast<char*>(dlogits) + first * ld_out * size;
+    const dim3 grid((unsigned)((long)q.rows * segments));
+    if (f32)
+      hipLaunchKernelGGL((score_grad_kernel<true>), grid, dim3(256), 0, s, q, g, h, out, (long)ld_out, segments);
+    else
+      hipLaunchKernelGGL((score_grad_kernel<false>), grid, dim3(256), 0, s, q, g, h, out, (long)ld_out, segments);
+  }
   return hip_check(hipGetLastError(), "token score gradient launch");
 }
 
@@ -137,6 +170,8 @@ int check_head(const void* hidden, long ld_hidden, const void* weight, long ld_w
   if (!hidden || !weight || !tokens) return set_error(kInvalid, "null operand pointer");
   if (rows < 1 || vocab < 1 || d < 1 || !fits_i32(rows) || !fits_i32(vocab) || !fits_i32(d))
     return set_error(kInvalid, "invalid LM-head sizes rows=%ld vocab=%ld d=%ld", rows, vocab, d);
+  // (64 threads a row join its parts, in one launch of fewer than 2^32.)
+  if (rows >= 1L << 26) return set_error(kInvalid, "too many rows for one launch");
   if (ld_hidden < d || ld_weight < d) return set_error(kInvalid, "leading dimension < d");
   if (!good_inv_t(inv_t)) return set_error(kInvalid, "the temperature must lie between 4.4e-39 and 8.5e37");
   p = GemmParams{};
