@@ -236,7 +236,7 @@ std::tuple<Tensor, Tensor> linear_backward(const Tensor& grad_in, const Tensor& 
   if (!want_w) return {dx, at::empty({0}, dw_options)};
   Tensor dw = at::empty({n, k}, dw_options);
   if (master) {
-    // fused_execution.mm_f32 of grad^T and x, FP32 sums unrounded.
+    // fused_execution.mm_f32_group of grad^T and x, FP32 sums unrounded.
     c10::DeviceGuard guard(grad.device());
     const ws_accumulate_problem item{grad.const_data_ptr(), 1, n, x.const_data_ptr(), x.stride(0), x.stride(1),
                                      dw.data_ptr<float>(), k, n, k};

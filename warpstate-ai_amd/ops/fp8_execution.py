@@ -27,7 +27,7 @@ import torch
 from torch.autograd import forward_ad
 
 from ops import _hip
-from ops.fused_execution import mm_f32
+from ops.fused_execution import mm_f32_group
 
 BF16, F32 = torch.bfloat16, torch.float32
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -326,7 +326,8 @@ def _fp8_linear_backward(grad: Tensor, x: Tensor, qt: Tensor, qt_scale: Tensor, 
     if want_x:
         _mm_buffers(g, g_scale, 1, wt, wt_scale, BLOCK, e8m0, dx, n)
     if want_w and master:
-        return dx, mm_f32(grad.T, x, round_bf16=False)
+        # The entry point that the native kernel calls, so that sums are taken in one order.
+        return dx, mm_f32_group([(grad.T, x)], round_bf16=False)[0]
     dw = torch.empty((n, k) if want_w else (0,), dtype=F32 if master else BF16, device=grad.device)
     if want_w:
         _mm_buffers(gt, gt_scale, 1, qt, qt_scale, 1, e8m0, dw, m)
@@ -377,7 +378,7 @@ def fp8_linear(x: Tensor, weight: Tensor, scale_dtype: torch.dtype = E8M0) -> Te
     r(q(dy)^T q(x)) with both operands quantized by columns; a step then keeps one byte per
     element of x and of W for the backward. An FP32 master's gradient is FP32, and the 8-bit
     matrix instruction's sums are not (``fp8_mm``): it is dy^T x of the BF16 tensors with FP32
-    sums (``mm_f32``), from x itself. First derivatives by
+    sums (``mm_f32_group``), from x itself. First derivatives by
     reverse mode only (forward-mode tensors and functorch's derivatives are refused)."""
     if x.dtype != BF16:
         raise ValueError("An 8-bit projection takes BF16 activations")
