@@ -16,8 +16,9 @@
 // a row go to lane l: the k order is another than the instruction's own, but the same for
 // both operands, and a block has one scale.
 //
-// Rates (the 256 x 256 tile, e8m0 / FP32 scales, B in blocks): 8192 x 10240 x 2048 138 / 164 us
-// (2.5 / 2.1 PFLOP/s), 16384 x 2048 x 11264 246 / 310 us (3.1 / 2.4), where BF16 products reach
+// Rates (the 256 x 256 tile, e8m0 / FP32 scales, B in blocks, one product in a loop): 8192 x 10240 x
+// 2048 141 / 171 us (2.4 / 2.0 PFLOP/s), 16384 x 2048 x 11264 241 / 309 us (3.1 / 2.4; 2.6 to 2.8 under
+// e8m0 in the clock that a training step's other products leave), where BF16 products reach
 // 1.4 to 1.5 and the instruction alone, in a loop on registers, 4.6. Between the two stand the
 // chain of a k-tile (fragment reads behind a barrier, then the MFMAs), the epilogue (about 4 us
 // a tile, a fifth of one with 16 k-tiles) and the clock under load.
@@ -25,7 +26,8 @@
 // Scales. e8m0: the instruction's own block scales (v_mfma_scale), no arithmetic beside it. A
 // lane gives the scale byte of its operand row; a dword holds the four bytes of four k-tiles, and is
 // shifted by one byte per k-tile. FP32: the block's product starts from zero, and
-// acc = fma(product, sA * sB, acc), four FP32 operations per MFMA beside it.
+// acc = fma(product, sA * sB, acc), four FP32 operations per MFMA beside it; sA * sB has to be in
+// FP32's range.
 #pragma once
 
 #include "gemm_ring.h"

@@ -7,9 +7,10 @@
 //   FP32: r(a r(1 / 448)), a = max(amax, 2^-100),
 // and q = rne(x * factor): 1 / scale exactly under e8m0; under FP32 r(448 r(1 / a)), within
 // 2^-23 of 448 / a, so that x * factor is at most 448 (1 + 2^-22), which rounds to 448. A block
-// with an infinity or a NaN gets the e8m0 NaN (255) or the FP32 scale inf / NaN, and its
-// infinities and NaNs become NaN (all of the block under e8m0). Magnitudes are compared as
-// integers, which ranks NaN above infinity above every number, so none is lost in the max.
+// with an infinity or a NaN gets the e8m0 NaN (255) or the FP32 scale inf / NaN, so that all of it
+// dequantizes to NaN (beside an infinity the FP32 factor is 0, and 0 times inf is NaN). Magnitudes
+// are compared as integers, which ranks NaN above infinity above every number, so none is lost in the
+// max.
 //
 // HBM-bound: x is read once (2 or 4 bytes an element), every form wanted of it written once
 // (1 byte each). 16384 x 5632 BF16 by rows and columns takes 82 us, 4.5 TB/s (the card copies at

@@ -99,8 +99,8 @@ __device__ __forceinline__ void score_finish(const ScoreOut& o, long row, const 
 // built for: 4096 x 32768 with the top 20 took 128 us while every logit's 64-bit key was formed
 // and compared in 121 registers, 125 with 112 bytes of scratch for a call, 83 inlined, 78 with the
 // 64 groups for k up to 32 (a quarter of the comparisons for a few more candidates: k = 32 90.6 ->
-// 87.7, k = 48 99.4 -> 104.4), 80 with distances taken before they are scaled. Of that the sums take
-// 67 (no top, 4.0 TB/s).
+// 87.7, k = 48 99.4 -> 104.4), 80 with distances taken before they are scaled, an operation more for
+// each logit. Of that the sums take 70 (no top, 3.8 TB/s; 67 while logits were scaled first).
 constexpr int kScoreGroups = 64;
 constexpr int kMaxTopK = kScoreGroups;
 constexpr int kScoreCandidates = 2048, kScoreWaveCandidates = kScoreCandidates / 4;

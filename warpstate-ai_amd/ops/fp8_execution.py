@@ -120,7 +120,7 @@ def quantize_rows(x: Tensor, scale_dtype: torch.dtype = E8M0) -> tuple[Tensor, T
     q times its block's scale is x to e4m3's precision. The scale of a block with largest
     magnitude amax is the least power of two 2^e >= amax / 448 (e >= -126), or
     max(amax, 2^-100) / 448 in FP32. A block that holds an infinity or a NaN dequantizes to
-    NaN there (everywhere under e8m0). The block's zeros stay zeros."""
+    NaN, all of it. Another block's zeros stay zeros."""
     native = _hip.host_ops()
     if native is not None and x.is_cuda and scale_dtype in _SCALE_TYPES:
         return native.native_quantize_rows(x.detach() if x.requires_grad else x,
@@ -241,7 +241,11 @@ def fp8_mm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor,
     about 1e-4 of the result's size for random operands, a twentieth of its BF16 rounding. That is why
     there is no FP32 result. ``out`` (BF16, unit column stride) receives the result instead of
     a new tensor. Operands in other layouts than rows of whole 16-byte pieces, and scales in
-    other layouts than ``quantize_rows`` gives, are copied first. No gradient is recorded."""
+    other layouts than ``quantize_rows`` gives, are copied first: on every call, for a reduction
+    that is no multiple of 16 (one row through 2048 x 5632 takes 12.6 us, through 2048 x 5624 27; through
+    11264 x 2040 42). A program that multiplies by one weight many times pads its reduction with
+    zeros before ``quantize_weight``. FP32 scales' products have to be in FP32's range. No gradient
+    is recorded."""
     native = _hip.host_ops()
     if native is not None and out is None and a.is_cuda:
         return native.native_fp8_mm(a, a_scale, b, b_scale)
@@ -378,8 +382,11 @@ def fp8_linear(x: Tensor, weight: Tensor, scale_dtype: torch.dtype = E8M0) -> Te
     r(q(dy)^T q(x)) with both operands quantized by columns; a step then keeps one byte per
     element of x and of W for the backward. An FP32 master's gradient is FP32, and the 8-bit
     matrix instruction's sums are not (``fp8_mm``): it is dy^T x of the BF16 tensors with FP32
-    sums (``mm_f32_group``), from x itself. First derivatives by
-    reverse mode only (forward-mode tensors and functorch's derivatives are refused)."""
+    sums (``mm_f32_group``), from x itself, which costs several times as much where N or K is no
+    multiple of 8 (4096 rows, forward and gradients: 1280 x 4480 156 us, 1285 x 4477 603).
+
+    First derivatives by reverse mode only (forward-mode tensors and functorch's derivatives are
+    refused)."""
     if x.dtype != BF16:
         raise ValueError("An 8-bit projection takes BF16 activations")
     if x.ndim < 1 or weight.ndim != 2 or x.shape[-1] != weight.shape[1]:

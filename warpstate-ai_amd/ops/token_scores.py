@@ -240,7 +240,8 @@ def linear_token_scores(hidden: Tensor, weight: Tensor, tokens: Tensor, temperat
     The logits are FP32 and never leave the registers. The backward recomputes them
     ``chunk_rows`` rows at a time (None: as many as 1 GiB of BF16 gradients holds); their
     gradient is rounded to BF16 once for the two products, whose sums are FP32, and so is the
-    weight's gradient over all chunks; both gradients come in their operand's type. Its
+    weight's gradient over all chunks. Both gradients come in their operand's type, the hidden
+    state's with BF16 precision in either (it is the gradient of the rounded operand). Its
     probabilities are off by up to 2^-24 of the row's log-sum-exp, as the FP32 logits are. Under
     torch.compile it runs eagerly (a graph break)."""
     if not (hidden.is_cuda and weight.is_cuda):
