@@ -58,9 +58,10 @@ Fp8Plan fp8_plan(long m, long n, long k, bool brow, int scale_type) {
   // the columns fill the card with tiles (16 rows) or with workgroups of 16 columns (32 rows,
   // a reduction that eight waves share in few steps). us of e8m0 products, few rows' kernel /
   // the best tile: 16 x 8192 x 2048 7.5 / 9.6, 16 x 16384 x 2048 12.3 / 9.9, 32 x 4096 x 2048 6.1 /
-  // 8.5, 32 x 6144 x 2048 10.4 / 9.4, 32 x 2048 x 5632 11.7 / 13.0, 32 x 2048 x 11264 21.1 / 15.8. Up to
-  // 16 rows the rule does not ask for K: 16 x 2048 x 5632 8.9 / 12.3, x 8192 12.5 / 11.9, x 11264 14.6 /
-  // 14.8, x 16384 22.0 / 17.5, 8 rows x 16384 18.0 / 17.2, one row x 16384 13.0 / 17.1.
+  // 8.5, 32 x 6144 x 2048 10.4 / 9.4, 32 x 2048 x 5632 11.7 / 13.0, 32 x 2048 x 8192 17.7 / 12.5 (the
+  // rule's edge), 32 x 2048 x 11264 21.1 / 15.8. Up to 16 rows the rule does not ask for K:
+  // 16 x 2048 x 5632 8.9 / 12.3, x 8192 12.5 / 11.9, x 11264 14.6 / 14.8, x 16384 22.0 / 17.5, 8 rows
+  // x 16384 18.0 / 17.2, one row x 16384 13.0 / 17.1.
   if (m <= 16 ? cdiv(n, 64) < cus : m <= 32 && cdiv(n, 16) <= cus && k <= 8192) return best;
   float t = 1e30f;
   for (int tile = 0; tile < kFastTiles; ++tile) {
