@@ -265,7 +265,8 @@ def fp8_mm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor,
         raise ValueError("out must have a unit column stride")
     dtype = a_scale.dtype
     sa, ld_sa, rows_a = _scale(a_scale, a, dtype, False, "a_scale")
-    sb, ld_sb, rows_b = _scale(b_scale, b, dtype, b_scale.shape[0] == n, "b_scale")
+    by_rows = b_scale.ndim == 2 and b_scale.shape[0] == n
+    sb, ld_sb, rows_b = _scale(b_scale, b, dtype, by_rows, "b_scale")
     a, b = _operand(a), _operand(b)
     wide = _ceil(k, 16)
     _launch(a, a.stride(0) if m > 1 else wide, sa, ld_sa, rows_a, b, b.stride(0) if n > 1 else wide,
