@@ -1,5 +1,6 @@
 """Token scores at the edges of what their documentation allows: tokens without a score under
-masked losses, the smallest and largest temperatures, more rows than one launch takes (GPU)."""
+masked losses, the smallest and largest temperatures, more rows than one launch takes,
+chunks past 32 bits (GPU)."""
 import pytest
 import torch
 
@@ -103,3 +104,19 @@ def test_more_rows_than_one_launch_takes(dtype):
         for a, b in zip(got, alone):
             assert torch.equal(a[part], b)
         assert torch.equal(dx[part], want) and bool(want.any())
+
+
+def test_chunks_past_32_bits_are_refused_before_the_forward():
+    """With gradients; without them, chunk_rows is not used."""
+    ts = _scores()
+    rows, vocab = 70000, 32768
+    hidden = torch.ones((rows, 8), device="cuda", dtype=BF16)
+    weight = torch.zeros((vocab, 8), device="cuda", dtype=BF16)
+    tokens = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="chunk_rows times the vocabulary"):
+        ts.linear_token_scores(hidden.requires_grad_(True), weight, tokens, 1.0, rows)
+    logprob, _ = ts.linear_token_scores(hidden.detach(), weight, tokens, 1.0, rows)
+    assert torch.allclose(logprob, torch.full_like(logprob, -15 * 0.6931472))
+    logprob, _ = ts.linear_token_scores(hidden, weight, tokens, 1.0, 65000)
+    dh, = torch.autograd.grad(logprob.sum(), [hidden])
+    assert not bool(dh.any())

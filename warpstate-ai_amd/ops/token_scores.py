@@ -40,6 +40,7 @@ Tensor = torch.Tensor
 # it (scores and gradients of 16384 rows, us, chunks of 8192 / 16384: 2048 over 32768 6426 /
 # 6240, 512 over 4096 610 / 399).
 CHUNK_LOGITS = 1 << 29
+MAX_CHUNK = 2 ** 31 - 1
 MAX_TOP_K = 64
 MAX_VOCAB = 524288
 # 1 / temperature: a normal FP32 number, and finite times log2 e.
@@ -255,6 +256,13 @@ def linear_token_scores(hidden: Tensor, weight: Tensor, tokens: Tensor, temperat
         chunk_rows = max(256, CHUNK_LOGITS // weight.shape[0] // 256 * 256)
     if chunk_rows < 1:
         raise ValueError("chunk_rows must be positive")
+    # (What the backward would refuse: a chunk's rows of logit gradients, padded to whole pieces.)
+    chunk, vocab = min(chunk_rows, hidden.shape[0]), weight.shape[0]
+    row = -(-vocab // 64) * 64 if vocab % 8 else vocab
+    if (chunk * row >= MAX_CHUNK and torch.is_grad_enabled()
+            and (hidden.requires_grad or weight.requires_grad)):
+        raise ValueError(f"chunk_rows times the vocabulary must be less than {MAX_CHUNK}, not "
+                         f"{chunk} x {row}")
     tokens = _check_tokens(tokens, hidden.shape[0], hidden.device)
     native = _hip.host_ops()
     scores = _LinearTokenScores.apply if native is None else native.native_head_scores
