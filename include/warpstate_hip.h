@@ -475,6 +475,52 @@ int ws_linear_token_scores_backward(const void* hidden, int64_t ld_hidden, const
                                     void* dhidden, int64_t ld_dhidden, void* dweight,
                                     int64_t ld_dweight, int dweight_bf16, void* stream);
 
+/* --- residual norm ---------------------------------------------------------------------
+ *
+ * s = r(x + residual) in the residual stream's type (BF16, or FP32 with stream_f32), then the
+ * RMSNorm of the rounded s: y = s rstd w, rstd = 1 / sqrt(mean(s^2) + eps), rounded once. x is BF16,
+ * the weight FP32; rows of 1 to 8192 columns, row strides in elements, outputs contiguous.
+ */
+
+/* y [rows, d] BF16, stream_out [rows, d] = s, rstd [rows]. */
+int ws_add_rmsnorm(const void* x, int64_t ldx, const void* residual, int64_t ld_residual,
+                   int stream_f32, const float* weight, float eps, int64_t rows, int64_t d, void* y,
+                   void* stream_out, float* rstd, void* stream);
+/* The unrounded y quantized by rows (WS_QUANT_ROWS of ws_fp8_quantize): q, ldq, scale and
+ * ld_scale as there. With a null residual s is x and stream_out is null. */
+int ws_rmsnorm_quantize(const void* x, int64_t ldx, const void* residual, int64_t ld_residual,
+                        int stream_f32, const float* weight, float eps, int64_t rows, int64_t d,
+                        int scale_type, void* q, int64_t ldq, void* scale, int64_t ld_scale,
+                        void* stream_out, void* stream);
+/* With stream_in [rows, d] = s and the forward's rstd, dy BF16 and dstream (nullable: zero) in the
+ * stream's type: dx [rows, d] BF16, the gradient of x and of a BF16 residual; dresidual (nullable)
+ * the same in FP32 for an FP32 stream; dweight [d]. `partial`: ws_add_rmsnorm_backward_partial_floats
+ * (which follows the device's compute units). */
+int64_t ws_add_rmsnorm_backward_partial_floats(int64_t rows, int64_t d);
+int ws_add_rmsnorm_backward(const void* stream_in, int stream_f32, const float* weight,
+                            const float* rstd, const void* dy, int64_t ld_dy, const void* dstream,
+                            int64_t ld_dstream, int64_t rows, int64_t d, void* dx, float* dresidual,
+                            float* dweight, float* partial, void* stream);
+
+/* --- embedding -------------------------------------------------------------------------
+ *
+ * y [rows, d] (BF16, or FP32 with y_f32) = scale * table[token] from a BF16 or FP32 table [vocab,
+ * d] (row stride ld_table). A token of -100 is ignored: its row is zeros. Any other token outside
+ * [0, vocab) gets NaN. Up to 33554430 rows of the table and 67108860 tokens.
+ */
+int ws_embedding(const void* table, int64_t ld_table, int table_f32, const int64_t* tokens,
+                 int64_t rows, int64_t vocab, int64_t d, float scale, void* y, int y_f32,
+                 void* stream);
+/* dtable [vocab, d] = scale * the sums of dy's rows (BF16, or FP32 with dy_f32) by token, FP32 in
+ * the order of the rows: the same bits on every call. Written in BF16 or FP32, or added to FP32
+ * values that are there (rows without tokens then stay as they are, unread). Tokens outside the
+ * vocabulary, ignored ones among them, take no part. `workspace`: 16-byte aligned. */
+enum WsEmbedGrad { WS_EMBED_WRITE_BF16 = 0, WS_EMBED_WRITE_F32 = 1, WS_EMBED_ADD_F32 = 2 };
+int64_t ws_embedding_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d);
+int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, const int64_t* tokens,
+                          int64_t rows, int64_t vocab, int64_t d, float scale, void* dtable,
+                          int64_t ld_dtable, int mode, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,89 @@
+"""What the residual norm and the embedding refuse, in Python and at the C entry points (CPU)."""
+import pytest
+import torch
+
+from ops import _hip
+
+BF16, F32 = torch.bfloat16, torch.float32
+GPU = 1 << 20  # a pointer that is never read: every call below fails its checks first
+
+
+def test_cpu_tensors_are_refused():
+    from ops.embedding_execution import embedding, embedding_accumulate_
+    from ops.residual_norm import add_rmsnorm, rmsnorm_quantize
+
+    x, w = torch.zeros((2, 8), dtype=BF16), torch.ones(8)
+    t = torch.zeros(2, dtype=torch.int64)
+    for call in (lambda: add_rmsnorm(x, x, w), lambda: rmsnorm_quantize(x, w),
+                 lambda: embedding(t, x), lambda: embedding_accumulate_(x.float(), t, x)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(rows=-1), "shape"), (dict(d=0), "shape"), (dict(d=8193), "8192"), (dict(x=None), "null"),
+    (dict(residual=None), "null"), (dict(w=None), "null"), (dict(y=None), "null"),
+    (dict(out=None), "null"), (dict(rstd=None), "null"), (dict(ldx=7), "overlap"),
+    (dict(ldr=7), "overlap"), (dict(rows=2 ** 31), "shape")])
+def test_add_rmsnorm_arguments(change, match):
+    a = dict(x=GPU, ldx=8, residual=GPU, ldr=8, w=GPU, rows=4, d=8, y=GPU, out=GPU, rstd=GPU) | change
+    with pytest.raises(RuntimeError, match=match):
+        _hip.call("ws_add_rmsnorm", a["x"], a["ldx"], a["residual"], a["ldr"], 0, a["w"], 1e-5, a["rows"],
+                  a["d"], a["y"], a["out"], a["rstd"], None)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(d=8193), "8192"), (dict(scale_type=2), "scale type"), (dict(q=None), "null"),
+    (dict(out=None), "null"), (dict(residual=None), "null"), (dict(ldq=24), "16-byte"),
+    (dict(q=GPU + 8), "16-byte"), (dict(ldq=0), "16-byte"), (dict(ld_scale=1, d=129, ldx=130, ldr=130, ldq=144),
+                                                             "overlap"),
+    (dict(scale_type=1, ld_scale=3), "overlap")])
+def test_rmsnorm_quantize_arguments(change, match):
+    a = dict(x=GPU, ldx=8, residual=GPU, ldr=8, w=GPU, rows=4, d=8, scale_type=0, q=GPU, ldq=16,
+             scale=GPU, ld_scale=4, out=GPU) | change
+    with pytest.raises(RuntimeError, match=match):
+        _hip.call("ws_rmsnorm_quantize", a["x"], a["ldx"], a["residual"], a["ldr"], 0, a["w"], 1e-5,
+                  a["rows"], a["d"], a["scale_type"], a["q"], a["ldq"], a["scale"], a["ld_scale"],
+                  a["out"], None)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(rows=0), "shape"), (dict(d=8193), "8192"), (dict(s=None), "null"), (dict(dy=None), "null"),
+    (dict(partial=None), "null"), (dict(dresidual=GPU), "BF16 stream"), (dict(ld_dy=7), "overlap"),
+    (dict(ds=GPU, ld_ds=7), "overlap")])
+def test_add_rmsnorm_backward_arguments(change, match):
+    a = dict(s=GPU, w=GPU, rstd=GPU, dy=GPU, ld_dy=8, ds=None, ld_ds=0, rows=4, d=8, dx=GPU,
+             dresidual=None, dw=GPU, partial=GPU) | change
+    with pytest.raises(RuntimeError, match=match):
+        _hip.call("ws_add_rmsnorm_backward", a["s"], 0, a["w"], a["rstd"], a["dy"], a["ld_dy"], a["ds"],
+                  a["ld_ds"], a["rows"], a["d"], a["dx"], a["dresidual"], a["dw"], a["partial"], None)
+
+
+def test_partial_floats_of_bad_sizes():
+    assert _hip.query("ws_add_rmsnorm_backward_partial_floats", 0, 8) == 0
+    assert _hip.query("ws_add_rmsnorm_backward_partial_floats", 4, 8193) == 0
+    assert _hip.query("ws_embedding_backward_workspace_bytes", -1, 8, 8) == 0
+    assert _hip.query("ws_embedding_backward_workspace_bytes", 8, 2 ** 31, 8) == 0
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(rows=-1), "shape"), (dict(vocab=0), "shape"), (dict(d=0), "shape"), (dict(table=None), "null"),
+    (dict(tokens=None), "null"), (dict(y=None), "null"), (dict(ld=7), "overlap"),
+    (dict(rows=2 ** 27), "shape"), (dict(vocab=2 ** 26), "shape")])
+def test_embedding_arguments(change, match):
+    a = dict(table=GPU, ld=8, tokens=GPU, rows=4, vocab=10, d=8, y=GPU) | change
+    with pytest.raises(RuntimeError, match=match):
+        _hip.call("ws_embedding", a["table"], a["ld"], 0, a["tokens"], a["rows"], a["vocab"], a["d"], 1.0,
+                  a["y"], 0, None)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(rows=-1), "shape"), (dict(vocab=0), "shape"), (dict(mode=3), "mode"), (dict(mode=-1), "mode"),
+    (dict(dy=None), "null"), (dict(tokens=None), "null"), (dict(out=None), "null"),
+    (dict(work=None), "null"), (dict(work=GPU + 4), "aligned"), (dict(ld_dy=7), "overlap"),
+    (dict(ld=7), "overlap")])
+def test_embedding_backward_arguments(change, match):
+    a = dict(dy=GPU, ld_dy=8, tokens=GPU, rows=4, vocab=10, d=8, out=GPU, ld=8, mode=0, work=GPU) | change
+    with pytest.raises(RuntimeError, match=match):
+        _hip.call("ws_embedding_backward", a["dy"], a["ld_dy"], 0, a["tokens"], a["rows"], a["vocab"],
+                  a["d"], 1.0, a["out"], a["ld"], a["mode"], a["work"], None)

@@ -1,6 +1,6 @@
 """Compile ``csrc/*.hip`` for gfx950 into ``lib/libwarpstate_hip.so``, the operators' host-side
 autograd kernels (``csrc/autograd.cpp``) into ``lib/libwarpstate_autograd.so`` and the host side
-of the 8-bit projections and token scores (``csrc/host_ops.cpp``) into
+of the operators beside the BF16 path (``csrc/host_ops.cpp``, ``csrc/host_layer.cpp``) into
 ``lib/libwarpstate_host.so``.
 
 Every translation unit is compiled on each call (in parallel), then linked into a fresh
@@ -47,6 +47,9 @@ def _compile(source: Path) -> Path:
     return obj
 
 
+HOST_SOURCES = [CSRC / "host_ops.cpp", CSRC / "host_layer.cpp"]
+
+
 def autograd_command(source: Path, target: Path) -> list[str]:
     """The host compiler's command for the C++ autograd kernels: PyTorch's headers, no device
     code."""
@@ -67,20 +70,21 @@ def _build_autograd() -> Path:
     return AUTOGRAD
 
 
-def host_command(source: Path, target: Path) -> list[str]:
+def host_command(sources: list[Path], target: Path) -> list[str]:
     """The host compiler's command for the C++ operators: PyTorch's and HIP's headers, linked
     to the kernels' library beside it."""
-    return [*autograd_command(source, target), "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+    first, *others = sources
+    return [*autograd_command(first, target), *map(str, others), "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
             f"-I{ROCM}/include", "-lc10_hip", f"-L{LIBRARY.parent}", f"-l:{LIBRARY.name}",
             "-Wl,-rpath,$ORIGIN"]
 
 
 def _build_host() -> Path:
     staging = HOST.with_name(HOST.name + ".tmp")
-    cmd = host_command(CSRC / "host_ops.cpp", staging)
+    cmd = host_command(HOST_SOURCES, staging)
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
-        raise RuntimeError(f"{CXX} failed for host_ops.cpp:\n{result.stderr}")
+        raise RuntimeError(f"{CXX} failed for the C++ operators:\n{result.stderr}")
     os.replace(staging, HOST)
     return HOST
 

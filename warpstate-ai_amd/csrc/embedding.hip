@@ -1,0 +1,117 @@
+// C ABI: embedding lookup and the table's gradient.
+#include "../../include/warpstate_hip.h"
+#include "embedding.h"
+#include "launch.h"
+
+using namespace ws;
+
+namespace {
+
+// Workgroups of 256 threads in one launch, which has fewer than 2^32 threads.
+constexpr int64_t kMostGroups = 1L << 24;
+
+int check_table(int64_t rows, int64_t vocab, int64_t d, int64_t ld) {
+  if (rows < 0 || vocab < 1 || d < 1 || rows > 4 * (kMostGroups - 1) || vocab > 2 * (kMostGroups - 1) || !fits_i32(d))
+    return set_error(kInvalid, "invalid embedding shape (%ld tokens, %ld x %ld)", (long)rows, (long)vocab, (long)d);
+  if (vocab > 1 && ld < d) return set_error(kInvalid, "rows overlap");
+  return kOk;
+}
+bool pieces(const void* p, long ld, int bytes) { return al(p, 16) && ld * bytes % 16 == 0; }
+
+// Positions of one piece of a token that occurs more often: 32, or as many as leave 1024 pieces.
+int64_t piece_rows(int64_t rows) { return rows <= 32 * 1024 ? 32 : (rows + 1023) / 1024; }
+
+struct GradLayout {
+  int64_t piece, pieces, start, perm, partial, bytes, ld_partial;
+};
+GradLayout grad_layout(int64_t rows, int64_t vocab, int64_t d) {
+  auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+  GradLayout l;
+  l.piece = piece_rows(rows);
+  l.pieces = rows > l.piece ? (rows + l.piece - 1) / l.piece : 0;  // otherwise no token occurs more often
+  l.ld_partial = (d + 7) / 8 * 8;
+  l.start = 0;
+  l.perm = up(4 * (vocab + 1));
+  l.partial = l.perm + up(4 * rows);
+  l.bytes = l.partial + up(8 * l.pieces * l.ld_partial);
+  return l;
+}
+
+template <bool GF32, int OUT>
+int launch_grad(const EmbedGradParams& p, bool vec, hipStream_t s) {
+  const dim3 grid((unsigned)cdiv((long)p.pieces + p.vocab, 4)), block(256);
+  if (vec) hipLaunchKernelGGL((embed_grad_kernel<GF32, OUT, true>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((embed_grad_kernel<GF32, OUT, false>), grid, block, 0, s, p);
+  if (int rc = hip_check(hipGetLastError(), "embedding gradient launch")) return rc;
+  if (p.pieces == 0) return kOk;
+  const dim3 join(p.pieces, cdiv(p.d, 2048));
+  if (vec) hipLaunchKernelGGL((embed_join_kernel<OUT, true>), join, block, 0, s, p);
+  else hipLaunchKernelGGL((embed_join_kernel<OUT, false>), join, block, 0, s, p);
+  return hip_check(hipGetLastError(), "embedding gradient join launch");
+}
+
+}  // namespace
+
+extern "C" int ws_embedding(const void* table, int64_t ld_table, int table_f32, const int64_t* tokens, int64_t rows,
+                            int64_t vocab, int64_t d, float scale, void* y, int y_f32, void* stream) {
+  if (int rc = check_table(rows, vocab, d, ld_table)) return rc;
+  if (rows == 0) return kOk;
+  if (!table || !tokens || !y) return set_error(kInvalid, "null pointer");
+  const bool vec = d % 8 == 0 && pieces(table, ld_table, table_f32 ? 4 : 2) && al(y, 16);
+  auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(cdiv(rows, 4)), dim3(256), 0, static_cast<hipStream_t>(stream), table,
+                       (long)ld_table, reinterpret_cast<const long*>(tokens), (int)rows, (int)vocab, (int)d, scale, y);
+    return hip_check(hipGetLastError(), "embedding launch");
+  };
+  if (table_f32)
+    return y_f32 ? (vec ? run(&embed_lookup_kernel<true, true, true>) : run(&embed_lookup_kernel<true, true, false>))
+                 : (vec ? run(&embed_lookup_kernel<true, false, true>) : run(&embed_lookup_kernel<true, false, false>));
+  return y_f32 ? (vec ? run(&embed_lookup_kernel<false, true, true>) : run(&embed_lookup_kernel<false, true, false>))
+               : (vec ? run(&embed_lookup_kernel<false, false, true>) : run(&embed_lookup_kernel<false, false, false>));
+}
+
+extern "C" int64_t ws_embedding_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d) {
+  if (rows < 0 || vocab < 1 || d < 1 || !fits_i32(rows) || !fits_i32(vocab) || !fits_i32(d)) return 0;
+  return grad_layout(rows, vocab, d).bytes;
+}
+
+extern "C" int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, const int64_t* tokens, int64_t rows,
+                                     int64_t vocab, int64_t d, float scale, void* dtable, int64_t ld_dtable,
+                                     int mode, void* workspace, void* stream) {
+  if (int rc = check_table(rows, vocab, d, ld_dtable)) return rc;
+  if (mode < WS_EMBED_WRITE_BF16 || mode > WS_EMBED_ADD_F32) return set_error(kInvalid, "unknown gradient mode %d", mode);
+  if (!dtable || !workspace || (rows > 0 && (!dy || !tokens))) return set_error(kInvalid, "null pointer");
+  if (rows > 1 && ld_dy < d) return set_error(kInvalid, "rows overlap");
+  if (!al(workspace, 16)) return set_error(kInvalid, "the workspace must be 16-byte aligned");
+  const GradLayout l = grad_layout(rows, vocab, d);
+  char* const work = static_cast<char*>(workspace);
+  EmbedGradParams p{};
+  p.dy = dy;
+  p.ld_dy = ld_dy;
+  p.tokens = reinterpret_cast<const long*>(tokens);
+  p.start = reinterpret_cast<int*>(work + l.start);
+  p.perm = reinterpret_cast<int*>(work + l.perm);
+  p.vocab = (int)vocab;
+  p.d = (int)d;
+  p.scale = scale;
+  p.out = dtable;
+  p.ld_out = ld_dtable;
+  p.piece = (int)l.piece;
+  p.pieces = (int)l.pieces;
+  p.partial = reinterpret_cast<float*>(work + l.partial);
+  p.ld_partial = l.ld_partial;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  // A workgroup per compute unit, more where their ranges would pass the counters' space.
+  int64_t range = cdiv(vocab, device_cus());
+  if (range > kSortRange) range = kSortRange;
+  hipLaunchKernelGGL(embed_sort_kernel, dim3(cdiv(vocab, range)), dim3(64 * kSortWaves), 0, s, p.tokens, (int)rows,
+                     (int)vocab, (int)range, const_cast<int*>(p.start), const_cast<int*>(p.perm));
+  if (int rc = hip_check(hipGetLastError(), "embedding sort launch")) return rc;
+  const bool vec = d % 8 == 0 && pieces(dy, ld_dy, dy_f32 ? 4 : 2) && pieces(dtable, ld_dtable, mode == WS_EMBED_WRITE_BF16 ? 2 : 4);
+#define WS_GRAD(G_)                                                                                   \
+  (mode == WS_EMBED_WRITE_BF16  ? launch_grad<G_, kEmbedBF16>(p, vec, s)                              \
+   : mode == WS_EMBED_WRITE_F32 ? launch_grad<G_, kEmbedF32>(p, vec, s)                               \
+                                : launch_grad<G_, kEmbedAdd>(p, vec, s))
+  return dy_f32 ? WS_GRAD(true) : WS_GRAD(false);
+#undef WS_GRAD
+}

@@ -1,0 +1,308 @@
+// Host side of the residual norm and the embedding as PyTorch operators in C++: the checks,
+// allocations, launches and autograd nodes of ops/residual_norm.py and ops/embedding_execution.py
+// without Python. Shapes and types only on fake tensors.
+//
+// Autograd kernels read no data; they call operators below autograd. First derivatives by reverse
+// mode only: tensors that carry a tangent are refused, and so is a second differentiation.
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include <cmath>
+
+#include "host_common.h"
+
+namespace {
+
+typedef std::tuple<Tensor, Tensor> TwoTensors;
+typedef std::tuple<Tensor, Tensor, Tensor> ThreeTensors;
+
+// A tensor's rows of its last dimension, with a unit column stride and no overlap: a view or a copy.
+Tensor rows_of(const Tensor& t) {
+  const int64_t cols = t.size(-1);
+  Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / cols, cols});
+  const bool unit = (r.stride(1) == 1 || cols == 1) && (r.size(0) <= 1 || r.stride(0) >= cols);
+  return unit ? r : r.contiguous();
+}
+int64_t last(const Tensor& t) { return t.dim() ? t.size(-1) : 0; }
+
+// Gradients that are not differentiable again: where a graph of the backward is recorded, they
+// refuse it.
+variable_list once(variable_list grads, const variable_list& from, const char* message) {
+  bool recorded = false;
+  for (const auto& t : from) recorded |= t.defined() && t.requires_grad();
+  if (!at::GradMode::is_enabled() || !recorded) return grads;
+  variable_list known;
+  for (auto& g : grads)
+    if (g.defined()) known.push_back(g.detach().set_requires_grad(true));
+  auto node = std::make_shared<torch::autograd::DelayedError>(message, (int64_t)known.size());
+  known = (*node)(std::move(known));
+  size_t next = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = known[next++];
+  return grads;
+}
+
+// --- residual norm --------------------------------------------------------------------------
+
+constexpr int64_t kMaxWidth = 8192;
+constexpr char kNormTwice[] = "the residual norm cannot be differentiated twice";
+
+void check_norm(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight) {
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 && x.dim() >= 1, "Expected BF16 rows");
+  const int64_t d = x.size(-1);
+  TORCH_CHECK_VALUE(d >= 1 && d <= kMaxWidth, "RMSNorm takes rows of 1 to ", kMaxWidth, " columns, not ", d);
+  TORCH_CHECK_VALUE(weight.scalar_type() == at::kFloat && weight.dim() == 1 && weight.size(0) == d &&
+                        weight.device() == x.device(),
+                    "The norm's weight must be a vector of ", d, " values on ", x.device());
+  if (residual.has_value())
+    TORCH_CHECK_VALUE((residual->scalar_type() == at::kBFloat16 || residual->scalar_type() == at::kFloat) &&
+                          residual->sizes() == x.sizes() && residual->device() == x.device(),
+                      "The residual must be BF16 or FP32, of shape ", x.sizes(), " on ", x.device());
+}
+
+ThreeTensors add_rmsnorm_rstd(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
+  check_norm(x, residual, weight);
+  c10::DeviceGuard guard(x.device());
+  const Tensor a = rows_of(x), r = rows_of(residual), w = weight.contiguous();
+  const int64_t rows = a.size(0), d = a.size(1);
+  Tensor y = at::empty(x.sizes(), x.options()), stream = at::empty(x.sizes(), residual.options());
+  Tensor rstd = floats(x, {rows});
+  check(ws_add_rmsnorm(ptr(a), row_stride(a), ptr(r), row_stride(r), r.scalar_type() == at::kFloat,
+                       w.const_data_ptr<float>(), (float)eps, rows, d, ptr(y), ptr(stream), rstd.data_ptr<float>(),
+                       stream_of(x)),
+        "ws_add_rmsnorm");
+  return {y, stream, rstd};
+}
+TwoTensors add_rmsnorm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
+  auto [y, stream, rstd] = add_rmsnorm_rstd(x, residual, weight, eps);
+  return {y, stream};
+}
+// (dx, dresidual, dweight); dresidual is empty for a BF16 stream, whose gradient is dx.
+ThreeTensors add_rmsnorm_backward(const Tensor& stream, const Tensor& weight, const Tensor& rstd, const Tensor& dy,
+                                  const std::optional<Tensor>& dstream) {
+  c10::DeviceGuard guard(stream.device());
+  const bool f32 = stream.scalar_type() == at::kFloat;
+  Tensor dx = at::empty(stream.sizes(), dy.options()), dweight = at::empty_like(weight, at::MemoryFormat::Contiguous);
+  Tensor dresidual = f32 ? at::empty(stream.sizes(), stream.options()) : at::empty({0}, stream.options());
+  if (stream.numel() == 0) return {dx, dresidual, dweight.zero_()};
+  const Tensor s = rows_of(stream), g = rows_of(dy), w = weight.contiguous();
+  const Tensor h = dstream.has_value() ? rows_of(*dstream) : Tensor();
+  const int64_t rows = s.size(0), d = s.size(1);
+  Tensor partial = floats(stream, {ws_add_rmsnorm_backward_partial_floats(rows, d)});
+  check(ws_add_rmsnorm_backward(s.const_data_ptr(), f32, w.const_data_ptr<float>(), rstd.const_data_ptr<float>(),
+                                g.const_data_ptr(), row_stride(g), ptr(h), h.defined() ? row_stride(h) : 0, rows, d,
+                                dx.data_ptr(), f32 ? dresidual.data_ptr<float>() : nullptr, dweight.data_ptr<float>(),
+                                partial.data_ptr<float>(), stream_of(stream)),
+        "ws_add_rmsnorm_backward");
+  return {dx, dresidual, dweight};
+}
+
+struct AddRmsnormFn : Function<AddRmsnormFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& weight,
+                               double eps) {
+    typedef const Tensor& T;
+    static const auto op = find<ThreeTensors(T, T, T, double)>("warpstate::native_add_rmsnorm_rstd");
+    auto [y, stream, rstd] = below(op, x, residual, weight, eps);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({stream, weight, rstd});
+    return {y, stream};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    typedef const Tensor& T;
+    static const auto op =
+        find<ThreeTensors(T, T, T, T, const std::optional<Tensor>&)>("warpstate::native_add_rmsnorm_backward");
+    const Tensor &dy = grads[0], &dstream = grads[1];
+    if (!dy.defined())  // the addition alone
+      return {dstream.defined() ? dstream.to(at::kBFloat16) : Tensor(), dstream, Tensor(), Tensor()};
+    const auto s = ctx->get_saved_variables();
+    auto [dx, dresidual, dweight] =
+        below(op, s[0], s[1], s[2], dy, dstream.defined() ? std::optional<Tensor>(dstream) : std::nullopt);
+    const bool f32 = s[0].scalar_type() == at::kFloat;
+    return once({dx, f32 ? dresidual : dx, dweight, Tensor()}, {s[0], s[1], dy, dstream}, kNormTwice);
+  }
+};
+TwoTensors add_rmsnorm_autograd(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
+  refuse_tangents("add_rmsnorm", x, residual, weight);
+  if (!records(x, residual, weight)) {
+    typedef const Tensor& T;
+    static const auto op = find<TwoTensors(T, T, T, double)>("warpstate::native_add_rmsnorm");
+    return below(op, x, residual, weight, eps);
+  }
+  variable_list v = AddRmsnormFn::apply(x, residual, weight, eps);
+  return {v[0], v[1]};
+}
+TwoTensors add_rmsnorm_meta(const Tensor& x, const Tensor& residual, const Tensor& weight, double) {
+  check_norm(x, residual, weight);
+  return {at::empty(x.sizes(), x.options()), at::empty(x.sizes(), residual.options())};
+}
+ThreeTensors add_rmsnorm_rstd_meta(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
+  auto [y, stream] = add_rmsnorm_meta(x, residual, weight, eps);
+  return {y, stream, floats(x, {x.numel() / x.size(-1)})};
+}
+ThreeTensors add_rmsnorm_backward_meta(const Tensor& stream, const Tensor& weight, const Tensor&, const Tensor& dy,
+                                       const std::optional<Tensor>&) {
+  const bool f32 = stream.scalar_type() == at::kFloat;
+  return {at::empty(stream.sizes(), dy.options()),
+          f32 ? at::empty(stream.sizes(), stream.options()) : at::empty({0}, stream.options()),
+          at::empty_like(weight, at::MemoryFormat::Contiguous)};
+}
+
+// (q, scale, stream) of ops/residual_norm.py's rmsnorm_quantize, the stream empty without a residual.
+ThreeTensors rmsnorm_quantize(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight, double eps,
+                              bool e8m0) {
+  check_norm(x, residual, weight);
+  TORCH_CHECK_VALUE(x.numel() > 0, "Quantization takes non-empty rows");
+  c10::DeviceGuard guard(x.device());
+  const Tensor a = rows_of(x), w = weight.contiguous();
+  const Tensor r = residual.has_value() ? rows_of(*residual) : Tensor();
+  const int64_t rows = a.size(0), d = a.size(1), n = blocks(d);
+  Tensor q = at::empty({rows, up(d, 16)}, x.options().dtype(at::kFloat8_e4m3fn));
+  Tensor scale = e8m0 ? at::empty({rows, up(n, 4)}, x.options().dtype(at::kFloat8_e8m0fnu)) : floats(x, {n, up(rows, 4)});
+  Tensor stream = r.defined() ? at::empty(x.sizes(), r.options()) : at::empty({0}, x.options());
+  check(ws_rmsnorm_quantize(a.const_data_ptr(), row_stride(a), ptr(r), r.defined() ? row_stride(r) : 0,
+                            r.defined() && r.scalar_type() == at::kFloat, w.const_data_ptr<float>(), (float)eps, rows,
+                            d, e8m0 ? WS_SCALE_E8M0 : WS_SCALE_F32, q.data_ptr(), q.size(1), scale.data_ptr(),
+                            scale.size(1), r.defined() ? stream.data_ptr() : nullptr, stream_of(x)),
+        "ws_rmsnorm_quantize");
+  if (q.size(1) != d) q = q.narrow(1, 0, d);
+  if (!e8m0) return {q, scale.narrow(1, 0, rows).t(), stream};
+  return {q, scale.size(1) == n ? scale : scale.narrow(1, 0, n), stream};
+}
+ThreeTensors rmsnorm_quantize_autograd(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight,
+                                       double eps, bool e8m0) {
+  typedef const Tensor& T;
+  static const auto op =
+      find<ThreeTensors(T, const std::optional<Tensor>&, T, double, bool)>("warpstate::native_rmsnorm_quantize");
+  refuse_tangents("rmsnorm_quantize", x, residual.has_value() ? *residual : x, weight);
+  return below(op, x, residual, weight, eps, e8m0);
+}
+
+// --- embedding ------------------------------------------------------------------------------
+
+constexpr char kEmbeddingTwice[] = "the embedding cannot be differentiated twice";
+typedef Tensor Embedding(const Tensor&, const Tensor&, double, bool);
+
+void check_embedding(const Tensor& tokens, const Tensor& table, double scale) {
+  TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong && tokens.device() == table.device(),
+                    "Tokens must be int64 on the table's device");
+  TORCH_CHECK_VALUE((table.scalar_type() == at::kBFloat16 || table.scalar_type() == at::kFloat) && table.dim() == 2 &&
+                        table.numel() > 0,
+                    "Expected a non-empty BF16 or FP32 table [vocab, d]");
+  TORCH_CHECK_VALUE(std::isfinite(scale), "The scale must be finite, not ", scale);
+}
+std::vector<int64_t> embedded(const Tensor& tokens, int64_t d) {
+  std::vector<int64_t> sizes = tokens.sizes().vec();
+  sizes.push_back(d);
+  return sizes;
+}
+Tensor embedding(const Tensor& tokens_in, const Tensor& table_in, double scale, bool f32) {
+  check_embedding(tokens_in, table_in, scale);
+  c10::DeviceGuard guard(table_in.device());
+  const Tensor tokens = tokens_in.contiguous(), table = rows_of(table_in);
+  Tensor y = at::empty(embedded(tokens, table.size(1)), table.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+  check(ws_embedding(table.const_data_ptr(), row_stride(table), table.scalar_type() == at::kFloat,
+                     static_cast<const int64_t*>(ptr(tokens)), tokens.numel(), table.size(0), table.size(1),
+                     (float)scale, ptr(y), f32, stream_of(table)),
+        "ws_embedding");
+  return y;
+}
+// The sums of dy by token into `out` [vocab, d].
+void embedding_sums(const Tensor& dy, const Tensor& tokens_in, double scale, const Tensor& out, int mode) {
+  c10::DeviceGuard guard(out.device());
+  const Tensor tokens = tokens_in.contiguous();
+  const int64_t rows = tokens.numel(), vocab = out.size(0), d = out.size(1);
+  const Tensor g = rows ? rows_of(dy) : Tensor();
+  Tensor work = bytes(out, {ws_embedding_backward_workspace_bytes(rows, vocab, d)});
+  check(ws_embedding_backward(ptr(g), rows ? row_stride(g) : 0, rows && g.scalar_type() == at::kFloat,
+                              static_cast<const int64_t*>(ptr(tokens)), rows, vocab, d, (float)scale, out.data_ptr(),
+                              row_stride(out), mode, work.data_ptr(), stream_of(out)),
+        "ws_embedding_backward");
+}
+Tensor embedding_backward(const Tensor& dy, const Tensor& tokens, int64_t vocab, double scale, bool f32) {
+  c10::DeviceGuard guard(dy.device());
+  Tensor out = at::empty({vocab, dy.size(-1)}, dy.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+  embedding_sums(dy, tokens, scale, out, f32 ? WS_EMBED_WRITE_F32 : WS_EMBED_WRITE_BF16);
+  return out;
+}
+void embedding_accumulate(Tensor& gradient, const Tensor& tokens, const Tensor& dy, double scale) {
+  TORCH_CHECK_VALUE(gradient.scalar_type() == at::kFloat && gradient.dim() == 2 && gradient.numel() > 0 &&
+                        (gradient.stride(1) == 1 || gradient.size(1) == 1) &&
+                        (gradient.size(0) == 1 || gradient.stride(0) >= gradient.size(1)),
+                    "The gradient must be a non-empty FP32 matrix with a unit column stride");
+  TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong && tokens.device() == gradient.device(),
+                    "Tokens must be int64 on the gradient's device");
+  TORCH_CHECK_VALUE((dy.scalar_type() == at::kBFloat16 || dy.scalar_type() == at::kFloat) &&
+                        dy.sizes() == embedded(tokens, gradient.size(1)) && dy.device() == gradient.device(),
+                    "Expected BF16 or FP32 rows of shape ", embedded(tokens, gradient.size(1)), " on ", gradient.device());
+  TORCH_CHECK_VALUE(std::isfinite(scale), "The scale must be finite, not ", scale);
+  embedding_sums(dy, tokens, scale, gradient, WS_EMBED_ADD_F32);
+}
+
+struct EmbeddingFn : Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& table, double scale, bool f32) {
+    static const auto op = find<Embedding>("warpstate::native_embedding");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["vocab"] = table.sym_size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["f32"] = table.scalar_type() == at::kFloat;
+    return below(op, tokens, table, scale, f32);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    typedef const Tensor& T;
+    static const auto op = find<Tensor(T, T, c10::SymInt, double, bool)>("warpstate::native_embedding_backward");
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    Tensor d = below(op, grads[0], ctx->get_saved_variables()[0], ctx->saved_data["vocab"].toSymInt(),
+                     ctx->saved_data["scale"].toDouble(), ctx->saved_data["f32"].toBool());
+    return once({Tensor(), d, Tensor(), Tensor()}, {grads[0]}, kEmbeddingTwice);
+  }
+};
+Tensor embedding_autograd(const Tensor& tokens, const Tensor& table, double scale, bool f32) {
+  static const auto op = find<Embedding>("warpstate::native_embedding");
+  refuse_tangents("embedding", table);
+  if (!records(table)) return below(op, tokens, table, scale, f32);
+  return EmbeddingFn::apply(tokens, table, scale, f32);
+}
+Tensor embedding_meta(const Tensor& tokens, const Tensor& table, double scale, bool f32) {
+  check_embedding(tokens, table, scale);
+  return at::empty(embedded(tokens, table.size(1)), table.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+}
+Tensor embedding_backward_meta(const Tensor& dy, const Tensor&, int64_t vocab, double, bool f32) {
+  return at::empty({vocab, dy.size(-1)}, dy.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(warpstate, m) {
+  m.def("native_add_rmsnorm(Tensor x, Tensor residual, Tensor weight, float eps) -> (Tensor, Tensor)");
+  m.def("native_add_rmsnorm_rstd(Tensor x, Tensor residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "native_add_rmsnorm_backward(Tensor stream, Tensor weight, Tensor rstd, Tensor dy, Tensor? dstream) -> "
+      "(Tensor, Tensor, Tensor)");
+  m.def(
+      "native_rmsnorm_quantize(Tensor x, Tensor? residual, Tensor weight, float eps, bool e8m0) -> (Tensor, Tensor, "
+      "Tensor)");
+  m.def("native_embedding(Tensor tokens, Tensor table, float scale, bool f32) -> Tensor");
+  m.def("native_embedding_backward(Tensor dy, Tensor tokens, SymInt vocab, float scale, bool f32) -> Tensor");
+  m.def("native_embedding_accumulate_(Tensor(a!) gradient, Tensor tokens, Tensor dy, float scale) -> ()");
+}
+TORCH_LIBRARY_IMPL(warpstate, CUDA, m) {
+  m.impl("native_add_rmsnorm", &add_rmsnorm);
+  m.impl("native_add_rmsnorm_rstd", &add_rmsnorm_rstd);
+  m.impl("native_add_rmsnorm_backward", &add_rmsnorm_backward);
+  m.impl("native_rmsnorm_quantize", &rmsnorm_quantize);
+  m.impl("native_embedding", &embedding);
+  m.impl("native_embedding_backward", &embedding_backward);
+  m.impl("native_embedding_accumulate_", &embedding_accumulate);
+}
+TORCH_LIBRARY_IMPL(warpstate, AutogradCUDA, m) {
+  m.impl("native_add_rmsnorm", &add_rmsnorm_autograd);
+  m.impl("native_rmsnorm_quantize", &rmsnorm_quantize_autograd);
+  m.impl("native_embedding", &embedding_autograd);
+}
+TORCH_LIBRARY_IMPL(warpstate, Meta, m) {
+  m.impl("native_add_rmsnorm", &add_rmsnorm_meta);
+  m.impl("native_add_rmsnorm_rstd", &add_rmsnorm_rstd_meta);
+  m.impl("native_add_rmsnorm_backward", &add_rmsnorm_backward_meta);
+  m.impl("native_embedding", &embedding_meta);
+  m.impl("native_embedding_backward", &embedding_backward_meta);
+}

@@ -105,6 +105,19 @@ SIGNATURES = {
     "ws_linear_token_scores_backward": (_i32, [_c_void_p, _i64, _c_void_p, _i64] + [_c_void_p] * 6
                                         + [_i64, _i64, _i64, _f32, _c_void_p, _i64, _c_void_p, _i64,
                                            _c_void_p, _i64, _i32, _c_void_p]),
+    "ws_add_rmsnorm": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _i32, _c_void_p, _f32, _i64, _i64]
+                       + [_c_void_p] * 4),
+    "ws_rmsnorm_quantize": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _i32, _c_void_p, _f32, _i64,
+                                   _i64, _i32, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
+                                   _c_void_p]),
+    "ws_add_rmsnorm_backward_partial_floats": (_i64, [_i64, _i64]),
+    "ws_add_rmsnorm_backward": (_i32, [_c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p, _i64,
+                                       _c_void_p, _i64, _i64, _i64] + [_c_void_p] * 5),
+    "ws_embedding": (_i32, [_c_void_p, _i64, _i32, _c_void_p, _i64, _i64, _i64, _f32, _c_void_p,
+                            _i32, _c_void_p]),
+    "ws_embedding_backward_workspace_bytes": (_i64, [_i64] * 3),
+    "ws_embedding_backward": (_i32, [_c_void_p, _i64, _i32, _c_void_p, _i64, _i64, _i64, _f32,
+                                     _c_void_p, _i64, _i32, _c_void_p, _c_void_p]),
 }
 
 
