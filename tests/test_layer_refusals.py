@@ -87,3 +87,37 @@ def test_embedding_backward_arguments(change, match):
     with pytest.raises(RuntimeError, match=match):
         _hip.call("ws_embedding_backward", a["dy"], a["ld_dy"], 0, a["tokens"], a["rows"], a["vocab"],
                   a["d"], 1.0, a["out"], a["ld"], a["mode"], a["work"], None)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(form=2), "form"), (dict(groups=0), "groups"), (dict(groups=65537), "groups"), (dict(rows=-1), "shape"),
+    (dict(n=12), "multiple of 8"), (dict(k=12), "multiple of 8"), (dict(n=0), "shape"), (dict(x=None), "null"),
+    (dict(w=None), "null"), (dict(offsets=None), "null"), (dict(y=None), "null"), (dict(x=GPU + 8), "aligned"),
+    (dict(ldx=20), "aligned"), (dict(ldx=8), "overlap"), (dict(ldw=8), "overlap"), (dict(ldy=8), "overlap"),
+    (dict(stride=12), "aligned"), (dict(stride=-8), "aligned"), (dict(ldy=4200000), "stride"),
+    (dict(rows=2 ** 30, n=2 ** 20, ldy=2 ** 20), "tiles")])
+def test_grouped_mm_arguments(change, match):
+    a = dict(x=GPU, ldx=16, w=GPU, ldw=16, stride=256, form=0, offsets=GPU, groups=2, rows=4, n=16, k=16, y=GPU,
+             ldy=16) | change
+    with pytest.raises(RuntimeError, match=match):
+        _hip.call("ws_grouped_mm", a["x"], a["ldx"], a["w"], a["ldw"], a["stride"], a["form"], a["offsets"],
+                  a["groups"], a["rows"], a["n"], a["k"], a["y"], a["ldy"], None)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(groups=0), "groups"), (dict(rows=-1), "shape"), (dict(n=12), "multiple of 8"), (dict(dy=None), "null"),
+    (dict(x=None), "null"), (dict(offsets=None), "null"), (dict(dw=None), "null"), (dict(dw=GPU + 8), "aligned"),
+    (dict(dy=GPU + 2), "aligned"), (dict(ldx=8), "overlap"), (dict(k=2200000, ldx=2200000), "stride"),
+    (dict(groups=65536, n=4096, k=4096, ld_dy=4096, ldx=4096), "tiles")])
+def test_grouped_weight_grad_arguments(change, match):
+    a = dict(dy=GPU, ld_dy=16, x=GPU, ldx=16, offsets=GPU, groups=2, rows=4, n=16, k=16, dw=GPU) | change
+    with pytest.raises(RuntimeError, match=match):
+        _hip.call("ws_grouped_weight_grad", a["dy"], a["ld_dy"], a["x"], a["ldx"], a["offsets"], a["groups"],
+                  a["rows"], a["n"], a["k"], a["dw"], 1, None)
+
+
+def test_grouped_tile_of_bad_sizes():
+    assert _hip.query("ws_grouped_tile", 0, 1, 8, 8, 0) == -1
+    assert _hip.query("ws_grouped_tile", 8, 0, 8, 8, 0) == -1
+    assert _hip.query("ws_grouped_tile", 8, 1, 12, 8, 0) == -1
+    assert _hip.query("ws_grouped_tile", 8, 1, 8, 8, 3) == -1

@@ -762,6 +762,123 @@ struct FEpiCEStatsLogits {
   }
 };
 
+// The k-loop of one 256 x 256 tile over k-tiles [kb, ke): A's tile rows [row0_a, row0_a + 256) below
+// rows_a, B's likewise (in a PAIRED tile 128 rows from row0_b and 128 from row0_b + half, both
+// below rows_b). sA and sB are the operands' LDS stages, abase and bbase this lane's fragment
+// offsets in their first ones. No load is in flight when it returns, but only the second group of waves
+// has passed every barrier of the first: another follows before the stages are used again.
+template <int AMODE, int BMODE, bool PAIRED>
+__device__ __forceinline__ void fast_k_loop(Acc16<4, 8>& acc, const OperandDesc& a, int row0_a, int rows_a,
+                                            const OperandDesc& b, int row0_b, int rows_b, int half, int K,
+                                            int kb, int ke, unsigned char* const sA, unsigned char* const sB,
+                                            const unsigned abase, const unsigned bbase, const int wave,
+                                            const int lane) {
+  constexpr int FA = 4, FB = 8;
+  const bool first = wave < 4;  // the group that runs a phase ahead and loads A
+  if (kb < ke) {
+    // This wave's share of its group's operand tile: one quarter, eight loads, at `base`
+    // plus `step` elements per k-tile.
+    typedef RingTile<256, 256, AMODE, false> TileA;
+    typedef RingTile<256, 256, BMODE, PAIRED> TileB;
+    const int gw = wave & 3;
+    unsigned off[kFIns];
+    const unsigned short* base;
+    long step;
+    if (first) {
+      TileA l;
+      l.init(a, row0_a, rows_a, 0, gw, lane);
+#pragma unroll
+      for (int i = 0; i < kFIns; ++i) off[i] = l.off[i];
+      base = a.ptr + (AMODE == kKContig ? row0_a * a.s_row : (long)row0_a);
+      step = AMODE == kKContig ? kFBK : kFBK * a.s_k;
+    } else {
+      TileB l;
+      l.init(b, row0_b, rows_b, half, gw, lane);
+#pragma unroll
+      for (int i = 0; i < kFIns; ++i) off[i] = l.off[i];
+      base = b.ptr + (BMODE == kKContig ? row0_b * b.s_row : (long)row0_b);
+      step = BMODE == kKContig ? kFBK : kFBK * b.s_k;
+    }
+    auto load = [&](int kt, unsigned char* stage) {
+      __amdgpu_buffer_rsrc_t rs = make_rsrc(base + kt * step, 0x7fffffff);
+      unsigned char* dst = stage + gw * 1024;
+      if ((kt + 1) * kFBK <= K) {
+#pragma unroll
+        for (int i = 0; i < kFIns; ++i) dma16(rs, dst + i * 4096, off[i]);
+      } else {
+        // Ragged: chunks at k >= K land as zeros. The lane index goes through an empty asm
+        // so that the k offsets are not kept live across the loop.
+        int l = lane;
+        asm volatile("" : "+v"(l));
+#pragma unroll
+        for (int i = 0; i < kFIns; ++i) {
+          const int k = first ? TileA::k_of(i, gw, l) : TileB::k_of(i, gw, l);
+          dma16(rs, dst + i * 4096, kt * kFBK + k >= K ? kOOB : off[i]);
+        }
+      }
+    };
+    if (first) {
+      load(kb, sA);
+      __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
+    } else {
+      load(kb, sB);
+      if (kb + 1 < ke) {
+        load(kb + 1, sB + kFTileBytes);
+        __builtin_amdgcn_s_waitcnt(wait_vmcnt(kFIns));  // B(kb)
+      } else {
+        __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
+      }
+    }
+    __builtin_amdgcn_s_barrier();
+    if (!first) __builtin_amdgcn_s_barrier();  // one phase behind from here on
+    unsigned ast = 0, bst = 0;  // byte offsets of the k-tile's stages
+    // k-tile kt; the last two (TAIL) load nothing past the piece: those loads would fetch
+    // another slice's operands or zeros, and the epilogue would wait for them.
+    auto k_tile = [&](int kt, auto tail) {
+      constexpr bool TAIL = decltype(tail)::value;
+      // Read phase. A(kt + 1) goes to the stage A(kt - 1) used and B(kt + 2) to the one
+      // B(kt - 1) used: both groups have read those.
+      if (!TAIL)
+        load(first ? kt + 1 : kt + 2,
+             first ? sA + (ast ^ kFTileBytes) : sB + (bst == 0 ? 2 * kFTileBytes : bst - kFTileBytes));
+      else if (first && kt + 1 < ke)
+        load(kt + 1, sA + (ast ^ kFTileBytes));
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8_t f[2 * (FA + FB)];
+      asm_frags<AMODE, BMODE, PAIRED, 0>(f, abase + ast, bbase + bst);
+      __builtin_amdgcn_sched_barrier(0);
+      // B(kt + 1) has landed (only the second group has older loads in flight here).
+      if (!TAIL) __builtin_amdgcn_s_waitcnt(wait_vmcnt(kFIns));
+      tie_wait(f);
+      __builtin_amdgcn_sched_barrier(0);
+      // In the last k-tile neither group has a load in flight from here on, so that the
+      // first group's epilogue may stage through LDS.
+      if (TAIL && !first) __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      // MFMA phase.
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < FA; ++i)
+#pragma unroll
+          for (int j = 0; j < FB; ++j)
+            acc.v[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[12 * s + FA + j], f[12 * s + i],
+                                                                   acc.v[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (first) __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));  // A(kt + 1) has landed
+      // The second group's last MFMA phase ends the loop: the first group is past it.
+      if (!TAIL || first || kt + 1 < ke) __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      ast ^= kFTileBytes;
+      bst = bst == 2 * kFTileBytes ? 0 : bst + kFTileBytes;
+    };
+    int kt = kb;
+    for (; kt + 2 < ke; ++kt) k_tile(kt, std::false_type{});
+    for (; kt < ke; ++kt) k_tile(kt, std::true_type{});
+  }
+}
+
 // --------------------------------------------------------------------------------------
 // The kernel.
 
@@ -778,7 +895,6 @@ __global__ void __launch_bounds__(kFNT) gemm_fast_kernel(const GemmParams p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / kFWN, wn = wave % kFWN;
-  const bool first = wave < 4;  // the group that runs a phase ahead and loads A
   const int bn_cols = PAIRED ? kFBN / 2 : kFBN;
   const int k_tiles_total = cdiv(p.K, kFBK);
   const int kt_begin = blockIdx.y * p.k_tiles_per_split;
@@ -807,108 +923,8 @@ __global__ void __launch_bounds__(kFNT) gemm_fast_kernel(const GemmParams p) {
 #pragma unroll
       for (int j = 0; j < FB; ++j) acc.v[i][j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
 
-    if (kb < ke) {
-      // This wave's share of its group's operand tile: one quarter, eight loads, at `base`
-      // plus `step` elements per k-tile.
-      typedef RingTile<256, 256, AMODE, false> TileA;
-      typedef RingTile<256, 256, BMODE, PAIRED> TileB;
-      const int gw = wave & 3;
-      unsigned off[kFIns];
-      const unsigned short* base;
-      long step;
-      if (first) {
-        TileA l;
-        l.init(q.a, row0_a, q.M, 0, gw, lane);
-#pragma unroll
-        for (int i = 0; i < kFIns; ++i) off[i] = l.off[i];
-        base = q.a.ptr + (AMODE == kKContig ? row0_a * q.a.s_row : (long)row0_a);
-        step = AMODE == kKContig ? kFBK : kFBK * q.a.s_k;
-      } else {
-        TileB l;
-        l.init(q.b, row0_b, PAIRED ? p.H : q.N, PAIRED ? p.H : 0, gw, lane);
-#pragma unroll
-        for (int i = 0; i < kFIns; ++i) off[i] = l.off[i];
-        base = q.b.ptr + (BMODE == kKContig ? row0_b * q.b.s_row : (long)row0_b);
-        step = BMODE == kKContig ? kFBK : kFBK * q.b.s_k;
-      }
-      auto load = [&](int kt, unsigned char* stage) {
-        __amdgpu_buffer_rsrc_t rs = make_rsrc(base + kt * step, 0x7fffffff);
-        unsigned char* dst = stage + gw * 1024;
-        if ((kt + 1) * kFBK <= p.K) {
-#pragma unroll
-          for (int i = 0; i < kFIns; ++i) dma16(rs, dst + i * 4096, off[i]);
-        } else {
-          // Ragged: chunks at k >= K land as zeros. The lane index goes through an empty asm
-          // so that the k offsets are not kept live across the loop.
-          int l = lane;
-          asm volatile("" : "+v"(l));
-#pragma unroll
-          for (int i = 0; i < kFIns; ++i) {
-            const int k = first ? TileA::k_of(i, gw, l) : TileB::k_of(i, gw, l);
-            dma16(rs, dst + i * 4096, kt * kFBK + k >= p.K ? kOOB : off[i]);
-          }
-        }
-      };
-      if (first) {
-        load(kb, sA);
-        __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
-      } else {
-        load(kb, sB);
-        if (kb + 1 < ke) {
-          load(kb + 1, sB + kFTileBytes);
-          __builtin_amdgcn_s_waitcnt(wait_vmcnt(kFIns));  // B(kb)
-        } else {
-          __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
-        }
-      }
-      __builtin_amdgcn_s_barrier();
-      if (!first) __builtin_amdgcn_s_barrier();  // one phase behind from here on
-      unsigned ast = 0, bst = 0;  // byte offsets of the k-tile's stages
-      // k-tile kt; the last two (TAIL) load nothing past the piece: those loads would fetch
-      // another slice's operands or zeros, and the epilogue would wait for them.
-      auto k_tile = [&](int kt, auto tail) {
-        constexpr bool TAIL = decltype(tail)::value;
-        // Read phase. A(kt + 1) goes to the stage A(kt - 1) used and B(kt + 2) to the one
-        // B(kt - 1) used: both groups have read those.
-        if (!TAIL)
-          load(first ? kt + 1 : kt + 2,
-               first ? sA + (ast ^ kFTileBytes) : sB + (bst == 0 ? 2 * kFTileBytes : bst - kFTileBytes));
-        else if (first && kt + 1 < ke)
-          load(kt + 1, sA + (ast ^ kFTileBytes));
-        __builtin_amdgcn_sched_barrier(0);
-        bf16x8_t f[2 * (FA + FB)];
-        asm_frags<AMODE, BMODE, PAIRED, 0>(f, abase + ast, bbase + bst);
-        __builtin_amdgcn_sched_barrier(0);
-        // B(kt + 1) has landed (only the second group has older loads in flight here).
-        if (!TAIL) __builtin_amdgcn_s_waitcnt(wait_vmcnt(kFIns));
-        tie_wait(f);
-        __builtin_amdgcn_sched_barrier(0);
-        // In the last k-tile neither group has a load in flight from here on, so that the
-        // first group's epilogue may stage through LDS.
-        if (TAIL && !first) __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        // MFMA phase.
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int i = 0; i < FA; ++i)
-#pragma unroll
-            for (int j = 0; j < FB; ++j)
-              acc.v[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[12 * s + FA + j], f[12 * s + i],
-                                                                     acc.v[i][j], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        if (first) __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));  // A(kt + 1) has landed
-        // The second group's last MFMA phase ends the loop: the first group is past it.
-        if (!TAIL || first || kt + 1 < ke) __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        ast ^= kFTileBytes;
-        bst = bst == 2 * kFTileBytes ? 0 : bst + kFTileBytes;
-      };
-      int kt = kb;
-      for (; kt + 2 < ke; ++kt) k_tile(kt, std::false_type{});
-      for (; kt < ke; ++kt) k_tile(kt, std::true_type{});
-    }
+    fast_k_loop<AMODE, BMODE, PAIRED>(acc, q.a, row0_a, q.M, q.b, row0_b, PAIRED ? p.H : q.N, PAIRED ? p.H : 0, p.K,
+                                      kb, ke, sA, sB, abase, bbase, wave, lane);
     const int m_base = row0_a + wm * TM;
     const int n_base = row0_b + (PAIRED ? wn * (TN / 2) : wn * TN);
     epi(acc, m_base, n_base, tm, tn);

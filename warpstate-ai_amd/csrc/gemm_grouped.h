@@ -1,0 +1,329 @@
+// Products grouped by expert: rows sorted by expert, each expert's with a weight of its own.
+//
+//   rows t in [offsets[e], offsets[e + 1]):  C[t] = A[t] B_e          (forward, input gradient)
+//   G_e = sum over those t of dY[t]^T X[t]                            (weight gradient)
+//
+// The offsets are on the device and the host knows only their number, so the grid is sized for
+// the most tiles that any offsets make, and a workgroup finds its tile from them: every wave
+// runs over the groups, a group on a lane, with a running sum of their tiles, and takes the group
+// whose tiles hold its index. Offsets are clamped to [0, rows]: whatever they hold, no access leaves the
+// operands. Rows before the first offset and behind the last form two groups without a
+// product, and get zeros.
+//
+// A group's tiles are those of a product of its own (gemm_fast.h, gemm_ring.h): the same loads, LDS
+// layouts, k-loops and epilogues, with the group's first row and row count in the place of the
+// matrix's. With few rows for each group the weights' bytes are the bound, and the kernel at
+// the end streams them.
+#pragma once
+
+#include "gemm_ring.h"
+
+namespace ws {
+
+struct GroupedParams {
+  OperandDesc a;                // rows of all groups
+  OperandDesc b;                // group 0's weight as the product's B
+  long b_group;                 // elements from one group's weight to the next
+  const long* offsets;          // [groups + 1]
+  int groups, rows, N, K, tiles_n;
+  int most;                     // tiles that the grid is sized for
+  unsigned short* c; long ldc;
+};
+
+struct GroupTile {
+  int group;     // -1: rows of no group
+  int lo, hi;    // its rows
+  int index;     // the tile within the group
+};
+
+// Rows [lo, hi) of pseudo-group g: 0 before the first offset, 1 .. groups the groups, groups + 1
+// behind the last offset; empty beyond.
+__device__ __forceinline__ void group_rows(const long* offsets, int groups, int rows, int g, int& lo, int& hi) {
+  auto at = [&](int i) { return (int)min((long)rows, max(0L, offsets[i])); };
+  lo = g == 0 || g > groups + 1 ? 0 : at(g - 1);
+  hi = g > groups + 1 ? 0 : g == groups + 1 ? rows : at(g);
+}
+
+// Pseudo-group g0 + lane's rows and tiles of BM rows, and the running sum of the tiles over the lanes.
+struct GroupLanes {
+  int lo, hi, tiles, upto;
+};
+template <int BM>
+__device__ __forceinline__ GroupLanes group_lanes(const GroupedParams& p, int g0, int lane) {
+  GroupLanes v;
+  group_rows(p.offsets, p.groups, p.rows, g0 + lane, v.lo, v.hi);
+  v.tiles = v.hi > v.lo ? cdiv(v.hi - v.lo, BM) * p.tiles_n : 0;
+  v.upto = v.tiles;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int other = __shfl_up(v.upto, off, kWave);
+    if (lane >= off) v.upto += other;
+  }
+  return v;
+}
+
+// The tiles that there are, `most` at most (what offsets that do not decrease make), and the groups
+// of the first 64 lanes.
+template <int BM>
+__device__ __forceinline__ int count_tiles(const GroupedParams& p, int lane, GroupLanes& v) {
+  v = group_lanes<BM>(p, 0, lane);
+  int total = min(p.most, __builtin_amdgcn_readlane(v.upto, 63));
+  for (int g0 = 64; g0 < p.groups + 2; g0 += 64)
+    total = min(p.most, total + __builtin_amdgcn_readlane(group_lanes<BM>(p, g0, lane).upto, 63));
+  return total;
+}
+
+// The tile at index w, below count_tiles' total.
+template <int BM>
+__device__ __forceinline__ GroupTile find_tile(const GroupedParams& p, int w, int lane, GroupLanes v) {
+  for (int g0 = 0;; v = group_lanes<BM>(p, g0, lane)) {
+    const unsigned long past = __builtin_amdgcn_ballot_w64(w < v.upto);
+    if (past != 0) {
+      const int l = __builtin_ctzl(past), g = g0 + l;
+      return GroupTile{g == 0 || g == p.groups + 1 ? -1 : g - 1, __builtin_amdgcn_readlane(v.lo, l),
+                       __builtin_amdgcn_readlane(v.hi, l), w - __builtin_amdgcn_readlane(v.upto - v.tiles, l)};
+    }
+    w -= __builtin_amdgcn_readlane(v.upto, 63);
+    g0 += 64;
+  }
+}
+
+// What the epilogues read of a GEMM's parameters.
+__device__ __forceinline__ GemmParams store_params(unsigned short* c, long ldc, int M, int N) {
+  GemmParams e{};
+  e.c = c;
+  e.ldc = ldc;
+  e.M = M;
+  e.N = N;
+  return e;
+}
+
+// 256 x 256 tiles, a workgroup per compute unit looping over them.
+template <int BMODE>
+__global__ void __launch_bounds__(kFNT) grouped_fast_kernel(const GroupedParams p) {
+  constexpr int TM = kFBM / kFWM, TN = kFBN / kFWN;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char fsmem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / kFWN, wn = wave % kFWN;
+  const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)fsmem;
+  const unsigned abase = lds0 + frag_base<kKContig>(wm * TM, lane);
+  const unsigned bbase = lds0 + 2 * kFTileBytes + frag_base<BMODE>(wn * TN, lane);
+  GroupLanes v;
+  const int total = count_tiles<kFBM>(p, lane, v);
+  for (int w = blockIdx.x; w < total; w += gridDim.x) {
+    // The groups are read again for each tile: kept over the k-loop they would cost it registers.
+    int l = lane;
+    opaque_lane(l);
+    const GroupTile t = find_tile<kFBM>(p, xcd_remap(w, total, gridDim.x), l, group_lanes<kFBM>(p, 0, l));
+    int tm, tn;
+    tile_position(t.index, cdiv(t.hi - t.lo, kFBM), p.tiles_n, tm, tn);
+    const int row0 = t.lo + tm * kFBM, col0 = tn * kFBN;
+    OperandDesc b = p.b;
+    b.ptr += max(t.group, 0) * p.b_group;
+    Acc16<4, 8> acc;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc.v[i][j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+    fast_k_loop<kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.N, 0, p.K, 0,
+                                        t.group < 0 ? 0 : cdiv(p.K, kFBK), fsmem, fsmem + 2 * kFTileBytes, abase,
+                                        bbase, wave, lane);
+    const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
+    FEpiStore<false, false>::run(e, acc, row0 + wm * TM, col0 + wn * TN, lane, tm, tn, wn, fsmem + wave * kFStageWave);
+    __builtin_amdgcn_s_barrier();
+  }
+}
+
+// Smaller tiles, one workgroup each.
+template <class Cfg, int BMODE>
+__global__ void __launch_bounds__(Cfg::NT) grouped_ring_kernel(const GroupedParams p) {
+  constexpr int FA = Cfg::FA, FB = Cfg::FB, TM = Cfg::TM, TN = Cfg::TN;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char rsmem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+  GroupLanes v;
+  const int total = count_tiles<Cfg::BM>(p, lane, v);
+  if ((int)blockIdx.x >= total) return;
+  const GroupTile t = find_tile<Cfg::BM>(p, xcd_remap(blockIdx.x, total, kRingWindow), lane, v);
+  int tm, tn;
+  tile_position(t.index, cdiv(t.hi - t.lo, Cfg::BM), p.tiles_n, tm, tn);
+  const int row0 = t.lo + tm * Cfg::BM, col0 = tn * Cfg::BN;
+  OperandDesc b = p.b;
+  b.ptr += max(t.group, 0) * p.b_group;
+  Acc16<FA, FB> acc;
+  ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.N, 0, p.K, 0,
+                                           t.group < 0 ? 0 : cdiv(p.K, kFBK), rsmem, wave, lane);
+  const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
+  FEpiStore<false, false>::run(e, acc, row0 + wm * TM, col0 + wn * TN, lane, tm, tn, wn,
+                               rsmem + wave * epi_wave<FA, FB>());
+}
+
+// --------------------------------------------------------------------------------------
+// Weight gradients: [M, N] per group, reduced over the group's rows.
+
+struct GroupedGradParams {
+  const unsigned short *a, *b;  // [rows, M] and [rows, N]
+  long lda, ldb;
+  const long* offsets;
+  int groups, rows, M, N, tiles_m, tiles_n;
+  void* g;                      // [groups, M, N], BF16 or FP32
+};
+
+struct GradTile {
+  OperandDesc a, b;
+  int group, K, tm, tn;
+};
+__device__ __forceinline__ GradTile grad_tile(const GroupedGradParams& p, int w) {
+  const int per = p.tiles_m * p.tiles_n;
+  GradTile t;
+  t.group = w / per;
+  tile_position(w - t.group * per, p.tiles_m, p.tiles_n, t.tm, t.tn);
+  int lo, hi;
+  group_rows(p.offsets, p.groups, p.rows, t.group + 1, lo, hi);
+  t.K = max(0, hi - lo);
+  t.a = OperandDesc{p.a + lo * p.lda, 1, p.lda};
+  t.b = OperandDesc{p.b + lo * p.ldb, 1, p.ldb};
+  return t;
+}
+template <bool F32, int FA, int FB>
+__device__ __forceinline__ void grad_store(const GroupedGradParams& p, const GradTile& t, Acc16<FA, FB>& acc, int m_base,
+                                           int n_base, int lane, int wn, unsigned char* stage) {
+  const long at = (long)t.group * p.M * p.N;
+  if constexpr (F32) {
+    FEpiAccF32<false>::add(static_cast<float*>(p.g) + at, p.N, p.M, p.N, kAccStore, acc, m_base, n_base, lane, t.tm, t.tn);
+  } else {
+    const GemmParams e = store_params(static_cast<unsigned short*>(p.g) + at, p.N, p.M, p.N);
+    FEpiStore<false, false>::run(e, acc, m_base, n_base, lane, t.tm, t.tn, wn, stage);
+  }
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(kFNT) grouped_grad_fast_kernel(const GroupedGradParams p) {
+  constexpr int TM = kFBM / kFWM, TN = kFBN / kFWN;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char fsmem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / kFWN, wn = wave % kFWN;
+  const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)fsmem;
+  const unsigned abase = lds0 + frag_base<kMNContig>(wm * TM, lane);
+  const unsigned bbase = lds0 + 2 * kFTileBytes + frag_base<kMNContig>(wn * TN, lane);
+  const int total = p.groups * p.tiles_m * p.tiles_n;
+  for (int w = blockIdx.x; w < total; w += gridDim.x) {
+    const GradTile t = grad_tile(p, xcd_remap(w, total, gridDim.x));
+    Acc16<4, 8> acc;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc.v[i][j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+    fast_k_loop<kMNContig, kMNContig, false>(acc, t.a, t.tm * kFBM, p.M, t.b, t.tn * kFBN, p.N, 0, t.K, 0,
+                                             cdiv(t.K, kFBK), fsmem, fsmem + 2 * kFTileBytes, abase, bbase, wave, lane);
+    grad_store<F32>(p, t, acc, t.tm * kFBM + wm * TM, t.tn * kFBN + wn * TN, lane, wn, fsmem + wave * kFStageWave);
+    __builtin_amdgcn_s_barrier();
+  }
+}
+
+template <class Cfg, bool F32>
+__global__ void __launch_bounds__(Cfg::NT) grouped_grad_ring_kernel(const GroupedGradParams p) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char rsmem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+  const GradTile t = grad_tile(p, xcd_remap(blockIdx.x, gridDim.x, kRingWindow));
+  Acc16<Cfg::FA, Cfg::FB> acc;
+  ring_k_loop<Cfg, kMNContig, kMNContig, false>(acc, t.a, t.tm * Cfg::BM, p.M, t.b, t.tn * Cfg::BN, p.N, 0, t.K, 0,
+                                                cdiv(t.K, kFBK), rsmem, wave, lane);
+  grad_store<F32>(p, t, acc, t.tm * Cfg::BM + wm * Cfg::TM, t.tn * Cfg::BN + wn * Cfg::TN, lane, wn,
+                  rsmem + wave * epi_wave<Cfg::FA, Cfg::FB>());
+}
+
+// --------------------------------------------------------------------------------------
+// Few rows for each group: tiles of 16 MT rows x 32 columns, one workgroup of four waves, each
+// with a quarter of the reduction (64 of every 256 k, so that together they read whole rows of the
+// weight). Fragments go from memory to registers as they are: a lane's piece is 16 bytes of one row,
+// and a k-tile's two pieces of a row are one line. The waves' sums are added through LDS, in
+// wave order. Rows and columns past the group's and the weight's read the last ones and are not
+// stored.
+constexpr int kFewCols = 32;
+
+template <int MT>
+__global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedParams p) {
+  constexpr int BM = 16 * MT;
+  __shared__ float sums[4][BM][kFewCols + 4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  GroupLanes v;
+  if ((int)blockIdx.x >= count_tiles<BM>(p, lane, v)) return;
+  const GroupTile t = find_tile<BM>(p, blockIdx.x, lane, v);
+  const int tm = t.index / p.tiles_n, tn = t.index - tm * p.tiles_n;
+  const int row0 = t.lo + tm * BM, col0 = tn * kFewCols;
+  f32x4_v acc[MT][2];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+  if (t.group >= 0) {
+    const int r = lane & 15, q = 8 * (lane >> 4);
+    const unsigned short* a[MT];
+    const unsigned short* b[2];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) a[i] = p.a.ptr + (long)min(row0 + 16 * i + r, t.hi - 1) * p.a.s_row + q;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      b[j] = p.b.ptr + t.group * p.b_group + (long)min(col0 + 16 * j + r, p.N - 1) * p.b.s_row + q;
+    // U k-tiles at a time, all of their pieces requested before the first product.
+    auto steps = [&](int k, auto count, auto load) {
+      constexpr int U = decltype(count)::value;
+      bf16x8_t fa[U][2][MT], fb[U][2][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int at = k + 256 * u + 32 * s;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) fb[u][s][j] = load(b[j], at);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) fa[u][s][i] = load(a[i], at);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[u][s][j], fa[u][s][i], acc[i][j], 0, 0, 0);
+    };
+    const auto whole = [](const unsigned short* row, int at) { return *reinterpret_cast<const bf16x8_t*>(row + at); };
+    constexpr int U = MT < 4 ? 4 : 2;
+    int k = 64 * wave;
+    for (; k + 256 * (U - 1) + 64 <= p.K; k += 256 * U) steps(k, std::integral_constant<int, U>{}, whole);
+    for (; k + 64 <= p.K; k += 256) steps(k, std::integral_constant<int, 1>{}, whole);
+    if (k < p.K)
+      steps(k, std::integral_constant<int, 1>{}, [&](const unsigned short* row, int at) {
+        bf16x8_t v = {};
+        if (at + q + 8 <= p.K) v = *reinterpret_cast<const bf16x8_t*>(row + at);
+        return v;
+      });
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      *reinterpret_cast<f32x4_v*>(&sums[wave][16 * i + (lane & 15)][16 * j + 4 * (lane >> 4)]) = acc[i][j];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int m = 16 * i + (threadIdx.x >> 4), n = 2 * (threadIdx.x & 15);
+    float v[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      v[e] = (sums[0][m][n + e] + sums[1][m][n + e]) + (sums[2][m][n + e] + sums[3][m][n + e]);
+    if (row0 + m < t.hi && col0 + n < p.N)  // N is a multiple of 8
+      *reinterpret_cast<unsigned*>(p.c + (long)(row0 + m) * p.ldc + col0 + n) = pack_bf16x2(v[0], v[1]);
+  }
+}
+
+}  // namespace ws

@@ -97,36 +97,21 @@ __device__ __forceinline__ void ring_step0(Acc16<Cfg::FA, Cfg::FB>& acc,
   }
 }
 
-// Workgroups that run at once (two on each of 256 CUs): the XCD remap deals each such window
-// of the raster out in eight runs of neighbouring tiles (against one run per XCD over the
-// whole grid, the paired tiles are 0.5-1 % faster).
-constexpr int kRingWindow = 512;
-
-template <class Cfg, int AMODE, int BMODE, bool PAIRED, class Epi>
-__global__ void __launch_bounds__(Cfg::NT) gemm_ring_kernel(const GemmParams p) {
-  static_assert(AMODE != kGeneric && BMODE != kGeneric, "vector operands only");
+// The accumulators of one tile over k-tiles [kb, ke): the operands' arguments are those of fast_k_loop
+// (gemm_fast.h). No load is in flight and every wave is done with the stages when it returns.
+template <class Cfg, int AMODE, int BMODE, bool PAIRED>
+__device__ __forceinline__ void ring_k_loop(Acc16<Cfg::FA, Cfg::FB>& acc, const OperandDesc& a, int row0_a, int rows_a,
+                                            const OperandDesc& b, int row0_b, int rows_b, int half, int K,
+                                            int kb, int ke, unsigned char* const rsmem, const int wave,
+                                            const int lane) {
   constexpr int FA = Cfg::FA, FB = Cfg::FB, NM = FA * FB, NF = FA + FB, S = Cfg::S;
   constexpr int TM = Cfg::TM, TN = Cfg::TN;
   constexpr bool kAsm = AMODE == kMNContig || BMODE == kMNContig;
-
-  extern __shared__ __attribute__((aligned(1024))) unsigned char rsmem[];
-  if (p.skip_if != nullptr && *p.skip_if != 0) return;  // uniform: the whole grid exits
-
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
-  const int kb = blockIdx.y * p.k_tiles_per_split;
-  const int ke = min(cdiv(p.K, kFBK), kb + p.k_tiles_per_split);
-
-  int tm, tn;
-  tile_position(xcd_remap(blockIdx.x, p.total_tiles, kRingWindow), p.tiles_m, p.tiles_n, tm, tn);
-  const int row0_a = tm * Cfg::BM;
-  const int row0_b = tn * (PAIRED ? Cfg::BN / 2 : Cfg::BN);
-
   RingTile<Cfg::BM, Cfg::NT, AMODE, false> la;
   RingTile<Cfg::BN, Cfg::NT, BMODE, PAIRED> lb;
-  la.init(p.a, row0_a, p.M, 0, wave, lane);
-  lb.init(p.b, row0_b, PAIRED ? p.H : p.N, PAIRED ? p.H : 0, wave, lane);
+  la.init(a, row0_a, rows_a, 0, wave, lane);
+  lb.init(b, row0_b, rows_b, half, wave, lane);
   constexpr int kWaitLoads = (RingTile<Cfg::BM, Cfg::NT, AMODE, false>::kIns +
                               RingTile<Cfg::BN, Cfg::NT, BMODE, PAIRED>::kIns) * (S - 2);
 
@@ -138,7 +123,6 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_ring_kernel(const GemmParams p) 
                                    : Cfg::BN / 2 + wn * (TN / 2) + 16 * (j - FB / 2))
                      : wn * TN + 16 * j;
 
-  Acc16<FA, FB> acc;
 #pragma unroll
   for (int i = 0; i < FA; ++i)
 #pragma unroll
@@ -149,8 +133,8 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_ring_kernel(const GemmParams p) 
   // more than that traffic (768 x 512 over 15360 tokens in four slices 38.5 -> 40.5 us).
   auto issue = [&](int kt, int stage) {
     unsigned char* st = rsmem + stage * Cfg::kStage;
-    la.issue(p.a, row0_a, kt * kFBK, p.K, st, wave, lane);
-    lb.issue(p.b, row0_b, kt * kFBK, p.K, st + Cfg::kTileA, wave, lane);
+    la.issue(a, row0_a, kt * kFBK, K, st, wave, lane);
+    lb.issue(b, row0_b, kt * kFBK, K, st + Cfg::kTileA, wave, lane);
   };
   if (kb < ke) {
 #pragma unroll
@@ -226,6 +210,35 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_ring_kernel(const GemmParams p) 
     __builtin_amdgcn_s_waitcnt(wait_vmcnt(0));
     __builtin_amdgcn_s_barrier();
   }
+}
+
+// Workgroups that run at once (two on each of 256 CUs): the XCD remap deals each such window
+// of the raster out in eight runs of neighbouring tiles (against one run per XCD over the
+// whole grid, the paired tiles are 0.5-1 % faster).
+constexpr int kRingWindow = 512;
+
+template <class Cfg, int AMODE, int BMODE, bool PAIRED, class Epi>
+__global__ void __launch_bounds__(Cfg::NT) gemm_ring_kernel(const GemmParams p) {
+  static_assert(AMODE != kGeneric && BMODE != kGeneric, "vector operands only");
+  constexpr int FA = Cfg::FA, FB = Cfg::FB, TM = Cfg::TM, TN = Cfg::TN;
+
+  extern __shared__ __attribute__((aligned(1024))) unsigned char rsmem[];
+  if (p.skip_if != nullptr && *p.skip_if != 0) return;  // uniform: the whole grid exits
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+  const int kb = blockIdx.y * p.k_tiles_per_split;
+  const int ke = min(cdiv(p.K, kFBK), kb + p.k_tiles_per_split);
+
+  int tm, tn;
+  tile_position(xcd_remap(blockIdx.x, p.total_tiles, kRingWindow), p.tiles_m, p.tiles_n, tm, tn);
+  const int row0_a = tm * Cfg::BM;
+  const int row0_b = tn * (PAIRED ? Cfg::BN / 2 : Cfg::BN);
+
+  Acc16<FA, FB> acc;
+  ring_k_loop<Cfg, AMODE, BMODE, PAIRED>(acc, p.a, row0_a, p.M, p.b, row0_b, PAIRED ? p.H : p.N, PAIRED ? p.H : 0, p.K,
+                                         kb, ke, rsmem, wave, lane);
   Epi::run(p, acc, row0_a + wm * TM, row0_b + (PAIRED ? wn * (TN / 2) : wn * TN), lane, tm, tn, wn,
            rsmem + wave * epi_wave<FA, FB>());
 }

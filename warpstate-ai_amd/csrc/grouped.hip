@@ -1,0 +1,207 @@
+// C ABI: products grouped by expert.
+#include "../../include/warpstate_hip.h"
+#include "gemm_grouped.h"
+#include "launch.h"
+
+using namespace ws;
+
+namespace {
+
+constexpr int64_t kMaxGroups = 65536;
+// Beside FastTile: the kernel for few rows, by its row tiles of 16.
+constexpr int kTileFew1 = kFastTiles, kTileFew2 = kFastTiles + 1, kTileFew4 = kFastTiles + 2;
+
+int tile_rows(int tile) {
+  switch (tile) {
+    case kTile256: return 256;
+    case kTile128x2:
+    case kTile128x1: return 128;
+    case kTileFew1: return 16;
+    case kTileFew2: return 32;
+    default: return 64;
+  }
+}
+int tile_cols(int tile) {
+  return tile >= kTileFew1 ? kFewCols : tile == kTile256 ? 256 : tile == kTile64 ? 64 : 128;
+}
+// Tiles of `rows` rows that any offsets make at most: a group ends in a part of one. (The rows of
+// no group form two more.)
+int64_t most_tiles(int64_t rows, int64_t groups, int bm) {
+  const int64_t used = groups + 2 < rows ? groups + 2 : rows;
+  return rows / bm + used;
+}
+
+// The tile for rows that are spread over the groups: by the cost table of single products, with
+// half a tile more rows for each group, which is what ragged ends cost on average.
+int pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int bmode) {
+  const int64_t used = groups < rows ? groups : rows;
+  int best = kTile256;
+  float t = 0.0f;
+  for (int tile = 0; tile < kFastTiles; ++tile) {
+    const float ti = tile_time(tile, rows + used * tile_rows(tile) / 2, n, k, kKContig, bmode, device_cus(), false, kEpiStore);
+    if (tile == 0 || ti < t) {
+      best = tile;
+      t = ti;
+    }
+  }
+  if (bmode != kKContig) return best;
+  if (rows <= 12 * used) return kTileFew1;
+  if (rows <= 24 * used) return kTileFew2;
+  return best;
+}
+int pick_grad(int64_t rows, int64_t groups, int64_t m, int64_t n) {
+  int best = kTile256;
+  float t = 0.0f;
+  for (int tile = 0; tile < kFastTiles; ++tile) {
+    const int64_t bm = tile_rows(tile);
+    const float ti = tile_time(tile, groups * (cdiv(m, bm) * bm), n, cdiv(rows, groups), kMNContig, kMNContig, device_cus(),
+                               false, kEpiF32);
+    if (tile == 0 || ti < t) {
+      best = tile;
+      t = ti;
+    }
+  }
+  return best;
+}
+
+int check_sizes(int64_t groups, int64_t rows, int64_t n, int64_t k) {
+  if (groups < 1 || groups > kMaxGroups) return set_error(kInvalid, "1 to %ld groups, not %ld", (long)kMaxGroups, (long)groups);
+  if (rows < 0 || n < 1 || k < 1 || !fits_i32(rows) || !fits_i32(n) || !fits_i32(k))
+    return set_error(kInvalid, "invalid grouped product shape (%ld rows, %ld x %ld)", (long)rows, (long)n, (long)k);
+  if (n % 8 != 0 || k % 8 != 0) return set_error(kInvalid, "grouped products take widths of a multiple of 8, not %ld and %ld", (long)n, (long)k);
+  return kOk;
+}
+// Rows of whole, aligned 16-byte pieces, 256 of which span less than 2 GiB.
+int check_rows(const void* p, int64_t ld, int64_t rows, int64_t cols, const char* what) {
+  if (!al(p, 16) || ld % 8 != 0) return set_error(kInvalid, "%s rows must be 16-byte aligned", what);
+  if (rows > 1 && ld < cols) return set_error(kInvalid, "%s rows overlap", what);
+  return check_out_stride(ld > cols ? ld : cols, 2, what);
+}
+
+template <class Cfg, int BMODE>
+int launch_ring(const GroupedParams& p, int64_t grid, hipStream_t s) {
+  const void* kern = reinterpret_cast<const void*>(&grouped_ring_kernel<Cfg, BMODE>);
+  if (int rc = ensure_lds(kern, Cfg::kLds)) return rc;
+  hipLaunchKernelGGL((grouped_ring_kernel<Cfg, BMODE>), dim3((unsigned)grid), dim3(Cfg::NT), Cfg::kLds, s, p);
+  return hip_check(hipGetLastError(), "grouped product launch");
+}
+template <int BMODE>
+int run_tile(const GroupedParams& p, int tile, int64_t grid, hipStream_t s) {
+  switch (tile) {
+    case kTile256: {
+      const void* kern = reinterpret_cast<const void*>(&grouped_fast_kernel<BMODE>);
+      if (int rc = ensure_lds(kern, kFLdsBytes)) return rc;
+      const int cus = device_cus();
+      hipLaunchKernelGGL((grouped_fast_kernel<BMODE>), dim3((unsigned)(grid < cus ? grid : cus)), dim3(kFNT), kFLdsBytes, s, p);
+      return hip_check(hipGetLastError(), "grouped product launch");
+    }
+    case kTile128x2: return launch_ring<Ring128x2, BMODE>(p, grid, s);
+    case kTile128x1: return launch_ring<Ring128x1, BMODE>(p, grid, s);
+    case kTile64x128: return launch_ring<Ring64x128, BMODE>(p, grid, s);
+    case kTile64: return launch_ring<Ring64, BMODE>(p, grid, s);
+  }
+  if constexpr (BMODE == kKContig) {
+    const dim3 g((unsigned)grid), block(256);
+    if (tile == kTileFew1) hipLaunchKernelGGL((grouped_few_kernel<1>), g, block, 0, s, p);
+    else if (tile == kTileFew2) hipLaunchKernelGGL((grouped_few_kernel<2>), g, block, 0, s, p);
+    else hipLaunchKernelGGL((grouped_few_kernel<4>), g, block, 0, s, p);
+    return hip_check(hipGetLastError(), "grouped product launch");
+  }
+  return set_error(kInvalid, "no grouped tile %d", tile);
+}
+
+template <class Cfg>
+int launch_grad_ring(const GroupedGradParams& p, bool f32, int64_t grid, hipStream_t s) {
+  auto run = [&](auto kernel) {
+    if (int rc = ensure_lds(reinterpret_cast<const void*>(kernel), Cfg::kLds)) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(Cfg::NT), Cfg::kLds, s, p);
+    return hip_check(hipGetLastError(), "grouped weight gradient launch");
+  };
+  return f32 ? run(&grouped_grad_ring_kernel<Cfg, true>) : run(&grouped_grad_ring_kernel<Cfg, false>);
+}
+
+}  // namespace
+
+extern "C" int ws_grouped_tile(int64_t rows, int64_t groups, int64_t n, int64_t k, int form) {
+  if (rows < 1 || check_sizes(groups, rows, n, k)) return -1;
+  switch (form) {
+    case WS_GROUPED_NT: return pick_grouped(rows, groups, n, k, kKContig);
+    case WS_GROUPED_NN: return pick_grouped(rows, groups, n, k, kMNContig);
+    case WS_GROUPED_GRAD: return pick_grad(rows, groups, n, k);
+  }
+  return -1;
+}
+
+extern "C" int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int64_t ld_weight, int64_t group_stride,
+                             int form, const int64_t* offsets, int64_t groups, int64_t rows, int64_t n, int64_t k,
+                             void* y, int64_t ldy, void* stream) {
+  if (form != WS_GROUPED_NT && form != WS_GROUPED_NN) return set_error(kInvalid, "unknown form %d", form);
+  if (int rc = check_sizes(groups, rows, n, k)) return rc;
+  if (rows == 0) return kOk;
+  if (!x || !weight || !offsets || !y) return set_error(kInvalid, "null pointer");
+  const bool nt = form == WS_GROUPED_NT;
+  if (int rc = check_rows(x, ldx, rows, k, "x")) return rc;
+  if (int rc = check_rows(weight, ld_weight, 2, nt ? k : n, "weight")) return rc;
+  if (int rc = check_rows(y, ldy, rows, n, "y")) return rc;
+  if (group_stride % 8 != 0 || group_stride < 0) return set_error(kInvalid, "weights must be 16-byte aligned");
+  const int tile = pick_grouped(rows, groups, n, k, nt ? kKContig : kMNContig);
+  GroupedParams p{};
+  p.a = OperandDesc{static_cast<const unsigned short*>(x), ldx, 1};
+  p.b = OperandDesc{static_cast<const unsigned short*>(weight), nt ? ld_weight : 1, nt ? 1 : ld_weight};
+  p.b_group = group_stride;
+  p.offsets = reinterpret_cast<const long*>(offsets);
+  p.groups = (int)groups;
+  p.rows = (int)rows;
+  p.N = (int)n;
+  p.K = (int)k;
+  p.tiles_n = cdiv(n, tile_cols(tile));
+  p.c = static_cast<unsigned short*>(y);
+  p.ldc = ldy;
+  const int64_t grid = most_tiles(rows, groups, tile_rows(tile)) * p.tiles_n;
+  if (grid >= 1L << 22) return set_error(kInvalid, "too many tiles (%ld rows, %ld columns, %ld groups)", (long)rows, (long)n, (long)groups);
+  p.most = (int)grid;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return nt ? run_tile<kKContig>(p, tile, grid, s) : run_tile<kMNContig>(p, tile, grid, s);
+}
+
+extern "C" int ws_grouped_weight_grad(const void* dy, int64_t ld_dy, const void* x, int64_t ldx, const int64_t* offsets,
+                                      int64_t groups, int64_t rows, int64_t n, int64_t k, void* dweight,
+                                      int dweight_f32, void* stream) {
+  if (int rc = check_sizes(groups, rows, n, k)) return rc;
+  if (!dweight || !offsets || (rows > 0 && (!dy || !x))) return set_error(kInvalid, "null pointer");
+  if (int rc = check_rows(dy, ld_dy, rows, n, "dy")) return rc;
+  if (int rc = check_rows(x, ldx, rows, k, "x")) return rc;
+  if (!al(dweight, 16)) return set_error(kInvalid, "the weight gradient must be 16-byte aligned");
+  if (int rc = check_out_stride(k, dweight_f32 ? 4 : 2, "dweight")) return rc;
+  const int tile = pick_grad(rows, groups, n, k);
+  GroupedGradParams p{};
+  p.a = static_cast<const unsigned short*>(dy);
+  p.lda = ld_dy;
+  p.b = static_cast<const unsigned short*>(x);
+  p.ldb = ldx;
+  p.offsets = reinterpret_cast<const long*>(offsets);
+  p.groups = (int)groups;
+  p.rows = (int)rows;
+  p.M = (int)n;
+  p.N = (int)k;
+  p.tiles_m = cdiv(n, tile_rows(tile));
+  p.tiles_n = cdiv(k, tile_cols(tile));
+  p.g = dweight;
+  const int64_t grid = groups * p.tiles_m * p.tiles_n;
+  if (grid >= 1L << 22) return set_error(kInvalid, "too many tiles (%ld groups of %ld x %ld)", (long)groups, (long)n, (long)k);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool f32 = dweight_f32 != 0;
+  switch (tile) {
+    case kTile128x2: return launch_grad_ring<Ring128x2>(p, f32, grid, s);
+    case kTile128x1: return launch_grad_ring<Ring128x1>(p, f32, grid, s);
+    case kTile64x128: return launch_grad_ring<Ring64x128>(p, f32, grid, s);
+    case kTile64: return launch_grad_ring<Ring64>(p, f32, grid, s);
+  }
+  auto run = [&](auto kernel) {
+    if (int rc = ensure_lds(reinterpret_cast<const void*>(kernel), kFLdsBytes)) return rc;
+    const int cus = device_cus();
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(grid < cus ? grid : cus)), dim3(kFNT), kFLdsBytes, s, p);
+    return hip_check(hipGetLastError(), "grouped weight gradient launch");
+  };
+  return f32 ? run(&grouped_grad_fast_kernel<true>) : run(&grouped_grad_fast_kernel<false>);
+}

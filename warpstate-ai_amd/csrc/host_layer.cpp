@@ -1,6 +1,7 @@
-// Host side of the residual norm and the embedding as PyTorch operators in C++: the checks,
-// allocations, launches and autograd nodes of ops/residual_norm.py and ops/embedding_execution.py
-// without Python. Shapes and types only on fake tensors.
+// Host side of the residual norm, the embedding and the experts' products as PyTorch operators in
+// C++: the checks, allocations, launches and autograd nodes of ops/residual_norm.py,
+// ops/embedding_execution.py and ops/grouped_execution.py without Python. Shapes and types only on fake
+// tensors.
 //
 // Autograd kernels read no data; they call operators below autograd. First derivatives by reverse
 // mode only: tensors that carry a tangent are refused, and so is a second differentiation.
@@ -270,6 +271,141 @@ Tensor embedding_backward_meta(const Tensor& dy, const Tensor&, int64_t vocab, d
   return at::empty({vocab, dy.size(-1)}, dy.options().dtype(f32 ? at::kFloat : at::kBFloat16));
 }
 
+// --- products grouped by expert -------------------------------------------------------------
+
+constexpr char kGroupedTwice[] = "grouped products cannot be differentiated twice";
+
+void check_grouped(const Tensor& x, const Tensor& weight, const Tensor& offsets) {
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 && x.dim() == 2, "Grouped products take BF16 rows [rows, k]");
+  TORCH_CHECK_VALUE((weight.scalar_type() == at::kBFloat16 || weight.scalar_type() == at::kFloat) &&
+                        weight.dim() == 3 && weight.numel() > 0 && weight.size(2) == x.size(1) &&
+                        weight.device() == x.device(),
+                    "Expected non-empty BF16 or FP32 weights [groups, n, ", x.size(1), "] on ", x.device());
+  TORCH_CHECK_VALUE(offsets.scalar_type() == at::kLong && offsets.dim() == 1 &&
+                        offsets.size(0) == weight.size(0) + 1 && offsets.device() == x.device(),
+                    "Offsets must be an int64 vector, one more than the groups, on ", x.device());
+}
+// A matrix as the kernels read it: 16-byte rows of a multiple of 8, itself or a copy padded with
+// zeros.
+bool whole_rows(const Tensor& t) {
+  int64_t i = t.dim() - 1, inner = t.size(i);
+  if (inner % 8 != 0 || (t.stride(i) != 1 && inner != 1) || t.storage_offset() % 8 != 0) return false;
+  while (i-- > 0) {
+    if (t.size(i) > 1 && (t.stride(i) % 8 != 0 || t.stride(i) < inner)) return false;
+    inner = t.size(i) * t.stride(i);
+  }
+  return true;
+}
+Tensor grouped_operand(const Tensor& t) {
+  const Tensor b = t.to(at::kBFloat16);
+  if (whole_rows(b) && (t.dim() == 2 || t.size(1) % 8 == 0)) return b;
+  std::vector<int64_t> sizes = b.sizes().vec();
+  for (size_t i = 1; i < sizes.size(); ++i) sizes[i] = up(sizes[i], 8);
+  Tensor out = at::zeros(sizes, b.options());
+  Tensor part = out.narrow(-1, 0, b.size(-1));
+  if (t.dim() == 3) part = part.narrow(1, 0, b.size(1));
+  part.copy_(b);
+  return out;
+}
+
+// On operands of grouped_operand: [rows, n] (form NT) or [rows, k] (NN), padded widths.
+Tensor grouped_rows(const Tensor& x, const Tensor& w, const Tensor& offsets_in, int64_t form) {
+  c10::DeviceGuard guard(x.device());
+  const Tensor offsets = offsets_in.contiguous();
+  const bool nt = form == WS_GROUPED_NT;
+  const int64_t rows = x.size(0), n = w.size(nt ? 1 : 2), k = w.size(nt ? 2 : 1);
+  Tensor y = at::empty({rows, n}, x.options());
+  check(ws_grouped_mm(ptr(x), row_stride(x), w.const_data_ptr(), w.size(1) > 1 ? w.stride(1) : w.size(2),
+                      w.size(0) > 1 ? w.stride(0) : 0, (int)form, offsets.const_data_ptr<int64_t>(), w.size(0), rows,
+                      n, k, ptr(y), n, stream_of(x)),
+        "ws_grouped_mm");
+  return y;
+}
+Tensor grouped_grad(const Tensor& dy, const Tensor& x, const Tensor& offsets_in, bool f32) {
+  c10::DeviceGuard guard(x.device());
+  const Tensor offsets = offsets_in.contiguous();
+  const int64_t groups = offsets.size(0) - 1, n = dy.size(1), k = x.size(1);
+  Tensor dw = at::empty({groups, n, k}, x.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+  check(ws_grouped_weight_grad(ptr(dy), row_stride(dy), ptr(x), row_stride(x), offsets.const_data_ptr<int64_t>(),
+                               groups, x.size(0), n, k, dw.data_ptr(), f32, stream_of(x)),
+        "ws_grouped_weight_grad");
+  return dw;
+}
+typedef Tensor GroupedRows(const Tensor&, const Tensor&, const Tensor&, int64_t);
+typedef Tensor GroupedGrad(const Tensor&, const Tensor&, const Tensor&, bool);
+Tensor first_columns(const Tensor& t, int64_t cols) {
+  return t.size(-1) == cols ? t : t.narrow(-1, 0, cols).contiguous();
+}
+
+Tensor grouped_mm(const Tensor& x, const Tensor& weight, const Tensor& offsets) {
+  check_grouped(x, weight, offsets);
+  c10::DeviceGuard guard(x.device());
+  return first_columns(grouped_rows(grouped_operand(x), grouped_operand(weight), offsets, WS_GROUPED_NT),
+                       weight.size(1));
+}
+
+struct GroupedMmFn : Function<GroupedMmFn> {
+  // Gradients go to the tensors that the operands a and w were made from.
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& a, const Tensor& w,
+                        const Tensor& offsets) {
+    static const auto op = find<GroupedRows>("warpstate::native_grouped_rows");
+    at::AutoDispatchBelowAutograd guard;
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({weight.requires_grad() ? a : Tensor(), x.requires_grad() ? w : Tensor(), offsets});
+    ctx->saved_data["want_x"] = x.requires_grad();
+    ctx->saved_data["want_w"] = weight.requires_grad();
+    ctx->saved_data["n"] = weight.size(1);
+    ctx->saved_data["k"] = x.size(1);
+    ctx->saved_data["f32"] = weight.scalar_type() == at::kFloat;
+    return first_columns(op.call(a, w, offsets, WS_GROUPED_NT), weight.size(1));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static const auto rows_op = find<GroupedRows>("warpstate::native_grouped_rows");
+    static const auto grad_op = find<GroupedGrad>("warpstate::native_grouped_grad");
+    variable_list d(5);
+    if (!grads[0].defined()) return d;
+    const auto s = ctx->get_saved_variables();
+    const int64_t n = ctx->saved_data["n"].toInt(), k = ctx->saved_data["k"].toInt();
+    {
+      at::AutoDispatchBelowAutograd guard;
+      const Tensor g = grouped_operand(grads[0]);
+      if (ctx->saved_data["want_x"].toBool()) d[0] = first_columns(rows_op.call(g, s[1], s[2], WS_GROUPED_NN), k);
+      if (ctx->saved_data["want_w"].toBool()) {
+        Tensor dw = grad_op.call(g, s[0], s[2], ctx->saved_data["f32"].toBool());
+        if (dw.size(1) != n || dw.size(2) != k) dw = dw.narrow(1, 0, n).narrow(2, 0, k).contiguous();
+        d[1] = dw;
+      }
+    }
+    return once(d, {s[0], s[1], grads[0]}, kGroupedTwice);
+  }
+};
+Tensor grouped_mm_autograd(const Tensor& x, const Tensor& weight, const Tensor& offsets) {
+  refuse_tangents("grouped_mm", x, weight);
+  if (!records(x, weight)) {
+    static const auto op = find<Tensor(const Tensor&, const Tensor&, const Tensor&)>("warpstate::native_grouped_mm");
+    return below(op, x, weight, offsets);
+  }
+  check_grouped(x, weight, offsets);
+  c10::DeviceGuard guard(x.device());
+  Tensor a, w;
+  {
+    at::AutoDispatchBelowAutograd below_autograd;
+    a = grouped_operand(x.detach());
+    w = grouped_operand(weight.detach());
+  }
+  return GroupedMmFn::apply(x, weight, a, w, offsets);
+}
+Tensor grouped_mm_meta(const Tensor& x, const Tensor& weight, const Tensor& offsets) {
+  check_grouped(x, weight, offsets);
+  return at::empty({x.size(0), weight.size(1)}, x.options());
+}
+Tensor grouped_rows_meta(const Tensor& x, const Tensor& w, const Tensor&, int64_t form) {
+  return at::empty({x.size(0), w.size(form == WS_GROUPED_NT ? 1 : 2)}, x.options());
+}
+Tensor grouped_grad_meta(const Tensor& dy, const Tensor& x, const Tensor& offsets, bool f32) {
+  return at::empty({offsets.size(0) - 1, dy.size(1), x.size(1)}, x.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(warpstate, m) {
@@ -284,6 +420,9 @@ TORCH_LIBRARY_FRAGMENT(warpstate, m) {
   m.def("native_embedding(Tensor tokens, Tensor table, float scale, bool f32) -> Tensor");
   m.def("native_embedding_backward(Tensor dy, Tensor tokens, SymInt vocab, float scale, bool f32) -> Tensor");
   m.def("native_embedding_accumulate_(Tensor(a!) gradient, Tensor tokens, Tensor dy, float scale) -> ()");
+  m.def("native_grouped_mm(Tensor x, Tensor weight, Tensor offsets) -> Tensor");
+  m.def("native_grouped_rows(Tensor x, Tensor w, Tensor offsets, int form) -> Tensor");
+  m.def("native_grouped_grad(Tensor dy, Tensor x, Tensor offsets, bool f32) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(warpstate, CUDA, m) {
   m.impl("native_add_rmsnorm", &add_rmsnorm);
@@ -293,11 +432,15 @@ TORCH_LIBRARY_IMPL(warpstate, CUDA, m) {
   m.impl("native_embedding", &embedding);
   m.impl("native_embedding_backward", &embedding_backward);
   m.impl("native_embedding_accumulate_", &embedding_accumulate);
+  m.impl("native_grouped_mm", &grouped_mm);
+  m.impl("native_grouped_rows", &grouped_rows);
+  m.impl("native_grouped_grad", &grouped_grad);
 }
 TORCH_LIBRARY_IMPL(warpstate, AutogradCUDA, m) {
   m.impl("native_add_rmsnorm", &add_rmsnorm_autograd);
   m.impl("native_rmsnorm_quantize", &rmsnorm_quantize_autograd);
   m.impl("native_embedding", &embedding_autograd);
+  m.impl("native_grouped_mm", &grouped_mm_autograd);
 }
 TORCH_LIBRARY_IMPL(warpstate, Meta, m) {
   m.impl("native_add_rmsnorm", &add_rmsnorm_meta);
@@ -305,4 +448,7 @@ TORCH_LIBRARY_IMPL(warpstate, Meta, m) {
   m.impl("native_add_rmsnorm_backward", &add_rmsnorm_backward_meta);
   m.impl("native_embedding", &embedding_meta);
   m.impl("native_embedding_backward", &embedding_backward_meta);
+  m.impl("native_grouped_mm", &grouped_mm_meta);
+  m.impl("native_grouped_rows", &grouped_rows_meta);
+  m.impl("native_grouped_grad", &grouped_grad_meta);
 }

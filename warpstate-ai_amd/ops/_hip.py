@@ -118,6 +118,11 @@ SIGNATURES = {
     "ws_embedding_backward_workspace_bytes": (_i64, [_i64] * 3),
     "ws_embedding_backward": (_i32, [_c_void_p, _i64, _i32, _c_void_p, _i64, _i64, _i64, _f32,
                                      _c_void_p, _i64, _i32, _c_void_p, _c_void_p]),
+    "ws_grouped_mm": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _i64, _i32, _c_void_p, _i64, _i64,
+                             _i64, _i64, _c_void_p, _i64, _c_void_p]),
+    "ws_grouped_weight_grad": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64,
+                                      _i64, _i64, _c_void_p, _i32, _c_void_p]),
+    "ws_grouped_tile": (_i32, [_i64, _i64, _i64, _i64, _i32]),
 }
 
 
