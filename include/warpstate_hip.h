@@ -532,8 +532,8 @@ int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, const int64
 /* y [rows, n] BF16 = x [rows, k] times the transpose of the group's weight [n, k] (WS_GROUPED_NT:
  * a projection), or times its weight [k, n] itself (WS_GROUPED_NN: the input gradient of one), both
  * row-major with row stride ld_weight, group_stride elements from one group's to the next. Rows
- * before the first offset and behind the last get zeros. Sums have the order of single
- * products on the same tile, so a row's bits may differ with the number of rows and groups. */
+ * before the first offset and behind the last get zeros. The sums of the tiles have
+ * one order, that of the kernel for few rows another. */
 enum WsGroupedForm { WS_GROUPED_NT = 0, WS_GROUPED_NN = 1, WS_GROUPED_GRAD = 2 };
 int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int64_t ld_weight,
                   int64_t group_stride, int form, const int64_t* offsets, int64_t groups,
@@ -544,8 +544,8 @@ int ws_grouped_weight_grad(const void* dy, int64_t ld_dy, const void* x, int64_t
                            const int64_t* offsets, int64_t groups, int64_t rows, int64_t n,
                            int64_t k, void* dweight, int dweight_f32, void* stream);
 /* What these sizes run on, without a launch (WS_GROUPED_GRAD: the weight gradient): 0 256 x 256,
- * 1 and 2 128 x 128 (two or one workgroup on a compute unit), 3 64 x 128, 4 64 x 64, 5 to 7 the
- * kernel for few rows (16, 32 or 64 of a group at a time); -1 for invalid sizes. */
+ * 1 and 2 128 x 128 (two or one workgroup on a compute unit), 3 64 x 128, 4 64 x 64, 5 the kernel
+ * for few rows; -1 for invalid sizes. */
 int ws_grouped_tile(int64_t rows, int64_t groups, int64_t n, int64_t k, int form);
 
 #ifdef __cplusplus

@@ -65,17 +65,18 @@ def _check(x, w, dy, offsets, y, dx=None, dw=None):
             assert not t[~seen.cuda()].any()
 
 
-# Rows, groups, n, k and the tiles that they run on: forward, input gradient, weight gradient.
-TILES = [((1, 1, 8, 8), None), ((1, 5, 64, 72), None), ((7, 3, 16, 200), None), ((16, 64, 96, 264), None),
-         ((100, 9, 264, 1000), None), ((200, 8, 520, 96), None), ((300, 4, 512, 512), None),
-         ((700, 70, 64, 64), None), ((2000, 130, 128, 136), None), ((1000, 5, 256, 128), None),
-         ((3000, 3, 2048, 512), None), ((4096, 8, 1288, 1280), None), ((4096, 64, 512, 1280), None),
-         ((6000, 32, 1280, 896), None), ((8192, 4, 1280, 520), None), ((16000, 6, 2048, 1032), None)]
+# Rows, groups, n, k. The last five reach the pieces of a last round of 256 x 256 tiles (no whole
+# round before it, one, and a last round that is long enough to stay whole).
+SIZES = [(1, 1, 8, 8), (1, 5, 64, 72), (7, 3, 16, 200), (16, 64, 96, 264), (100, 9, 264, 1000), (200, 8, 520, 96),
+         (300, 4, 512, 512), (700, 70, 64, 64), (1000, 130, 128, 136), (1000, 5, 256, 128), (3000, 3, 2048, 512),
+         (4096, 8, 1288, 1280), (4096, 64, 512, 1280), (6000, 32, 1280, 896), (8192, 4, 1280, 520),
+         (2600, 2, 2056, 1544), (9000, 4, 2304, 1608), (9000, 4, 1608, 2304), (12000, 3, 2304, 1536),
+         (16000, 6, 2048, 1032)]
 
 
 @pytest.mark.parametrize("kind", ["router", "one", "gaps", "even"])
-@pytest.mark.parametrize("sizes,_tiles", TILES)
-def test_forward_and_backward(sizes, _tiles, kind):
+@pytest.mark.parametrize("sizes", SIZES)
+def test_forward_and_backward(sizes, kind):
     from ops.grouped_execution import grouped_mm
 
     rows, groups, n, k = sizes
@@ -95,9 +96,10 @@ def test_forward_and_backward(sizes, _tiles, kind):
 def test_every_tile_is_reached():
     from ops import _hip
 
-    found = {form: {_hip.query("ws_grouped_tile", *sizes, form) for sizes, _ in TILES} for form in (NT, NN, GRAD)}
-    assert {0, 1, 3, 4, 5, 6} <= found[NT], found
-    assert {0, 1, 3, 4} <= found[NN] and {0, 1, 4} <= found[GRAD], found
+    found = {form: {_hip.query("ws_grouped_tile", r, g, *((k, n) if form == NN else (n, k)), form)
+                    for r, g, n, k in SIZES} for form in (NT, NN, GRAD)}
+    assert {0, 1, 3, 4, 5} <= found[NT], found
+    assert {0, 1, 3, 4} <= found[NN] and {0, 1, 3, 4} <= found[GRAD], found
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])

@@ -43,7 +43,7 @@ static __global__ void __launch_bounds__(256) embed_lookup_kernel(const void* ta
 // `range` tokens of the vocabulary and reads all positions twice, each of its sixteen waves a
 // sixteenth of them: it counts its own tokens by wave and the ones below its range, which is
 // where its part of perm begins, and then places its own. No workgroup waits for another.
-constexpr int kSortWaves = 16, kSortRange = 512;
+constexpr int kSortWaves = 16, kSortRange = 512, kSortAhead = 16;
 
 static __global__ void __launch_bounds__(64 * kSortWaves) embed_sort_kernel(const long* __restrict__ tokens, int rows,
                                                                             int vocab, int range,
@@ -58,12 +58,24 @@ static __global__ void __launch_bounds__(64 * kSortWaves) embed_sort_kernel(cons
   int* const mine = count[wave];
   for (int r = lane; r < n; r += 64) mine[r] = 0;
   __syncthreads();
-  int less = 0;
-#pragma unroll 4
-  for (int t = begin + lane; t < end; t += 64) {
-    const long token = tokens[t];
-    less += token >= 0 && token < lo;
-    if (token >= lo && token < lo + n) atomicAdd(&mine[token - lo], 1);
+  // kSortAhead tokens a lane at a time, as distances from the range's first; outside the vocabulary, or
+  // past the end, kNoToken.
+  constexpr int kNoToken = 0x7fffffff;
+  auto load = [&](int t0, int (&r)[kSortAhead]) {
+    long token[kSortAhead];
+#pragma unroll
+    for (int a = 0; a < kSortAhead; ++a) token[a] = t0 + 64 * a + lane < end ? tokens[t0 + 64 * a + lane] : -1;
+#pragma unroll
+    for (int a = 0; a < kSortAhead; ++a) r[a] = token[a] >= 0 && token[a] < vocab ? (int)token[a] - lo : kNoToken;
+  };
+  int less = 0, r[kSortAhead];
+  for (int t0 = begin; t0 < end; t0 += 64 * kSortAhead) {
+    load(t0, r);
+#pragma unroll
+    for (int a = 0; a < kSortAhead; ++a) {
+      less += r[a] < 0;
+      if (r[a] >= 0 && r[a] < n) atomicAdd(&mine[r[a]], 1);
+    }
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) less += __shfl_xor(less, off, kWave);
@@ -96,19 +108,19 @@ static __global__ void __launch_bounds__(64 * kSortWaves) embed_sort_kernel(cons
     if (lo + tid == vocab - 1) start[vocab] = at;
   }
   __syncthreads();
-  for (int t0 = begin; t0 < end; t0 += 64) {
-    const int t = t0 + lane;
-    const long token = t < end ? tokens[t] : -1;
-    const bool member = token >= lo && token < lo + n;
-    const int r = member ? (int)(token - lo) : -1;
-    // One token of the 64 positions at a time; its lanes are in the order of the positions.
-    for (unsigned long todo = __builtin_amdgcn_ballot_w64(member); todo != 0;) {
-      const int v = __builtin_amdgcn_readlane(r, __builtin_ctzl(todo));
-      const unsigned long same = __builtin_amdgcn_ballot_w64(r == v);
-      const int first = mine[v];
-      if (r == v) perm[first + __builtin_popcountl(same & ((1ul << lane) - 1))] = t;
-      mine[v] = first + __builtin_popcountl(same);  // by every lane, the same value
-      todo &= ~same;
+  for (int t0 = begin; t0 < end; t0 += 64 * kSortAhead) {
+    if (end - begin > 64 * kSortAhead) load(t0, r);  // else they are there still
+#pragma unroll
+    for (int a = 0; a < kSortAhead; ++a) {
+      // One token of the 64 positions at a time; its lanes are in the order of the positions.
+      for (unsigned long todo = __builtin_amdgcn_ballot_w64(r[a] >= 0 && r[a] < n); todo != 0;) {
+        const int v = __builtin_amdgcn_readlane(r[a], __builtin_ctzl(todo));
+        const unsigned long same = __builtin_amdgcn_ballot_w64(r[a] == v);
+        const int first = mine[v];
+        if (r[a] == v) perm[first + __builtin_popcountl(same & ((1ul << lane) - 1))] = t0 + 64 * a + lane;
+        mine[v] = first + __builtin_popcountl(same);  // by every lane, the same value
+        todo &= ~same;
+      }
     }
   }
 }
@@ -129,99 +141,193 @@ struct EmbedGradParams {
 };
 enum EmbedOut { kEmbedBF16 = 0, kEmbedF32 = 1, kEmbedAdd = 2 };
 
-// Sum of dy at perm[begin .. end) for the 8 NC columns at c, c + 512, ..: the positions of 64 rows
-// are one load, a position on each lane, then four rows of dy at a time are in flight. All 64 lanes
-// come here, those past the last column too: each holds a position that the others read.
-template <bool GF32, int NC, bool VEC>
-__device__ __forceinline__ void embed_sum(const EmbedGradParams& p, int begin, int end, int c, int lane,
-                                          float (&acc)[NC][8]) {
+// W elements of a row, 8 or 4: an FP32 output's pieces are four columns wide, so that a wave's stores
+// cover whole lines (16384 x 2048 into 32768 rows, us, pieces of 8 / 4: @E8@ / @E4@).
+template <bool F32, int W>
+struct EmbedPiece {
+  unsigned w[F32 ? W : W / 2];
+  __device__ __forceinline__ float at(int e) const {
+    if constexpr (F32) return __uint_as_float(w[e]);
+    else return (e & 1) ? hi_bf16(w[e >> 1]) : lo_bf16(w[e >> 1]);
+  }
+};
+template <bool F32, int W, bool VEC>
+__device__ __forceinline__ EmbedPiece<F32, W> embed_load(const void* base, long at, int left) {
+  constexpr int kWords = F32 ? W : W / 2;
+  EmbedPiece<F32, W> v;
+  const char* src = static_cast<const char*>(base) + at * (F32 ? 4 : 2);
+  if (VEC && left >= W) {
+    if constexpr (kWords == 2) {
+      const u32x2_t a = *reinterpret_cast<const u32x2_t*>(src);
+      v.w[0] = a[0];
+      v.w[1] = a[1];
+    } else {
 #pragma unroll
-  for (int i = 0; i < NC; ++i)
+      for (int q = 0; q < kWords / 4; ++q) {
+        const u32x4_t a = reinterpret_cast<const u32x4_t*>(src)[q];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[i][e] = 0.0f;
+        for (int d = 0; d < 4; ++d) v.w[4 * q + d] = a[d];
+      }
+    }
+    return v;
+  }
+#pragma unroll
+  for (int d = 0; d < kWords; ++d) v.w[d] = 0;
+  if (VEC) return v;  // whole pieces only
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    if (e >= left) continue;
+    if constexpr (F32) v.w[e] = reinterpret_cast<const unsigned*>(src)[e];
+    else v.w[e >> 1] |= (unsigned)reinterpret_cast<const unsigned short*>(src)[e] << (16 * (e & 1));
+  }
+  return v;
+}
+template <bool F32, int W, bool VEC>
+__device__ __forceinline__ void embed_write(const float (&f)[W], void* base, long at, int left) {
+  char* dst = static_cast<char*>(base) + at * (F32 ? 4 : 2);
+  if (VEC && left >= W) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int q = 0; q < W / 4; ++q)
+        reinterpret_cast<f32x4_t*>(dst)[q] = f32x4_t{f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]};
+    } else {
+      static_assert(F32 || W == 8, "BF16 pieces are 16 bytes");
+      *reinterpret_cast<u32x4_t*>(dst) = u32x4_t{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
+                                                 pack_bf16x2(f[W - 4], f[W - 3]), pack_bf16x2(f[W - 2], f[W - 1])};
+    }
+    return;
+  }
+  if (VEC) return;
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    if (e >= left) continue;
+    if constexpr (F32) reinterpret_cast<float*>(dst)[e] = f[e];
+    else reinterpret_cast<unsigned short*>(dst)[e] = to_bf16_bits(f[e]);
+  }
+}
+
+// Walks the positions [begin, end) of perm with the sums of dy over the NC pieces of W columns at c,
+// c + 64 W, ..: the positions of 64 rows are one load, a position on each lane (so all 64 lanes come here, those
+// past the last column too), and then kAhead rows of dy at a time are in flight. `before(at, acc)`
+// comes before the row at position `at` is added, and may store the sums and clear them.
+template <bool GF32, int NC, int W, bool VEC, class Before>
+__device__ __forceinline__ void embed_walk(const EmbedGradParams& p, int begin, int end, int c, int lane,
+                                           float (&acc)[NC][W], Before&& before) {
   constexpr int kAhead = GF32 ? 2 : 4;
   for (int b = begin; b < end; b += 64) {
     const int n = min(64, end - b);
     const int rows = lane < n ? p.perm[b + lane] : 0;
     for (int j = 0; j < n; j += kAhead) {
-      QuantRow<GF32> v[kAhead][NC];
+      EmbedPiece<GF32, W> v[kAhead][NC];
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
         const long row = __builtin_amdgcn_readlane(rows, min(j + a, n - 1));
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-          load_piece<GF32, VEC>(v[a][i], p.dy, row * p.ld_dy + c + 512 * i, p.d - c - 512 * i);
+          v[a][i] = embed_load<GF32, W, VEC>(p.dy, row * p.ld_dy + c + 64 * W * i, p.d - c - 64 * W * i);
       }
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
         if (j + a >= n) break;
+        before(b + j + a);
 #pragma unroll
         for (int i = 0; i < NC; ++i)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) acc[i][e] += v[a][i].at(e);
+          for (int e = 0; e < W; ++e) acc[i][e] += v[a][i].at(e);
       }
     }
   }
 }
-
-template <int OUT, bool VEC>
-__device__ __forceinline__ void embed_store(const EmbedGradParams& p, int v, int c, float (&acc)[8]) {
-  const long at = v * p.ld_out + c;
+template <int NC, int W>
+__device__ __forceinline__ void embed_clear(float (&acc)[NC][W]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] *= p.scale;
-  if constexpr (OUT == kEmbedAdd) {
-    QuantRow<true> old;
-    load_piece<true, VEC>(old, p.out, at, p.d - c);
+  for (int i = 0; i < NC; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += old.at(e);
-  }
-  store_piece<OUT != kEmbedBF16, VEC>(round_piece<OUT != kEmbedBF16>(acc), p.out, at, p.d - c);
+    for (int e = 0; e < W; ++e) acc[i][e] = 0.0f;
 }
 
-// A wave per piece of the sorted positions, then a wave per row of the table.
+template <int OUT, int W, bool VEC>
+__device__ __forceinline__ void embed_store(const EmbedGradParams& p, long v, int c, float (&acc)[W]) {
+  const long at = v * p.ld_out + c;
+#pragma unroll
+  for (int e = 0; e < W; ++e) acc[e] *= p.scale;
+  if constexpr (OUT == kEmbedAdd) {
+    const auto old = embed_load<true, W, VEC>(p.out, at, p.d - c);
+#pragma unroll
+    for (int e = 0; e < W; ++e) acc[e] += old.at(e);
+  }
+  embed_write<OUT != kEmbedBF16, W, VEC>(acc, p.out, at, p.d - c);
+}
+
+// A wave per piece of the sorted positions, then a wave per kEmbedRows rows of the table, whose
+// positions lie one after the other: the rows of dy of all of them are requested as one run, so
+// that a row with one token or none, the usual one, does not wait for its own chain of loads.
+constexpr int kEmbedRows = 4;
+
 template <bool GF32, int OUT, bool VEC>
 static __global__ void __launch_bounds__(256) embed_grad_kernel(const EmbedGradParams p) {
-  constexpr int NC = 4;
+  constexpr int W = OUT == kEmbedBF16 ? 8 : 4, NC = 32 / W, kSpan = 64 * W;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long task = blockIdx.x * 4L + wave;
-  float acc[NC][8];
+  float acc[NC][W];
   if (task < p.pieces) {
     const int total = p.start[p.vocab], begin = (int)task * p.piece;
     if (begin >= total) return;
     const int end = (int)min((long)total, (long)begin + p.piece);
     const long first = p.tokens[p.perm[begin]], last = p.tokens[p.perm[end - 1]];
-#pragma unroll
+#pragma unroll 1
     for (int part = 0; part < 2; ++part) {
       if (part == 1 && last == first) break;
       const long v = part ? last : first;
       const int s = p.start[v], e = p.start[v + 1];
       if (e - s <= p.piece) continue;
-      for (int c0 = 0; c0 < p.d; c0 += 512 * NC) {
-        const int c = c0 + 8 * lane;
-        embed_sum<GF32, NC, VEC>(p, part ? s : begin, part ? end : min(e, end), c, lane, acc);
+      for (int c0 = 0; c0 < p.d; c0 += kSpan * NC) {
+        const int c = c0 + W * lane;
+        embed_clear(acc);
+        embed_walk<GF32, NC, W, VEC>(p, part ? s : begin, part ? end : min(e, end), c, lane, acc, [](int) {});
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-          if (c + 512 * i < p.d)
-            store_piece<true, true>(round_piece<true>(acc[i]), p.partial,
-                                    (2 * task + part) * p.ld_partial + c + 512 * i, 8);
+          if (c + kSpan * i < p.d)
+            embed_write<true, W, true>(acc[i], p.partial, (2 * task + part) * p.ld_partial + c + kSpan * i, W);
       }
     }
     return;
   }
-  const int v = (int)(task - p.pieces);
-  if (v >= p.vocab) return;
-  const int s = p.start[v], e = p.start[v + 1];
-  if (e - s > p.piece || (OUT == kEmbedAdd && s == e)) return;
-  for (int c0 = 0; c0 < p.d; c0 += 512 * NC) {
-    const int c = c0 + 8 * lane;
-    embed_sum<GF32, NC, VEC>(p, s, e, c, lane, acc);
+  const long v0 = (task - p.pieces) * kEmbedRows;
+  if (v0 >= p.vocab) return;
+  const int rows = (int)min((long)kEmbedRows, p.vocab - v0);
+  // Lane r: where row r's positions begin (lane `rows`: where the last one's end).
+  const int begins = p.start[v0 + min(lane, rows)];
+  for (int c0 = 0; c0 < p.d; c0 += kSpan * NC) {
+    const int c = c0 + W * lane;
+    int r = 0;
+    // Row r is complete: stored, unless its token is summed in pieces (or nothing is added to it).
+    auto store = [&]() {
+      const int n = __builtin_amdgcn_readlane(begins, r + 1) - __builtin_amdgcn_readlane(begins, r);
+      if (n <= p.piece && (OUT != kEmbedAdd || n > 0)) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      if (c + 512 * i < p.d) embed_store<OUT, VEC>(p, v, c + 512 * i, acc[i]);
+        for (int i = 0; i < NC; ++i)
+          if (c + kSpan * i < p.d) embed_store<OUT, W, VEC>(p, v0 + r, c + kSpan * i, acc[i]);
+      }
+      embed_clear(acc);
+      ++r;
+    };
+    embed_clear(acc);
+    // Runs of rows between tokens that are summed in pieces.
+    while (r < rows) {
+      int to = r;
+      while (to < rows && __builtin_amdgcn_readlane(begins, to + 1) - __builtin_amdgcn_readlane(begins, to) <= p.piece) ++to;
+      embed_walk<GF32, NC, W, VEC>(p, __builtin_amdgcn_readlane(begins, r), __builtin_amdgcn_readlane(begins, to), c, lane, acc,
+                                [&](int at) {
+                                  while (at >= __builtin_amdgcn_readlane(begins, r + 1)) store();
+                                });
+      while (r < to || (r == to && r < rows)) store();  // the rest of the run, and the token after it
+    }
   }
 }
 
-// Adds the pieces of the token that begins in piece blockIdx.x and runs past it, in their order.
+// Adds the pieces of the token that begins in piece blockIdx.x and runs past it, in their order: a
+// quarter of them on each wave, 64 W columns a workgroup.
 template <int OUT, bool VEC>
 static __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedGradParams p) {
   const int total = p.start[p.vocab], q = blockIdx.x, begin = q * p.piece;
@@ -230,20 +336,33 @@ static __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedGradP
   const long v = p.tokens[p.perm[end - 1]];
   const int s = p.start[v], e = p.start[v + 1];
   if (e - s <= p.piece || s < begin) return;
-  const int c = 8 * (blockIdx.y * 256 + threadIdx.x);
-  if (c >= p.d) return;
-  QuantRow<true> x;
-  load_piece<true, true>(x, p.partial, (2L * q + (s > begin)) * p.ld_partial + c, 8);
-  float acc[8];
+  constexpr int W = OUT == kEmbedBF16 ? 8 : 4;
+  __shared__ float sums[4][W][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = W * (blockIdx.y * 64 + lane);
+  const int n = cdiv(e, p.piece) - q, share = cdiv(n, 4);  // pieces q .. q + n - 1
+  float acc[W] = {};
+  constexpr int kAhead = 8;
+  const int to = min(n, (wave + 1) * share);
+  for (int i = wave * share; i < to; i += kAhead) {
+    EmbedPiece<true, W> x[kAhead];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i] = x.at(i);
-#pragma unroll 4
-  for (int next = q + 1; (long)next * p.piece < e; ++next) {
-    load_piece<true, true>(x, p.partial, 2L * next * p.ld_partial + c, 8);
+    for (int a = 0; a < kAhead; ++a) {
+      const long row = 2L * (q + i + a) + (i + a == 0 && s > begin);
+      x[a] = embed_load<true, W, true>(p.partial, row * p.ld_partial + c, i + a < to && c < p.d ? W : 0);
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] += x.at(i);
+    for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+      for (int k = 0; k < W; ++k) acc[k] += x[a].at(k);
   }
-  embed_store<OUT, VEC>(p, (int)v, c, acc);
+#pragma unroll
+  for (int k = 0; k < W; ++k) sums[wave][k][lane] = acc[k];
+  __syncthreads();
+  if (wave > 0 || c >= p.d) return;
+#pragma unroll
+  for (int k = 0; k < W; ++k) acc[k] = (sums[0][k][lane] + sums[1][k][lane]) + (sums[2][k][lane] + sums[3][k][lane]);
+  embed_store<OUT, W, VEC>(p, v, c, acc);
 }
 
 }  // namespace ws

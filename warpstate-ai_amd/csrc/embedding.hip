@@ -39,12 +39,12 @@ GradLayout grad_layout(int64_t rows, int64_t vocab, int64_t d) {
 
 template <bool GF32, int OUT>
 int launch_grad(const EmbedGradParams& p, bool vec, hipStream_t s) {
-  const dim3 grid((unsigned)cdiv((long)p.pieces + p.vocab, 4)), block(256);
+  const dim3 grid((unsigned)cdiv(p.pieces + cdiv(p.vocab, kEmbedRows), 4)), block(256);
   if (vec) hipLaunchKernelGGL((embed_grad_kernel<GF32, OUT, true>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((embed_grad_kernel<GF32, OUT, false>), grid, block, 0, s, p);
   if (int rc = hip_check(hipGetLastError(), "embedding gradient launch")) return rc;
   if (p.pieces == 0) return kOk;
-  const dim3 join(p.pieces, cdiv(p.d, 2048));
+  const dim3 join(p.pieces, cdiv(p.d, OUT == kEmbedBF16 ? 512 : 256));
   if (vec) hipLaunchKernelGGL((embed_join_kernel<OUT, true>), join, block, 0, s, p);
   else hipLaunchKernelGGL((embed_join_kernel<OUT, false>), join, block, 0, s, p);
   return hip_check(hipGetLastError(), "embedding gradient join launch");

@@ -27,6 +27,8 @@ struct GroupedParams {
   const long* offsets;          // [groups + 1]
   int groups, rows, N, K, tiles_n;
   int most;                     // tiles that the grid is sized for
+  // 256 x 256 tiles: a last round of at most `tail` tiles is left to the tail kernel (-1: none is).
+  int round, tail;
   unsigned short* c; long ldc;
 };
 
@@ -98,6 +100,12 @@ __device__ __forceinline__ GemmParams store_params(unsigned short* c, long ldc, 
   return e;
 }
 
+// Of `total` 256 x 256 tiles, those that are done whole.
+__device__ __forceinline__ int whole_tiles(const GroupedParams& p, int total) {
+  const int rest = total % p.round;
+  return rest <= p.tail ? total - rest : total;
+}
+
 // 256 x 256 tiles, a workgroup per compute unit looping over them.
 template <int BMODE>
 __global__ void __launch_bounds__(kFNT) grouped_fast_kernel(const GroupedParams p) {
@@ -110,7 +118,7 @@ __global__ void __launch_bounds__(kFNT) grouped_fast_kernel(const GroupedParams 
   const unsigned abase = lds0 + frag_base<kKContig>(wm * TM, lane);
   const unsigned bbase = lds0 + 2 * kFTileBytes + frag_base<BMODE>(wn * TN, lane);
   GroupLanes v;
-  const int total = count_tiles<kFBM>(p, lane, v);
+  const int total = whole_tiles(p, count_tiles<kFBM>(p, lane, v));
   for (int w = blockIdx.x; w < total; w += gridDim.x) {
     // The groups are read again for each tile: kept over the k-loop they would cost it registers.
     int l = lane;
@@ -160,6 +168,39 @@ __global__ void __launch_bounds__(Cfg::NT) grouped_ring_kernel(const GroupedPara
                                rsmem + wave * epi_wave<FA, FB>());
 }
 
+// The last round's tiles in pieces of 64 x 128, one workgroup each, where they would leave most compute
+// units idle: as many of a tile's products again, but all units take part. The sums have the
+// 256 x 256 tile's order, so the bits do not tell which kernel made them.
+constexpr int kTailRows = 64, kTailCols = 128, kTailPieces = (kFBM / kTailRows) * (kFBN / kTailCols);
+
+template <class Cfg, int BMODE>
+__global__ void __launch_bounds__(Cfg::NT) grouped_tail_kernel(const GroupedParams p) {
+  constexpr int FA = Cfg::FA, FB = Cfg::FB, TM = Cfg::TM, TN = Cfg::TN;
+  static_assert(Cfg::BM == kTailRows && Cfg::BN == kTailCols, "pieces of a tile");
+  extern __shared__ __attribute__((aligned(1024))) unsigned char rsmem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+  GroupLanes v;
+  const int total = count_tiles<kFBM>(p, lane, v), whole = whole_tiles(p, total);
+  const int pieces = (total - whole) * kTailPieces;
+  if ((int)blockIdx.x >= pieces) return;
+  const int x = xcd_remap(blockIdx.x, pieces, kRingWindow), piece = x % kTailPieces;
+  const GroupTile t = find_tile<kFBM>(p, whole + x / kTailPieces, lane, v);
+  int tm, tn;
+  tile_position(t.index, cdiv(t.hi - t.lo, kFBM), p.tiles_n, tm, tn);
+  const int row0 = t.lo + tm * kFBM + piece / 2 * kTailRows, col0 = tn * kFBN + piece % 2 * kTailCols;
+  if (row0 >= t.hi || col0 >= p.N) return;
+  OperandDesc b = p.b;
+  b.ptr += max(t.group, 0) * p.b_group;
+  Acc16<FA, FB> acc;
+  ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.N, 0, p.K, 0,
+                                           t.group < 0 ? 0 : cdiv(p.K, kFBK), rsmem, wave, lane);
+  const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
+  FEpiStore<false, false>::run(e, acc, row0 + wm * TM, col0 + wn * TN, lane, tm, tn, wn,
+                               rsmem + wave * epi_wave<FA, FB>());
+}
+
 // --------------------------------------------------------------------------------------
 // Weight gradients: [M, N] per group, reduced over the group's rows.
 
@@ -175,11 +216,26 @@ struct GradTile {
   OperandDesc a, b;
   int group, K, tm, tn;
 };
-__device__ __forceinline__ GradTile grad_tile(const GroupedGradParams& p, int w) {
-  const int per = p.tiles_m * p.tiles_n;
+// Groups in the order in which their tiles are dealt out, lane r the group with the r-th most rows:
+// the tiles of one group take as long as it has rows, and long ones that come last leave the others
+// waiting. More than 64 groups keep their own order.
+__device__ __forceinline__ int grad_order(const GroupedGradParams& p, int lane) {
+  if (p.groups > 64) return lane;
+  int lo = 0, hi = 0;
+  if (lane < p.groups) group_rows(p.offsets, p.groups, p.rows, lane + 1, lo, hi);
+  const int rows = max(0, hi - lo);
+  int rank = lane < p.groups ? 0 : lane;
+  for (int j = 0; j < p.groups; ++j) {
+    const int other = __builtin_amdgcn_readlane(rows, j);
+    if (lane < p.groups) rank += other > rows || (other == rows && j < lane);
+  }
+  return __builtin_amdgcn_ds_permute(4 * rank, lane);
+}
+__device__ __forceinline__ GradTile grad_tile(const GroupedGradParams& p, int w, int order) {
+  const int per = p.tiles_m * p.tiles_n, place = w / per;
   GradTile t;
-  t.group = w / per;
-  tile_position(w - t.group * per, p.tiles_m, p.tiles_n, t.tm, t.tn);
+  t.group = p.groups > 64 ? place : __builtin_amdgcn_readlane(order, place);
+  tile_position(w - place * per, p.tiles_m, p.tiles_n, t.tm, t.tn);
   int lo, hi;
   group_rows(p.offsets, p.groups, p.rows, t.group + 1, lo, hi);
   t.K = max(0, hi - lo);
@@ -209,9 +265,11 @@ __global__ void __launch_bounds__(kFNT) grouped_grad_fast_kernel(const GroupedGr
   const unsigned lds0 = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)fsmem;
   const unsigned abase = lds0 + frag_base<kMNContig>(wm * TM, lane);
   const unsigned bbase = lds0 + 2 * kFTileBytes + frag_base<kMNContig>(wn * TN, lane);
-  const int total = p.groups * p.tiles_m * p.tiles_n;
+  const int total = p.groups * p.tiles_m * p.tiles_n, order = grad_order(p, lane);
   for (int w = blockIdx.x; w < total; w += gridDim.x) {
-    const GradTile t = grad_tile(p, xcd_remap(w, total, gridDim.x));
+    // Every other round runs backwards, so that a unit with a long tile in one has a short one in the next.
+    const int round = w / (int)gridDim.x, base = round * gridDim.x, x = xcd_remap(w, total, gridDim.x);
+    const GradTile t = grad_tile(p, round & 1 ? 2 * base + min((int)gridDim.x, total - base) - 1 - x : x, order);
     Acc16<4, 8> acc;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -230,7 +288,7 @@ __global__ void __launch_bounds__(Cfg::NT) grouped_grad_ring_kernel(const Groupe
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
-  const GradTile t = grad_tile(p, xcd_remap(blockIdx.x, gridDim.x, kRingWindow));
+  const GradTile t = grad_tile(p, xcd_remap(blockIdx.x, gridDim.x, kRingWindow), grad_order(p, lane));
   Acc16<Cfg::FA, Cfg::FB> acc;
   ring_k_loop<Cfg, kMNContig, kMNContig, false>(acc, t.a, t.tm * Cfg::BM, p.M, t.b, t.tn * Cfg::BN, p.N, 0, t.K, 0,
                                                 cdiv(t.K, kFBK), rsmem, wave, lane);
@@ -239,17 +297,16 @@ __global__ void __launch_bounds__(Cfg::NT) grouped_grad_ring_kernel(const Groupe
 }
 
 // --------------------------------------------------------------------------------------
-// Few rows for each group: tiles of 16 MT rows x 32 columns, one workgroup of four waves, each
+// Few rows for each group: tiles of 16 rows x 32 columns, one workgroup of four waves, each
 // with a quarter of the reduction (64 of every 256 k, so that together they read whole rows of the
 // weight). Fragments go from memory to registers as they are: a lane's piece is 16 bytes of one row,
 // and a k-tile's two pieces of a row are one line. The waves' sums are added through LDS, in
 // wave order. Rows and columns past the group's and the weight's read the last ones and are not
 // stored.
-constexpr int kFewCols = 32;
+constexpr int kFewRows = 16, kFewCols = 32;
 
-template <int MT>
-__global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedParams p) {
-  constexpr int BM = 16 * MT;
+static __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedParams p) {
+  constexpr int BM = kFewRows;
   __shared__ float sums[4][BM][kFewCols + 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   GroupLanes v;
@@ -257,24 +314,18 @@ __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedParams p)
   const GroupTile t = find_tile<BM>(p, blockIdx.x, lane, v);
   const int tm = t.index / p.tiles_n, tn = t.index - tm * p.tiles_n;
   const int row0 = t.lo + tm * BM, col0 = tn * kFewCols;
-  f32x4_v acc[MT][2];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+  f32x4_v acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
   if (t.group >= 0) {
     const int r = lane & 15, q = 8 * (lane >> 4);
-    const unsigned short* a[MT];
+    const unsigned short* const a = p.a.ptr + (long)min(row0 + r, t.hi - 1) * p.a.s_row + q;
     const unsigned short* b[2];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) a[i] = p.a.ptr + (long)min(row0 + 16 * i + r, t.hi - 1) * p.a.s_row + q;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
       b[j] = p.b.ptr + t.group * p.b_group + (long)min(col0 + 16 * j + r, p.N - 1) * p.b.s_row + q;
     // U k-tiles at a time, all of their pieces requested before the first product.
     auto steps = [&](int k, auto count, auto load) {
       constexpr int U = decltype(count)::value;
-      bf16x8_t fa[U][2][MT], fb[U][2][2];
+      bf16x8_t fa[U][2], fb[U][2][2];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -282,8 +333,7 @@ __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedParams p)
           const int at = k + 256 * u + 32 * s;
 #pragma unroll
           for (int j = 0; j < 2; ++j) fb[u][s][j] = load(b[j], at);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) fa[u][s][i] = load(a[i], at);
+          fa[u][s] = load(a, at);
         }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -291,13 +341,11 @@ __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedParams p)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[u][s][j], fa[u][s][i], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < 2; ++j)
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[u][s][j], fa[u][s], acc[j], 0, 0, 0);
     };
     const auto whole = [](const unsigned short* row, int at) { return *reinterpret_cast<const bf16x8_t*>(row + at); };
-    constexpr int U = MT < 4 ? 4 : 2;
+    constexpr int U = 4;
     int k = 64 * wave;
     for (; k + 256 * (U - 1) + 64 <= p.K; k += 256 * U) steps(k, std::integral_constant<int, U>{}, whole);
     for (; k + 64 <= p.K; k += 256) steps(k, std::integral_constant<int, 1>{}, whole);
@@ -309,21 +357,16 @@ __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedParams p)
       });
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      *reinterpret_cast<f32x4_v*>(&sums[wave][16 * i + (lane & 15)][16 * j + 4 * (lane >> 4)]) = acc[i][j];
+  for (int j = 0; j < 2; ++j)
+    *reinterpret_cast<f32x4_v*>(&sums[wave][lane & 15][16 * j + 4 * (lane >> 4)]) = acc[j];
   __syncthreads();
+  const int m = threadIdx.x >> 4, n = 2 * (threadIdx.x & 15);
+  float v2[2];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = 16 * i + (threadIdx.x >> 4), n = 2 * (threadIdx.x & 15);
-    float v[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      v[e] = (sums[0][m][n + e] + sums[1][m][n + e]) + (sums[2][m][n + e] + sums[3][m][n + e]);
-    if (row0 + m < t.hi && col0 + n < p.N)  // N is a multiple of 8
-      *reinterpret_cast<unsigned*>(p.c + (long)(row0 + m) * p.ldc + col0 + n) = pack_bf16x2(v[0], v[1]);
-  }
+  for (int e = 0; e < 2; ++e)
+    v2[e] = (sums[0][m][n + e] + sums[1][m][n + e]) + (sums[2][m][n + e] + sums[3][m][n + e]);
+  if (row0 + m < t.hi && col0 + n < p.N)  // N is a multiple of 8
+    *reinterpret_cast<unsigned*>(p.c + (long)(row0 + m) * p.ldc + col0 + n) = pack_bf16x2(v2[0], v2[1]);
 }
 
 }  // namespace ws

@@ -8,21 +8,24 @@ using namespace ws;
 namespace {
 
 constexpr int64_t kMaxGroups = 65536;
-// Beside FastTile: the kernel for few rows, by its row tiles of 16.
-constexpr int kTileFew1 = kFastTiles, kTileFew2 = kFastTiles + 1, kTileFew4 = kFastTiles + 2;
+// Beside FastTile: the kernel for few rows.
+constexpr int kTileFew = kFastTiles;
+// The last round of 256 x 256 tiles goes in pieces where it has at most this many tiles for 256 compute
+// units, and the reduction at least kTailK: us of the round whole / in pieces, by its cost: 32 tiles 1.0 /
+// 0.34 a k-tile, 64 1.0 / 0.5, 96 1.1 / 0.84, 128 1.1 / 1.0; the kernel itself takes 4 us.
+constexpr int kTailOf256 = 112, kTailK = 1536;
 
 int tile_rows(int tile) {
   switch (tile) {
     case kTile256: return 256;
     case kTile128x2:
     case kTile128x1: return 128;
-    case kTileFew1: return 16;
-    case kTileFew2: return 32;
+    case kTileFew: return kFewRows;
     default: return 64;
   }
 }
 int tile_cols(int tile) {
-  return tile >= kTileFew1 ? kFewCols : tile == kTile256 ? 256 : tile == kTile64 ? 64 : 128;
+  return tile == kTileFew ? kFewCols : tile == kTile256 ? 256 : tile == kTile64 ? 64 : 128;
 }
 // Tiles of `rows` rows that any offsets make at most: a group ends in a part of one. (The rows of
 // no group form two more.)
@@ -31,22 +34,33 @@ int64_t most_tiles(int64_t rows, int64_t groups, int bm) {
   return rows / bm + used;
 }
 
-// The tile for rows that are spread over the groups: by the cost table of single products, with
-// half a tile more rows for each group, which is what ragged ends cost on average.
+// The tile for rows that are spread over the groups: by the cost table of single products, for the
+// rows of the tiles that a group of average size makes (its last one is half full on average, and
+// there is one).
 int pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int bmode) {
   const int64_t used = groups < rows ? groups : rows;
+  // Up to 8 rows for each group (us, this kernel / the best tile): 64 rows in 8 groups of 5632 x 2048 41 /
+  // 43, 128 rows 54 / 42; 256 in 32 of 1280 x 896 17 / 17, 512 23 / 18.
+  if (bmode == kKContig && rows <= 8 * used) return kTileFew;
   int best = kTile256;
   float t = 0.0f;
   for (int tile = 0; tile < kFastTiles; ++tile) {
-    const float ti = tile_time(tile, rows + used * tile_rows(tile) / 2, n, k, kKContig, bmode, device_cus(), false, kEpiStore);
+    const int64_t bm = tile_rows(tile);
+    int64_t wide = rows + used * bm / 2;
+    if (wide < used * bm) wide = used * bm;
+    float ti = tile_time(tile, wide, n, k, kKContig, bmode, device_cus(), false, kEpiStore);
+    if (tile == kTile256 && k >= kTailK) {
+      const TileCost& c = tile_cost(tile, kKContig, bmode);
+      const int64_t tiles = cdiv(wide, 256) * (int64_t)cdiv(n, 256), rest = tiles % device_cus();
+      if (rest * 256 <= (int64_t)kTailOf256 * device_cus())
+        ti = (float)(tiles / device_cus()) * (c.alone * (float)cdiv(k, kFBK) + c.fixed) + 4.0f +
+             tile_time(kTile64x128, rest * 256, 256, k, kKContig, bmode, device_cus(), false, kEpiStore);
+    }
     if (tile == 0 || ti < t) {
       best = tile;
       t = ti;
     }
   }
-  if (bmode != kKContig) return best;
-  if (rows <= 12 * used) return kTileFew1;
-  if (rows <= 24 * used) return kTileFew2;
   return best;
 }
 int pick_grad(int64_t rows, int64_t groups, int64_t m, int64_t n) {
@@ -86,25 +100,33 @@ int launch_ring(const GroupedParams& p, int64_t grid, hipStream_t s) {
   return hip_check(hipGetLastError(), "grouped product launch");
 }
 template <int BMODE>
+int launch_whole(GroupedParams p, int64_t grid, hipStream_t s) {
+  const void* kern = reinterpret_cast<const void*>(&grouped_fast_kernel<BMODE>);
+  if (int rc = ensure_lds(kern, kFLdsBytes)) return rc;
+  const int cus = device_cus();
+  p.round = cus;
+  p.tail = p.K >= kTailK ? kTailOf256 * cus / 256 : -1;
+  hipLaunchKernelGGL((grouped_fast_kernel<BMODE>), dim3((unsigned)(grid < cus ? grid : cus)), dim3(kFNT), kFLdsBytes, s, p);
+  if (int rc = hip_check(hipGetLastError(), "grouped product launch")) return rc;
+  if (p.tail < 0) return kOk;
+  const void* tail = reinterpret_cast<const void*>(&grouped_tail_kernel<Ring64x128, BMODE>);
+  if (int rc = ensure_lds(tail, Ring64x128::kLds)) return rc;
+  const int64_t most = grid < p.tail ? grid : p.tail;
+  hipLaunchKernelGGL((grouped_tail_kernel<Ring64x128, BMODE>), dim3((unsigned)(most * kTailPieces)), dim3(Ring64x128::NT),
+                     Ring64x128::kLds, s, p);
+  return hip_check(hipGetLastError(), "grouped product launch");
+}
+template <int BMODE>
 int run_tile(const GroupedParams& p, int tile, int64_t grid, hipStream_t s) {
   switch (tile) {
-    case kTile256: {
-      const void* kern = reinterpret_cast<const void*>(&grouped_fast_kernel<BMODE>);
-      if (int rc = ensure_lds(kern, kFLdsBytes)) return rc;
-      const int cus = device_cus();
-      hipLaunchKernelGGL((grouped_fast_kernel<BMODE>), dim3((unsigned)(grid < cus ? grid : cus)), dim3(kFNT), kFLdsBytes, s, p);
-      return hip_check(hipGetLastError(), "grouped product launch");
-    }
+    case kTile256: return launch_whole<BMODE>(p, grid, s);
     case kTile128x2: return launch_ring<Ring128x2, BMODE>(p, grid, s);
     case kTile128x1: return launch_ring<Ring128x1, BMODE>(p, grid, s);
     case kTile64x128: return launch_ring<Ring64x128, BMODE>(p, grid, s);
     case kTile64: return launch_ring<Ring64, BMODE>(p, grid, s);
   }
   if constexpr (BMODE == kKContig) {
-    const dim3 g((unsigned)grid), block(256);
-    if (tile == kTileFew1) hipLaunchKernelGGL((grouped_few_kernel<1>), g, block, 0, s, p);
-    else if (tile == kTileFew2) hipLaunchKernelGGL((grouped_few_kernel<2>), g, block, 0, s, p);
-    else hipLaunchKernelGGL((grouped_few_kernel<4>), g, block, 0, s, p);
+    hipLaunchKernelGGL(grouped_few_kernel, dim3((unsigned)grid), dim3(256), 0, s, p);
     return hip_check(hipGetLastError(), "grouped product launch");
   }
   return set_error(kInvalid, "no grouped tile %d", tile);
