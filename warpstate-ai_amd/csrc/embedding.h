@@ -131,6 +131,7 @@ struct EmbedGradParams {
   const int* start;
   const int* perm;
   int vocab, d;
+  int group;  // rows of the table that a wave takes, fewer than 64
   float scale;
   void* out; long ld_out;
   // Tokens with more than `piece` positions are summed in pieces of perm that begin at multiples
@@ -182,18 +183,23 @@ __device__ __forceinline__ EmbedPiece<F32, W> embed_load(const void* base, long 
   }
   return v;
 }
-template <bool F32, int W, bool VEC>
+template <bool F32, int W, bool VEC, bool NT = false>
 __device__ __forceinline__ void embed_write(const float (&f)[W], void* base, long at, int left) {
   char* dst = static_cast<char*>(base) + at * (F32 ? 4 : 2);
   if (VEC && left >= W) {
     if constexpr (F32) {
 #pragma unroll
-      for (int q = 0; q < W / 4; ++q)
-        reinterpret_cast<f32x4_t*>(dst)[q] = f32x4_t{f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]};
+      for (int q = 0; q < W / 4; ++q) {
+        const f32x4_t v = {f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]};
+        if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<f32x4_t*>(dst) + q);
+        else reinterpret_cast<f32x4_t*>(dst)[q] = v;
+      }
     } else {
       static_assert(F32 || W == 8, "BF16 pieces are 16 bytes");
-      *reinterpret_cast<u32x4_t*>(dst) = u32x4_t{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                                 pack_bf16x2(f[W - 4], f[W - 3]), pack_bf16x2(f[W - 2], f[W - 1])};
+      const u32x4_t v = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[W - 4], f[W - 3]),
+                         pack_bf16x2(f[W - 2], f[W - 1])};
+      if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(dst));
+      else *reinterpret_cast<u32x4_t*>(dst) = v;
     }
     return;
   }
@@ -246,7 +252,7 @@ __device__ __forceinline__ void embed_clear(float (&acc)[NC][W]) {
     for (int e = 0; e < W; ++e) acc[i][e] = 0.0f;
 }
 
-template <int OUT, int W, bool VEC>
+template <int OUT, int W, bool VEC, bool NT>
 __device__ __forceinline__ void embed_store(const EmbedGradParams& p, long v, int c, float (&acc)[W]) {
   const long at = v * p.ld_out + c;
 #pragma unroll
@@ -256,15 +262,14 @@ __device__ __forceinline__ void embed_store(const EmbedGradParams& p, long v, in
 #pragma unroll
     for (int e = 0; e < W; ++e) acc[e] += old.at(e);
   }
-  embed_write<OUT != kEmbedBF16, W, VEC>(acc, p.out, at, p.d - c);
+  embed_write<OUT != kEmbedBF16, W, VEC, NT>(acc, p.out, at, p.d - c);
 }
 
-// A wave per piece of the sorted positions, then a wave per kEmbedRows rows of the table, whose
+// A wave per piece of the sorted positions, then a wave per `group` rows of the table, whose
 // positions lie one after the other: the rows of dy of all of them are requested as one run, so
-// that a row with one token or none, the usual one, does not wait for its own chain of loads.
-constexpr int kEmbedRows = 4;
-
-template <bool GF32, int OUT, bool VEC>
+// that a row with one token or none, the usual one, does not wait for its own chain of loads. NT:
+// the output goes around the caches.
+template <bool GF32, int OUT, bool VEC, bool NT>
 static __global__ void __launch_bounds__(256) embed_grad_kernel(const EmbedGradParams p) {
   constexpr int W = OUT == kEmbedBF16 ? 8 : 4, NC = 32 / W, kSpan = 64 * W;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -293,9 +298,9 @@ static __global__ void __launch_bounds__(256) embed_grad_kernel(const EmbedGradP
     }
     return;
   }
-  const long v0 = (task - p.pieces) * kEmbedRows;
+  const long v0 = (task - p.pieces) * p.group;
   if (v0 >= p.vocab) return;
-  const int rows = (int)min((long)kEmbedRows, p.vocab - v0);
+  const int rows = (int)min((long)p.group, p.vocab - v0);
   // Lane r: where row r's positions begin (lane `rows`: where the last one's end).
   const int begins = p.start[v0 + min(lane, rows)];
   for (int c0 = 0; c0 < p.d; c0 += kSpan * NC) {
@@ -307,7 +312,7 @@ static __global__ void __launch_bounds__(256) embed_grad_kernel(const EmbedGradP
       if (n <= p.piece && (OUT != kEmbedAdd || n > 0)) {
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-          if (c + kSpan * i < p.d) embed_store<OUT, W, VEC>(p, v0 + r, c + kSpan * i, acc[i]);
+          if (c + kSpan * i < p.d) embed_store<OUT, W, VEC, NT>(p, v0 + r, c + kSpan * i, acc[i]);
       }
       embed_clear(acc);
       ++r;
@@ -362,7 +367,7 @@ static __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedGradP
   if (wave > 0 || c >= p.d) return;
 #pragma unroll
   for (int k = 0; k < W; ++k) acc[k] = (sums[0][k][lane] + sums[1][k][lane]) + (sums[2][k][lane] + sums[3][k][lane]);
-  embed_store<OUT, W, VEC>(p, v, c, acc);
+  embed_store<OUT, W, VEC, false>(p, v, c, acc);
 }
 
 }  // namespace ws

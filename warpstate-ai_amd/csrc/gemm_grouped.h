@@ -27,8 +27,7 @@ struct GroupedParams {
   const long* offsets;          // [groups + 1]
   int groups, rows, N, K, tiles_n;
   int most;                     // tiles that the grid is sized for
-  // 256 x 256 tiles: a last round of at most `tail` tiles is left to the tail kernel (-1: none is).
-  int round, tail;
+  int pieces_most;              // a last round of at most so many 256 x 256 tiles goes in pieces
   unsigned short* c; long ldc;
 };
 
@@ -100,13 +99,37 @@ __device__ __forceinline__ GemmParams store_params(unsigned short* c, long ldc, 
   return e;
 }
 
-// Of `total` 256 x 256 tiles, those that are done whole.
-__device__ __forceinline__ int whole_tiles(const GroupedParams& p, int total) {
-  const int rest = total % p.round;
-  return rest <= p.tail ? total - rest : total;
+// A piece of the last round's tiles: BM x BN of tile whole + x / pieces, the (x % pieces)-th by rows. Its
+// sums have the 256 x 256 tile's order, so the bits do not tell which of the two made them.
+template <class Cfg, int BMODE>
+__device__ __forceinline__ void grouped_piece(const GroupedParams& p, int whole, int x, unsigned char* smem, int lane,
+                                              int wave) {
+  constexpr int kAcross = kFBN / Cfg::BN, kPieces = kFBM / Cfg::BM * kAcross;
+  const GroupTile t = find_tile<kFBM>(p, whole + x / kPieces, lane, group_lanes<kFBM>(p, 0, lane));
+  int tm, tn;
+  tile_position(t.index, cdiv(t.hi - t.lo, kFBM), p.tiles_n, tm, tn);
+  const int piece = x % kPieces;
+  const int row0 = t.lo + tm * kFBM + piece / kAcross * Cfg::BM, col0 = tn * kFBN + piece % kAcross * Cfg::BN;
+  if (row0 >= t.hi || col0 >= p.N) return;
+  const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+  OperandDesc b = p.b;
+  b.ptr += max(t.group, 0) * p.b_group;
+  Acc16<Cfg::FA, Cfg::FB> acc;
+  ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.N, 0, p.K, 0,
+                                           t.group < 0 ? 0 : cdiv(p.K, kFBK), smem, wave, lane);
+  const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
+  FEpiStore<false, false>::run(e, acc, row0 + wm * Cfg::TM, col0 + wn * Cfg::TN, lane, tm, tn, wn,
+                               smem + wave * epi_wave<Cfg::FA, Cfg::FB>());
+  __builtin_amdgcn_s_barrier();  // the next piece's loads go where the staging was
 }
 
-// 256 x 256 tiles, a workgroup per compute unit looping over them.
+// 256 x 256 tiles, a workgroup per compute unit looping over them. A last round that would leave most
+// units idle goes in pieces of 64 x 128 or 128 x 128 instead, so that all of them take part: with R of
+// 256 units in it, for each 64 of the reduction 1.0 us (R 32) to 1.4 (R 256) whole, and in pieces
+// @P64@ up to R 32 and @P128@ up to R 64, twice that up to R 128.
+typedef RingCfg<64, 128, 2, 4, 4> Piece64;
+typedef RingCfg<128, 128, 4, 2, 4> Piece128;
+
 template <int BMODE>
 __global__ void __launch_bounds__(kFNT) grouped_fast_kernel(const GroupedParams p) {
   constexpr int TM = kFBM / kFWM, TN = kFBN / kFWN;
@@ -118,12 +141,13 @@ __global__ void __launch_bounds__(kFNT) grouped_fast_kernel(const GroupedParams 
   const unsigned abase = lds0 + frag_base<kKContig>(wm * TM, lane);
   const unsigned bbase = lds0 + 2 * kFTileBytes + frag_base<BMODE>(wn * TN, lane);
   GroupLanes v;
-  const int total = whole_tiles(p, count_tiles<kFBM>(p, lane, v));
-  for (int w = blockIdx.x; w < total; w += gridDim.x) {
+  const int total = count_tiles<kFBM>(p, lane, v), rest = total % (int)gridDim.x;
+  const int whole = rest <= p.pieces_most ? total - rest : total;
+  for (int w = blockIdx.x; w < whole; w += gridDim.x) {
     // The groups are read again for each tile: kept over the k-loop they would cost it registers.
     int l = lane;
     opaque_lane(l);
-    const GroupTile t = find_tile<kFBM>(p, xcd_remap(w, total, gridDim.x), l, group_lanes<kFBM>(p, 0, l));
+    const GroupTile t = find_tile<kFBM>(p, xcd_remap(w, whole, gridDim.x), l, group_lanes<kFBM>(p, 0, l));
     int tm, tn;
     tile_position(t.index, cdiv(t.hi - t.lo, kFBM), p.tiles_n, tm, tn);
     const int row0 = t.lo + tm * kFBM, col0 = tn * kFBN;
@@ -140,6 +164,16 @@ __global__ void __launch_bounds__(kFNT) grouped_fast_kernel(const GroupedParams 
     const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
     FEpiStore<false, false>::run(e, acc, row0 + wm * TM, col0 + wn * TN, lane, tm, tn, wn, fsmem + wave * kFStageWave);
     __builtin_amdgcn_s_barrier();
+  }
+  if (whole == total) return;
+  int l = lane;
+  opaque_lane(l);
+  if (rest * 8 <= (int)gridDim.x) {
+    for (int x = blockIdx.x; x < rest * 8; x += gridDim.x)
+      grouped_piece<Piece64, BMODE>(p, whole, xcd_remap(x, rest * 8, gridDim.x), fsmem, l, wave);
+  } else {
+    for (int x = blockIdx.x; x < rest * 4; x += gridDim.x)
+      grouped_piece<Piece128, BMODE>(p, whole, xcd_remap(x, rest * 4, gridDim.x), fsmem, l, wave);
   }
 }
 
@@ -168,39 +202,6 @@ __global__ void __launch_bounds__(Cfg::NT) grouped_ring_kernel(const GroupedPara
                                rsmem + wave * epi_wave<FA, FB>());
 }
 
-// The last round's tiles in pieces of 64 x 128, one workgroup each, where they would leave most compute
-// units idle: as many of a tile's products again, but all units take part. The sums have the
-// 256 x 256 tile's order, so the bits do not tell which kernel made them.
-constexpr int kTailRows = 64, kTailCols = 128, kTailPieces = (kFBM / kTailRows) * (kFBN / kTailCols);
-
-template <class Cfg, int BMODE>
-__global__ void __launch_bounds__(Cfg::NT) grouped_tail_kernel(const GroupedParams p) {
-  constexpr int FA = Cfg::FA, FB = Cfg::FB, TM = Cfg::TM, TN = Cfg::TN;
-  static_assert(Cfg::BM == kTailRows && Cfg::BN == kTailCols, "pieces of a tile");
-  extern __shared__ __attribute__((aligned(1024))) unsigned char rsmem[];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
-  GroupLanes v;
-  const int total = count_tiles<kFBM>(p, lane, v), whole = whole_tiles(p, total);
-  const int pieces = (total - whole) * kTailPieces;
-  if ((int)blockIdx.x >= pieces) return;
-  const int x = xcd_remap(blockIdx.x, pieces, kRingWindow), piece = x % kTailPieces;
-  const GroupTile t = find_tile<kFBM>(p, whole + x / kTailPieces, lane, v);
-  int tm, tn;
-  tile_position(t.index, cdiv(t.hi - t.lo, kFBM), p.tiles_n, tm, tn);
-  const int row0 = t.lo + tm * kFBM + piece / 2 * kTailRows, col0 = tn * kFBN + piece % 2 * kTailCols;
-  if (row0 >= t.hi || col0 >= p.N) return;
-  OperandDesc b = p.b;
-  b.ptr += max(t.group, 0) * p.b_group;
-  Acc16<FA, FB> acc;
-  ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.N, 0, p.K, 0,
-                                           t.group < 0 ? 0 : cdiv(p.K, kFBK), rsmem, wave, lane);
-  const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
-  FEpiStore<false, false>::run(e, acc, row0 + wm * TM, col0 + wn * TN, lane, tm, tn, wn,
-                               rsmem + wave * epi_wave<FA, FB>());
-}
-
 // --------------------------------------------------------------------------------------
 // Weight gradients: [M, N] per group, reduced over the group's rows.
 
@@ -218,9 +219,11 @@ struct GradTile {
 };
 // Groups in the order in which their tiles are dealt out, lane r the group with the r-th most rows:
 // the tiles of one group take as long as it has rows, and long ones that come last leave the others
-// waiting. More than 64 groups keep their own order.
+// waiting. (16384 rows in eight groups, gradients of 2048 x 2048 in BF16: 168 -> 134 us.) More than
+// kOrdered groups keep their own order: finding another takes a small tile's workgroup too long.
+constexpr int kOrdered = 16;
 __device__ __forceinline__ int grad_order(const GroupedGradParams& p, int lane) {
-  if (p.groups > 64) return lane;
+  if (p.groups > kOrdered) return lane;
   int lo = 0, hi = 0;
   if (lane < p.groups) group_rows(p.offsets, p.groups, p.rows, lane + 1, lo, hi);
   const int rows = max(0, hi - lo);
@@ -234,7 +237,7 @@ __device__ __forceinline__ int grad_order(const GroupedGradParams& p, int lane) 
 __device__ __forceinline__ GradTile grad_tile(const GroupedGradParams& p, int w, int order) {
   const int per = p.tiles_m * p.tiles_n, place = w / per;
   GradTile t;
-  t.group = p.groups > 64 ? place : __builtin_amdgcn_readlane(order, place);
+  t.group = p.groups > kOrdered ? place : __builtin_amdgcn_readlane(order, place);
   tile_position(w - place * per, p.tiles_m, p.tiles_n, t.tm, t.tn);
   int lo, hi;
   group_rows(p.offsets, p.groups, p.rows, t.group + 1, lo, hi);
@@ -243,12 +246,43 @@ __device__ __forceinline__ GradTile grad_tile(const GroupedGradParams& p, int w,
   t.b = OperandDesc{p.b + lo * p.ldb, 1, p.ldb};
   return t;
 }
+// The wave's accumulators as FP32 rows of out [M, N], through its LDS staging rows in two halves, so
+// that the stores cover whole lines. (Stored from the fragments, 64 bytes of each of 16 rows at a
+// time, the largest gradients took @F0@ us instead of @F1@.)
+template <int FA, int FB>
+__device__ __forceinline__ void store_f32(float* out, int M, int N, Acc16<FA, FB>& acc, int m_base, int n_base, int lane,
+                                          unsigned char* stage) {
+  constexpr int kRow = FB * 64 + 16, LPR = FB * 4, RPI = 64 / LPR, HA = FA / 2, NQ = HA * 16 / RPI;
+  static_assert(FA % 2 == 0 && 64 % LPR == 0 && NQ >= 1 && HA * 16 * kRow <= epi_wave<FA, FB>(), "half a tile is staged");
+  opaque_lane(lane);
+  __amdgpu_buffer_rsrc_t rg = make_rsrc(out + (long)m_base * N + n_base, 0x7fffffff);
+  const int c4 = 4 * (lane % LPR);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int i = 0; i < HA; ++i)
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+        *reinterpret_cast<f32x4_v*>(stage + (16 * i + (lane & 15)) * kRow + (16 * j + 4 * (lane >> 4)) * 4) =
+            acc.v[h * HA + i][j];
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's staging writes landed
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int r = RPI * q + lane / LPR, m = 16 * HA * h + r;
+      const bool ok = m_base + m < M && n_base + c4 + 3 < N;  // N is a multiple of 8
+      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + r * kRow + c4 * 4);
+      __builtin_amdgcn_raw_buffer_store_b128(v, rg, store_off(ok, (long)m * N + c4, 4), 0, kEpiNT);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
 template <bool F32, int FA, int FB>
 __device__ __forceinline__ void grad_store(const GroupedGradParams& p, const GradTile& t, Acc16<FA, FB>& acc, int m_base,
                                            int n_base, int lane, int wn, unsigned char* stage) {
   const long at = (long)t.group * p.M * p.N;
   if constexpr (F32) {
-    FEpiAccF32<false>::add(static_cast<float*>(p.g) + at, p.N, p.M, p.N, kAccStore, acc, m_base, n_base, lane, t.tm, t.tn);
+    store_f32(static_cast<float*>(p.g) + at, p.M, p.N, acc, m_base, n_base, lane, stage);
   } else {
     const GemmParams e = store_params(static_cast<unsigned short*>(p.g) + at, p.N, p.M, p.N);
     FEpiStore<false, false>::run(e, acc, m_base, n_base, lane, t.tm, t.tn, wn, stage);

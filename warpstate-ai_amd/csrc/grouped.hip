@@ -10,10 +10,8 @@ namespace {
 constexpr int64_t kMaxGroups = 65536;
 // Beside FastTile: the kernel for few rows.
 constexpr int kTileFew = kFastTiles;
-// The last round of 256 x 256 tiles goes in pieces where it has at most this many tiles for 256 compute
-// units, and the reduction at least kTailK: us of the round whole / in pieces, by its cost: 32 tiles 1.0 /
-// 0.34 a k-tile, 64 1.0 / 0.5, 96 1.1 / 0.84, 128 1.1 / 1.0; the kernel itself takes 4 us.
-constexpr int kTailOf256 = 112, kTailK = 1536;
+// The most 256 x 256 tiles for 256 compute units whose round goes in pieces (grouped_fast_kernel).
+constexpr int kPiecesOf256 = 112;
 
 int tile_rows(int tile) {
   switch (tile) {
@@ -49,12 +47,12 @@ int pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int bmode) 
     int64_t wide = rows + used * bm / 2;
     if (wide < used * bm) wide = used * bm;
     float ti = tile_time(tile, wide, n, k, kKContig, bmode, device_cus(), false, kEpiStore);
-    if (tile == kTile256 && k >= kTailK) {
+    if (tile == kTile256) {
       const TileCost& c = tile_cost(tile, kKContig, bmode);
-      const int64_t tiles = cdiv(wide, 256) * (int64_t)cdiv(n, 256), rest = tiles % device_cus();
-      if (rest * 256 <= (int64_t)kTailOf256 * device_cus())
-        ti = (float)(tiles / device_cus()) * (c.alone * (float)cdiv(k, kFBK) + c.fixed) + 4.0f +
-             tile_time(kTile64x128, rest * 256, 256, k, kKContig, bmode, device_cus(), false, kEpiStore);
+      const int64_t tiles = cdiv(wide, 256) * (int64_t)cdiv(n, 256), cus = device_cus(), rest = tiles % cus;
+      const float kt = (float)cdiv(k, kFBK);
+      if (rest * 256 <= kPiecesOf256 * cus)
+        ti = (float)(tiles / cus) * (c.alone * kt + c.fixed) + (rest * 8 <= cus ? 0.35f : rest * 4 <= cus ? 0.5f : 1.0f) * kt + 4.0f;
     }
     if (tile == 0 || ti < t) {
       best = tile;
@@ -68,9 +66,12 @@ int pick_grad(int64_t rows, int64_t groups, int64_t m, int64_t n) {
   float t = 0.0f;
   for (int tile = 0; tile < kFastTiles; ++tile) {
     const int64_t bm = tile_rows(tile);
+    // With a k-tile or less for each group the smaller tile's stores start sooner (64 groups of 512 x
+    // 1280 over 4096 rows, BF16, 26 / 24 us; 8 of 5632 x 2048 over 32, FP32, 82 / 76).
+    if (tile == kTile256 && rows <= kFBK * groups) continue;
     const float ti = tile_time(tile, groups * (cdiv(m, bm) * bm), n, cdiv(rows, groups), kMNContig, kMNContig, device_cus(),
                                false, kEpiF32);
-    if (tile == 0 || ti < t) {
+    if (t == 0.0f || ti < t) {
       best = tile;
       t = ti;
     }
@@ -102,18 +103,13 @@ int launch_ring(const GroupedParams& p, int64_t grid, hipStream_t s) {
 template <int BMODE>
 int launch_whole(GroupedParams p, int64_t grid, hipStream_t s) {
   const void* kern = reinterpret_cast<const void*>(&grouped_fast_kernel<BMODE>);
+  static_assert(Piece64::kLds <= kFLdsBytes && Piece128::kLds <= kFLdsBytes && Piece64::NT == kFNT && Piece128::NT == kFNT,
+                "pieces run in the workgroup of a 256 x 256 tile");
   if (int rc = ensure_lds(kern, kFLdsBytes)) return rc;
+  // (All units, also for fewer tiles: these may go in pieces.)
   const int cus = device_cus();
-  p.round = cus;
-  p.tail = p.K >= kTailK ? kTailOf256 * cus / 256 : -1;
-  hipLaunchKernelGGL((grouped_fast_kernel<BMODE>), dim3((unsigned)(grid < cus ? grid : cus)), dim3(kFNT), kFLdsBytes, s, p);
-  if (int rc = hip_check(hipGetLastError(), "grouped product launch")) return rc;
-  if (p.tail < 0) return kOk;
-  const void* tail = reinterpret_cast<const void*>(&grouped_tail_kernel<Ring64x128, BMODE>);
-  if (int rc = ensure_lds(tail, Ring64x128::kLds)) return rc;
-  const int64_t most = grid < p.tail ? grid : p.tail;
-  hipLaunchKernelGGL((grouped_tail_kernel<Ring64x128, BMODE>), dim3((unsigned)(most * kTailPieces)), dim3(Ring64x128::NT),
-                     Ring64x128::kLds, s, p);
+  p.pieces_most = kPiecesOf256 * cus / 256;
+  hipLaunchKernelGGL((grouped_fast_kernel<BMODE>), dim3((unsigned)(grid * 8 < cus ? grid * 8 : cus)), dim3(kFNT), kFLdsBytes, s, p);
   return hip_check(hipGetLastError(), "grouped product launch");
 }
 template <int BMODE>
