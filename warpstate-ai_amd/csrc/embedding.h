@@ -143,7 +143,7 @@ struct EmbedGradParams {
 enum EmbedOut { kEmbedBF16 = 0, kEmbedF32 = 1, kEmbedAdd = 2 };
 
 // W elements of a row, 8 or 4: an FP32 output's pieces are four columns wide, so that a wave's stores
-// cover whole lines (16384 x 2048 into 32768 rows, us, pieces of 8 / 4: @E8@ / @E4@).
+// cover whole lines (16384 x 2048 into 32768 rows, the kernel alone, us, pieces of 8 / 4: 83 / 75).
 template <bool F32, int W>
 struct EmbedPiece {
   unsigned w[F32 ? W : W / 2];

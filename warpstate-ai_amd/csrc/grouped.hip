@@ -11,7 +11,7 @@ constexpr int64_t kMaxGroups = 65536;
 // Beside FastTile: the kernel for few rows.
 constexpr int kTileFew = kFastTiles;
 // The most 256 x 256 tiles for 256 compute units whose round goes in pieces (grouped_fast_kernel).
-constexpr int kPiecesOf256 = 112;
+constexpr int kPiecesOf256 = 64;
 
 int tile_rows(int tile) {
   switch (tile) {
@@ -52,7 +52,7 @@ int pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int bmode) 
       const int64_t tiles = cdiv(wide, 256) * (int64_t)cdiv(n, 256), cus = device_cus(), rest = tiles % cus;
       const float kt = (float)cdiv(k, kFBK);
       if (rest * 256 <= kPiecesOf256 * cus)
-        ti = (float)(tiles / cus) * (c.alone * kt + c.fixed) + (rest * 8 <= cus ? 0.35f : rest * 4 <= cus ? 0.5f : 1.0f) * kt + 4.0f;
+        ti = (float)(tiles / cus) * (c.alone * kt + c.fixed) + (rest * 8 <= cus ? 0.45f : 0.62f) * kt + 4.0f;
     }
     if (tile == 0 || ti < t) {
       best = tile;

@@ -5,8 +5,6 @@
 //
 // Autograd kernels read no data; they call operators below autograd. First derivatives by reverse
 // mode only: tensors that carry a tangent are refused, and so is a second differentiation.
-#include <torch/csrc/autograd/functions/basic_ops.h>
-
 #include <cmath>
 
 #include "host_common.h"
@@ -25,17 +23,28 @@ Tensor rows_of(const Tensor& t) {
 }
 int64_t last(const Tensor& t) { return t.dim() ? t.size(-1) : 0; }
 
-// Gradients that are not differentiable again: where a graph of the backward is recorded, they
-// refuse it.
+// Gradients that are not differentiable again: where a graph of the backward is recorded, they stand
+// behind a node that depends on everything they were made `from`, and refuses.
+struct OnceFn : Function<OnceFn> {
+  static variable_list forward(AutogradContext* ctx, at::TensorList grads, at::TensorList from, std::string message) {
+    ctx->saved_data["message"] = message;
+    variable_list out;
+    for (const auto& g : grads) out.push_back(g.alias());
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list) {
+    TORCH_CHECK(false, ctx->saved_data["message"].toStringRef());
+  }
+};
 variable_list once(variable_list grads, const variable_list& from, const char* message) {
-  bool recorded = false;
-  for (const auto& t : from) recorded |= t.defined() && t.requires_grad();
-  if (!at::GradMode::is_enabled() || !recorded) return grads;
-  variable_list known;
-  for (auto& g : grads)
-    if (g.defined()) known.push_back(g.detach().set_requires_grad(true));
-  auto node = std::make_shared<torch::autograd::DelayedError>(message, (int64_t)known.size());
-  known = (*node)(std::move(known));
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list known, sources;
+  for (const auto& t : from)
+    if (t.defined() && t.requires_grad()) sources.push_back(t);
+  if (sources.empty()) return grads;
+  for (const auto& g : grads)
+    if (g.defined()) known.push_back(g);
+  known = OnceFn::apply(at::TensorList(known), at::TensorList(sources), std::string(message));
   size_t next = 0;
   for (auto& g : grads)
     if (g.defined()) g = known[next++];
@@ -351,7 +360,8 @@ struct GroupedMmFn : Function<GroupedMmFn> {
     static const auto op = find<GroupedRows>("warpstate::native_grouped_rows");
     at::AutoDispatchBelowAutograd guard;
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({weight.requires_grad() ? a : Tensor(), x.requires_grad() ? w : Tensor(), offsets});
+    // (x and weight themselves only to depend on.)
+    ctx->save_for_backward({weight.requires_grad() ? a : Tensor(), x.requires_grad() ? w : Tensor(), offsets, x, weight});
     ctx->saved_data["want_x"] = x.requires_grad();
     ctx->saved_data["want_w"] = weight.requires_grad();
     ctx->saved_data["n"] = weight.size(1);
@@ -376,7 +386,7 @@ struct GroupedMmFn : Function<GroupedMmFn> {
         d[1] = dw;
       }
     }
-    return once(d, {s[0], s[1], grads[0]}, kGroupedTwice);
+    return once(d, {s[3], s[4], grads[0]}, kGroupedTwice);
   }
 };
 Tensor grouped_mm_autograd(const Tensor& x, const Tensor& weight, const Tensor& offsets) {

@@ -25,7 +25,7 @@ import math
 import torch
 
 from ops import _hip
-from ops.residual_norm import _refuse_tangents, _row_stride, _rows
+from ops.residual_norm import _once, _refuse_tangents, _row_stride, _rows
 
 BF16, F32 = torch.bfloat16, torch.float32
 Tensor = torch.Tensor
@@ -68,14 +68,14 @@ class _Embedding(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         if dy is None:
             return None, None, None, None
         vocab, d, scale, dtype = ctx.args
         out = torch.empty((vocab, d), dtype=dtype, device=dy.device)
-        _sums(dy, ctx.saved_tensors[0], scale, out, _WRITE_F32 if dtype == F32 else _WRITE_BF16)
-        return None, out, None, None
+        _sums(dy.detach(), ctx.saved_tensors[0], scale, out,
+              _WRITE_F32 if dtype == F32 else _WRITE_BF16)
+        return _once("the embedding", (None, out, None, None), dy)
 
 
 def embedding(tokens: Tensor, table: Tensor, scale: float = 1.0,

@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from ops import _hip
-from ops.residual_norm import _refuse_tangents, _row_stride
+from ops.residual_norm import _once, _refuse_tangents, _row_stride
 
 BF16, F32 = torch.bfloat16, torch.float32
 Tensor = torch.Tensor
@@ -88,30 +88,30 @@ class _GroupedMm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, a, w, offsets):
-        ctx.save_for_backward(a, w, offsets)
+        ctx.save_for_backward(a, w, offsets, x, weight)  # the last two only to depend on
         ctx.args = (weight.shape[1], x.shape[1], weight.dtype)
         ctx.set_materialize_grads(False)
         return _first(_product(a, w, offsets, _NT), weight.shape[1])
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         if dy is None:
             return None, None, None, None, None
-        a, w, offsets = ctx.saved_tensors
+        a, w, offsets, x, weight = ctx.saved_tensors
         n, k, dtype = ctx.args
-        g = _operand(dy)
         dx = dw = None
-        if ctx.needs_input_grad[0]:
-            dx = _first(_product(g, w, offsets, _NN), k)
-        if ctx.needs_input_grad[1]:
-            groups = w.shape[0]
-            dw = torch.empty((groups, g.shape[1], a.shape[1]), dtype=dtype, device=a.device)
-            _hip.call_on(a, "ws_grouped_weight_grad", g.data_ptr(), _row_stride(g), a.data_ptr(),
-                         _row_stride(a), offsets.data_ptr(), groups, a.shape[0], g.shape[1],
-                         a.shape[1], dw.data_ptr(), int(dtype == F32))
-            dw = _first(dw, n, k)
-        return dx, dw, None, None, None
+        with torch.no_grad():
+            g = _operand(dy)
+            if ctx.needs_input_grad[0]:
+                dx = _first(_product(g, w, offsets, _NN), k)
+            if ctx.needs_input_grad[1]:
+                groups = w.shape[0]
+                dw = torch.empty((groups, g.shape[1], a.shape[1]), dtype=dtype, device=a.device)
+                _hip.call_on(a, "ws_grouped_weight_grad", g.data_ptr(), _row_stride(g),
+                             a.data_ptr(), _row_stride(a), offsets.data_ptr(), groups, a.shape[0],
+                             g.shape[1], a.shape[1], dw.data_ptr(), int(dtype == F32))
+                dw = _first(dw, n, k)
+        return _once("a grouped product", (dx, dw, None, None, None), x, weight, dy)
 
 
 def grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:

@@ -62,6 +62,32 @@ def _refuse_tangents(name: str, *tensors: Tensor | None) -> None:
         raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
+class _Once(torch.autograd.Function):
+    """The first ``count`` tensors, behind a node that depends on all of them and refuses to be
+    differentiated."""
+
+    @staticmethod
+    def forward(ctx, message, count, *tensors):
+        ctx.message = message
+        return tuple(t.view_as(t) for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *_grads):
+        raise RuntimeError(ctx.message)
+
+
+def _once(name: str, grads: tuple, *sources: Tensor | None) -> tuple:
+    """``grads`` (tensors and None) of a backward; where a graph of it is recorded, they depend on
+    ``sources`` and refuse a second derivative."""
+    sources = [t for t in sources if t is not None and t.requires_grad]
+    if not torch.is_grad_enabled() or not sources:
+        return grads
+    known = [g for g in grads if g is not None]
+    wrapped = iter(_Once.apply(f"{name} cannot be differentiated twice", len(known), *known,
+                               *sources))
+    return tuple(None if g is None else next(wrapped) for g in grads)
+
+
 class _AddRmsnorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
@@ -78,27 +104,33 @@ class _AddRmsnorm(torch.autograd.Function):
         return y, stream
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dstream):
         if dy is None:  # the addition alone
             return None if dstream is None else dstream.to(BF16), dstream, None, None
         stream, weight, rstd = ctx.saved_tensors
-        f32 = stream.dtype == F32
-        dx = torch.empty(stream.shape, dtype=BF16, device=stream.device)
-        dresidual = torch.empty(stream.shape, dtype=F32, device=stream.device) if f32 else None
-        dweight = torch.empty(weight.shape, dtype=F32, device=stream.device)
-        if stream.numel() == 0:
-            return dx, dresidual if f32 else dx, dweight.zero_(), None
-        s, g, w = _rows(stream), _rows(dy), weight.contiguous()
-        h = None if dstream is None else _rows(dstream)
-        rows, d = s.shape
-        need = _hip.query_on(s, "ws_add_rmsnorm_backward_partial_floats", rows, d)
-        partial = torch.empty((need,), dtype=F32, device=s.device)
-        _hip.call_on(s, "ws_add_rmsnorm_backward", s.data_ptr(), int(f32), w.data_ptr(),
-                     rstd.data_ptr(), g.data_ptr(), _row_stride(g), _hip.ptr(h),
-                     0 if h is None else _row_stride(h), rows, d, dx.data_ptr(),
-                     _hip.ptr(dresidual), dweight.data_ptr(), partial.data_ptr())
-        return dx, dresidual if f32 else dx, dweight, None
+        with torch.no_grad():
+            grads = _backward(stream, weight, rstd, dy, dstream)
+        return _once("the residual norm", (*grads, None), stream, weight, dy, dstream)
+
+
+def _backward(stream, weight, rstd, dy, dstream):
+    """(dx, dresidual, dweight)."""
+    f32 = stream.dtype == F32
+    dx = torch.empty(stream.shape, dtype=BF16, device=stream.device)
+    dresidual = torch.empty(stream.shape, dtype=F32, device=stream.device) if f32 else None
+    dweight = torch.empty(weight.shape, dtype=F32, device=stream.device)
+    if stream.numel() == 0:
+        return dx, dresidual if f32 else dx, dweight.zero_()
+    s, g, w = _rows(stream), _rows(dy), weight.contiguous()
+    h = None if dstream is None else _rows(dstream)
+    rows, d = s.shape
+    need = _hip.query_on(s, "ws_add_rmsnorm_backward_partial_floats", rows, d)
+    partial = torch.empty((need,), dtype=F32, device=s.device)
+    _hip.call_on(s, "ws_add_rmsnorm_backward", s.data_ptr(), int(f32), w.data_ptr(),
+                 rstd.data_ptr(), g.data_ptr(), _row_stride(g), _hip.ptr(h),
+                 0 if h is None else _row_stride(h), rows, d, dx.data_ptr(), _hip.ptr(dresidual),
+                 dweight.data_ptr(), partial.data_ptr())
+    return dx, dresidual if f32 else dx, dweight
 
 
 def _weight(weight: Tensor) -> Tensor:
@@ -136,7 +168,7 @@ def rmsnorm_quantize(x: Tensor, weight: Tensor, eps: float = 1e-5, residual: Ten
         raise ValueError("Residual norms require CUDA tensors")
     if scale_dtype not in _SCALE_TYPES:
         raise ValueError("Scales are torch.float8_e8m0fnu or torch.float32")
-    weight, e8m0 = _weight(weight.detach()), scale_dtype == E8M0
+    weight, e8m0 = _weight(weight), scale_dtype == E8M0
     native = _hip.host_ops()
     if native is not None:
         q, scale, stream = native.native_rmsnorm_quantize(x, residual, weight, eps, e8m0)
@@ -146,7 +178,7 @@ def rmsnorm_quantize(x: Tensor, weight: Tensor, eps: float = 1e-5, residual: Ten
     if x.numel() == 0:
         raise ValueError("Quantization takes non-empty rows")
     x = x.detach()
-    a, w = _rows(x), weight.contiguous()
+    a, w = _rows(x), weight.detach().contiguous()
     rows, d = a.shape
     r = stream = None
     if residual is not None:
