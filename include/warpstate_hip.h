@@ -479,7 +479,7 @@ int ws_linear_token_scores_backward(const void* hidden, int64_t ld_hidden, const
  *
  * s = r(x + residual) in the residual stream's type (BF16, or FP32 with stream_f32), then the
  * RMSNorm of the rounded s: y = s rstd w, rstd = 1 / sqrt(mean(s^2) + eps), rounded once. x is BF16,
- * the weight FP32; rows of 1 to 8192 columns, row strides in elements, outputs contiguous.
+ * the weight FP32; up to 2^30 rows of 1 to 8192 columns, row strides in elements, outputs contiguous.
  */
 
 /* y [rows, d] BF16, stream_out [rows, d] = s, rstd [rows]. */
@@ -506,7 +506,7 @@ int ws_add_rmsnorm_backward(const void* stream_in, int stream_f32, const float* 
  *
  * y [rows, d] (BF16, or FP32 with y_f32) = scale * table[token] from a BF16 or FP32 table [vocab,
  * d] (row stride ld_table). A token of -100 is ignored: its row is zeros. Any other token outside
- * [0, vocab) gets NaN. Up to 33554430 rows of the table and 67108860 tokens.
+ * [0, vocab) gets NaN. Up to 2^22 rows of the table and 2^24 tokens.
  */
 int ws_embedding(const void* table, int64_t ld_table, int table_f32, const int64_t* tokens,
                  int64_t rows, int64_t vocab, int64_t d, float scale, void* y, int y_f32,
@@ -526,7 +526,7 @@ int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, const int64
  * Rows sorted by expert: rows offsets[e] to offsets[e + 1] of x belong to group e (offsets: groups + 1
  * int64 on the device, not decreasing). The offsets are read on the device only, and no value of theirs
  * leads an access out of the operands; decreasing ones leave rows of the result unspecified. BF16
- * operands, FP32 sums, 16-byte aligned rows, widths of a multiple of 8, 1 to 65536 groups.
+ * operands, FP32 sums, 16-byte aligned rows, widths of a multiple of 8, 1 to 65536 groups, up to 2^30 rows.
  */
 
 /* y [rows, n] BF16 = x [rows, k] times the transpose of the group's weight [n, k] (WS_GROUPED_NT:

@@ -102,6 +102,47 @@ def test_compiled_whole(name):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("odd", [False, True])
+def test_compiled_with_any_row_count(odd):
+    """One compiled function for all numbers of rows."""
+    from ops.embedding_execution import embedding
+    from ops.grouped_execution import grouped_mm
+    from ops.residual_norm import add_rmsnorm
+
+    g = torch.Generator().manual_seed(2)
+    d, n = (37, 11) if odd else (64, 48)
+    leaf = lambda *s: torch.randn(s, generator=g).cuda().requires_grad_(True)
+    table, weight, experts = leaf(30, d), leaf(d), leaf(3, n, d)
+
+    def step(tokens, offsets):
+        h = embedding(tokens, table, 0.5)
+        y, stream = add_rmsnorm(h, h.float(), weight)
+        return grouped_mm(y, experts, offsets), stream
+
+    compiled = torch.compile(step, fullgraph=True, backend="aot_eager", dynamic=True)
+    for rows in (5, 12, 700):
+        tokens = torch.randint(0, 30, (rows,), generator=g).cuda()
+        offsets = torch.tensor([0, rows // 3, rows // 2, rows]).cuda()
+        got, want = compiled(tokens, offsets), step(tokens, offsets)
+        up = [torch.ones_like(t) for t in want]
+        got = [*got, *torch.autograd.grad(got, [table, weight, experts], up)]
+        want = [*want, *torch.autograd.grad(want, [table, weight, experts], up)]
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), rows
+
+
+def test_inference_mode():
+    from ops.embedding_execution import embedding_accumulate_
+
+    for name, (call, x) in _calls().items():
+        want = call(x)
+        with torch.inference_mode():
+            assert torch.equal(call(x), want), name
+    with torch.inference_mode():
+        grad = torch.zeros((30, 8), device="cuda")
+        tokens, dy = torch.tensor([3, 3], device="cuda"), torch.ones((2, 8), device="cuda")
+        assert (embedding_accumulate_(grad, tokens, dy)[3] == 2).all()
+
+
 @pytest.mark.parametrize("requires", [False, True])
 def test_fake_tensors(requires):
     """Shapes and types without data."""

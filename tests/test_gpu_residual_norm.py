@@ -279,6 +279,25 @@ def test_python_form_gives_the_same_bits(stream, monkeypatch):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("scale_dtype", [E8M0, F32])
+def test_more_rows_than_one_launch_takes(scale_dtype):
+    from ops.residual_norm import add_rmsnorm, rmsnorm_quantize
+
+    rows, d = 4 * 2 ** 20 + 5, 8
+    g = torch.Generator("cuda").manual_seed(1)
+    x = torch.randn((rows, d), generator=g, device="cuda").to(BF16)
+    residual = torch.randn((rows, d), generator=g, device="cuda")
+    weight = torch.randn(d, generator=g, device="cuda")
+    y, out = add_rmsnorm(x, residual, weight, EPS)
+    assert torch.equal(out, x.float() + residual)
+    want = _formula(out, weight)
+    _close(y, want, want.abs() * (_half(BF16) + LANE_TERMS * U))
+    q, scale, out = rmsnorm_quantize(x, weight, EPS, residual=residual, scale_dtype=scale_dtype)
+    s = _scales(scale).expand(rows, d)
+    near = LANE_TERMS * U
+    _close(q.float().to(F64) * s, want, torch.maximum(want.abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + near) + near * want.abs())
+
+
 def test_past_2_31_elements():
     from ops.residual_norm import add_rmsnorm
 

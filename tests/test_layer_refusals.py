@@ -24,7 +24,7 @@ def test_cpu_tensors_are_refused():
     (dict(rows=-1), "shape"), (dict(d=0), "shape"), (dict(d=8193), "8192"), (dict(x=None), "null"),
     (dict(residual=None), "null"), (dict(w=None), "null"), (dict(y=None), "null"),
     (dict(out=None), "null"), (dict(rstd=None), "null"), (dict(ldx=7), "overlap"),
-    (dict(ldr=7), "overlap"), (dict(rows=2 ** 31), "shape")])
+    (dict(ldr=7), "overlap"), (dict(rows=2 ** 30 + 1), "shape")])
 def test_add_rmsnorm_arguments(change, match):
     a = dict(x=GPU, ldx=8, residual=GPU, ldr=8, w=GPU, rows=4, d=8, y=GPU, out=GPU, rstd=GPU) | change
     with pytest.raises(RuntimeError, match=match):
@@ -63,13 +63,13 @@ def test_partial_floats_of_bad_sizes():
     assert _hip.query("ws_add_rmsnorm_backward_partial_floats", 0, 8) == 0
     assert _hip.query("ws_add_rmsnorm_backward_partial_floats", 4, 8193) == 0
     assert _hip.query("ws_embedding_backward_workspace_bytes", -1, 8, 8) == 0
-    assert _hip.query("ws_embedding_backward_workspace_bytes", 8, 2 ** 31, 8) == 0
+    assert _hip.query("ws_embedding_backward_workspace_bytes", 8, 2 ** 22 + 1, 8) == 0
 
 
 @pytest.mark.parametrize("change,match", [
     (dict(rows=-1), "shape"), (dict(vocab=0), "shape"), (dict(d=0), "shape"), (dict(table=None), "null"),
     (dict(tokens=None), "null"), (dict(y=None), "null"), (dict(ld=7), "overlap"),
-    (dict(rows=2 ** 27), "shape"), (dict(vocab=2 ** 26), "shape")])
+    (dict(rows=2 ** 24 + 1), "shape"), (dict(vocab=2 ** 22 + 1), "shape")])
 def test_embedding_arguments(change, match):
     a = dict(table=GPU, ld=8, tokens=GPU, rows=4, vocab=10, d=8, y=GPU) | change
     with pytest.raises(RuntimeError, match=match):
@@ -95,7 +95,7 @@ def test_embedding_backward_arguments(change, match):
     (dict(w=None), "null"), (dict(offsets=None), "null"), (dict(y=None), "null"), (dict(x=GPU + 8), "aligned"),
     (dict(ldx=20), "aligned"), (dict(ldx=8), "overlap"), (dict(ldw=8), "overlap"), (dict(ldy=8), "overlap"),
     (dict(stride=12), "aligned"), (dict(stride=-8), "aligned"), (dict(ldy=4200000), "stride"),
-    (dict(rows=2 ** 30, n=2 ** 20, ldy=2 ** 20), "tiles")])
+    (dict(rows=2 ** 30, n=2 ** 20, ldy=2 ** 20), "tiles"), (dict(rows=2 ** 30 + 1), "shape")])
 def test_grouped_mm_arguments(change, match):
     a = dict(x=GPU, ldx=16, w=GPU, ldw=16, stride=256, form=0, offsets=GPU, groups=2, rows=4, n=16, k=16, y=GPU,
              ldy=16) | change

@@ -7,7 +7,7 @@ using namespace ws;
 
 namespace {
 
-constexpr int64_t kMaxGroups = 65536;
+constexpr int64_t kMaxGroups = 65536, kMaxRows = 1L << 30;
 // Beside FastTile: the kernel for few rows.
 constexpr int kTileFew = kFastTiles;
 // The most 256 x 256 tiles for 256 compute units whose round goes in pieces (grouped_fast_kernel).
@@ -81,7 +81,7 @@ int pick_grad(int64_t rows, int64_t groups, int64_t m, int64_t n) {
 
 int check_sizes(int64_t groups, int64_t rows, int64_t n, int64_t k) {
   if (groups < 1 || groups > kMaxGroups) return set_error(kInvalid, "1 to %ld groups, not %ld", (long)kMaxGroups, (long)groups);
-  if (rows < 0 || n < 1 || k < 1 || !fits_i32(rows) || !fits_i32(n) || !fits_i32(k))
+  if (rows < 0 || n < 1 || k < 1 || rows > kMaxRows || !fits_i32(n) || !fits_i32(k))
     return set_error(kInvalid, "invalid grouped product shape (%ld rows, %ld x %ld)", (long)rows, (long)n, (long)k);
   if (n % 8 != 0 || k % 8 != 0) return set_error(kInvalid, "grouped products take widths of a multiple of 8, not %ld and %ld", (long)n, (long)k);
   return kOk;

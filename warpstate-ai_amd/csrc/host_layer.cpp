@@ -21,7 +21,9 @@ Tensor rows_of(const Tensor& t) {
   const bool unit = (r.stride(1) == 1 || cols == 1) && (r.size(0) <= 1 || r.stride(0) >= cols);
   return unit ? r : r.contiguous();
 }
-int64_t last(const Tensor& t) { return t.dim() ? t.size(-1) : 0; }
+// A size that the checks and kernels go by: a number, also of a tensor traced with symbolic sizes (the row
+// counts, which may stay symbolic, are not asked for here).
+int64_t fixed(const Tensor& t, int64_t dim) { return t.sym_size(dim).guard_int(__FILE__, __LINE__); }
 
 // Gradients that are not differentiable again: where a graph of the backward is recorded, they stand
 // behind a node that depends on everything they were made `from`, and refuses.
@@ -58,15 +60,15 @@ constexpr char kNormTwice[] = "the residual norm cannot be differentiated twice"
 
 void check_norm(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight) {
   TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 && x.dim() >= 1, "Expected BF16 rows");
-  const int64_t d = x.size(-1);
+  const int64_t d = fixed(x, -1);
   TORCH_CHECK_VALUE(d >= 1 && d <= kMaxWidth, "RMSNorm takes rows of 1 to ", kMaxWidth, " columns, not ", d);
-  TORCH_CHECK_VALUE(weight.scalar_type() == at::kFloat && weight.dim() == 1 && weight.size(0) == d &&
+  TORCH_CHECK_VALUE(weight.scalar_type() == at::kFloat && weight.dim() == 1 && fixed(weight, 0) == d &&
                         weight.device() == x.device(),
                     "The norm's weight must be a vector of ", d, " values on ", x.device());
   if (residual.has_value())
     TORCH_CHECK_VALUE((residual->scalar_type() == at::kBFloat16 || residual->scalar_type() == at::kFloat) &&
-                          residual->sizes() == x.sizes() && residual->device() == x.device(),
-                      "The residual must be BF16 or FP32, of shape ", x.sizes(), " on ", x.device());
+                          residual->sym_sizes() == x.sym_sizes() && residual->device() == x.device(),
+                      "The residual must be BF16 or FP32, of shape ", x.sym_sizes(), " on ", x.device());
 }
 
 ThreeTensors add_rmsnorm_rstd(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
@@ -142,17 +144,17 @@ TwoTensors add_rmsnorm_autograd(const Tensor& x, const Tensor& residual, const T
 }
 TwoTensors add_rmsnorm_meta(const Tensor& x, const Tensor& residual, const Tensor& weight, double) {
   check_norm(x, residual, weight);
-  return {at::empty(x.sizes(), x.options()), at::empty(x.sizes(), residual.options())};
+  return {at::empty_symint(x.sym_sizes(), x.options()), at::empty_symint(x.sym_sizes(), residual.options())};
 }
 ThreeTensors add_rmsnorm_rstd_meta(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
   auto [y, stream] = add_rmsnorm_meta(x, residual, weight, eps);
-  return {y, stream, floats(x, {x.numel() / x.size(-1)})};
+  return {y, stream, at::empty_symint({x.sym_numel() / x.sym_size(-1)}, x.options().dtype(at::kFloat))};
 }
 ThreeTensors add_rmsnorm_backward_meta(const Tensor& stream, const Tensor& weight, const Tensor&, const Tensor& dy,
                                        const std::optional<Tensor>&) {
   const bool f32 = stream.scalar_type() == at::kFloat;
-  return {at::empty(stream.sizes(), dy.options()),
-          f32 ? at::empty(stream.sizes(), stream.options()) : at::empty({0}, stream.options()),
+  return {at::empty_symint(stream.sym_sizes(), dy.options()),
+          f32 ? at::empty_symint(stream.sym_sizes(), stream.options()) : at::empty({0}, stream.options()),
           at::empty_like(weight, at::MemoryFormat::Contiguous)};
 }
 
@@ -195,7 +197,7 @@ void check_embedding(const Tensor& tokens, const Tensor& table, double scale) {
   TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong && tokens.device() == table.device(),
                     "Tokens must be int64 on the table's device");
   TORCH_CHECK_VALUE((table.scalar_type() == at::kBFloat16 || table.scalar_type() == at::kFloat) && table.dim() == 2 &&
-                        table.numel() > 0,
+                        table.sym_numel() > 0,
                     "Expected a non-empty BF16 or FP32 table [vocab, d]");
   TORCH_CHECK_VALUE(std::isfinite(scale), "The scale must be finite, not ", scale);
 }
@@ -274,10 +276,12 @@ Tensor embedding_autograd(const Tensor& tokens, const Tensor& table, double scal
 }
 Tensor embedding_meta(const Tensor& tokens, const Tensor& table, double scale, bool f32) {
   check_embedding(tokens, table, scale);
-  return at::empty(embedded(tokens, table.size(1)), table.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+  c10::SymDimVector sizes(tokens.sym_sizes());
+  sizes.push_back(table.sym_size(1));
+  return at::empty_symint(sizes, table.options().dtype(f32 ? at::kFloat : at::kBFloat16));
 }
-Tensor embedding_backward_meta(const Tensor& dy, const Tensor&, int64_t vocab, double, bool f32) {
-  return at::empty({vocab, dy.size(-1)}, dy.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+Tensor embedding_backward_meta(const Tensor& dy, const Tensor&, c10::SymInt vocab, double, bool f32) {
+  return at::empty_symint({vocab, dy.sym_size(-1)}, dy.options().dtype(f32 ? at::kFloat : at::kBFloat16));
 }
 
 // --- products grouped by expert -------------------------------------------------------------
@@ -287,32 +291,34 @@ constexpr char kGroupedTwice[] = "grouped products cannot be differentiated twic
 void check_grouped(const Tensor& x, const Tensor& weight, const Tensor& offsets) {
   TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 && x.dim() == 2, "Grouped products take BF16 rows [rows, k]");
   TORCH_CHECK_VALUE((weight.scalar_type() == at::kBFloat16 || weight.scalar_type() == at::kFloat) &&
-                        weight.dim() == 3 && weight.numel() > 0 && weight.size(2) == x.size(1) &&
-                        weight.device() == x.device(),
-                    "Expected non-empty BF16 or FP32 weights [groups, n, ", x.size(1), "] on ", x.device());
+                        weight.dim() == 3 && fixed(weight, 0) > 0 && fixed(weight, 1) > 0 && fixed(weight, 2) > 0 &&
+                        fixed(weight, 2) == fixed(x, 1) && weight.device() == x.device(),
+                    "Expected non-empty BF16 or FP32 weights [groups, n, ", fixed(x, 1), "] on ", x.device());
   TORCH_CHECK_VALUE(offsets.scalar_type() == at::kLong && offsets.dim() == 1 &&
-                        offsets.size(0) == weight.size(0) + 1 && offsets.device() == x.device(),
+                        fixed(offsets, 0) == fixed(weight, 0) + 1 && offsets.device() == x.device(),
                     "Offsets must be an int64 vector, one more than the groups, on ", x.device());
 }
 // A matrix as the kernels read it: 16-byte rows of a multiple of 8, itself or a copy padded with
 // zeros.
 bool whole_rows(const Tensor& t) {
-  int64_t i = t.dim() - 1, inner = t.size(i);
-  if (inner % 8 != 0 || (t.stride(i) != 1 && inner != 1) || t.storage_offset() % 8 != 0) return false;
+  auto stride = [&](int64_t i) { return t.sym_stride(i).guard_int(__FILE__, __LINE__); };
+  int64_t i = t.dim() - 1, inner = fixed(t, i);
+  if (inner % 8 != 0 || (stride(i) != 1 && inner != 1) || t.sym_storage_offset().guard_int(__FILE__, __LINE__) % 8 != 0)
+    return false;
   while (i-- > 0) {
-    if (t.size(i) > 1 && (t.stride(i) % 8 != 0 || t.stride(i) < inner)) return false;
-    inner = t.size(i) * t.stride(i);
+    if (t.sym_size(i) > 1 && (stride(i) % 8 != 0 || stride(i) < inner)) return false;
+    if (i > 0) inner = fixed(t, i) * stride(i);
   }
   return true;
 }
 Tensor grouped_operand(const Tensor& t) {
   const Tensor b = t.to(at::kBFloat16);
-  if (whole_rows(b) && (t.dim() == 2 || t.size(1) % 8 == 0)) return b;
-  std::vector<int64_t> sizes = b.sizes().vec();
-  for (size_t i = 1; i < sizes.size(); ++i) sizes[i] = up(sizes[i], 8);
-  Tensor out = at::zeros(sizes, b.options());
-  Tensor part = out.narrow(-1, 0, b.size(-1));
-  if (t.dim() == 3) part = part.narrow(1, 0, b.size(1));
+  if (whole_rows(b) && (t.dim() == 2 || fixed(t, 1) % 8 == 0)) return b;
+  c10::SymDimVector sizes(b.sym_sizes());
+  for (int64_t i = 1; i < b.dim(); ++i) sizes[i] = up(fixed(b, i), 8);
+  Tensor out = at::zeros_symint(sizes, b.options());
+  Tensor part = out.narrow(-1, 0, fixed(b, -1));
+  if (t.dim() == 3) part = part.narrow(1, 0, fixed(b, 1));
   part.copy_(b);
   return out;
 }
@@ -343,7 +349,7 @@ Tensor grouped_grad(const Tensor& dy, const Tensor& x, const Tensor& offsets_in,
 typedef Tensor GroupedRows(const Tensor&, const Tensor&, const Tensor&, int64_t);
 typedef Tensor GroupedGrad(const Tensor&, const Tensor&, const Tensor&, bool);
 Tensor first_columns(const Tensor& t, int64_t cols) {
-  return t.size(-1) == cols ? t : t.narrow(-1, 0, cols).contiguous();
+  return fixed(t, -1) == cols ? t : t.narrow(-1, 0, cols).contiguous();
 }
 
 Tensor grouped_mm(const Tensor& x, const Tensor& weight, const Tensor& offsets) {
@@ -364,10 +370,10 @@ struct GroupedMmFn : Function<GroupedMmFn> {
     ctx->save_for_backward({weight.requires_grad() ? a : Tensor(), x.requires_grad() ? w : Tensor(), offsets, x, weight});
     ctx->saved_data["want_x"] = x.requires_grad();
     ctx->saved_data["want_w"] = weight.requires_grad();
-    ctx->saved_data["n"] = weight.size(1);
-    ctx->saved_data["k"] = x.size(1);
+    ctx->saved_data["n"] = fixed(weight, 1);
+    ctx->saved_data["k"] = fixed(x, 1);
     ctx->saved_data["f32"] = weight.scalar_type() == at::kFloat;
-    return first_columns(op.call(a, w, offsets, WS_GROUPED_NT), weight.size(1));
+    return first_columns(op.call(a, w, offsets, WS_GROUPED_NT), fixed(weight, 1));
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static const auto rows_op = find<GroupedRows>("warpstate::native_grouped_rows");
@@ -382,7 +388,7 @@ struct GroupedMmFn : Function<GroupedMmFn> {
       if (ctx->saved_data["want_x"].toBool()) d[0] = first_columns(rows_op.call(g, s[1], s[2], WS_GROUPED_NN), k);
       if (ctx->saved_data["want_w"].toBool()) {
         Tensor dw = grad_op.call(g, s[0], s[2], ctx->saved_data["f32"].toBool());
-        if (dw.size(1) != n || dw.size(2) != k) dw = dw.narrow(1, 0, n).narrow(2, 0, k).contiguous();
+        if (fixed(dw, 1) != n || fixed(dw, 2) != k) dw = dw.narrow(1, 0, n).narrow(2, 0, k).contiguous();
         d[1] = dw;
       }
     }
@@ -396,7 +402,6 @@ Tensor grouped_mm_autograd(const Tensor& x, const Tensor& weight, const Tensor& 
     return below(op, x, weight, offsets);
   }
   check_grouped(x, weight, offsets);
-  c10::DeviceGuard guard(x.device());
   Tensor a, w;
   {
     at::AutoDispatchBelowAutograd below_autograd;
@@ -407,13 +412,14 @@ Tensor grouped_mm_autograd(const Tensor& x, const Tensor& weight, const Tensor& 
 }
 Tensor grouped_mm_meta(const Tensor& x, const Tensor& weight, const Tensor& offsets) {
   check_grouped(x, weight, offsets);
-  return at::empty({x.size(0), weight.size(1)}, x.options());
+  return at::empty_symint({x.sym_size(0), weight.sym_size(1)}, x.options());
 }
 Tensor grouped_rows_meta(const Tensor& x, const Tensor& w, const Tensor&, int64_t form) {
-  return at::empty({x.size(0), w.size(form == WS_GROUPED_NT ? 1 : 2)}, x.options());
+  return at::empty_symint({x.sym_size(0), w.sym_size(form == WS_GROUPED_NT ? 1 : 2)}, x.options());
 }
 Tensor grouped_grad_meta(const Tensor& dy, const Tensor& x, const Tensor& offsets, bool f32) {
-  return at::empty({offsets.size(0) - 1, dy.size(1), x.size(1)}, x.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+  return at::empty_symint({offsets.sym_size(0) - 1, dy.sym_size(1), x.sym_size(1)},
+                          x.options().dtype(f32 ? at::kFloat : at::kBFloat16));
 }
 
 }  // namespace

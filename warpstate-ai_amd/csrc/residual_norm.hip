@@ -8,12 +8,12 @@ using namespace ws;
 
 namespace {
 
-constexpr int64_t kMaxWidth = 8192;
+constexpr int64_t kMaxWidth = 8192, kMaxRows = 1L << 30;
 // Rows of one launch: fewer than 2^32 threads.
 constexpr int64_t kLaunchRows = 1L << 22;
 
 int check_shape(int64_t rows, int64_t d) {
-  if (rows < 0 || d < 1 || !fits_i32(rows)) return set_error(kInvalid, "invalid RMSNorm shape");
+  if (rows < 0 || d < 1 || rows > kMaxRows) return set_error(kInvalid, "invalid RMSNorm shape");
   if (d > kMaxWidth) return set_error(kInvalid, "RMSNorm takes rows of at most %ld columns (got %ld)", kMaxWidth, (long)d);
   return kOk;
 }
@@ -160,7 +160,7 @@ extern "C" int ws_rmsnorm_quantize(const void* x, int64_t ldx, const void* resid
 }
 
 extern "C" int64_t ws_add_rmsnorm_backward_partial_floats(int64_t rows, int64_t d) {
-  if (rows < 1 || d < 1 || d > kMaxWidth || !fits_i32(rows)) return 0;
+  if (rows < 1 || d < 1 || d > kMaxWidth || rows > kMaxRows) return 0;
   return backward_groups(rows, d) * d;
 }
 

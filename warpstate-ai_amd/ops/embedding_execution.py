@@ -84,7 +84,8 @@ def embedding(tokens: Tensor, table: Tensor, scale: float = 1.0,
     master, any strides), in ``out_dtype`` (BF16 or FP32), with autograd to the table.
 
     Each row is scaled in FP32 and rounded once. The gradient comes in the table's type from FP32
-    sums, all of it written (rows without tokens are zeros)."""
+    sums, all of it written (rows without tokens are zeros). Up to 2^22 rows of the table and 2^24
+    tokens."""
     if not table.is_cuda:
         raise ValueError("Embeddings require CUDA tensors")
     if out_dtype not in (BF16, F32):
@@ -95,6 +96,11 @@ def embedding(tokens: Tensor, table: Tensor, scale: float = 1.0,
     _check(tokens, table, scale)
     _refuse_tangents("embedding", table)
     return _Embedding.apply(tokens, table, float(scale), out_dtype == F32)
+
+
+def _written(t: Tensor) -> None:
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
 
 
 @torch.no_grad()
@@ -108,7 +114,7 @@ def embedding_accumulate_(gradient: Tensor, tokens: Tensor, dy: Tensor, scale: f
     native = _hip.host_ops()
     if native is not None:
         native.native_embedding_accumulate_(gradient, tokens, dy, scale)
-        torch.autograd.graph.increment_version(gradient)
+        _written(gradient)
         return gradient
     if (gradient.dtype != F32 or gradient.ndim != 2 or gradient.numel() == 0
             or (gradient.stride(1) != 1 and gradient.shape[1] != 1)
@@ -123,5 +129,5 @@ def embedding_accumulate_(gradient: Tensor, tokens: Tensor, dy: Tensor, scale: f
     if not math.isfinite(scale):
         raise ValueError(f"The scale must be finite, not {scale}")
     _sums(dy, tokens, float(scale), gradient, _ADD_F32)
-    torch.autograd.graph.increment_version(gradient)
+    _written(gradient)
     return gradient
