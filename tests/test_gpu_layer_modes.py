@@ -102,6 +102,38 @@ def test_compiled_whole(name):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("stream", [True, False])
+def test_compiled_quantization(stream, native, monkeypatch):
+    """The 8-bit norm and the product that reads it in one compiled function; without the C++
+    operators they run eagerly in it, as do the others."""
+    from ops import _hip
+    from ops import fp8_execution as fp8
+    from ops.embedding_execution import embedding, embedding_accumulate_
+    from ops.grouped_execution import grouped_mm
+    from ops.residual_norm import add_rmsnorm, rmsnorm_quantize
+
+    if not native:
+        monkeypatch.setattr(_hip, "host_ops", lambda: None)
+    g = torch.Generator().manual_seed(4)
+    x, residual = (torch.randn((7, 200), generator=g).to(BF16).cuda() for _ in range(2))
+    weight, experts = torch.ones(200, device="cuda"), torch.randn((2, 200, 200), generator=g).to(BF16).cuda()
+    tokens, offsets = torch.arange(7, device="cuda"), torch.tensor([0, 3, 7], device="cuda")
+
+    def step(x):
+        q, scale, out = rmsnorm_quantize(x, weight, residual=residual if stream else None)
+        q32, scale32, _ = rmsnorm_quantize(x, weight, scale_dtype=F32)
+        y, _ = add_rmsnorm(x + embedding(tokens, residual), residual, weight)
+        grad = embedding_accumulate_(torch.zeros((9, 200), device="cuda"), tokens, y)
+        return (q.float(), scale.view(torch.uint8), out * 2, q32.float(), scale32 * 1, grad,
+                grouped_mm(y, experts, offsets))
+
+    want = step(x)
+    got = torch.compile(step, backend="aot_eager")(x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert [t.stride() for t in got[:2]] == [t.stride() for t in want[:2]]
+
+
 @pytest.mark.parametrize("odd", [False, True])
 def test_compiled_with_any_row_count(odd):
     """One compiled function for all numbers of rows."""

@@ -188,6 +188,18 @@ ThreeTensors rmsnorm_quantize_autograd(const Tensor& x, const std::optional<Tens
   return below(op, x, residual, weight, eps, e8m0);
 }
 
+ThreeTensors rmsnorm_quantize_meta(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight, double,
+                                   bool e8m0) {
+  check_norm(x, residual, weight);
+  TORCH_CHECK_VALUE(x.sym_numel() > 0, "Quantization takes non-empty rows");
+  const int64_t d = fixed(x, -1), n = blocks(d);
+  const c10::SymInt rows = x.sym_numel() / d;
+  Tensor q = at::empty_symint({rows, up(d, 16)}, x.options().dtype(at::kFloat8_e4m3fn)).narrow(1, 0, d);
+  Tensor scale = e8m0 ? at::empty_symint({rows, up(n, 4)}, x.options().dtype(at::kFloat8_e8m0fnu)).narrow(1, 0, n)
+                      : at::empty_symint({n, (rows + 3) / 4 * 4}, x.options().dtype(at::kFloat)).narrow_symint(1, 0, rows).t();
+  return {q, scale, residual.has_value() ? at::empty_symint(x.sym_sizes(), residual->options()) : at::empty({0}, x.options())};
+}
+
 // --- embedding ------------------------------------------------------------------------------
 
 constexpr char kEmbeddingTwice[] = "the embedding cannot be differentiated twice";
@@ -462,6 +474,7 @@ TORCH_LIBRARY_IMPL(warpstate, Meta, m) {
   m.impl("native_add_rmsnorm", &add_rmsnorm_meta);
   m.impl("native_add_rmsnorm_rstd", &add_rmsnorm_rstd_meta);
   m.impl("native_add_rmsnorm_backward", &add_rmsnorm_backward_meta);
+  m.impl("native_rmsnorm_quantize", &rmsnorm_quantize_meta);
   m.impl("native_embedding", &embedding_meta);
   m.impl("native_embedding_backward", &embedding_backward_meta);
   m.impl("native_grouped_mm", &grouped_mm_meta);

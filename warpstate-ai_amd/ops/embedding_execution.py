@@ -93,9 +93,15 @@ def embedding(tokens: Tensor, table: Tensor, scale: float = 1.0,
     native = _hip.host_ops()
     if native is not None:
         return native.native_embedding(tokens, table, scale, out_dtype == F32)
+    return _embedding(tokens, table, float(scale), out_dtype == F32)
+
+
+# (Without the C++ operators it runs eagerly inside a compiled function.)
+@torch.compiler.disable
+def _embedding(tokens: Tensor, table: Tensor, scale: float, f32: bool) -> Tensor:
     _check(tokens, table, scale)
     _refuse_tangents("embedding", table)
-    return _Embedding.apply(tokens, table, float(scale), out_dtype == F32)
+    return _Embedding.apply(tokens, table, scale, f32)
 
 
 def _written(t: Tensor) -> None:
@@ -103,12 +109,14 @@ def _written(t: Tensor) -> None:
         torch.autograd.graph.increment_version(t)
 
 
+@torch.compiler.disable
 @torch.no_grad()
 def embedding_accumulate_(gradient: Tensor, tokens: Tensor, dy: Tensor, scale: float = 1.0
                           ) -> Tensor:
     """gradient += scale * the sums of dy [..., d] (BF16 or FP32) by token, for an FP32 gradient
     [vocab, d] with a unit column stride. Rows without tokens are neither read nor written.
-    Returns the gradient; no graph is recorded."""
+    Returns the gradient; no graph is recorded. Under torch.compile it runs eagerly (a graph
+    break)."""
     if not gradient.is_cuda:
         raise ValueError("Embeddings require CUDA tensors")
     native = _hip.host_ops()

@@ -131,6 +131,12 @@ def grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:
     native = _hip.host_ops()
     if native is not None:
         return native.native_grouped_mm(x, weight, offsets)
+    return _grouped_mm(x, weight, offsets)
+
+
+# (Without the C++ operators it runs eagerly inside a compiled function.)
+@torch.compiler.disable
+def _grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:
     _check(x, weight, offsets)
     _refuse_tangents("grouped_mm", x, weight)
     return _GroupedMm.apply(x, weight, _operand(x.detach()), _operand(weight.detach()),

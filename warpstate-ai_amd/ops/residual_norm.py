@@ -153,9 +153,15 @@ def add_rmsnorm(x: Tensor, residual: Tensor, weight: Tensor, eps: float = 1e-5
     native = _hip.host_ops()
     if native is not None:
         return native.native_add_rmsnorm(x, residual, weight, eps)
+    return _add_rmsnorm(x, residual, weight, float(eps))
+
+
+# (The forms without the C++ operators run eagerly inside a compiled function.)
+@torch.compiler.disable
+def _add_rmsnorm(x: Tensor, residual: Tensor, weight: Tensor, eps: float) -> tuple[Tensor, Tensor]:
     _check(x, residual, weight)
     _refuse_tangents("add_rmsnorm", x, residual, weight)
-    return _AddRmsnorm.apply(x, residual, weight, float(eps))
+    return _AddRmsnorm.apply(x, residual, weight, eps)
 
 
 def rmsnorm_quantize(x: Tensor, weight: Tensor, eps: float = 1e-5, residual: Tensor | None = None,
@@ -173,6 +179,11 @@ def rmsnorm_quantize(x: Tensor, weight: Tensor, eps: float = 1e-5, residual: Ten
     if native is not None:
         q, scale, stream = native.native_rmsnorm_quantize(x, residual, weight, eps, e8m0)
         return q, scale, x.detach() if residual is None else stream
+    return _rmsnorm_quantize(x, residual, weight, float(eps), e8m0)
+
+
+@torch.compiler.disable
+def _rmsnorm_quantize(x, residual, weight, eps, e8m0):
     _check(x, residual, weight)
     _refuse_tangents("rmsnorm_quantize", x, residual, weight)
     if x.numel() == 0:
@@ -187,6 +198,6 @@ def rmsnorm_quantize(x: Tensor, weight: Tensor, eps: float = 1e-5, residual: Ten
     q, scale = _data(rows, d, x.device), _scales(rows, _blocks(d), e8m0, x.device)
     _hip.call_on(x, "ws_rmsnorm_quantize", a.data_ptr(), _row_stride(a), _hip.ptr(r),
                  0 if r is None else _row_stride(r), int(r is not None and r.dtype == F32),
-                 w.data_ptr(), float(eps), rows, d, int(not e8m0), q.data_ptr(), q.shape[1],
+                 w.data_ptr(), eps, rows, d, int(not e8m0), q.data_ptr(), q.shape[1],
                  scale.data_ptr(), scale.shape[1], _hip.ptr(stream))
     return (*_views(q, scale, d, e8m0, rows), x if stream is None else stream)
