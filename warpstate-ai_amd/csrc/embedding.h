@@ -15,10 +15,11 @@
 namespace ws {
 
 constexpr long kIgnoredToken = -100;
+typedef unsigned u32x2_any2 __attribute__((ext_vector_type(2), aligned(2)));
 
 // A wave per token, 64 x 8 columns at a time. Ignored tokens get zeros, others outside the
 // vocabulary NaN; neither reads the table.
-template <bool TF32, bool OF32, bool VEC>
+template <bool TF32, bool OF32, bool WHOLE>
 static __global__ void __launch_bounds__(256) embed_lookup_kernel(const void* table, long ld, const long* tokens,
                                                                   int rows, int vocab, int d, float scale, void* y) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -30,11 +31,11 @@ static __global__ void __launch_bounds__(256) embed_lookup_kernel(const void* ta
 #pragma unroll 4
   for (int c = 8 * lane; c < d; c += 512) {
     QuantRow<TF32> v;
-    if (known) load_piece<TF32, VEC>(v, table, token * ld + c, d - c);
+    if (known) load_piece<TF32, WHOLE>(v, table, token * ld + c, d - c);
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = known ? v.at(e) * scale : fill;
-    store_piece<OF32, VEC>(round_piece<OF32>(f), y, (long)row * d + c, d - c);
+    store_piece<OF32, WHOLE>(round_piece<OF32>(f), y, (long)row * d + c, d - c);
   }
 }
 
@@ -152,20 +153,20 @@ struct EmbedPiece {
     else return (e & 1) ? hi_bf16(w[e >> 1]) : lo_bf16(w[e >> 1]);
   }
 };
-template <bool F32, int W, bool VEC>
+template <bool F32, int W, bool WHOLE>
 __device__ __forceinline__ EmbedPiece<F32, W> embed_load(const void* base, long at, int left) {
   constexpr int kWords = F32 ? W : W / 2;
   EmbedPiece<F32, W> v;
   const char* src = static_cast<const char*>(base) + at * (F32 ? 4 : 2);
-  if (VEC && left >= W) {
+  if (left >= W) {
     if constexpr (kWords == 2) {
-      const u32x2_t a = *reinterpret_cast<const u32x2_t*>(src);
+      const u32x2_t a = *reinterpret_cast<const u32x2_any2*>(src);
       v.w[0] = a[0];
       v.w[1] = a[1];
     } else {
 #pragma unroll
       for (int q = 0; q < kWords / 4; ++q) {
-        const u32x4_t a = reinterpret_cast<const u32x4_t*>(src)[q];
+        const u32x4_t a = reinterpret_cast<const u32x4_any2*>(src)[q];
 #pragma unroll
         for (int d = 0; d < 4; ++d) v.w[4 * q + d] = a[d];
       }
@@ -174,7 +175,7 @@ __device__ __forceinline__ EmbedPiece<F32, W> embed_load(const void* base, long 
   }
 #pragma unroll
   for (int d = 0; d < kWords; ++d) v.w[d] = 0;
-  if (VEC) return v;  // whole pieces only
+  if (WHOLE || left <= 0) return v;
 #pragma unroll
   for (int e = 0; e < W; ++e) {
     if (e >= left) continue;
@@ -183,27 +184,28 @@ __device__ __forceinline__ EmbedPiece<F32, W> embed_load(const void* base, long 
   }
   return v;
 }
-template <bool F32, int W, bool VEC, bool NT = false>
+template <bool F32, int W, bool WHOLE, bool NT = false>
 __device__ __forceinline__ void embed_write(const float (&f)[W], void* base, long at, int left) {
   char* dst = static_cast<char*>(base) + at * (F32 ? 4 : 2);
-  if (VEC && left >= W) {
+  if (left >= W) {
     if constexpr (F32) {
 #pragma unroll
       for (int q = 0; q < W / 4; ++q) {
-        const f32x4_t v = {f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]};
-        if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<f32x4_t*>(dst) + q);
-        else reinterpret_cast<f32x4_t*>(dst)[q] = v;
+        const u32x4_t v = {__float_as_uint(f[4 * q]), __float_as_uint(f[4 * q + 1]), __float_as_uint(f[4 * q + 2]),
+                           __float_as_uint(f[4 * q + 3])};
+        if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any4*>(dst) + q);
+        else reinterpret_cast<u32x4_any4*>(dst)[q] = v;
       }
     } else {
       static_assert(F32 || W == 8, "BF16 pieces are 16 bytes");
       const u32x4_t v = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[W - 4], f[W - 3]),
                          pack_bf16x2(f[W - 2], f[W - 1])};
-      if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(dst));
-      else *reinterpret_cast<u32x4_t*>(dst) = v;
+      if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any2*>(dst));
+      else *reinterpret_cast<u32x4_any2*>(dst) = v;
     }
     return;
   }
-  if (VEC) return;
+  if (WHOLE || left <= 0) return;
 #pragma unroll
   for (int e = 0; e < W; ++e) {
     if (e >= left) continue;
@@ -216,7 +218,7 @@ __device__ __forceinline__ void embed_write(const float (&f)[W], void* base, lon
 // c + 64 W, ..: the positions of 64 rows are one load, a position on each lane (so all 64 lanes come here, those
 // past the last column too), and then kAhead rows of dy at a time are in flight. `before(at, acc)`
 // comes before the row at position `at` is added, and may store the sums and clear them.
-template <bool GF32, int NC, int W, bool VEC, class Before>
+template <bool GF32, int NC, int W, bool WHOLE, class Before>
 __device__ __forceinline__ void embed_walk(const EmbedGradParams& p, int begin, int end, int c, int lane,
                                            float (&acc)[NC][W], Before&& before) {
   constexpr int kAhead = GF32 ? 2 : 4;
@@ -230,7 +232,7 @@ __device__ __forceinline__ void embed_walk(const EmbedGradParams& p, int begin, 
         const long row = __builtin_amdgcn_readlane(rows, min(j + a, n - 1));
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-          v[a][i] = embed_load<GF32, W, VEC>(p.dy, row * p.ld_dy + c + 64 * W * i, p.d - c - 64 * W * i);
+          v[a][i] = embed_load<GF32, W, WHOLE>(p.dy, row * p.ld_dy + c + 64 * W * i, p.d - c - 64 * W * i);
       }
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
@@ -252,24 +254,24 @@ __device__ __forceinline__ void embed_clear(float (&acc)[NC][W]) {
     for (int e = 0; e < W; ++e) acc[i][e] = 0.0f;
 }
 
-template <int OUT, int W, bool VEC, bool NT>
+template <int OUT, int W, bool WHOLE, bool NT>
 __device__ __forceinline__ void embed_store(const EmbedGradParams& p, long v, int c, float (&acc)[W]) {
   const long at = v * p.ld_out + c;
 #pragma unroll
   for (int e = 0; e < W; ++e) acc[e] *= p.scale;
   if constexpr (OUT == kEmbedAdd) {
-    const auto old = embed_load<true, W, VEC>(p.out, at, p.d - c);
+    const auto old = embed_load<true, W, WHOLE>(p.out, at, p.d - c);
 #pragma unroll
     for (int e = 0; e < W; ++e) acc[e] += old.at(e);
   }
-  embed_write<OUT != kEmbedBF16, W, VEC, NT>(acc, p.out, at, p.d - c);
+  embed_write<OUT != kEmbedBF16, W, WHOLE, NT>(acc, p.out, at, p.d - c);
 }
 
 // A wave per piece of the sorted positions, then a wave per `group` rows of the table, whose
 // positions lie one after the other: the rows of dy of all of them are requested as one run, so
 // that a row with one token or none, the usual one, does not wait for its own chain of loads. NT:
 // the output goes around the caches.
-template <bool GF32, int OUT, bool VEC, bool NT>
+template <bool GF32, int OUT, bool WHOLE, bool NT>
 static __global__ void __launch_bounds__(256) embed_grad_kernel(const EmbedGradParams p) {
   constexpr int W = OUT == kEmbedBF16 ? 8 : 4, NC = 32 / W, kSpan = 64 * W;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -289,7 +291,7 @@ static __global__ void __launch_bounds__(256) embed_grad_kernel(const EmbedGradP
       for (int c0 = 0; c0 < p.d; c0 += kSpan * NC) {
         const int c = c0 + W * lane;
         embed_clear(acc);
-        embed_walk<GF32, NC, W, VEC>(p, part ? s : begin, part ? end : min(e, end), c, lane, acc, [](int) {});
+        embed_walk<GF32, NC, W, WHOLE>(p, part ? s : begin, part ? end : min(e, end), c, lane, acc, [](int) {});
 #pragma unroll
         for (int i = 0; i < NC; ++i)
           if (c + kSpan * i < p.d)
@@ -312,7 +314,7 @@ static __global__ void __launch_bounds__(256) embed_grad_kernel(const EmbedGradP
       if (n <= p.piece && (OUT != kEmbedAdd || n > 0)) {
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-          if (c + kSpan * i < p.d) embed_store<OUT, W, VEC, NT>(p, v0 + r, c + kSpan * i, acc[i]);
+          if (c + kSpan * i < p.d) embed_store<OUT, W, WHOLE, NT>(p, v0 + r, c + kSpan * i, acc[i]);
       }
       embed_clear(acc);
       ++r;
@@ -322,7 +324,7 @@ static __global__ void __launch_bounds__(256) embed_grad_kernel(const EmbedGradP
     while (r < rows) {
       int to = r;
       while (to < rows && __builtin_amdgcn_readlane(begins, to + 1) - __builtin_amdgcn_readlane(begins, to) <= p.piece) ++to;
-      embed_walk<GF32, NC, W, VEC>(p, __builtin_amdgcn_readlane(begins, r), __builtin_amdgcn_readlane(begins, to), c, lane, acc,
+      embed_walk<GF32, NC, W, WHOLE>(p, __builtin_amdgcn_readlane(begins, r), __builtin_amdgcn_readlane(begins, to), c, lane, acc,
                                 [&](int at) {
                                   while (at >= __builtin_amdgcn_readlane(begins, r + 1)) store();
                                 });
@@ -333,7 +335,7 @@ static __global__ void __launch_bounds__(256) embed_grad_kernel(const EmbedGradP
 
 // Adds the pieces of the token that begins in piece blockIdx.x and runs past it, in their order: a
 // quarter of them on each wave, 64 W columns a workgroup.
-template <int OUT, bool VEC>
+template <int OUT, bool WHOLE>
 static __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedGradParams p) {
   const int total = p.start[p.vocab], q = blockIdx.x, begin = q * p.piece;
   if (begin >= total) return;
@@ -367,7 +369,7 @@ static __global__ void __launch_bounds__(256) embed_join_kernel(const EmbedGradP
   if (wave > 0 || c >= p.d) return;
 #pragma unroll
   for (int k = 0; k < W; ++k) acc[k] = (sums[0][k][lane] + sums[1][k][lane]) + (sums[2][k][lane] + sums[3][k][lane]);
-  embed_store<OUT, W, VEC, false>(p, v, c, acc);
+  embed_store<OUT, W, WHOLE, false>(p, v, c, acc);
 }
 
 }  // namespace ws

@@ -16,8 +16,6 @@ int check_table(int64_t rows, int64_t vocab, int64_t d, int64_t ld) {
   if (vocab > 1 && ld < d) return set_error(kInvalid, "rows overlap");
   return kOk;
 }
-bool pieces(const void* p, long ld, int bytes) { return al(p, 16) && ld * bytes % 16 == 0; }
-
 // Positions of one piece of a token that occurs more often: 32, or as many as leave 1024 pieces.
 int64_t piece_rows(int64_t rows) { return rows <= 32 * 1024 ? 32 : (rows + 1023) / 1024; }
 
@@ -42,19 +40,19 @@ GradLayout grad_layout(int64_t rows, int64_t vocab, int64_t d) {
 bool past_caches(int64_t bytes) { return bytes > 256L << 20; }
 
 template <bool GF32, int OUT>
-int launch_grad(const EmbedGradParams& p, int64_t rows, bool vec, hipStream_t s) {
+int launch_grad(const EmbedGradParams& p, int64_t rows, bool whole, hipStream_t s) {
   const dim3 grid((unsigned)cdiv(p.pieces + cdiv(p.vocab, p.group), 4)), block(256);
   const bool nt = OUT != kEmbedAdd && past_caches(p.d * ((int64_t)p.vocab * (OUT == kEmbedBF16 ? 2 : 4) + rows * (GF32 ? 4 : 2)));
   auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, p); };
   if constexpr (OUT != kEmbedAdd) {
-    if (vec && nt) run(&embed_grad_kernel<GF32, OUT, true, true>);
+    if (whole && nt) run(&embed_grad_kernel<GF32, OUT, true, true>);
   }
-  if (vec && !nt) run(&embed_grad_kernel<GF32, OUT, true, false>);
-  if (!vec) run(&embed_grad_kernel<GF32, OUT, false, false>);
+  if (whole && !nt) run(&embed_grad_kernel<GF32, OUT, true, false>);
+  if (!whole) run(&embed_grad_kernel<GF32, OUT, false, false>);
   if (int rc = hip_check(hipGetLastError(), "embedding gradient launch")) return rc;
   if (p.pieces == 0) return kOk;
   const dim3 join(p.pieces, cdiv(p.d, OUT == kEmbedBF16 ? 512 : 256));
-  if (vec) hipLaunchKernelGGL((embed_join_kernel<OUT, true>), join, block, 0, s, p);
+  if (whole) hipLaunchKernelGGL((embed_join_kernel<OUT, true>), join, block, 0, s, p);
   else hipLaunchKernelGGL((embed_join_kernel<OUT, false>), join, block, 0, s, p);
   return hip_check(hipGetLastError(), "embedding gradient join launch");
 }
@@ -66,17 +64,17 @@ extern "C" int ws_embedding(const void* table, int64_t ld_table, int table_f32, 
   if (int rc = check_table(rows, vocab, d, ld_table)) return rc;
   if (rows == 0) return kOk;
   if (!table || !tokens || !y) return set_error(kInvalid, "null pointer");
-  const bool vec = d % 8 == 0 && pieces(table, ld_table, table_f32 ? 4 : 2) && al(y, 16);
+  const bool whole = d % 8 == 0;
   auto run = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(cdiv(rows, 4)), dim3(256), 0, static_cast<hipStream_t>(stream), table,
                        (long)ld_table, reinterpret_cast<const long*>(tokens), (int)rows, (int)vocab, (int)d, scale, y);
     return hip_check(hipGetLastError(), "embedding launch");
   };
   if (table_f32)
-    return y_f32 ? (vec ? run(&embed_lookup_kernel<true, true, true>) : run(&embed_lookup_kernel<true, true, false>))
-                 : (vec ? run(&embed_lookup_kernel<true, false, true>) : run(&embed_lookup_kernel<true, false, false>));
-  return y_f32 ? (vec ? run(&embed_lookup_kernel<false, true, true>) : run(&embed_lookup_kernel<false, true, false>))
-               : (vec ? run(&embed_lookup_kernel<false, false, true>) : run(&embed_lookup_kernel<false, false, false>));
+    return y_f32 ? (whole ? run(&embed_lookup_kernel<true, true, true>) : run(&embed_lookup_kernel<true, true, false>))
+                 : (whole ? run(&embed_lookup_kernel<true, false, true>) : run(&embed_lookup_kernel<true, false, false>));
+  return y_f32 ? (whole ? run(&embed_lookup_kernel<false, true, true>) : run(&embed_lookup_kernel<false, true, false>))
+               : (whole ? run(&embed_lookup_kernel<false, false, true>) : run(&embed_lookup_kernel<false, false, false>));
 }
 
 extern "C" int64_t ws_embedding_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d) {
@@ -120,11 +118,11 @@ extern "C" int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, 
   hipLaunchKernelGGL(embed_sort_kernel, dim3(cdiv(vocab, range)), dim3(64 * kSortWaves), 0, s, p.tokens, (int)rows,
                      (int)vocab, (int)range, const_cast<int*>(p.start), const_cast<int*>(p.perm));
   if (int rc = hip_check(hipGetLastError(), "embedding sort launch")) return rc;
-  const bool vec = d % 8 == 0 && pieces(dy, ld_dy, dy_f32 ? 4 : 2) && pieces(dtable, ld_dtable, mode == WS_EMBED_WRITE_BF16 ? 2 : 4);
+  const bool whole = d % 8 == 0;
 #define WS_GRAD(G_)                                                                                   \
-  (mode == WS_EMBED_WRITE_BF16  ? launch_grad<G_, kEmbedBF16>(p, rows, vec, s)                              \
-   : mode == WS_EMBED_WRITE_F32 ? launch_grad<G_, kEmbedF32>(p, rows, vec, s)                               \
-                                : launch_grad<G_, kEmbedAdd>(p, rows, vec, s))
+  (mode == WS_EMBED_WRITE_BF16  ? launch_grad<G_, kEmbedBF16>(p, rows, whole, s)                              \
+   : mode == WS_EMBED_WRITE_F32 ? launch_grad<G_, kEmbedF32>(p, rows, whole, s)                               \
+                                : launch_grad<G_, kEmbedAdd>(p, rows, whole, s))
   return dy_f32 ? WS_GRAD(true) : WS_GRAD(false);
 #undef WS_GRAD
 }

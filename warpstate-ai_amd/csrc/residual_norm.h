@@ -32,12 +32,17 @@ struct AddNormParams {
   void* scale; long ld_scale;
 };
 
-// Eight elements at p, of which `left` exist (zeros for the others).
-template <bool F32, bool VEC>
+// 16 bytes at any address of their elements: the vector instructions do not need more.
+typedef unsigned u32x4_any2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x4_any4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Eight elements from element `at` on, of which `left` exist (zeros for the others). WHOLE: rows are
+// whole pieces, so that left is at least eight or at most zero.
+template <bool F32, bool WHOLE>
 __device__ __forceinline__ void load_piece(QuantRow<F32>& v, const void* base, long at, int left) {
-  if (VEC && left >= 8) {
+  if (left >= 8) {
     if constexpr (F32) {
-      const auto* src = reinterpret_cast<const u32x4_t*>(static_cast<const float*>(base) + at);
+      const auto* src = reinterpret_cast<const u32x4_any4*>(static_cast<const float*>(base) + at);
       const u32x4_t a = src[0], b = src[1];
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
@@ -45,7 +50,7 @@ __device__ __forceinline__ void load_piece(QuantRow<F32>& v, const void* base, l
         v.w[4 + d] = b[d];
       }
     } else {
-      const u32x4_t a = *reinterpret_cast<const u32x4_t*>(static_cast<const unsigned short*>(base) + at);
+      const u32x4_t a = *reinterpret_cast<const u32x4_any2*>(static_cast<const unsigned short*>(base) + at);
 #pragma unroll
       for (int d = 0; d < 4; ++d) v.w[d] = a[d];
     }
@@ -53,7 +58,7 @@ __device__ __forceinline__ void load_piece(QuantRow<F32>& v, const void* base, l
   }
 #pragma unroll
   for (int d = 0; d < (F32 ? 8 : 4); ++d) v.w[d] = 0;
-  if (VEC) return;  // whole pieces only
+  if (WHOLE || left <= 0) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     if (e >= left) continue;
@@ -61,20 +66,20 @@ __device__ __forceinline__ void load_piece(QuantRow<F32>& v, const void* base, l
     else v.w[e >> 1] |= (unsigned)static_cast<const unsigned short*>(base)[at + e] << (16 * (e & 1));
   }
 }
-template <bool F32, bool VEC>
+template <bool F32, bool WHOLE>
 __device__ __forceinline__ void store_piece(const QuantRow<F32>& v, void* base, long at, int left) {
-  if (VEC && left >= 8) {
+  if (left >= 8) {
     if constexpr (F32) {
-      auto* dst = reinterpret_cast<u32x4_t*>(static_cast<float*>(base) + at);
+      auto* dst = reinterpret_cast<u32x4_any4*>(static_cast<float*>(base) + at);
       dst[0] = u32x4_t{v.w[0], v.w[1], v.w[2], v.w[3]};
       dst[1] = u32x4_t{v.w[4], v.w[5], v.w[6], v.w[7]};
     } else {
-      *reinterpret_cast<u32x4_t*>(static_cast<unsigned short*>(base) + at) =
+      *reinterpret_cast<u32x4_any2*>(static_cast<unsigned short*>(base) + at) =
           u32x4_t{v.w[0], v.w[1], v.w[2], v.w[3]};
     }
     return;
   }
-  if (VEC) return;
+  if (WHOLE || left <= 0) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     if (e >= left) continue;
@@ -110,7 +115,7 @@ enum AddNormOut { kNormBF16 = 0, kNormE8M0 = 1, kNormF32Scales = 2 };
 
 // WPR waves take a row (1: four rows per workgroup; 4: one), NC pieces per lane: d is at most
 // 512 NC WPR. ADD: there is a residual; without one s is x, and no stream is written.
-template <bool F32, bool ADD, int OUT, int NC, int WPR, bool VEC>
+template <bool F32, bool ADD, int OUT, int NC, int WPR, bool WHOLE>
 static __global__ void __launch_bounds__(256) add_rmsnorm_kernel(const AddNormParams p) {
   __shared__ float red[2][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -123,8 +128,8 @@ static __global__ void __launch_bounds__(256) add_rmsnorm_kernel(const AddNormPa
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = c0 + i * 512 * WPR;
-      load_piece<false, VEC>(x[i], p.x, (long)row * p.ldx + c, p.d - c);
-      if constexpr (ADD) load_piece<F32, VEC>(s[i], p.residual, (long)row * p.ldr + c, p.d - c);
+      load_piece<false, WHOLE>(x[i], p.x, (long)row * p.ldx + c, p.d - c);
+      if constexpr (ADD) load_piece<F32, WHOLE>(s[i], p.residual, (long)row * p.ldr + c, p.d - c);
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -133,7 +138,7 @@ static __global__ void __launch_bounds__(256) add_rmsnorm_kernel(const AddNormPa
       for (int e = 0; e < 8; ++e) f[e] = ADD ? x[i].at(e) + s[i].at(e) : x[i].at(e);
       s[i] = round_piece<F32>(f);
       const int c = c0 + i * 512 * WPR;
-      if constexpr (ADD) store_piece<F32, VEC>(s[i], p.stream, (long)row * p.d + c, p.d - c);
+      if constexpr (ADD) store_piece<F32, WHOLE>(s[i], p.stream, (long)row * p.d + c, p.d - c);
     }
   }
   float acc = 0.0f;
@@ -148,12 +153,12 @@ static __global__ void __launch_bounds__(256) add_rmsnorm_kernel(const AddNormPa
   for (int i = 0; i < NC; ++i) {
     const int c = c0 + i * 512 * WPR, left = p.d - c;
     QuantRow<true> w;
-    load_piece<true, VEC>(w, p.w, c, left);
+    load_piece<true, WHOLE>(w, p.w, c, left);
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = (s[i].at(e) * r) * w.at(e);
     if constexpr (OUT == kNormBF16) {
-      store_piece<false, VEC>(round_piece<false>(f), p.y, (long)row * p.d + c, left);
+      store_piece<false, WHOLE>(round_piece<false>(f), p.y, (long)row * p.d + c, left);
     } else {
       constexpr int SCALE = OUT == kNormE8M0 ? kScaleE8M0 : kScaleF32;
       unsigned m = 0;
@@ -188,7 +193,7 @@ struct AddNormGradParams {
 
 // Each lane keeps the weight and the weight gradient of its columns in registers over all rows of
 // its waves, so that the gradient's partial sums cost one row of FP32 per workgroup.
-template <bool F32, bool DS, int NC, int WPR, bool VEC>
+template <bool F32, bool DS, int NC, int WPR, bool WHOLE>
 static __global__ void __launch_bounds__(256) add_rmsnorm_bwd_kernel(const AddNormGradParams p) {
   __shared__ float red[2][4];
   __shared__ float sums[WPR == 1 ? 3 : 1][WPR == 1 ? 512 * NC : 1];
@@ -200,7 +205,7 @@ static __global__ void __launch_bounds__(256) add_rmsnorm_bwd_kernel(const AddNo
   for (int i = 0; i < NC; ++i) {
     const int c = c0 + i * 512 * WPR;
     QuantRow<true> v;
-    load_piece<true, VEC>(v, p.w, c, p.d - c);
+    load_piece<true, WHOLE>(v, p.w, c, p.d - c);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       w[i][e] = v.at(e);
@@ -214,9 +219,9 @@ static __global__ void __launch_bounds__(256) add_rmsnorm_bwd_kernel(const AddNo
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = c0 + i * 512 * WPR, left = p.d - c;
-      load_piece<F32, VEC>(s[i], p.s, (long)row * p.d + c, left);
-      load_piece<false, VEC>(dy[i], p.dy, (long)row * p.ld_dy + c, left);
-      if constexpr (DS) load_piece<F32, VEC>(ds[i], p.ds, (long)row * p.ld_ds + c, left);
+      load_piece<F32, WHOLE>(s[i], p.s, (long)row * p.d + c, left);
+      load_piece<false, WHOLE>(dy[i], p.dy, (long)row * p.ld_dy + c, left);
+      if constexpr (DS) load_piece<F32, WHOLE>(ds[i], p.ds, (long)row * p.ld_ds + c, left);
     }
     const float r = p.rstd[row];
     float dot = 0.0f;
@@ -238,9 +243,9 @@ static __global__ void __launch_bounds__(256) add_rmsnorm_bwd_kernel(const AddNo
         if constexpr (DS) f[e] += ds[i].at(e);
         dw[i][e] += ge * (se * r);
       }
-      store_piece<false, VEC>(round_piece<false>(f), p.dx, (long)row * p.d + c, left);
+      store_piece<false, WHOLE>(round_piece<false>(f), p.dx, (long)row * p.d + c, left);
       if constexpr (F32)
-        if (p.dresidual) store_piece<true, VEC>(round_piece<true>(f), p.dresidual, (long)row * p.d + c, left);
+        if (p.dresidual) store_piece<true, WHOLE>(round_piece<true>(f), p.dresidual, (long)row * p.d + c, left);
     }
   }
   // The waves' sums in wave order.
@@ -263,7 +268,7 @@ static __global__ void __launch_bounds__(256) add_rmsnorm_bwd_kernel(const AddNo
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = c0 + i * 512 * WPR;
-    store_piece<true, VEC>(round_piece<true>(dw[i]), p.partial, (long)blockIdx.x * p.d + c, p.d - c);
+    store_piece<true, WHOLE>(round_piece<true>(dw[i]), p.partial, (long)blockIdx.x * p.d + c, p.d - c);
   }
 }
 

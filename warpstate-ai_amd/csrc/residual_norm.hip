@@ -17,45 +17,40 @@ int check_shape(int64_t rows, int64_t d) {
   if (d > kMaxWidth) return set_error(kInvalid, "RMSNorm takes rows of at most %ld columns (got %ld)", kMaxWidth, (long)d);
   return kOk;
 }
-// Rows that 16-byte pieces read: whole pieces, aligned, over aligned strides.
-bool pieces(const void* p, long ld, int bytes) { return al(p, 16) && ld * bytes % 16 == 0; }
-
 // Few rows leave compute units idle at one wave a row: four waves take it then, and rows of more
 // than 2048 columns, whose pieces would not fit one wave's registers.
 int waves_per_row(int64_t rows, int64_t d) { return d > 2048 || rows <= 4L * device_cus() ? 4 : 1; }
 
-template <bool F32, bool ADD, int OUT, int NC, int WPR, bool VEC>
+template <bool F32, bool ADD, int OUT, int NC, int WPR, bool WHOLE>
 int launch_forward(AddNormParams p, hipStream_t s) {
-  hipLaunchKernelGGL((add_rmsnorm_kernel<F32, ADD, OUT, NC, WPR, VEC>), dim3(WPR == 1 ? cdiv(p.rows, 4) : p.rows),
+  hipLaunchKernelGGL((add_rmsnorm_kernel<F32, ADD, OUT, NC, WPR, WHOLE>), dim3(WPR == 1 ? cdiv(p.rows, 4) : p.rows),
                      dim3(256), 0, s, p);
   return hip_check(hipGetLastError(), "residual norm launch");
 }
-template <bool F32, bool ADD, int OUT, bool VEC>
+template <bool F32, bool ADD, int OUT, bool WHOLE>
 int run_forward(const AddNormParams& p, hipStream_t s) {
   if (waves_per_row(p.rows, p.d) == 4)
-    return p.d <= 2048 ? launch_forward<F32, ADD, OUT, 1, 4, VEC>(p, s)
-         : p.d <= 4096 ? launch_forward<F32, ADD, OUT, 2, 4, VEC>(p, s)
-                       : launch_forward<F32, ADD, OUT, 4, 4, VEC>(p, s);
-  return p.d <= 512    ? launch_forward<F32, ADD, OUT, 1, 1, VEC>(p, s)
-         : p.d <= 1024 ? launch_forward<F32, ADD, OUT, 2, 1, VEC>(p, s)
-                       : launch_forward<F32, ADD, OUT, 4, 1, VEC>(p, s);
+    return p.d <= 2048 ? launch_forward<F32, ADD, OUT, 1, 4, WHOLE>(p, s)
+         : p.d <= 4096 ? launch_forward<F32, ADD, OUT, 2, 4, WHOLE>(p, s)
+                       : launch_forward<F32, ADD, OUT, 4, 4, WHOLE>(p, s);
+  return p.d <= 512    ? launch_forward<F32, ADD, OUT, 1, 1, WHOLE>(p, s)
+         : p.d <= 1024 ? launch_forward<F32, ADD, OUT, 2, 1, WHOLE>(p, s)
+                       : launch_forward<F32, ADD, OUT, 4, 1, WHOLE>(p, s);
 }
 template <int OUT>
 int dispatch_forward(AddNormParams p, bool f32, hipStream_t s) {
   const int size = f32 ? 4 : 2;
   const bool add = p.residual != nullptr;
-  const bool vec = p.d % 8 == 0 && pieces(p.x, p.ldx, 2) && al(p.w, 16) &&
-                   (!add || (pieces(p.residual, p.ldr, size) && al(p.stream, 16))) &&
-                   (OUT != kNormBF16 || al(p.y, 16));
+  const bool whole = p.d % 8 == 0;
   for (int64_t left = p.rows; left > 0; left -= kLaunchRows) {
     p.rows = (int)(left < kLaunchRows ? left : kLaunchRows);
     int rc;
     if (OUT != kNormBF16 && !add)
-      rc = vec ? run_forward<false, OUT == kNormBF16, OUT, true>(p, s) : run_forward<false, OUT == kNormBF16, OUT, false>(p, s);
+      rc = whole ? run_forward<false, OUT == kNormBF16, OUT, true>(p, s) : run_forward<false, OUT == kNormBF16, OUT, false>(p, s);
     else if (f32)
-      rc = vec ? run_forward<true, true, OUT, true>(p, s) : run_forward<true, true, OUT, false>(p, s);
+      rc = whole ? run_forward<true, true, OUT, true>(p, s) : run_forward<true, true, OUT, false>(p, s);
     else
-      rc = vec ? run_forward<false, true, OUT, true>(p, s) : run_forward<false, true, OUT, false>(p, s);
+      rc = whole ? run_forward<false, true, OUT, true>(p, s) : run_forward<false, true, OUT, false>(p, s);
     if (rc) return rc;
     p.x += kLaunchRows * p.ldx;
     if (add) {
@@ -81,25 +76,25 @@ int backward_groups(int64_t rows, int64_t d) {
   return (int)(need < most ? need : most);
 }
 
-template <bool F32, bool DS, int NC, int WPR, bool VEC>
+template <bool F32, bool DS, int NC, int WPR, bool WHOLE>
 int launch_backward(const AddNormGradParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((add_rmsnorm_bwd_kernel<F32, DS, NC, WPR, VEC>), dim3(backward_groups(p.rows, p.d)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((add_rmsnorm_bwd_kernel<F32, DS, NC, WPR, WHOLE>), dim3(backward_groups(p.rows, p.d)), dim3(256), 0, s, p);
   return hip_check(hipGetLastError(), "residual norm backward launch");
 }
-template <bool F32, bool DS, bool VEC>
+template <bool F32, bool DS, bool WHOLE>
 int run_backward(const AddNormGradParams& p, hipStream_t s) {
   if (waves_per_row(p.rows, p.d) == 4)
-    return p.d <= 2048 ? launch_backward<F32, DS, 1, 4, VEC>(p, s)
-         : p.d <= 4096 ? launch_backward<F32, DS, 2, 4, VEC>(p, s)
-                       : launch_backward<F32, DS, 4, 4, VEC>(p, s);
-  return p.d <= 512    ? launch_backward<F32, DS, 1, 1, VEC>(p, s)
-         : p.d <= 1024 ? launch_backward<F32, DS, 2, 1, VEC>(p, s)
-                       : launch_backward<F32, DS, 4, 1, VEC>(p, s);
+    return p.d <= 2048 ? launch_backward<F32, DS, 1, 4, WHOLE>(p, s)
+         : p.d <= 4096 ? launch_backward<F32, DS, 2, 4, WHOLE>(p, s)
+                       : launch_backward<F32, DS, 4, 4, WHOLE>(p, s);
+  return p.d <= 512    ? launch_backward<F32, DS, 1, 1, WHOLE>(p, s)
+         : p.d <= 1024 ? launch_backward<F32, DS, 2, 1, WHOLE>(p, s)
+                       : launch_backward<F32, DS, 4, 1, WHOLE>(p, s);
 }
 template <bool F32>
-int dispatch_backward(const AddNormGradParams& p, bool vec, hipStream_t s) {
-  if (p.ds) return vec ? run_backward<F32, true, true>(p, s) : run_backward<F32, true, false>(p, s);
-  return vec ? run_backward<F32, false, true>(p, s) : run_backward<F32, false, false>(p, s);
+int dispatch_backward(const AddNormGradParams& p, bool whole, hipStream_t s) {
+  if (p.ds) return whole ? run_backward<F32, true, true>(p, s) : run_backward<F32, true, false>(p, s);
+  return whole ? run_backward<F32, false, true>(p, s) : run_backward<F32, false, false>(p, s);
 }
 
 }  // namespace
@@ -186,11 +181,9 @@ extern "C" int ws_add_rmsnorm_backward(const void* stream_in, int stream_f32, co
   p.dx = static_cast<unsigned short*>(dx);
   p.dresidual = dresidual;
   p.partial = partial;
-  const bool vec = d % 8 == 0 && al(stream_in, 16) && al(weight, 16) && pieces(dy, ld_dy, 2) &&
-                   (!dstream || pieces(dstream, ld_dstream, stream_f32 ? 4 : 2)) && al(dx, 16) &&
-                   al(dresidual, 16) && al(partial, 16);
+  const bool whole = d % 8 == 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (int rc = stream_f32 ? dispatch_backward<true>(p, vec, s) : dispatch_backward<false>(p, vec, s)) return rc;
+  if (int rc = stream_f32 ? dispatch_backward<true>(p, whole, s) : dispatch_backward<false>(p, whole, s)) return rc;
   const int groups = backward_groups(rows, d);
   const bool vec_reduce = d % 4 == 0 && al(partial, 16);
   hipLaunchKernelGGL(vec_reduce ? rms_weight_reduce_kernel<true> : rms_weight_reduce_kernel<false>,
