@@ -543,6 +543,13 @@ int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int64_t ld_wei
 int ws_grouped_weight_grad(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
                            const int64_t* offsets, int64_t groups, int64_t rows, int64_t n,
                            int64_t k, void* dweight, int dweight_f32, void* stream);
+/* Matrices of any width as these products take them, and back: for each group, rows [rows_in, cols_in]
+ * into rows [rows_out, cols_out] with zeros past the input's last row and column, rows and columns past
+ * the output's left out. BF16 or FP32, in the input's type or rounded from FP32 to BF16; any alignment
+ * of the types. Up to 2^26 rows of all groups. */
+int ws_copy_rows(const void* in, int in_f32, int64_t group_in, int64_t ld_in, int64_t rows_in,
+                 int64_t cols_in, void* out, int out_f32, int64_t group_out, int64_t ld_out,
+                 int64_t rows_out, int64_t cols_out, int64_t groups, void* stream);
 /* What these sizes run on, without a launch (WS_GROUPED_GRAD: the weight gradient): 0 256 x 256,
  * 1 and 2 128 x 128 (two or one workgroup on a compute unit), 3 64 x 128, 4 64 x 64, 5 the kernel
  * for few rows; -1 for invalid sizes. */

@@ -121,3 +121,15 @@ def test_grouped_tile_of_bad_sizes():
     assert _hip.query("ws_grouped_tile", 8, 0, 8, 8, 0) == -1
     assert _hip.query("ws_grouped_tile", 8, 1, 12, 8, 0) == -1
     assert _hip.query("ws_grouped_tile", 8, 1, 8, 8, 3) == -1
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(groups=-1), "sizes"), (dict(rows_in=-1), "sizes"), (dict(cols_out=2 ** 31), "sizes"),
+    (dict(groups=2 ** 25), "sizes"), (dict(x=None), "null"), (dict(out=None), "null"), (dict(ld_out=4), "overlap"),
+    (dict(group_out=20), "overlap"), (dict(out_f32=1), "type")])
+def test_copy_rows_arguments(change, match):
+    a = dict(x=GPU, in_f32=0, group_in=40, ld_in=8, rows_in=5, cols_in=8, out=GPU, out_f32=0, group_out=30, ld_out=6,
+             rows_out=5, cols_out=6, groups=2) | change
+    with pytest.raises(RuntimeError, match=match):
+        _hip.call("ws_copy_rows", a["x"], a["in_f32"], a["group_in"], a["ld_in"], a["rows_in"], a["cols_in"], a["out"],
+                  a["out_f32"], a["group_out"], a["ld_out"], a["rows_out"], a["cols_out"], a["groups"], None)

@@ -17,6 +17,7 @@
 #pragma once
 
 #include "gemm_ring.h"
+#include "residual_norm.h"
 
 namespace ws {
 
@@ -402,6 +403,34 @@ static __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedPa
     v2[e] = (sums[0][m][n + e] + sums[1][m][n + e]) + (sums[2][m][n + e] + sums[3][m][n + e]);
   if (row0 + m < t.hi && col0 + n < p.N)  // N is a multiple of 8
     *reinterpret_cast<unsigned*>(p.c + (long)(row0 + m) * p.ldc + col0 + n) = pack_bf16x2(v2[0], v2[1]);
+}
+
+// --------------------------------------------------------------------------------------
+// Matrices of any width as the products read them, and back: rows [rows_in, cols_in] of each group into
+// rows [rows_out, cols_out], what lies past the input written as zeros and what lies past the output
+// left out. Element (g, r, c) at g * group + r * ld + c on either side.
+struct CopyRowsParams {
+  const void* in; long group_in, ld_in; int rows_in, cols_in;
+  void* out; long group_out, ld_out; int rows_out, cols_out;
+  long rows;  // of all groups' output
+};
+
+template <bool IN32, bool OUT32>
+static __global__ void __launch_bounds__(256) copy_rows_kernel(const CopyRowsParams p) {
+  const int lane = threadIdx.x & 63;
+  const long row = blockIdx.x * 4L + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= p.rows) return;
+  const long g = row / p.rows_out;
+  const int r = (int)(row - g * p.rows_out), cols = r < p.rows_in ? p.cols_in : 0;
+#pragma unroll 4
+  for (int c = 8 * lane; c < p.cols_out; c += 512) {
+    QuantRow<IN32> v;
+    load_piece<IN32, false>(v, p.in, g * p.group_in + r * p.ld_in + c, cols - c);
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = v.at(e);
+    store_piece<OUT32, false>(round_piece<OUT32>(f), p.out, g * p.group_out + r * p.ld_out + c, p.cols_out - c);
+  }
 }
 
 }  // namespace ws

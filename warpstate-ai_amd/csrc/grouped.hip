@@ -223,3 +223,24 @@ extern "C" int ws_grouped_weight_grad(const void* dy, int64_t ld_dy, const void*
   };
   return f32 ? run(&grouped_grad_fast_kernel<true>) : run(&grouped_grad_fast_kernel<false>);
 }
+
+extern "C" int ws_copy_rows(const void* in, int in_f32, int64_t group_in, int64_t ld_in, int64_t rows_in, int64_t cols_in,
+                            void* out, int out_f32, int64_t group_out, int64_t ld_out, int64_t rows_out, int64_t cols_out,
+                            int64_t groups, void* stream) {
+  if (groups < 0 || rows_in < 0 || rows_out < 0 || cols_in < 0 || cols_out < 0 || !fits_i32(rows_in) ||
+      !fits_i32(rows_out) || !fits_i32(cols_in + 512) || !fits_i32(cols_out + 512) ||
+      (rows_out > 0 && groups > (1L << 26) / rows_out))
+    return set_error(kInvalid, "invalid sizes of copied rows");
+  if (groups == 0 || rows_out == 0 || cols_out == 0) return kOk;
+  if (!out || (!in && rows_in > 0 && cols_in > 0)) return set_error(kInvalid, "null pointer");
+  if (!in_f32 && out_f32) return set_error(kInvalid, "rows are copied in their type or rounded to BF16");
+  if ((rows_out > 1 && ld_out < cols_out) || (groups > 1 && group_out < ld_out * (rows_out - 1) + cols_out))
+    return set_error(kInvalid, "rows overlap");
+  CopyRowsParams p{in, group_in, ld_in, (int)rows_in, (int)cols_in, out, group_out, ld_out, (int)rows_out, (int)cols_out, groups * rows_out};
+  auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(p.rows, 4)), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+    return hip_check(hipGetLastError(), "row copy launch");
+  };
+  return in_f32 ? (out_f32 ? run(&copy_rows_kernel<true, true>) : run(&copy_rows_kernel<true, false>))
+                : run(&copy_rows_kernel<false, false>);
+}

@@ -323,16 +323,36 @@ bool whole_rows(const Tensor& t) {
   }
   return true;
 }
+typedef Tensor CopyRows(const Tensor&, c10::SymInt, c10::SymInt, bool);
+const auto& copy_rows_op() {
+  static const auto op = find<CopyRows>("warpstate::native_copy_rows");
+  return op;
+}
 Tensor grouped_operand(const Tensor& t) {
-  const Tensor b = t.to(at::kBFloat16);
-  if (whole_rows(b) && (t.dim() == 2 || fixed(t, 1) % 8 == 0)) return b;
-  c10::SymDimVector sizes(b.sym_sizes());
-  for (int64_t i = 1; i < b.dim(); ++i) sizes[i] = up(fixed(b, i), 8);
-  Tensor out = at::zeros_symint(sizes, b.options());
-  Tensor part = out.narrow(-1, 0, fixed(b, -1));
-  if (t.dim() == 3) part = part.narrow(1, 0, fixed(b, 1));
-  part.copy_(b);
+  if (whole_rows(t) && (t.dim() == 2 || fixed(t, 1) % 8 == 0)) return t.to(at::kBFloat16);
+  return copy_rows_op().call(t, t.dim() == 2 ? t.sym_size(0) : c10::SymInt(up(fixed(t, 1), 8)), up(fixed(t, -1), 8), true);
+}
+// t [rows, cols] or [groups, rows, cols] in other sizes, padded with zeros or cut off: a new tensor, in
+// BF16 or in t's type.
+Tensor copy_rows(const Tensor& t_in, int64_t rows, int64_t cols, bool bf16) {
+  c10::DeviceGuard guard(t_in.device());
+  const bool f32 = t_in.scalar_type() == at::kFloat;
+  const int64_t d = t_in.dim();
+  // (Expanded and overlapping rows can be read; other column strides are copied first.)
+  const Tensor t = t_in.stride(d - 1) == 1 || t_in.size(d - 1) == 1 ? t_in : t_in.contiguous();
+  const int64_t groups = d == 2 ? 1 : t.size(0), rows_in = t.size(d - 2), cols_in = t.size(d - 1);
+  std::vector<int64_t> sizes{rows, cols};
+  if (d == 3) sizes.insert(sizes.begin(), groups);
+  Tensor out = at::empty(sizes, t.options().dtype(bf16 ? at::kBFloat16 : t.scalar_type()));
+  check(ws_copy_rows(ptr(t), f32, d == 2 ? 0 : t.stride(0), t.stride(d - 2), rows_in, cols_in, ptr(out), f32 && !bf16,
+                     rows * cols, cols, rows, cols, groups, stream_of(t)),
+        "ws_copy_rows");
   return out;
+}
+Tensor copy_rows_meta(const Tensor& t, c10::SymInt rows, c10::SymInt cols, bool bf16) {
+  const auto options = t.options().dtype(bf16 ? at::kBFloat16 : t.scalar_type());
+  if (t.dim() == 2) return at::empty_symint({rows, cols}, options);
+  return at::empty_symint({t.sym_size(0), rows, cols}, options);
 }
 
 // On operands of grouped_operand: [rows, n] (form NT) or [rows, k] (NN), padded widths.
@@ -360,13 +380,14 @@ Tensor grouped_grad(const Tensor& dy, const Tensor& x, const Tensor& offsets_in,
 }
 typedef Tensor GroupedRows(const Tensor&, const Tensor&, const Tensor&, int64_t);
 typedef Tensor GroupedGrad(const Tensor&, const Tensor&, const Tensor&, bool);
+// Below autograd.
 Tensor first_columns(const Tensor& t, int64_t cols) {
-  return fixed(t, -1) == cols ? t : t.narrow(-1, 0, cols).contiguous();
+  return fixed(t, -1) == cols ? t : copy_rows_op().call(t, t.sym_size(0), cols, false);
 }
 
 Tensor grouped_mm(const Tensor& x, const Tensor& weight, const Tensor& offsets) {
   check_grouped(x, weight, offsets);
-  c10::DeviceGuard guard(x.device());
+  at::AutoDispatchBelowAutograd below_autograd;
   return first_columns(grouped_rows(grouped_operand(x), grouped_operand(weight), offsets, WS_GROUPED_NT),
                        weight.size(1));
 }
@@ -400,7 +421,7 @@ struct GroupedMmFn : Function<GroupedMmFn> {
       if (ctx->saved_data["want_x"].toBool()) d[0] = first_columns(rows_op.call(g, s[1], s[2], WS_GROUPED_NN), k);
       if (ctx->saved_data["want_w"].toBool()) {
         Tensor dw = grad_op.call(g, s[0], s[2], ctx->saved_data["f32"].toBool());
-        if (fixed(dw, 1) != n || fixed(dw, 2) != k) dw = dw.narrow(1, 0, n).narrow(2, 0, k).contiguous();
+        if (fixed(dw, 1) != n || fixed(dw, 2) != k) dw = copy_rows_op().call(dw, n, k, false);
         d[1] = dw;
       }
     }
@@ -449,6 +470,7 @@ TORCH_LIBRARY_FRAGMENT(warpstate, m) {
   m.def("native_embedding_backward(Tensor dy, Tensor tokens, SymInt vocab, float scale, bool f32) -> Tensor");
   m.def("native_embedding_accumulate_(Tensor(a!) gradient, Tensor tokens, Tensor dy, float scale) -> ()");
   m.def("native_grouped_mm(Tensor x, Tensor weight, Tensor offsets) -> Tensor");
+  m.def("native_copy_rows(Tensor t, SymInt rows, SymInt cols, bool bf16) -> Tensor");
   m.def("native_grouped_rows(Tensor x, Tensor w, Tensor offsets, int form) -> Tensor");
   m.def("native_grouped_grad(Tensor dy, Tensor x, Tensor offsets, bool f32) -> Tensor");
 }
@@ -461,6 +483,7 @@ TORCH_LIBRARY_IMPL(warpstate, CUDA, m) {
   m.impl("native_embedding_backward", &embedding_backward);
   m.impl("native_embedding_accumulate_", &embedding_accumulate);
   m.impl("native_grouped_mm", &grouped_mm);
+  m.impl("native_copy_rows", &copy_rows);
   m.impl("native_grouped_rows", &grouped_rows);
   m.impl("native_grouped_grad", &grouped_grad);
 }
@@ -478,6 +501,7 @@ TORCH_LIBRARY_IMPL(warpstate, Meta, m) {
   m.impl("native_embedding", &embedding_meta);
   m.impl("native_embedding_backward", &embedding_backward_meta);
   m.impl("native_grouped_mm", &grouped_mm_meta);
+  m.impl("native_copy_rows", &copy_rows_meta);
   m.impl("native_grouped_rows", &grouped_rows_meta);
   m.impl("native_grouped_grad", &grouped_grad_meta);
 }

@@ -122,6 +122,7 @@ SIGNATURES = {
                              _i64, _i64, _c_void_p, _i64, _c_void_p]),
     "ws_grouped_weight_grad": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64,
                                       _i64, _i64, _c_void_p, _i32, _c_void_p]),
+    "ws_copy_rows": (_i32, [_c_void_p, _i32] + [_i64] * 4 + [_c_void_p, _i32] + [_i64] * 5 + [_c_void_p]),
     "ws_grouped_tile": (_i32, [_i64, _i64, _i64, _i64, _i32]),
 }
 

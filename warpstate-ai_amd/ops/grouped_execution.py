@@ -52,16 +52,25 @@ def _whole_rows(t: Tensor) -> bool:
     return True
 
 
+def _copy_rows(t: Tensor, rows: int, cols: int, dtype: torch.dtype) -> Tensor:
+    """t [rows, cols] or [groups, rows, cols] in other sizes, padded with zeros or cut off."""
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        t = t.contiguous()
+    groups = t.shape[0] if t.ndim == 3 else 1
+    out = torch.empty((*t.shape[:-2], rows, cols), dtype=dtype, device=t.device)
+    _hip.call_on(t, "ws_copy_rows", t.data_ptr(), int(t.dtype == F32),
+                 t.stride(0) if t.ndim == 3 else 0, t.stride(-2), t.shape[-2], t.shape[-1],
+                 out.data_ptr(), int(dtype == F32), rows * cols, cols, rows, cols, groups)
+    return out
+
+
 def _operand(t: Tensor) -> Tensor:
     """A BF16 operand with 16-byte rows of a multiple of 8, and weights with a multiple of 8 of
     them: t itself or a copy, padded with zeros."""
-    t = t.to(BF16)
     if _whole_rows(t) and (t.ndim == 2 or t.shape[1] % 8 == 0):
-        return t
-    out = torch.zeros((t.shape[0], *(-(-n // 8) * 8 for n in t.shape[1:])), dtype=BF16,
-                      device=t.device)
-    out[tuple(slice(n) for n in t.shape)].copy_(t)
-    return out
+        return t.to(BF16)
+    rows = t.shape[0] if t.ndim == 2 else -(-t.shape[1] // 8) * 8
+    return _copy_rows(t, rows, -(-t.shape[-1] // 8) * 8, BF16)
 
 
 def _product(x: Tensor, w: Tensor, offsets: Tensor, form: int) -> Tensor:
@@ -80,7 +89,7 @@ def _first(t: Tensor, *sizes: int) -> Tensor:
     """The first of t's padded columns (and weight rows)."""
     if t.shape[-len(sizes):] == sizes:
         return t
-    return t[(..., *(slice(n) for n in sizes))].contiguous()
+    return _copy_rows(t, t.shape[0] if len(sizes) == 1 else sizes[0], sizes[-1], t.dtype)
 
 
 class _GroupedMm(torch.autograd.Function):
