@@ -482,23 +482,23 @@ int ws_linear_token_scores_backward(const void* hidden, int64_t ld_hidden, const
  * the weight FP32; up to 2^30 rows of 1 to 8192 columns, row strides in elements, outputs contiguous.
  */
 
-/* y [rows, d] BF16, stream_out [rows, d] = s, rstd [rows]. */
+/* y [rows, d] BF16, stream_out [rows, d] = s. */
 int ws_add_rmsnorm(const void* x, int64_t ldx, const void* residual, int64_t ld_residual,
                    int stream_f32, const float* weight, float eps, int64_t rows, int64_t d, void* y,
-                   void* stream_out, float* rstd, void* stream);
+                   void* stream_out, void* stream);
 /* The unrounded y quantized by rows (WS_QUANT_ROWS of ws_fp8_quantize): q, ldq, scale and
  * ld_scale as there. With a null residual s is x and stream_out is null. */
 int ws_rmsnorm_quantize(const void* x, int64_t ldx, const void* residual, int64_t ld_residual,
                         int stream_f32, const float* weight, float eps, int64_t rows, int64_t d,
                         int scale_type, void* q, int64_t ldq, void* scale, int64_t ld_scale,
                         void* stream_out, void* stream);
-/* With stream_in [rows, d] = s and the forward's rstd, dy BF16 and dstream (nullable: zero) in the
+/* With stream_in [rows, d] = s and the forward's eps, dy BF16 and dstream (nullable: zero) in the
  * stream's type: dx [rows, d] BF16, the gradient of x and of a BF16 residual; dresidual (nullable)
  * the same in FP32 for an FP32 stream; dweight [d]. `partial`: ws_add_rmsnorm_backward_partial_floats
- * (which follows the device's compute units). */
+ * (which follows the device's compute units; null if that is 0). */
 int64_t ws_add_rmsnorm_backward_partial_floats(int64_t rows, int64_t d);
 int ws_add_rmsnorm_backward(const void* stream_in, int stream_f32, const float* weight,
-                            const float* rstd, const void* dy, int64_t ld_dy, const void* dstream,
+                            float eps, const void* dy, int64_t ld_dy, const void* dstream,
                             int64_t ld_dstream, int64_t rows, int64_t d, void* dx, float* dresidual,
                             float* dweight, float* partial, void* stream);
 
@@ -514,7 +514,8 @@ int ws_embedding(const void* table, int64_t ld_table, int table_f32, const int64
 /* dtable [vocab, d] = scale * the sums of dy's rows (BF16, or FP32 with dy_f32) by token, FP32 in
  * the order of the rows: the same bits on every call. Written in BF16 or FP32, or added to FP32
  * values that are there (rows without tokens then stay as they are, unread). Tokens outside the
- * vocabulary, ignored ones among them, take no part. `workspace`: 16-byte aligned. */
+ * vocabulary, ignored ones among them, take no part. `workspace`: 16-byte aligned,
+ * ws_embedding_backward_workspace_bytes (null if that is 0). */
 enum WsEmbedGrad { WS_EMBED_WRITE_BF16 = 0, WS_EMBED_WRITE_F32 = 1, WS_EMBED_ADD_F32 = 2 };
 int64_t ws_embedding_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d);
 int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, const int64_t* tokens,
@@ -526,12 +527,15 @@ int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, const int64
  * Rows sorted by expert: rows offsets[e] to offsets[e + 1] of x belong to group e (offsets: groups + 1
  * int64 on the device, not decreasing). The offsets are read on the device only, and no value of theirs
  * leads an access out of the operands; decreasing ones leave rows of the result unspecified. BF16
- * operands, FP32 sums, 16-byte aligned rows, widths of a multiple of 8, 1 to 65536 groups, up to 2^30 rows.
+ * operands, FP32 sums, 16-byte aligned rows, weight rows of a multiple of 8 elements, 1 to 65536
+ * groups, up to 2^30 rows. The other width, n below, may be any; rows of that width reach to its
+ * next multiple of 8: y's are written up to there, and dy's, like x's under WS_GROUPED_NN, have
+ * to hold zeros.
  */
 
 /* y [rows, n] BF16 = x [rows, k] times the transpose of the group's weight [n, k] (WS_GROUPED_NT:
- * a projection), or times its weight [k, n] itself (WS_GROUPED_NN: the input gradient of one), both
- * row-major with row stride ld_weight, group_stride elements from one group's to the next. Rows
+ * a projection; k a multiple of 8), or times its weight [k, n] itself (WS_GROUPED_NN: the input
+ * gradient of one; n a multiple of 8), both row-major with row stride ld_weight, group_stride elements from one group's to the next. Rows
  * before the first offset and behind the last get zeros. The sums of the tiles have
  * one order, that of the kernel for few rows another. */
 enum WsGroupedForm { WS_GROUPED_NT = 0, WS_GROUPED_NN = 1, WS_GROUPED_GRAD = 2 };

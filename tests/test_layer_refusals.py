@@ -23,13 +23,13 @@ def test_cpu_tensors_are_refused():
 @pytest.mark.parametrize("change,match", [
     (dict(rows=-1), "shape"), (dict(d=0), "shape"), (dict(d=8193), "8192"), (dict(x=None), "null"),
     (dict(residual=None), "null"), (dict(w=None), "null"), (dict(y=None), "null"),
-    (dict(out=None), "null"), (dict(rstd=None), "null"), (dict(ldx=7), "overlap"),
+    (dict(out=None), "null"), (dict(ldx=7), "overlap"),
     (dict(ldr=7), "overlap"), (dict(rows=2 ** 30 + 1), "shape")])
 def test_add_rmsnorm_arguments(change, match):
-    a = dict(x=GPU, ldx=8, residual=GPU, ldr=8, w=GPU, rows=4, d=8, y=GPU, out=GPU, rstd=GPU) | change
+    a = dict(x=GPU, ldx=8, residual=GPU, ldr=8, w=GPU, rows=4, d=8, y=GPU, out=GPU) | change
     with pytest.raises(RuntimeError, match=match):
         _hip.call("ws_add_rmsnorm", a["x"], a["ldx"], a["residual"], a["ldr"], 0, a["w"], 1e-5, a["rows"],
-                  a["d"], a["y"], a["out"], a["rstd"], None)
+                  a["d"], a["y"], a["out"], None)
 
 
 @pytest.mark.parametrize("change,match", [
@@ -49,13 +49,13 @@ def test_rmsnorm_quantize_arguments(change, match):
 
 @pytest.mark.parametrize("change,match", [
     (dict(rows=0), "shape"), (dict(d=8193), "8192"), (dict(s=None), "null"), (dict(dy=None), "null"),
-    (dict(partial=None), "null"), (dict(dresidual=GPU), "BF16 stream"), (dict(ld_dy=7), "overlap"),
+    (dict(partial=None, rows=40), "null"), (dict(dresidual=GPU), "BF16 stream"), (dict(ld_dy=7), "overlap"),
     (dict(ds=GPU, ld_ds=7), "overlap")])
 def test_add_rmsnorm_backward_arguments(change, match):
-    a = dict(s=GPU, w=GPU, rstd=GPU, dy=GPU, ld_dy=8, ds=None, ld_ds=0, rows=4, d=8, dx=GPU,
+    a = dict(s=GPU, w=GPU, dy=GPU, ld_dy=8, ds=None, ld_ds=0, rows=4, d=8, dx=GPU,
              dresidual=None, dw=GPU, partial=GPU) | change
     with pytest.raises(RuntimeError, match=match):
-        _hip.call("ws_add_rmsnorm_backward", a["s"], 0, a["w"], a["rstd"], a["dy"], a["ld_dy"], a["ds"],
+        _hip.call("ws_add_rmsnorm_backward", a["s"], 0, a["w"], 1e-5, a["dy"], a["ld_dy"], a["ds"],
                   a["ld_ds"], a["rows"], a["d"], a["dx"], a["dresidual"], a["dw"], a["partial"], None)
 
 
@@ -80,7 +80,7 @@ def test_embedding_arguments(change, match):
 @pytest.mark.parametrize("change,match", [
     (dict(rows=-1), "shape"), (dict(vocab=0), "shape"), (dict(mode=3), "mode"), (dict(mode=-1), "mode"),
     (dict(dy=None), "null"), (dict(tokens=None), "null"), (dict(out=None), "null"),
-    (dict(work=None), "null"), (dict(work=GPU + 4), "aligned"), (dict(ld_dy=7), "overlap"),
+    (dict(work=None, rows=65), "null"), (dict(work=GPU + 4), "aligned"), (dict(ld_dy=7), "overlap"),
     (dict(ld=7), "overlap")])
 def test_embedding_backward_arguments(change, match):
     a = dict(dy=GPU, ld_dy=8, tokens=GPU, rows=4, vocab=10, d=8, out=GPU, ld=8, mode=0, work=GPU) | change
@@ -91,8 +91,8 @@ def test_embedding_backward_arguments(change, match):
 
 @pytest.mark.parametrize("change,match", [
     (dict(form=2), "form"), (dict(groups=0), "groups"), (dict(groups=65537), "groups"), (dict(rows=-1), "shape"),
-    (dict(n=12), "multiple of 8"), (dict(k=12), "multiple of 8"), (dict(n=0), "shape"), (dict(x=None), "null"),
-    (dict(w=None), "null"), (dict(offsets=None), "null"), (dict(y=None), "null"), (dict(x=GPU + 8), "aligned"),
+    (dict(form=1, n=12), "multiple of 8"), (dict(k=12), "multiple of 8"), (dict(n=0), "shape"), (dict(x=None), "null"),
+    (dict(n=17), "overlap"), (dict(form=1, k=17), "overlap"), (dict(w=None), "null"), (dict(offsets=None), "null"), (dict(y=None), "null"), (dict(x=GPU + 8), "aligned"),
     (dict(ldx=20), "aligned"), (dict(ldx=8), "overlap"), (dict(ldw=8), "overlap"), (dict(ldy=8), "overlap"),
     (dict(stride=12), "aligned"), (dict(stride=-8), "aligned"), (dict(ldy=4200000), "stride"),
     (dict(rows=2 ** 30, n=2 ** 20, ldy=2 ** 20), "tiles"), (dict(rows=2 ** 30 + 1), "shape")])
@@ -105,7 +105,8 @@ def test_grouped_mm_arguments(change, match):
 
 
 @pytest.mark.parametrize("change,match", [
-    (dict(groups=0), "groups"), (dict(rows=-1), "shape"), (dict(n=12), "multiple of 8"), (dict(dy=None), "null"),
+    (dict(groups=0), "groups"), (dict(rows=-1), "shape"), (dict(k=12), "multiple of 8"), (dict(dy=None), "null"),
+    (dict(n=17), "overlap"),
     (dict(x=None), "null"), (dict(offsets=None), "null"), (dict(dw=None), "null"), (dict(dw=GPU + 8), "aligned"),
     (dict(dy=GPU + 2), "aligned"), (dict(ldx=8), "overlap"), (dict(k=2200000, ldx=2200000), "stride"),
     (dict(groups=65536, n=4096, k=4096, ld_dy=4096, ldx=4096), "tiles")])
@@ -119,7 +120,7 @@ def test_grouped_weight_grad_arguments(change, match):
 def test_grouped_tile_of_bad_sizes():
     assert _hip.query("ws_grouped_tile", 0, 1, 8, 8, 0) == -1
     assert _hip.query("ws_grouped_tile", 8, 0, 8, 8, 0) == -1
-    assert _hip.query("ws_grouped_tile", 8, 1, 12, 8, 0) == -1
+    assert _hip.query("ws_grouped_tile", 8, 1, 0, 8, 0) == -1
     assert _hip.query("ws_grouped_tile", 8, 1, 8, 8, 3) == -1
 
 

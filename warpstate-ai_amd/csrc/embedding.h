@@ -128,7 +128,7 @@ static __global__ void __launch_bounds__(64 * kSortWaves) embed_sort_kernel(cons
 
 struct EmbedGradParams {
   const void* dy; long ld_dy;
-  const long* tokens;
+  const long* tokens; int rows;
   const int* start;
   const int* perm;
   int vocab, d;
@@ -329,6 +329,55 @@ static __global__ void __launch_bounds__(256) embed_grad_kernel(const EmbedGradP
                                   while (at >= __builtin_amdgcn_readlane(begins, r + 1)) store();
                                 });
       while (r < to || (r == to && r < rows)) store();  // the rest of the run, and the token after it
+    }
+  }
+}
+
+// At most 64 tokens need no sorting: every wave holds them all, one on a lane, and a row of the table
+// takes the lanes with its token in their order.
+constexpr int kFewTokens = 64;
+
+template <bool GF32, int OUT, bool WHOLE>
+static __global__ void __launch_bounds__(256) embed_few_kernel(const EmbedGradParams p) {
+  constexpr int W = OUT == kEmbedBF16 ? 8 : 4, NC = 32 / W, kSpan = 64 * W;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long v0 = (blockIdx.x * 4L + wave) * p.group;
+  if (v0 >= p.vocab) return;
+  const int rows = (int)min((long)p.group, p.vocab - v0);
+  const long token = lane < p.rows ? p.tokens[lane] : -1;
+  for (int c0 = 0; c0 < p.d; c0 += kSpan * NC) {
+    const int c = c0 + W * lane;
+    for (int r = 0; r < rows; ++r) {
+      unsigned long todo = __builtin_amdgcn_ballot_w64(token == v0 + r);
+      if (OUT == kEmbedAdd && todo == 0) continue;
+      float acc[NC][W];
+      embed_clear(acc);
+      while (todo != 0) {
+        constexpr int kAhead = 2;
+        EmbedPiece<GF32, W> v[kAhead][NC];
+        int n = 0;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          // (Past the last one some row is read, and not added.)
+          const long row = todo != 0 ? __builtin_ctzl(todo) : 0;
+          if (todo != 0) ++n;
+          todo &= todo - 1;
+#pragma unroll
+          for (int i = 0; i < NC; ++i)
+            v[a][i] = embed_load<GF32, W, WHOLE>(p.dy, row * p.ld_dy + c + kSpan * i, p.d - c - kSpan * i);
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          if (a >= n) break;
+#pragma unroll
+          for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int e = 0; e < W; ++e) acc[i][e] += v[a][i].at(e);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (c + kSpan * i < p.d) embed_store<OUT, W, WHOLE, false>(p, v0 + r, c + kSpan * i, acc[i]);
     }
   }
 }

@@ -23,6 +23,7 @@ struct GradLayout {
   int64_t piece, pieces, start, perm, partial, bytes, ld_partial;
 };
 GradLayout grad_layout(int64_t rows, int64_t vocab, int64_t d) {
+  if (rows <= kFewTokens) return GradLayout{};
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
   GradLayout l;
   l.piece = piece_rows(rows);
@@ -38,6 +39,14 @@ GradLayout grad_layout(int64_t rows, int64_t vocab, int64_t d) {
 // A gradient that the memory-side cache does not hold beside its input goes around it: 16384 rows into
 // 32768 x 2048 FP32 (268 MB), all kernels, 94 -> 70 us; BF16 (134 MB) 65 -> 67.
 bool past_caches(int64_t bytes) { return bytes > 256L << 20; }
+
+template <bool GF32, int OUT>
+int launch_few(const EmbedGradParams& p, bool whole, hipStream_t s) {
+  const dim3 grid((unsigned)cdiv(cdiv(p.vocab, p.group), 4)), block(256);
+  if (whole) hipLaunchKernelGGL((embed_few_kernel<GF32, OUT, true>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((embed_few_kernel<GF32, OUT, false>), grid, block, 0, s, p);
+  return hip_check(hipGetLastError(), "embedding gradient launch");
+}
 
 template <bool GF32, int OUT>
 int launch_grad(const EmbedGradParams& p, int64_t rows, bool whole, hipStream_t s) {
@@ -87,7 +96,8 @@ extern "C" int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, 
                                      int mode, void* workspace, void* stream) {
   if (int rc = check_table(rows, vocab, d, ld_dtable)) return rc;
   if (mode < WS_EMBED_WRITE_BF16 || mode > WS_EMBED_ADD_F32) return set_error(kInvalid, "unknown gradient mode %d", mode);
-  if (!dtable || !workspace || (rows > 0 && (!dy || !tokens))) return set_error(kInvalid, "null pointer");
+  const bool few = rows <= kFewTokens;
+  if (!dtable || (!workspace && !few) || (rows > 0 && (!dy || !tokens))) return set_error(kInvalid, "null pointer");
   if (rows > 1 && ld_dy < d) return set_error(kInvalid, "rows overlap");
   if (!al(workspace, 16)) return set_error(kInvalid, "the workspace must be 16-byte aligned");
   const GradLayout l = grad_layout(rows, vocab, d);
@@ -96,6 +106,7 @@ extern "C" int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, 
   p.dy = dy;
   p.ld_dy = ld_dy;
   p.tokens = reinterpret_cast<const long*>(tokens);
+  p.rows = (int)rows;
   p.start = reinterpret_cast<int*>(work + l.start);
   p.perm = reinterpret_cast<int*>(work + l.perm);
   p.vocab = (int)vocab;
@@ -112,17 +123,21 @@ extern "C" int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, 
   p.partial = reinterpret_cast<float*>(work + l.partial);
   p.ld_partial = l.ld_partial;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool whole = d % 8 == 0;
+#define WS_GRAD(RUN_, ...)                                                                                       \
+  (dy_f32 ? (mode == WS_EMBED_WRITE_BF16  ? RUN_<true, kEmbedBF16>(__VA_ARGS__)                                  \
+             : mode == WS_EMBED_WRITE_F32 ? RUN_<true, kEmbedF32>(__VA_ARGS__)                                   \
+                                          : RUN_<true, kEmbedAdd>(__VA_ARGS__))                                  \
+          : (mode == WS_EMBED_WRITE_BF16  ? RUN_<false, kEmbedBF16>(__VA_ARGS__)                                 \
+             : mode == WS_EMBED_WRITE_F32 ? RUN_<false, kEmbedF32>(__VA_ARGS__)                                  \
+                                          : RUN_<false, kEmbedAdd>(__VA_ARGS__)))
+  if (few) return WS_GRAD(launch_few, p, whole, s);
   // A workgroup per compute unit, more where their ranges would pass the counters' space.
   int64_t range = cdiv(vocab, device_cus());
   if (range > kSortRange) range = kSortRange;
   hipLaunchKernelGGL(embed_sort_kernel, dim3(cdiv(vocab, range)), dim3(64 * kSortWaves), 0, s, p.tokens, (int)rows,
                      (int)vocab, (int)range, const_cast<int*>(p.start), const_cast<int*>(p.perm));
   if (int rc = hip_check(hipGetLastError(), "embedding sort launch")) return rc;
-  const bool whole = d % 8 == 0;
-#define WS_GRAD(G_)                                                                                   \
-  (mode == WS_EMBED_WRITE_BF16  ? launch_grad<G_, kEmbedBF16>(p, rows, whole, s)                              \
-   : mode == WS_EMBED_WRITE_F32 ? launch_grad<G_, kEmbedF32>(p, rows, whole, s)                               \
-                                : launch_grad<G_, kEmbedAdd>(p, rows, whole, s))
-  return dy_f32 ? WS_GRAD(true) : WS_GRAD(false);
+  return WS_GRAD(launch_grad, p, rows, whole, s);
 #undef WS_GRAD
 }

@@ -27,6 +27,7 @@ struct GroupedParams {
   long b_group;                 // elements from one group's weight to the next
   const long* offsets;          // [groups + 1]
   int groups, rows, N, K, tiles_n;
+  int b_rows;                   // columns of the product that the weight has; those up to N get zeros
   int most;                     // tiles that the grid is sized for
   int pieces_most;              // a last round of at most so many 256 x 256 tiles goes in pieces
   unsigned short* c; long ldc;
@@ -116,7 +117,7 @@ __device__ __forceinline__ void grouped_piece(const GroupedParams& p, int whole,
   OperandDesc b = p.b;
   b.ptr += max(t.group, 0) * p.b_group;
   Acc16<Cfg::FA, Cfg::FB> acc;
-  ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.N, 0, p.K, 0,
+  ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.b_rows, 0, p.K, 0,
                                            t.group < 0 ? 0 : cdiv(p.K, kFBK), smem, wave, lane);
   const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
   FEpiStore<false, false>::run(e, acc, row0 + wm * Cfg::TM, col0 + wn * Cfg::TN, lane, tm, tn, wn,
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(kFNT) grouped_fast_kernel(const GroupedParams 
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc.v[i][j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
-    fast_k_loop<kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.N, 0, p.K, 0,
+    fast_k_loop<kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.b_rows, 0, p.K, 0,
                                         t.group < 0 ? 0 : cdiv(p.K, kFBK), fsmem, fsmem + 2 * kFTileBytes, abase,
                                         bbase, wave, lane);
     const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(Cfg::NT) grouped_ring_kernel(const GroupedPara
   OperandDesc b = p.b;
   b.ptr += max(t.group, 0) * p.b_group;
   Acc16<FA, FB> acc;
-  ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.N, 0, p.K, 0,
+  ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.b_rows, 0, p.K, 0,
                                            t.group < 0 ? 0 : cdiv(p.K, kFBK), rsmem, wave, lane);
   const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
   FEpiStore<false, false>::run(e, acc, row0 + wm * TM, col0 + wn * TN, lane, tm, tn, wn,
@@ -337,8 +338,8 @@ __global__ void __launch_bounds__(Cfg::NT) grouped_grad_ring_kernel(const Groupe
 // with a quarter of the reduction (64 of every 256 k, so that together they read whole rows of the
 // weight). Fragments go from memory to registers as they are: a lane's piece is 16 bytes of one row,
 // and a k-tile's two pieces of a row are one line. The waves' sums are added through LDS, in
-// wave order. Rows and columns past the group's and the weight's read the last ones and are not
-// stored.
+// wave order. Rows past the group's read its last one and are not stored; columns past the weight's
+// read its last one, and what they get, up to N, is no part of the result.
 constexpr int kFewRows = 16, kFewCols = 32;
 
 static __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedParams p) {
@@ -357,7 +358,7 @@ static __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedPa
     const unsigned short* b[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-      b[j] = p.b.ptr + t.group * p.b_group + (long)min(col0 + 16 * j + r, p.N - 1) * p.b.s_row + q;
+      b[j] = p.b.ptr + t.group * p.b_group + (long)min(col0 + 16 * j + r, p.b_rows - 1) * p.b.s_row + q;
     // U k-tiles at a time, all of their pieces requested before the first product.
     auto steps = [&](int k, auto count, auto load) {
       constexpr int U = decltype(count)::value;

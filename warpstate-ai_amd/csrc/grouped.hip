@@ -83,9 +83,13 @@ int check_sizes(int64_t groups, int64_t rows, int64_t n, int64_t k) {
   if (groups < 1 || groups > kMaxGroups) return set_error(kInvalid, "1 to %ld groups, not %ld", (long)kMaxGroups, (long)groups);
   if (rows < 0 || n < 1 || k < 1 || rows > kMaxRows || !fits_i32(n) || !fits_i32(k))
     return set_error(kInvalid, "invalid grouped product shape (%ld rows, %ld x %ld)", (long)rows, (long)n, (long)k);
-  if (n % 8 != 0 || k % 8 != 0) return set_error(kInvalid, "grouped products take widths of a multiple of 8, not %ld and %ld", (long)n, (long)k);
   return kOk;
 }
+// The width of the weights' rows.
+int check_width(int64_t width) {
+  return width % 8 == 0 ? kOk : set_error(kInvalid, "grouped products take weight rows of a multiple of 8, not %ld", (long)width);
+}
+int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 // Rows of whole, aligned 16-byte pieces, 256 of which span less than 2 GiB.
 int check_rows(const void* p, int64_t ld, int64_t rows, int64_t cols, const char* what) {
   if (!al(p, 16) || ld % 8 != 0) return set_error(kInvalid, "%s rows must be 16-byte aligned", what);
@@ -158,9 +162,11 @@ extern "C" int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int
   if (rows == 0) return kOk;
   if (!x || !weight || !offsets || !y) return set_error(kInvalid, "null pointer");
   const bool nt = form == WS_GROUPED_NT;
-  if (int rc = check_rows(x, ldx, rows, k, "x")) return rc;
+  if (int rc = check_width(nt ? k : n)) return rc;
+  const int64_t wide = up8(n);
+  if (int rc = check_rows(x, ldx, rows, up8(k), "x")) return rc;
   if (int rc = check_rows(weight, ld_weight, 2, nt ? k : n, "weight")) return rc;
-  if (int rc = check_rows(y, ldy, rows, n, "y")) return rc;
+  if (int rc = check_rows(y, ldy, rows, wide, "y")) return rc;
   if (group_stride % 8 != 0 || group_stride < 0) return set_error(kInvalid, "weights must be 16-byte aligned");
   const int tile = pick_grouped(rows, groups, n, k, nt ? kKContig : kMNContig);
   GroupedParams p{};
@@ -170,9 +176,10 @@ extern "C" int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int
   p.offsets = reinterpret_cast<const long*>(offsets);
   p.groups = (int)groups;
   p.rows = (int)rows;
-  p.N = (int)n;
+  p.N = (int)wide;
   p.K = (int)k;
-  p.tiles_n = cdiv(n, tile_cols(tile));
+  p.b_rows = (int)n;
+  p.tiles_n = cdiv(wide, tile_cols(tile));
   p.c = static_cast<unsigned short*>(y);
   p.ldc = ldy;
   const int64_t grid = most_tiles(rows, groups, tile_rows(tile)) * p.tiles_n;
@@ -186,8 +193,9 @@ extern "C" int ws_grouped_weight_grad(const void* dy, int64_t ld_dy, const void*
                                       int64_t groups, int64_t rows, int64_t n, int64_t k, void* dweight,
                                       int dweight_f32, void* stream) {
   if (int rc = check_sizes(groups, rows, n, k)) return rc;
+  if (int rc = check_width(k)) return rc;
   if (!dweight || !offsets || (rows > 0 && (!dy || !x))) return set_error(kInvalid, "null pointer");
-  if (int rc = check_rows(dy, ld_dy, rows, n, "dy")) return rc;
+  if (int rc = check_rows(dy, ld_dy, rows, up8(n), "dy")) return rc;
   if (int rc = check_rows(x, ldx, rows, k, "x")) return rc;
   if (!al(dweight, 16)) return set_error(kInvalid, "the weight gradient must be 16-byte aligned");
   if (int rc = check_out_stride(k, dweight_f32 ? 4 : 2, "dweight")) return rc;

@@ -71,25 +71,19 @@ void check_norm(const Tensor& x, const std::optional<Tensor>& residual, const Te
                       "The residual must be BF16 or FP32, of shape ", x.sym_sizes(), " on ", x.device());
 }
 
-ThreeTensors add_rmsnorm_rstd(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
+TwoTensors add_rmsnorm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
   check_norm(x, residual, weight);
   c10::DeviceGuard guard(x.device());
   const Tensor a = rows_of(x), r = rows_of(residual), w = weight.contiguous();
   const int64_t rows = a.size(0), d = a.size(1);
   Tensor y = at::empty(x.sizes(), x.options()), stream = at::empty(x.sizes(), residual.options());
-  Tensor rstd = floats(x, {rows});
   check(ws_add_rmsnorm(ptr(a), row_stride(a), ptr(r), row_stride(r), r.scalar_type() == at::kFloat,
-                       w.const_data_ptr<float>(), (float)eps, rows, d, ptr(y), ptr(stream), rstd.data_ptr<float>(),
-                       stream_of(x)),
+                       w.const_data_ptr<float>(), (float)eps, rows, d, ptr(y), ptr(stream), stream_of(x)),
         "ws_add_rmsnorm");
-  return {y, stream, rstd};
-}
-TwoTensors add_rmsnorm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
-  auto [y, stream, rstd] = add_rmsnorm_rstd(x, residual, weight, eps);
   return {y, stream};
 }
 // (dx, dresidual, dweight); dresidual is empty for a BF16 stream, whose gradient is dx.
-ThreeTensors add_rmsnorm_backward(const Tensor& stream, const Tensor& weight, const Tensor& rstd, const Tensor& dy,
+ThreeTensors add_rmsnorm_backward(const Tensor& stream, const Tensor& weight, double eps, const Tensor& dy,
                                   const std::optional<Tensor>& dstream) {
   c10::DeviceGuard guard(stream.device());
   const bool f32 = stream.scalar_type() == at::kFloat;
@@ -99,11 +93,12 @@ ThreeTensors add_rmsnorm_backward(const Tensor& stream, const Tensor& weight, co
   const Tensor s = rows_of(stream), g = rows_of(dy), w = weight.contiguous();
   const Tensor h = dstream.has_value() ? rows_of(*dstream) : Tensor();
   const int64_t rows = s.size(0), d = s.size(1);
-  Tensor partial = floats(stream, {ws_add_rmsnorm_backward_partial_floats(rows, d)});
-  check(ws_add_rmsnorm_backward(s.const_data_ptr(), f32, w.const_data_ptr<float>(), rstd.const_data_ptr<float>(),
+  const int64_t need = ws_add_rmsnorm_backward_partial_floats(rows, d);
+  Tensor partial = need ? floats(stream, {need}) : Tensor();
+  check(ws_add_rmsnorm_backward(s.const_data_ptr(), f32, w.const_data_ptr<float>(), (float)eps,
                                 g.const_data_ptr(), row_stride(g), ptr(h), h.defined() ? row_stride(h) : 0, rows, d,
                                 dx.data_ptr(), f32 ? dresidual.data_ptr<float>() : nullptr, dweight.data_ptr<float>(),
-                                partial.data_ptr<float>(), stream_of(stream)),
+                                static_cast<float*>(ptr(partial)), stream_of(stream)),
         "ws_add_rmsnorm_backward");
   return {dx, dresidual, dweight};
 }
@@ -112,22 +107,23 @@ struct AddRmsnormFn : Function<AddRmsnormFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& weight,
                                double eps) {
     typedef const Tensor& T;
-    static const auto op = find<ThreeTensors(T, T, T, double)>("warpstate::native_add_rmsnorm_rstd");
-    auto [y, stream, rstd] = below(op, x, residual, weight, eps);
+    static const auto op = find<TwoTensors(T, T, T, double)>("warpstate::native_add_rmsnorm");
+    auto [y, stream] = below(op, x, residual, weight, eps);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({stream, weight, rstd});
+    ctx->save_for_backward({stream, weight});
+    ctx->saved_data["eps"] = eps;
     return {y, stream};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     typedef const Tensor& T;
     static const auto op =
-        find<ThreeTensors(T, T, T, T, const std::optional<Tensor>&)>("warpstate::native_add_rmsnorm_backward");
+        find<ThreeTensors(T, T, double, T, const std::optional<Tensor>&)>("warpstate::native_add_rmsnorm_backward");
     const Tensor &dy = grads[0], &dstream = grads[1];
     if (!dy.defined())  // the addition alone
       return {dstream.defined() ? dstream.to(at::kBFloat16) : Tensor(), dstream, Tensor(), Tensor()};
     const auto s = ctx->get_saved_variables();
     auto [dx, dresidual, dweight] =
-        below(op, s[0], s[1], s[2], dy, dstream.defined() ? std::optional<Tensor>(dstream) : std::nullopt);
+        below(op, s[0], s[1], ctx->saved_data["eps"].toDouble(), dy, dstream.defined() ? std::optional<Tensor>(dstream) : std::nullopt);
     const bool f32 = s[0].scalar_type() == at::kFloat;
     return once({dx, f32 ? dresidual : dx, dweight, Tensor()}, {s[0], s[1], dy, dstream}, kNormTwice);
   }
@@ -146,11 +142,7 @@ TwoTensors add_rmsnorm_meta(const Tensor& x, const Tensor& residual, const Tenso
   check_norm(x, residual, weight);
   return {at::empty_symint(x.sym_sizes(), x.options()), at::empty_symint(x.sym_sizes(), residual.options())};
 }
-ThreeTensors add_rmsnorm_rstd_meta(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps) {
-  auto [y, stream] = add_rmsnorm_meta(x, residual, weight, eps);
-  return {y, stream, at::empty_symint({x.sym_numel() / x.sym_size(-1)}, x.options().dtype(at::kFloat))};
-}
-ThreeTensors add_rmsnorm_backward_meta(const Tensor& stream, const Tensor& weight, const Tensor&, const Tensor& dy,
+ThreeTensors add_rmsnorm_backward_meta(const Tensor& stream, const Tensor& weight, double, const Tensor& dy,
                                        const std::optional<Tensor>&) {
   const bool f32 = stream.scalar_type() == at::kFloat;
   return {at::empty_symint(stream.sym_sizes(), dy.options()),
@@ -235,10 +227,11 @@ void embedding_sums(const Tensor& dy, const Tensor& tokens_in, double scale, con
   const Tensor tokens = tokens_in.contiguous();
   const int64_t rows = tokens.numel(), vocab = out.size(0), d = out.size(1);
   const Tensor g = rows ? rows_of(dy) : Tensor();
-  Tensor work = bytes(out, {ws_embedding_backward_workspace_bytes(rows, vocab, d)});
+  const int64_t need = ws_embedding_backward_workspace_bytes(rows, vocab, d);
+  Tensor work = need ? bytes(out, {need}) : Tensor();
   check(ws_embedding_backward(ptr(g), rows ? row_stride(g) : 0, rows && g.scalar_type() == at::kFloat,
                               static_cast<const int64_t*>(ptr(tokens)), rows, vocab, d, (float)scale, out.data_ptr(),
-                              row_stride(out), mode, work.data_ptr(), stream_of(out)),
+                              row_stride(out), mode, ptr(work), stream_of(out)),
         "ws_embedding_backward");
 }
 Tensor embedding_backward(const Tensor& dy, const Tensor& tokens, int64_t vocab, double scale, bool f32) {
@@ -310,8 +303,8 @@ void check_grouped(const Tensor& x, const Tensor& weight, const Tensor& offsets)
                         fixed(offsets, 0) == fixed(weight, 0) + 1 && offsets.device() == x.device(),
                     "Offsets must be an int64 vector, one more than the groups, on ", x.device());
 }
-// A matrix as the kernels read it: 16-byte rows of a multiple of 8, itself or a copy padded with
-// zeros.
+// A matrix as the kernels read it: 16-byte rows of a multiple of 8, itself or a copy whose rows are
+// padded with zeros.
 bool whole_rows(const Tensor& t) {
   auto stride = [&](int64_t i) { return t.sym_stride(i).guard_int(__FILE__, __LINE__); };
   int64_t i = t.dim() - 1, inner = fixed(t, i);
@@ -329,8 +322,8 @@ const auto& copy_rows_op() {
   return op;
 }
 Tensor grouped_operand(const Tensor& t) {
-  if (whole_rows(t) && (t.dim() == 2 || fixed(t, 1) % 8 == 0)) return t.to(at::kBFloat16);
-  return copy_rows_op().call(t, t.dim() == 2 ? t.sym_size(0) : c10::SymInt(up(fixed(t, 1), 8)), up(fixed(t, -1), 8), true);
+  if (whole_rows(t)) return t.to(at::kBFloat16);
+  return copy_rows_op().call(t, t.sym_size(t.dim() - 2), up(fixed(t, -1), 8), true);
 }
 // t [rows, cols] or [groups, rows, cols] in other sizes, padded with zeros or cut off: a new tensor, in
 // BF16 or in t's type.
@@ -355,23 +348,24 @@ Tensor copy_rows_meta(const Tensor& t, c10::SymInt rows, c10::SymInt cols, bool 
   return at::empty_symint({t.sym_size(0), rows, cols}, options);
 }
 
-// On operands of grouped_operand: [rows, n] (form NT) or [rows, k] (NN), padded widths.
+// On operands of grouped_operand: [rows, n up to the next multiple of 8] (form NT) or [rows, padded k]
+// (NN, x and the reduction reach to w's rows).
 Tensor grouped_rows(const Tensor& x, const Tensor& w, const Tensor& offsets_in, int64_t form) {
   c10::DeviceGuard guard(x.device());
   const Tensor offsets = offsets_in.contiguous();
   const bool nt = form == WS_GROUPED_NT;
   const int64_t rows = x.size(0), n = w.size(nt ? 1 : 2), k = w.size(nt ? 2 : 1);
-  Tensor y = at::empty({rows, n}, x.options());
+  Tensor y = at::empty({rows, up(n, 8)}, x.options());
   check(ws_grouped_mm(ptr(x), row_stride(x), w.const_data_ptr(), w.size(1) > 1 ? w.stride(1) : w.size(2),
                       w.size(0) > 1 ? w.stride(0) : 0, (int)form, offsets.const_data_ptr<int64_t>(), w.size(0), rows,
-                      n, k, ptr(y), n, stream_of(x)),
+                      n, k, ptr(y), y.size(1), stream_of(x)),
         "ws_grouped_mm");
   return y;
 }
-Tensor grouped_grad(const Tensor& dy, const Tensor& x, const Tensor& offsets_in, bool f32) {
+Tensor grouped_grad(const Tensor& dy, const Tensor& x, const Tensor& offsets_in, int64_t n, bool f32) {
   c10::DeviceGuard guard(x.device());
   const Tensor offsets = offsets_in.contiguous();
-  const int64_t groups = offsets.size(0) - 1, n = dy.size(1), k = x.size(1);
+  const int64_t groups = offsets.size(0) - 1, k = x.size(1);
   Tensor dw = at::empty({groups, n, k}, x.options().dtype(f32 ? at::kFloat : at::kBFloat16));
   check(ws_grouped_weight_grad(ptr(dy), row_stride(dy), ptr(x), row_stride(x), offsets.const_data_ptr<int64_t>(),
                                groups, x.size(0), n, k, dw.data_ptr(), f32, stream_of(x)),
@@ -379,7 +373,7 @@ Tensor grouped_grad(const Tensor& dy, const Tensor& x, const Tensor& offsets_in,
   return dw;
 }
 typedef Tensor GroupedRows(const Tensor&, const Tensor&, const Tensor&, int64_t);
-typedef Tensor GroupedGrad(const Tensor&, const Tensor&, const Tensor&, bool);
+typedef Tensor GroupedGrad(const Tensor&, const Tensor&, const Tensor&, int64_t, bool);
 // Below autograd.
 Tensor first_columns(const Tensor& t, int64_t cols) {
   return fixed(t, -1) == cols ? t : copy_rows_op().call(t, t.sym_size(0), cols, false);
@@ -420,8 +414,8 @@ struct GroupedMmFn : Function<GroupedMmFn> {
       const Tensor g = grouped_operand(grads[0]);
       if (ctx->saved_data["want_x"].toBool()) d[0] = first_columns(rows_op.call(g, s[1], s[2], WS_GROUPED_NN), k);
       if (ctx->saved_data["want_w"].toBool()) {
-        Tensor dw = grad_op.call(g, s[0], s[2], ctx->saved_data["f32"].toBool());
-        if (fixed(dw, 1) != n || fixed(dw, 2) != k) dw = copy_rows_op().call(dw, n, k, false);
+        Tensor dw = grad_op.call(g, s[0], s[2], n, ctx->saved_data["f32"].toBool());
+        if (fixed(dw, 2) != k) dw = copy_rows_op().call(dw, n, k, false);
         d[1] = dw;
       }
     }
@@ -448,10 +442,10 @@ Tensor grouped_mm_meta(const Tensor& x, const Tensor& weight, const Tensor& offs
   return at::empty_symint({x.sym_size(0), weight.sym_size(1)}, x.options());
 }
 Tensor grouped_rows_meta(const Tensor& x, const Tensor& w, const Tensor&, int64_t form) {
-  return at::empty_symint({x.sym_size(0), w.sym_size(form == WS_GROUPED_NT ? 1 : 2)}, x.options());
+  return at::empty_symint({x.sym_size(0), up(fixed(w, form == WS_GROUPED_NT ? 1 : 2), 8)}, x.options());
 }
-Tensor grouped_grad_meta(const Tensor& dy, const Tensor& x, const Tensor& offsets, bool f32) {
-  return at::empty_symint({offsets.sym_size(0) - 1, dy.sym_size(1), x.sym_size(1)},
+Tensor grouped_grad_meta(const Tensor&, const Tensor& x, const Tensor& offsets, int64_t n, bool f32) {
+  return at::empty_symint({offsets.sym_size(0) - 1, n, x.sym_size(1)},
                           x.options().dtype(f32 ? at::kFloat : at::kBFloat16));
 }
 
@@ -459,9 +453,8 @@ Tensor grouped_grad_meta(const Tensor& dy, const Tensor& x, const Tensor& offset
 
 TORCH_LIBRARY_FRAGMENT(warpstate, m) {
   m.def("native_add_rmsnorm(Tensor x, Tensor residual, Tensor weight, float eps) -> (Tensor, Tensor)");
-  m.def("native_add_rmsnorm_rstd(Tensor x, Tensor residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)");
   m.def(
-      "native_add_rmsnorm_backward(Tensor stream, Tensor weight, Tensor rstd, Tensor dy, Tensor? dstream) -> "
+      "native_add_rmsnorm_backward(Tensor stream, Tensor weight, float eps, Tensor dy, Tensor? dstream) -> "
       "(Tensor, Tensor, Tensor)");
   m.def(
       "native_rmsnorm_quantize(Tensor x, Tensor? residual, Tensor weight, float eps, bool e8m0) -> (Tensor, Tensor, "
@@ -472,11 +465,10 @@ TORCH_LIBRARY_FRAGMENT(warpstate, m) {
   m.def("native_grouped_mm(Tensor x, Tensor weight, Tensor offsets) -> Tensor");
   m.def("native_copy_rows(Tensor t, SymInt rows, SymInt cols, bool bf16) -> Tensor");
   m.def("native_grouped_rows(Tensor x, Tensor w, Tensor offsets, int form) -> Tensor");
-  m.def("native_grouped_grad(Tensor dy, Tensor x, Tensor offsets, bool f32) -> Tensor");
+  m.def("native_grouped_grad(Tensor dy, Tensor x, Tensor offsets, int n, bool f32) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(warpstate, CUDA, m) {
   m.impl("native_add_rmsnorm", &add_rmsnorm);
-  m.impl("native_add_rmsnorm_rstd", &add_rmsnorm_rstd);
   m.impl("native_add_rmsnorm_backward", &add_rmsnorm_backward);
   m.impl("native_rmsnorm_quantize", &rmsnorm_quantize);
   m.impl("native_embedding", &embedding);
@@ -495,7 +487,6 @@ TORCH_LIBRARY_IMPL(warpstate, AutogradCUDA, m) {
 }
 TORCH_LIBRARY_IMPL(warpstate, Meta, m) {
   m.impl("native_add_rmsnorm", &add_rmsnorm_meta);
-  m.impl("native_add_rmsnorm_rstd", &add_rmsnorm_rstd_meta);
   m.impl("native_add_rmsnorm_backward", &add_rmsnorm_backward_meta);
   m.impl("native_rmsnorm_quantize", &rmsnorm_quantize_meta);
   m.impl("native_embedding", &embedding_meta);

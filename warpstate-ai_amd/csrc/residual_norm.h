@@ -7,7 +7,8 @@
 // e4m3 with a scale per block of 128 (quant.h), from FP32 either way. With g = dy w and the
 // stream's own upstream gradient ds,
 //   d = ds + rstd (g - s rstd^2 mean(g s)),  dweight = sum over rows of dy s rstd,
-// and d is the gradient of both inputs, rounded to the type of each.
+// and d is the gradient of both inputs, rounded to the type of each. The backward reads s anyway and
+// takes rstd from it again, so that nothing but the stream is kept for it.
 //
 // HBM-bound: each input is read once and each output written once, with the row in registers
 // between. A row's pieces of eight columns lie on consecutive lanes, so that 16 lanes hold a block
@@ -26,7 +27,6 @@ struct AddNormParams {
   float eps;
   unsigned short* y;               // [rows, d]
   void* stream;                    // [rows, d], the stream's type
-  float* rstd;
   unsigned char* q; long ldq;      // bytes past d up to q_cols, the next multiple of 16, are zeros
   int q_cols;
   void* scale; long ld_scale;
@@ -100,8 +100,8 @@ __device__ __forceinline__ QuantRow<F32> round_piece(const float (&f)[8]) {
   return v;
 }
 
-// The sum of v over the WPR waves of a row, in wave order. `slot` alternates between two calls
-// in a row, so that one barrier per sum is enough.
+// The sum of v over the WPR waves of a row, in wave order. `slot` differs between two sums with no
+// barrier but theirs between them, so that one barrier per sum is enough.
 template <int WPR>
 __device__ __forceinline__ float row_sum(float v, float (*red)[4], int slot, int lane, int wave) {
   v = wave_sum(v);
@@ -148,7 +148,6 @@ static __global__ void __launch_bounds__(256) add_rmsnorm_kernel(const AddNormPa
     for (int e = 0; e < 8; ++e) acc += s[i].at(e) * s[i].at(e);
   acc = row_sum<WPR>(acc, red, 0, lane, wave);
   const float r = 1.0f / sqrtf(acc / (float)p.d + p.eps);
-  if (OUT == kNormBF16 && lane == 0 && (WPR == 1 || wave == 0)) p.rstd[row] = r;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = c0 + i * 512 * WPR, left = p.d - c;
@@ -182,7 +181,8 @@ static __global__ void __launch_bounds__(256) add_rmsnorm_kernel(const AddNormPa
 
 struct AddNormGradParams {
   const void* s;                            // [rows, d], the stream's type
-  const float* w; const float* rstd;
+  const float* w;
+  float eps;
   const unsigned short* dy; long ld_dy;
   const void* ds; long ld_ds;               // the stream's type; unused without DS
   int rows, d;
@@ -195,7 +195,7 @@ struct AddNormGradParams {
 // its waves, so that the gradient's partial sums cost one row of FP32 per workgroup.
 template <bool F32, bool DS, int NC, int WPR, bool WHOLE>
 static __global__ void __launch_bounds__(256) add_rmsnorm_bwd_kernel(const AddNormGradParams p) {
-  __shared__ float red[2][4];
+  __shared__ float red[4][4];
   __shared__ float sums[WPR == 1 ? 3 : 1][WPR == 1 ? 512 * NC : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c0 = 8 * (WPR == 1 ? lane : (int)threadIdx.x);
@@ -223,18 +223,26 @@ static __global__ void __launch_bounds__(256) add_rmsnorm_bwd_kernel(const AddNo
       load_piece<false, WHOLE>(dy[i], p.dy, (long)row * p.ld_dy + c, left);
       if constexpr (DS) load_piece<F32, WHOLE>(ds[i], p.ds, (long)row * p.ld_ds + c, left);
     }
-    const float r = p.rstd[row];
-    float dot = 0.0f;
+    float dot = 0.0f, square = 0.0f;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dot += (dy[i].at(e) * w[i][e]) * s[i].at(e);
-    dot = row_sum<WPR>(dot, red, slot, lane, wave);
+      for (int e = 0; e < 8; ++e) {
+        dot += (dy[i].at(e) * w[i][e]) * s[i].at(e);
+        square += s[i].at(e) * s[i].at(e);
+      }
+    dot = row_sum<WPR>(dot, red, 2 * slot, lane, wave);
+    square = row_sum<WPR>(square, red, 2 * slot + 1, lane, wave);
     slot ^= 1;
+    const float r = 1.0f / sqrtf(square / (float)p.d + p.eps);
     const float m = dot / (float)p.d * (r * r);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = c0 + i * 512 * WPR, left = p.d - c;
+      if constexpr (!F32) {  // keeps s and dy packed over the sums; unpacked they cost a workgroup's registers
+#pragma unroll
+        for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(s[i].w[e]), "+v"(dy[i].w[e]));
+      }
       float f[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

@@ -106,12 +106,12 @@ SIGNATURES = {
                                         + [_i64, _i64, _i64, _f32, _c_void_p, _i64, _c_void_p, _i64,
                                            _c_void_p, _i64, _i32, _c_void_p]),
     "ws_add_rmsnorm": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _i32, _c_void_p, _f32, _i64, _i64]
-                       + [_c_void_p] * 4),
+                       + [_c_void_p] * 3),
     "ws_rmsnorm_quantize": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _i32, _c_void_p, _f32, _i64,
                                    _i64, _i32, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
                                    _c_void_p]),
     "ws_add_rmsnorm_backward_partial_floats": (_i64, [_i64, _i64]),
-    "ws_add_rmsnorm_backward": (_i32, [_c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p, _i64,
+    "ws_add_rmsnorm_backward": (_i32, [_c_void_p, _i32, _c_void_p, _f32, _c_void_p, _i64,
                                        _c_void_p, _i64, _i64, _i64] + [_c_void_p] * 5),
     "ws_embedding": (_i32, [_c_void_p, _i64, _i32, _c_void_p, _i64, _i64, _i64, _f32, _c_void_p,
                             _i32, _c_void_p]),

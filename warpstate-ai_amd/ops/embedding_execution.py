@@ -47,10 +47,10 @@ def _sums(dy: Tensor, tokens: Tensor, scale: float, out: Tensor, mode: int) -> N
     rows, (vocab, d) = tokens.numel(), out.shape
     g = _rows(dy) if rows else None
     need = _hip.query("ws_embedding_backward_workspace_bytes", rows, vocab, d)
-    work = torch.empty((need,), dtype=torch.uint8, device=out.device)
+    work = torch.empty((need,), dtype=torch.uint8, device=out.device) if need else None
     _hip.call_on(out, "ws_embedding_backward", _hip.ptr(g), _row_stride(g) if rows else 0,
                  int(dy.dtype == F32), tokens.data_ptr(), rows, vocab, d, scale, out.data_ptr(),
-                 _row_stride(out), mode, work.data_ptr())
+                 _row_stride(out), mode, _hip.ptr(work))
 
 
 class _Embedding(torch.autograd.Function):

@@ -65,31 +65,32 @@ def _copy_rows(t: Tensor, rows: int, cols: int, dtype: torch.dtype) -> Tensor:
 
 
 def _operand(t: Tensor) -> Tensor:
-    """A BF16 operand with 16-byte rows of a multiple of 8, and weights with a multiple of 8 of
-    them: t itself or a copy, padded with zeros."""
-    if _whole_rows(t) and (t.ndim == 2 or t.shape[1] % 8 == 0):
+    """A BF16 operand with 16-byte rows of a multiple of 8: t itself, or a copy whose rows are
+    padded with zeros."""
+    if _whole_rows(t):
         return t.to(BF16)
-    rows = t.shape[0] if t.ndim == 2 else -(-t.shape[1] // 8) * 8
-    return _copy_rows(t, rows, -(-t.shape[-1] // 8) * 8, BF16)
+    return _copy_rows(t, t.shape[-2], _up(t.shape[-1]), BF16)
+
+
+def _up(n: int) -> int:
+    return -(-n // 8) * 8
 
 
 def _product(x: Tensor, w: Tensor, offsets: Tensor, form: int) -> Tensor:
-    """On operands of ``_operand``."""
+    """On operands of ``_operand``: columns up to the next multiple of 8."""
     rows, (groups, n, k) = x.shape[0], w.shape
     if form == _NN:
         n, k = k, n
-    y = torch.empty((rows, n), dtype=BF16, device=x.device)
+    y = torch.empty((rows, _up(n)), dtype=BF16, device=x.device)
     _hip.call_on(x, "ws_grouped_mm", x.data_ptr(), _row_stride(x), w.data_ptr(),
                  w.stride(1) if w.shape[1] > 1 else w.shape[2], w.stride(0) if groups > 1 else 0,
-                 form, offsets.data_ptr(), groups, rows, n, k, y.data_ptr(), n)
+                 form, offsets.data_ptr(), groups, rows, n, k, y.data_ptr(), y.shape[1])
     return y
 
 
-def _first(t: Tensor, *sizes: int) -> Tensor:
-    """The first of t's padded columns (and weight rows)."""
-    if t.shape[-len(sizes):] == sizes:
-        return t
-    return _copy_rows(t, t.shape[0] if len(sizes) == 1 else sizes[0], sizes[-1], t.dtype)
+def _first(t: Tensor, cols: int) -> Tensor:
+    """The first of t's padded columns."""
+    return t if t.shape[-1] == cols else _copy_rows(t, t.shape[-2], cols, t.dtype)
 
 
 class _GroupedMm(torch.autograd.Function):
@@ -115,11 +116,11 @@ class _GroupedMm(torch.autograd.Function):
                 dx = _first(_product(g, w, offsets, _NN), k)
             if ctx.needs_input_grad[1]:
                 groups = w.shape[0]
-                dw = torch.empty((groups, g.shape[1], a.shape[1]), dtype=dtype, device=a.device)
+                dw = torch.empty((groups, n, a.shape[1]), dtype=dtype, device=a.device)
                 _hip.call_on(a, "ws_grouped_weight_grad", g.data_ptr(), _row_stride(g),
-                             a.data_ptr(), _row_stride(a), offsets.data_ptr(), groups, a.shape[0],
-                             g.shape[1], a.shape[1], dw.data_ptr(), int(dtype == F32))
-                dw = _first(dw, n, k)
+                             a.data_ptr(), _row_stride(a), offsets.data_ptr(), groups, a.shape[0], n,
+                             a.shape[1], dw.data_ptr(), int(dtype == F32))
+                dw = _first(dw, k)
         return _once("a grouped product", (dx, dw, None, None, None), x, weight, dy)
 
 
@@ -133,8 +134,8 @@ def grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:
     gradient of x. No value of theirs leads an access out of the operands, but rows that
     decreasing ones name twice or not at all are unspecified. Sums are FP32. A row's bits depend on the
     kernel that the sizes choose, not on the other rows' values. Operands whose rows are not whole
-    16-byte pieces (a width that is no multiple of 8, other strides) are copied first, on every
-    call."""
+    16-byte pieces (weights or rows with k no multiple of 8, other strides) are copied first, on
+    every call: a program that uses such weights many times pads their rows once."""
     if not x.is_cuda:
         raise ValueError("Grouped products require CUDA tensors")
     native = _hip.host_ops()

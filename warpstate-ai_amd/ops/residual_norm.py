@@ -95,11 +95,11 @@ class _AddRmsnorm(torch.autograd.Function):
         rows, d = a.shape
         y = torch.empty(x.shape, dtype=BF16, device=x.device)
         stream = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-        rstd = torch.empty((rows,), dtype=F32, device=x.device)
         _hip.call_on(x, "ws_add_rmsnorm", a.data_ptr(), _row_stride(a), r.data_ptr(),
                      _row_stride(r), int(r.dtype == F32), w.data_ptr(), eps, rows, d, y.data_ptr(),
-                     stream.data_ptr(), rstd.data_ptr())
-        ctx.save_for_backward(stream, weight, rstd)
+                     stream.data_ptr())
+        ctx.save_for_backward(stream, weight)
+        ctx.eps = eps
         ctx.set_materialize_grads(False)
         return y, stream
 
@@ -107,13 +107,13 @@ class _AddRmsnorm(torch.autograd.Function):
     def backward(ctx, dy, dstream):
         if dy is None:  # the addition alone
             return None if dstream is None else dstream.to(BF16), dstream, None, None
-        stream, weight, rstd = ctx.saved_tensors
+        stream, weight = ctx.saved_tensors
         with torch.no_grad():
-            grads = _backward(stream, weight, rstd, dy, dstream)
+            grads = _backward(stream, weight, ctx.eps, dy, dstream)
         return _once("the residual norm", (*grads, None), stream, weight, dy, dstream)
 
 
-def _backward(stream, weight, rstd, dy, dstream):
+def _backward(stream, weight, eps, dy, dstream):
     """(dx, dresidual, dweight)."""
     f32 = stream.dtype == F32
     dx = torch.empty(stream.shape, dtype=BF16, device=stream.device)
@@ -125,11 +125,11 @@ def _backward(stream, weight, rstd, dy, dstream):
     h = None if dstream is None else _rows(dstream)
     rows, d = s.shape
     need = _hip.query_on(s, "ws_add_rmsnorm_backward_partial_floats", rows, d)
-    partial = torch.empty((need,), dtype=F32, device=s.device)
+    partial = torch.empty((need,), dtype=F32, device=s.device) if need else None
     _hip.call_on(s, "ws_add_rmsnorm_backward", s.data_ptr(), int(f32), w.data_ptr(),
-                 rstd.data_ptr(), g.data_ptr(), _row_stride(g), _hip.ptr(h),
+                 eps, g.data_ptr(), _row_stride(g), _hip.ptr(h),
                  0 if h is None else _row_stride(h), rows, d, dx.data_ptr(), _hip.ptr(dresidual),
-                 dweight.data_ptr(), partial.data_ptr())
+                 dweight.data_ptr(), _hip.ptr(partial))
     return dx, dresidual if f32 else dx, dweight
 
 
