@@ -506,7 +506,7 @@ int ws_add_rmsnorm_backward(const void* stream_in, int stream_f32, const float* 
  *
  * y [rows, d] (BF16, or FP32 with y_f32) = scale * table[token] from a BF16 or FP32 table [vocab,
  * d] (row stride ld_table). A token of -100 is ignored: its row is zeros. Any other token outside
- * [0, vocab) gets NaN. Up to 2^22 rows of the table and 2^24 tokens.
+ * [0, vocab) gets NaN. Up to 2^22 rows of 2^20 columns of the table, and 2^24 tokens.
  */
 int ws_embedding(const void* table, int64_t ld_table, int table_f32, const int64_t* tokens,
                  int64_t rows, int64_t vocab, int64_t d, float scale, void* y, int y_f32,

@@ -69,7 +69,8 @@ def test_partial_floats_of_bad_sizes():
 @pytest.mark.parametrize("change,match", [
     (dict(rows=-1), "shape"), (dict(vocab=0), "shape"), (dict(d=0), "shape"), (dict(table=None), "null"),
     (dict(tokens=None), "null"), (dict(y=None), "null"), (dict(ld=7), "overlap"),
-    (dict(rows=2 ** 24 + 1), "shape"), (dict(vocab=2 ** 22 + 1), "shape")])
+    (dict(rows=2 ** 24 + 1), "shape"), (dict(vocab=2 ** 22 + 1), "shape"),
+    (dict(d=2 ** 20 + 1, ld=2 ** 20 + 1), "shape")])
 def test_embedding_arguments(change, match):
     a = dict(table=GPU, ld=8, tokens=GPU, rows=4, vocab=10, d=8, y=GPU) | change
     with pytest.raises(RuntimeError, match=match):
@@ -81,7 +82,7 @@ def test_embedding_arguments(change, match):
     (dict(rows=-1), "shape"), (dict(vocab=0), "shape"), (dict(mode=3), "mode"), (dict(mode=-1), "mode"),
     (dict(dy=None), "null"), (dict(tokens=None), "null"), (dict(out=None), "null"),
     (dict(work=None, rows=65), "null"), (dict(work=GPU + 4), "aligned"), (dict(ld_dy=7), "overlap"),
-    (dict(ld=7), "overlap")])
+    (dict(ld=7), "overlap"), (dict(d=2 ** 20 + 1, ld=2 ** 20 + 1, ld_dy=2 ** 20 + 1), "shape")])
 def test_embedding_backward_arguments(change, match):
     a = dict(dy=GPU, ld_dy=8, tokens=GPU, rows=4, vocab=10, d=8, out=GPU, ld=8, mode=0, work=GPU) | change
     with pytest.raises(RuntimeError, match=match):

@@ -84,8 +84,8 @@ def embedding(tokens: Tensor, table: Tensor, scale: float = 1.0,
     master, any strides), in ``out_dtype`` (BF16 or FP32), with autograd to the table.
 
     Each row is scaled in FP32 and rounded once. The gradient comes in the table's type from FP32
-    sums, all of it written (rows without tokens are zeros). Up to 2^22 rows of the table and 2^24
-    tokens."""
+    sums, all of it written (rows without tokens are zeros). Up to 2^22 rows of 2^20
+    columns and 2^24 tokens."""
     if not table.is_cuda:
         raise ValueError("Embeddings require CUDA tensors")
     if out_dtype not in (BF16, F32):
