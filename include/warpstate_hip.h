@@ -555,8 +555,8 @@ int ws_copy_rows(const void* in, int in_f32, int64_t group_in, int64_t ld_in, in
                  int64_t cols_in, void* out, int out_f32, int64_t group_out, int64_t ld_out,
                  int64_t rows_out, int64_t cols_out, int64_t groups, void* stream);
 /* What these sizes run on, without a launch (WS_GROUPED_GRAD: the weight gradient): 0 256 x 256,
- * 1 and 2 128 x 128 (two or one workgroup on a compute unit), 3 64 x 128, 4 64 x 64, 5 the kernel
- * for few rows; -1 for invalid sizes. */
+ * 1 and 2 128 x 128 (two or one workgroup on a compute unit), 3 64 x 128, 4 64 x 64, 5 and 6 the kernel
+ * for few rows (tiles of 32 or 16 columns); -1 for invalid sizes. */
 int ws_grouped_tile(int64_t rows, int64_t groups, int64_t n, int64_t k, int form);
 
 #ifdef __cplusplus

@@ -67,7 +67,8 @@ def _check(x, w, dy, offsets, y, dx=None, dw=None):
 
 # Rows, groups, n, k. The last five reach the pieces of a last round of 256 x 256 tiles (no whole
 # round before it, one, and a last round that is long enough to stay whole).
-SIZES = [(1, 1, 8, 8), (1, 5, 64, 72), (7, 3, 16, 200), (16, 64, 96, 264), (100, 9, 264, 1000), (200, 8, 520, 96),
+SIZES = [(1, 1, 8, 8), (1, 5, 64, 72), (7, 3, 16, 200), (16, 64, 96, 264), (20, 8, 1288, 2056), (40, 8, 1288, 264),
+         (100, 8, 520, 264), (100, 9, 264, 1000), (200, 8, 520, 96),
          (300, 4, 512, 512), (700, 70, 64, 64), (1000, 130, 128, 136), (1000, 5, 256, 128), (3000, 3, 2048, 512),
          (4096, 8, 1288, 1280), (4096, 64, 512, 1280), (6000, 32, 1280, 896), (8192, 4, 1280, 520),
          (2600, 2, 2056, 1544), (9000, 4, 2304, 1608), (9000, 4, 1608, 2304), (12000, 3, 2304, 1536),
@@ -98,7 +99,7 @@ def test_every_tile_is_reached():
 
     found = {form: {_hip.query("ws_grouped_tile", r, g, *((k, n) if form == NN else (n, k)), form)
                     for r, g, n, k in SIZES} for form in (NT, NN, GRAD)}
-    assert {0, 1, 3, 4, 5} <= found[NT], found
+    assert {0, 1, 3, 4, 5, 6} <= found[NT], found
     assert {0, 1, 3, 4} <= found[NN] and {0, 1, 3, 4} <= found[GRAD], found
 
 

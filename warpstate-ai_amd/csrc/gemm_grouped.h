@@ -334,42 +334,50 @@ __global__ void __launch_bounds__(Cfg::NT) grouped_grad_ring_kernel(const Groupe
 }
 
 // --------------------------------------------------------------------------------------
-// Few rows for each group: tiles of 16 rows x 32 columns, one workgroup of four waves, each
+// Few rows for each group: tiles of 16 rows x COLS columns, one workgroup of four waves, each
 // with a quarter of the reduction (64 of every 256 k, so that together they read whole rows of the
 // weight). Fragments go from memory to registers as they are: a lane's piece is 16 bytes of one row,
 // and a k-tile's two pieces of a row are one line. The waves' sums are added through LDS, in
 // wave order. Rows past the group's read its last one and are not stored; columns past the weight's
 // read its last one, and what they get, up to N, is no part of the result.
-constexpr int kFewRows = 16, kFewCols = 32;
+//
+// The weights' bytes are the bound. Neighbouring tiles run on one XCD, so that what it reads at a time is one
+// run of the weight, and two k-tiles are in flight: with four, the registers leave fewer workgroups
+// (32 rows in 8 groups of 5632 x 2048, launch order and four / these 40 / 34 us, 40 rows in 8 of 2048 x 8192 61 / 50).
+constexpr int kFewRows = 16;
 
+template <int COLS>
 static __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedParams p) {
-  constexpr int BM = kFewRows;
-  __shared__ float sums[4][BM][kFewCols + 4];
+  constexpr int BM = kFewRows, NJ = COLS / 16;
+  __shared__ float sums[4][BM][COLS + 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   GroupLanes v;
-  if ((int)blockIdx.x >= count_tiles<BM>(p, lane, v)) return;
-  const GroupTile t = find_tile<BM>(p, blockIdx.x, lane, v);
+  const int total = count_tiles<BM>(p, lane, v);
+  if ((int)blockIdx.x >= total) return;
+  const GroupTile t = find_tile<BM>(p, xcd_remap(blockIdx.x, total, kRingWindow), lane, v);
   const int tm = t.index / p.tiles_n, tn = t.index - tm * p.tiles_n;
-  const int row0 = t.lo + tm * BM, col0 = tn * kFewCols;
-  f32x4_v acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  const int row0 = t.lo + tm * BM, col0 = tn * COLS;
+  f32x4_v acc[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) acc[j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
   if (t.group >= 0) {
     const int r = lane & 15, q = 8 * (lane >> 4);
     const unsigned short* const a = p.a.ptr + (long)min(row0 + r, t.hi - 1) * p.a.s_row + q;
-    const unsigned short* b[2];
+    const unsigned short* b[NJ];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NJ; ++j)
       b[j] = p.b.ptr + t.group * p.b_group + (long)min(col0 + 16 * j + r, p.b_rows - 1) * p.b.s_row + q;
     // U k-tiles at a time, all of their pieces requested before the first product.
     auto steps = [&](int k, auto count, auto load) {
       constexpr int U = decltype(count)::value;
-      bf16x8_t fa[U][2], fb[U][2][2];
+      bf16x8_t fa[U][2], fb[U][2][NJ];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const int at = k + 256 * u + 32 * s;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) fb[u][s][j] = load(b[j], at);
+          for (int j = 0; j < NJ; ++j) fb[u][s][j] = load(b[j], at);
           fa[u][s] = load(a, at);
         }
       __builtin_amdgcn_sched_barrier(0);
@@ -378,11 +386,11 @@ static __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedPa
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < NJ; ++j)
             acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[u][s][j], fa[u][s], acc[j], 0, 0, 0);
     };
     const auto whole = [](const unsigned short* row, int at) { return *reinterpret_cast<const bf16x8_t*>(row + at); };
-    constexpr int U = 4;
+    constexpr int U = 2;
     int k = 64 * wave;
     for (; k + 256 * (U - 1) + 64 <= p.K; k += 256 * U) steps(k, std::integral_constant<int, U>{}, whole);
     for (; k + 64 <= p.K; k += 256) steps(k, std::integral_constant<int, 1>{}, whole);
@@ -394,10 +402,11 @@ static __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedPa
       });
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < NJ; ++j)
     *reinterpret_cast<f32x4_v*>(&sums[wave][lane & 15][16 * j + 4 * (lane >> 4)]) = acc[j];
   __syncthreads();
-  const int m = threadIdx.x >> 4, n = 2 * (threadIdx.x & 15);
+  const int m = threadIdx.x / (COLS / 2), n = 2 * (threadIdx.x % (COLS / 2));
+  if (m >= BM) return;
   float v2[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e)

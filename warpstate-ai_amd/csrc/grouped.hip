@@ -8,8 +8,8 @@ using namespace ws;
 namespace {
 
 constexpr int64_t kMaxGroups = 65536, kMaxRows = 1L << 30;
-// Beside FastTile: the kernel for few rows.
-constexpr int kTileFew = kFastTiles;
+// Beside FastTile: the kernel for few rows, tiles of 32 and of 16 columns.
+constexpr int kTileFew = kFastTiles, kTileFew16 = kFastTiles + 1;
 // The most 256 x 256 tiles for 256 compute units whose round goes in pieces (grouped_fast_kernel).
 constexpr int kPiecesOf256 = 64;
 
@@ -18,12 +18,13 @@ int tile_rows(int tile) {
     case kTile256: return 256;
     case kTile128x2:
     case kTile128x1: return 128;
-    case kTileFew: return kFewRows;
+    case kTileFew:
+    case kTileFew16: return kFewRows;
     default: return 64;
   }
 }
 int tile_cols(int tile) {
-  return tile == kTileFew ? kFewCols : tile == kTile256 ? 256 : tile == kTile64 ? 64 : 128;
+  return tile == kTileFew ? 32 : tile == kTileFew16 ? 16 : tile == kTile256 ? 256 : tile == kTile64 ? 64 : 128;
 }
 // Tiles of `rows` rows that any offsets make at most: a group ends in a part of one. (The rows of
 // no group form two more.)
@@ -37,9 +38,20 @@ int64_t most_tiles(int64_t rows, int64_t groups, int bm) {
 // there is one).
 int pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int bmode) {
   const int64_t used = groups < rows ? groups : rows;
-  // Up to 8 rows for each group (us, this kernel / the best tile): 64 rows in 8 groups of 5632 x 2048 41 /
-  // 43, 128 rows 54 / 42; 256 in 32 of 1280 x 896 17 / 17, 512 23 / 18.
-  if (bmode == kKContig && rows <= 8 * used) return kTileFew;
+  if (bmode == kKContig) {
+    // Up to 6 rows for each group, above which some groups take two tiles of 16 (us, this kernel / the best
+    // tile): 48 rows in 8 groups of 5632 x 2048 41 / 43, of 1024 x 8192 31 / 39, 64 rows 42 / 43 and 44 / 39; 256
+    // in 32 of 1024 x 1280 20 / 17. Up to 16 where its tiles leave units idle, and larger ones more so: 32 in
+    // 2 of 1024 x 2048 6 / 11, 128 in 8 of 512 x 1280 6 / 8.5.
+    const int64_t tiles = (int64_t)cdiv(n, 32) * (used + rows / 16), cus = device_cus();
+    if (rows <= 6 * used || (rows <= 16 * used && tiles <= cus)) {
+      // Tiles of 16 columns, whose rows of x are read twice as often, for idle units, and for long
+      // reductions with very few rows (32 / 16 columns): 64 rows in 8 groups of 512 x 1280 5.9 / 4.9, 96 6.1 /
+      // 6.8; 8 in 8 of 5632 x 2048 33 / 28, 32 34 / 31; 32 in 8 of 7168 x 1472 30.5 / 32.5; 256 in 32 of
+      // 1024 x 2048 26 / 29.
+      return 4 * tiles <= 3 * cus || (k >= 2048 && rows <= 4 * used) ? kTileFew16 : kTileFew;
+    }
+  }
   int best = kTile256;
   float t = 0.0f;
   for (int tile = 0; tile < kFastTiles; ++tile) {
@@ -126,7 +138,7 @@ int run_tile(const GroupedParams& p, int tile, int64_t grid, hipStream_t s) {
     case kTile64: return launch_ring<Ring64, BMODE>(p, grid, s);
   }
   if constexpr (BMODE == kKContig) {
-    hipLaunchKernelGGL(grouped_few_kernel, dim3((unsigned)grid), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(tile == kTileFew ? grouped_few_kernel<32> : grouped_few_kernel<16>, dim3((unsigned)grid), dim3(256), 0, s, p);
     return hip_check(hipGetLastError(), "grouped product launch");
   }
   return set_error(kInvalid, "no grouped tile %d", tile);
