@@ -536,12 +536,15 @@ int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, const int64
 /* y [rows, n] BF16 = x [rows, k] times the transpose of the group's weight [n, k] (WS_GROUPED_NT:
  * a projection; k a multiple of 8), or times its weight [k, n] itself (WS_GROUPED_NN: the input
  * gradient of one; n a multiple of 8), both row-major with row stride ld_weight, group_stride elements from one group's to the next. Rows
- * before the first offset and behind the last get zeros. The sums of the tiles have
- * one order, that of the kernel for few rows another. */
+ * before the first offset and behind the last get zeros. The sums of the tiles have one order, those
+ * of the kernel for few rows, and of long reductions that are cut in slices, another. `workspace`:
+ * 16-byte aligned, ws_grouped_workspace_floats (which follows the device's compute units; null if that
+ * is 0). */
 enum WsGroupedForm { WS_GROUPED_NT = 0, WS_GROUPED_NN = 1, WS_GROUPED_GRAD = 2 };
 int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int64_t ld_weight,
                   int64_t group_stride, int form, const int64_t* offsets, int64_t groups,
-                  int64_t rows, int64_t n, int64_t k, void* y, int64_t ldy, void* stream);
+                  int64_t rows, int64_t n, int64_t k, void* y, int64_t ldy, float* workspace, void* stream);
+int64_t ws_grouped_workspace_floats(int64_t rows, int64_t groups, int64_t n, int64_t k, int form);
 /* dweight [groups, n, k] (contiguous, BF16 or FP32) = the sums over each group's rows of
  * dy^T x, dy [rows, n] and x [rows, k]; a group without rows gets zeros. */
 int ws_grouped_weight_grad(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,

@@ -68,7 +68,7 @@ def _check(x, w, dy, offsets, y, dx=None, dw=None):
 # Rows, groups, n, k. The last five reach the pieces of a last round of 256 x 256 tiles (no whole
 # round before it, one, and a last round that is long enough to stay whole).
 SIZES = [(1, 1, 8, 8), (1, 5, 64, 72), (7, 3, 16, 200), (16, 64, 96, 264), (20, 8, 1288, 2056), (40, 8, 1288, 264),
-         (100, 8, 520, 264), (100, 9, 264, 1000), (200, 8, 520, 96),
+         (100, 8, 520, 264), (300, 16, 2056, 136), (100, 9, 264, 1000), (200, 8, 520, 96),
          (300, 4, 512, 512), (700, 70, 64, 64), (1000, 130, 128, 136), (1000, 5, 256, 128), (3000, 3, 2048, 512),
          (4096, 8, 1288, 1280), (4096, 64, 512, 1280), (6000, 32, 1280, 896), (8192, 4, 1280, 520),
          (2600, 2, 2056, 1544), (9000, 4, 2304, 1608), (9000, 4, 1608, 2304), (12000, 3, 2304, 1536),
@@ -94,13 +94,50 @@ def test_forward_and_backward(sizes, kind):
         assert torch.equal(grouped_mm(x, w, offsets.cuda()), y)
 
 
+# Rows, groups, n, k of products that are cut in slices of the reduction, forward or to x.
+SLICED = [(64, 2, 136, 2056), (100, 3, 72, 4000), (300, 2, 520, 3000), (513, 4, 264, 2304), (300, 3, 3000, 520),
+          (200, 1, 1288, 5000), (300, 16, 520, 2056), (539, 1, 728, 11720), (1154, 1, 10248, 360), (2373, 1, 8640, 256),
+          (100, 3, 4104, 2056), (90, 3, 2056, 136)]
+
+
+def test_every_tile_is_cut():
+    from ops import _hip
+
+    found = set()
+    for form in (NT, NN):
+        for r, g, n, k in SLICED:
+            sizes = (r, g, *((k, n) if form == NN else (n, k)), form)
+            if _hip.query("ws_grouped_workspace_floats", *sizes):
+                found.add((form, _hip.query("ws_grouped_tile", *sizes)))
+    assert {(NT, 2), (NT, 3), (NT, 4), (NN, 2), (NN, 3), (NN, 4)} <= found, found
+
+
+@pytest.mark.parametrize("kind", ["router", "gaps"])
+@pytest.mark.parametrize("sizes", SLICED)
+def test_slices(sizes, kind):
+    from ops import _hip
+    from ops.grouped_execution import grouped_mm
+
+    rows, groups, n, k = sizes
+    x, w, dy = _make(rows, groups, n, k, BF16, seed=rows + k)
+    assert max(_hip.query("ws_grouped_workspace_floats", rows, groups, n, k, NT),
+               _hip.query("ws_grouped_workspace_floats", rows, groups, k, n, NN)) > 0
+    offsets = _offsets(rows, groups, kind, seed=n)
+    x.requires_grad_(True)
+    y = grouped_mm(x, w, offsets.cuda())
+    dx, = torch.autograd.grad(y, x, dy)
+    _check(x.detach(), w, dy, offsets, y, dx)
+    again = grouped_mm(x, w, offsets.cuda())
+    assert torch.equal(y, again) and torch.equal(dx, torch.autograd.grad(again, x, dy)[0])
+
+
 def test_every_tile_is_reached():
     from ops import _hip
 
     found = {form: {_hip.query("ws_grouped_tile", r, g, *((k, n) if form == NN else (n, k)), form)
                     for r, g, n, k in SIZES} for form in (NT, NN, GRAD)}
-    assert {0, 1, 3, 4, 5, 6} <= found[NT], found
-    assert {0, 1, 3, 4} <= found[NN] and {0, 1, 3, 4} <= found[GRAD], found
+    assert {0, 1, 2, 3, 4, 5, 6} <= found[NT], found
+    assert {0, 1, 2, 3, 4} <= found[NN] and {0, 1, 3, 4} <= found[GRAD], found
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -175,7 +212,7 @@ def test_no_rows():
     assert y.shape == (0, 16) and dx.shape == (0, 24) and not dw.any()
 
 
-@pytest.mark.parametrize("sizes", [(16, 6, 64, 256), (300, 6, 264, 256), (5000, 6, 512, 256)])
+@pytest.mark.parametrize("sizes", [(16, 6, 64, 256), (300, 6, 264, 256), (5000, 6, 512, 256), (150, 6, 264, 4096)])
 def test_any_offsets_stay_inside(sizes):
     """Values that name rows that there are not, or name them twice, change no memory but the
     result's; rows behind y and beside it stay as they were."""
@@ -185,15 +222,19 @@ def test_any_offsets_stay_inside(sizes):
     x, w, dy = _make(rows, groups, n, k)
     wide = torch.full((rows + 2, n + 16), 7.0, dtype=BF16, device="cuda")
     dw = torch.full((groups + 1, n, k), 7.0, device="cuda")
+    need = _hip.query_on(x, "ws_grouped_workspace_floats", rows, groups, n, k, NT)
+    assert (need > 0) == (k == 4096)
+    work = torch.full((need + 64,), 7.0, device="cuda")
     for values in ([0, 5, 3, rows, rows + 9, 2 ** 40, -4], [-2 ** 62] * 7, [2 ** 62] * 7,
                    [rows, 0, rows, 0, rows, 0, rows], [3] * 7):
         offsets = torch.tensor(values, device="cuda")
         _hip.call_on(x, "ws_grouped_mm", x.data_ptr(), k, w.data_ptr(), k, n * k, NT, offsets.data_ptr(),
-                     groups, rows, n, k, wide[1:, 8:].data_ptr(), n + 16)
+                     groups, rows, n, k, wide[1:, 8:].data_ptr(), n + 16, work.data_ptr())
         _hip.call_on(x, "ws_grouped_weight_grad", dy.data_ptr(), n, x.data_ptr(), k, offsets.data_ptr(),
                      groups, rows, n, k, dw.data_ptr(), 1)
         assert (wide[0] == 7).all() and (wide[rows + 1] == 7).all()
         assert (wide[:, :8] == 7).all() and (wide[:, n + 8:] == 7).all() and (dw[groups] == 7).all()
+        assert (work[need:] == 7).all()
 
 
 def test_bad_values_stay_in_their_group():

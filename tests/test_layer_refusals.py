@@ -60,6 +60,10 @@ def test_add_rmsnorm_backward_arguments(change, match):
 
 
 def test_partial_floats_of_bad_sizes():
+    assert _hip.query("ws_grouped_workspace_floats", 0, 2, 16, 2048, 0) == 0
+    assert _hip.query("ws_grouped_workspace_floats", 100, 2, 16, 2048, 2) == 0
+    assert _hip.query("ws_grouped_workspace_floats", 100, 2, 13, 2048, 0) % (100 * 16) == 0
+    assert _hip.query("ws_grouped_workspace_floats", 100, 2, 13, 2048, 0) > 0
     assert _hip.query("ws_add_rmsnorm_backward_partial_floats", 0, 8) == 0
     assert _hip.query("ws_add_rmsnorm_backward_partial_floats", 4, 8193) == 0
     assert _hip.query("ws_embedding_backward_workspace_bytes", -1, 8, 8) == 0
@@ -96,13 +100,14 @@ def test_embedding_backward_arguments(change, match):
     (dict(n=17), "overlap"), (dict(form=1, k=17), "overlap"), (dict(w=None), "null"), (dict(offsets=None), "null"), (dict(y=None), "null"), (dict(x=GPU + 8), "aligned"),
     (dict(ldx=20), "aligned"), (dict(ldx=8), "overlap"), (dict(ldw=8), "overlap"), (dict(ldy=8), "overlap"),
     (dict(stride=12), "aligned"), (dict(stride=-8), "aligned"), (dict(ldy=4200000), "stride"),
-    (dict(rows=2 ** 30, n=2 ** 20, ldy=2 ** 20), "tiles"), (dict(rows=2 ** 30 + 1), "shape")])
+    (dict(rows=2 ** 30, n=2 ** 20, ldy=2 ** 20), "tiles"), (dict(rows=2 ** 30 + 1), "shape"),
+    (dict(work=GPU + 4), "aligned"), (dict(rows=100, k=2048, ldx=2048, ldw=2048), "null")])
 def test_grouped_mm_arguments(change, match):
     a = dict(x=GPU, ldx=16, w=GPU, ldw=16, stride=256, form=0, offsets=GPU, groups=2, rows=4, n=16, k=16, y=GPU,
-             ldy=16) | change
+             ldy=16, work=None) | change
     with pytest.raises(RuntimeError, match=match):
         _hip.call("ws_grouped_mm", a["x"], a["ldx"], a["w"], a["ldw"], a["stride"], a["form"], a["offsets"],
-                  a["groups"], a["rows"], a["n"], a["k"], a["y"], a["ldy"], None)
+                  a["groups"], a["rows"], a["n"], a["k"], a["y"], a["ldy"], a["work"], None)
 
 
 @pytest.mark.parametrize("change,match", [

@@ -31,6 +31,8 @@ struct GroupedParams {
   int most;                     // tiles that the grid is sized for
   int pieces_most;              // a last round of at most so many 256 x 256 tiles goes in pieces
   unsigned short* c; long ldc;
+  int per;                      // k-tiles of a slice of the reduction (grouped_ring_kernel<SLICED>)
+  float* partial;               // [slices, rows, N]
 };
 
 struct GroupTile {
@@ -179,8 +181,41 @@ __global__ void __launch_bounds__(kFNT) grouped_fast_kernel(const GroupedParams 
   }
 }
 
-// Smaller tiles, one workgroup each.
-template <class Cfg, int BMODE>
+// The wave's accumulators as FP32 rows of out [M, N], through its LDS staging rows in two halves, so
+// that the stores cover whole lines; NT: they go around the caches. (Stored from the fragments, 64 bytes of
+// each of 16 rows at a time, and through them, a step of eight experts' 11264 x 2048 masters over
+// 16384 rows took 2000 us instead of 1960.)
+template <bool NT, int FA, int FB>
+__device__ __forceinline__ void store_f32(float* out, int M, int N, Acc16<FA, FB>& acc, int m_base, int n_base, int lane,
+                                          unsigned char* stage) {
+  constexpr int kRow = FB * 64 + 16, LPR = FB * 4, RPI = 64 / LPR, HA = FA / 2, NQ = HA * 16 / RPI;
+  static_assert(FA % 2 == 0 && 64 % LPR == 0 && NQ >= 1 && HA * 16 * kRow <= epi_wave<FA, FB>(), "half a tile is staged");
+  opaque_lane(lane);
+  __amdgpu_buffer_rsrc_t rg = make_rsrc(out + (long)m_base * N + n_base, 0x7fffffff);
+  const int c4 = 4 * (lane % LPR);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int i = 0; i < HA; ++i)
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+        *reinterpret_cast<f32x4_v*>(stage + (16 * i + (lane & 15)) * kRow + (16 * j + 4 * (lane >> 4)) * 4) =
+            acc.v[h * HA + i][j];
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's staging writes landed
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int r = RPI * q + lane / LPR, m = 16 * HA * h + r;
+      const bool ok = m_base + m < M && n_base + c4 + 3 < N;  // N is a multiple of 8
+      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + r * kRow + c4 * 4);
+      __builtin_amdgcn_raw_buffer_store_b128(v, rg, store_off(ok, (long)m * N + c4, 4), 0, NT ? kEpiNT : 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+// Smaller tiles, one workgroup each. SLICED: slice blockIdx.y of the reduction, in FP32, for
+// grouped_join_kernel.
+template <class Cfg, int BMODE, bool SLICED>
 __global__ void __launch_bounds__(Cfg::NT) grouped_ring_kernel(const GroupedParams p) {
   constexpr int FA = Cfg::FA, FB = Cfg::FB, TM = Cfg::TM, TN = Cfg::TN;
   extern __shared__ __attribute__((aligned(1024))) unsigned char rsmem[];
@@ -196,12 +231,39 @@ __global__ void __launch_bounds__(Cfg::NT) grouped_ring_kernel(const GroupedPara
   const int row0 = t.lo + tm * Cfg::BM, col0 = tn * Cfg::BN;
   OperandDesc b = p.b;
   b.ptr += max(t.group, 0) * p.b_group;
+  const int tiles = t.group < 0 ? 0 : cdiv(p.K, kFBK), kb = SLICED ? blockIdx.y * p.per : 0;
   Acc16<FA, FB> acc;
-  ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.b_rows, 0, p.K, 0,
-                                           t.group < 0 ? 0 : cdiv(p.K, kFBK), rsmem, wave, lane);
+  ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.b_rows, 0, p.K, kb,
+                                           SLICED ? min(tiles, kb + p.per) : tiles, rsmem, wave, lane);
+  if constexpr (SLICED) {
+    store_f32<false>(p.partial + (long)blockIdx.y * p.rows * p.N, t.hi, p.N, acc, row0 + wm * TM, col0 + wn * TN, lane,
+                     rsmem + wave * epi_wave<FA, FB>());
+    return;
+  }
   const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
   FEpiStore<false, false>::run(e, acc, row0 + wm * TM, col0 + wn * TN, lane, tm, tn, wn,
                                rsmem + wave * epi_wave<FA, FB>());
+}
+
+// The slices' sums in their order, eight columns a thread.
+static __global__ void __launch_bounds__(256) grouped_join_kernel(const float* partial, int slices, long rows, int N,
+                                                                  unsigned short* c, long ldc) {
+  const long at = (blockIdx.x * 256L + threadIdx.x) * 8, size = rows * N;
+  if (at >= size) return;
+  float sum[8] = {};
+#pragma unroll 4
+  for (int i = 0; i < slices; ++i) {
+    const f32x4_v* src = reinterpret_cast<const f32x4_v*>(partial + i * size + at);
+    const f32x4_v a = src[0], b = src[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sum[e] += a[e];
+      sum[4 + e] += b[e];
+    }
+  }
+  const long row = at / N;
+  *reinterpret_cast<u32x4_t*>(c + row * ldc + (at - row * N)) =
+      u32x4_t{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]), pack_bf16x2(sum[4], sum[5]), pack_bf16x2(sum[6], sum[7])};
 }
 
 // --------------------------------------------------------------------------------------
@@ -248,44 +310,12 @@ __device__ __forceinline__ GradTile grad_tile(const GroupedGradParams& p, int w,
   t.b = OperandDesc{p.b + lo * p.ldb, 1, p.ldb};
   return t;
 }
-// The wave's accumulators as FP32 rows of out [M, N], through its LDS staging rows in two halves, so
-// that the stores cover whole lines, and go around the caches. (Stored from the fragments, 64 bytes of
-// each of 16 rows at a time, and through them, a step of eight experts' 11264 x 2048 masters over
-// 16384 rows took 2000 us instead of 1960.)
-template <int FA, int FB>
-__device__ __forceinline__ void store_f32(float* out, int M, int N, Acc16<FA, FB>& acc, int m_base, int n_base, int lane,
-                                          unsigned char* stage) {
-  constexpr int kRow = FB * 64 + 16, LPR = FB * 4, RPI = 64 / LPR, HA = FA / 2, NQ = HA * 16 / RPI;
-  static_assert(FA % 2 == 0 && 64 % LPR == 0 && NQ >= 1 && HA * 16 * kRow <= epi_wave<FA, FB>(), "half a tile is staged");
-  opaque_lane(lane);
-  __amdgpu_buffer_rsrc_t rg = make_rsrc(out + (long)m_base * N + n_base, 0x7fffffff);
-  const int c4 = 4 * (lane % LPR);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int i = 0; i < HA; ++i)
-#pragma unroll
-      for (int j = 0; j < FB; ++j)
-        *reinterpret_cast<f32x4_v*>(stage + (16 * i + (lane & 15)) * kRow + (16 * j + 4 * (lane >> 4)) * 4) =
-            acc.v[h * HA + i][j];
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's staging writes landed
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int r = RPI * q + lane / LPR, m = 16 * HA * h + r;
-      const bool ok = m_base + m < M && n_base + c4 + 3 < N;  // N is a multiple of 8
-      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + r * kRow + c4 * 4);
-      __builtin_amdgcn_raw_buffer_store_b128(v, rg, store_off(ok, (long)m * N + c4, 4), 0, kEpiNT);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  }
-}
 template <bool F32, int FA, int FB>
 __device__ __forceinline__ void grad_store(const GroupedGradParams& p, const GradTile& t, Acc16<FA, FB>& acc, int m_base,
                                            int n_base, int lane, int wn, unsigned char* stage) {
   const long at = (long)t.group * p.M * p.N;
   if constexpr (F32) {
-    store_f32(static_cast<float*>(p.g) + at, p.M, p.N, acc, m_base, n_base, lane, stage);
+    store_f32<true>(static_cast<float*>(p.g) + at, p.M, p.N, acc, m_base, n_base, lane, stage);
   } else {
     const GemmParams e = store_params(static_cast<unsigned short*>(p.g) + at, p.N, p.M, p.N);
     FEpiStore<false, false>::run(e, acc, m_base, n_base, lane, t.tm, t.tn, wn, stage);

@@ -1,4 +1,6 @@
 // C ABI: products grouped by expert.
+#include <cmath>
+
 #include "../../include/warpstate_hip.h"
 #include "gemm_grouped.h"
 #include "launch.h"
@@ -13,6 +15,11 @@ constexpr int kTileFew = kFastTiles, kTileFew16 = kFastTiles + 1;
 // The most 256 x 256 tiles for 256 compute units whose round goes in pieces (grouped_fast_kernel).
 constexpr int kPiecesOf256 = 64;
 
+// The most slices of a reduction (never 256 x 256 tiles nor two 128 x 128 a unit, which others were faster than in
+// slices), and the least k-tiles of one.
+constexpr int kMaxSlices = 8, kSliceTiles = 4;
+
+int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 int tile_rows(int tile) {
   switch (tile) {
     case kTile256: return 256;
@@ -33,10 +40,16 @@ int64_t most_tiles(int64_t rows, int64_t groups, int bm) {
   return rows / bm + used;
 }
 
-// The tile for rows that are spread over the groups: by the cost table of single products, for the
+// The tile for rows that are spread over the groups, by the cost table of single products, for the
 // rows of the tiles that a group of average size makes (its last one is half full on average, and
-// there is one).
-int pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int bmode) {
+// there is one); and the slices of a long reduction whose tiles leave units idle (us, whole / in slices: 64 rows
+// in 2 groups of 2048 x 11264 50 / 25, 494 in 3 of 960 x 9704 46 / 29, 64 in 8 of 2048 x 5632 34 / 37). What is
+// added to the table was fitted to 440 drawn sizes: the choice is 3 % behind the best tile and slices, 2 % for
+// reductions up to 2048 (the table alone 19 and 5 %, the best tiles without slices 15 %).
+struct GroupedPlan {
+  int tile, slices;
+};
+GroupedPlan pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int bmode) {
   const int64_t used = groups < rows ? groups : rows;
   if (bmode == kKContig) {
     // Up to 6 rows for each group, above which some groups take two tiles of 16 (us, this kernel / the best
@@ -49,26 +62,42 @@ int pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int bmode) 
       // reductions with very few rows (32 / 16 columns): 64 rows in 8 groups of 512 x 1280 5.9 / 4.9, 96 6.1 /
       // 6.8; 8 in 8 of 5632 x 2048 33 / 28, 32 34 / 31; 32 in 8 of 7168 x 1472 30.5 / 32.5; 256 in 32 of
       // 1024 x 2048 26 / 29.
-      return 4 * tiles <= 3 * cus || (k >= 2048 && rows <= 4 * used) ? kTileFew16 : kTileFew;
+      return {4 * tiles <= 3 * cus || (k >= 2048 && rows <= 4 * used) ? kTileFew16 : kTileFew, 1};
     }
   }
-  int best = kTile256;
+  // Two workgroups on a unit with few stages hide less of what comes from HBM, one with more hides more.
+  static const float slower[kFastTiles] = {1.0f, 1.2f, 0.9f, 1.0f, 1.0f};
+  GroupedPlan best = {kTile256, 1};
   float t = 0.0f;
   for (int tile = 0; tile < kFastTiles; ++tile) {
-    const int64_t bm = tile_rows(tile);
+    const int64_t bm = tile_rows(tile), cus = device_cus();
     int64_t wide = rows + used * bm / 2;
     if (wide < used * bm) wide = used * bm;
-    float ti = tile_time(tile, wide, n, k, kKContig, bmode, device_cus(), false, kEpiStore);
-    if (tile == kTile256) {
-      const TileCost& c = tile_cost(tile, kKContig, bmode);
-      const int64_t tiles = cdiv(wide, 256) * (int64_t)cdiv(n, 256), cus = device_cus(), rest = tiles % cus;
-      const float kt = (float)cdiv(k, kFBK);
-      if (rest * 256 <= kPiecesOf256 * cus)
-        ti = (float)(tiles / cus) * (c.alone * kt + c.fixed) + (rest * 8 <= cus ? 0.45f : 0.62f) * kt + 4.0f;
-    }
-    if (tile == 0 || ti < t) {
-      best = tile;
-      t = ti;
+    // Many groups make some tiles more or fewer: a round that is just full is not counted on.
+    if (used >= 16) wide += (int64_t)(0.2f * (float)bm * std::sqrt((float)used));
+    // What the tiles read, each weight once for every tile of rows, at the caches' rate, and what HBM gives. (1000
+    // rows in 8 groups of 2048 x 5632: 64 x 128, by the table, 83 us, 128 x 128 61.)
+    const float fn = (float)n, fk = 2.0f * (float)k, frows = (float)rows, fused = (float)used;
+    float read = ((float)(rows / bm + used) * fn * fk + (float)cdiv(n, tile_cols(tile)) * frows * fk) / 12e6f;
+    const float once = (fused * fn * fk + frows * (2.0f * fn + fk)) / 7e6f;
+    if (read < once) read = once;
+    for (int slices = 1; slices <= (tile == kTile256 || tile == kTile128x2 ? 1 : kMaxSlices); slices *= 2) {
+      if (slices > 1 && k < (int64_t)slices * kSliceTiles * kFBK) break;
+      float ti = slower[tile] * tile_time(tile, wide, n, k, kKContig, bmode, cus, false, kEpiStore, slices);
+      if (tile == kTile256) {
+        const TileCost& c = tile_cost(tile, kKContig, bmode);
+        const int64_t tiles = cdiv(wide, 256) * (int64_t)cdiv(n, 256), rest = tiles % cus;
+        const float kt = (float)cdiv(k, kFBK);
+        if (rest * 256 <= kPiecesOf256 * cus)
+          ti = (float)(tiles / cus) * (c.alone * kt + c.fixed) + (rest * 8 <= cus ? 0.45f : 0.62f) * kt + 4.0f;
+      }
+      if (ti < read) ti = read;
+      // The second kernel, and the slices' sums there and back.
+      if (slices > 1) ti += 4.0f + frows * fn * (float)(8 * slices) / 4e6f;
+      if ((tile == 0 && slices == 1) || ti < t) {
+        best = {tile, slices};
+        t = ti;
+      }
     }
   }
   return best;
@@ -101,7 +130,6 @@ int check_sizes(int64_t groups, int64_t rows, int64_t n, int64_t k) {
 int check_width(int64_t width) {
   return width % 8 == 0 ? kOk : set_error(kInvalid, "grouped products take weight rows of a multiple of 8, not %ld", (long)width);
 }
-int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 // Rows of whole, aligned 16-byte pieces, 256 of which span less than 2 GiB.
 int check_rows(const void* p, int64_t ld, int64_t rows, int64_t cols, const char* what) {
   if (!al(p, 16) || ld % 8 != 0) return set_error(kInvalid, "%s rows must be 16-byte aligned", what);
@@ -109,12 +137,19 @@ int check_rows(const void* p, int64_t ld, int64_t rows, int64_t cols, const char
   return check_out_stride(ld > cols ? ld : cols, 2, what);
 }
 
-template <class Cfg, int BMODE>
-int launch_ring(const GroupedParams& p, int64_t grid, hipStream_t s) {
-  const void* kern = reinterpret_cast<const void*>(&grouped_ring_kernel<Cfg, BMODE>);
-  if (int rc = ensure_lds(kern, Cfg::kLds)) return rc;
-  hipLaunchKernelGGL((grouped_ring_kernel<Cfg, BMODE>), dim3((unsigned)grid), dim3(Cfg::NT), Cfg::kLds, s, p);
-  return hip_check(hipGetLastError(), "grouped product launch");
+template <class Cfg, int BMODE, bool CUT = true>
+int launch_ring(const GroupedParams& p, int slices, int64_t grid, hipStream_t s) {
+  auto run = [&](auto kernel) {
+    if (int rc = ensure_lds(reinterpret_cast<const void*>(kernel), Cfg::kLds)) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid, slices), dim3(Cfg::NT), Cfg::kLds, s, p);
+    return hip_check(hipGetLastError(), "grouped product launch");
+  };
+  if constexpr (!CUT) return run(&grouped_ring_kernel<Cfg, BMODE, false>);
+  if (slices == 1) return run(&grouped_ring_kernel<Cfg, BMODE, false>);
+  if (int rc = run(&grouped_ring_kernel<Cfg, BMODE, CUT>)) return rc;
+  hipLaunchKernelGGL(grouped_join_kernel, dim3((unsigned)cdiv((int64_t)p.rows * p.N, 2048)), dim3(256), 0, s, p.partial, slices,
+                     (long)p.rows, p.N, p.c, p.ldc);
+  return hip_check(hipGetLastError(), "grouped product join launch");
 }
 template <int BMODE>
 int launch_whole(GroupedParams p, int64_t grid, hipStream_t s) {
@@ -129,13 +164,14 @@ int launch_whole(GroupedParams p, int64_t grid, hipStream_t s) {
   return hip_check(hipGetLastError(), "grouped product launch");
 }
 template <int BMODE>
-int run_tile(const GroupedParams& p, int tile, int64_t grid, hipStream_t s) {
+int run_tile(const GroupedParams& p, GroupedPlan plan, int64_t grid, hipStream_t s) {
+  const int tile = plan.tile, slices = plan.slices;
   switch (tile) {
     case kTile256: return launch_whole<BMODE>(p, grid, s);
-    case kTile128x2: return launch_ring<Ring128x2, BMODE>(p, grid, s);
-    case kTile128x1: return launch_ring<Ring128x1, BMODE>(p, grid, s);
-    case kTile64x128: return launch_ring<Ring64x128, BMODE>(p, grid, s);
-    case kTile64: return launch_ring<Ring64, BMODE>(p, grid, s);
+    case kTile128x2: return launch_ring<Ring128x2, BMODE, false>(p, 1, grid, s);
+    case kTile128x1: return launch_ring<Ring128x1, BMODE>(p, slices, grid, s);
+    case kTile64x128: return launch_ring<Ring64x128, BMODE>(p, slices, grid, s);
+    case kTile64: return launch_ring<Ring64, BMODE>(p, slices, grid, s);
   }
   if constexpr (BMODE == kKContig) {
     hipLaunchKernelGGL(tile == kTileFew ? grouped_few_kernel<32> : grouped_few_kernel<16>, dim3((unsigned)grid), dim3(256), 0, s, p);
@@ -159,16 +195,22 @@ int launch_grad_ring(const GroupedGradParams& p, bool f32, int64_t grid, hipStre
 extern "C" int ws_grouped_tile(int64_t rows, int64_t groups, int64_t n, int64_t k, int form) {
   if (rows < 1 || check_sizes(groups, rows, n, k)) return -1;
   switch (form) {
-    case WS_GROUPED_NT: return pick_grouped(rows, groups, n, k, kKContig);
-    case WS_GROUPED_NN: return pick_grouped(rows, groups, n, k, kMNContig);
+    case WS_GROUPED_NT: return pick_grouped(rows, groups, n, k, kKContig).tile;
+    case WS_GROUPED_NN: return pick_grouped(rows, groups, n, k, kMNContig).tile;
     case WS_GROUPED_GRAD: return pick_grad(rows, groups, n, k);
   }
   return -1;
 }
 
+extern "C" int64_t ws_grouped_workspace_floats(int64_t rows, int64_t groups, int64_t n, int64_t k, int form) {
+  if (rows < 1 || check_sizes(groups, rows, n, k) || (form != WS_GROUPED_NT && form != WS_GROUPED_NN)) return 0;
+  const int slices = pick_grouped(rows, groups, n, k, form == WS_GROUPED_NT ? kKContig : kMNContig).slices;
+  return slices > 1 ? slices * rows * up8(n) : 0;
+}
+
 extern "C" int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int64_t ld_weight, int64_t group_stride,
                              int form, const int64_t* offsets, int64_t groups, int64_t rows, int64_t n, int64_t k,
-                             void* y, int64_t ldy, void* stream) {
+                             void* y, int64_t ldy, float* workspace, void* stream) {
   if (form != WS_GROUPED_NT && form != WS_GROUPED_NN) return set_error(kInvalid, "unknown form %d", form);
   if (int rc = check_sizes(groups, rows, n, k)) return rc;
   if (rows == 0) return kOk;
@@ -180,8 +222,13 @@ extern "C" int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int
   if (int rc = check_rows(weight, ld_weight, 2, nt ? k : n, "weight")) return rc;
   if (int rc = check_rows(y, ldy, rows, wide, "y")) return rc;
   if (group_stride % 8 != 0 || group_stride < 0) return set_error(kInvalid, "weights must be 16-byte aligned");
-  const int tile = pick_grouped(rows, groups, n, k, nt ? kKContig : kMNContig);
+  const GroupedPlan plan = pick_grouped(rows, groups, n, k, nt ? kKContig : kMNContig);
+  const int tile = plan.tile;
+  if (plan.slices > 1 && !workspace) return set_error(kInvalid, "null pointer");
+  if (!al(workspace, 16)) return set_error(kInvalid, "the workspace must be 16-byte aligned");
   GroupedParams p{};
+  p.per = cdiv(cdiv(k, kFBK), plan.slices);
+  p.partial = workspace;
   p.a = OperandDesc{static_cast<const unsigned short*>(x), ldx, 1};
   p.b = OperandDesc{static_cast<const unsigned short*>(weight), nt ? ld_weight : 1, nt ? 1 : ld_weight};
   p.b_group = group_stride;
@@ -198,7 +245,7 @@ extern "C" int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int
   if (grid >= 1L << 22) return set_error(kInvalid, "too many tiles (%ld rows, %ld columns, %ld groups)", (long)rows, (long)n, (long)groups);
   p.most = (int)grid;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return nt ? run_tile<kKContig>(p, tile, grid, s) : run_tile<kMNContig>(p, tile, grid, s);
+  return nt ? run_tile<kKContig>(p, plan, grid, s) : run_tile<kMNContig>(p, plan, grid, s);
 }
 
 extern "C" int ws_grouped_weight_grad(const void* dy, int64_t ld_dy, const void* x, int64_t ldx, const int64_t* offsets,

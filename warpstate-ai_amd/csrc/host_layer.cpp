@@ -356,9 +356,11 @@ Tensor grouped_rows(const Tensor& x, const Tensor& w, const Tensor& offsets_in, 
   const bool nt = form == WS_GROUPED_NT;
   const int64_t rows = x.size(0), n = w.size(nt ? 1 : 2), k = w.size(nt ? 2 : 1);
   Tensor y = at::empty({rows, up(n, 8)}, x.options());
+  const int64_t need = ws_grouped_workspace_floats(rows, w.size(0), n, k, (int)form);
+  Tensor work = need ? floats(x, {need}) : Tensor();
   check(ws_grouped_mm(ptr(x), row_stride(x), w.const_data_ptr(), w.size(1) > 1 ? w.stride(1) : w.size(2),
                       w.size(0) > 1 ? w.stride(0) : 0, (int)form, offsets.const_data_ptr<int64_t>(), w.size(0), rows,
-                      n, k, ptr(y), y.size(1), stream_of(x)),
+                      n, k, ptr(y), y.size(1), static_cast<float*>(ptr(work)), stream_of(x)),
         "ws_grouped_mm");
   return y;
 }

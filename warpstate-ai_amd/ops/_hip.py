@@ -119,7 +119,8 @@ SIGNATURES = {
     "ws_embedding_backward": (_i32, [_c_void_p, _i64, _i32, _c_void_p, _i64, _i64, _i64, _f32,
                                      _c_void_p, _i64, _i32, _c_void_p, _c_void_p]),
     "ws_grouped_mm": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _i64, _i32, _c_void_p, _i64, _i64,
-                             _i64, _i64, _c_void_p, _i64, _c_void_p]),
+                             _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p]),
+    "ws_grouped_workspace_floats": (_i64, [_i64, _i64, _i64, _i64, _i32]),
     "ws_grouped_weight_grad": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64,
                                       _i64, _i64, _c_void_p, _i32, _c_void_p]),
     "ws_copy_rows": (_i32, [_c_void_p, _i32] + [_i64] * 4 + [_c_void_p, _i32] + [_i64] * 5 + [_c_void_p]),

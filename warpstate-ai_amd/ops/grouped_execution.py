@@ -82,9 +82,12 @@ def _product(x: Tensor, w: Tensor, offsets: Tensor, form: int) -> Tensor:
     if form == _NN:
         n, k = k, n
     y = torch.empty((rows, _up(n)), dtype=BF16, device=x.device)
+    need = _hip.query_on(x, "ws_grouped_workspace_floats", rows, groups, n, k, form)
+    work = torch.empty((need,), dtype=F32, device=x.device) if need else None
     _hip.call_on(x, "ws_grouped_mm", x.data_ptr(), _row_stride(x), w.data_ptr(),
                  w.stride(1) if w.shape[1] > 1 else w.shape[2], w.stride(0) if groups > 1 else 0,
-                 form, offsets.data_ptr(), groups, rows, n, k, y.data_ptr(), y.shape[1])
+                 form, offsets.data_ptr(), groups, rows, n, k, y.data_ptr(), y.shape[1],
+                 _hip.ptr(work))
     return y
 
 
