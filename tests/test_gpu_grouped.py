@@ -94,6 +94,29 @@ def test_forward_and_backward(sizes, kind):
         assert torch.equal(grouped_mm(x, w, offsets.cuda()), y)
 
 
+@pytest.mark.parametrize("sizes", [(900, 4500, 24, 40), (600, 300, 200, 136), (5000, 200, 72, 520), (2000, 1500, 264, 40),
+                                   (7001, 400, 520, 72), (3000, 64, 2056, 24), (20000, 4, 40, 264)])
+def test_many_groups(sizes):
+    """More groups than lanes, and more than 64 on a lane; short reductions, of which a workgroup takes
+    several tiles."""
+    from ops.grouped_execution import grouped_mm
+
+    rows, groups, n, k = sizes
+    x, w, dy = _make(rows, groups, n, k, seed=rows)
+    for kind in ("gaps", "router"):
+        offsets = _offsets(rows, groups, kind, seed=n)
+        owner = torch.bucketize(torch.arange(rows), offsets, right=True) - 1  # -1 or groups: none
+        owner[owner == groups] = -1
+        x.requires_grad_(True)
+        y = grouped_mm(x, w, offsets.cuda())
+        dx, = torch.autograd.grad(y, x, dy)
+        x.requires_grad_(False)
+        mine = w[owner.clamp_min(0).cuda()].to(F64) * (owner >= 0).cuda()[:, None, None]
+        a, g = x.to(F64)[:, None], dy.to(F64)[:, None]
+        _close(y, (a * mine).sum(2), (a * mine).abs().sum(2), k)
+        _close(dx, (g.mT * mine).sum(1), (g.mT * mine).abs().sum(1), n)
+
+
 # Rows, groups, n, k of products that are cut in slices of the reduction, forward or to x.
 SLICED = [(64, 2, 136, 2056), (100, 3, 72, 4000), (300, 2, 520, 3000), (513, 4, 264, 2304), (300, 3, 3000, 520),
           (200, 1, 1288, 5000), (300, 16, 520, 2056), (539, 1, 728, 11720), (1154, 1, 10248, 360), (2373, 1, 8640, 256),

@@ -5,7 +5,7 @@
 //
 // The offsets are on the device and the host knows only their number, so the grid is sized for
 // the most tiles that any offsets make, and a workgroup finds its tile from them: every wave
-// runs over the groups, a group on a lane, with a running sum of their tiles, and takes the group
+// runs over the groups, one or more on a lane, with a running sum of their tiles, and takes the group
 // whose tiles hold its index. Offsets are clamped to [0, rows]: whatever they hold, no access leaves the
 // operands. Rows before the first offset and behind the last form two groups without a
 // product, and get zeros.
@@ -28,6 +28,8 @@ struct GroupedParams {
   const long* offsets;          // [groups + 1]
   int groups, rows, N, K, tiles_n;
   int b_rows;                   // columns of the product that the weight has; those up to N get zeros
+  int chunk;                    // groups on each of 64 lanes
+  int run;                      // tiles of a workgroup, one after the other (not 256 x 256)
   int most;                     // tiles that the grid is sized for
   int pieces_most;              // a last round of at most so many 256 x 256 tiles goes in pieces
   unsigned short* c; long ldc;
@@ -41,56 +43,94 @@ struct GroupTile {
   int index;     // the tile within the group
 };
 
-// Rows [lo, hi) of pseudo-group g: 0 before the first offset, 1 .. groups the groups, groups + 1
-// behind the last offset; empty beyond.
-__device__ __forceinline__ void group_rows(const long* offsets, int groups, int rows, int g, int& lo, int& hi) {
-  auto at = [&](int i) { return (int)min((long)rows, max(0L, offsets[i])); };
-  lo = g == 0 || g > groups + 1 ? 0 : at(g - 1);
-  hi = g > groups + 1 ? 0 : g == groups + 1 ? rows : at(g);
+__device__ __forceinline__ int group_offset(const GroupedParams& p, int g) {
+  return (int)min((long)p.rows, max(0L, p.offsets[min(g, p.groups)]));
 }
 
-// Pseudo-group g0 + lane's rows and tiles of BM rows, and the running sum of the tiles over the lanes.
+// A lane's groups, `chunk` from lane * chunk on: their tiles of BM rows (the grid's `most` at most), and
+// the running sum over the lanes. lo, hi: the rows where chunk is 1 (up to 64 groups).
 struct GroupLanes {
   int lo, hi, tiles, upto;
 };
-template <int BM>
-__device__ __forceinline__ GroupLanes group_lanes(const GroupedParams& p, int g0, int lane) {
-  GroupLanes v;
-  group_rows(p.offsets, p.groups, p.rows, g0 + lane, v.lo, v.hi);
-  v.tiles = v.hi > v.lo ? cdiv(v.hi - v.lo, BM) * p.tiles_n : 0;
-  v.upto = v.tiles;
+__device__ __forceinline__ int lanes_upto(int tiles, int lane) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int other = __shfl_up(v.upto, off, kWave);
-    if (lane >= off) v.upto += other;
+    const int other = __shfl_up(tiles, off, kWave);
+    if (lane >= off) tiles += other;
   }
+  return tiles;
+}
+template <int BM>
+__device__ __forceinline__ int row_tiles(const GroupedParams& p, int lo, int hi) {
+  return hi > lo ? cdiv(hi - lo, BM) * p.tiles_n : 0;
+}
+template <int BM>
+__device__ __forceinline__ GroupLanes group_lanes(const GroupedParams& p, int lane) {
+  GroupLanes v;
+  v.lo = group_offset(p, lane * p.chunk);  // past the last group: its end, twice
+  v.hi = v.tiles = 0;
+  if (p.chunk == 1) {
+    v.hi = group_offset(p, lane + 1);
+    v.tiles = row_tiles<BM>(p, v.lo, v.hi);
+  } else {
+    constexpr int kAhead = 8;
+    int lo = v.lo;
+    for (int b = 0; b < p.chunk; b += kAhead) {
+      int hi[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) hi[a] = group_offset(p, lane * p.chunk + b + a + 1);
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        if (b + a < p.chunk) v.tiles = min(p.most, v.tiles + row_tiles<BM>(p, lo, hi[a]));
+        lo = hi[a];
+      }
+    }
+  }
+  v.upto = lanes_upto(v.tiles, lane);
   return v;
 }
 
-// The tiles that there are, `most` at most (what offsets that do not decrease make), and the groups
-// of the first 64 lanes.
+// The tiles that there are, `most` at most (what offsets that do not decrease make): the groups', those of the
+// rows before the first offset and of those behind the last.
 template <int BM>
 __device__ __forceinline__ int count_tiles(const GroupedParams& p, int lane, GroupLanes& v) {
-  v = group_lanes<BM>(p, 0, lane);
-  int total = min(p.most, __builtin_amdgcn_readlane(v.upto, 63));
-  for (int g0 = 64; g0 < p.groups + 2; g0 += 64)
-    total = min(p.most, total + __builtin_amdgcn_readlane(group_lanes<BM>(p, g0, lane).upto, 63));
-  return total;
+  v = group_lanes<BM>(p, lane);
+  return min(p.most, __builtin_amdgcn_readlane(v.upto, 63) + row_tiles<BM>(p, 0, group_offset(p, 0)) +
+                         row_tiles<BM>(p, group_offset(p, p.groups), p.rows));
 }
 
 // The tile at index w, below count_tiles' total.
 template <int BM>
 __device__ __forceinline__ GroupTile find_tile(const GroupedParams& p, int w, int lane, GroupLanes v) {
-  for (int g0 = 0;; v = group_lanes<BM>(p, g0, lane)) {
-    const unsigned long past = __builtin_amdgcn_ballot_w64(w < v.upto);
-    if (past != 0) {
-      const int l = __builtin_ctzl(past), g = g0 + l;
-      return GroupTile{g == 0 || g == p.groups + 1 ? -1 : g - 1, __builtin_amdgcn_readlane(v.lo, l),
-                       __builtin_amdgcn_readlane(v.hi, l), w - __builtin_amdgcn_readlane(v.upto - v.tiles, l)};
-    }
-    w -= __builtin_amdgcn_readlane(v.upto, 63);
-    g0 += 64;
+  const int grouped = __builtin_amdgcn_readlane(v.upto, 63);
+  if (w >= grouped) {
+    w -= grouped;
+    const int first = group_offset(p, 0), before = row_tiles<BM>(p, 0, first);
+    return w < before ? GroupTile{-1, 0, first, w} : GroupTile{-1, group_offset(p, p.groups), p.rows, w - before};
   }
+  int l = __builtin_ctzl(__builtin_amdgcn_ballot_w64(w < v.upto)), base = 0;
+  if (p.chunk > 1) {  // the same over the groups of that lane, 64 at a time
+    w -= __builtin_amdgcn_readlane(v.upto - v.tiles, l);
+    base = l * p.chunk;
+    for (const int end = base + p.chunk;; base += 64) {
+      v.lo = group_offset(p, base + lane);
+      v.hi = group_offset(p, base + lane + 1);
+      v.tiles = base + lane < end ? row_tiles<BM>(p, v.lo, v.hi) : 0;
+      v.upto = lanes_upto(v.tiles, lane);
+      const unsigned long past = __builtin_amdgcn_ballot_w64(w < v.upto);
+      l = past != 0 ? __builtin_ctzl(past) : 0;
+      if (past != 0 || base + 64 >= end) break;
+      w -= __builtin_amdgcn_readlane(v.upto, 63);
+    }
+  }
+  return GroupTile{base + l, __builtin_amdgcn_readlane(v.lo, l), __builtin_amdgcn_readlane(v.hi, l),
+                   w - __builtin_amdgcn_readlane(v.upto - v.tiles, l)};
+}
+// The tile after t.
+template <int BM>
+__device__ __forceinline__ GroupTile next_tile(const GroupedParams& p, GroupTile t, int w, int lane) {
+  if (++t.index < row_tiles<BM>(p, t.lo, t.hi)) return t;
+  return find_tile<BM>(p, w, lane, group_lanes<BM>(p, lane));
 }
 
 // What the epilogues read of a GEMM's parameters.
@@ -109,7 +149,7 @@ template <class Cfg, int BMODE>
 __device__ __forceinline__ void grouped_piece(const GroupedParams& p, int whole, int x, unsigned char* smem, int lane,
                                               int wave) {
   constexpr int kAcross = kFBN / Cfg::BN, kPieces = kFBM / Cfg::BM * kAcross;
-  const GroupTile t = find_tile<kFBM>(p, whole + x / kPieces, lane, group_lanes<kFBM>(p, 0, lane));
+  const GroupTile t = find_tile<kFBM>(p, whole + x / kPieces, lane, group_lanes<kFBM>(p, lane));
   int tm, tn;
   tile_position(t.index, cdiv(t.hi - t.lo, kFBM), p.tiles_n, tm, tn);
   const int piece = x % kPieces;
@@ -151,7 +191,7 @@ __global__ void __launch_bounds__(kFNT) grouped_fast_kernel(const GroupedParams 
     // The groups are read again for each tile: kept over the k-loop they would cost it registers.
     int l = lane;
     opaque_lane(l);
-    const GroupTile t = find_tile<kFBM>(p, xcd_remap(w, whole, gridDim.x), l, group_lanes<kFBM>(p, 0, l));
+    const GroupTile t = find_tile<kFBM>(p, xcd_remap(w, whole, gridDim.x), l, group_lanes<kFBM>(p, l));
     int tm, tn;
     tile_position(t.index, cdiv(t.hi - t.lo, kFBM), p.tiles_n, tm, tn);
     const int row0 = t.lo + tm * kFBM, col0 = tn * kFBN;
@@ -223,26 +263,33 @@ __global__ void __launch_bounds__(Cfg::NT) grouped_ring_kernel(const GroupedPara
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
   GroupLanes v;
-  const int total = count_tiles<Cfg::BM>(p, lane, v);
-  if ((int)blockIdx.x >= total) return;
-  const GroupTile t = find_tile<Cfg::BM>(p, xcd_remap(blockIdx.x, total, kRingWindow), lane, v);
-  int tm, tn;
-  tile_position(t.index, cdiv(t.hi - t.lo, Cfg::BM), p.tiles_n, tm, tn);
-  const int row0 = t.lo + tm * Cfg::BM, col0 = tn * Cfg::BN;
-  OperandDesc b = p.b;
-  b.ptr += max(t.group, 0) * p.b_group;
-  const int tiles = t.group < 0 ? 0 : cdiv(p.K, kFBK), kb = SLICED ? blockIdx.y * p.per : 0;
-  Acc16<FA, FB> acc;
-  ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.b_rows, 0, p.K, kb,
-                                           SLICED ? min(tiles, kb + p.per) : tiles, rsmem, wave, lane);
-  if constexpr (SLICED) {
-    store_f32<false>(p.partial + (long)blockIdx.y * p.rows * p.N, t.hi, p.N, acc, row0 + wm * TM, col0 + wn * TN, lane,
-                     rsmem + wave * epi_wave<FA, FB>());
-    return;
+  const int total = count_tiles<Cfg::BM>(p, lane, v), blocks = cdiv(total, p.run);
+  if ((int)blockIdx.x >= blocks) return;
+  int w = xcd_remap(blockIdx.x, blocks, kRingWindow) * p.run;
+  const int end = min(total, w + p.run);
+  GroupTile t = find_tile<Cfg::BM>(p, w, lane, v);
+  while (true) {
+    int tm, tn;
+    tile_position(t.index, cdiv(t.hi - t.lo, Cfg::BM), p.tiles_n, tm, tn);
+    const int row0 = t.lo + tm * Cfg::BM, col0 = tn * Cfg::BN;
+    OperandDesc b = p.b;
+    b.ptr += max(t.group, 0) * p.b_group;
+    const int tiles = t.group < 0 ? 0 : cdiv(p.K, kFBK), kb = SLICED ? blockIdx.y * p.per : 0;
+    Acc16<FA, FB> acc;
+    ring_k_loop<Cfg, kKContig, BMODE, false>(acc, p.a, row0, t.hi, b, col0, p.b_rows, 0, p.K, kb,
+                                             SLICED ? min(tiles, kb + p.per) : tiles, rsmem, wave, lane);
+    if constexpr (SLICED) {
+      store_f32<false>(p.partial + (long)blockIdx.y * p.rows * p.N, t.hi, p.N, acc, row0 + wm * TM, col0 + wn * TN, lane,
+                       rsmem + wave * epi_wave<FA, FB>());
+    } else {
+      const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
+      FEpiStore<false, false>::run(e, acc, row0 + wm * TM, col0 + wn * TN, lane, tm, tn, wn,
+                                   rsmem + wave * epi_wave<FA, FB>());
+    }
+    if (SLICED || ++w >= end) return;
+    __builtin_amdgcn_s_barrier();  // the next tile's loads go where the staging was
+    t = next_tile<Cfg::BM>(p, t, w, lane);
   }
-  const GemmParams e = store_params(p.c, p.ldc, t.hi, p.N);
-  FEpiStore<false, false>::run(e, acc, row0 + wm * TM, col0 + wn * TN, lane, tm, tn, wn,
-                               rsmem + wave * epi_wave<FA, FB>());
 }
 
 // The slices' sums in their order, eight columns a thread.
@@ -277,6 +324,11 @@ struct GroupedGradParams {
   void* g;                      // [groups, M, N], BF16 or FP32
 };
 
+__device__ __forceinline__ void grad_rows(const GroupedGradParams& p, int g, int& lo, int& hi) {
+  auto at = [&](int i) { return (int)min((long)p.rows, max(0L, p.offsets[i])); };
+  lo = at(g);
+  hi = at(g + 1);
+}
 struct GradTile {
   OperandDesc a, b;
   int group, K, tm, tn;
@@ -289,7 +341,7 @@ constexpr int kOrdered = 16;
 __device__ __forceinline__ int grad_order(const GroupedGradParams& p, int lane) {
   if (p.groups > kOrdered) return lane;
   int lo = 0, hi = 0;
-  if (lane < p.groups) group_rows(p.offsets, p.groups, p.rows, lane + 1, lo, hi);
+  if (lane < p.groups) grad_rows(p, lane, lo, hi);
   const int rows = max(0, hi - lo);
   int rank = lane < p.groups ? 0 : lane;
   for (int j = 0; j < p.groups; ++j) {
@@ -304,7 +356,7 @@ __device__ __forceinline__ GradTile grad_tile(const GroupedGradParams& p, int w,
   t.group = p.groups > kOrdered ? place : __builtin_amdgcn_readlane(order, place);
   tile_position(w - place * per, p.tiles_m, p.tiles_n, t.tm, t.tn);
   int lo, hi;
-  group_rows(p.offsets, p.groups, p.rows, t.group + 1, lo, hi);
+  grad_rows(p, t.group, lo, hi);
   t.K = max(0, hi - lo);
   t.a = OperandDesc{p.a + lo * p.lda, 1, p.lda};
   t.b = OperandDesc{p.b + lo * p.ldb, 1, p.ldb};
@@ -376,73 +428,82 @@ __global__ void __launch_bounds__(Cfg::NT) grouped_grad_ring_kernel(const Groupe
 // (32 rows in 8 groups of 5632 x 2048, launch order and four / these 40 / 34 us, 40 rows in 8 of 2048 x 8192 61 / 50).
 constexpr int kFewRows = 16;
 
-template <int COLS>
+// RUN: p.run tiles of a workgroup, for which the registers leave fewer of them.
+template <int COLS, bool RUN>
 static __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedParams p) {
   constexpr int BM = kFewRows, NJ = COLS / 16;
   __shared__ float sums[4][BM][COLS + 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   GroupLanes v;
-  const int total = count_tiles<BM>(p, lane, v);
-  if ((int)blockIdx.x >= total) return;
-  const GroupTile t = find_tile<BM>(p, xcd_remap(blockIdx.x, total, kRingWindow), lane, v);
-  const int tm = t.index / p.tiles_n, tn = t.index - tm * p.tiles_n;
-  const int row0 = t.lo + tm * BM, col0 = tn * COLS;
-  f32x4_v acc[NJ];
+  const int total = count_tiles<BM>(p, lane, v), run = RUN ? p.run : 1, blocks = cdiv(total, run);
+  if ((int)blockIdx.x >= blocks) return;
+  int w = xcd_remap(blockIdx.x, blocks, kRingWindow) * run;
+  const int end = min(total, w + run);
+  GroupTile t = find_tile<BM>(p, w, lane, v);
+  while (true) {
+    const int tm = t.index / p.tiles_n, tn = t.index - tm * p.tiles_n;
+    const int row0 = t.lo + tm * BM, col0 = tn * COLS;
+    f32x4_v acc[NJ];
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) acc[j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
-  if (t.group >= 0) {
-    const int r = lane & 15, q = 8 * (lane >> 4);
-    const unsigned short* const a = p.a.ptr + (long)min(row0 + r, t.hi - 1) * p.a.s_row + q;
-    const unsigned short* b[NJ];
+    for (int j = 0; j < NJ; ++j) acc[j] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+    if (t.group >= 0) {
+      const int r = lane & 15, q = 8 * (lane >> 4);
+      const unsigned short* const a = p.a.ptr + (long)min(row0 + r, t.hi - 1) * p.a.s_row + q;
+      const unsigned short* b[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        b[j] = p.b.ptr + t.group * p.b_group + (long)min(col0 + 16 * j + r, p.b_rows - 1) * p.b.s_row + q;
+      // U k-tiles at a time, all of their pieces requested before the first product.
+      auto steps = [&](int k, auto count, auto load) {
+        constexpr int U = decltype(count)::value;
+        bf16x8_t fa[U][2], fb[U][2][NJ];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int at = k + 256 * u + 32 * s;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) fb[u][s][j] = load(b[j], at);
+            fa[u][s] = load(a, at);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+              acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[u][s][j], fa[u][s], acc[j], 0, 0, 0);
+      };
+      const auto whole = [](const unsigned short* row, int at) { return *reinterpret_cast<const bf16x8_t*>(row + at); };
+      constexpr int U = 2;
+      int k = 64 * wave;
+      for (; k + 256 * (U - 1) + 64 <= p.K; k += 256 * U) steps(k, std::integral_constant<int, U>{}, whole);
+      for (; k + 64 <= p.K; k += 256) steps(k, std::integral_constant<int, 1>{}, whole);
+      if (k < p.K)
+        steps(k, std::integral_constant<int, 1>{}, [&](const unsigned short* row, int at) {
+          bf16x8_t v = {};
+          if (at + q + 8 <= p.K) v = *reinterpret_cast<const bf16x8_t*>(row + at);
+          return v;
+        });
+    }
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
-      b[j] = p.b.ptr + t.group * p.b_group + (long)min(col0 + 16 * j + r, p.b_rows - 1) * p.b.s_row + q;
-    // U k-tiles at a time, all of their pieces requested before the first product.
-    auto steps = [&](int k, auto count, auto load) {
-      constexpr int U = decltype(count)::value;
-      bf16x8_t fa[U][2], fb[U][2][NJ];
+      *reinterpret_cast<f32x4_v*>(&sums[wave][lane & 15][16 * j + 4 * (lane >> 4)]) = acc[j];
+    __syncthreads();
+    const int m = threadIdx.x / (COLS / 2), n = 2 * (threadIdx.x % (COLS / 2));
+    if (m < BM) {
+      float v2[2];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const int at = k + 256 * u + 32 * s;
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) fb[u][s][j] = load(b[j], at);
-          fa[u][s] = load(a, at);
-        }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j)
-            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[u][s][j], fa[u][s], acc[j], 0, 0, 0);
-    };
-    const auto whole = [](const unsigned short* row, int at) { return *reinterpret_cast<const bf16x8_t*>(row + at); };
-    constexpr int U = 2;
-    int k = 64 * wave;
-    for (; k + 256 * (U - 1) + 64 <= p.K; k += 256 * U) steps(k, std::integral_constant<int, U>{}, whole);
-    for (; k + 64 <= p.K; k += 256) steps(k, std::integral_constant<int, 1>{}, whole);
-    if (k < p.K)
-      steps(k, std::integral_constant<int, 1>{}, [&](const unsigned short* row, int at) {
-        bf16x8_t v = {};
-        if (at + q + 8 <= p.K) v = *reinterpret_cast<const bf16x8_t*>(row + at);
-        return v;
-      });
+      for (int e = 0; e < 2; ++e)
+        v2[e] = (sums[0][m][n + e] + sums[1][m][n + e]) + (sums[2][m][n + e] + sums[3][m][n + e]);
+      if (row0 + m < t.hi && col0 + n < p.N)  // N is a multiple of 8
+        *reinterpret_cast<unsigned*>(p.c + (long)(row0 + m) * p.ldc + col0 + n) = pack_bf16x2(v2[0], v2[1]);
+    }
+    if (!RUN || ++w >= end) return;
+    __syncthreads();  // the sums have been read
+    t = next_tile<BM>(p, t, w, lane);
   }
-#pragma unroll
-  for (int j = 0; j < NJ; ++j)
-    *reinterpret_cast<f32x4_v*>(&sums[wave][lane & 15][16 * j + 4 * (lane >> 4)]) = acc[j];
-  __syncthreads();
-  const int m = threadIdx.x / (COLS / 2), n = 2 * (threadIdx.x % (COLS / 2));
-  if (m >= BM) return;
-  float v2[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-    v2[e] = (sums[0][m][n + e] + sums[1][m][n + e]) + (sums[2][m][n + e] + sums[3][m][n + e]);
-  if (row0 + m < t.hi && col0 + n < p.N)  // N is a multiple of 8
-    *reinterpret_cast<unsigned*>(p.c + (long)(row0 + m) * p.ldc + col0 + n) = pack_bf16x2(v2[0], v2[1]);
 }
 
 // --------------------------------------------------------------------------------------

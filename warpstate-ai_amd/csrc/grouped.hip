@@ -40,6 +40,13 @@ int64_t most_tiles(int64_t rows, int64_t groups, int bm) {
   return rows / bm + used;
 }
 
+// Tiles of a workgroup, one after the other: with a short reduction, finding one among the groups takes longer than
+// its product (us, one / several: 512 rows in 512 groups of 2048 x 16 135 / 34, 4096 in 256 of 2048 x 64 45 / 31).
+int tiles_of_run(int64_t tiles, int64_t k) {
+  const int64_t most = tiles / (4 * (int64_t)device_cus());
+  return k > 256 || most < 2 ? 1 : most < 16 ? (int)most : 16;
+}
+
 // The tile for rows that are spread over the groups, by the cost table of single products, for the
 // rows of the tiles that a group of average size makes (its last one is half full on average, and
 // there is one); and the slices of a long reduction whose tiles leave units idle (us, whole / in slices: 64 rows
@@ -141,7 +148,7 @@ template <class Cfg, int BMODE, bool CUT = true>
 int launch_ring(const GroupedParams& p, int slices, int64_t grid, hipStream_t s) {
   auto run = [&](auto kernel) {
     if (int rc = ensure_lds(reinterpret_cast<const void*>(kernel), Cfg::kLds)) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid, slices), dim3(Cfg::NT), Cfg::kLds, s, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(grid, p.run), slices), dim3(Cfg::NT), Cfg::kLds, s, p);
     return hip_check(hipGetLastError(), "grouped product launch");
   };
   if constexpr (!CUT) return run(&grouped_ring_kernel<Cfg, BMODE, false>);
@@ -174,7 +181,9 @@ int run_tile(const GroupedParams& p, GroupedPlan plan, int64_t grid, hipStream_t
     case kTile64: return launch_ring<Ring64, BMODE>(p, slices, grid, s);
   }
   if constexpr (BMODE == kKContig) {
-    hipLaunchKernelGGL(tile == kTileFew ? grouped_few_kernel<32> : grouped_few_kernel<16>, dim3((unsigned)grid), dim3(256), 0, s, p);
+    const auto kernel = p.run > 1 ? (tile == kTileFew ? grouped_few_kernel<32, true> : grouped_few_kernel<16, true>)
+                                  : (tile == kTileFew ? grouped_few_kernel<32, false> : grouped_few_kernel<16, false>);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(grid, p.run)), dim3(256), 0, s, p);
     return hip_check(hipGetLastError(), "grouped product launch");
   }
   return set_error(kInvalid, "no grouped tile %d", tile);
@@ -244,6 +253,8 @@ extern "C" int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int
   const int64_t grid = most_tiles(rows, groups, tile_rows(tile)) * p.tiles_n;
   if (grid >= 1L << 22) return set_error(kInvalid, "too many tiles (%ld rows, %ld columns, %ld groups)", (long)rows, (long)n, (long)groups);
   p.most = (int)grid;
+  p.chunk = cdiv(groups, 64);
+  p.run = tile == kTile256 || plan.slices > 1 ? 1 : tiles_of_run(grid, k);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return nt ? run_tile<kKContig>(p, plan, grid, s) : run_tile<kMNContig>(p, plan, grid, s);
 }
