@@ -195,7 +195,7 @@ _host_tried = False
 
 
 def host_ops():
-    """The operators of ``csrc/host_ops.cpp`` (``torch.ops.warpstate``), loaded once, or None
+    """The operators of ``csrc/host_ops.cpp`` and ``csrc/host_layer.cpp``, loaded once, or None
     where they are not built or belong to another PyTorch: their callers then allocate and
     launch from Python, with the same results for more host time. Where the kernels are built,
     that is warned about."""
