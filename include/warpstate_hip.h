@@ -527,7 +527,7 @@ int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, const int64
  * Rows sorted by expert: rows offsets[e] to offsets[e + 1] of x belong to group e (offsets: groups + 1
  * int64 on the device, not decreasing). The offsets are read on the device only, and no value of theirs
  * leads an access out of the operands; decreasing ones leave rows of the result unspecified. BF16
- * operands, FP32 sums, 16-byte aligned rows, weight rows of a multiple of 8 elements, 1 to 65536
+ * operands, FP32 sums, 16-byte aligned rows, weight rows of a multiple of 8 elements, 1 to 16384
  * groups, up to 2^30 rows. The other width, n below, may be any; rows of that width reach to its
  * next multiple of 8: y's are written up to there, and dy's, like x's under WS_GROUPED_NN, have
  * to hold zeros.

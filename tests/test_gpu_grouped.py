@@ -95,7 +95,8 @@ def test_forward_and_backward(sizes, kind):
 
 
 @pytest.mark.parametrize("sizes", [(900, 4500, 24, 40), (600, 300, 200, 136), (5000, 200, 72, 520), (2000, 1500, 264, 40),
-                                   (7001, 400, 520, 72), (3000, 64, 2056, 24), (20000, 4, 40, 264)])
+                                   (7001, 400, 520, 72), (3000, 64, 2056, 24), (20000, 4, 40, 264),
+                                   (16384, 16384, 16, 64)])
 def test_many_groups(sizes):
     """More groups than lanes, and more than 64 on a lane; short reductions, of which a workgroup takes
     several tiles."""

@@ -95,7 +95,7 @@ def test_embedding_backward_arguments(change, match):
 
 
 @pytest.mark.parametrize("change,match", [
-    (dict(form=2), "form"), (dict(groups=0), "groups"), (dict(groups=65537), "groups"), (dict(rows=-1), "shape"),
+    (dict(form=2), "form"), (dict(groups=0), "groups"), (dict(groups=16385), "groups"), (dict(rows=-1), "shape"),
     (dict(form=1, n=12), "multiple of 8"), (dict(k=12), "multiple of 8"), (dict(n=0), "shape"), (dict(x=None), "null"),
     (dict(n=17), "overlap"), (dict(form=1, k=17), "overlap"), (dict(w=None), "null"), (dict(offsets=None), "null"), (dict(y=None), "null"), (dict(x=GPU + 8), "aligned"),
     (dict(ldx=20), "aligned"), (dict(ldx=8), "overlap"), (dict(ldw=8), "overlap"), (dict(ldy=8), "overlap"),
@@ -115,7 +115,7 @@ def test_grouped_mm_arguments(change, match):
     (dict(n=17), "overlap"),
     (dict(x=None), "null"), (dict(offsets=None), "null"), (dict(dw=None), "null"), (dict(dw=GPU + 8), "aligned"),
     (dict(dy=GPU + 2), "aligned"), (dict(ldx=8), "overlap"), (dict(k=2200000, ldx=2200000), "stride"),
-    (dict(groups=65536, n=4096, k=4096, ld_dy=4096, ldx=4096), "tiles")])
+    (dict(groups=16384, n=4096, k=4096, ld_dy=4096, ldx=4096), "tiles")])
 def test_grouped_weight_grad_arguments(change, match):
     a = dict(dy=GPU, ld_dy=16, x=GPU, ldx=16, offsets=GPU, groups=2, rows=4, n=16, k=16, dw=GPU) | change
     with pytest.raises(RuntimeError, match=match):

@@ -126,10 +126,17 @@ __device__ __forceinline__ GroupTile find_tile(const GroupedParams& p, int w, in
   return GroupTile{base + l, __builtin_amdgcn_readlane(v.lo, l), __builtin_amdgcn_readlane(v.hi, l),
                    w - __builtin_amdgcn_readlane(v.upto - v.tiles, l)};
 }
-// The tile after t.
+// The tile after t, at index w: in its group, or the first of one of the next four, or searched for.
 template <int BM>
 __device__ __forceinline__ GroupTile next_tile(const GroupedParams& p, GroupTile t, int w, int lane) {
   if (++t.index < row_tiles<BM>(p, t.lo, t.hi)) return t;
+  if (t.group >= 0) {
+    const int last = min(t.group + 4, p.groups - 1);
+    for (int g = t.group + 1; g <= last; ++g) {
+      const int lo = group_offset(p, g), hi = group_offset(p, g + 1);
+      if (hi > lo) return GroupTile{g, lo, hi, 0};
+    }
+  }
   return find_tile<BM>(p, w, lane, group_lanes<BM>(p, lane));
 }
 

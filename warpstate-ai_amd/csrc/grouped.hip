@@ -9,7 +9,8 @@ using namespace ws;
 
 namespace {
 
-constexpr int64_t kMaxGroups = 65536, kMaxRows = 1L << 30;
+// (Every workgroup searches all groups.)
+constexpr int64_t kMaxGroups = 16384, kMaxRows = 1L << 30;
 // Beside FastTile: the kernel for few rows, tiles of 32 and of 16 columns.
 constexpr int kTileFew = kFastTiles, kTileFew16 = kFastTiles + 1;
 // The most 256 x 256 tiles for 256 compute units whose round goes in pieces (grouped_fast_kernel).

@@ -131,7 +131,8 @@ def grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:
     """y [rows, n] BF16 for BF16 rows x [rows, k], weights [groups, n, k] (nn.Linear layout for each
     group; BF16, or FP32 masters, rounded to BF16 first as F.linear under BF16 autocast does) and
     int64 ``offsets`` [groups + 1] on the device: rows offsets[e] to offsets[e + 1] are multiplied
-    by weight e. With autograd to x (BF16) and the weights (their type, from FP32 sums).
+    by weight e. With autograd to x (BF16) and the weights (their type, from FP32 sums). Up to 16384
+    groups.
 
     Offsets must not decrease; rows before the first and behind the last get zeros, in y and in the
     gradient of x. No value of theirs leads an access out of the operands, but rows that
