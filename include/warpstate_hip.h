@@ -535,9 +535,11 @@ int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, const int64
 
 /* y [rows, n] BF16 = x [rows, k] times the transpose of the group's weight [n, k] (WS_GROUPED_NT:
  * a projection; k a multiple of 8), or times its weight [k, n] itself (WS_GROUPED_NN: the input
- * gradient of one; n a multiple of 8), both row-major with row stride ld_weight, group_stride elements from one group's to the next. Rows
- * before the first offset and behind the last get zeros. The sums of the tiles have one order, those
- * of the kernel for few rows, and of long reductions that are cut in slices, another. `workspace`:
+ * gradient of one; n a multiple of 8), both row-major with row stride ld_weight, group_stride elements
+ * from one group's to the next. Where ws_grouped_tile is 5 or 6, x and the weights may have any k, any
+ * strides and the alignment of their elements. Rows before the first offset and behind the last get
+ * zeros. The sums of the tiles have one order, those of the kernel for few rows, and of long
+ * reductions that are cut in slices, another. `workspace`:
  * 16-byte aligned, ws_grouped_workspace_floats (which follows the device's compute units; null if that
  * is 0). */
 enum WsGroupedForm { WS_GROUPED_NT = 0, WS_GROUPED_NN = 1, WS_GROUPED_GRAD = 2 };

@@ -118,6 +118,28 @@ def test_many_groups(sizes):
         _close(dx, (g.mT * mine).sum(1), (g.mT * mine).abs().sum(1), n)
 
 
+@pytest.mark.parametrize("rows,groups,n,k", [(1, 1, 1, 1), (5, 3, 33, 7), (20, 8, 1288, 2051), (40, 8, 1287, 263),
+                                             (100, 8, 520, 65), (9, 2, 40, 127), (300, 90, 264, 61)])
+def test_few_rows_of_any_width(rows, groups, n, k):
+    """Without gradients the weights and rows are read where they lie: NaN around them has no part."""
+    from ops import _hip
+    from ops.grouped_execution import grouped_mm
+
+    assert _hip.query("ws_grouped_tile", rows, groups, n, k, NT) >= 5
+    x, w, _ = _make(rows, groups, n, k, seed=k)
+    offsets = _offsets(rows, groups, "router", seed=n)
+    wide_x = torch.full((rows + 1, k + 3), float("nan"), dtype=BF16, device="cuda")
+    wide_w = torch.full((groups, n + 1, k + 5), float("nan"), dtype=BF16, device="cuda")
+    wide_x[:rows, 1:k + 1] = x
+    wide_w[:, :n, 3:k + 3] = w
+    with torch.no_grad():
+        y = grouped_mm(wide_x[:rows, 1:k + 1], wide_w[:, :n, 3:k + 3], offsets.cuda())
+        assert torch.equal(y, grouped_mm(x, w, offsets.cuda()))
+        assert torch.equal(y, grouped_mm(x.T.contiguous().T, w.mT.contiguous().mT, offsets.cuda()))
+    assert torch.equal(y, grouped_mm(x, w.requires_grad_(True), offsets.cuda()))  # (padded copies)
+    _check(x, w.detach(), None, offsets, y.detach())
+
+
 # Rows, groups, n, k of products that are cut in slices of the reduction, forward or to x.
 SLICED = [(64, 2, 136, 2056), (100, 3, 72, 4000), (300, 2, 520, 3000), (513, 4, 264, 2304), (300, 3, 3000, 520),
           (200, 1, 1288, 5000), (300, 16, 520, 2056), (539, 1, 728, 11720), (1154, 1, 10248, 360), (2373, 1, 8640, 256),

@@ -101,9 +101,11 @@ def test_embedding_backward_arguments(change, match):
     (dict(ldx=20), "aligned"), (dict(ldx=8), "overlap"), (dict(ldw=8), "overlap"), (dict(ldy=8), "overlap"),
     (dict(stride=12), "aligned"), (dict(stride=-8), "aligned"), (dict(ldy=4200000), "stride"),
     (dict(rows=2 ** 30, n=2 ** 20, ldy=2 ** 20), "tiles"), (dict(rows=2 ** 30 + 1), "shape"),
+    (dict(rows=4, ldx=8), "overlap"), (dict(rows=4, ldw=8), "overlap"), (dict(rows=4, x=GPU + 1), "aligned"),
+    (dict(rows=4, w=GPU + 1), "aligned"), (dict(rows=4, stride=-8), "aligned"),
     (dict(work=GPU + 4), "aligned"), (dict(rows=100, k=2048, ldx=2048, ldw=2048), "null")])
 def test_grouped_mm_arguments(change, match):
-    a = dict(x=GPU, ldx=16, w=GPU, ldw=16, stride=256, form=0, offsets=GPU, groups=2, rows=4, n=16, k=16, y=GPU,
+    a = dict(x=GPU, ldx=16, w=GPU, ldw=16, stride=256, form=0, offsets=GPU, groups=2, rows=40, n=16, k=16, y=GPU,
              ldy=16, work=None) | change
     with pytest.raises(RuntimeError, match=match):
         _hip.call("ws_grouped_mm", a["x"], a["ldx"], a["w"], a["ldw"], a["stride"], a["form"], a["offsets"],

@@ -428,12 +428,14 @@ __global__ void __launch_bounds__(Cfg::NT) grouped_grad_ring_kernel(const Groupe
 // weight). Fragments go from memory to registers as they are: a lane's piece is 16 bytes of one row,
 // and a k-tile's two pieces of a row are one line. The waves' sums are added through LDS, in
 // wave order. Rows past the group's read its last one and are not stored; columns past the weight's
-// read its last one, and what they get, up to N, is no part of the result.
+// read its last one, and what they get, up to N, is no part of the result. Operands have any alignment and
+// any K: the pieces need none.
 //
 // The weights' bytes are the bound. Neighbouring tiles run on one XCD, so that what it reads at a time is one
 // run of the weight, and two k-tiles are in flight: with four, the registers leave fewer workgroups
 // (32 rows in 8 groups of 5632 x 2048, launch order and four / these 40 / 34 us, 40 rows in 8 of 2048 x 8192 61 / 50).
 constexpr int kFewRows = 16;
+typedef bf16x8_t bf16x8_any __attribute__((aligned(2)));
 
 // RUN: p.run tiles of a workgroup, for which the registers leave fewer of them.
 template <int COLS, bool RUN>
@@ -482,16 +484,20 @@ static __global__ void __launch_bounds__(256) grouped_few_kernel(const GroupedPa
             for (int j = 0; j < NJ; ++j)
               acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[u][s][j], fa[u][s], acc[j], 0, 0, 0);
       };
-      const auto whole = [](const unsigned short* row, int at) { return *reinterpret_cast<const bf16x8_t*>(row + at); };
+      const auto whole = [](const unsigned short* row, int at) -> bf16x8_t { return *reinterpret_cast<const bf16x8_any*>(row + at); };
       constexpr int U = 2;
       int k = 64 * wave;
       for (; k + 256 * (U - 1) + 64 <= p.K; k += 256 * U) steps(k, std::integral_constant<int, U>{}, whole);
       for (; k + 64 <= p.K; k += 256) steps(k, std::integral_constant<int, 1>{}, whole);
       if (k < p.K)
         steps(k, std::integral_constant<int, 1>{}, [&](const unsigned short* row, int at) {
-          bf16x8_t v = {};
-          if (at + q + 8 <= p.K) v = *reinterpret_cast<const bf16x8_t*>(row + at);
-          return v;
+          const int left = p.K - at - q;
+          if (left >= 8) return whole(row, at);
+          u32x4_t v = {0, 0, 0, 0};
+#pragma unroll
+          for (int e = 0; e < 7; ++e)
+            if (e < left) v[e >> 1] |= (unsigned)row[at + e] << (16 * (e & 1));
+          return __builtin_bit_cast(bf16x8_t, v);
         });
     }
 #pragma unroll

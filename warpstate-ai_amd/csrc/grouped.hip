@@ -226,14 +226,20 @@ extern "C" int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int
   if (rows == 0) return kOk;
   if (!x || !weight || !offsets || !y) return set_error(kInvalid, "null pointer");
   const bool nt = form == WS_GROUPED_NT;
-  if (int rc = check_width(nt ? k : n)) return rc;
-  const int64_t wide = up8(n);
-  if (int rc = check_rows(x, ldx, rows, up8(k), "x")) return rc;
-  if (int rc = check_rows(weight, ld_weight, 2, nt ? k : n, "weight")) return rc;
-  if (int rc = check_rows(y, ldy, rows, wide, "y")) return rc;
-  if (group_stride % 8 != 0 || group_stride < 0) return set_error(kInvalid, "weights must be 16-byte aligned");
   const GroupedPlan plan = pick_grouped(rows, groups, n, k, nt ? kKContig : kMNContig);
   const int tile = plan.tile;
+  const int64_t wide = up8(n);
+  if (tile == kTileFew || tile == kTileFew16) {  // operands of any alignment and width
+    if (rows > 1 && ldx < k) return set_error(kInvalid, "x rows overlap");
+    if (ld_weight < k) return set_error(kInvalid, "weight rows overlap");
+    if (!al(x, 2) || !al(weight, 2) || group_stride < 0) return set_error(kInvalid, "operands must be aligned to their elements");
+  } else {
+    if (int rc = check_width(nt ? k : n)) return rc;
+    if (int rc = check_rows(x, ldx, rows, up8(k), "x")) return rc;
+    if (int rc = check_rows(weight, ld_weight, 2, nt ? k : n, "weight")) return rc;
+    if (group_stride % 8 != 0 || group_stride < 0) return set_error(kInvalid, "weights must be 16-byte aligned");
+  }
+  if (int rc = check_rows(y, ldy, rows, wide, "y")) return rc;
   if (plan.slices > 1 && !workspace) return set_error(kInvalid, "null pointer");
   if (!al(workspace, 16)) return set_error(kInvalid, "the workspace must be 16-byte aligned");
   GroupedParams p{};

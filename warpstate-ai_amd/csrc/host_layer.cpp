@@ -381,9 +381,19 @@ Tensor first_columns(const Tensor& t, int64_t cols) {
   return fixed(t, -1) == cols ? t : copy_rows_op().call(t, t.sym_size(0), cols, false);
 }
 
+// A BF16 operand as the kernel for few rows reads it: with unit column strides and rows apart, else a copy.
+Tensor any_rows(const Tensor& t) {
+  const int64_t d = t.dim(), cols = t.size(d - 1);
+  const bool apart = (t.stride(d - 1) == 1 || cols == 1) && (t.size(d - 2) <= 1 || t.stride(d - 2) >= cols);
+  return apart ? t : t.contiguous();
+}
 Tensor grouped_mm(const Tensor& x, const Tensor& weight, const Tensor& offsets) {
   check_grouped(x, weight, offsets);
   at::AutoDispatchBelowAutograd below_autograd;
+  c10::DeviceGuard guard(x.device());
+  if (weight.scalar_type() == at::kBFloat16 &&
+      ws_grouped_tile(x.size(0), weight.size(0), weight.size(1), weight.size(2), WS_GROUPED_NT) >= 5)
+    return first_columns(grouped_rows(any_rows(x), any_rows(weight), offsets, WS_GROUPED_NT), weight.size(1));
   return first_columns(grouped_rows(grouped_operand(x), grouped_operand(weight), offsets, WS_GROUPED_NT),
                        weight.size(1));
 }

@@ -139,7 +139,8 @@ def grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:
     decreasing ones name twice or not at all are unspecified. Sums are FP32. A row's bits depend on the
     kernel that the sizes choose, not on the other rows' values. Operands whose rows are not whole
     16-byte pieces (weights or rows with k no multiple of 8, other strides) are copied first, on
-    every call: a program that uses such weights many times pads their rows once."""
+    every call: a program that uses such weights many times pads their rows once. BF16 weights are
+    read as they are where there are few rows and no gradients."""
     if not x.is_cuda:
         raise ValueError("Grouped products require CUDA tensors")
     native = _hip.host_ops()
