@@ -203,6 +203,30 @@ def test_odd_widths(rows, groups, n, k, dtype):
     _check(x.detach(), w, dy, offsets, y, dx, dw)
 
 
+@pytest.mark.parametrize("sizes", [(300, 2, 520, 3000), (512, 512, 264, 40), (40, 8, 1288, 263)])
+def test_replays(sizes):
+    """A captured product follows other rows and offsets, with eager work between the replays; slices,
+    several tiles of a workgroup, rows read where they lie."""
+    from ops.grouped_execution import grouped_mm
+
+    rows, groups, n, k = sizes
+    x, w, _ = _make(rows, groups, n, k)
+    offsets = _offsets(rows, groups, "router").cuda()
+    with torch.no_grad():
+        grouped_mm(x, w, offsets)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = grouped_mm(x, w, offsets)
+        for seed, kind in enumerate(("gaps", "one", "even", "router"), 1):
+            x.copy_(_make(rows, groups, n, k, seed=seed)[0])
+            offsets.copy_(_offsets(rows, groups, kind, seed))
+            graph.replay()
+            torch.cuda.synchronize()
+            kept = y.clone()
+            assert torch.equal(kept, grouped_mm(x, w, offsets)), kind
+
+
 def test_layouts():
     """Row strides, odd offsets, transposed operands, an expanded gradient and expanded weights: the
     same bits as contiguous operands."""
