@@ -60,17 +60,17 @@ struct GroupedPlan {
 GroupedPlan pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int bmode) {
   const int64_t used = groups < rows ? groups : rows;
   if (bmode == kKContig) {
-    // Up to 6 rows for each group, above which some groups take two tiles of 16 (us, this kernel / the best
-    // tile): 48 rows in 8 groups of 5632 x 2048 41 / 43, of 1024 x 8192 31 / 39, 64 rows 42 / 43 and 44 / 39; 256
-    // in 32 of 1024 x 1280 20 / 17. Up to 16 where its tiles leave units idle, and larger ones more so: 32 in
-    // 2 of 1024 x 2048 6 / 11, 128 in 8 of 512 x 1280 6 / 8.5.
+    // Up to 6 rows for each group, above which some groups take two tiles of 16 (us, this kernel / the best other):
+    // 48 rows in 8 groups of 5632 x 2048 41 / 41, of 1024 x 8192 29 / 31, 64 rows 41 / 43 and 44 / 31; 256 in 32 of
+    // 1024 x 1280 20 / 17. Up to 16 where its tiles leave units idle, and larger ones more so, or 8 where the reduction is
+    // long enough for many slices: 32 in 2 of 2048 x 2048 8 / 9.5, of 2048 x 11264 32 / 23, 32 in 4 of 1024 x 4096
+    // 9 / 12, 64 13 / 12; 128 in 8 of 512 x 1280 6 / 8.5.
     const int64_t tiles = (int64_t)cdiv(n, 32) * (used + rows / 16), cus = device_cus();
-    if (rows <= 6 * used || (rows <= 16 * used && tiles <= cus)) {
+    if (rows <= 6 * used || (rows <= (k < 4096 ? 16 : 8) * used && tiles <= cus)) {
       // Tiles of 16 columns, whose rows of x are read twice as often, for idle units, and for long
-      // reductions with very few rows (32 / 16 columns): 64 rows in 8 groups of 512 x 1280 5.9 / 4.9, 96 6.1 /
-      // 6.8; 8 in 8 of 5632 x 2048 33 / 28, 32 34 / 31; 32 in 8 of 7168 x 1472 30.5 / 32.5; 256 in 32 of
-      // 1024 x 2048 26 / 29.
-      return {4 * tiles <= 3 * cus || (k >= 2048 && rows <= 4 * used) ? kTileFew16 : kTileFew, 1};
+      // reductions with very few rows (32 / 16 columns): 48 rows in 8 groups of 512 x 2048 7.7 / 6.0, 96 8.1 /
+      // 9.4; 32 in 8 of 5632 x 2048 41 / 35; 32 in 8 of 7168 x 1472 30.5 / 32.5; 256 in 32 of 1024 x 2048 29.5 / 32.
+      return {4 * tiles <= 3 * cus || (k >= 2048 && rows <= 6 * used) ? kTileFew16 : kTileFew, 1};
     }
   }
   // Two workgroups on a unit with few stages hide less of what comes from HBM, one with more hides more.
