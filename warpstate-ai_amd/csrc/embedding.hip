@@ -113,10 +113,13 @@ extern "C" int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, 
   p.perm = reinterpret_cast<int*>(work + l.perm);
   p.vocab = (int)vocab;
   p.d = (int)d;
-  // Waves enough where most rows have tokens, few chains of loads where most have none (us, all kernels,
-  // 2 / 4 rows a wave: 16384 tokens into 32768 x 2048 68 / 71, into 2000 x 1280 36 / 39, 64 tokens
-  // into 32768 x 2048 58 / 54).
-  p.group = rows >= 4 * vocab ? 1 : 4 * rows >= vocab ? 2 : 4;
+  // A row of the table for each wave, so that frequent tokens next to each other do not wait for one another;
+  // two, or four, where most rows are empty and their waves take longer than up to 4 KB of zeros (us, all kernels,
+  // 1 / 2 / 4 rows a wave, tokens of a Zipf distribution in any order and, in brackets, with the frequent ones
+  // adjacent: 16384 into 32768 x 2048 FP32 65 / 68 / 68 (99 / 99 / 113); 7000 into 32768 x 1280 BF16 55 / 49 / 42
+  // (60 / 67 / 81); 2000 into 32768 x 2048 FP32 58 / 62 / 60; 100 into 32768 x 1280 BF16 29 / 23 / 21).
+  const int64_t row_bytes = d * (mode == WS_EMBED_WRITE_BF16 ? 2 : 4);
+  p.group = 64 * rows < vocab ? 4 : 4 * rows < vocab && row_bytes <= 4096 ? 2 : 1;
   p.scale = scale;
   p.out = dtable;
   p.ld_out = ld_dtable;
