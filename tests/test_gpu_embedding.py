@@ -63,7 +63,8 @@ def test_lookup(rows, vocab, d, table_dtype, out):
     (1, 1, 1, F32, BF16), (31, 7, 64, BF16, BF16), (32, 600, 512, F32, BF16), (33, 40, 77, BF16, BF16),
     (64, 9, 2100, F32, F32), (64, 333, 4104, BF16, BF16), (65, 9, 2100, F32, BF16),
     (1000, 3000, 1280, BF16, F32), (1025, 511, 2048, F32, F32), (2500, 97, 1001, F32, BF16),
-    (5000, 140001, 24, F32, BF16), (40000, 5000, 256, F32, BF16), (40001, 300, 2056, BF16, BF16)])
+    (5000, 140001, 24, F32, BF16), (40000, 5000, 256, F32, BF16), (40001, 300, 2056, BF16, BF16),
+    (70, 5001, 136, F32, BF16)])
 def test_gradient(rows, vocab, d, table_dtype, out, kind):
     from ops.embedding_execution import embedding
 
