@@ -528,7 +528,8 @@ int ws_embedding_backward(const void* dy, int64_t ld_dy, int dy_f32, const int64
  * int64 on the device, not decreasing). The offsets are read on the device only, and no value of theirs
  * leads an access out of the operands; decreasing ones leave rows of the result unspecified. BF16
  * operands, FP32 sums, 16-byte aligned rows, weight rows of a multiple of 8 elements, 1 to 16384
- * groups, up to 2^30 rows. The other width, n below, may be any; rows of that width reach to its
+ * groups, up to 2^30 rows; in tiles of 256 x 256, fewer than 2^24 for a product, (rows / 256 + groups + 2)
+ * ceil(n / 256), and fewer than 2^22 for a weight gradient, groups ceil(n / 256) ceil(k / 256). The other width, n below, may be any; rows of that width reach to its
  * next multiple of 8: y's are written up to there, and dy's, like x's under WS_GROUPED_NN, have
  * to hold zeros.
  */
@@ -552,6 +553,11 @@ int64_t ws_grouped_workspace_floats(int64_t rows, int64_t groups, int64_t n, int
 int ws_grouped_weight_grad(const void* dy, int64_t ld_dy, const void* x, int64_t ldx,
                            const int64_t* offsets, int64_t groups, int64_t rows, int64_t n,
                            int64_t k, void* dweight, int dweight_f32, void* stream);
+/* Whether the gradients of a product y = x w^T of these sizes, with widths padded to multiples of 8, fit what
+ * the calls above take: dx (WS_GROUPED_NN) and dweight where asked for. No launch; for a forward that would
+ * otherwise be recorded in vain. */
+int ws_grouped_backward_check(int64_t rows, int64_t groups, int64_t n, int64_t k, int dx, int dweight,
+                              int dweight_f32);
 /* Matrices of any width as these products take them, and back: for each group, rows [rows_in, cols_in]
  * into rows [rows_out, cols_out] with zeros past the input's last row and column, rows and columns past
  * the output's left out. BF16 or FP32, in the input's type or rounded from FP32 to BF16; any alignment

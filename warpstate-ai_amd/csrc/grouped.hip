@@ -11,6 +11,9 @@ namespace {
 
 // (Every workgroup searches all groups.)
 constexpr int64_t kMaxGroups = 16384, kMaxRows = 1L << 30;
+// Workgroups of a launch (of up to 512 threads, which have to be fewer than 2^32); and a product's tiles, of which
+// a workgroup takes several: the search adds up to 66 times their number in 32 bits.
+constexpr int64_t kMaxBlocks = 1L << 22, kMaxTiles = 1L << 24;
 // Beside FastTile: the kernel for few rows, tiles of 32 and of 16 columns.
 constexpr int kTileFew = kFastTiles, kTileFew16 = kFastTiles + 1;
 // The most 256 x 256 tiles for 256 compute units whose round goes in pieces (grouped_fast_kernel).
@@ -41,11 +44,21 @@ int64_t most_tiles(int64_t rows, int64_t groups, int bm) {
   return rows / bm + used;
 }
 
+// The tiles that the grid of a product with n columns is sized for. Those of 256 x 256 are the fewest.
+int64_t grid_tiles(int64_t rows, int64_t groups, int64_t n, int tile) {
+  return most_tiles(rows, groups, tile_rows(tile)) * cdiv(n, tile_cols(tile));
+}
+int64_t grad_tiles(int64_t groups, int64_t m, int64_t n, int tile) {
+  return groups * cdiv(m, tile_rows(tile)) * cdiv(n, tile_cols(tile));
+}
+
 // Tiles of a workgroup, one after the other: with a short reduction, finding one among the groups takes longer than
 // its product (us, one / several: 512 rows in 512 groups of 2048 x 16 135 / 34, 4096 in 256 of 2048 x 64 45 / 31).
+// With any reduction, as many as bring the workgroups down to what a launch takes.
 int tiles_of_run(int64_t tiles, int64_t k) {
-  const int64_t most = tiles / (4 * (int64_t)device_cus());
-  return k > 256 || most < 2 ? 1 : most < 16 ? (int)most : 16;
+  const int64_t most = tiles / (4 * (int64_t)device_cus()), run = k > 256 || most < 2 ? 1 : most < 16 ? most : 16;
+  const int64_t least = (tiles + kMaxBlocks - 1) / kMaxBlocks;
+  return (int)(run < least ? least : run);
 }
 
 // The tile for rows that are spread over the groups, by the cost table of single products, for the
@@ -66,11 +79,13 @@ GroupedPlan pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int
     // long enough for many slices: 32 in 2 of 2048 x 2048 8 / 9.5, of 2048 x 11264 32 / 23, 32 in 4 of 1024 x 4096
     // 9 / 12, 64 13 / 12; 128 in 8 of 512 x 1280 6 / 8.5.
     const int64_t tiles = (int64_t)cdiv(n, 32) * (used + rows / 16), cus = device_cus();
-    if (rows <= 6 * used || (rows <= (k < 4096 ? 16 : 8) * used && tiles <= cus)) {
+    if ((rows <= 6 * used || (rows <= (k < 4096 ? 16 : 8) * used && tiles <= cus)) &&
+        grid_tiles(rows, groups, n, kTileFew) < kMaxTiles) {
       // Tiles of 16 columns, whose rows of x are read twice as often, for idle units, and for long
       // reductions with very few rows (32 / 16 columns): 48 rows in 8 groups of 512 x 2048 7.7 / 6.0, 96 8.1 /
       // 9.4; 32 in 8 of 5632 x 2048 41 / 35; 32 in 8 of 7168 x 1472 30.5 / 32.5; 256 in 32 of 1024 x 2048 29.5 / 32.
-      return {4 * tiles <= 3 * cus || (k >= 2048 && rows <= 6 * used) ? kTileFew16 : kTileFew, 1};
+      const bool narrow = 4 * tiles <= 3 * cus || (k >= 2048 && rows <= 6 * used);
+      return {narrow && grid_tiles(rows, groups, n, kTileFew16) <= kMaxBlocks ? kTileFew16 : kTileFew, 1};
     }
   }
   // Two workgroups on a unit with few stages hide less of what comes from HBM, one with more hides more.
@@ -78,6 +93,7 @@ GroupedPlan pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int
   GroupedPlan best = {kTile256, 1};
   float t = 0.0f;
   for (int tile = 0; tile < kFastTiles; ++tile) {
+    if (tile != kTile256 && grid_tiles(rows, groups, n, tile) >= kMaxTiles) continue;
     const int64_t bm = tile_rows(tile), cus = device_cus();
     int64_t wide = rows + used * bm / 2;
     if (wide < used * bm) wide = used * bm;
@@ -90,7 +106,7 @@ GroupedPlan pick_grouped(int64_t rows, int64_t groups, int64_t n, int64_t k, int
     const float once = (fused * fn * fk + frows * (2.0f * fn + fk)) / 7e6f;
     if (read < once) read = once;
     for (int slices = 1; slices <= (tile == kTile256 || tile == kTile128x2 ? 1 : kMaxSlices); slices *= 2) {
-      if (slices > 1 && k < (int64_t)slices * kSliceTiles * kFBK) break;
+      if (slices > 1 && (k < (int64_t)slices * kSliceTiles * kFBK || grid_tiles(rows, groups, n, tile) > kMaxBlocks)) break;
       float ti = slower[tile] * tile_time(tile, wide, n, k, kKContig, bmode, cus, false, kEpiStore, slices);
       if (tile == kTile256) {
         const TileCost& c = tile_cost(tile, kKContig, bmode);
@@ -117,7 +133,7 @@ int pick_grad(int64_t rows, int64_t groups, int64_t m, int64_t n) {
     const int64_t bm = tile_rows(tile);
     // With a k-tile or less for each group the smaller tile's stores start sooner (64 groups of 512 x
     // 1280 over 4096 rows, BF16, 26 / 24 us; 8 of 5632 x 2048 over 32, FP32, 82 / 76).
-    if (tile == kTile256 && rows <= kFBK * groups) continue;
+    if (tile == kTile256 ? rows <= kFBK * groups : grad_tiles(groups, m, n, tile) >= kMaxBlocks) continue;
     const float ti = tile_time(tile, groups * (cdiv(m, bm) * bm), n, cdiv(rows, groups), kMNContig, kMNContig, device_cus(),
                                false, kEpiF32);
     if (t == 0.0f || ti < t) {
@@ -143,6 +159,17 @@ int check_rows(const void* p, int64_t ld, int64_t rows, int64_t cols, const char
   if (!al(p, 16) || ld % 8 != 0) return set_error(kInvalid, "%s rows must be 16-byte aligned", what);
   if (rows > 1 && ld < cols) return set_error(kInvalid, "%s rows overlap", what);
   return check_out_stride(ld > cols ? ld : cols, 2, what);
+}
+
+int check_tiles(int64_t tiles, int64_t most, int64_t rows, int64_t groups, int64_t n, int64_t k) {
+  return tiles < most ? kOk
+                      : set_error(kInvalid, "too many tiles (%ld rows, %ld groups of %ld x %ld)", (long)rows, (long)groups,
+                                  (long)n, (long)k);
+}
+// What the weight gradient asks of sizes alone: where 256 x 256 tiles are few enough, so are those that are chosen.
+int check_grad(int64_t rows, int64_t groups, int64_t n, int64_t k, int elem_bytes) {
+  if (int rc = check_out_stride(k, elem_bytes, "dweight")) return rc;
+  return check_tiles(grad_tiles(groups, n, k, kTile256), kMaxBlocks, rows, groups, n, k);
 }
 
 template <class Cfg, int BMODE, bool CUT = true>
@@ -204,12 +231,20 @@ int launch_grad_ring(const GroupedGradParams& p, bool f32, int64_t grid, hipStre
 
 extern "C" int ws_grouped_tile(int64_t rows, int64_t groups, int64_t n, int64_t k, int form) {
   if (rows < 1 || check_sizes(groups, rows, n, k)) return -1;
-  switch (form) {
-    case WS_GROUPED_NT: return pick_grouped(rows, groups, n, k, kKContig).tile;
-    case WS_GROUPED_NN: return pick_grouped(rows, groups, n, k, kMNContig).tile;
-    case WS_GROUPED_GRAD: return pick_grad(rows, groups, n, k);
+  if (form == WS_GROUPED_GRAD) return grad_tiles(groups, n, k, kTile256) < kMaxBlocks ? pick_grad(rows, groups, n, k) : -1;
+  if ((form != WS_GROUPED_NT && form != WS_GROUPED_NN) || grid_tiles(rows, groups, n, kTile256) >= kMaxTiles) return -1;
+  return pick_grouped(rows, groups, n, k, form == WS_GROUPED_NT ? kKContig : kMNContig).tile;
+}
+
+extern "C" int ws_grouped_backward_check(int64_t rows, int64_t groups, int64_t n, int64_t k, int dx, int dweight,
+                                         int dweight_f32) {
+  if (int rc = check_sizes(groups, rows, n, k)) return rc;
+  const int64_t wide_n = up8(n), wide_k = up8(k);
+  if (int rc = check_out_stride(wide_n > wide_k ? wide_n : wide_k, 2, "gradient")) return rc;
+  if (dx && rows > 0) {
+    if (int rc = check_tiles(grid_tiles(rows, groups, wide_k, kTile256), kMaxTiles, rows, groups, n, k)) return rc;
   }
-  return -1;
+  return dweight ? check_grad(rows, groups, n, wide_k, dweight_f32 ? 4 : 2) : kOk;
 }
 
 extern "C" int64_t ws_grouped_workspace_floats(int64_t rows, int64_t groups, int64_t n, int64_t k, int form) {
@@ -257,8 +292,8 @@ extern "C" int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int
   p.tiles_n = cdiv(wide, tile_cols(tile));
   p.c = static_cast<unsigned short*>(y);
   p.ldc = ldy;
-  const int64_t grid = most_tiles(rows, groups, tile_rows(tile)) * p.tiles_n;
-  if (grid >= 1L << 22) return set_error(kInvalid, "too many tiles (%ld rows, %ld columns, %ld groups)", (long)rows, (long)n, (long)groups);
+  if (int rc = check_tiles(grid_tiles(rows, groups, n, kTile256), kMaxTiles, rows, groups, n, k)) return rc;
+  const int64_t grid = grid_tiles(rows, groups, n, tile);
   p.most = (int)grid;
   p.chunk = cdiv(groups, 64);
   p.run = tile == kTile256 || plan.slices > 1 ? 1 : tiles_of_run(grid, k);
@@ -275,7 +310,7 @@ extern "C" int ws_grouped_weight_grad(const void* dy, int64_t ld_dy, const void*
   if (int rc = check_rows(dy, ld_dy, rows, up8(n), "dy")) return rc;
   if (int rc = check_rows(x, ldx, rows, k, "x")) return rc;
   if (!al(dweight, 16)) return set_error(kInvalid, "the weight gradient must be 16-byte aligned");
-  if (int rc = check_out_stride(k, dweight_f32 ? 4 : 2, "dweight")) return rc;
+  if (int rc = check_grad(rows, groups, n, k, dweight_f32 ? 4 : 2)) return rc;
   const int tile = pick_grad(rows, groups, n, k);
   GroupedGradParams p{};
   p.a = static_cast<const unsigned short*>(dy);
@@ -290,8 +325,7 @@ extern "C" int ws_grouped_weight_grad(const void* dy, int64_t ld_dy, const void*
   p.tiles_m = cdiv(n, tile_rows(tile));
   p.tiles_n = cdiv(k, tile_cols(tile));
   p.g = dweight;
-  const int64_t grid = groups * p.tiles_m * p.tiles_n;
-  if (grid >= 1L << 22) return set_error(kInvalid, "too many tiles (%ld groups of %ld x %ld)", (long)groups, (long)n, (long)k);
+  const int64_t grid = grad_tiles(groups, n, k, tile);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool f32 = dweight_f32 != 0;
   switch (tile) {

@@ -441,6 +441,11 @@ Tensor grouped_mm_autograd(const Tensor& x, const Tensor& weight, const Tensor& 
     return below(op, x, weight, offsets);
   }
   check_grouped(x, weight, offsets);
+  // (A symbolic number of rows is left to the backward.)
+  if (const auto rows = x.sym_size(0).maybe_as_int())
+    check(ws_grouped_backward_check(*rows, fixed(weight, 0), fixed(weight, 1), fixed(x, 1), x.requires_grad(),
+                                    weight.requires_grad(), weight.scalar_type() == at::kFloat),
+          "ws_grouped_backward_check");
   Tensor a, w;
   {
     at::AutoDispatchBelowAutograd below_autograd;

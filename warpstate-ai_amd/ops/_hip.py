@@ -123,6 +123,7 @@ SIGNATURES = {
     "ws_grouped_workspace_floats": (_i64, [_i64, _i64, _i64, _i64, _i32]),
     "ws_grouped_weight_grad": (_i32, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64,
                                       _i64, _i64, _c_void_p, _i32, _c_void_p]),
+    "ws_grouped_backward_check": (_i32, [_i64] * 4 + [_i32] * 3),
     "ws_copy_rows": (_i32, [_c_void_p, _i32] + [_i64] * 4 + [_c_void_p, _i32] + [_i64] * 5 + [_c_void_p]),
     "ws_grouped_tile": (_i32, [_i64, _i64, _i64, _i64, _i32]),
 }

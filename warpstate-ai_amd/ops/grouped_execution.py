@@ -132,7 +132,9 @@ def grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:
     group; BF16, or FP32 masters, rounded to BF16 first as F.linear under BF16 autocast does) and
     int64 ``offsets`` [groups + 1] on the device: rows offsets[e] to offsets[e + 1] are multiplied
     by weight e. With autograd to x (BF16) and the weights (their type, from FP32 sums). Up to 16384
-    groups.
+    groups and 2^30 rows; in tiles of 256 x 256, fewer than 2^24 of the result (and of x's gradient: of
+    (rows / 256 + groups + 2) ceil(n / 256)) and fewer than 2^22 of the weights. A call whose gradients
+    would pass that is refused where it is recorded.
 
     Offsets must not decrease; rows before the first and behind the last get zeros, in y and in the
     gradient of x. No value of theirs leads an access out of the operands, but rows that
@@ -154,5 +156,8 @@ def grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:
 def _grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:
     _check(x, weight, offsets)
     _refuse_tangents("grouped_mm", x, weight)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        _hip.call("ws_grouped_backward_check", x.shape[0], *weight.shape, int(x.requires_grad),
+                  int(weight.requires_grad), int(weight.dtype == F32))
     return _GroupedMm.apply(x, weight, _operand(x.detach()), _operand(weight.detach()),
                             offsets.contiguous())
