@@ -209,8 +209,10 @@ int run_tile(const GroupedParams& p, GroupedPlan plan, int64_t grid, hipStream_t
     case kTile64: return launch_ring<Ring64, BMODE>(p, slices, grid, s);
   }
   if constexpr (BMODE == kKContig) {
-    const auto kernel = p.run > 1 ? (tile == kTileFew ? grouped_few_kernel<32, true> : grouped_few_kernel<16, true>)
-                                  : (tile == kTileFew ? grouped_few_kernel<32, false> : grouped_few_kernel<16, false>);
+    // (Several tiles a workgroup are of 32 columns: 16 are for idle units, or for reductions above 256.)
+    const auto kernel = tile == kTileFew16 ? grouped_few_kernel<16, false>
+                        : p.run > 1        ? grouped_few_kernel<32, true>
+                                           : grouped_few_kernel<32, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(grid, p.run)), dim3(256), 0, s, p);
     return hip_check(hipGetLastError(), "grouped product launch");
   }
@@ -296,7 +298,7 @@ extern "C" int ws_grouped_mm(const void* x, int64_t ldx, const void* weight, int
   const int64_t grid = grid_tiles(rows, groups, n, tile);
   p.most = (int)grid;
   p.chunk = cdiv(groups, 64);
-  p.run = tile == kTile256 || plan.slices > 1 ? 1 : tiles_of_run(grid, k);
+  p.run = tile == kTile256 || tile == kTileFew16 || plan.slices > 1 ? 1 : tiles_of_run(grid, k);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return nt ? run_tile<kKContig>(p, plan, grid, s) : run_tile<kMNContig>(p, plan, grid, s);
 }
