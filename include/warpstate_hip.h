@@ -561,7 +561,7 @@ int ws_grouped_backward_check(int64_t rows, int64_t groups, int64_t n, int64_t k
 /* Matrices of any width as these products take them, and back: for each group, rows [rows_in, cols_in]
  * into rows [rows_out, cols_out] with zeros past the input's last row and column, rows and columns past
  * the output's left out. BF16 or FP32, in the input's type or rounded from FP32 to BF16; any alignment
- * of the types. Up to 2^26 rows of all groups. */
+ * of the types. Up to 2^24 groups. */
 int ws_copy_rows(const void* in, int in_f32, int64_t group_in, int64_t ld_in, int64_t rows_in,
                  int64_t cols_in, void* out, int out_f32, int64_t group_out, int64_t ld_out,
                  int64_t rows_out, int64_t cols_out, int64_t groups, void* stream);

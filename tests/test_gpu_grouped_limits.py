@@ -93,3 +93,25 @@ def test_a_gradient_that_does_not_fit_is_refused_at_once(native, monkeypatch):
     if native:  # (without gradients the weights are read where they lie)
         with torch.no_grad():
             assert (grouped_mm(x, leaf.expand(groups, n, n), offsets) == n).all()
+
+
+def test_copies_of_very_many_rows():
+    """67 million rows of a width that is padded, and of a gradient that is cut off again."""
+    from ops.grouped_execution import grouped_mm
+
+    rows, groups, n, k = 100, 16384, 4100, 3
+    g = torch.Generator("cuda").manual_seed(4)
+    x = torch.randn((rows, k), generator=g, device="cuda", dtype=BF16)
+    w = torch.randn((groups, n, k), generator=g, device="cuda").requires_grad_(True)
+    dy = torch.randn((rows, n), generator=g, device="cuda", dtype=BF16)
+    owner = torch.arange(rows) // 2 * 334
+    owner[-2:] = groups - 1
+    y = grouped_mm(x, w, torch.searchsorted(owner, torch.arange(groups + 1)).cuda())
+    dw, = torch.autograd.grad(y, w, dy)
+    seen = dw.view(groups, -1).count_nonzero(1).cpu()
+    seen[owner] = 0
+    assert not seen.any()
+    for lo in range(0, rows, 2):
+        a, b, d = x[lo:lo + 2].to(F64), w.detach()[owner[lo]].to(BF16).to(F64), dy[lo:lo + 2].to(F64)
+        _close(y[lo:lo + 2], a @ b.T, a.abs() @ b.abs().T, k)
+        _close(dw[owner[lo]], d.T @ a, d.abs().T @ a.abs(), 2)

@@ -532,18 +532,18 @@ struct CopyRowsParams {
 template <bool IN32, bool OUT32>
 static __global__ void __launch_bounds__(256) copy_rows_kernel(const CopyRowsParams p) {
   const int lane = threadIdx.x & 63;
-  const long row = blockIdx.x * 4L + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= p.rows) return;
-  const long g = row / p.rows_out;
-  const int r = (int)(row - g * p.rows_out), cols = r < p.rows_in ? p.cols_in : 0;
+  for (long row = blockIdx.x * 4L + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < p.rows; row += gridDim.x * 4L) {
+    const long g = row / p.rows_out;
+    const int r = (int)(row - g * p.rows_out), cols = r < p.rows_in ? p.cols_in : 0;
 #pragma unroll 4
-  for (int c = 8 * lane; c < p.cols_out; c += 512) {
-    QuantRow<IN32> v;
-    load_piece<IN32, false>(v, p.in, g * p.group_in + r * p.ld_in + c, cols - c);
-    float f[8];
+    for (int c = 8 * lane; c < p.cols_out; c += 512) {
+      QuantRow<IN32> v;
+      load_piece<IN32, false>(v, p.in, g * p.group_in + r * p.ld_in + c, cols - c);
+      float f[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = v.at(e);
-    store_piece<OUT32, false>(round_piece<OUT32>(f), p.out, g * p.group_out + r * p.ld_out + c, p.cols_out - c);
+      for (int e = 0; e < 8; ++e) f[e] = v.at(e);
+      store_piece<OUT32, false>(round_piece<OUT32>(f), p.out, g * p.group_out + r * p.ld_out + c, p.cols_out - c);
+    }
   }
 }
 

@@ -349,8 +349,7 @@ extern "C" int ws_copy_rows(const void* in, int in_f32, int64_t group_in, int64_
                             void* out, int out_f32, int64_t group_out, int64_t ld_out, int64_t rows_out, int64_t cols_out,
                             int64_t groups, void* stream) {
   if (groups < 0 || rows_in < 0 || rows_out < 0 || cols_in < 0 || cols_out < 0 || !fits_i32(rows_in) ||
-      !fits_i32(rows_out) || !fits_i32(cols_in + 512) || !fits_i32(cols_out + 512) ||
-      (rows_out > 0 && groups > (1L << 26) / rows_out))
+      !fits_i32(rows_out) || !fits_i32(cols_in + 512) || !fits_i32(cols_out + 512) || groups > 1L << 24)
     return set_error(kInvalid, "invalid sizes of copied rows");
   if (groups == 0 || rows_out == 0 || cols_out == 0) return kOk;
   if (!out || (!in && rows_in > 0 && cols_in > 0)) return set_error(kInvalid, "null pointer");
@@ -358,8 +357,9 @@ extern "C" int ws_copy_rows(const void* in, int in_f32, int64_t group_in, int64_
   if ((rows_out > 1 && ld_out < cols_out) || (groups > 1 && group_out < ld_out * (rows_out - 1) + cols_out))
     return set_error(kInvalid, "rows overlap");
   CopyRowsParams p{in, group_in, ld_in, (int)rows_in, (int)cols_in, out, group_out, ld_out, (int)rows_out, (int)cols_out, groups * rows_out};
+  const int64_t blocks = p.rows < 4 * kMaxBlocks ? cdiv(p.rows, 4) : kMaxBlocks;
   auto run = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(p.rows, 4)), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream), p);
     return hip_check(hipGetLastError(), "row copy launch");
   };
   return in_f32 ? (out_f32 ? run(&copy_rows_kernel<true, true>) : run(&copy_rows_kernel<true, false>))
