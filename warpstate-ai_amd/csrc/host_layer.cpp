@@ -26,7 +26,8 @@ Tensor rows_of(const Tensor& t) {
 int64_t fixed(const Tensor& t, int64_t dim) { return t.sym_size(dim).guard_int(__FILE__, __LINE__); }
 
 // Gradients that are not differentiable again: where a graph of the backward is recorded, they stand
-// behind a node that depends on everything they were made `from`, and refuses.
+// behind a node that depends on everything they were made `from`, and refuses. `inputs`: how many of the first inputs
+// of the node that is being evaluated it depends on too, by their edges, so that none has to be saved for that.
 struct OnceFn : Function<OnceFn> {
   static variable_list forward(AutogradContext* ctx, at::TensorList grads, at::TensorList from, std::string message) {
     ctx->saved_data["message"] = message;
@@ -38,11 +39,17 @@ struct OnceFn : Function<OnceFn> {
     TORCH_CHECK(false, ctx->saved_data["message"].toStringRef());
   }
 };
-variable_list once(variable_list grads, const variable_list& from, const char* message) {
+variable_list once(variable_list grads, const variable_list& from, const char* message, size_t inputs = 0) {
   if (!at::GradMode::is_enabled()) return grads;
   variable_list known, sources;
   for (const auto& t : from)
     if (t.defined() && t.requires_grad()) sources.push_back(t);
+  if (const auto node = torch::autograd::get_current_node())
+    for (size_t i = 0; i < inputs && i < node->num_outputs(); ++i)
+      if (const auto& edge = node->next_edge(i); edge.is_valid()) {
+        sources.push_back(at::empty({0}));
+        torch::autograd::impl::set_gradient_edge(sources.back(), edge);
+      }
   if (sources.empty()) return grads;
   for (const auto& g : grads)
     if (g.defined()) known.push_back(g);
@@ -399,14 +406,14 @@ Tensor grouped_mm(const Tensor& x, const Tensor& weight, const Tensor& offsets) 
 }
 
 struct GroupedMmFn : Function<GroupedMmFn> {
-  // Gradients go to the tensors that the operands a and w were made from.
+  // Gradients go to the tensors x and weight, which the operands a and w were made from. Kept is what they read: dx the
+  // weights, dW the rows.
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& a, const Tensor& w,
                         const Tensor& offsets) {
     static const auto op = find<GroupedRows>("warpstate::native_grouped_rows");
     at::AutoDispatchBelowAutograd guard;
     ctx->set_materialize_grads(false);
-    // (x and weight themselves only to depend on.)
-    ctx->save_for_backward({weight.requires_grad() ? a : Tensor(), x.requires_grad() ? w : Tensor(), offsets, x, weight});
+    ctx->save_for_backward({weight.requires_grad() ? a : Tensor(), x.requires_grad() ? w : Tensor(), offsets});
     ctx->saved_data["want_x"] = x.requires_grad();
     ctx->saved_data["want_w"] = weight.requires_grad();
     ctx->saved_data["n"] = fixed(weight, 1);
@@ -431,7 +438,7 @@ struct GroupedMmFn : Function<GroupedMmFn> {
         d[1] = dw;
       }
     }
-    return once(d, {s[3], s[4], grads[0]}, kGroupedTwice);
+    return once(d, {grads[0]}, kGroupedTwice, 2);
   }
 };
 Tensor grouped_mm_autograd(const Tensor& x, const Tensor& weight, const Tensor& offsets) {
@@ -446,11 +453,11 @@ Tensor grouped_mm_autograd(const Tensor& x, const Tensor& weight, const Tensor& 
     check(ws_grouped_backward_check(*rows, fixed(weight, 0), fixed(weight, 1), fixed(x, 1), x.requires_grad(),
                                     weight.requires_grad(), weight.scalar_type() == at::kFloat),
           "ws_grouped_backward_check");
-  Tensor a, w;
+  Tensor a = x.detach(), w = weight.detach();
   {
     at::AutoDispatchBelowAutograd below_autograd;
-    a = grouped_operand(x.detach());
-    w = grouped_operand(weight.detach());
+    a = grouped_operand(a);
+    w = grouped_operand(w);
   }
   return GroupedMmFn::apply(x, weight, a, w, offsets);
 }

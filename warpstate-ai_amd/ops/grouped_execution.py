@@ -97,11 +97,14 @@ def _first(t: Tensor, cols: int) -> Tensor:
 
 
 class _GroupedMm(torch.autograd.Function):
-    """Of ``_operand``'s a and w, with gradients to the tensors they came from."""
+    """Of ``_operand``'s a and w, with gradients to the tensors x and weight, which they came from. Kept
+    is what these read: dx the weights, dW the rows. ``inputs``: tensors without elements that depend
+    on x and weight."""
 
     @staticmethod
-    def forward(ctx, x, weight, a, w, offsets):
-        ctx.save_for_backward(a, w, offsets, x, weight)  # the last two only to depend on
+    def forward(ctx, x, weight, a, w, offsets, inputs):
+        want_x, want_w = ctx.needs_input_grad[:2]
+        ctx.save_for_backward(a if want_w else None, w if want_x else None, offsets, *inputs)
         ctx.args = (weight.shape[1], x.shape[1], weight.dtype)
         ctx.set_materialize_grads(False)
         return _first(_product(a, w, offsets, _NT), weight.shape[1])
@@ -109,8 +112,8 @@ class _GroupedMm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         if dy is None:
-            return None, None, None, None, None
-        a, w, offsets, x, weight = ctx.saved_tensors
+            return None, None, None, None, None, None
+        a, w, offsets, *inputs = ctx.saved_tensors
         n, k, dtype = ctx.args
         dx = dw = None
         with torch.no_grad():
@@ -118,13 +121,13 @@ class _GroupedMm(torch.autograd.Function):
             if ctx.needs_input_grad[0]:
                 dx = _first(_product(g, w, offsets, _NN), k)
             if ctx.needs_input_grad[1]:
-                groups = w.shape[0]
+                groups = offsets.shape[0] - 1
                 dw = torch.empty((groups, n, a.shape[1]), dtype=dtype, device=a.device)
                 _hip.call_on(a, "ws_grouped_weight_grad", g.data_ptr(), _row_stride(g),
                              a.data_ptr(), _row_stride(a), offsets.data_ptr(), groups, a.shape[0], n,
                              a.shape[1], dw.data_ptr(), int(dtype == F32))
                 dw = _first(dw, k)
-        return _once("a grouped product", (dx, dw, None, None, None), x, weight, dy)
+        return _once("a grouped product", (dx, dw, None, None, None, None), *inputs, dy)
 
 
 def grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:
@@ -156,8 +159,11 @@ def grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:
 def _grouped_mm(x: Tensor, weight: Tensor, offsets: Tensor) -> Tensor:
     _check(x, weight, offsets)
     _refuse_tangents("grouped_mm", x, weight)
+    inputs = ()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         _hip.call("ws_grouped_backward_check", x.shape[0], *weight.shape, int(x.requires_grad),
                   int(weight.requires_grad), int(weight.dtype == F32))
+        # (Copies: a view would keep the whole of its tensor.)
+        inputs = tuple(t[:0].clone() for t in (x, weight) if t.requires_grad)
     return _GroupedMm.apply(x, weight, _operand(x.detach()), _operand(weight.detach()),
-                            offsets.contiguous())
+                            offsets.contiguous(), inputs)
