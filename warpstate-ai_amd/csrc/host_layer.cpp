@@ -204,13 +204,17 @@ ThreeTensors rmsnorm_quantize_meta(const Tensor& x, const std::optional<Tensor>&
 constexpr char kEmbeddingTwice[] = "the embedding cannot be differentiated twice";
 typedef Tensor Embedding(const Tensor&, const Tensor&, double, bool);
 
+// (The kernels multiply in FP32.)
+void check_scale(double scale) {
+  TORCH_CHECK_VALUE(std::isfinite((float)scale), "The scale must be finite in FP32, not ", scale);
+}
 void check_embedding(const Tensor& tokens, const Tensor& table, double scale) {
   TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong && tokens.device() == table.device(),
                     "Tokens must be int64 on the table's device");
   TORCH_CHECK_VALUE((table.scalar_type() == at::kBFloat16 || table.scalar_type() == at::kFloat) && table.dim() == 2 &&
                         table.sym_numel() > 0,
                     "Expected a non-empty BF16 or FP32 table [vocab, d]");
-  TORCH_CHECK_VALUE(std::isfinite(scale), "The scale must be finite, not ", scale);
+  check_scale(scale);
 }
 std::vector<int64_t> embedded(const Tensor& tokens, int64_t d) {
   std::vector<int64_t> sizes = tokens.sizes().vec();
@@ -257,7 +261,7 @@ void embedding_accumulate(Tensor& gradient, const Tensor& tokens, const Tensor& 
   TORCH_CHECK_VALUE((dy.scalar_type() == at::kBFloat16 || dy.scalar_type() == at::kFloat) &&
                         dy.sizes() == embedded(tokens, gradient.size(1)) && dy.device() == gradient.device(),
                     "Expected BF16 or FP32 rows of shape ", embedded(tokens, gradient.size(1)), " on ", gradient.device());
-  TORCH_CHECK_VALUE(std::isfinite(scale), "The scale must be finite, not ", scale);
+  check_scale(scale);
   embedding_sums(dy, tokens, scale, gradient, WS_EMBED_ADD_F32);
 }
 

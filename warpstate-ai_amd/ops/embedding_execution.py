@@ -21,6 +21,7 @@ and so is a second differentiation.
 from __future__ import annotations
 
 import math
+from ctypes import c_float
 
 import torch
 
@@ -32,13 +33,17 @@ Tensor = torch.Tensor
 _WRITE_BF16, _WRITE_F32, _ADD_F32 = 0, 1, 2
 
 
+def _check_scale(scale: float) -> None:
+    if not math.isfinite(c_float(scale).value):  # (the kernels multiply in FP32)
+        raise ValueError(f"The scale must be finite in FP32, not {scale}")
+
+
 def _check(tokens: Tensor, table: Tensor, scale: float) -> None:
     if tokens.dtype != torch.int64 or tokens.device != table.device:
         raise ValueError("Tokens must be int64 on the table's device")
     if table.dtype not in (BF16, F32) or table.ndim != 2 or table.numel() == 0:
         raise ValueError("Expected a non-empty BF16 or FP32 table [vocab, d]")
-    if not math.isfinite(scale):
-        raise ValueError(f"The scale must be finite, not {scale}")
+    _check_scale(scale)
 
 
 def _sums(dy: Tensor, tokens: Tensor, scale: float, out: Tensor, mode: int) -> None:
@@ -134,8 +139,7 @@ def embedding_accumulate_(gradient: Tensor, tokens: Tensor, dy: Tensor, scale: f
     if dy.dtype not in (BF16, F32) or dy.shape != shape or dy.device != gradient.device:
         raise ValueError(f"Expected BF16 or FP32 rows of shape {list(shape)} on "
                          f"{gradient.device}")
-    if not math.isfinite(scale):
-        raise ValueError(f"The scale must be finite, not {scale}")
+    _check_scale(scale)
     _sums(dy, tokens, float(scale), gradient, _ADD_F32)
     _written(gradient)
     return gradient
