@@ -53,7 +53,7 @@ int64_t grad_tiles(int64_t groups, int64_t m, int64_t n, int tile) {
 }
 
 // Tiles of a workgroup, one after the other: with a short reduction, finding one among the groups takes longer than
-// its product (us, one / several: 512 rows in 512 groups of 2048 x 16 135 / 34, 4096 in 256 of 2048 x 64 45 / 31).
+// its product (us, one / several: 512 rows, one each in 512 groups of 2048 x 16, 135 / 34, 4096 in 256 of 2048 x 64 45 / 31).
 // With any reduction, as many as bring the workgroups down to what a launch takes.
 int tiles_of_run(int64_t tiles, int64_t k) {
   const int64_t most = tiles / (4 * (int64_t)device_cus()), run = k > 256 || most < 2 ? 1 : most < 16 ? most : 16;
@@ -65,8 +65,9 @@ int tiles_of_run(int64_t tiles, int64_t k) {
 // rows of the tiles that a group of average size makes (its last one is half full on average, and
 // there is one); and the slices of a long reduction whose tiles leave units idle (us, whole / in slices: 64 rows
 // in 2 groups of 2048 x 11264 50 / 25, 494 in 3 of 960 x 9704 46 / 29, 64 in 8 of 2048 x 5632 34 / 37). What is
-// added to the table was fitted to 440 drawn sizes: the choice is 3 % behind the best tile and slices, 2 % for
-// reductions up to 2048 (the table alone 19 and 5 %, the best tiles without slices 15 %).
+// added to the table was fitted to 440 drawn sizes: over the 427 that the kernel for few rows does not take, the choice
+// is 3 % behind the best tile and slices, 2 % for reductions up to 2048 (the table alone 19 and 5 %, the best tiles
+// without slices 15 %).
 struct GroupedPlan {
   int tile, slices;
 };
