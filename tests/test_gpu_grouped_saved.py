@@ -114,3 +114,34 @@ def test_second_derivatives_stay_refused(wants, interior, form):
         for leaf in leaves:
             with pytest.raises(RuntimeError, match="twice"):
                 torch.autograd.grad(g.float().sum(), [leaf], retain_graph=True, allow_unused=True)
+
+
+def test_recomputed(form):
+    """Under checkpointing, whose second forward has to keep the same tensors."""
+    from torch.utils.checkpoint import checkpoint
+
+    from ops.grouped_execution import grouped_mm
+
+    for wants, k, dtype in (("x", 72, BF16), ("w", 77, F32), ("xw", 77, BF16)):
+        x, w, dy, offsets = _problem(k, dtype, wants)
+        leaves = [t for t, name in ((x, "x"), (w, "w")) if name in wants]
+        offsets = offsets.cuda()
+        want = torch.autograd.grad(grouped_mm(x, w, offsets), leaves, dy)
+        got = torch.autograd.grad(checkpoint(grouped_mm, x, w, offsets, use_reentrant=False), leaves, dy)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_compiled_backward():
+    """The backward itself compiled."""
+    from torch._dynamo import compiled_autograd
+
+    from ops.grouped_execution import grouped_mm
+
+    x, w, dy, offsets = _problem(72, F32, "xw")
+    offsets = offsets.cuda()
+    grouped_mm(x, w, offsets).backward(dy)
+    want = [x.grad.clone(), w.grad.clone()]
+    x.grad = w.grad = None
+    with compiled_autograd._enable(torch.compile(backend="aot_eager")):
+        grouped_mm(x, w, offsets).backward(dy)
+    assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
